@@ -20,6 +20,8 @@
  *                                   pages the same sequence of calls -- copy, roll the copy or the source back into the
  *                                   shared prefix, append -- needs the partly used shared page copied first
  *   mla_page_table_seq_keep         llama_kv_cache_seq_keep, :285-313
+ *   mla_page_table_seq_evict        no counterpart (the reference's cache drops ranges of positions only): the pages a sequence gives back
+ *                                   when gqa_evict_launch (include/gqa_attn.h) cuts it to some rows of its own choice, moved up in place
  *   mla_page_table_seq_add          llama_kv_cache_seq_add, :285-345: the reference marks the cache has_shift, and its next
  *                                   update aborts on that (GGML_ASSERT(!lctx.kv_self.has_shift), "we do not support shift",
  *                                   src/llama-execute-kvupdate.cpp:151-155: the keys in the cache were rotated for their old
@@ -51,7 +53,7 @@ extern "C" {
 #define MLA_PT_ERR_NOT_CONTIG (-3) /* a position that neither extends its sequence by one nor overwrites an existing cell */
 #define MLA_PT_ERR_UNSUPPORTED (-4) /* seq_rm of a range that is neither a suffix nor the whole sequence; find_slot: overwriting a row of
                                        a page that another sequence maps too, or appending into one (see mla_page_table_seq_unshare);
-                                       seq_add that would move a cached position */
+                                       seq_add that would move a cached position; seq_evict of a sequence with a shared page */
 
 typedef struct mla_page_table mla_page_table;
 
@@ -79,6 +81,12 @@ int mla_page_table_seq_cp(mla_page_table * t, int32_t seq_src, int32_t seq_dst, 
  * copy_src_row / copy_dst_row / copy_n_rows (each may be NULL) receive the row run the caller copies on the device
  * (copy_n_rows = 0: nothing to do).  MLA_PT_ERR_NO_SPACE when no page is free. */
 int mla_page_table_seq_unshare(mla_page_table * t, int32_t seq_id, int32_t * copy_src_row, int32_t * copy_dst_row, int32_t * copy_n_rows);
+
+/* Cuts a sequence to its first n_keep rows (n_keep >= 1; fewer rows: nothing to do) ahead of an eviction on the device that moves the rows to
+ * be kept there, in place.  MLA_PT_ERR_UNSUPPORTED, and nothing changed, when another sequence maps one of its pages: the move would
+ * rewrite that sequence's rows.  Block table and lengths for the eviction itself are filled (mla_page_table_fill_inputs) before this
+ * call; the pages it frees may be handed out at once, to writes that are queued behind the eviction. */
+int mla_page_table_seq_evict(mla_page_table * t, int32_t seq_id, int32_t n_keep);
 
 /* Adds delta to positions [p0, p1) of a sequence: 0 when the range holds no cell or delta == 0, else MLA_PT_ERR_UNSUPPORTED
  * (nothing changed). */

@@ -4,6 +4,7 @@ import os
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -26,14 +27,17 @@ def _run(cmd):
 
 
 def build(verbose=False):
-    objs = []
-    for src in ("mla_kernels.hip", "mla_decode_kernel.hip", "mla_kv_write.hip", "mla_front.hip", "ggml_mla_backend.cpp", "mla_page_table.cpp"):
+    def compile(src):
         obj = os.path.join(CSRC, os.path.splitext(src)[0] + ".o")
         cmd = [HIPCC] + COMMON + (["-x", "hip"] if src == "ggml_mla_backend.cpp" else []) + ["-c", os.path.join(CSRC, src), "-o", obj]
         out = _run(cmd)
         if verbose and out.strip():
             print(out)
-        objs.append(obj)
+        return obj
+
+    with ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:
+        objs = list(pool.map(compile, ("mla_kernels.hip", "mla_decode_kernel.hip", "mla_kv_write.hip", "mla_front.hip", "gqa_front.hip", "gqa_attn.hip",
+                                       "gqa_evict.hip", "ggml_mla_backend.cpp", "mla_page_table.cpp")))
     _run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs + ["-ldl"])
     return LIB
 

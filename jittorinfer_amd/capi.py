@@ -72,6 +72,12 @@ def library():
             getattr(lib, name).argtypes = [C.POINTER(cls), C.c_void_p]
         lib.mla_front_batch_launch.restype = C.c_int
         lib.mla_front_batch_launch.argtypes = [C.POINTER(MlaFrontOp), C.c_int32, C.c_void_p]
+        for name, cls in (("gqa_norm_rope", GqaNormRopeArgs), ("gqa_attn", GqaAttnArgs), ("gqa_evict", GqaEvictArgs)):
+            getattr(lib, name + "_check").restype = getattr(lib, name + "_launch").restype = C.c_int
+            getattr(lib, name + "_check").argtypes = [C.POINTER(cls)]
+            getattr(lib, name + "_launch").argtypes = [C.POINTER(cls), C.c_void_p]
+        lib.gqa_attn_workspace_size.restype = C.c_size_t
+        lib.gqa_attn_workspace_size.argtypes = [C.POINTER(GqaAttnArgs)]
         lib.mla_page_table_create.restype = C.c_void_p
         lib.mla_page_table_create.argtypes = [C.c_int32] * 3
         lib.mla_page_table_free.argtypes = [C.c_void_p]
@@ -81,6 +87,7 @@ def library():
         lib.mla_page_table_seq_cp.argtypes = [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32] + [C.POINTER(C.c_int32)] * 3
         lib.mla_page_table_seq_unshare.argtypes = [C.c_void_p, C.c_int32] + [C.POINTER(C.c_int32)] * 3
         lib.mla_page_table_seq_keep.argtypes = [C.c_void_p, C.c_int32]
+        lib.mla_page_table_seq_evict.argtypes = [C.c_void_p, C.c_int32, C.c_int32]
         lib.mla_page_table_seq_add.argtypes = [C.c_void_p] + [C.c_int32] * 4
         lib.mla_page_table_defrag.argtypes = [C.c_void_p, C.POINTER(C.c_int32)]
         for name in ("mla_page_table_seq_len", "mla_page_table_free_pages", "mla_page_table_used_cells"):
@@ -113,8 +120,10 @@ def native():
         except ImportError as e:
             raise RuntimeError("jittorinfer_amd/_native.so is missing or does not load (%s): build it with `python jittorinfer_amd/build.py`" % e)
         names = ("mla_attn_workspace_size", "mla_attn_launch", "mla_kv_write_launch", "mla_kv_write_rope_launch", "mla_rope_launch",
-                 "mla_mul_mat_launch", "mla_copy_f32_launch", "mla_front_batch_launch")
-        mod.bind(*[C.cast(getattr(lib, n), C.c_void_p).value for n in names], _workspace, _workspaces, torch._C._cuda_getCurrentRawStream)
+                 "mla_mul_mat_launch", "mla_copy_f32_launch", "mla_front_batch_launch", "gqa_norm_rope_launch", "gqa_attn_workspace_size",
+                 "gqa_attn_launch", "gqa_evict_launch")
+        mod.bind(*[C.cast(getattr(lib, n), C.c_void_p).value for n in names], _workspace, _workspaces, torch._C._cuda_getCurrentRawStream,
+                 torch._C._cuda_isCurrentStreamCapturing)
         _native = mod
     return _native
 
@@ -336,6 +345,86 @@ def copy_f32(src, dst, stream=None, batch=None):
     return (_native or native()).copy(src, dst, stream, batch)
 
 
+class GqaPool(C.Structure):
+    """gqa_pool of include/gqa_attn.h."""
+    _fields_ = [("data", C.c_void_p), ("nb_page", C.c_int64), ("nb_row", C.c_int64), ("nb_head", C.c_int64)]
+
+
+class GqaNormRopeArgs(C.Structure):
+    """gqa_norm_rope_args of include/gqa_attn.h."""
+    _fields_ = [("n_tok", C.c_int32), ("n_head", C.c_int32), ("n_head_kv", C.c_int32), ("dk", C.c_int32), ("dv", C.c_int32),
+                ("src_type", C.c_int32), ("w_type", C.c_int32), ("dst_type", C.c_int32), ("kv_type", C.c_int32), ("n_seq", C.c_int32),
+                ("q", C.c_void_p), ("q_nb1", C.c_int64), ("q_nb2", C.c_int64), ("k", C.c_void_p), ("k_nb1", C.c_int64), ("k_nb2", C.c_int64),
+                ("v", C.c_void_p), ("v_nb1", C.c_int64), ("v_nb2", C.c_int64), ("q_weight", C.c_void_p), ("k_weight", C.c_void_p),
+                ("eps", C.c_float), ("n_dims", C.c_int32), ("mode", C.c_int32), ("n_ctx_orig", C.c_int32),
+                ("freq_base", C.c_double), ("freq_scale", C.c_double), ("ext_factor", C.c_double), ("attn_factor", C.c_double),
+                ("beta_fast", C.c_double), ("beta_slow", C.c_double), ("freq_factors", C.c_void_p), ("pos", C.c_void_p),
+                ("q_dst", C.c_void_p), ("qd_nb1", C.c_int64), ("qd_nb2", C.c_int64), ("k_cache", GqaPool), ("v_cache", GqaPool),
+                ("n_pages", C.c_int64), ("block_table", C.c_void_p), ("bt_stride", C.c_int64), ("seq_ids", C.c_void_p), ("slots", C.c_void_p)]
+
+
+class GqaAttnArgs(C.Structure):
+    """gqa_attn_args of include/gqa_attn.h."""
+    _fields_ = [("n_seq", C.c_int32), ("n_head", C.c_int32), ("n_head_kv", C.c_int32), ("dk", C.c_int32), ("dv", C.c_int32),
+                ("q_type", C.c_int32), ("kv_type", C.c_int32), ("dst_type", C.c_int32), ("scale", C.c_float), ("logit_softcap", C.c_float),
+                ("window", C.c_int32), ("n_workgroups", C.c_int32), ("q", C.c_void_p), ("q_nb1", C.c_int64), ("q_nb2", C.c_int64),
+                ("k", GqaPool), ("v", GqaPool), ("n_pages", C.c_int64), ("block_table", C.c_void_p), ("bt_stride", C.c_int64),
+                ("seq_lens", C.c_void_p), ("mask", C.c_void_p), ("mask_nb1", C.c_int64), ("mask_ne0", C.c_int64), ("weights", C.c_void_p),
+                ("w_nb1", C.c_int64), ("w_nb2", C.c_int64), ("dst", C.c_void_p), ("d_nb1", C.c_int64), ("d_nb2", C.c_int64),
+                ("workspace", C.c_void_p), ("workspace_size", C.c_size_t)]
+
+
+class GqaEvictArgs(C.Structure):
+    """gqa_evict_args of include/gqa_attn.h."""
+    _fields_ = [("n_seq", C.c_int32), ("n_head_kv", C.c_int32), ("n_keep", C.c_int32), ("n_sink", C.c_int32), ("n_recent", C.c_int32),
+                ("k_row_bytes", C.c_int32), ("v_row_bytes", C.c_int32), ("_pad", C.c_int32), ("k", GqaPool), ("v", GqaPool),
+                ("n_pages", C.c_int64), ("block_table", C.c_void_p), ("bt_stride", C.c_int64), ("seq_lens", C.c_void_p),
+                ("weights", C.c_void_p), ("w_nb1", C.c_int64), ("w_nb2", C.c_int64), ("weights_dst", C.c_void_p), ("wd_nb1", C.c_int64),
+                ("wd_nb2", C.c_int64), ("kept", C.c_void_p), ("new_lens", C.c_void_p)]
+
+
+def gqa_norm_rope(q, k, v, pos, *, n_dims, mode=0, n_ctx_orig=0, freq_base=10000.0, freq_scale=1.0, ext_factor=0.0, attn_factor=1.0,
+                  beta_fast=32.0, beta_slow=1.0, freq_factors=None, q_weight=None, k_weight=None, eps=1e-6, q_out=None,
+                  k_cache=None, v_cache=None, block_table=None, seq_ids=None, slots=None, stream=None):
+    """RMS norm of every head's query and key, their rotation and the write of keys and values into a paged cache, in one pass on the current
+    torch stream (gqa_norm_rope_launch, include/gqa_attn.h).
+
+    q         [n_tok, n_head, dk], k [n_tok, n_head_kv, dk], v [n_tok, n_head_kv, dv]: float32, bfloat16 or float16 alike, any strides
+              over contiguous rows (views of one projection's output); v may be None, and k with it: queries alone
+    pos       int32 [n_tok]; the rotation's keywords are those of ggml_rope_ext, n_dims=0 rotates nothing
+    q_weight, k_weight  [dk] or None: no norm
+    k_cache, v_cache    bfloat16 or float16 [pages, 128, n_head_kv, dk | dv]; token t goes to row slots[t] (default: pos[t]) of sequence
+              seq_ids[t] of the int32 block_table [n_seq, pages]; rows outside it are skipped
+    Returns the queries, q_out or a new tensor of the cache's type (of q's without a cache); q_out=q works in place."""
+    return (_native or native()).gqa_norm_rope(q, k, v, pos, q_weight, k_weight, eps, n_dims, mode, n_ctx_orig, freq_base, freq_scale, ext_factor,
+                                               attn_factor, beta_fast, beta_slow, freq_factors, q_out, k_cache, v_cache, block_table, seq_ids, slots, stream)
+
+
+def gqa_attn(q, k_cache, v_cache, block_table, seq_lens, *, scale, logit_softcap=0.0, window=0, mask=None, weights=None, out=None,
+             n_workgroups=0, stream=None):
+    """Attention of one new token of every sequence over its pages, on the current torch stream (gqa_attn_launch, include/gqa_attn.h).
+
+    q         [n_seq, n_head, dk], the cache's type or float32; n_head a multiple of the cache's heads
+    k_cache, v_cache    bfloat16 or float16 [pages, 128, n_head_kv, dk | dv], (dk, dv) one of (64, 64), (128, 128), (192, 128), (256, 256)
+    block_table, seq_lens  int32 [n_seq, width], [n_seq]; window > 0: the last `window` rows alone
+    mask      float16 [n_seq, n] or None, added to the scores; -inf takes a row out, a row past n is out
+    weights   float32 [n_seq, n_head_kv, >= width * 128] or None: the softmax weights of a group's heads are added to it
+    Returns out, [n_seq, n_head, dv] of q's type by default; a sequence without a row gets zeros.
+    v_cache=None: the weights alone (returned), over a cache of one head of 576 values, the latent cache of ggml_flash_attn_ext."""
+    return (_native or native()).gqa_attn(q, k_cache, v_cache, block_table, seq_lens, scale, logit_softcap, window, mask, weights, out, n_workgroups, stream)
+
+
+def gqa_evict(weights, block_table, seq_lens, k_cache, v_cache=None, *, n_keep, n_sink=0, n_recent=0, weights_out=None, kept=None, new_lens=None, stream=None):
+    """Cuts every sequence of more than n_keep rows to the n_keep that matter, on the current torch stream (gqa_evict_launch,
+    include/gqa_attn.h): for every KV head the first n_sink rows, the last n_recent and the heaviest of the rest (equal weights: the lower row)
+    move up, in order, inside the sequence's pages.  Caches are [pages, 128, n_head_kv, row] of any element type with rows of whole 4 bytes
+    (a latent cache: [pages, 128, 1, 576], or 612 bytes of Q8_0).  Pages mapped by several sequences must not be evicted from
+    (PageTable.seq_evict refuses them).
+    Returns kept int32 [n_seq, n_head_kv, n_keep] (the row that is now row j, -1 past the new length), new_lens int32 [n_seq] and the
+    weights that moved along, 0 past the new length (weights_out=weights: in place)."""
+    return (_native or native()).gqa_evict(weights, block_table, seq_lens, k_cache, v_cache, n_keep, n_sink, n_recent, weights_out, kept, new_lens, stream)
+
+
 class PageTable:
     """Host-side page allocator / block-table builder (include/mla_page_table.h): the paged counterpart of the reference's
     llama_kv_cache bookkeeping (src/llama-kv-cache.cpp) and of the mask builder of llama_set_inputs.  numpy in, numpy out."""
@@ -393,6 +482,14 @@ class PageTable:
 
     def seq_keep(self, seq_id):
         return self._lib.mla_page_table_seq_keep(self._h, seq_id) == 0
+
+    def seq_evict(self, seq_id, n_keep):
+        """Before gqa_evict cuts the sequence to n_keep rows on the device (with the block table filled before this call): gives the pages past
+        them back.  False: a page is shared with another sequence, nothing changed and the sequence must not be evicted from."""
+        rc = self._lib.mla_page_table_seq_evict(self._h, seq_id, n_keep)
+        if rc not in (0, -4):
+            raise ValueError("mla_page_table_seq_evict: %d" % rc)
+        return rc == 0
 
     def seq_add(self, seq_id, p0, p1, delta):
         """True when nothing had to move (no cell in the range, or delta 0); False: refused, cached positions cannot be shifted."""

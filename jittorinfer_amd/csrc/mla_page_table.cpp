@@ -172,6 +172,14 @@ int mla_page_table_seq_unshare(mla_page_table * t, int32_t seq_id, int32_t * cop
     return 0;
 }
 
+int mla_page_table_seq_evict(mla_page_table * t, int32_t seq_id, int32_t n_keep) {
+    if (!seq_ok(t, seq_id) || n_keep < 1) return MLA_PT_ERR_BAD_ARG;
+    if (t->len[seq_id] <= n_keep) return 0;
+    for (int32_t p : t->pages[seq_id]) if (t->refcount[p] > 1) return MLA_PT_ERR_UNSUPPORTED;
+    truncate(t, seq_id, n_keep);
+    return 0;
+}
+
 int mla_page_table_seq_add(mla_page_table * t, int32_t seq_id, int32_t p0, int32_t p1, int32_t delta) {
     if (!seq_ok(t, seq_id)) return MLA_PT_ERR_BAD_ARG;
     if (p0 < 0) p0 = 0;

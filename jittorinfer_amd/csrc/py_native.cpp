@@ -1,4 +1,4 @@
-// The Python entry points' way from torch tensors to the C ABI (include/mla_attn.h, mla_kv_write.h, mla_front.h): one call that checks the
+// The Python entry points' way from torch tensors to the C ABI (include/mla_attn.h, mla_kv_write.h, mla_front.h, gqa_attn.h): one call that checks the
 // tensors, fills the argument block and launches.  Filling a ctypes structure field by field took 6 us of a 13 us attention call and
 // most of the 70 us a layer of a decode step spent on the host, more than its kernels run for small batches; here it takes
 // under 1 us a call.  Every function takes its arguments by position; capi.py gives them names and defaults.
@@ -12,10 +12,12 @@
 #include <vector>
 
 #include <ATen/ops/empty.h>
+#include <c10/core/DeviceGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 
+#include "../../include/gqa_attn.h"
 #include "../../include/mla_attn.h"
 #include "../../include/mla_front.h"
 #include "../../include/mla_kv_write.h"
@@ -44,7 +46,11 @@ struct Bound {
     decltype(&mla_mul_mat_launch)      mul_mat;
     decltype(&mla_copy_f32_launch)     copy;
     decltype(&mla_front_batch_launch)  front_batch;
-    PyObject * workspace, * workspaces, * raw_stream;
+    decltype(&gqa_norm_rope_launch)    norm_rope;
+    decltype(&gqa_attn_workspace_size) gqa_workspace_size;
+    decltype(&gqa_attn_launch)         gqa_attn;
+    decltype(&gqa_evict_launch)        evict;
+    PyObject * workspace, * workspaces, * raw_stream, * capturing;
 } lib;
 
 #define REQUIRE(cond)                                        \
@@ -104,7 +110,7 @@ int64_t row_bytes(long kv_type) { return kv_type == MLA_TYPE_F16 || kv_type == M
 
 // The scratch area of (device, stream): a look-up in the Python layer's table; too small or missing, the Python layer makes one.  The
 // caller keeps what is returned until its launch is queued: another thread may give areas back meanwhile.
-THPObjectPtr workspace(PyObject * q, void * st, size_t need, mla_attn_args & a) {
+template <typename Args> THPObjectPtr workspace(PyObject * q, void * st, size_t need, Args & a) {
     THPObjectPtr dev(PyObject_GetAttrString(q, "device")), handle(dev ? PyLong_FromVoidPtr(st) : nullptr);
     THPObjectPtr key(handle ? PyTuple_Pack(2, dev.get(), handle.get()) : nullptr);
     if (!key) return THPObjectPtr();
@@ -373,18 +379,246 @@ PyObject * front_batch(PyObject *, PyObject * const * v, Py_ssize_t n) {
     Py_RETURN_NONE;
 }
 
-// bind(addresses of the eight entry points in Bound's order, workspace function, workspace table, torch's raw current stream)
-PyObject * bind(PyObject *, PyObject * const * v, Py_ssize_t n) {
-    if (!arg_count(n, 11)) return nullptr;
-    void * p[8];
-    for (int i = 0; i < 8; i++) p[i] = PyLong_AsVoidPtr(v[i]);
+// ---- the cache of ordinary heads (include/gqa_attn.h)
+
+int mla_type(const at::Tensor & t) {
+    switch (t.scalar_type()) {
+        case at::kFloat:    return MLA_TYPE_F32;
+        case at::kHalf:     return MLA_TYPE_F16;
+        case at::kBFloat16: return MLA_TYPE_BF16;
+        default:            return -1;
+    }
+}
+at::ScalarType torch_type(int type) { return type == MLA_TYPE_F32 ? at::kFloat : type == MLA_TYPE_F16 ? at::kHalf : at::kBFloat16; }
+bool ints(const at::Tensor & t, int64_t n) { return t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && t.is_contiguous(); }
+bool table_ok(const at::Tensor & t) { return t.scalar_type() == at::kInt && t.dim() == 2 && t.is_contiguous() && t.size(1) >= 1; }
+// `dim` dimensions, the last one contiguous; the elements of a tensor that is written must not lie on each other: from the smallest
+// stride up, each steps past all that the ones before it reach.
+bool rows_ok(const at::Tensor & t, int64_t dim, bool written) {
+    if (t.dim() != dim || (t.size(-1) > 1 && t.stride(-1) != 1)) return false;
+    if (!written || t.numel() == 0) return true;
+    std::vector<std::pair<int64_t, int64_t>> steps;
+    for (int64_t d = 0; d < dim; d++) if (t.size(d) > 1) steps.emplace_back(t.stride(d), t.size(d));
+    std::sort(steps.begin(), steps.end());
+    int64_t reach = 0;
+    for (const auto & [stride, size] : steps) {
+        if (stride <= reach) return false;
+        reach += stride * (size - 1);
+    }
+    return true;
+}
+bool cache_ok(const at::Tensor & c, int type) { return mla_type(c) == type && rows_ok(c, 4, true) && c.size(0) >= 1 && c.size(1) == PAGE; }
+gqa_pool pool_of(const at::Tensor & c) {
+    const int64_t es = (int64_t) c.element_size();
+    return gqa_pool{ c.data_ptr(), c.stride(0) * es, c.stride(1) * es, c.stride(2) * es };
+}
+// The stream to launch on.  What a call makes for itself (results, scratch) belongs to the device's current stream, so a call on another one
+// brings its own (`makes` = false).
+bool gqa_stream(PyObject * o, const at::Tensor & t, bool makes, void *& st) {
+    if (!stream_of(Py_None, t, st)) return false;
+    if (o == Py_None) return true;
+    void * const current = st;
+    if (!stream_of(o, t, st)) return false;
+    if (!makes || st == current) return true;
+    PyErr_SetString(PyExc_ValueError, "a launch on another stream than the current one takes its result tensors from the caller");
+    return false;
+}
+#define SAME_DEVICE(t) REQUIRE(!(t) || (t)->device() == q.device())
+
+// gqa_norm_rope(q, k, v, pos, q_weight, k_weight, eps, n_dims, mode, n_ctx_orig, freq_base, freq_scale, ext_factor, attn_factor, beta_fast,
+//               beta_slow, freq_factors, q_out, k_cache, v_cache, block_table, seq_ids, slots, stream) -> q_out
+PyObject * gqa_norm_rope(PyObject *, PyObject * const * o, Py_ssize_t n) {
+    if (!arg_count(n, 24)) return nullptr;
+    const at::Tensor * qp = tensor(o[0]), * pos = qp ? tensor(o[3]) : nullptr, * k, * v, * qw, * kw, * ff, * outp, * kc, * vc, * table, * ids, * slots;
+    if (!pos || !optional_tensor(o[1], k) || !optional_tensor(o[2], v) || !optional_tensor(o[4], qw) || !optional_tensor(o[5], kw) || !optional_tensor(o[16], ff) ||
+        !optional_tensor(o[17], outp) || !optional_tensor(o[18], kc) || !optional_tensor(o[19], vc) || !optional_tensor(o[20], table) || !optional_tensor(o[21], ids) || !optional_tensor(o[22], slots))
+        return nullptr;
+    const at::Tensor & q = *qp;
+    if (!on_gpu(q)) return nullptr;
+    for (const at::Tensor * t : { pos, k, v, qw, kw, ff, outp, kc, vc, table, ids, slots }) SAME_DEVICE(t);
+    gqa_norm_rope_args a;
+    memset(&a, 0, sizeof a);
+    a.eps = (float) PyFloat_AsDouble(o[6]);
+    a.n_dims = (int32_t) PyLong_AsLong(o[7]); a.mode = (int32_t) PyLong_AsLong(o[8]); a.n_ctx_orig = (int32_t) PyLong_AsLong(o[9]);
+    a.freq_base = PyFloat_AsDouble(o[10]); a.freq_scale = PyFloat_AsDouble(o[11]); a.ext_factor = PyFloat_AsDouble(o[12]);
+    a.attn_factor = PyFloat_AsDouble(o[13]); a.beta_fast = PyFloat_AsDouble(o[14]); a.beta_slow = PyFloat_AsDouble(o[15]);
     if (PyErr_Occurred()) return nullptr;
-    REQUIRE(PyCallable_Check(v[8]) && PyDict_Check(v[9]) && PyCallable_Check(v[10]));
+    REQUIRE(mla_type(q) >= 0 && rows_ok(q, 3, false));
+    const int64_t n_tok = q.size(0), es = (int64_t) q.element_size();
+    a.n_tok = (int32_t) n_tok; a.n_head = (int32_t) q.size(1); a.dk = (int32_t) q.size(2);
+    a.src_type = a.w_type = mla_type(q);
+    a.q = q.data_ptr(); a.q_nb1 = q.stride(1) * es; a.q_nb2 = q.stride(0) * es;
+    REQUIRE(ints(*pos, n_tok));
+    a.pos = (const int32_t *) pos->data_ptr();
+    a.kv_type = MLA_TYPE_BF16;
+    if (qw || kw) {
+        a.w_type = mla_type(qw ? *qw : *kw);
+        for (const at::Tensor * w : { qw, kw }) REQUIRE(!w || (mla_type(*w) == a.w_type && a.w_type >= 0 && w->dim() == 1 && w->size(0) == a.dk && w->is_contiguous()));
+        a.q_weight = qw ? qw->data_ptr() : nullptr; a.k_weight = kw ? kw->data_ptr() : nullptr;
+    }
+    if (ff) {
+        REQUIRE(ff->scalar_type() == at::kFloat && ff->dim() == 1 && ff->size(0) >= a.n_dims / 2 && ff->is_contiguous());
+        a.freq_factors = (const float *) ff->data_ptr();
+    }
+    if (k) {
+        REQUIRE(kc && table && ids && (v != nullptr) == (vc != nullptr));
+        REQUIRE(k->scalar_type() == q.scalar_type() && rows_ok(*k, 3, false) && k->size(0) == n_tok && k->size(2) == a.dk);
+        a.kv_type = mla_type(*kc);
+        REQUIRE(a.kv_type > 0 && cache_ok(*kc, a.kv_type) && kc->size(2) == k->size(1) && kc->size(3) == a.dk);
+        REQUIRE(table_ok(*table) && ints(*ids, n_tok) && (!slots || ints(*slots, n_tok)));
+        a.n_head_kv = (int32_t) k->size(1); a.n_seq = (int32_t) table->size(0); a.n_pages = kc->size(0);
+        a.k = k->data_ptr(); a.k_nb1 = k->stride(1) * es; a.k_nb2 = k->stride(0) * es;
+        a.k_cache = pool_of(*kc);
+        a.block_table = (const int32_t *) table->data_ptr(); a.bt_stride = table->size(1);
+        a.seq_ids = (const int32_t *) ids->data_ptr(); a.slots = slots ? (const int32_t *) slots->data_ptr() : nullptr;
+        if (v) {
+            REQUIRE(v->scalar_type() == q.scalar_type() && rows_ok(*v, 3, false) && v->size(0) == n_tok && v->size(1) == a.n_head_kv);
+            REQUIRE(cache_ok(*vc, a.kv_type) && vc->size(0) == a.n_pages && vc->size(2) == a.n_head_kv && vc->size(3) == v->size(2));
+            a.dv = (int32_t) v->size(2);
+            a.v = v->data_ptr(); a.v_nb1 = v->stride(1) * es; a.v_nb2 = v->stride(0) * es;
+            a.v_cache = pool_of(*vc);
+        }
+    } else REQUIRE(!v && !kc && !vc && !kw);
+    const c10::DeviceGuard guard(q.device());
+    void * st;
+    if (!gqa_stream(o[23], q, !outp, st)) return nullptr;
+    at::Tensor made;
+    if (!outp) { made = at::empty(q.sizes(), q.options().dtype(kc ? kc->scalar_type() : q.scalar_type())); outp = &made; }
+    const at::Tensor & out = *outp;
+    a.dst_type = mla_type(out);
+    REQUIRE(a.dst_type >= 0 && out.sizes() == q.sizes() && rows_ok(out, 3, true));
+    const int64_t od = (int64_t) out.element_size();
+    a.q_dst = out.data_ptr(); a.qd_nb1 = out.stride(1) * od; a.qd_nb2 = out.stride(0) * od;
+    const int rc = unlocked([&] { return lib.norm_rope(&a, st); });
+    if (rc) return failed("gqa_norm_rope_launch", rc);
+    return made.defined() ? THPVariable_Wrap(made) : Py_NewRef(o[17]);
+}
+
+// gqa_attn(q, k_cache, v_cache, block_table, seq_lens, scale, logit_softcap, window, mask, weights, out, n_workgroups, stream) -> out, or weights without v_cache
+PyObject * gqa_attn(PyObject *, PyObject * const * o, Py_ssize_t n) {
+    if (!arg_count(n, 13)) return nullptr;
+    const at::Tensor * qp = tensor(o[0]), * kc = qp ? tensor(o[1]) : nullptr, * table = kc ? tensor(o[3]) : nullptr, * lens = table ? tensor(o[4]) : nullptr, * vc, * mask, * weights, * outp;
+    if (!lens || !optional_tensor(o[2], vc) || !optional_tensor(o[8], mask) || !optional_tensor(o[9], weights) || !optional_tensor(o[10], outp)) return nullptr;
+    const at::Tensor & q = *qp;
+    if (!on_gpu(q)) return nullptr;
+    for (const at::Tensor * t : { kc, table, lens, vc, mask, weights, outp }) SAME_DEVICE(t);
+    gqa_attn_args a;
+    memset(&a, 0, sizeof a);
+    a.scale = (float) PyFloat_AsDouble(o[5]); a.logit_softcap = (float) PyFloat_AsDouble(o[6]);
+    const int64_t window = PyLong_AsLongLong(o[7]);
+    a.n_workgroups = (int32_t) PyLong_AsLong(o[11]);
+    if (PyErr_Occurred()) return nullptr;
+    REQUIRE(window >= 0 && window < ((int64_t) 1 << 31));
+    a.window = (int32_t) window;
+    REQUIRE(mla_type(q) >= 0 && rows_ok(q, 3, false));
+    const int64_t n_seq = q.size(0), n_head = q.size(1), es = (int64_t) q.element_size();
+    a.n_seq = (int32_t) n_seq; a.n_head = (int32_t) n_head; a.dk = (int32_t) q.size(2);
+    a.q_type = mla_type(q); a.q = q.data_ptr(); a.q_nb1 = q.stride(1) * es; a.q_nb2 = q.stride(0) * es;
+    a.kv_type = mla_type(*kc);
+    REQUIRE(a.kv_type > 0 && cache_ok(*kc, a.kv_type) && kc->size(3) == a.dk);
+    a.n_head_kv = (int32_t) kc->size(2); a.n_pages = kc->size(0); a.k = pool_of(*kc);
+    if (vc) {
+        REQUIRE(cache_ok(*vc, a.kv_type) && vc->size(0) == a.n_pages && vc->size(2) == a.n_head_kv);
+        a.dv = (int32_t) vc->size(3); a.v = pool_of(*vc);
+    } else REQUIRE(weights && !outp);
+    REQUIRE(table_ok(*table) && table->size(0) == n_seq && ints(*lens, n_seq));
+    a.block_table = (const int32_t *) table->data_ptr(); a.bt_stride = table->size(1); a.seq_lens = (const int32_t *) lens->data_ptr();
+    if (mask) {
+        REQUIRE(mask->scalar_type() == at::kHalf && rows_ok(*mask, 2, false) && mask->size(0) == n_seq);
+        a.mask = mask->data_ptr(); a.mask_nb1 = mask->stride(0) * 2; a.mask_ne0 = mask->size(1);
+        if (!a.mask) { PyErr_SetString(PyExc_ValueError, "a mask without columns leaves no row"); return nullptr; }
+    }
+    if (weights) {
+        REQUIRE(weights->scalar_type() == at::kFloat && rows_ok(*weights, 3, true) && weights->size(0) == n_seq && weights->size(1) == a.n_head_kv && weights->size(2) >= a.bt_stride * PAGE);
+        a.weights = (float *) weights->data_ptr(); a.w_nb1 = weights->stride(1) * 4; a.w_nb2 = weights->stride(0) * 4;
+    }
+    const c10::DeviceGuard guard(q.device());
+    void * st;
+    if (!gqa_stream(o[12], q, vc && !outp, st)) return nullptr;
+    at::Tensor made;
+    if (vc) {
+        if (!outp) { made = at::empty({ n_seq, n_head, (int64_t) a.dv }, q.options()); outp = &made; }
+        const at::Tensor & out = *outp;
+        const int64_t od = (int64_t) out.element_size();
+        a.dst_type = mla_type(out);
+        REQUIRE(a.dst_type >= 0 && out.dim() == 3 && out.size(0) == n_seq && out.size(1) == n_head && out.size(2) == a.dv && rows_ok(out, 3, true));
+        a.dst = out.data_ptr(); a.d_nb1 = out.stride(1) * od; a.d_nb2 = out.stride(0) * od;
+    } else a.dst_type = MLA_TYPE_F32;
+    const size_t need = lib.gqa_workspace_size(&a);
+    // Under graph capture the scratch is the graph's own: two graphs captured on one stream may be replayed side by side.
+    THPObjectPtr ws, capturing(PyObject_CallNoArgs(lib.capturing));
+    if (!capturing) return nullptr;
+    at::Tensor own;
+    if (capturing.get() == Py_True) {
+        own = at::empty({ (int64_t) need }, q.options().dtype(at::kByte));
+        a.workspace = own.data_ptr(); a.workspace_size = need;
+    } else if (need) {
+        ws = workspace(o[0], st, need, a);
+        if (!ws) return nullptr;
+    }
+    const int rc = unlocked([&] { return lib.gqa_attn(&a, st); });
+    if (rc) return failed("gqa_attn_launch", rc);
+    return made.defined() ? THPVariable_Wrap(made) : Py_NewRef(vc ? o[10] : o[9]);
+}
+
+// gqa_evict(weights, block_table, seq_lens, k_cache, v_cache, n_keep, n_sink, n_recent, weights_out, kept, new_lens, stream) -> (kept, new_lens, weights_out)
+PyObject * gqa_evict(PyObject *, PyObject * const * o, Py_ssize_t n) {
+    if (!arg_count(n, 12)) return nullptr;
+    const at::Tensor * qp = tensor(o[0]), * table = qp ? tensor(o[1]) : nullptr, * lens = table ? tensor(o[2]) : nullptr, * kc = lens ? tensor(o[3]) : nullptr, * vc, * wop, * keptp, * newp;
+    if (!kc || !optional_tensor(o[4], vc) || !optional_tensor(o[8], wop) || !optional_tensor(o[9], keptp) || !optional_tensor(o[10], newp)) return nullptr;
+    const at::Tensor & q = *qp;                               // the weights
+    if (!on_gpu(q)) return nullptr;
+    for (const at::Tensor * t : { table, lens, kc, vc, wop, keptp, newp }) SAME_DEVICE(t);
+    gqa_evict_args a;
+    memset(&a, 0, sizeof a);
+    a.n_keep = (int32_t) PyLong_AsLong(o[5]); a.n_sink = (int32_t) PyLong_AsLong(o[6]); a.n_recent = (int32_t) PyLong_AsLong(o[7]);
+    if (PyErr_Occurred()) return nullptr;
+    REQUIRE(table_ok(*table));
+    const int64_t n_seq = table->size(0), cap = table->size(1) * PAGE;
+    REQUIRE(ints(*lens, n_seq));
+    a.n_seq = (int32_t) n_seq;
+    a.block_table = (const int32_t *) table->data_ptr(); a.bt_stride = table->size(1); a.seq_lens = (const int32_t *) lens->data_ptr();
+    REQUIRE(rows_ok(*kc, 4, true) && kc->size(0) >= 1 && kc->size(1) == PAGE);
+    a.n_head_kv = (int32_t) kc->size(2); a.n_pages = kc->size(0); a.k = pool_of(*kc);
+    a.k_row_bytes = (int32_t) (kc->size(3) * (int64_t) kc->element_size());
+    if (vc) {
+        REQUIRE(rows_ok(*vc, 4, true) && vc->size(0) == a.n_pages && vc->size(1) == PAGE && vc->size(2) == a.n_head_kv);
+        a.v = pool_of(*vc); a.v_row_bytes = (int32_t) (vc->size(3) * (int64_t) vc->element_size());
+    }
+    REQUIRE(q.scalar_type() == at::kFloat && rows_ok(q, 3, false) && q.size(0) == n_seq && q.size(1) == a.n_head_kv && q.size(2) == cap);
+    a.weights = (const float *) q.data_ptr(); a.w_nb1 = q.stride(1) * 4; a.w_nb2 = q.stride(0) * 4;
+    const c10::DeviceGuard guard(q.device());
+    void * st;
+    if (!gqa_stream(o[11], q, !wop || !keptp || !newp, st)) return nullptr;
+    at::Tensor wo = wop ? *wop : at::empty({ n_seq, (int64_t) a.n_head_kv, cap }, q.options());
+    REQUIRE(a.n_keep >= 0);
+    at::Tensor kept = keptp ? *keptp : at::empty({ n_seq, (int64_t) a.n_head_kv, (int64_t) a.n_keep }, q.options().dtype(at::kInt));
+    at::Tensor fresh = newp ? *newp : at::empty({ n_seq }, q.options().dtype(at::kInt));
+    REQUIRE(wo.scalar_type() == at::kFloat && rows_ok(wo, 3, true) && wo.size(0) == n_seq && wo.size(1) == a.n_head_kv && wo.size(2) == cap);
+    REQUIRE(kept.scalar_type() == at::kInt && kept.dim() == 3 && kept.is_contiguous() && kept.size(0) == n_seq && kept.size(1) == a.n_head_kv && kept.size(2) == a.n_keep);
+    REQUIRE(ints(fresh, n_seq));
+    a.weights_dst = (float *) wo.data_ptr(); a.wd_nb1 = wo.stride(1) * 4; a.wd_nb2 = wo.stride(0) * 4;
+    a.kept = (int32_t *) kept.data_ptr(); a.new_lens = (int32_t *) fresh.data_ptr();
+    const int rc = unlocked([&] { return lib.evict(&a, st); });
+    if (rc) return failed("gqa_evict_launch", rc);
+    THPObjectPtr r0(keptp ? Py_NewRef(o[9]) : THPVariable_Wrap(kept)), r1(newp ? Py_NewRef(o[10]) : THPVariable_Wrap(fresh)), r2(wop ? Py_NewRef(o[8]) : THPVariable_Wrap(wo));
+    return r0 && r1 && r2 ? PyTuple_Pack(3, r0.get(), r1.get(), r2.get()) : nullptr;
+}
+
+// bind(addresses of the twelve entry points in Bound's order, workspace function, workspace table, torch's raw current stream, whether it is capturing)
+PyObject * bind(PyObject *, PyObject * const * v, Py_ssize_t n) {
+    if (!arg_count(n, 16)) return nullptr;
+    void * p[12];
+    for (int i = 0; i < 12; i++) p[i] = PyLong_AsVoidPtr(v[i]);
+    if (PyErr_Occurred()) return nullptr;
+    REQUIRE(PyCallable_Check(v[12]) && PyDict_Check(v[13]) && PyCallable_Check(v[14]) && PyCallable_Check(v[15]));
     lib.workspace_size = (decltype(lib.workspace_size)) p[0]; lib.attn = (decltype(lib.attn)) p[1];
     lib.kv_write = (decltype(lib.kv_write)) p[2]; lib.kv_write_rope = (decltype(lib.kv_write_rope)) p[3];
     lib.rope = (decltype(lib.rope)) p[4]; lib.mul_mat = (decltype(lib.mul_mat)) p[5];
     lib.copy = (decltype(lib.copy)) p[6]; lib.front_batch = (decltype(lib.front_batch)) p[7];
-    lib.workspace = Py_NewRef(v[8]); lib.workspaces = Py_NewRef(v[9]); lib.raw_stream = Py_NewRef(v[10]);
+    lib.norm_rope = (decltype(lib.norm_rope)) p[8]; lib.gqa_workspace_size = (decltype(lib.gqa_workspace_size)) p[9];
+    lib.gqa_attn = (decltype(lib.gqa_attn)) p[10]; lib.evict = (decltype(lib.evict)) p[11];
+    lib.workspace = Py_NewRef(v[12]); lib.workspaces = Py_NewRef(v[13]); lib.raw_stream = Py_NewRef(v[14]); lib.capturing = Py_NewRef(v[15]);
     Py_RETURN_NONE;
 }
 
@@ -398,7 +632,7 @@ template <PyObject * (*F)(PyObject *, PyObject * const *, Py_ssize_t)> PyObject 
 }
 
 #define FAST(name) { #name, (PyCFunction) (void (*)(void)) entry<name>, METH_FASTCALL, nullptr }
-PyMethodDef methods[] = { FAST(bind), FAST(attn), FAST(rope), FAST(mul_mat), FAST(copy), FAST(kv_write), FAST(front_batch), { nullptr, nullptr, 0, nullptr } };
+PyMethodDef methods[] = { FAST(bind), FAST(attn), FAST(rope), FAST(mul_mat), FAST(copy), FAST(kv_write), FAST(front_batch), FAST(gqa_norm_rope), FAST(gqa_attn), FAST(gqa_evict), { nullptr, nullptr, 0, nullptr } };
 PyModuleDef module = { PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr };
 
 }  // namespace
