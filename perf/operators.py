@@ -239,7 +239,7 @@ def _run_attn(s):
         import jittorinfer_amd as J
         out = J.gqa_attn(s["q"], s["k_cache"], s["v_cache"], s["block_table"], s["seq_lens"], scale=s["scale"], logit_softcap=s["softcap"], window=s["window"],
                          mask=s["row_mask"], weights=s["sums"])
-        return {"out": out, "weights": s["sums"]}
+        return {"out": out if s["dv"] else None, "weights": s["sums"]}
     t, page, live = _rows(s)
     n_seq, kv_heads = s["n_seq"], s["kv_heads"]
     k = s["k_cache"][page, t % PAGE].transpose(1, 2).float()                     # [n_seq, kv_heads, n, dk]
