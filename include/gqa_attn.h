@@ -130,7 +130,7 @@ int    gqa_attn_launch(const gqa_attn_args * args, void * stream);
 typedef struct gqa_evict_args {
     int32_t n_seq, n_head_kv;
     int32_t n_keep, n_sink, n_recent;   /* n_sink + n_recent <= n_keep */
-    int32_t k_row_bytes, v_row_bytes;   /* bytes of a head's row: multiples of 4 (any cache type, Q8_0 latent rows of 612 among them) */
+    int32_t k_row_bytes, v_row_bytes;   /* bytes of a head's row: multiples of 4 from 8 to 16384 (any cache type, Q8_0 latent rows of 612 among them) */
     int32_t _pad;
     gqa_pool k, v;                      /* v.data NULL: keys only */
     int64_t n_pages;
@@ -143,9 +143,12 @@ typedef struct gqa_evict_args {
     int64_t wd_nb1, wd_nb2;
     int32_t * kept;                     /* [n_seq][n_head_kv][n_keep] */
     int32_t * new_lens;                 /* [n_seq]; not seq_lens itself */
+    void *  workspace;                  /* gqa_evict_workspace_size() bytes, 256-byte aligned */
+    size_t  workspace_size;
 } gqa_evict_args;
 
-int gqa_evict_check(const gqa_evict_args * args);
+int    gqa_evict_check(const gqa_evict_args * args);          /* the workspace aside */
+size_t gqa_evict_workspace_size(const gqa_evict_args * args); /* 0 for refused arguments */
 int gqa_evict_launch(const gqa_evict_args * args, void * stream);
 
 #ifdef __cplusplus

@@ -76,8 +76,9 @@ def library():
             getattr(lib, name + "_check").restype = getattr(lib, name + "_launch").restype = C.c_int
             getattr(lib, name + "_check").argtypes = [C.POINTER(cls)]
             getattr(lib, name + "_launch").argtypes = [C.POINTER(cls), C.c_void_p]
-        lib.gqa_attn_workspace_size.restype = C.c_size_t
-        lib.gqa_attn_workspace_size.argtypes = [C.POINTER(GqaAttnArgs)]
+        for name, cls in (("gqa_attn", GqaAttnArgs), ("gqa_evict", GqaEvictArgs)):
+            getattr(lib, name + "_workspace_size").restype = C.c_size_t
+            getattr(lib, name + "_workspace_size").argtypes = [C.POINTER(cls)]
         lib.mla_page_table_create.restype = C.c_void_p
         lib.mla_page_table_create.argtypes = [C.c_int32] * 3
         lib.mla_page_table_free.argtypes = [C.c_void_p]
@@ -121,7 +122,7 @@ def native():
             raise RuntimeError("jittorinfer_amd/_native.so is missing or does not load (%s): build it with `python jittorinfer_amd/build.py`" % e)
         names = ("mla_attn_workspace_size", "mla_attn_launch", "mla_kv_write_launch", "mla_kv_write_rope_launch", "mla_rope_launch",
                  "mla_mul_mat_launch", "mla_copy_f32_launch", "mla_front_batch_launch", "gqa_norm_rope_launch", "gqa_attn_workspace_size",
-                 "gqa_attn_launch", "gqa_evict_launch")
+                 "gqa_attn_launch", "gqa_evict_workspace_size", "gqa_evict_launch")
         mod.bind(*[C.cast(getattr(lib, n), C.c_void_p).value for n in names], _workspace, _workspaces, torch._C._cuda_getCurrentRawStream,
                  torch._C._cuda_isCurrentStreamCapturing)
         _native = mod
@@ -380,7 +381,7 @@ class GqaEvictArgs(C.Structure):
                 ("k_row_bytes", C.c_int32), ("v_row_bytes", C.c_int32), ("_pad", C.c_int32), ("k", GqaPool), ("v", GqaPool),
                 ("n_pages", C.c_int64), ("block_table", C.c_void_p), ("bt_stride", C.c_int64), ("seq_lens", C.c_void_p),
                 ("weights", C.c_void_p), ("w_nb1", C.c_int64), ("w_nb2", C.c_int64), ("weights_dst", C.c_void_p), ("wd_nb1", C.c_int64),
-                ("wd_nb2", C.c_int64), ("kept", C.c_void_p), ("new_lens", C.c_void_p)]
+                ("wd_nb2", C.c_int64), ("kept", C.c_void_p), ("new_lens", C.c_void_p), ("workspace", C.c_void_p), ("workspace_size", C.c_size_t)]
 
 
 def gqa_norm_rope(q, k, v, pos, *, n_dims, mode=0, n_ctx_orig=0, freq_base=10000.0, freq_scale=1.0, ext_factor=0.0, attn_factor=1.0,

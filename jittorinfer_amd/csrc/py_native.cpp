@@ -49,6 +49,7 @@ struct Bound {
     decltype(&gqa_norm_rope_launch)    norm_rope;
     decltype(&gqa_attn_workspace_size) gqa_workspace_size;
     decltype(&gqa_attn_launch)         gqa_attn;
+    decltype(&gqa_evict_workspace_size) evict_workspace_size;
     decltype(&gqa_evict_launch)        evict;
     PyObject * workspace, * workspaces, * raw_stream, * capturing;
 } lib;
@@ -423,6 +424,23 @@ bool gqa_stream(PyObject * o, const at::Tensor & t, bool makes, void *& st) {
     PyErr_SetString(PyExc_ValueError, "a launch on another stream than the current one takes its result tensors from the caller");
     return false;
 }
+// Scratch of a launch.  Under graph capture it is the graph's own: two graphs captured on one stream may be replayed side by side.
+struct GqaScratch {
+    THPObjectPtr ws;
+    at::Tensor   own;
+    template <typename Args> bool take(PyObject * o, const at::Tensor & t, void * st, size_t need, Args & a) {
+        THPObjectPtr capturing(PyObject_CallNoArgs(lib.capturing));
+        if (!capturing) return false;
+        if (capturing.get() == Py_True) {
+            own = at::empty({ (int64_t) need }, t.options().dtype(at::kByte));
+            a.workspace = own.data_ptr(); a.workspace_size = need;
+        } else if (need) {
+            ws = workspace(o, st, need, a);
+            return (bool) ws;
+        }
+        return true;
+    }
+};
 #define SAME_DEVICE(t) REQUIRE(!(t) || (t)->device() == q.device())
 
 // gqa_norm_rope(q, k, v, pos, q_weight, k_weight, eps, n_dims, mode, n_ctx_orig, freq_base, freq_scale, ext_factor, attn_factor, beta_fast,
@@ -545,17 +563,8 @@ PyObject * gqa_attn(PyObject *, PyObject * const * o, Py_ssize_t n) {
         a.dst = out.data_ptr(); a.d_nb1 = out.stride(1) * od; a.d_nb2 = out.stride(0) * od;
     } else a.dst_type = MLA_TYPE_F32;
     const size_t need = lib.gqa_workspace_size(&a);
-    // Under graph capture the scratch is the graph's own: two graphs captured on one stream may be replayed side by side.
-    THPObjectPtr ws, capturing(PyObject_CallNoArgs(lib.capturing));
-    if (!capturing) return nullptr;
-    at::Tensor own;
-    if (capturing.get() == Py_True) {
-        own = at::empty({ (int64_t) need }, q.options().dtype(at::kByte));
-        a.workspace = own.data_ptr(); a.workspace_size = need;
-    } else if (need) {
-        ws = workspace(o[0], st, need, a);
-        if (!ws) return nullptr;
-    }
+    GqaScratch scratch;
+    if (!scratch.take(o[0], q, st, need, a)) return nullptr;
     const int rc = unlocked([&] { return lib.gqa_attn(&a, st); });
     if (rc) return failed("gqa_attn_launch", rc);
     return made.defined() ? THPVariable_Wrap(made) : Py_NewRef(vc ? o[10] : o[9]);
@@ -599,26 +608,29 @@ PyObject * gqa_evict(PyObject *, PyObject * const * o, Py_ssize_t n) {
     REQUIRE(ints(fresh, n_seq));
     a.weights_dst = (float *) wo.data_ptr(); a.wd_nb1 = wo.stride(1) * 4; a.wd_nb2 = wo.stride(0) * 4;
     a.kept = (int32_t *) kept.data_ptr(); a.new_lens = (int32_t *) fresh.data_ptr();
+    GqaScratch scratch;
+    if (!scratch.take(o[0], q, st, lib.evict_workspace_size(&a), a)) return nullptr;
     const int rc = unlocked([&] { return lib.evict(&a, st); });
     if (rc) return failed("gqa_evict_launch", rc);
     THPObjectPtr r0(keptp ? Py_NewRef(o[9]) : THPVariable_Wrap(kept)), r1(newp ? Py_NewRef(o[10]) : THPVariable_Wrap(fresh)), r2(wop ? Py_NewRef(o[8]) : THPVariable_Wrap(wo));
     return r0 && r1 && r2 ? PyTuple_Pack(3, r0.get(), r1.get(), r2.get()) : nullptr;
 }
 
-// bind(addresses of the twelve entry points in Bound's order, workspace function, workspace table, torch's raw current stream, whether it is capturing)
+// bind(addresses of the thirteen entry points in Bound's order, workspace function, workspace table, torch's raw current stream, whether it is capturing)
 PyObject * bind(PyObject *, PyObject * const * v, Py_ssize_t n) {
-    if (!arg_count(n, 16)) return nullptr;
-    void * p[12];
-    for (int i = 0; i < 12; i++) p[i] = PyLong_AsVoidPtr(v[i]);
+    if (!arg_count(n, 17)) return nullptr;
+    void * p[13];
+    for (int i = 0; i < 13; i++) p[i] = PyLong_AsVoidPtr(v[i]);
     if (PyErr_Occurred()) return nullptr;
-    REQUIRE(PyCallable_Check(v[12]) && PyDict_Check(v[13]) && PyCallable_Check(v[14]) && PyCallable_Check(v[15]));
+    REQUIRE(PyCallable_Check(v[13]) && PyDict_Check(v[14]) && PyCallable_Check(v[15]) && PyCallable_Check(v[16]));
     lib.workspace_size = (decltype(lib.workspace_size)) p[0]; lib.attn = (decltype(lib.attn)) p[1];
     lib.kv_write = (decltype(lib.kv_write)) p[2]; lib.kv_write_rope = (decltype(lib.kv_write_rope)) p[3];
     lib.rope = (decltype(lib.rope)) p[4]; lib.mul_mat = (decltype(lib.mul_mat)) p[5];
     lib.copy = (decltype(lib.copy)) p[6]; lib.front_batch = (decltype(lib.front_batch)) p[7];
     lib.norm_rope = (decltype(lib.norm_rope)) p[8]; lib.gqa_workspace_size = (decltype(lib.gqa_workspace_size)) p[9];
-    lib.gqa_attn = (decltype(lib.gqa_attn)) p[10]; lib.evict = (decltype(lib.evict)) p[11];
-    lib.workspace = Py_NewRef(v[12]); lib.workspaces = Py_NewRef(v[13]); lib.raw_stream = Py_NewRef(v[14]); lib.capturing = Py_NewRef(v[15]);
+    lib.gqa_attn = (decltype(lib.gqa_attn)) p[10]; lib.evict_workspace_size = (decltype(lib.evict_workspace_size)) p[11];
+    lib.evict = (decltype(lib.evict)) p[12];
+    lib.workspace = Py_NewRef(v[13]); lib.workspaces = Py_NewRef(v[14]); lib.raw_stream = Py_NewRef(v[15]); lib.capturing = Py_NewRef(v[16]);
     Py_RETURN_NONE;
 }
 

@@ -176,7 +176,7 @@ CUT_REFUSED = [
     (dict(n_seq=-1), SHAPE), (dict(n_head_kv=0), SHAPE), (dict(n_keep=0), SHAPE), (dict(n_sink=-1), SHAPE), (dict(n_recent=-1), SHAPE), (dict(n_sink=60, n_recent=41), SHAPE),
     (dict(n_sink=2 ** 31 - 1, n_recent=2 ** 31 - 1), SHAPE), (dict(n_pages=0), SHAPE), (dict(bt_stride=0), SHAPE), (dict(bt_stride=1 << 23), SHAPE), (dict(n_seq=40000), SHAPE),
     (dict(weights=None), NULL), (dict(weights_dst=None), NULL), (dict(kept=None), NULL), (dict(new_lens=None), NULL), (dict(block_table=None), NULL), (dict(seq_lens=None), NULL), (dict(k__data=None), NULL),
-    (dict(k_row_bytes=255), ALIGN), (dict(k_row_bytes=0), SHAPE), (dict(v__nb_row=511), ALIGN), (dict(v__data=(1 << 24) + 1), ALIGN), (dict(k__nb_head=-256), SHAPE),
+    (dict(k_row_bytes=255), ALIGN), (dict(k_row_bytes=0), SHAPE), (dict(k_row_bytes=4), SHAPE), (dict(v_row_bytes=16388), SHAPE), (dict(v__nb_row=511), ALIGN), (dict(v__data=(1 << 24) + 1), ALIGN), (dict(k__nb_head=-256), SHAPE),
     (dict(weights=32769), ALIGN), (dict(wd_nb2=4095), ALIGN), (dict(weights_dst=32768, wd_nb1=4096), SHAPE), (dict(new_lens=16384), UNSUPPORTED),
 ]
 
@@ -195,6 +195,12 @@ def test_evict_accepts():
     for kw in (dict(), dict(v=J.GqaPool(), v_row_bytes=0), dict(k_row_bytes=612), dict(weights_dst=32768), dict(n_sink=0, n_recent=100), dict(n_seq=0, weights=None)):
         a = _cut(**kw)
         assert lib.gqa_evict_check(C.byref(a)) == 0, kw
+    a = _cut()
+    need = lib.gqa_evict_workspace_size(C.byref(a))
+    assert need > 0 and lib.gqa_evict_launch(C.byref(a), None) == WORKSPACE
+    a.workspace, a.workspace_size = 1 << 30, need - 1
+    assert lib.gqa_evict_launch(C.byref(a), None) == WORKSPACE
+    assert lib.gqa_evict_workspace_size(C.byref(_cut(n_keep=0))) == 0
 
 
 def test_exports_and_mirrors_match_the_header(tmp_path):
@@ -202,7 +208,7 @@ def test_exports_and_mirrors_match_the_header(tmp_path):
     text = open(os.path.join(ROOT, "include", "gqa_attn.h")).read()
     bare = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
     declared = set(re.findall(r"\b(gqa_\w+)\s*\(", bare))
-    assert declared == {p + s for p in ("gqa_norm_rope", "gqa_attn", "gqa_evict") for s in ("_check", "_launch")} | {"gqa_attn_workspace_size"}
+    assert declared == {p + s for p in ("gqa_norm_rope", "gqa_attn", "gqa_evict") for s in ("_check", "_launch")} | {"gqa_attn_workspace_size", "gqa_evict_workspace_size"}
     for name in declared:
         assert hasattr(J.library(), name)
     mirrors = {"gqa_pool": J.GqaPool, "gqa_norm_rope_args": J.GqaNormRopeArgs, "gqa_attn_args": J.GqaAttnArgs, "gqa_evict_args": J.GqaEvictArgs}
