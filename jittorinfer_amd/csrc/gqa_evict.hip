@@ -18,7 +18,9 @@ using namespace mla;
 namespace {
 
 constexpr int PAGE = MLA_PAGE_TOKENS;
-constexpr int SEL_THREADS = 1024, SEL_PER = 8, SEL_RUNS = 4, SEL_CHUNK = SEL_THREADS * SEL_PER * SEL_RUNS;
+constexpr int SEL_THREADS = 1024, SEL_PER = 8, SEL_RUN = SEL_THREADS * SEL_PER, SEL_RUNS = 4, SEL_CHUNK = SEL_RUN * SEL_RUNS;
+constexpr int SEL_ONE = SEL_CHUNK;                   // rows up to which one workgroup a group selects
+constexpr int SEL_MANY = 8192;                       // runs of 8192 rows up to which several do: beyond, the groups alone fill the chip, and the histograms 128 MB
 constexpr int BINS = 2048;
 
 struct EvictP {
@@ -51,27 +53,105 @@ __device__ __forceinline__ int scan_wave(int v, int lane) {       // inclusive
     return v;
 }
 
+// The digit at which the rows of a histogram, counted from the largest digit down, reach `left`, and how many of the digit's own rows those are.
+// One wave: lane t sums the 32 bins 2047 - 32 t and down (rotated, so that the lanes meet different banks), a scan finds the lane, another the bin.
+struct Pick { unsigned digit; int left; };
+__device__ __forceinline__ Pick pick(const unsigned * hist, int left, int lane) {
+    int sum = 0;
+#pragma unroll
+    for (int i = 0; i < 32; i++) sum += (int) hist[BINS - 1 - 32 * lane - ((i + lane) & 31)];
+    const int incl = scan_wave(sum, lane);
+    const int at   = __ffsll(__ballot(incl - sum < left && incl >= left)) - 1;
+    const int base = __shfl(incl - sum, at, 64);
+    const int bin  = BINS - 1 - 32 * at - (lane & 31);
+    const int mine = lane < 32 ? (int) hist[bin] : 0;
+    const int upto = base + scan_wave(mine, lane);
+    const int win  = __ffsll(__ballot(lane < 32 && upto - mine < left && upto >= left)) - 1;
+    return Pick{ (unsigned) __shfl(bin, win, 64), left - __shfl(upto - mine, win, 64) };
+}
+
+// Digits of a key, from the top: 11, 11 and 10 bits.
+__device__ __forceinline__ constexpr int shift_of(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
+__device__ __forceinline__ constexpr int bits_of(int pass) { return pass == 2 ? 10 : 11; }
+
+// What a (sequence, KV head) has to decide.
+struct Group {
+    int n, c0, c1, places;                                         // rows; those that compete: [c0, c1), for so many places
+    const float * w; float * wd; int32_t * kept;
+};
+__device__ __forceinline__ Group group_of(const EvictP & p, int group) {
+    Group g;
+    const int b = group / p.n_head_kv, h = group - b * p.n_head_kv;
+    g.n  = len_of(p, b);
+    g.c0 = p.n_sink; g.c1 = g.n - p.n_recent;                      // (c0 < c1 where rows leave: n_sink + n_recent <= n_keep < n)
+    g.places = p.n_keep - p.n_sink - p.n_recent;
+    g.w  = (const float *) (p.w + (int64_t) b * p.w_nb2 + (int64_t) h * p.w_nb1);
+    g.wd = (float *) (p.wd + (int64_t) b * p.wd_nb2 + (int64_t) h * p.wd_nb1);
+    g.kept = p.kept + (int64_t) group * p.n_keep;
+    return g;
+}
+
+// 8 rows from i0 on; past the length nothing is read.
+__device__ __forceinline__ void load_rows(const Group & g, int i0, float (&x)[SEL_PER]) {
+    if (((uintptr_t) g.w & 15) == 0 && i0 + SEL_PER <= g.n) {
+        const f32x4 a = *(const f32x4 *) (g.w + i0), c = *(const f32x4 *) (g.w + i0 + 4);
+#pragma unroll
+        for (int e = 0; e < 4; e++) { x[e] = a[e]; x[4 + e] = c[e]; }
+    } else {
+#pragma unroll
+        for (int e = 0; e < SEL_PER; e++) x[e] = i0 + e < g.n ? g.w[i0 + e] : 0.f;
+    }
+}
+__device__ __forceinline__ void count_rows(const Group & g, int i0, const float (&x)[SEL_PER], int pass, unsigned prefix, unsigned * hist) {
+#pragma unroll
+    for (int e = 0; e < SEL_PER; e++) {
+        const unsigned k = key_of(x[e]);
+        if (i0 + e >= g.c0 && i0 + e < g.c1 && (pass == 0 || (k >> (shift_of(pass) + bits_of(pass))) == prefix))
+            atomicAdd(&hist[(k >> shift_of(pass)) & ((1u << bits_of(pass)) - 1)], 1u);
+    }
+}
+// Of 8 rows: those that stay whatever the others do (bits 0 .. 7), and those equal to the smallest weight that stays, `last` (bits 16 ..).
+__device__ __forceinline__ unsigned sort_rows(const Group & g, int i0, const float (&x)[SEL_PER], unsigned last) {
+    unsigned m = 0;
+#pragma unroll
+    for (int e = 0; e < SEL_PER; e++) {
+        const int i = i0 + e;
+        const unsigned k = key_of(x[e]);
+        const bool in = i < g.n, held = i < g.c0 || i >= g.c1;
+        if (in && (held || (g.places > 0 && k > last))) m |= 1u << e;
+        else if (in && g.places > 0 && k == last) m |= 0x10000u << e;
+    }
+    return m;
+}
+__device__ __forceinline__ int count_both(unsigned m) { return __popc(m & 0xffffu) | (__popc(m >> 16) << 16); }
+// Writes them out: `sure` rows kept for certain and `ties` equal ones come before these 8.
+__device__ __forceinline__ void place_rows(const Group & g, int i0, const float (&x)[SEL_PER], unsigned m, int sure, int ties, int left) {
+#pragma unroll
+    for (int e = 0; e < SEL_PER; e++) {
+        const bool is_sure = m >> e & 1, is_tie = m >> (16 + e) & 1;
+        if (is_sure || (is_tie && ties < left)) {
+            const int j = sure + min(ties, left);
+            g.kept[j] = i0 + e;
+            g.wd[j]   = x[e];
+        }
+        sure += is_sure; ties += is_tie;
+    }
+}
+
+// One workgroup a group.
 __global__ void __launch_bounds__(SEL_THREADS) gqa_select_kernel(const EvictP p) {
-    __shared__ unsigned hist[BINS];
+    __shared__ unsigned hist[2][BINS];
     __shared__ int      part[SEL_RUNS][16];
-    __shared__ unsigned sh_digit;
-    __shared__ int      sh_left;
-    const int b = blockIdx.x / p.n_head_kv, h = blockIdx.x - b * p.n_head_kv;
+    __shared__ Pick     sh_pick;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int n = len_of(p, b), m = min(n, p.n_keep);
-    const float * w  = (const float *) (p.w + (int64_t) b * p.w_nb2 + (int64_t) h * p.w_nb1);
-    float *       wd = (float *) (p.wd + (int64_t) b * p.wd_nb2 + (int64_t) h * p.wd_nb1);
-    int32_t *     kept = p.kept + (int64_t) blockIdx.x * p.n_keep;
-    if (h == 0 && tid == 0) p.new_lens[b] = m;
+    const Group g = group_of(p, blockIdx.x);
+    if (blockIdx.x % p.n_head_kv == 0 && tid == 0) p.new_lens[blockIdx.x / p.n_head_kv] = min(g.n, p.n_keep);
     for (int i = blockIdx.x * SEL_THREADS + tid; i < p.n_sync; i += gridDim.x * SEL_THREADS) p.sync[i] = 0u;
-    if (n <= p.n_keep) {                                           // nothing leaves
-        for (int i = tid; i < p.n_keep; i += SEL_THREADS) kept[i] = i < n ? i : -1;
-        for (int64_t i = tid; i < p.cap; i += SEL_THREADS) wd[i] = i < n ? w[i] : 0.f;
+    if (g.n <= p.n_keep) {                                         // nothing leaves
+        for (int i = tid; i < p.n_keep; i += SEL_THREADS) g.kept[i] = i < g.n ? i : -1;
+        for (int64_t i = tid; i < p.cap; i += SEL_THREADS) g.wd[i] = i < g.n ? g.w[i] : 0.f;
         return;
     }
-    const int  c0 = p.n_sink, c1 = n - p.n_recent;                 // the rows that compete (c0 < c1: n_sink + n_recent <= n_keep < n)
-    const int  places = p.n_keep - p.n_sink - p.n_recent;
-    const bool vec = ((uintptr_t) w & 15) == 0;
     // A chunk: 4 runs of 8192 rows, 8 consecutive ones a thread in each.  All its loads are under way at once, and a sequence of one chunk
     // (32768 rows) is read once: its rows stay in registers over the passes.
     float x[SEL_RUNS][SEL_PER];
@@ -80,100 +160,150 @@ __global__ void __launch_bounds__(SEL_THREADS) gqa_select_kernel(const EvictP p)
         if (base == held) return;
         held = base;
 #pragma unroll
-        for (int g = 0; g < SEL_RUNS; g++) {
-            const int i0 = base + (g * SEL_THREADS + tid) * SEL_PER;       // rows past the length: nothing is read
-            if (vec && i0 + SEL_PER <= n) {
-                const f32x4 a = *(const f32x4 *) (w + i0), c = *(const f32x4 *) (w + i0 + 4);
-#pragma unroll
-                for (int e = 0; e < 4; e++) { x[g][e] = a[e]; x[g][4 + e] = c[e]; }
-            } else if (base + g * SEL_THREADS * SEL_PER < n) {
-#pragma unroll
-                for (int e = 0; e < SEL_PER; e++) x[g][e] = i0 + e < n ? w[i0 + e] : 0.f;
-            }
-        }
+        for (int r = 0; r < SEL_RUNS; r++) if (base + r * SEL_RUN < g.n) load_rows(g, base + r * SEL_RUN + tid * SEL_PER, x[r]);
     };
-
-    unsigned prefix = 0;                                           // the digits found so far
-    int      left = places;                                        // rows still to be taken among those that share them
-    if (places > 0) {
+    Pick got{ 0u, g.places };                                      // the digits found so far; rows still to be taken among those that share them
+    if (g.places > 0) {
+        hist[0][2 * tid] = hist[0][2 * tid + 1] = 0u;
+        load(0);
+        __syncthreads();
+#pragma unroll
         for (int pass = 0; pass < 3; pass++) {
-            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-            for (int i = tid; i < BINS; i += SEL_THREADS) hist[i] = 0;
-            __syncthreads();
-            for (int base = 0; base < c1; base += SEL_CHUNK) {
+            unsigned * now = hist[pass & 1], * next = hist[(pass & 1) ^ 1];
+            for (int base = 0; base < g.c1; base += SEL_CHUNK) {
                 load(base);
 #pragma unroll
-                for (int g = 0; g < SEL_RUNS; g++) {
-                    const int i0 = base + (g * SEL_THREADS + tid) * SEL_PER;
-                    if (base + g * SEL_THREADS * SEL_PER >= c1) continue;
-#pragma unroll
-                    for (int e = 0; e < SEL_PER; e++) {
-                        const int i = i0 + e;
-                        const unsigned k = key_of(x[g][e]);
-                        if (i >= c0 && i < c1 && (pass == 0 || (k >> (shift + bits)) == prefix)) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
-                    }
-                }
+                for (int r = 0; r < SEL_RUNS; r++) if (base + r * SEL_RUN < g.c1) count_rows(g, base + r * SEL_RUN + tid * SEL_PER, x[r], pass, got.digit, now);
+            }
+            next[2 * tid] = next[2 * tid + 1] = 0u;
+            __syncthreads();
+            if (wave == 0) {
+                const Pick q = pick(now, got.left, lane);
+                if (lane == 0) sh_pick = q;
             }
             __syncthreads();
-            // the digit at which the rows from the top on reach `left`: thread t holds bins 2047 - 2t and 2046 - 2t
-            const int hi = (int) hist[BINS - 1 - 2 * tid], lo = (int) hist[BINS - 2 - 2 * tid];
-            int incl = scan_wave(hi + lo, lane);
-            if (lane == 63) part[0][wave] = incl;
-            __syncthreads();
-            for (int q = 0; q < wave; q++) incl += part[0][q];
-            const int above = incl - hi - lo;
-            if (above < left && incl >= left) {
-                const bool first = above + hi >= left;
-                sh_digit = (unsigned) (BINS - 1 - 2 * tid - (first ? 0 : 1));
-                sh_left  = left - above - (first ? 0 : hi);
-            }
-            __syncthreads();
-            prefix = (prefix << bits) | sh_digit;
-            left   = sh_left;
-            __syncthreads();
+            got.digit = (got.digit << bits_of(pass)) | sh_pick.digit;
+            got.left  = sh_pick.left;
         }
     }
-    // prefix: the key of the smallest weight that stays, `left` rows of which do
-    int taken = 0, ties = 0;                                       // rows before this run: surely kept, and equal to the smallest
-    for (int base = 0; base < n; base += SEL_CHUNK) {
+    // got: the key of the smallest weight that stays, and how many rows of it do
+    int sure = 0, ties = 0;                                        // rows before this run
+    for (int base = 0; base < g.n; base += SEL_CHUNK) {
         load(base);
-        int sure[SEL_RUNS], tie[SEL_RUNS], incl[SEL_RUNS];         // bit e: row 8 (..) + e of the run
+        unsigned m[SEL_RUNS];
+        int      incl[SEL_RUNS];
 #pragma unroll
-        for (int g = 0; g < SEL_RUNS; g++) {
-            sure[g] = tie[g] = 0;
-#pragma unroll
-            for (int e = 0; e < SEL_PER; e++) {
-                const int i = base + (g * SEL_THREADS + tid) * SEL_PER + e;
-                if (i >= n) continue;
-                const unsigned k = key_of(x[g][e]);
-                if (i < c0 || i >= c1 || (places > 0 && k > prefix)) sure[g] |= 1 << e;
-                else if (places > 0 && k == prefix) tie[g] |= 1 << e;
-            }
-            incl[g] = scan_wave(__popc(sure[g]) | (__popc(tie[g]) << 16), lane);     // (at most 8192 of either in a run)
-            if (lane == 63) part[g][wave] = incl[g];
+        for (int r = 0; r < SEL_RUNS; r++) {
+            m[r] = base + r * SEL_RUN < g.n ? sort_rows(g, base + r * SEL_RUN + tid * SEL_PER, x[r], got.digit) : 0u;
+            incl[r] = scan_wave(count_both(m[r]), lane);           // (at most 8192 of either in a run)
+            if (lane == 63) part[r][wave] = incl[r];
         }
         __syncthreads();                                           // (also: every row of the chunk has been read before one is overwritten)
 #pragma unroll
-        for (int g = 0; g < SEL_RUNS; g++) {
-            if (base + g * SEL_THREADS * SEL_PER >= n) continue;
-            int before = incl[g] - (__popc(sure[g]) | (__popc(tie[g]) << 16)), all = 0;
-            for (int q = 0; q < 16; q++) { if (q < wave) before += part[g][q]; all += part[g][q]; }
-            int s = taken + (before & 0xffff), t = ties + (before >> 16);
-#pragma unroll
-            for (int e = 0; e < SEL_PER; e++) {
-                const bool is_sure = sure[g] >> e & 1, is_tie = tie[g] >> e & 1;
-                if (is_sure || (is_tie && t < left)) {
-                    const int j = s + min(t, left);
-                    kept[j] = base + (g * SEL_THREADS + tid) * SEL_PER + e;
-                    wd[j]   = x[g][e];
-                }
-                s += is_sure; t += is_tie;
-            }
-            taken += all & 0xffff; ties += all >> 16;
+        for (int r = 0; r < SEL_RUNS; r++) {
+            if (base + r * SEL_RUN >= g.n) continue;
+            const int upto = scan_wave(lane < 16 ? part[r][lane] : 0, lane);
+            const int all = __shfl(upto, 15, 64), ahead = wave ? __shfl(upto, wave - 1, 64) : 0;
+            const int before = ahead + incl[r] - count_both(m[r]);
+            place_rows(g, base + r * SEL_RUN + tid * SEL_PER, x[r], m[r], sure + (before & 0xffff), ties + (before >> 16), got.left);
+            sure += all & 0xffff; ties += all >> 16;
         }
         __syncthreads();
     }
-    for (int64_t i = p.n_keep + tid; i < p.cap; i += SEL_THREADS) wd[i] = 0.f;
+    for (int64_t i = p.n_keep + tid; i < p.cap; i += SEL_THREADS) g.wd[i] = 0.f;
+}
+
+// The same over several workgroups a group, a run of 8192 rows each, in four launches: PASS 0, 1, 2 leave every run's histogram of a digit,
+// PASS 1, 2, 3 add up those of the pass before and pick its digit, each workgroup for itself.  PASS 3 writes the rows that stay, behind those of the
+// runs in front: every run publishes its two counts (in one word, that is its flag too) and waits for the words of the runs before it; runs are
+// numbered by a ticket and publish before they wait, so they wait for running workgroups only.
+struct Rank { unsigned * hist; uint64_t * counts; Pick * picks; unsigned * ticket; int runs; };   // hist [2][groups][runs][BINS], counts [groups][runs], picks [groups][2]
+
+template <int PASS>
+__global__ void __launch_bounds__(SEL_THREADS) gqa_rank_kernel(const EvictP p, const Rank k) {
+    __shared__ unsigned hist[BINS];
+    __shared__ int      part[16];
+    __shared__ Pick     sh_pick;
+    __shared__ unsigned sh_ticket;
+    __shared__ unsigned long long sh_before;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int groups = p.n_seq * p.n_head_kv;
+    int number = (int) blockIdx.x;
+    if constexpr (PASS == 0) {
+        for (int i = blockIdx.x * SEL_THREADS + tid; i < p.n_sync; i += gridDim.x * SEL_THREADS) p.sync[i] = 0u;
+        if (tid == 0) k.counts[blockIdx.x] = 0;
+        if (blockIdx.x == 0 && tid == 0) *k.ticket = 0u;
+    }
+    if constexpr (PASS == 3) {
+        if (tid == 0) { sh_ticket = __hip_atomic_fetch_add(k.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); sh_before = 0; }
+        __syncthreads();
+        number = (int) sh_ticket;
+    }
+    const int   run = number / groups, group = number - run * groups;      // a group's first run before any group's second
+    const Group g = group_of(p, group);
+    const int   i0 = run * SEL_RUN + tid * SEL_PER;
+    if constexpr (PASS < 3) {
+        if (g.n <= p.n_keep || g.places == 0) return;
+    } else {
+        if (run == 0 && group % p.n_head_kv == 0 && tid == 0) p.new_lens[group / p.n_head_kv] = min(g.n, p.n_keep);
+        if (g.n <= p.n_keep) {
+            const int64_t end = run == k.runs - 1 ? (p.cap > p.n_keep ? p.cap : p.n_keep) : (int64_t) (run + 1) * SEL_RUN;
+            for (int64_t i = (int64_t) run * SEL_RUN + tid; i < end; i += SEL_THREADS) {
+                if (i < p.n_keep) g.kept[i] = i < g.n ? (int) i : -1;
+                if (i < p.cap) g.wd[i] = i < g.n ? g.w[i] : 0.f;
+            }
+            return;
+        }
+    }
+    float x[SEL_PER];
+    load_rows(g, i0, x);
+    Pick got{ 0u, g.places };
+    if (PASS > 0 && g.places > 0) {
+        const unsigned * from = k.hist + ((size_t) ((PASS - 1) & 1) * groups + group) * k.runs * BINS;
+        const int        live = min(k.runs, (g.c1 + SEL_RUN - 1) / SEL_RUN);
+        unsigned a = 0, c = 0;
+        for (int r = 0; r < live; r++) { a += from[r * BINS + tid]; c += from[r * BINS + SEL_THREADS + tid]; }
+        hist[tid] = a; hist[SEL_THREADS + tid] = c;
+        if constexpr (PASS > 1) got = k.picks[group * 2 + (PASS & 1)];      // the pass before's: digits but the last
+        __syncthreads();
+        if (wave == 0) {
+            const Pick q = pick(hist, got.left, lane);
+            if (lane == 0) sh_pick = q;
+        }
+        __syncthreads();
+        got.digit = (got.digit << bits_of(PASS - 1)) | sh_pick.digit;
+        got.left  = sh_pick.left;
+        if (PASS < 3 && run == 0 && tid == 0) k.picks[group * 2 + ((PASS + 1) & 1)] = got;
+    }
+    if constexpr (PASS < 3) {
+        if (run * SEL_RUN >= g.c1) return;
+        hist[tid] = hist[SEL_THREADS + tid] = 0u;
+        __syncthreads();
+        count_rows(g, i0, x, PASS, got.digit, hist);
+        __syncthreads();
+        unsigned * to = k.hist + (((size_t) (PASS & 1) * groups + group) * k.runs + run) * BINS;
+        to[tid] = hist[tid]; to[SEL_THREADS + tid] = hist[SEL_THREADS + tid];
+    } else {
+        const unsigned m = sort_rows(g, i0, x, got.digit);
+        const int incl = scan_wave(count_both(m), lane);
+        if (lane == 63) part[wave] = incl;
+        __syncthreads();                                           // (every row of the run is in a register: it may be overwritten from here on)
+        const int upto = scan_wave(lane < 16 ? part[lane] : 0, lane);
+        const int all = __shfl(upto, 15, 64), ahead = wave ? __shfl(upto, wave - 1, 64) : 0;
+        uint64_t * counts = k.counts + (size_t) group * k.runs;
+        if (tid == 0) __hip_atomic_store(counts + run, (uint64_t) 1 << 63 | (uint64_t) (all >> 16) << 31 | (uint64_t) (all & 0xffff), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (int r = tid; r < run; r += SEL_THREADS) {             // (sums below 2^31 in each half)
+            uint64_t v;
+            while (!((v = __hip_atomic_load(counts + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) >> 63)) __builtin_amdgcn_s_sleep(1);
+            atomicAdd(&sh_before, (unsigned long long) (v << 1 >> 1));
+        }
+        __syncthreads();
+        const int sure = (int) (sh_before & 0x7fffffffu), ties = (int) (sh_before >> 31);
+        const int before = ahead + incl - count_both(m);
+        place_rows(g, i0, x, m, sure + (before & 0xffff), ties + (before >> 16), got.left);
+        const int64_t end = min((int64_t) (run + 1) * SEL_RUN, p.cap);      // the run's own share of the rows past the new length
+        for (int64_t i = max((int64_t) run * SEL_RUN, (int64_t) p.n_keep) + tid; i < end; i += SEL_THREADS) g.wd[i] = 0.f;
+    }
 }
 
 constexpr int MOVE_THREADS = 512, MOVE_R = 12, MOVE_UNITS = MOVE_THREADS * MOVE_R;     // units a workgroup holds in registers: 96 KB of 16 bytes each
@@ -260,7 +390,8 @@ struct Plan {
     bool    w16;              // units of 16 bytes, else of 4
     Seg     k, v;
     int64_t segments;         // of all heads, K and V
-    size_t  bytes;            // of the workspace: the ticket and a flag a segment
+    int     runs;             // of the selection over several workgroups; 0: one
+    size_t  off_ticket, off_counts, off_picks, off_hist, bytes;    // of the workspace: the move's ticket and a flag a segment come first
 };
 
 Plan make_plan(const gqa_evict_args * a) {
@@ -270,7 +401,17 @@ Plan make_plan(const gqa_evict_args * a) {
     pl.k = make_seg(a->k_row_bytes, pl.w16 ? 16 : 4, n_keep);
     pl.v = a->v.data ? make_seg(a->v_row_bytes, pl.w16 ? 16 : 4, n_keep) : Seg{ 1, 1, 0, 0u };
     pl.segments = (int64_t) a->n_seq * a->n_head_kv * (pl.k.count + pl.v.count);
-    pl.bytes = (size_t) (1 + pl.segments) * 4;
+    const size_t groups = (size_t) a->n_seq * a->n_head_kv;
+    const int64_t runs = (cap + SEL_RUN - 1) / SEL_RUN;
+    pl.runs = cap > SEL_ONE && n_keep && (int64_t) groups * runs <= SEL_MANY ? (int) runs : 0;
+    size_t at = 0;
+    auto take = [&](size_t n) { const size_t o = at; at += (n + 255) & ~(size_t) 255; return o; };
+    take((size_t) (1 + pl.segments) * 4);
+    pl.off_ticket = take(4);
+    pl.off_counts = take(groups * pl.runs * 8);
+    pl.off_picks  = take(groups * 2 * sizeof(Pick));
+    pl.off_hist   = take(groups * 2 * pl.runs * BINS * 4);
+    pl.bytes = at;
     return pl;
 }
 
@@ -314,7 +455,15 @@ extern "C" int gqa_evict_launch(const gqa_evict_args * a, void * stream) {
     if (!a->workspace || ((uintptr_t) a->workspace & 255) || a->workspace_size < pl.bytes) return MLA_ERR_WORKSPACE;
     const unsigned groups = (unsigned) (a->n_seq * a->n_head_kv);
     p.sync = (unsigned *) a->workspace; p.n_sync = (int) (1 + pl.segments);
-    hipLaunchKernelGGL(gqa_select_kernel, dim3(groups), dim3(SEL_THREADS), 0, (hipStream_t) stream, p);
+    if (pl.runs) {
+        char * ws = (char *) a->workspace;
+        const Rank k{ (unsigned *) (ws + pl.off_hist), (uint64_t *) (ws + pl.off_counts), (Pick *) (ws + pl.off_picks), (unsigned *) (ws + pl.off_ticket), pl.runs };
+        const dim3 grid(groups * (unsigned) pl.runs);
+        hipLaunchKernelGGL(gqa_rank_kernel<0>, grid, dim3(SEL_THREADS), 0, (hipStream_t) stream, p, k);
+        hipLaunchKernelGGL(gqa_rank_kernel<1>, grid, dim3(SEL_THREADS), 0, (hipStream_t) stream, p, k);
+        hipLaunchKernelGGL(gqa_rank_kernel<2>, grid, dim3(SEL_THREADS), 0, (hipStream_t) stream, p, k);
+        hipLaunchKernelGGL(gqa_rank_kernel<3>, grid, dim3(SEL_THREADS), 0, (hipStream_t) stream, p, k);
+    } else hipLaunchKernelGGL(gqa_select_kernel, dim3(groups), dim3(SEL_THREADS), 0, (hipStream_t) stream, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int) e;
     if (pl.segments == 0) return 0;

@@ -122,25 +122,23 @@ def evict(weights, bt, lens, k_cache, v_cache, n_keep, n_sink, n_recent):
         n = min(max(int(lens[b]), 0), cap)
         new_lens[b] = min(n, n_keep)
         for h in range(kv_heads):
-            rows = list(range(n))
+            rows = torch.arange(n)
             if n > n_keep:
                 middle = rows[n_sink:n - n_recent]
-                w = weights[b, h].tolist()
-                key = [float("-inf") if math.isnan(w[i]) else w[i] for i in middle]
-                nan = [1 if math.isnan(w[i]) else 0 for i in middle]          # below -inf itself
-                order = sorted(range(len(middle)), key=lambda j: (nan[j], -key[j], j))
-                rows = rows[:n_sink] + sorted(middle[j] for j in order[:n_keep - n_sink - n_recent]) + rows[n - n_recent:]
-            kept[b, h, :len(rows)] = torch.tensor(rows, dtype=torch.int32)
+                w = weights[b, h, middle]
+                nan = torch.isnan(w)                                          # below -inf itself
+                order = torch.argsort(torch.where(nan, float("-inf"), w), descending=True, stable=True)
+                order = order[torch.argsort(nan[order].int(), stable=True)]
+                rows = torch.cat((rows[:n_sink], middle[order[:n_keep - n_sink - n_recent]].sort().values, rows[n - n_recent:]))
+            kept[b, h, :len(rows)] = rows.int()
             out[b, h, :len(rows)] = weights[b, h, rows]
-            for j, i in enumerate(rows):
-                if i == j:
-                    continue
-                src, dst = int(bt[b, i // PAGE]), int(bt[b, j // PAGE])
-                if not (0 <= src < k_cache.shape[0] and 0 <= dst < k_cache.shape[0]):
-                    continue
-                k_new[dst, j % PAGE, h] = k_cache[src, i % PAGE, h]
-                if v_new is not None:
-                    v_new[dst, j % PAGE, h] = v_cache[src, i % PAGE, h]
+            to = torch.arange(len(rows))
+            page = lambda i: bt[b].long()[i // PAGE]
+            there = (page(rows) >= 0) & (page(rows) < k_cache.shape[0]) & (page(to) >= 0) & (page(to) < k_cache.shape[0])
+            rows, to = rows[there], to[there]
+            k_new[page(to), to % PAGE, h] = k_cache[page(rows), rows % PAGE, h]
+            if v_new is not None:
+                v_new[page(to), to % PAGE, h] = v_cache[page(rows), rows % PAGE, h]
     return kept, new_lens, out, k_new, v_new
 
 

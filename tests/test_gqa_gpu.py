@@ -505,8 +505,49 @@ def test_evict_ties_and_odd_weights(gpu, kind):
     _check_evict(gpu, w, bt, lens, k, v, 2400, 0, 0, in_place=True)
 
 
+@pytest.mark.parametrize("kind", ["spread", "equal", "few", "odd"])
+def test_evict_sequences_selected_by_several_workgroups(gpu, kind):
+    """Block tables of more than 32768 rows: lengths that end inside a run of 8192, fill some of the runs, and are not cut at all."""
+    lens = [40000, 33000, 8192, 8193, 30000, 100, 20000]
+    w, bt, lens, k, _ = _evict_case(46, lens, 313, 1, 16, 0, BF16)
+    gen = torch.Generator().manual_seed(46)
+    if kind == "equal":
+        w[:] = 2.5
+    elif kind == "few":
+        w = torch.randint(0, 3, w.shape, generator=gen).float()
+    elif kind == "odd":
+        r = torch.rand(w.shape, generator=gen)
+        w[r < 0.3] = float("nan")
+        w[(r >= 0.3) & (r < 0.9)] = -1.0
+    _check_evict(gpu, w, bt, lens, k, None, 8000, 4, 1000)
+    _check_evict(gpu, w, bt, lens, k, None, 20000, 0, 0, in_place=True)
+    _check_evict(gpu, w, bt, lens, k, None, 30001, 30001, 0, in_place=True)
+    _check_evict(gpu, w, bt, lens, k, None, 39999, 3, 39990)
+    _check_evict(gpu, w, bt, lens, k, None, 313 * 128 + 5, 3, 4)
+
+
+def test_evict_many_long_sequences(gpu):
+    """So many heads that one workgroup each selects, in several chunks."""
+    import jittorinfer_amd as J
+    width, heads, n = 264, 1700, 33700
+    gen = torch.Generator().manual_seed(47)
+    w = torch.rand((1, heads, width * 128), generator=gen)
+    k = torch.arange(width * 128, dtype=torch.int32).view(width, 128, 1, 1).expand(width, 128, heads, 2).contiguous()
+    bt, lens = torch.arange(width, dtype=torch.int32)[None], torch.tensor([n], dtype=torch.int32)
+    d = k.to(gpu)
+    kept, new, out = J.gqa_evict(w.to(gpu), bt.to(gpu), lens.to(gpu), d, n_keep=20000, n_sink=2, n_recent=100)
+    key = w[0, :, :n].clone()
+    key[:, :2], key[:, n - 100:] = 2.0, 2.0
+    want = torch.sort(torch.sort(key.to(gpu), dim=1, descending=True, stable=True).indices[:, :20000], dim=1).values
+    assert torch.equal(kept[0].long(), want) and new.tolist() == [20000]
+    assert torch.equal(out[0, :, :20000], torch.gather(w[0].to(gpu), 1, want)) and (out[0, :, 20000:] == 0).all()
+    flat = d.view(width * 128, heads, 2)
+    assert torch.equal(flat[:20000, :, 0].T.long(), want) and torch.equal(flat[:20000, :, 1].T.long(), want)
+    assert torch.equal(flat[20000:].cpu(), k.view(width * 128, heads, 2)[20000:])
+
+
 def test_evict_long_sequences(gpu):
-    """Several chunks of the selection and of the move."""
+    """Several segments of the move, over all the rows one workgroup's selection holds in registers."""
     w, bt, lens, k, _ = _evict_case(42, [20000, 17001], 157, 1, 64, 0, BF16)
     _check_evict(gpu, w, bt, lens, k, None, 9001, 4, 1000)
     w[:, :, ::2] = 1.0
