@@ -25,6 +25,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "mla_common.hpp"
 #include "../../include/gqa_attn.h"
 
@@ -34,12 +36,12 @@ namespace {
 
 struct AttnP {
     const char * q; int64_t q_nb1, q_nb2; int q_f32;
-    const char * k; int64_t k_page, k_head; int k_row;
-    const char * v; int64_t v_page, v_head; int v_row;
+    const char * k; unsigned k_page; int64_t k_head; int k_row;
+    const char * v; unsigned v_page; int64_t v_head; int v_row;
     int64_t n_pages;
     const int32_t * block_table; int64_t bt_stride;
     const int32_t * seq_lens;
-    const char * mask; int64_t mask_nb1, mask_ne0;
+    const char * mask; int64_t mask_nb1; int mask_len;             // mask_len: rows past it are out
     float * weights; int64_t w_nb1, w_nb2;
     char * dst; int64_t d_nb1, d_nb2; int dst_f32;
     float scale_log2;             // scale * log2(e)
@@ -56,7 +58,7 @@ struct AttnP {
 
 constexpr int PAGE = MLA_PAGE_TOKENS;
 
-// Workgroups a CU holds: a wave's tile of K and V, its Q fragments and its accumulators take up to 256 registers for heads up to 128 wide
+// Workgroups a CU holds: a wave's tile of K and V, its Q fragments and its accumulators take up to 256 registers for heads up to 192 wide
 // and one block of 16 query heads, more (two waves a SIMD would spill) beyond.
 constexpr int wg_per_cu(int dk, int nb) { return dk <= 64 || (dk <= 192 && nb == 1) ? 2 : 1; }
 
@@ -68,19 +70,29 @@ template <bool F16> __device__ __forceinline__ unsigned short to16(float f) {
     if constexpr (F16) return bitcast<unsigned short>((_Float16) f);
     else               return bitcast<unsigned short>((__bf16) f);
 }
+template <bool F16> __device__ __forceinline__ unsigned pair16(float a, float b) { return to16<F16>(a) | ((unsigned) to16<F16>(b) << 16); }
 template <bool F16> __device__ __forceinline__ float from16(unsigned short h) {
     if constexpr (F16) return (float) bitcast<_Float16>(h);
     else               return __uint_as_float((unsigned) h << 16);
 }
 
+// Values that are the same in every lane, told to the compiler; and lengths and page ids read through the scalar cache (nothing writes them while the
+// kernel runs): a vector load among those of K and V would have the wave wait for all that were issued before it.
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int scalar_at(const int32_t * p, int64_t i) { return *(const int32_t __attribute__((address_space(4))) *) (uintptr_t) (p + i); }
+
 // The rows a sequence attends to, [first, last).
 struct Span { int first, last; };
-__device__ __forceinline__ Span span_of(const AttnP & p, int b) {
-    int64_t n = p.seq_lens[b];
-    n = n < 0 ? 0 : n > p.cap ? p.cap : n;
-    const int64_t first = p.window > 0 && n > p.window ? n - p.window : 0;
-    if (p.mask && n > p.mask_ne0) n = p.mask_ne0;
-    return n > first ? Span{ (int) first, (int) n } : Span{ 0, 0 };
+__device__ __forceinline__ Span span_from(const AttnP & p, int n) {
+    n = min(max(n, 0), (int) p.cap);                              // (the host has checked that the room is below 2^31)
+    const int first = p.window > 0 ? max(n - p.window, 0) : 0;
+    n = min(n, p.mask_len);
+    return n > first ? Span{ first, n } : Span{ 0, 0 };
+}
+__device__ __forceinline__ Span span_of(const AttnP & p, int b) { return span_from(p, p.seq_lens[b]); }
+__device__ __forceinline__ Span span_uni(const AttnP & p, int b) {        // b the same in every lane
+    const Span s = span_from(p, scalar_at(p.seq_lens, b));
+    return Span{ uni(s.first), uni(s.last) };
 }
 __device__ __forceinline__ int pages_of(Span s) { return s.last > s.first ? (s.last + PAGE - 1) / PAGE - s.first / PAGE : 0; }
 
@@ -104,279 +116,294 @@ template <int DV> struct VGeom {
     static constexpr int COLS   = W * GROUPS;           // MFMAs (columns of a lane)
 };
 
-// threads 256 = 4 waves; wave w takes quarter w of every page of the run.
+// The deal, computed by every wave for itself (no barrier, and for up to 256 sequences one load of the lengths): the units there are and the
+// sequence of unit u.  A lane takes 4 consecutive sequences of 256.
+struct Place { int total, seq, before; };    // units in all; the sequence unit `find` lies in, and the units before that sequence
+template <typename Find> __device__ __forceinline__ Place locate(const AttnP & p, int lane, Find find) {
+    int own[4], mine = 0, total = 0;
+    auto fetch = [&](int b0) {
+        mine = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int b = b0 + lane * 4 + e;
+            own[e] = b < p.n_seq ? pages_of(span_of(p, b)) * p.head_blocks : 0;
+            mine += own[e];
+        }
+    };
+    for (int b0 = 0; b0 < p.n_seq; b0 += 256) { fetch(b0); total += wave_sum(mine); }
+    total = uni(total);
+    const int u = find(total);
+    Place r{ total, 0, 0 };
+    if (u < 0) return r;
+    for (int b0 = 0, before = 0; b0 < p.n_seq; b0 += 256) {
+        if (p.n_seq > 256) fetch(b0);
+        int incl = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(incl, d, 64); if (lane >= d) incl += o; }
+        const int all = __shfl(incl, 63, 64);
+        if (u < before + all) {
+            const int at = __ffsll(__ballot(u < before + incl)) - 1;      // the first lane whose sequences reach past u
+            int ahead = before + __shfl(incl - mine, at, 64), e = 0;
+            for (; e < 3; e++) {
+                const int n = __shfl(e == 0 ? own[0] : e == 1 ? own[1] : own[2], at, 64);
+                if (u < ahead + n) break;
+                ahead += n;
+            }
+            r.seq = b0 + at * 4 + e; r.before = ahead;
+            return r;
+        }
+        before += all;
+    }
+    return r;
+}
+
+// The mask's four numbers of rows t .. t + 3, in one load where their place allows it; rows outside the span: -inf.
+__device__ __forceinline__ u32x2 mask4(const AttnP & p, int b, int t, Span s) {
+    const char * src = p.mask + (int64_t) b * p.mask_nb1 + (int64_t) t * 2;
+    if (t >= s.first && t + 4 <= s.last && ((uintptr_t) src & 7) == 0) return *(const u32x2 *) src;
+    unsigned short h[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) h[j] = t + j >= s.first && t + j < s.last ? *(const unsigned short *) (src + 2 * j) : (unsigned short) 0xfc00;
+    return u32x2{ h[0] | ((unsigned) h[1] << 16), h[2] | ((unsigned) h[3] << 16) };
+}
+// A score in log2 units from the product q . k, before the mask.
+template <bool BIAS> __device__ __forceinline__ float scaled(const AttnP & p, float a) {
+    if (BIAS && p.cap_out != 0.f) return p.cap_out - 2.f * p.cap_out * __builtin_amdgcn_rcpf(fast_exp2(p.cap_in * a) + 1.f);
+    return p.scale_log2 * a;
+}
+// Page `page` of a pool, at a head's offset (products of 32 bits are the scalar unit's; one of 64 would put the address into vector registers).
+__device__ __forceinline__ const char * page_base(const char * data, int page, unsigned nb_page, int64_t head) {
+    return data + head + (int64_t) ((uint64_t) __umulhi((unsigned) page, nb_page) << 32 | (unsigned) page * nb_page);
+}
+
+// Wave w takes quarter w of every page of the run.
 template <bool F16, int DK, int DV, int NB, bool BIAS>
 __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const AttnP p) {
     constexpr int  KC    = DK / 32;
-    constexpr bool Q_LDS = DK > 256;                    // 18 operand fragments a head block: shared by the waves out of LDS
-    constexpr int  QP    = DK * 2 + 16;                 // its row pitch
-    constexpr int  ROWS  = NB * 16;
-    using VG = VGeom<DV ? DV : 64>;
+    constexpr int  ROWS  = NB * 16, NW = 4;
+    using VG = VGeom<DV>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    __shared__ int    sh_total, sh_seq, sh_before, sh_part[4];
-    __shared__ float2 sh_ml[4][ROWS];
+    __shared__ float2 sh_ml[NW][ROWS];
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, lg = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), l15 = lane & 15, lg = lane >> 4;
     const int wg = blockIdx.x;
 
     // ---- which units are this workgroup's
-    if (threadIdx.x == 0) sh_total = 0;
-    __syncthreads();
-    {
-        int mine = 0;
-        for (int b = threadIdx.x; b < p.n_seq; b += 256) mine += pages_of(span_of(p, b));
-        mine = wave_sum(mine);
-        if (lane == 0 && mine) atomicAdd(&sh_total, mine);   // (integers: any order)
-    }
-    __syncthreads();
-    const int  total = sh_total * p.head_blocks;
-    const Deal deal{ total / p.n_wg, total % p.n_wg };
-    int        u = run_start(deal, wg);
-    const int  u_end = run_start(deal, wg + 1);
+    int   u = 0, u_end = 0;
+    Deal  deal{ 0, 0 };
+    const Place at = locate(p, lane, [&](int total) {
+        deal = Deal{ total / p.n_wg, total % p.n_wg };
+        u = run_start(deal, wg); u_end = run_start(deal, wg + 1);
+        return u < u_end ? u : -1;
+    });
+    u = uni(u); u_end = uni(u_end);
     if (u >= u_end) return;
-    {
-        int before = 0;
-        for (int b0 = 0; b0 < p.n_seq; b0 += 256) {
-            const int b = b0 + (int) threadIdx.x;
-            const int n = b < p.n_seq ? pages_of(span_of(p, b)) * p.head_blocks : 0;
-            int incl = n;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(incl, d, 64); if (lane >= d) incl += o; }
-            if (lane == 63) sh_part[wave] = incl;
-            __syncthreads();
-            int ahead = before;
-            for (int w = 0; w < wave; w++) ahead += sh_part[w];
-            if (n > 0 && u >= ahead + incl - n && u < ahead + incl) { sh_seq = b; sh_before = ahead + incl - n; }
-            before += sh_part[0] + sh_part[1] + sh_part[2] + sh_part[3];
-            __syncthreads();
-            if (u < before) break;
-        }
-    }
-    int  b = sh_seq;
-    Span s = span_of(p, b);
-    int  np = pages_of(s);
-    int  hb = (u - sh_before) / np, pg = (u - sh_before) % np;
+    deal = Deal{ uni(deal.base), uni(deal.more) };
+    int  b = uni(at.seq);
+    Span s = span_uni(p, b);
+    int  np = uni(pages_of(s));
+    int  hb = uni((u - uni(at.before)) / np), pg = u - uni(at.before) - hb * np;
 
     for (bool fresh = true; u < u_end; fresh = false) {
-        const int  n = min(np - pg, u_end - u);              // pages of this piece
+        b = uni(b); hb = uni(hb); pg = uni(pg); np = uni(np); s = Span{ uni(s.first), uni(s.last) };
+        const int  n = uni(min(np - pg, u_end - u));         // pages of this piece
         const bool begins = pg == 0, whole = begins && n == np;
-        const int  kvh = hb / p.row_blocks, row0 = (hb - kvh * p.row_blocks) * ROWS;   // first head of the group taken here
+        const int  kvh = uni(hb / p.row_blocks), row0 = (hb - kvh * p.row_blocks) * ROWS;   // first head of the group taken here
         const int  heads = min(ROWS, p.group - row0);
         const int  head0 = kvh * p.group + row0;
         if (begins && threadIdx.x == 0) p.items[(int64_t) b * p.head_blocks + hb] = make_int2(2 * wg + (fresh ? 0 : 1), owner_of(deal, u + np - 1));
 
-        // ---- Q: operand fragments, lane (h, g) k = 32 c + 8 g .. + 7; heads past the group: zeros
-        u32x4 qf[Q_LDS ? 1 : NB * KC];
-        auto q_frag = [&](int row, int off) -> u32x4 {       // 8 values from value `off` on
-            if (row >= heads) return u32x4{ 0u, 0u, 0u, 0u };
-            const char * src = p.q + (int64_t) b * p.q_nb2 + (int64_t) (head0 + row) * p.q_nb1;
-            if (!p.q_f32) return *(const u32x4 *) (src + off * 2);
-            const f32x4 x = *(const f32x4 *) (src + off * 4), y = *(const f32x4 *) (src + off * 4 + 16);
-            return u32x4{ pack2<F16>(x.x, x.y), pack2<F16>(x.z, x.w), pack2<F16>(y.x, y.y), pack2<F16>(y.z, y.w) };
-        };
-        if constexpr (Q_LDS) {
-            for (int i = threadIdx.x; i < ROWS * (DK / 8); i += 256) {
-                const int row = i / (DK / 8), c = i - row * (DK / 8);
-                *(u32x4 *) (lds + row * QP + c * 16) = q_frag(row, c * 8);
+        const int       bt0 = b * (int) p.bt_stride + s.first / PAGE + pg;       // (the host has checked that it fits)
+        const int       t_page0 = (s.first / PAGE + pg) * PAGE;
+        u32x4 kf[2][KC];
+        u32x2 vf[8][VG::COLS / 4];
+        // the slots in the page whose rows a lane loads: rows outside the span are replaced by the nearest one inside
+        auto slot = [&](int i, int r) { return min(max(wave * 32 + r, s.first - (t_page0 + i * PAGE)), s.last - 1 - (t_page0 + i * PAGE)); };
+        const int64_t k_off = (int64_t) kvh * p.k_head, v_off = (int64_t) kvh * p.v_head;
+        auto load_k = [&](int i, int page) {
+            const char * base = page_base(p.k, page, p.k_page, k_off);
+#pragma unroll
+            for (int blk = 0; blk < 2; blk++) {
+                const unsigned row = slot(i, blk * 16 + l15) * p.k_row + lg * 16;
+#pragma unroll
+                for (int c = 0; c < KC; c++) kf[blk][c] = *(const u32x4 *) (base + row + c * 64);
             }
-            __syncthreads();
+        };
+        auto load_v = [&](int i, int page) {
+            const char * base = page_base(p.v, page, p.v_page, v_off);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const unsigned row = slot(i, (e >> 2) * 16 + lg * 4 + (e & 3)) * p.v_row + l15 * (VG::W * 2);
+#pragma unroll
+                for (int gr = 0; gr < VG::GROUPS; gr++) {
+                    if constexpr (VG::W == 8) {
+                        const u32x4 x = *(const u32x4 *) (base + row + gr * 256);
+                        vf[e][2 * gr] = u32x2{ x[0], x[1] }; vf[e][2 * gr + 1] = u32x2{ x[2], x[3] };
+                    } else vf[e][gr] = *(const u32x2 *) (base + row);
+                }
+            }
+        };
+        auto id_at = [&](int i) { return scalar_at(p.block_table, bt0 + min(i, n - 1)); };        // page of the piece's page i
+        auto good = [&](int id) { return id >= 0 && id < p.n_pages; };          // (a bad id: page 0 is read, not used)
+
+        u32x2 mk[2];                                            // the mask of a tile's rows
+        auto load_mask = [&](int i) {
+            if constexpr (BIAS)
+                if (p.mask)
+#pragma unroll
+                    for (int blk = 0; blk < 2; blk++) mk[blk] = mask4(p, b, t_page0 + i * PAGE + wave * 32 + blk * 16 + lg * 4, s);
+        };
+
+        int id = id_at(0), id_next = id_at(1);                  // (ids are fetched a tile ahead of their rows)
+        load_k(0, good(id) ? id : 0);
+        load_v(0, good(id) ? id : 0);
+        load_mask(0);
+        // ---- Q: operand fragments, lane (h, g) k = 32 c + 8 g .. + 7; heads past the group: zeros
+        u32x4 qf[NB * KC];
+        auto q_at = [&](int row, int off) { return p.q + (int64_t) b * p.q_nb2 + (int64_t) (head0 + min(row, heads - 1)) * p.q_nb1 + off * (p.q_f32 ? 4 : 2); };   // 8 values from `off` on
+        auto q_half = [&](int row, int off) {
+            const u32x4 x = *(const u32x4 *) q_at(row, off);
+            return row < heads ? x : u32x4{ 0u, 0u, 0u, 0u };
+        };
+        auto q_full = [&](int row, int off) {
+            const f32x4 x = *(const f32x4 *) q_at(row, off), y = *(const f32x4 *) (q_at(row, off) + 16);
+            return row < heads ? u32x4{ pair16<F16>(x.x, x.y), pair16<F16>(x.z, x.w), pair16<F16>(y.x, y.y), pair16<F16>(y.z, y.w) } : u32x4{ 0u, 0u, 0u, 0u };
+        };
+        if (p.q_f32) {
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int c = 0; c < KC; c++) qf[nb * KC + c] = q_full(nb * 16 + l15, c * 32 + lg * 8);
         } else {
 #pragma unroll
             for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-                for (int c = 0; c < KC; c++) qf[nb * KC + c] = q_frag(nb * 16 + l15, c * 32 + lg * 8);
+                for (int c = 0; c < KC; c++) qf[nb * KC + c] = q_half(nb * 16 + l15, c * 32 + lg * 8);
         }
 
         float m[NB], l[NB];
-        f32x4 acc[NB][DV ? VG::COLS : 1];
+        f32x4 acc[NB][VG::COLS];
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
             m[nb] = -INFINITY; l[nb] = 0.f;
 #pragma unroll
-            for (int c = 0; c < (DV ? VG::COLS : 1); c++) acc[nb][c] = f32x4{ 0.f, 0.f, 0.f, 0.f };
+            for (int c = 0; c < VG::COLS; c++) acc[nb][c] = f32x4{ 0.f, 0.f, 0.f, 0.f };
         }
 
-        const int32_t * bt = p.block_table + (int64_t) b * p.bt_stride + s.first / PAGE + pg;
-        const int       t_page0 = (s.first / PAGE + pg) * PAGE;
-        u32x4 kf[2][KC];
-        u32x2 vf[8][DV ? VG::COLS / 4 : 1];
-        // the slots in the page whose rows a lane loads: rows outside the span are replaced by the nearest one inside
-        auto slot = [&](int i, int r) { return min(max(wave * 32 + r, s.first - (t_page0 + i * PAGE)), s.last - 1 - (t_page0 + i * PAGE)); };
-        auto load_k = [&](int i, int64_t page) {
-            const char * base = p.k + page * p.k_page + (int64_t) kvh * p.k_head;
-#pragma unroll
-            for (int blk = 0; blk < 2; blk++) {
-                const char * row = base + slot(i, blk * 16 + l15) * p.k_row + lg * 16;
-#pragma unroll
-                for (int c = 0; c < KC; c++) kf[blk][c] = *(const u32x4 *) (row + c * 64);
-            }
-        };
-        auto load_v = [&](int i, int64_t page) {
-            if constexpr (DV > 0) {
-                const char * base = p.v + page * p.v_page + (int64_t) kvh * p.v_head;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const char * row = base + slot(i, (e >> 2) * 16 + lg * 4 + (e & 3)) * p.v_row + l15 * (VG::W * 2);
-#pragma unroll
-                    for (int gr = 0; gr < VG::GROUPS; gr++) {
-                        if constexpr (VG::W == 8) {
-                            const u32x4 x = *(const u32x4 *) (row + gr * 256);
-                            vf[e][2 * gr] = u32x2{ x[0], x[1] }; vf[e][2 * gr + 1] = u32x2{ x[2], x[3] };
-                        } else vf[e][gr] = *(const u32x2 *) row;
-                    }
-                }
-            }
-        };
-        auto page_at = [&](int i, bool & ok) -> int64_t {      // page of the piece's page i; a bad id: page 0 is read, not used
-            const int id = bt[i];
-            ok = id >= 0 && id < p.n_pages;
-            return ok ? id : 0;
-        };
-
-        bool    ok;
-        int64_t page = page_at(0, ok);
-        load_k(0, page);
-        load_v(0, page);
-        for (int i = 0; i < n; i++) {
-            const int  t0 = t_page0 + i * PAGE + wave * 32;     // first row of the tile
+        // One tile; MORE: another one follows (known to the compiler, so that the loads under way are counted: a branch around them would have every
+        // wait be for all of them)
+        auto tile = [&](auto more_tag, int i) __attribute__((always_inline)) {
+            constexpr bool MORE = decltype(more_tag)::value;
+            const int  t0 = t_page0 + i * PAGE + wave * 32;  // first row of the tile
             const int  lo = max(s.first - t0, 0), hi = min(s.last - t0, 32);
-            const bool use = ok && hi > lo, all = lo == 0 && hi == 32;
-            bool       ok_next = false;
-            const int64_t next = i + 1 < n ? page_at(i + 1, ok_next) : 0;
+            const bool use = good(id) && hi > lo, all = lo == 0 && hi == 32;
+            const int  next = good(id_next) ? id_next : 0;
+            id = id_next;
+            id_next = id_at(i + 2);
 
-            f32x4 sc[NB][2];
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++) {
-                sc[nb][0] = f32x4{ 0.f, 0.f, 0.f, 0.f }; sc[nb][1] = sc[nb][0];
-#pragma unroll
-                for (int c = 0; c < KC; c++) {
-                    u32x4 qq;
-                    if constexpr (Q_LDS) qq = *(const u32x4 *) (lds + (nb * 16 + l15) * QP + c * 64 + lg * 16);
-                    else                 qq = qf[nb * KC + c];
-                    sc[nb][0] = mfma16<F16>(kf[0][c], qq, sc[nb][0]);
-                    sc[nb][1] = mfma16<F16>(kf[1][c], qq, sc[nb][1]);
-                }
-            }
-            if (i + 1 < n) load_k(i + 1, next);
-
-            // scores in log2 units
-            float mk[2][4];
+            // the mask's numbers, and the rows it takes out (rows outside the span among them: they repeat one inside, which may be masked)
+            float mf[2][4];
             bool  out[2][4];
             if constexpr (BIAS) {
-#pragma unroll
-                for (int blk = 0; blk < 2; blk++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int r = blk * 16 + lg * 4 + j;
-                        mk[blk][j] = 0.f; out[blk][j] = true;          // (rows outside the span repeat one inside, which may be masked)
-                        if (p.mask && r >= lo && r < hi) {
-                            const float x = f16_bits_to_f32(*(const unsigned short *) (p.mask + (int64_t) b * p.mask_nb1 + (int64_t) (t0 + r) * 2));
-                            out[blk][j] = x == -INFINITY;
-                            mk[blk][j]  = x * LOG2E;
-                        }
-                    }
-            }
-            float x[NB][2][4];
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-                for (int blk = 0; blk < 2; blk++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        float y;
-                        if constexpr (BIAS) {
-                            if (p.cap_out != 0.f) y = p.cap_out - 2.f * p.cap_out * __builtin_amdgcn_rcpf(fast_exp2(p.cap_in * sc[nb][blk][j]) + 1.f);
-                            else                  y = p.scale_log2 * sc[nb][blk][j];
-                            if (p.mask) y = out[blk][j] ? -INFINITY : y + mk[blk][j];
-                        } else y = p.scale_log2 * sc[nb][blk][j];
-                        x[nb][blk][j] = y;
-                    }
-            if (!use || !all) {
-#pragma unroll
-                for (int nb = 0; nb < NB; nb++)
+                if (p.mask) {
 #pragma unroll
                     for (int blk = 0; blk < 2; blk++)
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
-                            const int r = blk * 16 + lg * 4 + j;
-                            if (!use || r < lo || r >= hi) x[nb][blk][j] = -INFINITY;
+                            const float f = f16_bits_to_f32((mk[blk][j >> 1] >> (16 * (j & 1))) & 0xffffu);
+                            out[blk][j] = f == -INFINITY;
+                            mf[blk][j]  = f * LOG2E;
                         }
+                    if constexpr (MORE) load_mask(i + 1);
+                }
             }
-            if (p.scores) {
+
+            u32x4 ph[NB], pl[NB];
 #pragma unroll
-                for (int nb = 0; nb < NB; nb++)
-                    if (nb * 16 + l15 < heads) {
-                        float * to = p.scores + ((int64_t) b * p.n_head + head0 + nb * 16 + l15) * p.cap + t0 + lg * 4;
-                        *(f32x4 *) to        = f32x4{ x[nb][0][0], x[nb][0][1], x[nb][0][2], x[nb][0][3] };
-                        *(f32x4 *) (to + 16) = f32x4{ x[nb][1][0], x[nb][1][1], x[nb][1][2], x[nb][1][3] };
+            for (int nb = 0; nb < NB; nb++) {
+                f32x4 sc[2] = { { 0.f, 0.f, 0.f, 0.f }, { 0.f, 0.f, 0.f, 0.f } };
+#pragma unroll
+                for (int c = 0; c < KC; c++) {
+                    sc[0] = mfma16<F16>(kf[0][c], qf[nb * KC + c], sc[0]);
+                    sc[1] = mfma16<F16>(kf[1][c], qf[nb * KC + c], sc[1]);
+                }
+                if (MORE && nb == NB - 1) load_k(i + 1, next);
+
+                float x[8];                                     // scores in log2 units
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    x[e] = scaled<BIAS>(p, sc[e >> 2][e & 3]);
+                    if constexpr (BIAS) if (p.mask) x[e] = out[e >> 2][e & 3] ? -INFINITY : x[e] + mf[e >> 2][e & 3];
+                }
+                if (!use || !all) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const int r = (e >> 2) * 16 + lg * 4 + (e & 3);
+                        if (!use || r < lo || r >= hi) x[e] = -INFINITY;
                     }
+                }
+                if (p.scores && nb * 16 + l15 < heads) {
+                    float * to = p.scores + ((int64_t) b * p.n_head + head0 + nb * 16 + l15) * p.cap + t0 + lg * 4;
+                    *(f32x4 *) to        = f32x4{ x[0], x[1], x[2], x[3] };
+                    *(f32x4 *) (to + 16) = f32x4{ x[4], x[5], x[6], x[7] };
+                }
+                float top = x[0];
+#pragma unroll
+                for (int e = 1; e < 8; e++) top = fmaxf(top, x[e]);
+                if (__any(top > m[nb] + 8.f)) {
+                    top = fmaxf(top, __shfl_xor(top, 16, 64));
+                    top = fmaxf(top, __shfl_xor(top, 32, 64));
+                    const float nm = fmaxf(top, m[nb]);
+                    const float a  = m[nb] == nm ? 1.f : fast_exp2(m[nb] - nm);
+                    m[nb] = nm;
+                    l[nb] *= a;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const float aj = __shfl(a, lg * 4 + j, 64);
+#pragma unroll
+                        for (int c = 0; c < VG::COLS; c++) acc[nb][c][j] *= aj;
+                    }
+                }
+                const float mm = m[nb] == -INFINITY ? 0.f : m[nb];
+#pragma unroll
+                for (int e = 0; e < 8; e++) { x[e] = fast_exp2(x[e] - mm); l[nb] += x[e]; }
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    ph[nb][e] = pair16<F16>(x[2 * e], x[2 * e + 1]);
+                    pl[nb][e] = pair16<F16>(x[2 * e] - from16<F16>((unsigned short) ph[nb][e]), x[2 * e + 1] - from16<F16>((unsigned short) (ph[nb][e] >> 16)));
+                }
             }
             if (use) {
-                u32x4 ph[NB], pl[NB];
+                if constexpr (BIAS) {
+                    // a row the mask takes out has p = 0, and 0 * NaN must not count
+                    if (p.mask) {
 #pragma unroll
-                for (int nb = 0; nb < NB; nb++) {
-                    float top = x[nb][0][0];
+                        for (int e = 0; e < 8; e++)
 #pragma unroll
-                    for (int e = 1; e < 8; e++) top = fmaxf(top, x[nb][e >> 2][e & 3]);
-                    if (__any(top > m[nb] + 8.f)) {
-                        top = fmaxf(top, __shfl_xor(top, 16, 64));
-                        top = fmaxf(top, __shfl_xor(top, 32, 64));
-                        const float nm = fmaxf(top, m[nb]);
-                        const float a  = m[nb] == nm ? 1.f : fast_exp2(m[nb] - nm);
-                        m[nb] = nm;
-                        l[nb] *= a;
-                        if constexpr (DV > 0) {
-#pragma unroll
-                            for (int j = 0; j < 4; j++) {
-                                const float aj = __shfl(a, lg * 4 + j, 64);
-#pragma unroll
-                                for (int c = 0; c < VG::COLS; c++) acc[nb][c][j] *= aj;
-                            }
-                        }
-                    }
-                    const float mm = m[nb] == -INFINITY ? 0.f : m[nb];
-                    float e8[8];
-#pragma unroll
-                    for (int e = 0; e < 8; e++) { e8[e] = fast_exp2(x[nb][e >> 2][e & 3] - mm); l[nb] += e8[e]; }
-                    if constexpr (DV > 0) {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const unsigned short h0 = to16<F16>(e8[2 * e]), h1 = to16<F16>(e8[2 * e + 1]);
-                            ph[nb][e] = h0 | ((unsigned) h1 << 16);
-                            pl[nb][e] = to16<F16>(e8[2 * e] - from16<F16>(h0)) | ((unsigned) to16<F16>(e8[2 * e + 1] - from16<F16>(h1)) << 16);
-                        }
+                            for (int c = 0; c < VG::COLS / 4; c++)
+                                if (out[e >> 2][e & 3]) vf[e][c] = u32x2{ 0u, 0u };
                     }
                 }
-                if constexpr (DV > 0) {
-                    if constexpr (BIAS) {
-                        // a row the mask takes out has p = 0, and 0 * NaN must not count
-                        if (p.mask) {
 #pragma unroll
-                            for (int e = 0; e < 8; e++)
+                for (int c = 0; c < VG::COLS; c++) {
+                    u32x4 bf;
 #pragma unroll
-                                for (int c = 0; c < VG::COLS / 4; c++)
-                                    if (out[e >> 2][e & 3]) vf[e][c] = u32x2{ 0u, 0u };
-                        }
-                    }
+                    for (int e = 0; e < 4; e++)
+                        bf[e] = __builtin_amdgcn_perm(vf[2 * e + 1][c >> 2][(c >> 1) & 1], vf[2 * e][c >> 2][(c >> 1) & 1], c & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-                    for (int c = 0; c < VG::COLS; c++) {
-                        u32x4 bf;
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            bf[e] = __builtin_amdgcn_perm(vf[2 * e + 1][c >> 2][(c >> 1) & 1], vf[2 * e][c >> 2][(c >> 1) & 1], c & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-                        for (int nb = 0; nb < NB; nb++) {
-                            acc[nb][c] = mfma16<F16>(ph[nb], bf, acc[nb][c]);
-                            acc[nb][c] = mfma16<F16>(pl[nb], bf, acc[nb][c]);
-                        }
+                    for (int nb = 0; nb < NB; nb++) {
+                        acc[nb][c] = mfma16<F16>(ph[nb], bf, acc[nb][c]);
+                        acc[nb][c] = mfma16<F16>(pl[nb], bf, acc[nb][c]);
                     }
                 }
             }
-            if (i + 1 < n) load_v(i + 1, next);
-            page = next; ok = ok_next;
-        }
+            if constexpr (MORE) load_v(i + 1, next);
+        };
+        int i = 0;
+        for (; i + 1 < n; i++) tile(std::true_type{}, i);
+        tile(std::false_type{}, i);
 
-        // ---- the four waves' results meet in LDS
+        // ---- the waves' results meet in LDS
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
             float t = l[nb];
@@ -388,9 +415,9 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
         auto joined = [&](int row) -> float2 {               // maximum and sum over the waves
             float M = -INFINITY, L = 0.f;
 #pragma unroll
-            for (int w = 0; w < 4; w++) M = fmaxf(M, sh_ml[w][row].x);
+            for (int w = 0; w < NW; w++) M = fmaxf(M, sh_ml[w][row].x);
 #pragma unroll
-            for (int w = 0; w < 4; w++) L += sh_ml[w][row].y == 0.f ? 0.f : sh_ml[w][row].y * fast_exp2(sh_ml[w][row].x - M);
+            for (int w = 0; w < NW; w++) L += sh_ml[w][row].y == 0.f ? 0.f : sh_ml[w][row].y * fast_exp2(sh_ml[w][row].x - M);
             return make_float2(M, L);
         };
         const int64_t piece = 2 * (int64_t) wg + (fresh ? 0 : 1);
@@ -399,41 +426,39 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
             if (!whole) p.part_ml[piece * ROWS + r] = ml;
             else if (p.scores) p.lse[(int64_t) b * p.n_head + head0 + r] = make_float2(ml.x == -INFINITY ? 0.f : ml.x, ml.y == 0.f ? 0.f : 1.f / ml.y);
         }
-        if constexpr (DV > 0) {
-            float * tile = (float *) lds;                     // [4][16][DV]
+        float * part = (float *) lds;                         // [4][16][DV]
 #pragma unroll
-            for (int nb = 0; nb < NB; nb++) {
-                if (nb) __syncthreads();
+        for (int nb = 0; nb < NB; nb++) {
+            if (nb) __syncthreads();
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int    row = nb * 16 + lg * 4 + j;
-                    const float  mw  = sh_ml[wave][row].x;
-                    const float2 ml  = joined(row);
-                    const float  f   = mw == -INFINITY ? 0.f : fast_exp2(mw - ml.x);
-                    float * to = tile + (wave * 16 + lg * 4 + j) * DV + l15 * VG::W;
+            for (int j = 0; j < 4; j++) {
+                const int    row = nb * 16 + lg * 4 + j;
+                const float  mw  = sh_ml[wave][row].x;
+                const float2 ml  = joined(row);
+                const float  f   = mw == -INFINITY ? 0.f : fast_exp2(mw - ml.x);
+                float * to = part + (wave * 16 + lg * 4 + j) * DV + l15 * VG::W;
 #pragma unroll
-                    for (int gr = 0; gr < VG::GROUPS; gr++)
+                for (int gr = 0; gr < VG::GROUPS; gr++)
 #pragma unroll
-                        for (int c = 0; c < VG::W; c += 4) {
-                            const int a = gr * VG::W + c;
-                            *(f32x4 *) (to + gr * 128 + c) = f32x4{ acc[nb][a][j] * f, acc[nb][a + 1][j] * f, acc[nb][a + 2][j] * f, acc[nb][a + 3][j] * f };
-                        }
-                }
-                __syncthreads();
-                for (int i = threadIdx.x; i < 4 * DV; i += 256) {     // 16 rows of DV / 4 runs of 4
-                    const int r = i / (DV / 4), c = (i - r * (DV / 4)) * 4, row = nb * 16 + r;
-                    if (row >= heads) continue;
-                    f32x4 o = *(const f32x4 *) (tile + r * DV + c);
-#pragma unroll
-                    for (int w = 1; w < 4; w++) o += *(const f32x4 *) (tile + (w * 16 + r) * DV + c);
-                    if (!whole) *(f32x4 *) (p.part_o + (piece * ROWS + row) * DV + c) = o;
-                    else {
-                        const float L = joined(row).y, inv = L == 0.f ? 0.f : 1.f / L;   // (a NaN stays one)
-                        char * to = p.dst + (int64_t) b * p.d_nb2 + (int64_t) (head0 + row) * p.d_nb1;
-                        o *= inv;
-                        if (p.dst_f32) *(f32x4 *) (to + c * 4) = o;
-                        else *(u32x2 *) (to + c * 2) = u32x2{ to16<F16>(o.x) | ((unsigned) to16<F16>(o.y) << 16), to16<F16>(o.z) | ((unsigned) to16<F16>(o.w) << 16) };
+                    for (int c = 0; c < VG::W; c += 4) {
+                        const int a = gr * VG::W + c;
+                        *(f32x4 *) (to + gr * 128 + c) = f32x4{ acc[nb][a][j] * f, acc[nb][a + 1][j] * f, acc[nb][a + 2][j] * f, acc[nb][a + 3][j] * f };
                     }
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < 4 * DV; i += 256) {     // 16 rows of DV / 4 runs of 4
+                const int r = i / (DV / 4), c = (i - r * (DV / 4)) * 4, row = nb * 16 + r;
+                if (row >= heads) continue;
+                f32x4 o = *(const f32x4 *) (part + r * DV + c);
+#pragma unroll
+                for (int w = 1; w < 4; w++) o += *(const f32x4 *) (part + (w * 16 + r) * DV + c);
+                if (!whole) *(f32x4 *) (p.part_o + (piece * ROWS + row) * DV + c) = o;
+                else {
+                    const float L = joined(row).y, inv = L == 0.f ? 0.f : 1.f / L;   // (a NaN stays one)
+                    char * to = p.dst + (int64_t) b * p.d_nb2 + (int64_t) (head0 + row) * p.d_nb1;
+                    o *= inv;
+                    if (p.dst_f32) *(f32x4 *) (to + c * 4) = o;
+                    else *(u32x2 *) (to + c * 2) = u32x2{ pair16<F16>(o.x, o.y), pair16<F16>(o.z, o.w) };
                 }
             }
         }
@@ -442,7 +467,158 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
         u += n; pg = 0;
         if (++hb == p.head_blocks && u < u_end) {
             hb = 0;
-            do { b++; s = span_of(p, b); np = pages_of(s); } while (np == 0);   // (u < u_end <= total: there is such a sequence)
+            do { b++; s = span_uni(p, b); np = uni(pages_of(s)); } while (np == 0);   // (u < u_end <= total: there is such a sequence)
+        }
+    }
+}
+
+// Scores of a latent cache (rows of 576, one KV head) for its weights: (m, l) and every score, as gqa_attn_kernel leaves them, without V.  Up to
+// 128 heads share a row, 128 flop a byte: the rows of Q lie in LDS (147 KB) and are read, 16 heads at a time, against a tile of 32 rows of K
+// in registers, by eight waves, so that every SIMD still has two.  The loop over blocks of heads is a loop: eight copies of its body, run once or
+// twice by a workgroup, cost three times as long to fetch as to run.
+constexpr int LK = 576, LPITCH = LK * 2 + 16, LWAVES = 8, LROWS = 128;
+template <bool F16, bool BIAS>
+__global__ void __launch_bounds__(64 * LWAVES) gqa_scores_kernel(const AttnP p) {
+    constexpr int KC = LK / 32;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ float2 sh_ml[LWAVES][LROWS];
+    const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), quarter = wave & 3, l15 = lane & 15, lg = lane >> 4;
+    const int wg = blockIdx.x;
+    int   u = 0, u_end = 0;
+    Deal  deal{ 0, 0 };
+    const Place at = locate(p, lane, [&](int total) {
+        deal = Deal{ total / p.n_wg, total % p.n_wg };
+        u = run_start(deal, wg); u_end = run_start(deal, wg + 1);
+        return u < u_end ? u : -1;
+    });
+    u = uni(u); u_end = uni(u_end);
+    if (u >= u_end) return;
+    deal = Deal{ uni(deal.base), uni(deal.more) };
+    int  b = uni(at.seq);
+    Span s = span_uni(p, b);
+    int  np = uni(pages_of(s));
+    int  hb = uni((u - uni(at.before)) / np), pg = u - uni(at.before) - hb * np;
+
+    for (bool fresh = true; u < u_end; fresh = false) {
+        b = uni(b); hb = uni(hb); pg = uni(pg); np = uni(np); s = Span{ uni(s.first), uni(s.last) };
+        const int  n = uni(min(np - pg, u_end - u));
+        const bool begins = pg == 0, whole = begins && n == np;
+        const int  head0 = hb * LROWS, heads = min(LROWS, p.group - head0);
+        if (begins && threadIdx.x == 0) p.items[(int64_t) b * p.head_blocks + hb] = make_int2(2 * wg + (fresh ? 0 : 1), owner_of(deal, u + np - 1));
+        const int bt0 = b * (int) p.bt_stride + s.first / PAGE + pg, t_page0 = (s.first / PAGE + pg) * PAGE;
+        auto id_at = [&](int i) { return scalar_at(p.block_table, bt0 + min(i, n - 1)); };
+        auto good = [&](int id) { return id >= 0 && id < p.n_pages; };
+        u32x4 kf[2][KC];
+        auto load_k = [&](int i, int page) {
+            const char * base = page_base(p.k, page, p.k_page, 0);
+#pragma unroll
+            for (int blk = 0; blk < 2; blk++) {
+                const int t = t_page0 + i * PAGE;
+                const unsigned row = min(max(quarter * 32 + blk * 16 + l15, s.first - t), s.last - 1 - t) * p.k_row + lg * 16;
+#pragma unroll
+                for (int c = 0; c < KC; c++) kf[blk][c] = *(const u32x4 *) (base + row + c * 64);
+            }
+        };
+        int i = wave >> 2;                                     // waves 0 .. 3 the even pages of the run, 4 .. 7 the odd ones
+        int id = id_at(i);
+        if (i < n) load_k(i, good(id) ? id : 0);
+
+        // ---- Q to LDS: several pieces a thread under way at once (one by one, they were most of this kernel's time); rows past the group: zeros
+        constexpr int PIECES = LROWS * (LK / 8), BATCH = 6;
+        static_assert(PIECES % (64 * LWAVES * BATCH) == 0, "whole batches");
+        for (int i0 = threadIdx.x; i0 < PIECES; i0 += 64 * LWAVES * BATCH) {
+            u32x4 v[BATCH], w[BATCH];
+            auto src = [&](int k) {
+                const int f = i0 + k * 64 * LWAVES, row = f / (LK / 8);
+                return p.q + (int64_t) b * p.q_nb2 + (int64_t) (head0 + min(row, heads - 1)) * p.q_nb1 + (f - row * (LK / 8)) * (p.q_f32 ? 32 : 16);
+            };
+#pragma unroll
+            for (int k = 0; k < BATCH; k++) v[k] = *(const u32x4 *) src(k);
+            if (p.q_f32) {
+#pragma unroll
+                for (int k = 0; k < BATCH; k++) w[k] = *(const u32x4 *) (src(k) + 16);
+#pragma unroll
+                for (int k = 0; k < BATCH; k++) {
+                    const f32x4 x = bitcast<f32x4>(v[k]), y = bitcast<f32x4>(w[k]);
+                    v[k] = u32x4{ pair16<F16>(x.x, x.y), pair16<F16>(x.z, x.w), pair16<F16>(y.x, y.y), pair16<F16>(y.z, y.w) };
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < BATCH; k++) {
+                const int f = i0 + k * 64 * LWAVES, row = f / (LK / 8);
+                *(u32x4 *) (lds + row * LPITCH + (f - row * (LK / 8)) * 16) = row < heads ? v[k] : u32x4{ 0u, 0u, 0u, 0u };
+            }
+        }
+        // (a wave's own rows of sh_ml hold its running maxima and sums: LDS operations of a wave stay in order)
+        for (int r = lane; r < LROWS; r += 64) sh_ml[wave][r] = make_float2(-INFINITY, 0.f);
+        __syncthreads();
+
+        for (; i < n; i += LWAVES / 4) {
+            const int  t0 = t_page0 + i * PAGE + quarter * 32;
+            const bool use = good(id);
+            id = id_at(i + LWAVES / 4);
+            u32x2 mk[2] = { { 0u, 0u }, { 0u, 0u } };
+            if constexpr (BIAS)
+                if (p.mask)
+#pragma unroll
+                    for (int blk = 0; blk < 2; blk++) mk[blk] = mask4(p, b, t0 + blk * 16 + lg * 4, s);
+            float * to = p.scores + ((int64_t) b * p.n_head + head0 + l15) * p.cap + t0 + lg * 4;
+#pragma unroll 1
+            for (int h = l15; h - l15 < heads; h += 16, to += 16 * p.cap) {
+                f32x4 sc[2] = { { 0.f, 0.f, 0.f, 0.f }, { 0.f, 0.f, 0.f, 0.f } };
+                const char * q = lds + h * LPITCH + lg * 16;
+#pragma unroll
+                for (int c = 0; c < KC; c++) {
+                    const u32x4 qq = *(const u32x4 *) (q + c * 64);
+                    sc[0] = mfma16<F16>(kf[0][c], qq, sc[0]);
+                    sc[1] = mfma16<F16>(kf[1][c], qq, sc[1]);
+                }
+                float x[8], top = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int r = t0 + (e >> 2) * 16 + lg * 4 + (e & 3);
+                    x[e] = scaled<BIAS>(p, sc[e >> 2][e & 3]);
+                    if constexpr (BIAS)
+                        if (p.mask) {
+                            const float f = f16_bits_to_f32((mk[e >> 2][(e >> 1) & 1] >> (16 * (e & 1))) & 0xffffu);
+                            x[e] = f == -INFINITY ? -INFINITY : x[e] + f * LOG2E;
+                        }
+                    if (!use || r < s.first || r >= s.last) x[e] = -INFINITY;
+                    top = fmaxf(top, x[e]);
+                }
+                if (h < heads) {
+                    *(f32x4 *) to        = f32x4{ x[0], x[1], x[2], x[3] };
+                    *(f32x4 *) (to + 16) = f32x4{ x[4], x[5], x[6], x[7] };
+                }
+                const float2 ml = sh_ml[wave][h];
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(fmaxf(top, __shfl_xor(top, 32, 64)), ml.x);
+                const float mm = top == -INFINITY ? 0.f : top;
+                float l = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) l += fast_exp2(x[e] - mm);
+                l += __shfl_xor(l, 16, 64);
+                l += __shfl_xor(l, 32, 64);
+                if (lg == 0) sh_ml[wave][h] = make_float2(top, l + (ml.y == 0.f ? 0.f : ml.y * fast_exp2(ml.x - mm)));
+            }
+            if (i + LWAVES / 4 < n) load_k(i + LWAVES / 4, good(id) ? id : 0);
+        }
+        __syncthreads();
+        const int64_t piece = 2 * (int64_t) wg + (fresh ? 0 : 1);
+        for (int r = threadIdx.x; r < heads; r += 64 * LWAVES) {
+            float M = -INFINITY, L = 0.f;
+#pragma unroll
+            for (int w = 0; w < LWAVES; w++) M = fmaxf(M, sh_ml[w][r].x);
+#pragma unroll
+            for (int w = 0; w < LWAVES; w++) L += sh_ml[w][r].y == 0.f ? 0.f : sh_ml[w][r].y * fast_exp2(sh_ml[w][r].x - M);
+            if (!whole) p.part_ml[piece * LROWS + r] = make_float2(M, L);
+            else        p.lse[(int64_t) b * p.n_head + head0 + r] = make_float2(M == -INFINITY ? 0.f : M, L == 0.f ? 0.f : 1.f / L);
+        }
+        __syncthreads();                                       // LDS is free again for the next piece
+        u += n; pg = 0;
+        if (++hb == p.head_blocks && u < u_end) {
+            hb = 0;
+            do { b++; s = span_uni(p, b); np = uni(pages_of(s)); } while (np == 0);
         }
     }
 }
@@ -459,13 +635,13 @@ __global__ void __launch_bounds__(256) gqa_join_kernel(const AttnP p, const int 
     const int cols = p.dv / 4;                                // runs of 4 columns
     auto store = [&](int c, f32x4 o) {
         if (p.dst_f32) *(f32x4 *) (dst + c * 16) = o;
-        else *(u32x2 *) (dst + c * 8) = u32x2{ to16<F16>(o.x) | ((unsigned) to16<F16>(o.y) << 16), to16<F16>(o.z) | ((unsigned) to16<F16>(o.w) << 16) };
+        else *(u32x2 *) (dst + c * 8) = u32x2{ pair16<F16>(o.x, o.y), pair16<F16>(o.z, o.w) };
     };
+    const int2 it = p.items[(int64_t) b * p.head_blocks + kvh * p.row_blocks + rb];   // (meaningless, and not used, where there is no row)
     if (pages_of(span_of(p, b)) == 0) {
         for (int c = threadIdx.x; c < cols; c += 256) store(c, f32x4{ 0.f, 0.f, 0.f, 0.f });
         return;
     }
-    const int2 it = p.items[(int64_t) b * p.head_blocks + kvh * p.row_blocks + rb];
     const int  v0 = it.x >> 1, n = it.y - v0 + 1;
     if (n == 1) return;
     auto slot = [&](int i) -> int64_t { return ((int64_t) (i ? 2 * (v0 + i) : it.x)) * rows + row; };
@@ -503,20 +679,32 @@ __global__ void __launch_bounds__(256) gqa_join_kernel(const AttnP p, const int 
     }
 }
 
-// weights[b][g][i] += sum over the group's heads of exp2(s - m) / l, from the scores the first kernel left: 4 rows a thread.
-__global__ void __launch_bounds__(256) gqa_weights_kernel(const AttnP p) {
+// weights[b][g][i] += sum over the group's heads of exp2(s - m) / l, from the scores the first kernel left.  A thread takes 4 rows and
+// every parts-th head (parts: 16, or the power of two that holds a smaller group); the parts are added in one order.
+__global__ void __launch_bounds__(256) gqa_weights_kernel(const AttnP p, const int parts) {
+    __shared__ f32x4 sum[256];
     const int  b = blockIdx.y / p.n_head_kv, kvh = blockIdx.y - b * p.n_head_kv;
     const Span s = span_of(p, b);
-    const int  t = (int) (blockIdx.x * 1024 + threadIdx.x * 4);
-    if (t >= s.last || t + 4 <= s.first) return;
+    const int  quads = 256 / parts, part = (int) threadIdx.x / quads, quad = (int) threadIdx.x - part * quads;
+    const int  t = ((int) blockIdx.x * quads + quad) * 4;
+    if ((int) blockIdx.x * quads * 4 >= s.last || ((int) blockIdx.x + 1) * quads * 4 <= s.first) return;
     const int64_t h0 = (int64_t) b * p.n_head + (int64_t) kvh * p.group;
+    const bool    in = t < s.last && t + 4 > s.first;
     f32x4 w = { 0.f, 0.f, 0.f, 0.f };
-    for (int h = 0; h < p.group; h++) {
-        const float2 ml = p.lse[h0 + h];
-        const f32x4  x  = *(const f32x4 *) (p.scores + (h0 + h) * p.cap + t);
+    if (in)
+        for (int h = part; h < p.group; h += parts) {
+            const float2 ml = p.lse[h0 + h];
+            const f32x4  x  = *(const f32x4 *) (p.scores + (h0 + h) * p.cap + t);
 #pragma unroll
-        for (int j = 0; j < 4; j++) w[j] += fast_exp2(x[j] - ml.x) * ml.y;
+            for (int j = 0; j < 4; j++) w[j] += fast_exp2(x[j] - ml.x) * ml.y;
+        }
+    if (parts > 1) {
+        sum[threadIdx.x] = w;
+        __syncthreads();
+        if (part) return;
+        for (int q = 1; q < parts; q++) w += sum[q * quads + quad];
     }
+    if (!in) return;
     float * to = (float *) ((char *) p.weights + (int64_t) b * p.w_nb2 + (int64_t) kvh * p.w_nb1) + t;
 #pragma unroll
     for (int j = 0; j < 4; j++) if (t + j >= s.first && t + j < s.last) to[j] += w[j];
@@ -535,12 +723,14 @@ struct Plan {
 Plan make_plan(const gqa_attn_args * a) {
     Plan pl;
     const int group = a->n_head / a->n_head_kv;
-    pl.nb = a->dv == 0 ? 8 : group > 16 ? 2 : 1;              // 16 heads a block of the operand; two where the group fills them
+    // blocks of 16 heads a wave holds: two where the group fills them and the registers allow it (heads of 256: a second block has its own workgroups,
+    // which find K and V in the caches), eight over a latent cache, whose Q lies in LDS
+    pl.nb = a->dv == 0 ? LROWS / 16 : group > 16 && a->dk < 256 ? 2 : 1;
     pl.rows = pl.nb * 16;
     pl.row_blocks = (group + pl.rows - 1) / pl.rows;
     pl.items = (int64_t) a->n_seq * a->n_head_kv * pl.row_blocks;
     const int64_t units = pl.items * a->bt_stride;
-    const int fill = 256 * wg_per_cu(a->dk, pl.nb);
+    const int fill = 256 * (a->dv ? wg_per_cu(a->dk, pl.nb) : 1);
     pl.n_wg = (int) (units < fill ? units : fill);
     if (a->n_workgroups > 0) pl.n_wg = (int) (units < a->n_workgroups ? units : a->n_workgroups);
     size_t at = 0;
@@ -557,16 +747,20 @@ Plan make_plan(const gqa_attn_args * a) {
     return pl;
 }
 
-template <bool F16, int DK, int DV, int NB, bool BIAS>
-hipError_t launch_main(const AttnP & p, hipStream_t st) {
-    constexpr int lds = DV ? 4 * 16 * DV * 4 : NB * 16 * (DK * 2 + 16);
-    static_assert(lds <= 160 * 1024 - 8192, "LDS");
+template <typename K> hipError_t launch_lds(K kernel, const AttnP & p, int threads, int lds, hipStream_t st) {
     if (lds > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute((const void *) gqa_attn_kernel<F16, DK, DV, NB, BIAS>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        const hipError_t e = hipFuncSetAttribute((const void *) kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((gqa_attn_kernel<F16, DK, DV, NB, BIAS>), dim3((unsigned) p.n_wg), dim3(256), lds, st, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned) p.n_wg), dim3((unsigned) threads), lds, st, p);
     return hipGetLastError();
+}
+template <bool F16, int DK, int DV, int NB, bool BIAS>
+hipError_t launch_main(const AttnP & p, hipStream_t st) { return launch_lds(gqa_attn_kernel<F16, DK, DV, NB, BIAS>, p, 256, 4 * 16 * DV * 4, st); }
+template <bool F16, bool BIAS>
+hipError_t launch_scores(const AttnP & p, hipStream_t st) {
+    static_assert(LROWS * LPITCH + LWAVES * LROWS * 8 <= 160 * 1024, "LDS");
+    return launch_lds(gqa_scores_kernel<F16, BIAS>, p, 64 * LWAVES, LROWS * LPITCH, st);
 }
 
 template <bool F16, int NB, bool BIAS>
@@ -575,7 +769,9 @@ hipError_t launch_widths(const AttnP & p, int dk, hipStream_t st) {
         case 64:  return launch_main<F16, 64, 64, NB, BIAS>(p, st);
         case 128: return launch_main<F16, 128, 128, NB, BIAS>(p, st);
         case 192: return launch_main<F16, 192, 128, NB, BIAS>(p, st);
-        default:  return launch_main<F16, 256, 256, NB, BIAS>(p, st);
+        default:
+            if constexpr (NB == 1) return launch_main<F16, 256, 256, NB, BIAS>(p, st);
+            else                   return hipErrorInvalidValue;        // (make_plan: one block)
     }
 }
 
@@ -583,20 +779,23 @@ template <bool F16>
 hipError_t launch_all(const AttnP & p, const Plan & pl, int dk, hipStream_t st) {
     const bool bias = p.mask || p.cap_out != 0.f;
     hipError_t e;
-    if (dk == 576)       e = bias ? launch_main<F16, 576, 0, 8, true>(p, st) : launch_main<F16, 576, 0, 8, false>(p, st);
+    if (dk == LK)        e = bias ? launch_scores<F16, true>(p, st) : launch_scores<F16, false>(p, st);
     else if (pl.nb == 2) e = bias ? launch_widths<F16, 2, true>(p, dk, st) : launch_widths<F16, 2, false>(p, dk, st);
     else                 e = bias ? launch_widths<F16, 1, true>(p, dk, st) : launch_widths<F16, 1, false>(p, dk, st);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((gqa_join_kernel<F16>), dim3((unsigned) (p.n_seq * p.n_head)), dim3(256), 0, st, p, pl.rows);
     if ((e = hipGetLastError()) != hipSuccess || !p.scores) return e;
-    hipLaunchKernelGGL(gqa_weights_kernel, dim3((unsigned) ((p.cap + 1023) / 1024), (unsigned) (p.n_seq * p.n_head_kv)), dim3(256), 0, st, p);
+    int parts = 1;
+    while (parts < 16 && parts < p.group) parts *= 2;
+    const int rows = 1024 / parts;
+    hipLaunchKernelGGL(gqa_weights_kernel, dim3((unsigned) ((p.cap + rows - 1) / rows), (unsigned) (p.n_seq * p.n_head_kv)), dim3(256), 0, st, p, parts);
     return hipGetLastError();
 }
 
 int check_pool(const gqa_pool & c) {
     if (!c.data) return MLA_ERR_NULL;
     if (!al16(c.data) || (c.nb_page & 15) || (c.nb_row & 15) || (c.nb_head & 15)) return MLA_ERR_BAD_ALIGNMENT;
-    if (c.nb_page < 0 || c.nb_head < 0 || c.nb_row < 0 || c.nb_row > (1 << 23)) return MLA_ERR_BAD_SHAPE;   // 128 rows within 31 bits
+    if (c.nb_page < 0 || c.nb_head < 0 || c.nb_row < 0 || c.nb_row > (1 << 23) || c.nb_page >= ((int64_t) 1 << 32)) return MLA_ERR_BAD_SHAPE;   // 128 rows within 31 bits, a page within 32
     return 0;
 }
 
@@ -649,10 +848,11 @@ extern "C" int gqa_attn_launch(const gqa_attn_args * a, void * stream) {
     char * ws = (char *) a->workspace;
     AttnP  p;
     p.q = (const char *) a->q; p.q_nb1 = a->q_nb1; p.q_nb2 = a->q_nb2; p.q_f32 = a->q_type == MLA_TYPE_F32;
-    p.k = (const char *) a->k.data; p.k_page = a->k.nb_page; p.k_head = a->k.nb_head; p.k_row = (int) a->k.nb_row;
-    p.v = (const char *) a->v.data; p.v_page = a->v.nb_page; p.v_head = a->v.nb_head; p.v_row = (int) a->v.nb_row;
+    p.k = (const char *) a->k.data; p.k_page = (unsigned) a->k.nb_page; p.k_head = a->k.nb_head; p.k_row = (int) a->k.nb_row;
+    p.v = (const char *) a->v.data; p.v_page = (unsigned) a->v.nb_page; p.v_head = a->v.nb_head; p.v_row = (int) a->v.nb_row;
     p.n_pages = a->n_pages; p.block_table = a->block_table; p.bt_stride = a->bt_stride; p.seq_lens = a->seq_lens;
-    p.mask = (const char *) a->mask; p.mask_nb1 = a->mask_nb1; p.mask_ne0 = a->mask_ne0;
+    p.mask = (const char *) a->mask; p.mask_nb1 = a->mask_nb1;
+    p.mask_len = a->mask && a->mask_ne0 < a->bt_stride * PAGE ? (int) a->mask_ne0 : (int) (a->bt_stride * PAGE);
     p.weights = a->weights; p.w_nb1 = a->w_nb1; p.w_nb2 = a->w_nb2;
     p.dst = (char *) a->dst; p.d_nb1 = a->d_nb1; p.d_nb2 = a->d_nb2; p.dst_f32 = a->dst_type == MLA_TYPE_F32;
     p.scale_log2 = a->scale * LOG2E;

@@ -262,7 +262,16 @@ __global__ void __launch_bounds__(SEL_THREADS) gqa_rank_kernel(const EvictP p, c
         const unsigned * from = k.hist + ((size_t) ((PASS - 1) & 1) * groups + group) * k.runs * BINS;
         const int        live = min(k.runs, (g.c1 + SEL_RUN - 1) / SEL_RUN);
         unsigned a = 0, c = 0;
-        for (int r = 0; r < live; r++) { a += from[r * BINS + tid]; c += from[r * BINS + SEL_THREADS + tid]; }
+        for (int r0 = 0; r0 < live; r0 += 8) {                     // 16 loads under way at a time
+            unsigned v[16];
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+                const unsigned * row = from + (size_t) min(r0 + r, live - 1) * BINS + tid;
+                v[2 * r] = row[0]; v[2 * r + 1] = row[SEL_THREADS];
+            }
+#pragma unroll
+            for (int r = 0; r < 8; r++) if (r0 + r < live) { a += v[2 * r]; c += v[2 * r + 1]; }
+        }
         hist[tid] = a; hist[SEL_THREADS + tid] = c;
         if constexpr (PASS > 1) got = k.picks[group * 2 + (PASS & 1)];      // the pass before's: digits but the last
         __syncthreads();
