@@ -18,6 +18,9 @@ using namespace mla;
 namespace {
 
 constexpr int MAX_PAIRS = 128;
+// Below this a token's sets of rows have workgroups of their own (one token of 40 rows: 6.2 -> 4.6 us), from there on one workgroup takes them all
+// and makes the table once.
+constexpr int FEW_TOKENS = 256;
 
 enum { T_F32 = 0, T_F16 = 1, T_BF16 = 2 };
 
@@ -34,7 +37,7 @@ struct FrontP {
     const float * ff;
     int   n_tok, n_head, n_head_kv, dk, dv, n_dims, neox, n_seq;
     int   w_type, dst_type;
-    float eps, mscale;
+    float eps, inv_dk, mscale;
     double turns[MAX_PAIRS];      // frequency of a pair, turns per position (YaRN blended in)
 };
 
@@ -58,8 +61,13 @@ __device__ __forceinline__ void load_weights(const char * w, int type, int at, f
     else if (type == T_F16) { const Raw8<T_F16> r = load8<T_F16>(w + (int64_t) at * 2); unpack8<T_F16>(r, x); }
     else                    { const Raw8<T_BF16> r = load8<T_BF16>(w + (int64_t) at * 2); unpack8<T_BF16>(r, x); }
 }
+// Rounded by the hardware's conversions (to nearest even; pack2's integer form of the bf16 rounding is 6 instructions a value, a third of the kernel's).
+template <bool F16> __device__ __forceinline__ unsigned pair16(float a, float b) {
+    if constexpr (F16) return bitcast<unsigned short>((_Float16) a) | ((unsigned) bitcast<unsigned short>((_Float16) b) << 16);
+    else               return bitcast<unsigned short>((__bf16) a) | ((unsigned) bitcast<unsigned short>((__bf16) b) << 16);
+}
 template <bool F16> __device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
-    return u32x4{ pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]), pack2<F16>(x[4], x[5]), pack2<F16>(x[6], x[7]) };
+    return u32x4{ pair16<F16>(x[0], x[1]), pair16<F16>(x[2], x[3]), pair16<F16>(x[4], x[5]), pair16<F16>(x[6], x[7]) };
 }
 __device__ __forceinline__ void store8(char * to, int type, const float (&x)[8]) {
     if (type == T_F16)       *(u32x4 *) to = pack8<true>(x);
@@ -77,25 +85,39 @@ __device__ __forceinline__ int64_t page_of(const FrontP & p, int t, int & row) {
     return page < 0 || page >= p.n_pages ? -1 : page;
 }
 
-// One workgroup a token; LPR lanes a row of dk values (the power of two that holds dk / 8).
-template <int SRC, bool KV_F16, int LPR>
+// Grid: (tokens, parts); LPR lanes a row of dk values (the power of two that holds dk / 8).  A workgroup takes every parts-th set of 256 / LPR rows
+// of its token, SETS of them at a time whose loads are all under way while the table is made, and part 0 the values.
+template <int SRC, bool KV_F16, int LPR, int SETS>
 __global__ void __launch_bounds__(256) gqa_norm_rope_kernel(const FrontP p) {
     __shared__ float2 cs[MAX_PAIRS];
-    constexpr int ROWS = 256 / LPR;
-    const int t = blockIdx.x;
+    constexpr int ROWS = 256 / LPR, ES = SRC == T_F32 ? 4 : 2;
+    const int t = blockIdx.x, parts = gridDim.y;
     const int sub = threadIdx.x % LPR, r0 = threadIdx.x / LPR;
     const int e0 = sub * 8;
     const bool live = e0 < p.dk;
-    const int  n_rows = p.n_head + (p.k.src ? p.n_head_kv : 0);
+    const int  n_rows = p.n_head + (p.k.src ? p.n_head_kv : 0), n_sets = (n_rows + ROWS - 1) / ROWS;
     const int  half = p.n_dims / 2;
-    auto at = [&](int r) -> const char * {
-        const bool isq = r < p.n_head;
-        const Rows & x = isq ? p.q : p.k;
-        return x.src + (int64_t) t * x.nb2 + (int64_t) (isq ? r : r - p.n_head) * x.nb1 + (live ? e0 : 0) * (SRC == T_F32 ? 4 : 2);
+    Raw8<SRC> raw[SETS], val;
+    auto load_sets = [&](int set0) {                               // (sets past the last repeat it)
+#pragma unroll
+        for (int i = 0; i < SETS; i++) {
+            const int  r = min(min(set0 + i * parts, n_sets - 1) * ROWS + r0, n_rows - 1);
+            const bool isq = r < p.n_head;
+            const char * src = (isq ? p.q.src : p.k.src) + (int64_t) t * (isq ? p.q.nb2 : p.k.nb2) + (int64_t) (isq ? r : r - p.n_head) * (isq ? p.q.nb1 : p.k.nb1);
+            if (i == 0 || set0 + i * parts < n_sets) raw[i] = load8<SRC>(src + (live ? e0 : 0) * ES);
+        }
     };
-    // the first rows are on their way while the table is made
-    Raw8<SRC> raw = load8<SRC>(at(min(r0, n_rows - 1)));
+    load_sets(blockIdx.y);
+    // values: runs of 8, the first 256 of them ahead like the rows
+    const int  per = p.dv / 8, n_val = p.v.src && blockIdx.y == 0 ? p.n_head_kv * per : 0;
+    auto val_at = [&](int i) { const int h = i / per, c = i - h * per; return p.v.src + (int64_t) t * p.v.nb2 + (int64_t) h * p.v.nb1 + c * 8 * ES; };
+    if ((int) threadIdx.x < n_val) val = load8<SRC>(val_at(threadIdx.x));
+    float gq[8], gk[8];                                            // the weights of this lane's values
+    if (p.qw) load_weights(p.qw, p.w_type, live ? e0 : 0, gq);
+    if (p.kw) load_weights(p.kw, p.w_type, live ? e0 : 0, gk);
     const int pos = p.pos[t];
+    int     row = 0;
+    const int64_t page = p.k.src ? page_of(p, t, row) : -1;
     for (int i = threadIdx.x; i < half; i += 256) {
         double f = p.turns[i];
         if (p.ff) f /= (double) p.ff[i];
@@ -103,62 +125,62 @@ __global__ void __launch_bounds__(256) gqa_norm_rope_kernel(const FrontP p) {
         const float  w = (float) (a - rint(a));                    // a fraction of a turn, in [-1/2, 1/2]
         cs[i] = make_float2(cospif(2.f * w) * p.mscale, sinpif(2.f * w) * p.mscale);
     }
-    int     row;
-    const int64_t page = p.k.src ? page_of(p, t, row) : -1;
-    if (p.v.src && page >= 0) {                                    // values: as they are
-        const int per = p.dv / 8;
-        for (int i = threadIdx.x; i < p.n_head_kv * per; i += 256) {
+    if (page >= 0)
+        for (int i = threadIdx.x; i < n_val; i += 256) {           // as they are
             const int h = i / per, c = i - h * per;
+            if (i >= 256) val = load8<SRC>(val_at(i));
             float x[8];
-            unpack8<SRC>(load8<SRC>(p.v.src + (int64_t) t * p.v.nb2 + (int64_t) h * p.v.nb1 + c * (SRC == T_F32 ? 32 : 16)), x);
+            unpack8<SRC>(val, x);
             *(u32x4 *) (p.vc + page * p.v_page + row * p.v_row + h * p.v_head + c * 16) = pack8<KV_F16>(x);
         }
-    }
     __syncthreads();
-    for (int r = r0; r - r0 < n_rows; r += ROWS) {                 // (every lane of a wave takes part in the shuffles)
-        const bool has = r < n_rows, isq = r < p.n_head;
-        float x[8];
-        unpack8<SRC>(raw, x);
-        if (r - r0 + ROWS < n_rows) raw = load8<SRC>(at(min(r + ROWS, n_rows - 1)));
-        const char * w = isq ? p.qw : p.kw;
-        if (w) {
-            float ss = 0.f, g[8];
-            load_weights(w, p.w_type, live ? e0 : 0, g);
-            if (live)
+    for (int set0 = blockIdx.y; set0 < n_sets; set0 += SETS * parts) {
+        if (set0 != (int) blockIdx.y) load_sets(set0);
 #pragma unroll
-                for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
+        for (int i = 0; i < SETS; i++) {                           // (every lane of a wave takes part in the shuffles)
+            if (set0 + i * parts >= n_sets) break;
+            const int  r = (set0 + i * parts) * ROWS + r0;
+            const bool has = r < n_rows, isq = r < p.n_head;
+            float x[8];
+            unpack8<SRC>(raw[i], x);
+            if (isq ? p.qw != nullptr : p.kw != nullptr) {
+                float ss = 0.f;
+                if (live)
 #pragma unroll
-            for (int d = 1; d < LPR; d <<= 1) ss += __shfl_xor(ss, d, 64);
-            const float inv = 1.f / sqrtf(ss / (float) p.dk + p.eps);
+                    for (int e = 0; e < 8; e++) ss = fmaf(x[e], x[e], ss);
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = x[i] * inv * g[i];
-        }
-        if (half) {
-            float y[8];
-            if (p.neox) {
-                // the other half of a pair: value e0 + n_dims/2 for the first half, e0 - n_dims/2 for the second (n_dims/2 a multiple of 8)
-                const bool low = e0 < half, in = e0 < p.n_dims;
-                const int  from = (int) (threadIdx.x & 63) + (in ? (low ? half / 8 : -(half / 8)) : 0);
+                for (int d = 1; d < LPR; d <<= 1) ss += __shfl_xor(ss, d, 64);
+                const float inv = __builtin_amdgcn_rsqf(fmaf(ss, p.inv_dk, p.eps));    // (off by 2^-23 of itself at most)
 #pragma unroll
-                for (int i = 0; i < 8; i++) y[i] = __shfl(x[i], from, 64);
-                if (in)
+                for (int e = 0; e < 8; e++) x[e] = x[e] * inv * (isq ? gq[e] : gk[e]);
+            }
+            if (half) {
+                float y[8];
+                if (p.neox) {
+                    // the other half of a pair: value e0 + n_dims/2 for the first half, e0 - n_dims/2 for the second (n_dims/2 a multiple of 8)
+                    const bool low = e0 < half, in = e0 < p.n_dims;
+                    const int  from = (int) (threadIdx.x & 63) + (in ? (low ? half / 8 : -(half / 8)) : 0);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float2 c = cs[low ? e0 + i : e0 - half + i];
-                        x[i] = low ? fmaf(x[i], c.x, -y[i] * c.y) : fmaf(y[i], c.y, x[i] * c.x);
+                    for (int e = 0; e < 8; e++) y[e] = __shfl(x[e], from, 64);
+                    if (in)
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const float2 c = cs[low ? e0 + e : e0 - half + e];
+                            x[e] = low ? fmaf(x[e], c.x, -y[e] * c.y) : fmaf(y[e], c.y, x[e] * c.x);
+                        }
+                } else if (e0 < p.n_dims) {
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        const float2 c = cs[(e0 + e) / 2];
+                        const float  a = x[e], b = x[e + 1];
+                        x[e] = fmaf(a, c.x, -b * c.y); x[e + 1] = fmaf(a, c.y, b * c.x);
                     }
-            } else if (e0 < p.n_dims) {
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    const float2 c = cs[(e0 + i) / 2];
-                    const float  a = x[i], b = x[i + 1];
-                    x[i] = fmaf(a, c.x, -b * c.y); x[i + 1] = fmaf(a, c.y, b * c.x);
                 }
             }
+            if (!has || !live) continue;
+            if (isq) store8(p.q_dst + (int64_t) t * p.qd_nb2 + (int64_t) r * p.qd_nb1 + e0 * (p.dst_type == T_F32 ? 4 : 2), p.dst_type, x);
+            else if (page >= 0) *(u32x4 *) (p.kc + page * p.k_page + row * p.k_row + (r - p.n_head) * p.k_head + e0 * 2) = pack8<KV_F16>(x);
         }
-        if (!has || !live) continue;
-        if (isq) store8(p.q_dst + (int64_t) t * p.qd_nb2 + (int64_t) r * p.qd_nb1 + e0 * (p.dst_type == T_F32 ? 4 : 2), p.dst_type, x);
-        else if (page >= 0) *(u32x4 *) (p.kc + page * p.k_page + row * p.k_row + (r - p.n_head) * p.k_head + e0 * 2) = pack8<KV_F16>(x);
     }
 }
 
@@ -166,12 +188,17 @@ int type_of(int ggml) { return ggml == MLA_TYPE_F32 ? T_F32 : ggml == MLA_TYPE_F
 bool known(int ggml) { return ggml == MLA_TYPE_F32 || ggml == MLA_TYPE_F16 || ggml == MLA_TYPE_BF16; }
 bool al16(const void * ptr) { return ((uintptr_t) ptr & 15) == 0; }
 
+template <int SRC, bool KV_F16, int LPR>
+void launch_lanes(const FrontP & p, hipStream_t st) {
+    const int rows = 256 / LPR, sets = (p.n_head + (p.k.src ? p.n_head_kv : 0) + rows - 1) / rows;
+    if (p.n_tok < FEW_TOKENS) hipLaunchKernelGGL((gqa_norm_rope_kernel<SRC, KV_F16, LPR, 1>), dim3((unsigned) p.n_tok, (unsigned) (sets < 64 ? sets : 64)), dim3(256), 0, st, p);
+    else                      hipLaunchKernelGGL((gqa_norm_rope_kernel<SRC, KV_F16, LPR, 4>), dim3((unsigned) p.n_tok), dim3(256), 0, st, p);
+}
 template <int SRC, bool KV_F16>
 void launch_rows(const FrontP & p, hipStream_t st) {
-    const dim3 grid((unsigned) p.n_tok);
-    if (p.dk <= 64)       hipLaunchKernelGGL((gqa_norm_rope_kernel<SRC, KV_F16, 8>), grid, dim3(256), 0, st, p);
-    else if (p.dk <= 128) hipLaunchKernelGGL((gqa_norm_rope_kernel<SRC, KV_F16, 16>), grid, dim3(256), 0, st, p);
-    else                  hipLaunchKernelGGL((gqa_norm_rope_kernel<SRC, KV_F16, 32>), grid, dim3(256), 0, st, p);
+    if (p.dk <= 64)       launch_lanes<SRC, KV_F16, 8>(p, st);
+    else if (p.dk <= 128) launch_lanes<SRC, KV_F16, 16>(p, st);
+    else                  launch_lanes<SRC, KV_F16, 32>(p, st);
 }
 template <bool KV_F16>
 void launch_src(const FrontP & p, int src, hipStream_t st) {
@@ -233,7 +260,7 @@ extern "C" int gqa_norm_rope_launch(const gqa_norm_rope_args * a, void * stream)
     p.n_tok = a->n_tok; p.n_head = a->n_head; p.n_head_kv = a->n_head_kv; p.dk = a->dk; p.dv = a->dv; p.n_dims = a->n_dims; p.n_seq = a->n_seq;
     p.neox = a->mode == MLA_ROPE_MODE_NEOX;
     p.w_type = type_of(a->w_type); p.dst_type = type_of(a->dst_type);
-    p.eps = a->eps; p.mscale = (float) a->attn_factor;
+    p.eps = a->eps; p.inv_dk = 1.f / (float) a->dk; p.mscale = (float) a->attn_factor;
     // f_i = freq_base^(-2i / n_dims), scaled by freq_scale where YaRN interpolates (ggml/src/ggml-cpu/ggml-cpu.c:10272-10293, the
     // correction dims of ggml/src/ggml.c:3529-3541), in turns
     const double n = a->n_dims, base = a->freq_base, pi = 3.14159265358979323846;
