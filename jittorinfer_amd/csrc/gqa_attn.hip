@@ -46,9 +46,10 @@ struct AttnP {
     char * dst; int64_t d_nb1, d_nb2; int dst_f32;
     float scale_log2;             // scale * log2(e)
     float cap_in, cap_out;        // soft cap c: c * tanh(x / c) = c - 2c / (exp2(cap_in * q.k) + 1), times log2(e); cap_out = 0: none
-    int window, n_seq, n_head, n_head_kv, group, row_blocks, head_blocks, dv;
+    int window, n_seq, n_head, n_head_kv, group, row_blocks, head_blocks, dv, quad;
+    int rows;                     // heads of a head block, as partial results lie: row_blocks of up to 16 or 32 (128) a KV head, or (quad) four KV heads' groups
     int n_wg;
-    float *  part_o;              // [2 * n_wg][rows][DV]
+    float *  part_o;              // [2 * n_wg][rows][dv]
     float2 * part_ml;             // [2 * n_wg][rows]: maximum (log2 units), sum
     int2 *   items;               // [n_seq * head_blocks]: (2 * first workgroup + whether the item begins inside its run, last workgroup)
     float *  scores;              // [n_seq][n_head][cap] in log2 units, or nullptr
@@ -176,14 +177,16 @@ __device__ __forceinline__ const char * page_base(const char * data, int page, u
     return data + head + (int64_t) ((uint64_t) __umulhi((unsigned) page, nb_page) << 32 | (unsigned) page * nb_page);
 }
 
-// Wave w takes quarter w of every page of the run.
-template <bool F16, int DK, int DV, int NB, bool BIAS>
+// Wave w takes quarter w of every page of the run.  QUAD: wave w takes whole pages of KV head w of four, which are the run's head block: a row's four
+// heads are read side by side, and the waves have nothing to join.
+template <bool F16, int DK, int DV, int NB, bool BIAS, bool QUAD>
 __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const AttnP p) {
+    static_assert(NB == 1 || !QUAD, "one block of heads a wave");
     constexpr int  KC    = DK / 32;
     constexpr int  ROWS  = NB * 16, NW = 4;
     using VG = VGeom<DV>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    __shared__ float2 sh_ml[NW][ROWS];
+    __shared__ float2 sh_ml[QUAD ? 1 : NW][ROWS];
 
     const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), l15 = lane & 15, lg = lane >> 4;
     const int wg = blockIdx.x;
@@ -208,7 +211,7 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
         b = uni(b); hb = uni(hb); pg = uni(pg); np = uni(np); s = Span{ uni(s.first), uni(s.last) };
         const int  n = uni(min(np - pg, u_end - u));         // pages of this piece
         const bool begins = pg == 0, whole = begins && n == np;
-        const int  kvh = uni(hb / p.row_blocks), row0 = (hb - kvh * p.row_blocks) * ROWS;   // first head of the group taken here
+        const int  kvh = QUAD ? hb * 4 + wave : uni(hb / p.row_blocks), row0 = QUAD ? 0 : (hb - kvh * p.row_blocks) * ROWS;   // first head of the group taken here
         const int  heads = min(ROWS, p.group - row0);
         const int  head0 = kvh * p.group + row0;
         if (begins && threadIdx.x == 0) p.items[(int64_t) b * p.head_blocks + hb] = make_int2(2 * wg + (fresh ? 0 : 1), owner_of(deal, u + np - 1));
@@ -217,8 +220,13 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
         const int       t_page0 = (s.first / PAGE + pg) * PAGE;
         u32x4 kf[2][KC];
         u32x2 vf[8][VG::COLS / 4];
+        // tile i of this wave: its page of the piece and its first row there
+        auto page_of = [&](int i) { return QUAD ? i >> 2 : i; };
+        auto slot0 = [&](int i) { return QUAD ? (i & 3) * 32 : wave * 32; };
+        // (of four quarters those that have rows)
+        const int i_begin = QUAD ? max(s.first - t_page0, 0) / 32 : 0, i_end = QUAD ? min(4 * n, (s.last - t_page0 + 31) / 32) : n;
         // the slots in the page whose rows a lane loads: rows outside the span are replaced by the nearest one inside
-        auto slot = [&](int i, int r) { return min(max(wave * 32 + r, s.first - (t_page0 + i * PAGE)), s.last - 1 - (t_page0 + i * PAGE)); };
+        auto slot = [&](int i, int r) { const int t = t_page0 + page_of(i) * PAGE; return min(max(slot0(i) + r, s.first - t), s.last - 1 - t); };
         const int64_t k_off = (int64_t) kvh * p.k_head, v_off = (int64_t) kvh * p.v_head;
         auto load_k = [&](int i, int page) {
             const char * base = page_base(p.k, page, p.k_page, k_off);
@@ -243,7 +251,7 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
                 }
             }
         };
-        auto id_at = [&](int i) { return scalar_at(p.block_table, bt0 + min(i, n - 1)); };        // page of the piece's page i
+        auto id_at = [&](int i) { return scalar_at(p.block_table, bt0 + min(page_of(i), n - 1)); };        // page id of tile i
         auto good = [&](int id) { return id >= 0 && id < p.n_pages; };          // (a bad id: page 0 is read, not used)
 
         u32x2 mk[2];                                            // the mask of a tile's rows
@@ -251,13 +259,13 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
             if constexpr (BIAS)
                 if (p.mask)
 #pragma unroll
-                    for (int blk = 0; blk < 2; blk++) mk[blk] = mask4(p, b, t_page0 + i * PAGE + wave * 32 + blk * 16 + lg * 4, s);
+                    for (int blk = 0; blk < 2; blk++) mk[blk] = mask4(p, b, t_page0 + page_of(i) * PAGE + slot0(i) + blk * 16 + lg * 4, s);
         };
 
-        int id = id_at(0), id_next = id_at(1);                  // (ids are fetched a tile ahead of their rows)
-        load_k(0, good(id) ? id : 0);
-        load_v(0, good(id) ? id : 0);
-        load_mask(0);
+        int id = id_at(i_begin), id_next = id_at(i_begin + 1);  // (ids are fetched a tile ahead of their rows)
+        load_k(i_begin, good(id) ? id : 0);
+        load_v(i_begin, good(id) ? id : 0);
+        load_mask(i_begin);
         // ---- Q: operand fragments, lane (h, g) k = 32 c + 8 g .. + 7; heads past the group: zeros
         u32x4 qf[NB * KC];
         auto q_at = [&](int row, int off) { return p.q + (int64_t) b * p.q_nb2 + (int64_t) (head0 + min(row, heads - 1)) * p.q_nb1 + off * (p.q_f32 ? 4 : 2); };   // 8 values from `off` on
@@ -294,7 +302,7 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
         // wait be for all of them)
         auto tile = [&](auto more_tag, int i) __attribute__((always_inline)) {
             constexpr bool MORE = decltype(more_tag)::value;
-            const int  t0 = t_page0 + i * PAGE + wave * 32;  // first row of the tile
+            const int  t0 = t_page0 + page_of(i) * PAGE + slot0(i);  // first row of the tile
             const int  lo = max(s.first - t0, 0), hi = min(s.last - t0, 32);
             const bool use = good(id) && hi > lo, all = lo == 0 && hi == 32;
             const int  next = good(id_next) ? id_next : 0;
@@ -399,18 +407,45 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
             }
             if constexpr (MORE) load_v(i + 1, next);
         };
-        int i = 0;
-        for (; i + 1 < n; i++) tile(std::true_type{}, i);
+        int i = i_begin;
+        for (; i + 1 < i_end; i++) tile(std::true_type{}, i);
         tile(std::false_type{}, i);
 
-        // ---- the waves' results meet in LDS
+        const int64_t piece = 2 * (int64_t) wg + (fresh ? 0 : 1);
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
-            float t = l[nb];
-            t += __shfl_xor(t, 16, 64);
-            t += __shfl_xor(t, 32, 64);
-            if (lg == 0) sh_ml[wave][nb * 16 + l15] = make_float2(m[nb], t);
+            l[nb] += __shfl_xor(l[nb], 16, 64);
+            l[nb] += __shfl_xor(l[nb], 32, 64);
         }
+        if constexpr (QUAD) {
+            const float inv = l[0] == 0.f ? 0.f : 1.f / l[0];    // (a NaN stays one)
+            if (lg == 0 && l15 < heads) {
+                if (!whole) p.part_ml[piece * p.rows + wave * p.group + l15] = make_float2(m[0], l[0]);
+                else if (p.scores) p.lse[(int64_t) b * p.n_head + head0 + l15] = make_float2(m[0] == -INFINITY ? 0.f : m[0], inv);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int   row = lg * 4 + j;
+                const float f = whole ? __shfl(inv, row, 64) : 1.f;
+                if (row >= heads) continue;
+                char *  dst = p.dst + (int64_t) b * p.d_nb2 + (int64_t) (head0 + row) * p.d_nb1;
+                float * part = p.part_o + (piece * p.rows + wave * p.group + row) * DV;
+#pragma unroll
+                for (int gr = 0; gr < VG::GROUPS; gr++)
+#pragma unroll
+                    for (int c = 0; c < VG::W; c += 4) {
+                        const int   a = gr * VG::W + c, col = gr * 128 + l15 * VG::W + c;
+                        const f32x4 o = f32x4{ acc[0][a][j], acc[0][a + 1][j], acc[0][a + 2][j], acc[0][a + 3][j] } * f;
+                        if (!whole)         *(f32x4 *) (part + col) = o;
+                        else if (p.dst_f32) *(f32x4 *) (dst + col * 4) = o;
+                        else                *(u32x2 *) (dst + col * 2) = u32x2{ pair16<F16>(o.x, o.y), pair16<F16>(o.z, o.w) };
+                    }
+            }
+        } else {
+        // ---- the waves' results meet in LDS
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+            if (lg == 0) sh_ml[wave][nb * 16 + l15] = make_float2(m[nb], l[nb]);
         __syncthreads();
         auto joined = [&](int row) -> float2 {               // maximum and sum over the waves
             float M = -INFINITY, L = 0.f;
@@ -420,10 +455,9 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
             for (int w = 0; w < NW; w++) L += sh_ml[w][row].y == 0.f ? 0.f : sh_ml[w][row].y * fast_exp2(sh_ml[w][row].x - M);
             return make_float2(M, L);
         };
-        const int64_t piece = 2 * (int64_t) wg + (fresh ? 0 : 1);
         for (int r = threadIdx.x; r < heads; r += 256) {
             const float2 ml = joined(r);
-            if (!whole) p.part_ml[piece * ROWS + r] = ml;
+            if (!whole) p.part_ml[piece * p.rows + r] = ml;
             else if (p.scores) p.lse[(int64_t) b * p.n_head + head0 + r] = make_float2(ml.x == -INFINITY ? 0.f : ml.x, ml.y == 0.f ? 0.f : 1.f / ml.y);
         }
         float * part = (float *) lds;                         // [4][16][DV]
@@ -452,7 +486,7 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
                 f32x4 o = *(const f32x4 *) (part + r * DV + c);
 #pragma unroll
                 for (int w = 1; w < 4; w++) o += *(const f32x4 *) (part + (w * 16 + r) * DV + c);
-                if (!whole) *(f32x4 *) (p.part_o + (piece * ROWS + row) * DV + c) = o;
+                if (!whole) *(f32x4 *) (p.part_o + (piece * p.rows + row) * DV + c) = o;
                 else {
                     const float L = joined(row).y, inv = L == 0.f ? 0.f : 1.f / L;   // (a NaN stays one)
                     char * to = p.dst + (int64_t) b * p.d_nb2 + (int64_t) (head0 + row) * p.d_nb1;
@@ -463,6 +497,7 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
             }
         }
         __syncthreads();                                      // LDS is free again for the next piece
+        }
 
         u += n; pg = 0;
         if (++hb == p.head_blocks && u < u_end) {
@@ -611,7 +646,7 @@ __global__ void __launch_bounds__(64 * LWAVES) gqa_scores_kernel(const AttnP p) 
             for (int w = 0; w < LWAVES; w++) M = fmaxf(M, sh_ml[w][r].x);
 #pragma unroll
             for (int w = 0; w < LWAVES; w++) L += sh_ml[w][r].y == 0.f ? 0.f : sh_ml[w][r].y * fast_exp2(sh_ml[w][r].x - M);
-            if (!whole) p.part_ml[piece * LROWS + r] = make_float2(M, L);
+            if (!whole) p.part_ml[piece * p.rows + r] = make_float2(M, L);
             else        p.lse[(int64_t) b * p.n_head + head0 + r] = make_float2(M == -INFINITY ? 0.f : M, L == 0.f ? 0.f : 1.f / L);
         }
         __syncthreads();                                       // LDS is free again for the next piece
@@ -624,53 +659,72 @@ __global__ void __launch_bounds__(64 * LWAVES) gqa_scores_kernel(const AttnP p) 
 }
 
 // Joins what the runs left of one head (grid: a workgroup per (sequence, head)): o = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M), pieces in
-// the order of the rows.  Heads whose rows one run covered are done; heads without a row get zeros.
+// the order of the rows, eight under way at a time a thread.  Heads whose rows one run covered are done; heads without a row get zeros.
+constexpr int JOIN = 256;
 template <bool F16>
-__global__ void __launch_bounds__(256) gqa_join_kernel(const AttnP p, const int rows) {
-    __shared__ float  red[8];
-    __shared__ f32x4  sum[256];
+__global__ void __launch_bounds__(JOIN) gqa_join_kernel(const AttnP p) {
+    __shared__ float  red[2][JOIN / 64], weight[JOIN];
+    __shared__ f32x4  sum[JOIN];
     const int b = blockIdx.x / p.n_head, h = blockIdx.x - b * p.n_head;
-    const int kvh = h / p.group, r_all = h - kvh * p.group, rb = r_all / rows, row = r_all - rb * rows;
+    const int kvh = h / p.group, r = h - kvh * p.group;
+    const int hb = p.quad ? kvh >> 2 : kvh * p.row_blocks + r / p.rows, row = p.quad ? (kvh & 3) * p.group + r : r % p.rows;
     char *    dst = p.dst ? p.dst + (int64_t) b * p.d_nb2 + (int64_t) h * p.d_nb1 : nullptr;
     const int cols = p.dv / 4;                                // runs of 4 columns
     auto store = [&](int c, f32x4 o) {
         if (p.dst_f32) *(f32x4 *) (dst + c * 16) = o;
         else *(u32x2 *) (dst + c * 8) = u32x2{ pair16<F16>(o.x, o.y), pair16<F16>(o.z, o.w) };
     };
-    const int2 it = p.items[(int64_t) b * p.head_blocks + kvh * p.row_blocks + rb];   // (meaningless, and not used, where there is no row)
+    const int2 it = p.items[(int64_t) b * p.head_blocks + hb];   // (meaningless, and not used, where there is no row)
     if (pages_of(span_of(p, b)) == 0) {
-        for (int c = threadIdx.x; c < cols; c += 256) store(c, f32x4{ 0.f, 0.f, 0.f, 0.f });
+        for (int c = threadIdx.x; c < cols; c += JOIN) store(c, f32x4{ 0.f, 0.f, 0.f, 0.f });
         return;
     }
     const int  v0 = it.x >> 1, n = it.y - v0 + 1;
     if (n == 1) return;
-    auto slot = [&](int i) -> int64_t { return ((int64_t) (i ? 2 * (v0 + i) : it.x)) * rows + row; };
-
-    float M = -INFINITY;
-    for (int i = threadIdx.x; i < n; i += 256) M = fmaxf(M, p.part_ml[slot(i)].x);
+    auto slot = [&](int i) -> int64_t { return ((int64_t) (i ? 2 * (v0 + i) : it.x)) * p.rows + row; };
+    auto over_waves = [&](float v, bool maximum) {            // the same in every thread
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = M;
-    __syncthreads();
-    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        for (int d = 1; d < 64; d <<= 1) { const float o = __shfl_xor(v, d, 64); v = maximum ? fmaxf(v, o) : v + o; }
+        if ((threadIdx.x & 63) == 0) red[maximum][threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = red[maximum][0];
+        for (int w = 1; w < JOIN / 64; w++) v = maximum ? fmaxf(v, red[maximum][w]) : v + red[maximum][w];
+        return v;
+    };
+    // rows and factors of the first pieces are requested together: after the item's, their addresses depend on nothing
+    const int groups = cols ? JOIN / cols : 1, g = cols ? (int) threadIdx.x / cols : 0, c = (int) threadIdx.x - g * cols;   // (cols: 16, 32 or 64)
+    f32x4 x[8];
+    auto rows = [&](int k, int end) {                         // pieces k, k + groups, ..; past the end: the last one
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = *(const f32x4 *) (p.part_o + slot(min(k + e * groups, end - 1)) * p.dv + c * 4);
+    };
+    const float2 first = (int) threadIdx.x < n ? p.part_ml[slot(threadIdx.x)] : make_float2(-INFINITY, 0.f);
+    if (cols) rows(g, min(JOIN, n));
+    float M = first.x;
+    for (int i = threadIdx.x + JOIN; i < n; i += JOIN) M = fmaxf(M, p.part_ml[slot(i)].x);
+    M = over_waves(M, true);
+    // pieces in runs of JOIN: their factors, then their rows
     float L = 0.f;
-    for (int i = threadIdx.x; i < n; i += 256) { const float2 ml = p.part_ml[slot(i)]; if (ml.y != 0.f) L += ml.y * fast_exp2(ml.x - M); }
+    f32x4 o = { 0.f, 0.f, 0.f, 0.f };
+    for (int i0 = 0; i0 < n; i0 += JOIN) {
+        const int    end = min(i0 + JOIN, n);
+        const float2 ml  = i0 == 0 ? first : i0 + (int) threadIdx.x < end ? p.part_ml[slot(i0 + threadIdx.x)] : make_float2(0.f, 0.f);
+        const float  w   = ml.y == 0.f ? 0.f : fast_exp2(ml.x - M);
+        L += ml.y * w;
+        if (i0) __syncthreads();
+        weight[threadIdx.x] = w;
+        __syncthreads();
+        if (cols)
+            for (int k = i0 + g; k < end; k += groups * 8) {
+                if (k >= groups) rows(k, end);                // (the first ones are here)
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) L += __shfl_xor(L, d, 64);
-    if ((threadIdx.x & 63) == 0) red[4 + (threadIdx.x >> 6)] = L;
-    __syncthreads();
-    L = (red[4] + red[5]) + (red[6] + red[7]);
+                for (int e = 0; e < 8; e++) if (k + e * groups < end) o += x[e] * weight[k + e * groups - i0];
+            }
+    }
+    L = over_waves(L, false);
     const float inv = L == 0.f ? 0.f : 1.f / L;
     if (p.scores && threadIdx.x == 0) p.lse[(int64_t) b * p.n_head + h] = make_float2(M == -INFINITY ? 0.f : M, inv);
     if (!cols) return;
-
-    const int groups = 256 / cols, g = threadIdx.x / cols, c = threadIdx.x - g * cols;   // (cols: 16, 32 or 64)
-    f32x4 o = { 0.f, 0.f, 0.f, 0.f };
-    for (int i = g; i < n; i += groups) {
-        const int64_t at = slot(i);
-        const float2  ml = p.part_ml[at];
-        if (ml.y != 0.f) o += *(const f32x4 *) (p.part_o + at * p.dv + c * 4) * fast_exp2(ml.x - M);
-    }
     sum[threadIdx.x] = o;
     __syncthreads();
     if (g == 0) {
@@ -715,20 +769,32 @@ __global__ void __launch_bounds__(256) gqa_weights_kernel(const AttnP p, const i
 bool al16(const void * ptr) { return ((uintptr_t) ptr & 15) == 0; }
 
 struct Plan {
-    int     nb, rows, row_blocks, n_wg;
+    int     nb, rows, row_blocks, head_blocks, n_wg;
+    bool    quad;
     int64_t items;
     size_t  off_ml, off_items, off_scores, off_lse, bytes;    // of the workspace; partial rows first
 };
 
+// Both sides of the rules below, whole calls on one MI355X, bf16.  Two blocks of 16 heads a wave against one: 64 heads on 2, 64 x 16384 rows 196 against
+// 306 us, 32 x 2048 rows (1024 pages) 25 against 31; 32 heads on 1, 32 x 2048 rows (512 pages) 19.3 against 17.9, 1 x 1024 14.7 against 12.6.
+// Four KV heads a workgroup against one, rows row by row: 16 heads of 64, 32 x 8192 rows 185 against 224 us; 32 on 8 of 128, 8 x 16384 rows (8192 pages) 102
+// against 110, 16 x 4096 (4096 pages) 50 against 51; 16 on 4 of 64, 8 x 16384 (4096 pages) 32 against 30, 1 x 8192 14.4 against 13.0.  Heads
+// of 256: 187 against 187.  Head by head the pages are contiguous anyway: 32 on 8 of 128, 32 x 8192 rows 193 against 187.
+constexpr int64_t TWO_BLOCKS = 1024, QUADS = 8192;
 Plan make_plan(const gqa_attn_args * a) {
     Plan pl;
     const int group = a->n_head / a->n_head_kv;
+    const int64_t pages = (int64_t) a->n_seq * a->n_head_kv * a->bt_stride;      // at most
     // blocks of 16 heads a wave holds: two where the group fills them and the registers allow it (heads of 256: a second block has its own workgroups,
     // which find K and V in the caches), eight over a latent cache, whose Q lies in LDS
-    pl.nb = a->dv == 0 ? LROWS / 16 : group > 16 && a->dk < 256 ? 2 : 1;
-    pl.rows = pl.nb * 16;
-    pl.row_blocks = (group + pl.rows - 1) / pl.rows;
-    pl.items = (int64_t) a->n_seq * a->n_head_kv * pl.row_blocks;
+    pl.nb = a->dv == 0 ? LROWS / 16 : group > 16 && a->dk < 256 && pages >= TWO_BLOCKS ? 2 : 1;
+    // four KV heads a workgroup where a row's heads lie side by side in both caches
+    const bool side = a->k.nb_row >= a->n_head_kv * a->k.nb_head && a->v.nb_row >= a->n_head_kv * a->v.nb_head;
+    pl.quad = a->dv != 0 && a->dk < 256 && group <= 16 && a->n_head_kv % 4 == 0 && side && pages >= QUADS;
+    pl.rows = pl.quad ? 4 * group : pl.nb * 16;
+    pl.row_blocks = pl.quad ? 1 : (group + pl.rows - 1) / pl.rows;
+    pl.head_blocks = pl.quad ? a->n_head_kv / 4 : a->n_head_kv * pl.row_blocks;
+    pl.items = (int64_t) a->n_seq * pl.head_blocks;
     const int64_t units = pl.items * a->bt_stride;
     const int fill = 256 * (a->dv ? wg_per_cu(a->dk, pl.nb) : 1);
     pl.n_wg = (int) (units < fill ? units : fill);
@@ -756,7 +822,10 @@ template <typename K> hipError_t launch_lds(K kernel, const AttnP & p, int threa
     return hipGetLastError();
 }
 template <bool F16, int DK, int DV, int NB, bool BIAS>
-hipError_t launch_main(const AttnP & p, hipStream_t st) { return launch_lds(gqa_attn_kernel<F16, DK, DV, NB, BIAS>, p, 256, 4 * 16 * DV * 4, st); }
+hipError_t launch_main(const AttnP & p, hipStream_t st) {
+    if constexpr (NB == 1 && DK < 256) if (p.quad) return launch_lds(gqa_attn_kernel<F16, DK, DV, NB, BIAS, true>, p, 256, 0, st);
+    return launch_lds(gqa_attn_kernel<F16, DK, DV, NB, BIAS, false>, p, 256, 4 * 16 * DV * 4, st);
+}
 template <bool F16, bool BIAS>
 hipError_t launch_scores(const AttnP & p, hipStream_t st) {
     static_assert(LROWS * LPITCH + LWAVES * LROWS * 8 <= 160 * 1024, "LDS");
@@ -783,7 +852,7 @@ hipError_t launch_all(const AttnP & p, const Plan & pl, int dk, hipStream_t st) 
     else if (pl.nb == 2) e = bias ? launch_widths<F16, 2, true>(p, dk, st) : launch_widths<F16, 2, false>(p, dk, st);
     else                 e = bias ? launch_widths<F16, 1, true>(p, dk, st) : launch_widths<F16, 1, false>(p, dk, st);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((gqa_join_kernel<F16>), dim3((unsigned) (p.n_seq * p.n_head)), dim3(256), 0, st, p, pl.rows);
+    hipLaunchKernelGGL((gqa_join_kernel<F16>), dim3((unsigned) (p.n_seq * p.n_head)), dim3(JOIN), 0, st, p);
     if ((e = hipGetLastError()) != hipSuccess || !p.scores) return e;
     int parts = 1;
     while (parts < 16 && parts < p.group) parts *= 2;
@@ -859,7 +928,7 @@ extern "C" int gqa_attn_launch(const gqa_attn_args * a, void * stream) {
     p.cap_in  = a->logit_softcap > 0.f ? 2.f * LOG2E * a->scale / a->logit_softcap : 0.f;
     p.cap_out = a->logit_softcap * LOG2E;
     p.window = a->window; p.n_seq = a->n_seq; p.n_head = a->n_head; p.n_head_kv = a->n_head_kv; p.group = a->n_head / a->n_head_kv;
-    p.row_blocks = pl.row_blocks; p.head_blocks = a->n_head_kv * pl.row_blocks; p.dv = a->dv; p.n_wg = pl.n_wg;
+    p.row_blocks = pl.row_blocks; p.head_blocks = pl.head_blocks; p.rows = pl.rows; p.quad = pl.quad; p.dv = a->dv; p.n_wg = pl.n_wg;
     p.part_o = (float *) ws; p.part_ml = (float2 *) (ws + pl.off_ml); p.items = (int2 *) (ws + pl.off_items);
     p.scores = a->weights ? (float *) (ws + pl.off_scores) : nullptr; p.lse = a->weights ? (float2 *) (ws + pl.off_lse) : nullptr;
     p.cap = a->bt_stride * PAGE;

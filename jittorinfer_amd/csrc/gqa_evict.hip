@@ -19,8 +19,9 @@ namespace {
 
 constexpr int PAGE = MLA_PAGE_TOKENS;
 constexpr int SEL_THREADS = 1024, SEL_PER = 8, SEL_RUN = SEL_THREADS * SEL_PER, SEL_RUNS = 4, SEL_CHUNK = SEL_RUN * SEL_RUNS;
-constexpr int SEL_ONE = SEL_CHUNK;                   // rows up to which one workgroup a group selects
-constexpr int SEL_MANY = 8192;                       // runs of 8192 rows up to which several do: beyond, the groups alone fill the chip, and the histograms 128 MB
+// One workgroup a group, or one a run of 8192 rows in four launches.  Measured, a whole call: 8 groups of 16384 rows 27.6 against 32.4 us, of 32768
+// rows 39.7 against 34.0; 64 groups of 32768 rows 56.3 against 56.4, of 131072 195 against 173; 256 groups of 65536 rows 295 against 348.
+constexpr int SEL_ONE = 3 * SEL_RUN, SEL_GROUPS = 64, SEL_MANY = 8192;       // (SEL_MANY runs at most: 128 MB of histograms)
 constexpr int BINS = 2048;
 
 struct EvictP {
@@ -412,7 +413,7 @@ Plan make_plan(const gqa_evict_args * a) {
     pl.segments = (int64_t) a->n_seq * a->n_head_kv * (pl.k.count + pl.v.count);
     const size_t groups = (size_t) a->n_seq * a->n_head_kv;
     const int64_t runs = (cap + SEL_RUN - 1) / SEL_RUN;
-    pl.runs = cap > SEL_ONE && n_keep && (int64_t) groups * runs <= SEL_MANY ? (int) runs : 0;
+    pl.runs = cap > SEL_ONE && n_keep && groups <= SEL_GROUPS && (int64_t) groups * runs <= SEL_MANY ? (int) runs : 0;
     size_t at = 0;
     auto take = [&](size_t n) { const size_t o = at; at += (n + 255) & ~(size_t) 255; return o; };
     take((size_t) (1 + pl.segments) * 4);

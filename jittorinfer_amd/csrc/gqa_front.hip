@@ -20,7 +20,7 @@ namespace {
 constexpr int MAX_PAIRS = 128;
 // Below this a token's sets of rows have workgroups of their own (one token of 40 rows: 6.2 -> 4.6 us), from there on one workgroup takes them all
 // and makes the table once.
-constexpr int FEW_TOKENS = 256;
+constexpr int FEW_TOKENS = 1024;
 
 enum { T_F32 = 0, T_F16 = 1, T_BF16 = 2 };
 

@@ -72,6 +72,20 @@ def test_attn_widths_types_layouts(gpu, dk, dv, dtype, layout):
 def test_attn_groups(gpu, heads, kv_heads):
     """A query head for itself, groups that fill a block of 16, that pass it, and more than the two blocks a wave holds."""
     _check_attn(gpu, *_attn_case(heads, [5, 200, 0, 129], 2, heads, kv_heads, 64, 64, BF16))
+    _check_attn(gpu, *_attn_case(heads, [5, 200, 0, 129], 300, heads, kv_heads, 64, 64, BF16))       # a wide block table: two blocks of 16 a wave
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dk,dv", WIDTHS)
+@pytest.mark.parametrize("heads,kv_heads,layout", [(8, 4, "cells"), (24, 8, "heads"), (64, 4, "cells")])
+def test_attn_four_heads_a_workgroup(gpu, heads, kv_heads, layout, dk, dv, dtype):
+    """Block tables with room for 8192 pages and more, KV heads in fours: a wave takes a head of its own; runs that end inside a page list,
+    windows that begin and lengths that end inside any quarter of a page."""
+    case = _attn_case(dk + heads, [0, 1, 31, 33, 64, 97, 128, 129, 300, 640], 256, heads, kv_heads, dk, dv, dtype, layout)
+    _check_attn(gpu, *case)
+    _check_attn(gpu, *case, window=70)
+    _check_attn(gpu, *case, window=200, n_workgroups=5, logit_softcap=20.0, mask=_mask(torch.Generator().manual_seed(4), 10, 256 * 128))
+    _check_attn(gpu, *case, out_type=F32, n_workgroups=3, mask=torch.zeros((10, 300), dtype=F16))
 
 
 @pytest.mark.parametrize("n_workgroups", [1, 2, 3, 5, 8, 64, 4096])
