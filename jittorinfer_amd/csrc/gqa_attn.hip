@@ -27,10 +27,10 @@
 
 #include <type_traits>
 
-#include "mla_common.hpp"
-#include "../../include/gqa_attn.h"
+#include "gqa_common.hpp"
 
 using namespace mla;
+using namespace mla::gqa;
 
 namespace {
 
@@ -57,8 +57,6 @@ struct AttnP {
     int64_t  cap;                 // bt_stride * 128
 };
 
-constexpr int PAGE = MLA_PAGE_TOKENS;
-
 // Workgroups a CU holds: a wave's tile of K and V, its Q fragments and its accumulators take up to 256 registers for heads up to 192 wide
 // and one block of 16 query heads, more (two waves a SIMD would spill) beyond.
 constexpr int wg_per_cu(int dk, int nb) { return dk <= 64 || (dk <= 192 && nb == 1) ? 2 : 1; }
@@ -67,16 +65,6 @@ template <bool F16> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f3
     if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(bitcast<f16x8>(a), bitcast<f16x8>(b), c, 0, 0, 0);
     else               return __builtin_amdgcn_mfma_f32_16x16x32_bf16(bitcast<bf16x8>(a), bitcast<bf16x8>(b), c, 0, 0, 0);
 }
-template <bool F16> __device__ __forceinline__ unsigned short to16(float f) {
-    if constexpr (F16) return bitcast<unsigned short>((_Float16) f);
-    else               return bitcast<unsigned short>((__bf16) f);
-}
-template <bool F16> __device__ __forceinline__ unsigned pair16(float a, float b) { return to16<F16>(a) | ((unsigned) to16<F16>(b) << 16); }
-template <bool F16> __device__ __forceinline__ float from16(unsigned short h) {
-    if constexpr (F16) return (float) bitcast<_Float16>(h);
-    else               return __uint_as_float((unsigned) h << 16);
-}
-
 // Values that are the same in every lane, told to the compiler; and lengths and page ids read through the scalar cache (nothing writes them while the
 // kernel runs): a vector load among those of K and V would have the wave wait for all that were issued before it.
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -96,12 +84,6 @@ __device__ __forceinline__ Span span_uni(const AttnP & p, int b) {        // b t
     return Span{ uni(s.first), uni(s.last) };
 }
 __device__ __forceinline__ int pages_of(Span s) { return s.last > s.first ? (s.last + PAGE - 1) / PAGE - s.first / PAGE : 0; }
-
-__device__ __forceinline__ int wave_sum(int v) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
-    return v;
-}
 
 // Run of workgroup v of n when `total` units are dealt: the first total % n take one more.
 struct Deal { int base, more; };
@@ -131,22 +113,18 @@ template <typename Find> __device__ __forceinline__ Place locate(const AttnP & p
             mine += own[e];
         }
     };
-    for (int b0 = 0; b0 < p.n_seq; b0 += 256) { fetch(b0); total += wave_sum(mine); }
-    total = uni(total);
+    for (int b0 = 0; b0 < p.n_seq; b0 += 256) { fetch(b0); total += lane_of(scan_wave(mine), 63); }
     const int u = find(total);
     Place r{ total, 0, 0 };
     if (u < 0) return r;
     for (int b0 = 0, before = 0; b0 < p.n_seq; b0 += 256) {
         if (p.n_seq > 256) fetch(b0);
-        int incl = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(incl, d, 64); if (lane >= d) incl += o; }
-        const int all = __shfl(incl, 63, 64);
+        const int incl = scan_wave(mine), all = lane_of(incl, 63);
         if (u < before + all) {
             const int at = __ffsll(__ballot(u < before + incl)) - 1;      // the first lane whose sequences reach past u
-            int ahead = before + __shfl(incl - mine, at, 64), e = 0;
+            int ahead = before + lane_of(incl - mine, at), e = 0;
             for (; e < 3; e++) {
-                const int n = __shfl(e == 0 ? own[0] : e == 1 ? own[1] : own[2], at, 64);
+                const int n = lane_of(e == 0 ? own[0] : e == 1 ? own[1] : own[2], at);
                 if (u < ahead + n) break;
                 ahead += n;
             }
@@ -765,8 +743,6 @@ __global__ void __launch_bounds__(256) gqa_weights_kernel(const AttnP p, const i
 }
 
 // ---------------------------------------------------------------- host
-
-bool al16(const void * ptr) { return ((uintptr_t) ptr & 15) == 0; }
 
 struct Plan {
     int     nb, rows, row_blocks, head_blocks, n_wg;

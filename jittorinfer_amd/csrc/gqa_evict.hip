@@ -10,14 +10,13 @@
 // flags order reads before writes and carry no data.  Segments are numbered by a ticket as workgroups start, and a workgroup raises its flag
 // before it waits: every flag it waits for belongs to one that is running already, whatever the order of dispatch.
 
-#include "mla_common.hpp"
-#include "../../include/gqa_attn.h"
+#include "gqa_common.hpp"
 
 using namespace mla;
+using namespace mla::gqa;
 
 namespace {
 
-constexpr int PAGE = MLA_PAGE_TOKENS;
 constexpr int SEL_THREADS = 1024, SEL_PER = 8, SEL_RUN = SEL_THREADS * SEL_PER, SEL_RUNS = 4, SEL_CHUNK = SEL_RUN * SEL_RUNS;
 // One workgroup a group, or one a run of 8192 rows in four launches.  Measured, a whole call: 8 groups of 16384 rows 27.6 against 32.4 us, of 32768
 // rows 39.7 against 34.0; 64 groups of 32768 rows 56.3 against 56.4, of 131072 195 against 173; 256 groups of 65536 rows 295 against 348.
@@ -48,12 +47,6 @@ __device__ __forceinline__ unsigned key_of(float x) {
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-__device__ __forceinline__ int scan_wave(int v, int lane) {       // inclusive
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(v, d, 64); if (lane >= d) v += o; }
-    return v;
-}
-
 // The digit at which the rows of a histogram, counted from the largest digit down, reach `left`, and how many of the digit's own rows those are.
 // One wave: lane t sums the 32 bins 2047 - 32 t and down (rotated, so that the lanes meet different banks), a scan finds the lane, another the bin.
 struct Pick { unsigned digit; int left; };
@@ -61,14 +54,14 @@ __device__ __forceinline__ Pick pick(const unsigned * hist, int left, int lane) 
     int sum = 0;
 #pragma unroll
     for (int i = 0; i < 32; i++) sum += (int) hist[BINS - 1 - 32 * lane - ((i + lane) & 31)];
-    const int incl = scan_wave(sum, lane);
+    const int incl = scan_wave(sum);
     const int at   = __ffsll(__ballot(incl - sum < left && incl >= left)) - 1;
-    const int base = __shfl(incl - sum, at, 64);
+    const int base = lane_of(incl - sum, at);
     const int bin  = BINS - 1 - 32 * at - (lane & 31);
     const int mine = lane < 32 ? (int) hist[bin] : 0;
-    const int upto = base + scan_wave(mine, lane);
+    const int upto = base + scan_wave(mine);
     const int win  = __ffsll(__ballot(lane < 32 && upto - mine < left && upto >= left)) - 1;
-    return Pick{ (unsigned) __shfl(bin, win, 64), left - __shfl(upto - mine, win, 64) };
+    return Pick{ (unsigned) lane_of(bin, win), left - lane_of(upto - mine, win) };
 }
 
 // Digits of a key, from the top: 11, 11 and 10 bits.
@@ -144,7 +137,7 @@ __global__ void __launch_bounds__(SEL_THREADS) gqa_select_kernel(const EvictP p)
     __shared__ unsigned hist[2][BINS];
     __shared__ int      part[SEL_RUNS][16];
     __shared__ Pick     sh_pick;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Group g = group_of(p, blockIdx.x);
     if (blockIdx.x % p.n_head_kv == 0 && tid == 0) p.new_lens[blockIdx.x / p.n_head_kv] = min(g.n, p.n_keep);
     for (int i = blockIdx.x * SEL_THREADS + tid; i < p.n_sync; i += gridDim.x * SEL_THREADS) p.sync[i] = 0u;
@@ -196,15 +189,15 @@ __global__ void __launch_bounds__(SEL_THREADS) gqa_select_kernel(const EvictP p)
 #pragma unroll
         for (int r = 0; r < SEL_RUNS; r++) {
             m[r] = base + r * SEL_RUN < g.n ? sort_rows(g, base + r * SEL_RUN + tid * SEL_PER, x[r], got.digit) : 0u;
-            incl[r] = scan_wave(count_both(m[r]), lane);           // (at most 8192 of either in a run)
+            incl[r] = scan_wave(count_both(m[r]));           // (at most 8192 of either in a run)
             if (lane == 63) part[r][wave] = incl[r];
         }
         __syncthreads();                                           // (also: every row of the chunk has been read before one is overwritten)
 #pragma unroll
         for (int r = 0; r < SEL_RUNS; r++) {
             if (base + r * SEL_RUN >= g.n) continue;
-            const int upto = scan_wave(lane < 16 ? part[r][lane] : 0, lane);
-            const int all = __shfl(upto, 15, 64), ahead = wave ? __shfl(upto, wave - 1, 64) : 0;
+            const int upto = scan_wave(lane < 16 ? part[r][lane] : 0);
+            const int all = lane_of(upto, 15), ahead = wave ? lane_of(upto, wave - 1) : 0;
             const int before = ahead + incl[r] - count_both(m[r]);
             place_rows(g, base + r * SEL_RUN + tid * SEL_PER, x[r], m[r], sure + (before & 0xffff), ties + (before >> 16), got.left);
             sure += all & 0xffff; ties += all >> 16;
@@ -227,7 +220,7 @@ __global__ void __launch_bounds__(SEL_THREADS) gqa_rank_kernel(const EvictP p, c
     __shared__ Pick     sh_pick;
     __shared__ unsigned sh_ticket;
     __shared__ unsigned long long sh_before;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int groups = p.n_seq * p.n_head_kv;
     int number = (int) blockIdx.x;
     if constexpr (PASS == 0) {
@@ -295,11 +288,11 @@ __global__ void __launch_bounds__(SEL_THREADS) gqa_rank_kernel(const EvictP p, c
         to[tid] = hist[tid]; to[SEL_THREADS + tid] = hist[SEL_THREADS + tid];
     } else {
         const unsigned m = sort_rows(g, i0, x, got.digit);
-        const int incl = scan_wave(count_both(m), lane);
+        const int incl = scan_wave(count_both(m));
         if (lane == 63) part[wave] = incl;
         __syncthreads();                                           // (every row of the run is in a register: it may be overwritten from here on)
-        const int upto = scan_wave(lane < 16 ? part[lane] : 0, lane);
-        const int all = __shfl(upto, 15, 64), ahead = wave ? __shfl(upto, wave - 1, 64) : 0;
+        const int upto = scan_wave(lane < 16 ? part[lane] : 0);
+        const int all = lane_of(upto, 15), ahead = wave ? lane_of(upto, wave - 1) : 0;
         uint64_t * counts = k.counts + (size_t) group * k.runs;
         if (tid == 0) __hip_atomic_store(counts + run, (uint64_t) 1 << 63 | (uint64_t) (all >> 16) << 31 | (uint64_t) (all & 0xffff), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         for (int r = tid; r < run; r += SEL_THREADS) {             // (sums below 2^31 in each half)

@@ -9,11 +9,11 @@
 
 #include <math.h>
 
-#include "mla_common.hpp"
-#include "../../include/gqa_attn.h"
+#include "gqa_common.hpp"
 #include "../../include/mla_front.h"
 
 using namespace mla;
+using namespace mla::gqa;
 
 namespace {
 
@@ -60,11 +60,6 @@ __device__ __forceinline__ void load_weights(const char * w, int type, int at, f
     if (type == T_F32)      { const Raw8<T_F32> r = load8<T_F32>(w + (int64_t) at * 4); unpack8<T_F32>(r, x); }
     else if (type == T_F16) { const Raw8<T_F16> r = load8<T_F16>(w + (int64_t) at * 2); unpack8<T_F16>(r, x); }
     else                    { const Raw8<T_BF16> r = load8<T_BF16>(w + (int64_t) at * 2); unpack8<T_BF16>(r, x); }
-}
-// Rounded by the hardware's conversions (to nearest even; pack2's integer form of the bf16 rounding is 6 instructions a value, a third of the kernel's).
-template <bool F16> __device__ __forceinline__ unsigned pair16(float a, float b) {
-    if constexpr (F16) return bitcast<unsigned short>((_Float16) a) | ((unsigned) bitcast<unsigned short>((_Float16) b) << 16);
-    else               return bitcast<unsigned short>((__bf16) a) | ((unsigned) bitcast<unsigned short>((__bf16) b) << 16);
 }
 template <bool F16> __device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
     return u32x4{ pair16<F16>(x[0], x[1]), pair16<F16>(x[2], x[3]), pair16<F16>(x[4], x[5]), pair16<F16>(x[6], x[7]) };
@@ -186,7 +181,6 @@ __global__ void __launch_bounds__(256) gqa_norm_rope_kernel(const FrontP p) {
 
 int type_of(int ggml) { return ggml == MLA_TYPE_F32 ? T_F32 : ggml == MLA_TYPE_F16 ? T_F16 : T_BF16; }
 bool known(int ggml) { return ggml == MLA_TYPE_F32 || ggml == MLA_TYPE_F16 || ggml == MLA_TYPE_BF16; }
-bool al16(const void * ptr) { return ((uintptr_t) ptr & 15) == 0; }
 
 template <int SRC, bool KV_F16, int LPR>
 void launch_lanes(const FrontP & p, hipStream_t st) {

@@ -398,13 +398,14 @@ bool table_ok(const at::Tensor & t) { return t.scalar_type() == at::kInt && t.di
 bool rows_ok(const at::Tensor & t, int64_t dim, bool written) {
     if (t.dim() != dim || (t.size(-1) > 1 && t.stride(-1) != 1)) return false;
     if (!written || t.numel() == 0) return true;
-    std::vector<std::pair<int64_t, int64_t>> steps;
-    for (int64_t d = 0; d < dim; d++) if (t.size(d) > 1) steps.emplace_back(t.stride(d), t.size(d));
-    std::sort(steps.begin(), steps.end());
+    std::pair<int64_t, int64_t> steps[4];                     // (dim <= 4)
+    int n = 0;
+    for (int64_t d = 0; d < dim; d++) if (t.size(d) > 1) steps[n++] = { t.stride(d), t.size(d) };
+    std::sort(steps, steps + n);
     int64_t reach = 0;
-    for (const auto & [stride, size] : steps) {
-        if (stride <= reach) return false;
-        reach += stride * (size - 1);
+    for (int i = 0; i < n; i++) {
+        if (steps[i].first <= reach) return false;
+        reach += steps[i].first * (steps[i].second - 1);
     }
     return true;
 }
