@@ -23,6 +23,7 @@
 // KV head) whole writes its result; the others leave (o, m, l) in f32 for the second kernel, which joins them in the order of the rows.
 // With weights the first kernel also leaves every score, 4 bytes a (head, row), and a third one adds exp(s - m) / l over the group.
 
+#include <limits.h>
 #include <math.h>
 
 #include <type_traits>
@@ -99,42 +100,43 @@ template <int DV> struct VGeom {
     static constexpr int COLS   = W * GROUPS;           // MFMAs (columns of a lane)
 };
 
-// The deal, computed by every wave for itself (no barrier, and for up to 256 sequences one load of the lengths): the units there are and the
-// sequence of unit u.  A lane takes 4 consecutive sequences of 256.
-struct Place { int total, seq, before; };    // units in all; the sequence unit `find` lies in, and the units before that sequence
-template <typename Find> __device__ __forceinline__ Place locate(const AttnP & p, int lane, Find find) {
-    int own[4], mine = 0, total = 0;
-    auto fetch = [&](int b0) {
-        mine = 0;
+// The deal, computed by every wave for itself (no barrier, and for up to 256 sequences one load of the lengths): how many pages there are, in all
+// head blocks, and the sequence of unit u, where a unit is `per` pages of a head block (the last of a head block fewer).  A lane takes 4
+// consecutive sequences of 256.
+struct Place { int seq, before; };           // the sequence a unit lies in (-1: past the last), and the units before that sequence
+struct Lengths {
+    int own[4];                              // pages of this lane's sequences
+    __device__ __forceinline__ void fetch(const AttnP & p, int lane, int b0) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int b = b0 + lane * 4 + e;
-            own[e] = b < p.n_seq ? pages_of(span_of(p, b)) * p.head_blocks : 0;
-            mine += own[e];
-        }
-    };
-    for (int b0 = 0; b0 < p.n_seq; b0 += 256) { fetch(b0); total += lane_of(scan_wave(mine), 63); }
-    const int u = find(total);
-    Place r{ total, 0, 0 };
-    if (u < 0) return r;
-    for (int b0 = 0, before = 0; b0 < p.n_seq; b0 += 256) {
-        if (p.n_seq > 256) fetch(b0);
-        const int incl = scan_wave(mine), all = lane_of(incl, 63);
-        if (u < before + all) {
-            const int at = __ffsll(__ballot(u < before + incl)) - 1;      // the first lane whose sequences reach past u
-            int ahead = before + lane_of(incl - mine, at), e = 0;
-            for (; e < 3; e++) {
-                const int n = lane_of(e == 0 ? own[0] : e == 1 ? own[1] : own[2], at);
-                if (u < ahead + n) break;
-                ahead += n;
-            }
-            r.seq = b0 + at * 4 + e; r.before = ahead;
-            return r;
-        }
-        before += all;
+        for (int e = 0; e < 4; e++) { const int b = b0 + lane * 4 + e; own[e] = b < p.n_seq ? pages_of(span_of(p, b)) : 0; }
     }
-    return r;
-}
+    __device__ __forceinline__ int all_pages(const AttnP & p, int lane) {
+        int total = 0;
+        for (int b0 = 0; b0 < p.n_seq; b0 += 256) { fetch(p, lane, b0); total += lane_of(scan_wave(own[0] + own[1] + own[2] + own[3]), 63); }
+        return total * p.head_blocks;
+    }
+    __device__ __forceinline__ Place place(const AttnP & p, int lane, int u, int per) {      // after all_pages
+        for (int b0 = 0, before = 0; b0 < p.n_seq; b0 += 256) {
+            if (p.n_seq > 256) fetch(p, lane, b0);
+            int n[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) n[e] = (per == 1 ? own[e] : (own[e] + per - 1) / per) * p.head_blocks;
+            const int mine = n[0] + n[1] + n[2] + n[3], incl = scan_wave(mine), all = lane_of(incl, 63);
+            if (u < before + all) {
+                const int at = __ffsll(__ballot(u < before + incl)) - 1;      // the first lane whose sequences reach past u
+                int ahead = before + lane_of(incl - mine, at), e = 0;
+                for (; e < 3; e++) {
+                    const int k = lane_of(e == 0 ? n[0] : e == 1 ? n[1] : n[2], at);
+                    if (u < ahead + k) break;
+                    ahead += k;
+                }
+                return Place{ b0 + at * 4 + e, ahead };
+            }
+            before += all;
+        }
+        return Place{ -1, 0 };
+    }
+};
 
 // The mask's four numbers of rows t .. t + 3, in one load where their place allows it; rows outside the span: -inf.
 __device__ __forceinline__ u32x2 mask4(const AttnP & p, int b, int t, Span s) {
@@ -170,16 +172,13 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
     const int wg = blockIdx.x;
 
     // ---- which units are this workgroup's
-    int   u = 0, u_end = 0;
-    Deal  deal{ 0, 0 };
-    const Place at = locate(p, lane, [&](int total) {
-        deal = Deal{ total / p.n_wg, total % p.n_wg };
-        u = run_start(deal, wg); u_end = run_start(deal, wg + 1);
-        return u < u_end ? u : -1;
-    });
-    u = uni(u); u_end = uni(u_end);
+    Lengths    lens;
+    const int  total = lens.all_pages(p, lane);
+    const Deal deal{ uni(total / p.n_wg), uni(total % p.n_wg) };
+    int        u = uni(run_start(deal, wg));
+    const int  u_end = uni(run_start(deal, wg + 1));
     if (u >= u_end) return;
-    deal = Deal{ uni(deal.base), uni(deal.more) };
+    const Place at = lens.place(p, lane, u, 1);
     int  b = uni(at.seq);
     Span s = span_uni(p, b);
     int  np = uni(pages_of(s));
@@ -497,27 +496,22 @@ __global__ void __launch_bounds__(64 * LWAVES) gqa_scores_kernel(const AttnP p) 
     __shared__ float2 sh_ml[LWAVES][LROWS];
     const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), quarter = wave & 3, l15 = lane & 15, lg = lane >> 4;
     const int wg = blockIdx.x;
-    int   u = 0, u_end = 0;
-    Deal  deal{ 0, 0 };
-    const Place at = locate(p, lane, [&](int total) {
-        deal = Deal{ total / p.n_wg, total % p.n_wg };
-        u = run_start(deal, wg); u_end = run_start(deal, wg + 1);
-        return u < u_end ? u : -1;
-    });
-    u = uni(u); u_end = uni(u_end);
-    if (u >= u_end) return;
-    deal = Deal{ uni(deal.base), uni(deal.more) };
-    int  b = uni(at.seq);
-    Span s = span_uni(p, b);
-    int  np = uni(pages_of(s));
-    int  hb = uni((u - uni(at.before)) / np), pg = u - uni(at.before) - hb * np;
-
-    for (bool fresh = true; u < u_end; fresh = false) {
-        b = uni(b); hb = uni(hb); pg = uni(pg); np = uni(np); s = Span{ uni(s.first), uni(s.last) };
-        const int  n = uni(min(np - pg, u_end - u));
-        const bool begins = pg == 0, whole = begins && n == np;
+    // A workgroup's Q is 147 KB to stage, so no run crosses from one (sequence, head block) to another: units of `per` pages, as many as there
+    // are workgroups at most; with as many head blocks as workgroups, whole ones in turn.
+    Lengths   lens;
+    const int total = lens.all_pages(p, lane), spare = p.n_wg - p.n_seq * p.head_blocks;
+    const int per = spare > 0 ? max(1, uni((total + spare - 1) / spare)) : INT_MAX / 2;
+    for (int u = wg;; u += p.n_wg) {
+        const Place at = lens.place(p, lane, u, per);
+        const int b = uni(at.seq);
+        if (b < 0) return;
+        const Span s = span_uni(p, b);
+        const int np = uni(pages_of(s)), units = uni((np + per - 1) / per);
+        const int hb = uni((u - uni(at.before)) / units), pg = (u - uni(at.before) - hb * units) * per;
+        const int n = uni(min(np - pg, per));
+        const bool whole = n == np;
         const int  head0 = hb * LROWS, heads = min(LROWS, p.group - head0);
-        if (begins && threadIdx.x == 0) p.items[(int64_t) b * p.head_blocks + hb] = make_int2(2 * wg + (fresh ? 0 : 1), owner_of(deal, u + np - 1));
+        if (pg == 0 && threadIdx.x == 0) p.items[(int64_t) b * p.head_blocks + hb] = make_int2(2 * u, u + units - 1);    // (units of one: u < n_wg)
         const int bt0 = b * (int) p.bt_stride + s.first / PAGE + pg, t_page0 = (s.first / PAGE + pg) * PAGE;
         auto id_at = [&](int i) { return scalar_at(p.block_table, bt0 + min(i, n - 1)); };
         auto good = [&](int id) { return id >= 0 && id < p.n_pages; };
@@ -532,36 +526,36 @@ __global__ void __launch_bounds__(64 * LWAVES) gqa_scores_kernel(const AttnP p) 
                 for (int c = 0; c < KC; c++) kf[blk][c] = *(const u32x4 *) (base + row + c * 64);
             }
         };
-        int i = wave >> 2;                                     // waves 0 .. 3 the even pages of the run, 4 .. 7 the odd ones
+        int i = wave >> 2;                                     // waves 0 .. 3 the even pages of the unit, 4 .. 7 the odd ones
         int id = id_at(i);
-        if (i < n) load_k(i, good(id) ? id : 0);
 
-        // ---- Q to LDS: several pieces a thread under way at once (one by one, they were most of this kernel's time); rows past the group: zeros
-        constexpr int PIECES = LROWS * (LK / 8), BATCH = 6;
-        static_assert(PIECES % (64 * LWAVES * BATCH) == 0, "whole batches");
-        for (int i0 = threadIdx.x; i0 < PIECES; i0 += 64 * LWAVES * BATCH) {
-            u32x4 v[BATCH], w[BATCH];
-            auto src = [&](int k) {
-                const int f = i0 + k * 64 * LWAVES, row = f / (LK / 8);
-                return p.q + (int64_t) b * p.q_nb2 + (int64_t) (head0 + min(row, heads - 1)) * p.q_nb1 + (f - row * (LK / 8)) * (p.q_f32 ? 32 : 16);
-            };
+        // ---- Q to LDS, six pieces a thread under way at a time, the first tile of K behind the last six; rows past the group: zeros
+        constexpr int PIECES = LROWS * (LK / 8) / (64 * LWAVES);
+        static_assert(PIECES * 64 * LWAVES == LROWS * (LK / 8) && PIECES % 6 == 0, "whole pieces");
+        auto stage = [&](int k0, auto behind) {
+            u32x4 v[6], w[6];
+            auto row_of = [&](int k) { return (int) (threadIdx.x + (k0 + k) * 64 * LWAVES) / (LK / 8); };
+            auto col_of = [&](int k) { return (int) (threadIdx.x + (k0 + k) * 64 * LWAVES) % (LK / 8); };
+            auto src = [&](int k) { return p.q + (int64_t) b * p.q_nb2 + (int64_t) (head0 + min(row_of(k), heads - 1)) * p.q_nb1 + col_of(k) * (p.q_f32 ? 32 : 16); };
 #pragma unroll
-            for (int k = 0; k < BATCH; k++) v[k] = *(const u32x4 *) src(k);
+            for (int k = 0; k < 6; k++) v[k] = *(const u32x4 *) src(k);
             if (p.q_f32) {
 #pragma unroll
-                for (int k = 0; k < BATCH; k++) w[k] = *(const u32x4 *) (src(k) + 16);
+                for (int k = 0; k < 6; k++) w[k] = *(const u32x4 *) (src(k) + 16);
 #pragma unroll
-                for (int k = 0; k < BATCH; k++) {
+                for (int k = 0; k < 6; k++) {
                     const f32x4 x = bitcast<f32x4>(v[k]), y = bitcast<f32x4>(w[k]);
                     v[k] = u32x4{ pair16<F16>(x.x, x.y), pair16<F16>(x.z, x.w), pair16<F16>(y.x, y.y), pair16<F16>(y.z, y.w) };
                 }
             }
+            behind();
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int k = 0; k < BATCH; k++) {
-                const int f = i0 + k * 64 * LWAVES, row = f / (LK / 8);
-                *(u32x4 *) (lds + row * LPITCH + (f - row * (LK / 8)) * 16) = row < heads ? v[k] : u32x4{ 0u, 0u, 0u, 0u };
-            }
-        }
+            for (int k = 0; k < 6; k++) *(u32x4 *) (lds + row_of(k) * LPITCH + col_of(k) * 16) = row_of(k) < heads ? v[k] : u32x4{ 0u, 0u, 0u, 0u };
+        };
+#pragma unroll 1
+        for (int k0 = 0; k0 < PIECES - 6; k0 += 6) stage(k0, [] {});
+        stage(PIECES - 6, [&] { load_k(min(i, n - 1), good(id) ? id : 0); });     // (a wave without a page of its own: the last one's, unused)
         // (a wave's own rows of sh_ml hold its running maxima and sums: LDS operations of a wave stay in order)
         for (int r = lane; r < LROWS; r += 64) sh_ml[wave][r] = make_float2(-INFINITY, 0.f);
         __syncthreads();
@@ -617,7 +611,7 @@ __global__ void __launch_bounds__(64 * LWAVES) gqa_scores_kernel(const AttnP p) 
             if (i + LWAVES / 4 < n) load_k(i + LWAVES / 4, good(id) ? id : 0);
         }
         __syncthreads();
-        const int64_t piece = 2 * (int64_t) wg + (fresh ? 0 : 1);
+        const int64_t piece = 2 * (int64_t) u;
         for (int r = threadIdx.x; r < heads; r += 64 * LWAVES) {
             float M = -INFINITY, L = 0.f;
 #pragma unroll
@@ -627,12 +621,7 @@ __global__ void __launch_bounds__(64 * LWAVES) gqa_scores_kernel(const AttnP p) 
             if (!whole) p.part_ml[piece * p.rows + r] = make_float2(M, L);
             else        p.lse[(int64_t) b * p.n_head + head0 + r] = make_float2(M == -INFINITY ? 0.f : M, L == 0.f ? 0.f : 1.f / L);
         }
-        __syncthreads();                                       // LDS is free again for the next piece
-        u += n; pg = 0;
-        if (++hb == p.head_blocks && u < u_end) {
-            hb = 0;
-            do { b++; s = span_uni(p, b); np = uni(pages_of(s)); } while (np == 0);
-        }
+        __syncthreads();                                       // LDS is free again for the next unit
     }
 }
 
@@ -771,7 +760,7 @@ Plan make_plan(const gqa_attn_args * a) {
     pl.row_blocks = pl.quad ? 1 : (group + pl.rows - 1) / pl.rows;
     pl.head_blocks = pl.quad ? a->n_head_kv / 4 : a->n_head_kv * pl.row_blocks;
     pl.items = (int64_t) a->n_seq * pl.head_blocks;
-    const int64_t units = pl.items * a->bt_stride;
+    const int64_t units = pl.items * a->bt_stride + (a->dv ? 0 : pl.items);       // (the scores' deal keeps a workgroup an item aside for what is left over)
     const int fill = 256 * (a->dv ? wg_per_cu(a->dk, pl.nb) : 1);
     pl.n_wg = (int) (units < fill ? units : fill);
     if (a->n_workgroups > 0) pl.n_wg = (int) (units < a->n_workgroups ? units : a->n_workgroups);
