@@ -26,6 +26,7 @@
 #include <limits.h>
 #include <math.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "gqa_common.hpp"
@@ -778,23 +779,32 @@ Plan make_plan(const gqa_attn_args * a) {
     return pl;
 }
 
-template <typename K> hipError_t launch_lds(K kernel, const AttnP & p, int threads, int lds, hipStream_t st) {
-    if (lds > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute((const void *) kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+// LDS over the 64 KB a kernel gets unasked: granted once a device, whatever it asks for later.
+template <typename K> hipError_t launch_lds(K kernel, const AttnP & p, int threads, int lds, std::atomic<uint64_t> & granted, hipStream_t st) {
+    if (lds >= 60 * 1024) {                                   // (the kernels' own shared arrays come on top)
+        int dev = 0;
+        hipError_t e = hipGetDevice(&dev);
         if (e != hipSuccess) return e;
+        const uint64_t bit = dev < 64 ? (uint64_t) 1 << dev : 0;
+        if (!(granted.load(std::memory_order_relaxed) & bit)) {
+            if ((e = hipFuncSetAttribute((const void *) kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds)) != hipSuccess) return e;
+            granted.fetch_or(bit, std::memory_order_relaxed);
+        }
     }
     hipLaunchKernelGGL(kernel, dim3((unsigned) p.n_wg), dim3((unsigned) threads), lds, st, p);
     return hipGetLastError();
 }
 template <bool F16, int DK, int DV, int NB, bool BIAS>
 hipError_t launch_main(const AttnP & p, hipStream_t st) {
-    if constexpr (NB == 1 && DK < 256) if (p.quad) return launch_lds(gqa_attn_kernel<F16, DK, DV, NB, BIAS, true>, p, 256, 0, st);
-    return launch_lds(gqa_attn_kernel<F16, DK, DV, NB, BIAS, false>, p, 256, 4 * 16 * DV * 4, st);
+    static std::atomic<uint64_t> granted{ 0 };
+    if constexpr (NB == 1 && DK < 256) if (p.quad) return launch_lds(gqa_attn_kernel<F16, DK, DV, NB, BIAS, true>, p, 256, 0, granted, st);
+    return launch_lds(gqa_attn_kernel<F16, DK, DV, NB, BIAS, false>, p, 256, 4 * 16 * DV * 4, granted, st);
 }
 template <bool F16, bool BIAS>
 hipError_t launch_scores(const AttnP & p, hipStream_t st) {
     static_assert(LROWS * LPITCH + LWAVES * LROWS * 8 <= 160 * 1024, "LDS");
-    return launch_lds(gqa_scores_kernel<F16, BIAS>, p, 64 * LWAVES, LROWS * LPITCH, st);
+    static std::atomic<uint64_t> granted{ 0 };
+    return launch_lds(gqa_scores_kernel<F16, BIAS>, p, 64 * LWAVES, LROWS * LPITCH, granted, st);
 }
 
 template <bool F16, int NB, bool BIAS>
@@ -846,9 +856,9 @@ extern "C" int gqa_attn_check(const gqa_attn_args * a) {
     if (a->n_seq == 0) return 0;
     if (!a->q || !a->block_table || !a->seq_lens) return MLA_ERR_NULL;
     if (a->n_pages < 1 || a->bt_stride < 1) return MLA_ERR_BAD_SHAPE;
-    // rows, units of work and workgroups are counted in 31 bits
+    // rows are counted in 30 bits, units of work and workgroups in 31
     const int64_t lim = (int64_t) 1 << 31;
-    if (a->bt_stride * PAGE >= lim || (int64_t) a->n_seq * a->n_head >= (1 << 24) || (int64_t) a->n_seq * a->n_head_kv > 65535 || (int64_t) a->n_seq * a->n_head * a->bt_stride >= lim)
+    if (a->bt_stride >= lim / 2 / PAGE || (int64_t) a->n_seq * a->n_head >= (1 << 24) || (int64_t) a->n_seq * a->n_head_kv > 65535 || (int64_t) a->n_seq * a->n_head * a->bt_stride >= lim)
         return MLA_ERR_BAD_SHAPE;
     int rc = check_pool(a->k);
     if (rc) return rc;

@@ -425,7 +425,7 @@ extern "C" int gqa_evict_check(const gqa_evict_args * a) {
     if (a->n_seq < 0 || a->n_head_kv < 1 || a->n_keep < 1 || a->n_sink < 0 || a->n_recent < 0 || (int64_t) a->n_sink + a->n_recent > a->n_keep) return MLA_ERR_BAD_SHAPE;
     if (a->n_seq == 0) return 0;
     if (!a->weights || !a->weights_dst || !a->kept || !a->new_lens || !a->block_table || !a->seq_lens) return MLA_ERR_NULL;
-    if (a->n_pages < 1 || a->bt_stride < 1 || a->bt_stride * PAGE >= ((int64_t) 1 << 30) || (int64_t) a->n_seq * a->n_head_kv > 65535) return MLA_ERR_BAD_SHAPE;
+    if (a->n_pages < 1 || a->bt_stride < 1 || a->bt_stride >= ((int64_t) 1 << 30) / PAGE || (int64_t) a->n_seq * a->n_head_kv > 65535) return MLA_ERR_BAD_SHAPE;
     int rc = check_pool(a->k, a->k_row_bytes);
     if (!rc && a->v.data) rc = check_pool(a->v, a->v_row_bytes);
     if (rc) return rc;

@@ -9,6 +9,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <mutex>
 #include <vector>
 
 #include <ATen/ops/empty.h>
@@ -33,6 +34,14 @@ struct Unlocked {
 };
 template <typename F> int unlocked(F f) {
     const Unlocked u;
+    return f();
+}
+// The same for a launch of several kernels that hand each other scratch: two threads on one stream share it, and the kernels of one call must
+// not be queued between those of another.  One lock per scratch area, by its address.
+template <typename F> int unlocked(const void * scratch, F f) {
+    static std::mutex locks[64];
+    const Unlocked u;
+    const std::lock_guard<std::mutex> l(locks[((uintptr_t) scratch >> 9) % 64]);
     return f();
 }
 
@@ -176,7 +185,7 @@ PyObject * attn(PyObject *, PyObject * const * v, Py_ssize_t n) {
     if (!stream_of(v[14], q, st)) return nullptr;
     THPObjectPtr ws = workspace(v[0], st, lib.workspace_size(&a), a);
     if (!ws) return nullptr;
-    const int rc = unlocked([&] { return lib.attn(&a, st); });
+    const int rc = unlocked(a.workspace, [&] { return lib.attn(&a, st); });
     if (rc) return failed("mla_attn_launch", rc);
     if (made.defined()) return THPVariable_Wrap(made);
     Py_INCREF(v[10]);
@@ -566,7 +575,7 @@ PyObject * gqa_attn(PyObject *, PyObject * const * o, Py_ssize_t n) {
     const size_t need = lib.gqa_workspace_size(&a);
     GqaScratch scratch;
     if (!scratch.take(o[0], q, st, need, a)) return nullptr;
-    const int rc = unlocked([&] { return lib.gqa_attn(&a, st); });
+    const int rc = unlocked(a.workspace, [&] { return lib.gqa_attn(&a, st); });
     if (rc) return failed("gqa_attn_launch", rc);
     return made.defined() ? THPVariable_Wrap(made) : Py_NewRef(vc ? o[10] : o[9]);
 }
@@ -611,7 +620,7 @@ PyObject * gqa_evict(PyObject *, PyObject * const * o, Py_ssize_t n) {
     a.kept = (int32_t *) kept.data_ptr(); a.new_lens = (int32_t *) fresh.data_ptr();
     GqaScratch scratch;
     if (!scratch.take(o[0], q, st, lib.evict_workspace_size(&a), a)) return nullptr;
-    const int rc = unlocked([&] { return lib.evict(&a, st); });
+    const int rc = unlocked(a.workspace, [&] { return lib.evict(&a, st); });
     if (rc) return failed("gqa_evict_launch", rc);
     THPObjectPtr r0(keptp ? Py_NewRef(o[9]) : THPVariable_Wrap(kept)), r1(newp ? Py_NewRef(o[10]) : THPVariable_Wrap(fresh)), r2(wop ? Py_NewRef(o[8]) : THPVariable_Wrap(wo));
     return r0 && r1 && r2 ? PyTuple_Pack(3, r0.get(), r1.get(), r2.get()) : nullptr;

@@ -299,6 +299,55 @@ def test_attn_graphs(gpu):
             assert torch.equal(eager, out) and torch.equal(want, sums), step
 
 
+@pytest.mark.parametrize("dk,dv,kv_heads", [(256, 256, 2), (576, 0, 1), (64, 64, 4)])
+def test_attn_in_a_graph_widths(gpu, dk, dv, kv_heads):
+    """The kernels that ask for more LDS, and the four-head one, captured before they ever ran, and replayed while lengths change."""
+    import jittorinfer_amd as J
+    q, k, v, bt, lens = _attn_case(dk, [1024] * 2, 8 if dk != 64 else 2200, 8, kv_heads, dk, dv, F16, stale=0.0)
+    d = [t.to(gpu) if t is not None else None for t in (q, k, v, bt, lens)]
+    sums = torch.zeros((2, kv_heads, bt.shape[1] * 128), device=gpu)
+    out = torch.empty((2, 8, dv), dtype=F16, device=gpu) if dv else None
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        J.gqa_attn(*d, scale=0.05, weights=sums, out=out)
+    for step in range(3):
+        n = [1000 - 333 * step, 1 + 500 * step]
+        d[4].copy_(torch.tensor(n, dtype=torch.int32))
+        sums.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        want, off, w, w_off = R.attn(q, k, v, bt, n, 0.05)
+        if dv:
+            _near(out, want, off, F16, str(step))
+        _near(sums, w, w_off, F32, str(step))
+
+
+def test_two_threads_on_one_stream(gpu):
+    """Calls of two threads share their stream's scratch: the kernels of a call stay together."""
+    import threading
+    import jittorinfer_amd as J
+    cases, want = [], []
+    for seed in (60, 61):
+        c = [t.to(gpu) for t in _attn_case(seed, [900, 500, 1024], 8, 8, 2, 128, 128, BF16)]
+        cases.append(c)
+        want.append(J.gqa_attn(*c, scale=0.1))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        outs = [J.gqa_attn(*cases[i], scale=0.1) for _ in range(200)]
+        torch.cuda.synchronize()
+        bad.extend(1 for o in outs if not torch.equal(o, want[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 def test_attn_on_another_stream(gpu):
     import jittorinfer_amd as J
     q, k, v, bt, lens = _attn_case(21, [300, 129], 3, 4, 2, 64, 64, BF16)
