@@ -42,7 +42,7 @@ typedef struct gqa_pool {
  * Angles are taken in 64 bits, so they are exact to f32 at any position; ggml_rope_ext's own f32 recurrence (mla_rope_launch) is off by
  * about pos * 2^-22 radians.  Queries go to q_dst, keys (and values, as they are) to their rows of the cache: token t of sequence
  * seq_ids[t] to row slots[t] (NULL: pos[t]); rows outside the block table, negative ones and bad pages are skipped, as the cache write
- * of include/mla_kv_write.h skips them. */
+ * of include/mla_kv_write.h skips them.  Two tokens of one call that name the same row leave parts of either there. */
 typedef struct gqa_norm_rope_args {
     int32_t n_tok, n_head, n_head_kv;
     int32_t dk, dv;          /* values per key / query head and per value head: multiples of 8, at most 256 */
@@ -67,9 +67,9 @@ typedef struct gqa_norm_rope_args {
     double  freq_base, freq_scale, ext_factor, attn_factor, beta_fast, beta_slow;   /* freq_base > 1 */
     const float *   freq_factors; /* [n_dims / 2] or NULL */
     const int32_t * pos;     /* [n_tok] */
-    void *  q_dst;           /* [n_tok][n_head][dk]; may be q itself when the types agree */
+    void *  q_dst;           /* [n_tok][n_head][dk]; may be q itself with the same type and strides, else apart from it */
     int64_t qd_nb1, qd_nb2;
-    gqa_pool k_cache, v_cache;
+    gqa_pool k_cache, v_cache;   /* apart from each other */
     int64_t  n_pages;
     const int32_t * block_table; /* [n_seq][bt_stride] */
     int64_t         bt_stride;
@@ -87,7 +87,7 @@ int gqa_norm_rope_launch(const gqa_norm_rope_args * args, void * stream);
  * infinities); a row past the mask's end is out too.  A sequence with no row left (length 0, everything masked) gets zeros.  Lengths
  * below 0 count as 0, above the block table's room as that room.
  * weights (optional): weights[b][g][i] += sum over the query heads of KV head g of p_i, in f32 and in one order; rows outside the
- * window or the length keep their values.
+ * window or the length keep their values.  dst and weights lie apart from each other, from themselves and from all that is read.
  * Supported widths (dk, dv): (64, 64), (128, 128), (192, 128), (256, 256), and (576, 0) without `v` and dst: the weights alone over a latent cache. */
 typedef struct gqa_attn_args {
     int32_t n_seq, n_head, n_head_kv; /* n_head a multiple of n_head_kv */
@@ -132,14 +132,14 @@ typedef struct gqa_evict_args {
     int32_t n_keep, n_sink, n_recent;   /* n_sink + n_recent <= n_keep */
     int32_t k_row_bytes, v_row_bytes;   /* bytes of a head's row: multiples of 4 from 8 to 16384 (any cache type, Q8_0 latent rows of 612 among them) */
     int32_t _pad;
-    gqa_pool k, v;                      /* v.data NULL: keys only */
+    gqa_pool k, v;                      /* v.data NULL: keys only; else apart from each other (two halves of one row are) */
     int64_t n_pages;
     const int32_t * block_table;
     int64_t         bt_stride;
     const int32_t * seq_lens;
     const float * weights;              /* f32 [n_seq][n_head_kv][bt_stride * 128] */
     int64_t w_nb1, w_nb2;
-    float * weights_dst;                /* the same shape; may be `weights` itself (with the same strides) */
+    float * weights_dst;                /* the same shape; may be `weights` itself with the same strides, else apart from it */
     int64_t wd_nb1, wd_nb2;
     int32_t * kept;                     /* [n_seq][n_head_kv][n_keep] */
     int32_t * new_lens;                 /* [n_seq]; not seq_lens itself */

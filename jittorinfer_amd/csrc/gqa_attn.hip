@@ -18,10 +18,13 @@
 //     the common tile has no reduction across lanes and no rescaling.
 //   * K of the next tile is requested when this tile's scores are done, V when its products are.
 //
-// Work: the list of all (sequence, KV head, page) units, in that order, is dealt to the workgroups in equal runs, from the lengths on
+// Work: the list of all (sequence, head block, page) units, in that order, is dealt to the workgroups in equal runs, from the lengths on
 // the device (nothing on the host depends on them, so a captured launch stays valid while they change).  A run that covers a (sequence,
-// KV head) whole writes its result; the others leave (o, m, l) in f32 for the second kernel, which joins them in the order of the rows.
-// With weights the first kernel also leaves every score, 4 bytes a (head, row), and a third one adds exp(s - m) / l over the group.
+// head block) whole writes its result; the others leave (o, m, l) in f32 for gqa_join_kernel, which joins them in the order of the rows.
+// With weights the first kernel also leaves every score, 4 bytes a (head, row), and gqa_weights_kernel adds exp(s - m) / l over the group.
+//
+// Measured, 32 query heads on 8 of 128, bf16, a whole call: 32 x 8192 rows 191 us = 5.6 TB/s (head by head 186 = 5.8; a large copy moves 4.9), 64 x 16384
+// 748 us = 5.7 (702 = 6.1), 1 x 1024 rows 11.4 us, latency alone: 6.7 of it this kernel, 4.5 the join.
 
 #include <limits.h>
 #include <math.h>
@@ -488,7 +491,8 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
 // Scores of a latent cache (rows of 576, one KV head) for its weights: (m, l) and every score, as gqa_attn_kernel leaves them, without V.  Up to
 // 128 heads share a row, 128 flop a byte: the rows of Q lie in LDS (147 KB) and are read, 16 heads at a time, against a tile of 32 rows of K
 // in registers, by eight waves, so that every SIMD still has two.  The loop over blocks of heads is a loop: eight copies of its body, run once or
-// twice by a workgroup, cost three times as long to fetch as to run.
+// twice by a workgroup, took twice as long, most of it to fetch them.  8 x 8192 rows, 128 heads: 27 us, of which the rows are 11 at the
+// memory's rate and the products 6; then 4.7 to join and 7.1 to add up.
 constexpr int LK = 576, LPITCH = LK * 2 + 16, LWAVES = 8, LROWS = 128;
 template <bool F16, bool BIAS>
 __global__ void __launch_bounds__(64 * LWAVES) gqa_scores_kernel(const AttnP p) {
@@ -741,12 +745,14 @@ struct Plan {
     size_t  off_ml, off_items, off_scores, off_lse, bytes;    // of the workspace; partial rows first
 };
 
-// Both sides of the rules below, whole calls on one MI355X, bf16.  Two blocks of 16 heads a wave against one: 64 heads on 2, 64 x 16384 rows 196 against
-// 306 us, 32 x 2048 rows (1024 pages) 25 against 31; 32 heads on 1, 32 x 2048 rows (512 pages) 19.3 against 17.9, 1 x 1024 14.7 against 12.6.
-// Four KV heads a workgroup against one, rows row by row: 16 heads of 64, 32 x 8192 rows 185 against 224 us; 32 on 8 of 128, 8 x 16384 rows (8192 pages) 102
-// against 110, 16 x 4096 (4096 pages) 50 against 51; 16 on 4 of 64, 8 x 16384 (4096 pages) 32 against 30, 1 x 8192 14.4 against 13.0.  Heads
-// of 256: 187 against 187.  Head by head the pages are contiguous anyway: 32 on 8 of 128, 32 x 8192 rows 193 against 187.
-constexpr int64_t TWO_BLOCKS = 1024, QUADS = 8192;
+// Both sides of the rules below: whole calls on one MI355X, bf16, pages in brackets (of all KV heads, as many as the block table has room for).
+// Two blocks of 16 heads a wave against one: 64 heads on 2 of 128, 64 x 16384 rows (16384) 198 against 316 us, 32 x 8192 (4096) 54 against 90,
+// 32 x 2048 (1024) 26 against 32; 32 on 1 of 128, 8 x 16384 (1024) 23.3 against 22.6, 32 x 2048 (512) 20.4 against 18.0, 1 x 1024 14.3 against 11.4.
+// Four KV heads a workgroup against one, rows row by row: 16 heads on 16 of 64, 32 x 8192 (32768) 187 against 220, 4 x 4096 (2048) 18.6 against 20.6;
+// 16 on 16 of 192 / 128, 8 x 16384 (16384) 228 against 237; 32 on 8 of 128, 8 x 16384 (8192) 101 against 111, 4 x 4096 (1024) 20.3 against 20.1; 16 on 4
+// of 64, 32 x 8192 (8192) 51 against 52, 1 x 131072 (4096) 33.3 against 29.5.  Head by head a page of a head is contiguous anyway: 32 on 8 of 128,
+// 32 x 8192 194 against 186.  Heads of 256, 512 bytes a row each: 187 against 187.
+constexpr int64_t TWO_BLOCKS = 1024, QUADS_OF_MANY = 2048, QUADS = 8192;
 Plan make_plan(const gqa_attn_args * a) {
     Plan pl;
     const int group = a->n_head / a->n_head_kv;
@@ -756,7 +762,7 @@ Plan make_plan(const gqa_attn_args * a) {
     pl.nb = a->dv == 0 ? LROWS / 16 : group > 16 && a->dk < 256 && pages >= TWO_BLOCKS ? 2 : 1;
     // four KV heads a workgroup where a row's heads lie side by side in both caches
     const bool side = a->k.nb_row >= a->n_head_kv * a->k.nb_head && a->v.nb_row >= a->n_head_kv * a->v.nb_head;
-    pl.quad = a->dv != 0 && a->dk < 256 && group <= 16 && a->n_head_kv % 4 == 0 && side && pages >= QUADS;
+    pl.quad = a->dv != 0 && a->dk < 256 && group <= 16 && a->n_head_kv % 4 == 0 && side && pages >= (a->n_head_kv >= 8 ? QUADS_OF_MANY : QUADS);
     pl.rows = pl.quad ? 4 * group : pl.nb * 16;
     pl.row_blocks = pl.quad ? 1 : (group + pl.rows - 1) / pl.rows;
     pl.head_blocks = pl.quad ? a->n_head_kv / 4 : a->n_head_kv * pl.row_blocks;

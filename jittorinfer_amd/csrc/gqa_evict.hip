@@ -2,13 +2,17 @@
 //
 // Selection (gqa_select_kernel, a workgroup per (sequence, KV head)): the weights' bits, made monotone, are searched digit by digit for the
 // smallest weight that stays (11 + 11 + 10 bits, a histogram in LDS each), then one pass in the order of the rows writes the rows that stay:
-// those above it, and of those equal to it the first ones, counted by a scan.  Reads the weights four times, from HBM once.
+// those above it, and of those equal to it the first ones, counted by a scan.  Bound by its chain of passes and barriers, not by bytes: 12.1 us for 8
+// groups of 8192 rows, 14.3 for 256.  Block tables of more rows take several workgroups a group (gqa_rank_kernel: 26 us for 100000 rows, 93 in one).
 //
 // Moving (gqa_move_kernel): row kept[j] goes to row j <= kept[j], in place, read once and written once.  A workgroup takes a segment of
 // rows of one head of K or of V, loads all its sources into registers, says so in a flag, waits until the rows it is about to overwrite have been
 // read -- their readers are segments in front of it, two at most -- and stores.  Nothing is ever read that was written in this launch, so the
 // flags order reads before writes and carry no data.  Segments are numbered by a ticket as workgroups start, and a workgroup raises its flag
-// before it waits: every flag it waits for belongs to one that is running already, whatever the order of dispatch.
+// before it waits: every flag it waits for belongs to one that is running already, whatever the order of dispatch.  Bound by HBM where there is
+// much to move: 32 sequences of 8 heads cut from up to 8192 rows to 2048, 479 MB read and written in 106 us = 4.5 TB/s (a large copy: 4.9); two latent
+// caches cut from 100000 rows to 40000 41 us; 8192 rows of one sequence to 4096 12.2 us.  (A workgroup a stripe of columns, all rows in
+// order, needed no flags and took 234 us for the second: 36 workgroups cannot keep enough loads under way.)
 
 #include "gqa_common.hpp"
 
@@ -18,8 +22,8 @@ using namespace mla::gqa;
 namespace {
 
 constexpr int SEL_THREADS = 1024, SEL_PER = 8, SEL_RUN = SEL_THREADS * SEL_PER, SEL_RUNS = 4, SEL_CHUNK = SEL_RUN * SEL_RUNS;
-// One workgroup a group, or one a run of 8192 rows in four launches.  Measured, a whole call: 8 groups of 16384 rows 27.6 against 32.4 us, of 32768
-// rows 39.7 against 34.0; 64 groups of 32768 rows 56.3 against 56.4, of 131072 195 against 173; 256 groups of 65536 rows 295 against 348.
+// One workgroup a group, or one a run of 8192 rows in four launches.  Measured, a whole call: 8 groups of 16384 rows 24.9 against 32.3 us, of 32768
+// rows 36.9 against 34.0; 64 groups of 32768 rows 53.4 against 55.5, of 131072 190 against 169; 256 groups of 65536 rows 293 against 344.
 constexpr int SEL_ONE = 3 * SEL_RUN, SEL_GROUPS = 64, SEL_MANY = 8192;       // (SEL_MANY runs at most: 128 MB of histograms)
 constexpr int BINS = 2048;
 
@@ -431,7 +435,9 @@ extern "C" int gqa_evict_check(const gqa_evict_args * a) {
     if (rc) return rc;
     if (((uintptr_t) a->weights & 3) || (a->w_nb1 & 3) || (a->w_nb2 & 3) || ((uintptr_t) a->weights_dst & 3) || (a->wd_nb1 & 3) || (a->wd_nb2 & 3)) return MLA_ERR_BAD_ALIGNMENT;
     if (a->weights == a->weights_dst && (a->w_nb1 != a->wd_nb1 || a->w_nb2 != a->wd_nb2)) return MLA_ERR_BAD_SHAPE;
-    if (a->new_lens == a->seq_lens) return MLA_ERR_UNSUPPORTED;
+    if (a->new_lens == a->seq_lens || a->v.data == a->k.data) return MLA_ERR_UNSUPPORTED;
+    const int64_t apart = (const char *) a->weights_dst - (const char *) a->weights, row = a->bt_stride * PAGE * 4;
+    if (apart && apart > -row && apart < row) return MLA_ERR_UNSUPPORTED;
     const Plan pl = make_plan(a);
     if (pl.k.count > MOVE_SEGMENTS || pl.v.count > MOVE_SEGMENTS || pl.segments >= ((int64_t) 1 << 30)) return MLA_ERR_BAD_SHAPE;
     return 0;

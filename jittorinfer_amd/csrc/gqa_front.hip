@@ -5,7 +5,7 @@
 // bytes a load), 8 to 32 lanes a row; the sum of squares and the partners of a NeoX pair (half the rotated width away) come from
 // other lanes by shuffles, so a row never touches LDS.  The (cos, sin) table of a token is built once by its workgroup: the position times
 // the frequency in turns, in 64 bits, of which only the fraction of a turn is kept -- a far position costs no accuracy -- and the
-// sine and cosine of that in f32.
+// sine and cosine of that in f32.  8111 tokens of 32 + 8 + 8 rows of 128 in bf16: 44 us = 4.5 TB/s (a large copy: 4.9).
 
 #include <math.h>
 
@@ -18,8 +18,8 @@ using namespace mla::gqa;
 namespace {
 
 constexpr int MAX_PAIRS = 128;
-// Below this a token's sets of rows have workgroups of their own (one token of 40 rows: 6.2 -> 4.6 us), from there on one workgroup takes them all
-// and makes the table once.
+// Below this a token's sets of rows have workgroups of their own, from there on one workgroup takes them all and makes the table once.  A whole call,
+// 40 rows of 128: 1 token 6.9 against 8.3 us, 256 tokens 6.4 against 7.6; 2048 tokens 17.2 against 17.4, 8192 tokens 50.8 against 44.3.
 constexpr int FEW_TOKENS = 1024;
 
 enum { T_F32 = 0, T_F16 = 1, T_BF16 = 2 };
@@ -227,7 +227,10 @@ extern "C" int gqa_norm_rope_check(const gqa_norm_rope_args * a) {
     if (!rc) rc = check_rows(a->q_dst, a->qd_nb1, a->qd_nb2);
     if (!rc && a->q_weight) rc = check_rows(a->q_weight, 0, 0);
     if (rc) return rc;
+    const int64_t apart = (const char *) a->q_dst - (const char *) a->q, row = (int64_t) a->dk * (a->src_type == MLA_TYPE_F32 ? 4 : 2), row_dst = (int64_t) a->dk * (a->dst_type == MLA_TYPE_F32 ? 4 : 2);
+    if (apart == 0 ? a->src_type != a->dst_type || a->qd_nb1 != a->q_nb1 || a->qd_nb2 != a->q_nb2 : apart > -row_dst && apart < row) return MLA_ERR_UNSUPPORTED;
     if (a->k) {
+        if (a->v && a->v_cache.data == a->k_cache.data) return a->v_cache.data ? MLA_ERR_UNSUPPORTED : MLA_ERR_NULL;
         if (!a->block_table || !a->seq_ids) return MLA_ERR_NULL;
         if (a->n_pages < 1 || a->bt_stride < 1) return MLA_ERR_BAD_SHAPE;
         if ((rc = check_rows(a->k, a->k_nb1, a->k_nb2)) || (rc = check_pool(a->k_cache))) return rc;

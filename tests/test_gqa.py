@@ -203,6 +203,25 @@ def test_evict_accepts():
     assert lib.gqa_evict_workspace_size(C.byref(_cut(n_keep=0))) == 0
 
 
+@pytest.mark.parametrize("kw", [dict(weights_dst=32768 + 4), dict(weights_dst=32768 - 2044), dict(weights_dst=32768 + 2044), dict(v=_pool(128))], ids=str)
+def test_evict_refuses_what_overlaps(kw):
+    a = _cut(**kw)
+    assert J.library().gqa_evict_check(C.byref(a)) == UNSUPPORTED and J.library().gqa_evict_launch(C.byref(a), None) == UNSUPPORTED
+    for dst in (32768, 32768 + 2048, 32768 - 2048):       # itself; rows between the rows (4 rows of 2048 bytes in 8192)
+        a = _cut(w_nb1=4096, w_nb2=8192, wd_nb1=4096, wd_nb2=8192, weights_dst=dst)
+        assert J.library().gqa_evict_check(C.byref(a)) == 0
+
+
+@pytest.mark.parametrize("kw", [dict(q_dst=4096, qd_nb1=512, qd_nb2=4096), dict(q_dst=4096, dst_type=J.MLA_TYPE_F16), dict(q_dst=4096 + 16), dict(q_dst=4096 - 240), dict(q_dst=4096 - 256, dst_type=J.MLA_TYPE_F32),
+                                dict(v_cache=_pool(128))], ids=str)
+def test_norm_rope_refuses_what_overlaps(kw):
+    a = _rows(**kw)
+    assert J.library().gqa_norm_rope_check(C.byref(a)) == UNSUPPORTED and J.library().gqa_norm_rope_launch(C.byref(a), None) == UNSUPPORTED
+    for dst in (4096, 4096 + 256, 4096 - 256):
+        a = _rows(q_nb1=512, q_nb2=4096, qd_nb1=512, qd_nb2=4096, q_dst=dst)
+        assert J.library().gqa_norm_rope_check(C.byref(a)) == 0
+
+
 def test_exports_and_mirrors_match_the_header(tmp_path):
     """Every function the header declares is exported; every ctypes mirror has the C compiler's size and field offsets."""
     text = open(os.path.join(ROOT, "include", "gqa_attn.h")).read()
