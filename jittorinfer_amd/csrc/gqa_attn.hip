@@ -21,7 +21,7 @@
 // Work: the list of all (sequence, head block, page) units, in that order, is dealt to the workgroups in equal runs, from the lengths on
 // the device (nothing on the host depends on them, so a captured launch stays valid while they change).  A run that covers a (sequence,
 // head block) whole writes its result; the others leave (o, m, l) in f32 for gqa_join_kernel, which joins them in the order of the rows.
-// With weights the first kernel also leaves every score, 4 bytes a (head, row), and gqa_weights_kernel adds exp(s - m) / l over the group.
+// With weights the first kernel also leaves every score, 4 bytes a (head, row), and gqa_join_kernel adds exp(s - m) / l over the group too.
 //
 // Measured, 32 query heads on 8 of 128, bf16, a whole call: 32 x 8192 rows 191 us = 5.6 TB/s (head by head 186 = 5.8; a large copy moves 4.9), 64 x 16384
 // 748 us = 5.7 (702 = 6.1), 1 x 1024 rows 11.4 us, latency alone: 6.7 of it this kernel, 4.5 the join.
@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
 // 128 heads share a row, 128 flop a byte: the rows of Q lie in LDS (147 KB) and are read, 16 heads at a time, against a tile of 32 rows of K
 // in registers, by eight waves, so that every SIMD still has two.  The loop over blocks of heads is a loop: eight copies of its body, run once or
 // twice by a workgroup, took twice as long, most of it to fetch them.  8 x 8192 rows, 128 heads: 27 us, of which the rows are 11 at the
-// memory's rate and the products 6; then 4.7 to join and 7.1 to add up.
+// memory's rate and the products 6; then 11.6 to join and add them up.
 constexpr int LK = 576, LPITCH = LK * 2 + 16, LWAVES = 8, LROWS = 128;
 template <bool F16, bool BIAS>
 __global__ void __launch_bounds__(64 * LWAVES) gqa_scores_kernel(const AttnP p) {
@@ -630,17 +630,15 @@ __global__ void __launch_bounds__(64 * LWAVES) gqa_scores_kernel(const AttnP p) 
     }
 }
 
-// Joins what the runs left of one head (grid: a workgroup per (sequence, head)): o = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M), pieces in
-// the order of the rows, eight under way at a time a thread.  Heads whose rows one run covered are done; heads without a row get zeros.
+// Joins what the runs left of one head: o = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M), pieces in the order of the rows, eight under
+// way at a time a thread.  Heads whose rows one run covered are done; heads without a row get zeros.
 constexpr int JOIN = 256;
 template <bool F16>
-__global__ void __launch_bounds__(JOIN) gqa_join_kernel(const AttnP p) {
+__device__ __forceinline__ void join_head(const AttnP & p, int b, int kvh, int r, f32x4 * sum) {
     __shared__ float  red[2][JOIN / 64], weight[JOIN];
-    __shared__ f32x4  sum[JOIN];
-    const int b = blockIdx.x / p.n_head, h = blockIdx.x - b * p.n_head;
-    const int kvh = h / p.group, r = h - kvh * p.group;
+    const int h = kvh * p.group + r;
     const int hb = p.quad ? kvh >> 2 : kvh * p.row_blocks + r / p.rows, row = p.quad ? (kvh & 3) * p.group + r : r % p.rows;
-    char *    dst = p.dst ? p.dst + (int64_t) b * p.d_nb2 + (int64_t) h * p.d_nb1 : nullptr;
+    char *    dst = p.dst + (int64_t) b * p.d_nb2 + (int64_t) h * p.d_nb1;
     const int cols = p.dv / 4;                                // runs of 4 columns
     auto store = [&](int c, f32x4 o) {
         if (p.dst_f32) *(f32x4 *) (dst + c * 16) = o;
@@ -664,14 +662,14 @@ __global__ void __launch_bounds__(JOIN) gqa_join_kernel(const AttnP p) {
         return v;
     };
     // rows and factors of the first pieces are requested together: after the item's, their addresses depend on nothing
-    const int groups = cols ? JOIN / cols : 1, g = cols ? (int) threadIdx.x / cols : 0, c = (int) threadIdx.x - g * cols;   // (cols: 16, 32 or 64)
+    const int groups = JOIN / cols, g = (int) threadIdx.x / cols, c = (int) threadIdx.x - g * cols;   // (cols: 16, 32 or 64)
     f32x4 x[8];
     auto rows = [&](int k, int end) {                         // pieces k, k + groups, ..; past the end: the last one
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] = *(const f32x4 *) (p.part_o + slot(min(k + e * groups, end - 1)) * p.dv + c * 4);
     };
     const float2 first = (int) threadIdx.x < n ? p.part_ml[slot(threadIdx.x)] : make_float2(-INFINITY, 0.f);
-    if (cols) rows(g, min(JOIN, n));
+    rows(g, min(JOIN, n));
     float M = first.x;
     for (int i = threadIdx.x + JOIN; i < n; i += JOIN) M = fmaxf(M, p.part_ml[slot(i)].x);
     M = over_waves(M, true);
@@ -686,17 +684,14 @@ __global__ void __launch_bounds__(JOIN) gqa_join_kernel(const AttnP p) {
         if (i0) __syncthreads();
         weight[threadIdx.x] = w;
         __syncthreads();
-        if (cols)
-            for (int k = i0 + g; k < end; k += groups * 8) {
-                if (k >= groups) rows(k, end);                // (the first ones are here)
+        for (int k = i0 + g; k < end; k += groups * 8) {
+            if (k >= groups) rows(k, end);                    // (the first ones are here)
 #pragma unroll
-                for (int e = 0; e < 8; e++) if (k + e * groups < end) o += x[e] * weight[k + e * groups - i0];
-            }
+            for (int e = 0; e < 8; e++) if (k + e * groups < end) o += x[e] * weight[k + e * groups - i0];
+        }
     }
     L = over_waves(L, false);
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    if (p.scores && threadIdx.x == 0) p.lse[(int64_t) b * p.n_head + h] = make_float2(M == -INFINITY ? 0.f : M, inv);
-    if (!cols) return;
     sum[threadIdx.x] = o;
     __syncthreads();
     if (g == 0) {
@@ -706,34 +701,105 @@ __global__ void __launch_bounds__(JOIN) gqa_join_kernel(const AttnP p) {
 }
 
 // weights[b][g][i] += sum over the group's heads of exp2(s - m) / l, from the scores the first kernel left.  A thread takes 4 rows and
-// every parts-th head (parts: 16, or the power of two that holds a smaller group); the parts are added in one order.
-__global__ void __launch_bounds__(256) gqa_weights_kernel(const AttnP p, const int parts) {
-    __shared__ f32x4 sum[256];
-    const int  b = blockIdx.y / p.n_head_kv, kvh = blockIdx.y - b * p.n_head_kv;
+// every parts-th head (parts: 16, or the power of two that holds a smaller group); the parts are added in one order.  (m, l) of a head is
+// joined from its pieces by every workgroup for itself, while its first scores are under way, which costs less than a launch in between: 6.5 us with the
+// results of 8 x 4096 rows of 16 heads, where two launches took 10.2.  (2048 workgroups in all, or a quarter of them: 12.7 us either way over 8 x 8192 of 128.)
+constexpr int SUM_HEADS = 256, SUM_BLOCKS = 2048;
+template <int HEADS>                                          // scores under way at a time
+__device__ __forceinline__ void sum_weights(const AttnP & p, int b, int kvh, int block, int blocks, int parts, f32x4 * sum) {
+    __shared__ float2 lse[SUM_HEADS];
     const Span s = span_of(p, b);
-    const int  quads = 256 / parts, part = (int) threadIdx.x / quads, quad = (int) threadIdx.x - part * quads;
-    const int  t = ((int) blockIdx.x * quads + quad) * 4;
-    if ((int) blockIdx.x * quads * 4 >= s.last || ((int) blockIdx.x + 1) * quads * 4 <= s.first) return;
+    const int  quads = JOIN / parts, part = (int) threadIdx.x / quads, quad = (int) threadIdx.x - part * quads, rows = quads * 4;
     const int64_t h0 = (int64_t) b * p.n_head + (int64_t) kvh * p.group;
-    const bool    in = t < s.last && t + 4 > s.first;
-    f32x4 w = { 0.f, 0.f, 0.f, 0.f };
-    if (in)
-        for (int h = part; h < p.group; h += parts) {
-            const float2 ml = p.lse[h0 + h];
-            const f32x4  x  = *(const f32x4 *) (p.scores + (h0 + h) * p.cap + t);
+    auto join = [&](int c, int heads, auto load) {            // heads c .. c + heads - 1 of the group, some lanes of a wave each, and the first scores
+        constexpr int AHEAD = HEADS == 1 ? 2 : 8;             // pieces under way at a time a lane (16 lanes a head or more, or 1)
+        int lanes = 64;
+        while (lanes * heads > JOIN) lanes >>= 1;
+        const int  h = (int) threadIdx.x / lanes, sub = (int) threadIdx.x & (lanes - 1), r = c + min(h, heads - 1);
+        const int  hb = p.quad ? kvh >> 2 : kvh * p.row_blocks + r / p.rows, row = p.quad ? (kvh & 3) * p.group + r : r % p.rows;
+        const int2 it = p.items[(int64_t) b * p.head_blocks + hb];
+        const int  v0 = it.x >> 1, n = it.y - v0 + 1;
+        float2 ml[AHEAD], got = p.lse[h0 + r];                    // (of a head that one run covered; else meaningless)
+        auto pieces = [&](int i0) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) w[j] += fast_exp2(x[j] - ml.x) * ml.y;
+            for (int e = 0; e < AHEAD; e++) {
+                const int i = min(i0 + e * lanes, n - 1);
+                ml[e] = p.part_ml[((int64_t) (i ? 2 * (v0 + i) : it.x)) * p.rows + row];
+            }
+        };
+        pieces(sub);
+        load(c + part);
+        if (n > 1) {
+            float M = -INFINITY, L = 0.f;
+            for (int i0 = sub; i0 < n; i0 += AHEAD * lanes) {
+                if (i0 != sub) pieces(i0);
+                float top = M;
+#pragma unroll
+                for (int e = 0; e < AHEAD; e++) top = fmaxf(top, ml[e].x);
+                L = L == 0.f ? 0.f : L * fast_exp2(M - top);
+#pragma unroll
+                for (int e = 0; e < AHEAD; e++) L += i0 + e * lanes >= n || ml[e].y == 0.f ? 0.f : ml[e].y * fast_exp2(ml[e].x - top);
+                M = top;
+            }
+            for (int d = 1; d < lanes; d <<= 1) {
+                const float m = __shfl_xor(M, d, 64), l = __shfl_xor(L, d, 64), top = fmaxf(M, m);
+                L = (L == 0.f ? 0.f : L * fast_exp2(M - top)) + (l == 0.f ? 0.f : l * fast_exp2(m - top));
+                M = top;
+            }
+            got = make_float2(M == -INFINITY ? 0.f : M, L == 0.f ? 0.f : 1.f / L);
         }
-    if (parts > 1) {
-        sum[threadIdx.x] = w;
+        if (h < heads && sub == 0) lse[h] = got;
         __syncthreads();
-        if (part) return;
-        for (int q = 1; q < parts; q++) w += sum[q * quads + quad];
-    }
-    if (!in) return;
-    float * to = (float *) ((char *) p.weights + (int64_t) b * p.w_nb2 + (int64_t) kvh * p.w_nb1) + t;
+    };
+    bool first = true;
+    for (int rb = s.first / rows + block; rb * rows < s.last; rb += blocks, first = false) {
+        const int  t  = rb * rows + quad * 4;
+        const bool in = t < s.last && t + 4 > s.first;
+        f32x4 w = { 0.f, 0.f, 0.f, 0.f };
+        for (int c = 0; c < p.group; c += SUM_HEADS) {
+            const int end = min(c + SUM_HEADS, p.group);
+            f32x4 x[HEADS];
+            const float * from = p.scores + h0 * p.cap + (in ? t : s.first & ~3);
+            auto load = [&](int h) {                          // heads h, h + parts, ..; past the end: the last one
 #pragma unroll
-    for (int j = 0; j < 4; j++) if (t + j >= s.first && t + j < s.last) to[j] += w[j];
+                for (int e = 0; e < HEADS; e++) x[e] = *(const f32x4 *) (from + (int64_t) min(h + e * parts, end - 1) * p.cap);
+            };
+            if (first || p.group > SUM_HEADS) {
+                if (!first || c) __syncthreads();             // (the heads before these are done with)
+                join(c, end - c, load);
+            } else load(c + part);
+            for (int h = c + part; h < end; h += HEADS * parts) {
+                if (h >= c + parts) load(h);
+#pragma unroll
+                for (int e = 0; e < HEADS; e++) {
+                    if (h + e * parts >= end) break;
+                    const float2 ml = lse[h + e * parts - c];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) w[j] += fast_exp2(x[e][j] - ml.x) * ml.y;
+                }
+            }
+        }
+        if (parts > 1) {
+            if (!first) __syncthreads();
+            sum[threadIdx.x] = w;
+            __syncthreads();
+            if (part == 0) for (int q = 1; q < parts; q++) w += sum[q * quads + quad];
+        }
+        if (part || !in) continue;
+        float * to = (float *) ((char *) p.weights + (int64_t) b * p.w_nb2 + (int64_t) kvh * p.w_nb1) + t;
+#pragma unroll
+        for (int j = 0; j < 4; j++) if (t + j >= s.first && t + j < s.last) to[j] += w[j];
+    }
+}
+
+// What follows the runs, in one launch.  Grid: x = the heads of a group (none without a result), then the workgroups that share a sequence's
+// rows (none without weights); y = a (sequence, KV head).
+template <bool F16, int HEADS>
+__global__ void __launch_bounds__(JOIN) gqa_join_kernel(const AttnP p, const int joins, const int parts) {
+    __shared__ f32x4 sum[JOIN];
+    const int b = blockIdx.y / p.n_head_kv, kvh = blockIdx.y - b * p.n_head_kv;
+    if ((int) blockIdx.x < joins) join_head<F16>(p, b, kvh, (int) blockIdx.x, sum);
+    else if constexpr (HEADS > 0) sum_weights<HEADS>(p, b, kvh, (int) blockIdx.x - joins, (int) gridDim.x - joins, parts, sum);
 }
 
 // ---------------------------------------------------------------- host
@@ -833,12 +899,17 @@ hipError_t launch_all(const AttnP & p, const Plan & pl, int dk, hipStream_t st) 
     else if (pl.nb == 2) e = bias ? launch_widths<F16, 2, true>(p, dk, st) : launch_widths<F16, 2, false>(p, dk, st);
     else                 e = bias ? launch_widths<F16, 1, true>(p, dk, st) : launch_widths<F16, 1, false>(p, dk, st);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((gqa_join_kernel<F16>), dim3((unsigned) (p.n_seq * p.n_head)), dim3(JOIN), 0, st, p);
-    if ((e = hipGetLastError()) != hipSuccess || !p.scores) return e;
+    const int joins = p.dv ? p.group : 0, groups = p.n_seq * p.n_head_kv;
+    if (!p.scores) {
+        hipLaunchKernelGGL((gqa_join_kernel<F16, 0>), dim3((unsigned) joins, (unsigned) groups), dim3(JOIN), 0, st, p, joins, 0);
+        return hipGetLastError();
+    }
     int parts = 1;
     while (parts < 16 && parts < p.group) parts *= 2;
-    const int rows = 1024 / parts;
-    hipLaunchKernelGGL(gqa_weights_kernel, dim3((unsigned) ((p.cap + rows - 1) / rows), (unsigned) (p.n_seq * p.n_head_kv)), dim3(256), 0, st, p, parts);
+    const int64_t blocks = (p.cap * parts + 4 * JOIN - 1) / (4 * JOIN), share = (SUM_BLOCKS + groups - 1) / groups;
+    const dim3 grid((unsigned) (joins + (blocks < share ? blocks : share)), (unsigned) groups);
+    if (p.group <= parts) hipLaunchKernelGGL((gqa_join_kernel<F16, 1>), grid, dim3(JOIN), 0, st, p, joins, parts);
+    else                  hipLaunchKernelGGL((gqa_join_kernel<F16, 8>), grid, dim3(JOIN), 0, st, p, joins, parts);
     return hipGetLastError();
 }
 

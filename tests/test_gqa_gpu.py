@@ -212,6 +212,19 @@ def test_weights_over_a_latent_cache(gpu, dtype, heads):
     _check_attn(gpu, q, k, None, bt, lens, mask=mask)
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(window=1500), dict(window=2100, n_workgroups=40), dict(n_workgroups=7)], ids=str)
+def test_weights_of_many_rows(gpu, kw):
+    """More rows than the workgroups that add them up take at once; few and many pieces to a head."""
+    _check_attn(gpu, *_attn_case(30, [2500, 2177, 1, 0, 129, 2400, 300, 2499], 20, 72, 8, 64, 64, BF16), **kw)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(n_workgroups=5)], ids=str)
+def test_weights_of_groups_past_256_heads(gpu, kw):
+    _check_attn(gpu, *_attn_case(31, [5, 300, 0, 129], 3, 600, 2, 64, 64, F16), **kw)
+    _check_attn(gpu, *_attn_case(32, [200, 0, 385], 4, 300, 1, 576, 0, BF16), **kw)
+    _check_attn(gpu, *_attn_case(33, [1400, 0, 1345] + [0, 1] * 49, 11, 300, 1, 64, 64, BF16), **kw)
+
+
 def test_attn_scores_far_apart(gpu):
     """Scores that grow by hundreds along a sequence, and fall: the running maximum moves, and leaves nothing of what came before."""
     q, k, v, bt, lens = _attn_case(16, [512, 512], 4, 4, 2, 64, 64, F16)
