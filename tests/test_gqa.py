@@ -23,6 +23,11 @@ def _pool(width, heads=2, es=2, base=1 << 20):
     return J.GqaPool(base, 128 * heads * width * es, heads * width * es, width * es)
 
 
+def _name(x):
+    """A test's name: the same in every process, whatever addresses its objects have."""
+    return " ".join("%s=%s" % (n, v) if isinstance(v, int) else n for n, v in x.items()) if isinstance(x, dict) else str(x)
+
+
 def _attn(**kw):
     """A call that is accepted, on made-up addresses (never dereferenced), with some fields replaced."""
     a = J.GqaAttnArgs()
@@ -92,7 +97,7 @@ def test_attn_accepts_and_wants_scratch():
         assert lib.gqa_attn_check(C.byref(a)) == 0
 
 
-@pytest.mark.parametrize("kw,code", [(dict(weights=None), NULL), (dict(dst=32768), UNSUPPORTED), (dict(v=_pool(512, 1)), UNSUPPORTED)], ids=str)
+@pytest.mark.parametrize("kw,code", [(dict(weights=None), NULL), (dict(dst=32768), UNSUPPORTED), (dict(v=_pool(512, 1)), UNSUPPORTED)], ids=_name)
 def test_latent_weights_refuse(kw, code):
     a = _latent()
     assert J.library().gqa_attn_check(C.byref(a)) == 0
@@ -203,7 +208,7 @@ def test_evict_accepts():
     assert lib.gqa_evict_workspace_size(C.byref(_cut(n_keep=0))) == 0
 
 
-@pytest.mark.parametrize("kw", [dict(weights_dst=32768 + 4), dict(weights_dst=32768 - 2044), dict(weights_dst=32768 + 2044), dict(v=_pool(128))], ids=str)
+@pytest.mark.parametrize("kw", [dict(weights_dst=32768 + 4), dict(weights_dst=32768 - 2044), dict(weights_dst=32768 + 2044), dict(v=_pool(128))], ids=_name)
 def test_evict_refuses_what_overlaps(kw):
     a = _cut(**kw)
     assert J.library().gqa_evict_check(C.byref(a)) == UNSUPPORTED and J.library().gqa_evict_launch(C.byref(a), None) == UNSUPPORTED
@@ -213,7 +218,7 @@ def test_evict_refuses_what_overlaps(kw):
 
 
 @pytest.mark.parametrize("kw", [dict(q_dst=4096, qd_nb1=512, qd_nb2=4096), dict(q_dst=4096, dst_type=J.MLA_TYPE_F16), dict(q_dst=4096 + 16), dict(q_dst=4096 - 240), dict(q_dst=4096 - 256, dst_type=J.MLA_TYPE_F32),
-                                dict(v_cache=_pool(128))], ids=str)
+                                dict(v_cache=_pool(128))], ids=_name)
 def test_norm_rope_refuses_what_overlaps(kw):
     a = _rows(**kw)
     assert J.library().gqa_norm_rope_check(C.byref(a)) == UNSUPPORTED and J.library().gqa_norm_rope_launch(C.byref(a), None) == UNSUPPORTED
