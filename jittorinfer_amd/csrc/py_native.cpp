@@ -391,6 +391,13 @@ PyObject * front_batch(PyObject *, PyObject * const * v, Py_ssize_t n) {
 
 // ---- the cache of ordinary heads (include/gqa_attn.h)
 
+bool int_of(PyObject * o, int32_t & v) {                      // (a number past 32 bits is an error, not its low half)
+    const long x = PyLong_AsLong(o);
+    v = (int32_t) x;
+    if (!PyErr_Occurred() && x != v) PyErr_SetString(PyExc_OverflowError, "an integer argument does not fit 32 bits");
+    return !PyErr_Occurred();
+}
+constexpr int64_t INTS = (int64_t) 1 << 31;                   // sizes below
 int mla_type(const at::Tensor & t) {
     switch (t.scalar_type()) {
         case at::kFloat:    return MLA_TYPE_F32;
@@ -467,11 +474,11 @@ PyObject * gqa_norm_rope(PyObject *, PyObject * const * o, Py_ssize_t n) {
     gqa_norm_rope_args a;
     memset(&a, 0, sizeof a);
     a.eps = (float) PyFloat_AsDouble(o[6]);
-    a.n_dims = (int32_t) PyLong_AsLong(o[7]); a.mode = (int32_t) PyLong_AsLong(o[8]); a.n_ctx_orig = (int32_t) PyLong_AsLong(o[9]);
+    if (PyErr_Occurred() || !int_of(o[7], a.n_dims) || !int_of(o[8], a.mode) || !int_of(o[9], a.n_ctx_orig)) return nullptr;
     a.freq_base = PyFloat_AsDouble(o[10]); a.freq_scale = PyFloat_AsDouble(o[11]); a.ext_factor = PyFloat_AsDouble(o[12]);
     a.attn_factor = PyFloat_AsDouble(o[13]); a.beta_fast = PyFloat_AsDouble(o[14]); a.beta_slow = PyFloat_AsDouble(o[15]);
     if (PyErr_Occurred()) return nullptr;
-    REQUIRE(mla_type(q) >= 0 && rows_ok(q, 3, false));
+    REQUIRE(mla_type(q) >= 0 && rows_ok(q, 3, false) && q.size(0) < INTS && q.size(1) < INTS && q.size(2) < INTS);
     const int64_t n_tok = q.size(0), es = (int64_t) q.element_size();
     a.n_tok = (int32_t) n_tok; a.n_head = (int32_t) q.size(1); a.dk = (int32_t) q.size(2);
     a.src_type = a.w_type = mla_type(q);
@@ -492,8 +499,8 @@ PyObject * gqa_norm_rope(PyObject *, PyObject * const * o, Py_ssize_t n) {
         REQUIRE(kc && table && ids && (v != nullptr) == (vc != nullptr));
         REQUIRE(k->scalar_type() == q.scalar_type() && rows_ok(*k, 3, false) && k->size(0) == n_tok && k->size(2) == a.dk);
         a.kv_type = mla_type(*kc);
-        REQUIRE(a.kv_type > 0 && cache_ok(*kc, a.kv_type) && kc->size(2) == k->size(1) && kc->size(3) == a.dk);
-        REQUIRE(table_ok(*table) && ints(*ids, n_tok) && (!slots || ints(*slots, n_tok)));
+        REQUIRE(a.kv_type > 0 && cache_ok(*kc, a.kv_type) && kc->size(2) == k->size(1) && kc->size(2) < INTS && kc->size(3) == a.dk);
+        REQUIRE(table_ok(*table) && table->size(0) < INTS && ints(*ids, n_tok) && (!slots || ints(*slots, n_tok)));
         a.n_head_kv = (int32_t) k->size(1); a.n_seq = (int32_t) table->size(0); a.n_pages = kc->size(0);
         a.k = k->data_ptr(); a.k_nb1 = k->stride(1) * es; a.k_nb2 = k->stride(0) * es;
         a.k_cache = pool_of(*kc);
@@ -501,7 +508,7 @@ PyObject * gqa_norm_rope(PyObject *, PyObject * const * o, Py_ssize_t n) {
         a.seq_ids = (const int32_t *) ids->data_ptr(); a.slots = slots ? (const int32_t *) slots->data_ptr() : nullptr;
         if (v) {
             REQUIRE(v->scalar_type() == q.scalar_type() && rows_ok(*v, 3, false) && v->size(0) == n_tok && v->size(1) == a.n_head_kv);
-            REQUIRE(cache_ok(*vc, a.kv_type) && vc->size(0) == a.n_pages && vc->size(2) == a.n_head_kv && vc->size(3) == v->size(2));
+            REQUIRE(cache_ok(*vc, a.kv_type) && vc->size(0) == a.n_pages && vc->size(2) == a.n_head_kv && vc->size(3) == v->size(2) && v->size(2) < INTS);
             a.dv = (int32_t) v->size(2);
             a.v = v->data_ptr(); a.v_nb1 = v->stride(1) * es; a.v_nb2 = v->stride(0) * es;
             a.v_cache = pool_of(*vc);
@@ -534,19 +541,18 @@ PyObject * gqa_attn(PyObject *, PyObject * const * o, Py_ssize_t n) {
     memset(&a, 0, sizeof a);
     a.scale = (float) PyFloat_AsDouble(o[5]); a.logit_softcap = (float) PyFloat_AsDouble(o[6]);
     const int64_t window = PyLong_AsLongLong(o[7]);
-    a.n_workgroups = (int32_t) PyLong_AsLong(o[11]);
-    if (PyErr_Occurred()) return nullptr;
-    REQUIRE(window >= 0 && window < ((int64_t) 1 << 31));
+    if (PyErr_Occurred() || !int_of(o[11], a.n_workgroups)) return nullptr;
+    REQUIRE(window >= 0 && window < INTS);
     a.window = (int32_t) window;
-    REQUIRE(mla_type(q) >= 0 && rows_ok(q, 3, false));
+    REQUIRE(mla_type(q) >= 0 && rows_ok(q, 3, false) && q.size(0) < INTS && q.size(1) < INTS && q.size(2) < INTS);
     const int64_t n_seq = q.size(0), n_head = q.size(1), es = (int64_t) q.element_size();
     a.n_seq = (int32_t) n_seq; a.n_head = (int32_t) n_head; a.dk = (int32_t) q.size(2);
     a.q_type = mla_type(q); a.q = q.data_ptr(); a.q_nb1 = q.stride(1) * es; a.q_nb2 = q.stride(0) * es;
     a.kv_type = mla_type(*kc);
-    REQUIRE(a.kv_type > 0 && cache_ok(*kc, a.kv_type) && kc->size(3) == a.dk);
+    REQUIRE(a.kv_type > 0 && cache_ok(*kc, a.kv_type) && kc->size(2) < INTS && kc->size(3) == a.dk);
     a.n_head_kv = (int32_t) kc->size(2); a.n_pages = kc->size(0); a.k = pool_of(*kc);
     if (vc) {
-        REQUIRE(cache_ok(*vc, a.kv_type) && vc->size(0) == a.n_pages && vc->size(2) == a.n_head_kv);
+        REQUIRE(cache_ok(*vc, a.kv_type) && vc->size(0) == a.n_pages && vc->size(2) == a.n_head_kv && vc->size(3) < INTS);
         a.dv = (int32_t) vc->size(3); a.v = pool_of(*vc);
     } else REQUIRE(weights && !outp);
     REQUIRE(table_ok(*table) && table->size(0) == n_seq && ints(*lens, n_seq));
@@ -554,7 +560,7 @@ PyObject * gqa_attn(PyObject *, PyObject * const * o, Py_ssize_t n) {
     if (mask) {
         REQUIRE(mask->scalar_type() == at::kHalf && rows_ok(*mask, 2, false) && mask->size(0) == n_seq);
         a.mask = mask->data_ptr(); a.mask_nb1 = mask->stride(0) * 2; a.mask_ne0 = mask->size(1);
-        if (!a.mask) { PyErr_SetString(PyExc_ValueError, "a mask without columns leaves no row"); return nullptr; }
+        if (!a.mask && n_seq) { PyErr_SetString(PyExc_ValueError, "a mask without columns leaves no row"); return nullptr; }
     }
     if (weights) {
         REQUIRE(weights->scalar_type() == at::kFloat && rows_ok(*weights, 3, true) && weights->size(0) == n_seq && weights->size(1) == a.n_head_kv && weights->size(2) >= a.bt_stride * PAGE);
@@ -590,18 +596,17 @@ PyObject * gqa_evict(PyObject *, PyObject * const * o, Py_ssize_t n) {
     for (const at::Tensor * t : { table, lens, kc, vc, wop, keptp, newp }) SAME_DEVICE(t);
     gqa_evict_args a;
     memset(&a, 0, sizeof a);
-    a.n_keep = (int32_t) PyLong_AsLong(o[5]); a.n_sink = (int32_t) PyLong_AsLong(o[6]); a.n_recent = (int32_t) PyLong_AsLong(o[7]);
-    if (PyErr_Occurred()) return nullptr;
+    if (!int_of(o[5], a.n_keep) || !int_of(o[6], a.n_sink) || !int_of(o[7], a.n_recent)) return nullptr;
     REQUIRE(table_ok(*table));
     const int64_t n_seq = table->size(0), cap = table->size(1) * PAGE;
     REQUIRE(ints(*lens, n_seq));
     a.n_seq = (int32_t) n_seq;
     a.block_table = (const int32_t *) table->data_ptr(); a.bt_stride = table->size(1); a.seq_lens = (const int32_t *) lens->data_ptr();
-    REQUIRE(rows_ok(*kc, 4, true) && kc->size(0) >= 1 && kc->size(1) == PAGE);
+    REQUIRE(n_seq < INTS && rows_ok(*kc, 4, true) && kc->size(0) >= 1 && kc->size(1) == PAGE && kc->size(2) < INTS && kc->size(3) < INTS / 16);
     a.n_head_kv = (int32_t) kc->size(2); a.n_pages = kc->size(0); a.k = pool_of(*kc);
     a.k_row_bytes = (int32_t) (kc->size(3) * (int64_t) kc->element_size());
     if (vc) {
-        REQUIRE(rows_ok(*vc, 4, true) && vc->size(0) == a.n_pages && vc->size(1) == PAGE && vc->size(2) == a.n_head_kv);
+        REQUIRE(rows_ok(*vc, 4, true) && vc->size(0) == a.n_pages && vc->size(1) == PAGE && vc->size(2) == a.n_head_kv && vc->size(3) < INTS / 16);
         a.v = pool_of(*vc); a.v_row_bytes = (int32_t) (vc->size(3) * (int64_t) vc->element_size());
     }
     REQUIRE(q.scalar_type() == at::kFloat && rows_ok(q, 3, false) && q.size(0) == n_seq && q.size(1) == a.n_head_kv && q.size(2) == cap);

@@ -720,6 +720,34 @@ def test_calls_that_are_refused(gpu):
         a=dict(n_keep=0), n_sink=11, n_recent=-1, b=dict(n_sink=5, n_recent=6), new_lens=lens), (RuntimeError,))
 
 
+def test_empty_batches_with_everything(gpu):
+    """No sequence, no token: nothing to do, whatever else is handed in."""
+    import jittorinfer_amd as J
+    z = lambda *s, dtype=BF16: torch.zeros(s, dtype=dtype, device=gpu)
+    k, bt, lens, w = z(3, 128, 2, 64), z(0, 2, dtype=torch.int32), z(0, dtype=torch.int32), z(0, 2, 256, dtype=F32)
+    assert J.gqa_attn(z(0, 4, 64), k, k.clone(), bt, lens, scale=1.0, mask=z(0, 256, dtype=F16), weights=w, window=5).shape == (0, 4, 64)
+    assert J.gqa_attn(z(0, 4, 576), z(3, 128, 1, 576), None, bt, lens, scale=1.0, weights=z(0, 1, 256, dtype=F32)).shape == (0, 1, 256)
+    kept, new, out = J.gqa_evict(w, bt, lens, k, k.clone(), n_keep=10)
+    assert kept.shape == (0, 2, 10) and new.shape == (0,) and out.shape == w.shape
+    assert J.gqa_norm_rope(z(0, 4, 64), z(0, 2, 64), z(0, 2, 64), lens, n_dims=64, k_cache=k, v_cache=k.clone(), block_table=bt, seq_ids=lens).shape == (0, 4, 64)
+    assert not k.any()
+
+
+def test_integers_past_32_bits_are_refused(gpu):
+    import jittorinfer_amd as J
+    z = lambda *s, dtype=BF16: torch.zeros(s, dtype=dtype, device=gpu)
+    k, bt, lens, w = z(3, 128, 2, 64), z(2, 1, dtype=torch.int32), z(2, dtype=torch.int32), z(2, 2, 128, dtype=F32)
+    far = (1 << 32) + 8
+    for name in ("n_keep", "n_sink", "n_recent"):
+        with pytest.raises(OverflowError):
+            J.gqa_evict(w, bt, lens, k, k.clone(), **{"n_keep": 20, name: far})
+    with pytest.raises(OverflowError):
+        J.gqa_attn(z(2, 4, 64), k, k.clone(), bt, lens, scale=1.0, n_workgroups=far)
+    for name in ("n_dims", "mode", "n_ctx_orig"):
+        with pytest.raises(OverflowError):
+            J.gqa_norm_rope(z(2, 4, 64), None, None, lens, **{"n_dims": 8, name: far})
+
+
 # ---------------------------------------------------------------- together
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
