@@ -14,7 +14,7 @@
 //     columns {8i + c} one MFMA each.
 //   * P goes in as two 16-bit numbers, hi + lo: the matrix cores are idle otherwise, and P rounded once (2^-9 in bf16) would be the
 //     largest error of the whole pass.
-//   * the running maximum moves only when a score passes it by more than 2^8 (exp2 sums then reach 2^8 a key, far from f32's range), so
+//   * the running maximum moves only when a score passes it by more than 2^8 (2^4 in f16; sums then reach 2^8 a key, far from f32's range), so
 //     the common tile has no reduction across lanes and no rescaling.
 //   * K of the next tile is requested when this tile's scores are done, V when its products are.
 //
@@ -168,6 +168,9 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
     static_assert(NB == 1 || !QUAD, "one block of heads a wave");
     constexpr int  KC    = DK / 32;
     constexpr int  ROWS  = NB * 16, NW = 4;
+    // P is taken relative to a reference that lies REF below the maximum when it is set and stays until a score passes that maximum by SLACK (log2 units).
+    // Halves of 16 bits hold P to 2^-16 of itself; f16's end at 2^-25, so there P runs up to 2^15, and what is lost of a row is 2^-36 of the largest.
+    constexpr float REF = F16 ? 11.f : 0.f, SLACK = F16 ? 4.f : 8.f;
     using VG = VGeom<DV>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ float2 sh_ml[QUAD ? 1 : NW][ROWS];
@@ -339,10 +342,10 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
                 float top = x[0];
 #pragma unroll
                 for (int e = 1; e < 8; e++) top = fmaxf(top, x[e]);
-                if (__any(top > m[nb] + 8.f)) {
+                if (__any(top > m[nb] + (REF + SLACK))) {
                     top = fmaxf(top, __shfl_xor(top, 16, 64));
                     top = fmaxf(top, __shfl_xor(top, 32, 64));
-                    const float nm = fmaxf(top, m[nb]);
+                    const float nm = fmaxf(top - REF, m[nb]);
                     const float a  = m[nb] == nm ? 1.f : fast_exp2(m[nb] - nm);
                     m[nb] = nm;
                     l[nb] *= a;

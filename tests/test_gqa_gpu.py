@@ -236,6 +236,31 @@ def test_attn_scores_far_apart(gpu):
     _check_attn(gpu, q, k, v, bt, lens, n_workgroups=2)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("above", [9.0, 11.0, 13.0, 15.0, 17.5, 22.0])
+@pytest.mark.parametrize("at", [0, 777, 16383])
+def test_attn_one_row_far_above_many(gpu, dtype, above, at):
+    """A row with a value of 0 holds nearly all of the weight: what is left is the sum of many weights of 2^-13 to 2^-32 of the largest."""
+    import jittorinfer_amd as J
+    n = 16384
+    gen = torch.Generator().manual_seed(34)
+    q, k, v, bt, lens = _attn_case(34, [n], n // 128, 4, 2, 64, 64, dtype)
+    rows = torch.arange(n)
+    page, row = bt[0].long()[rows // 128], rows % 128
+    q[:] = 0
+    q[..., 0] = 8
+    k[page, row] = 0
+    k[page[at], row[at], :, 0] = above
+    v[page, row] = (torch.rand((n, 2, 64), generator=gen) + 0.5).to(dtype)
+    v[page[at], row[at]] = 0
+    out, off, _, _ = R.attn(q, k, v, bt, [n], 1 / 8)
+    # in f16 the two halves of a weight end at 2^-25, 2^-36 of the largest (2^11 at least): an error of that a row
+    off = off + (n * 1.5 * 2.0 ** -36 if dtype == F16 else 0.0)
+    for n_workgroups in (0, 1):
+        got = J.gqa_attn(q.to(gpu), k.to(gpu), v.to(gpu), bt.to(gpu), lens.to(gpu), scale=1 / 8, n_workgroups=n_workgroups, out=torch.empty(out.shape, dtype=F32, device=gpu))
+        _near(got, out, off, F32)
+
+
 def test_attn_same_call_same_bits(gpu):
     import jittorinfer_amd as J
     q, k, v, bt, lens = (t.to(gpu) for t in _attn_case(17, [900, 33, 513], 8, 8, 2, 128, 128, BF16))
