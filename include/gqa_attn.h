@@ -44,7 +44,7 @@ typedef struct gqa_pool {
  * seq_ids[t] to row slots[t] (NULL: pos[t]); rows outside the block table, negative ones and bad pages are skipped, as the cache write
  * of include/mla_kv_write.h skips them.  Two tokens of one call that name the same row leave parts of either there. */
 typedef struct gqa_norm_rope_args {
-    int32_t n_tok, n_head, n_head_kv;
+    int32_t n_tok, n_head, n_head_kv;   /* n_tok below 2^24 */
     int32_t dk, dv;          /* values per key / query head and per value head: multiples of 8, at most 256 */
     int32_t src_type;        /* of q, k, v: MLA_TYPE_F32 | MLA_TYPE_F16 | MLA_TYPE_BF16 */
     int32_t w_type;          /* of the weights: the same three */

@@ -439,7 +439,8 @@ extern "C" int gqa_evict_check(const gqa_evict_args * a) {
     const int64_t apart = (const char *) a->weights_dst - (const char *) a->weights, row = a->bt_stride * PAGE * 4;
     if (apart && apart > -row && apart < row) return MLA_ERR_UNSUPPORTED;
     const Plan pl = make_plan(a);
-    if (pl.k.count > MOVE_SEGMENTS || pl.v.count > MOVE_SEGMENTS || pl.segments >= ((int64_t) 1 << 30)) return MLA_ERR_BAD_SHAPE;
+    // (a launch holds fewer than 2^32 threads)
+    if (pl.k.count > MOVE_SEGMENTS || pl.v.count > MOVE_SEGMENTS || pl.segments >= ((int64_t) 1 << 32) / MOVE_THREADS) return MLA_ERR_BAD_SHAPE;
     return 0;
 }
 

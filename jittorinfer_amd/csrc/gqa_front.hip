@@ -214,7 +214,7 @@ extern "C" int gqa_norm_rope_check(const gqa_norm_rope_args * a) {
     if (!a) return MLA_ERR_NULL;
     if (!known(a->src_type) || !known(a->w_type) || !known(a->dst_type)) return MLA_ERR_BAD_TYPE;
     if (a->k && a->kv_type != MLA_TYPE_F16 && a->kv_type != MLA_TYPE_BF16) return MLA_ERR_BAD_TYPE;
-    if (a->n_tok < 0 || a->n_head < 1 || a->dk < 8 || a->dk % 8 || a->dk > 256) return MLA_ERR_BAD_SHAPE;
+    if (a->n_tok < 0 || a->n_tok >= (1 << 24) || a->n_head < 1 || a->dk < 8 || a->dk % 8 || a->dk > 256) return MLA_ERR_BAD_SHAPE;
     if (a->k && (a->n_head_kv < 1 || a->n_seq < 0)) return MLA_ERR_BAD_SHAPE;
     if (a->v && (!a->k || a->dv < 8 || a->dv % 8 || a->dv > 256)) return MLA_ERR_BAD_SHAPE;
     if (a->mode != MLA_ROPE_MODE_NORM && a->mode != MLA_ROPE_MODE_NEOX) return MLA_ERR_UNSUPPORTED;

@@ -208,6 +208,15 @@ def test_evict_accepts():
     assert lib.gqa_evict_workspace_size(C.byref(_cut(n_keep=0))) == 0
 
 
+def test_launches_of_more_threads_than_there_are_refused():
+    """Nothing starts of a call whose last kernel could not: 65532 heads of rows of 612 bytes, 40 rows a workgroup."""
+    lib = J.library()
+    far = dict(n_seq=32766, k_row_bytes=612, v=J.GqaPool(), bt_stride=1024, w_nb1=1024 * 512, w_nb2=1024 * 1024, wd_nb1=1024 * 512, wd_nb2=1024 * 1024, weights_dst=1 << 40)
+    assert lib.gqa_evict_check(C.byref(_cut(n_keep=100000, **far))) == SHAPE and lib.gqa_evict_workspace_size(C.byref(_cut(n_keep=100000, **far))) == 0
+    assert lib.gqa_evict_check(C.byref(_cut(n_keep=5000, **far))) == 0
+    assert lib.gqa_norm_rope_check(C.byref(_rows(n_tok=1 << 24))) == SHAPE and lib.gqa_norm_rope_check(C.byref(_rows(n_tok=(1 << 24) - 1))) == 0
+
+
 @pytest.mark.parametrize("kw", [dict(weights_dst=32768 + 4), dict(weights_dst=32768 - 2044), dict(weights_dst=32768 + 2044), dict(v=_pool(128))], ids=_name)
 def test_evict_refuses_what_overlaps(kw):
     a = _cut(**kw)
