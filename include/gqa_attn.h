@@ -88,7 +88,7 @@ int gqa_norm_rope_launch(const gqa_norm_rope_args * args, void * stream);
  * below 0 count as 0, above the block table's room as that room.
  * weights (optional): weights[b][g][i] += sum over the query heads of KV head g of p_i, in f32 and in one order; rows outside the
  * window or the length keep their values.  dst and weights lie apart from each other, from themselves and from all that is read.
- * Supported widths (dk, dv): (64, 64), (128, 128), (192, 128), (256, 256), and (576, 0) without `v` and dst: the weights alone over a latent cache. */
+ * Supported widths (dk, dv): (64, 64), (128, 128), (192, 128), (256, 256), and (576, 0) with one KV head, without `v` and dst: the weights alone over a latent cache. */
 typedef struct gqa_attn_args {
     int32_t n_seq, n_head, n_head_kv; /* n_head a multiple of n_head_kv */
     int32_t dk, dv;

@@ -930,7 +930,7 @@ extern "C" int gqa_attn_check(const gqa_attn_args * a) {
     if (a->kv_type != MLA_TYPE_BF16 && a->kv_type != MLA_TYPE_F16) return MLA_ERR_BAD_TYPE;
     if ((a->q_type != MLA_TYPE_F32 && a->q_type != a->kv_type) || (a->dst_type != MLA_TYPE_F32 && a->dst_type != a->kv_type)) return MLA_ERR_BAD_TYPE;
     if (a->n_seq < 0 || a->n_head < 1 || a->n_head_kv < 1 || a->n_head % a->n_head_kv || a->window < 0 || a->n_workgroups < 0 || a->n_workgroups > 65536) return MLA_ERR_BAD_SHAPE;
-    const bool widths = a->dk == 64 || a->dk == 128 || a->dk == 256 ? a->dv == a->dk : (a->dk == 192 && a->dv == 128) || (a->dk == 576 && a->dv == 0);
+    const bool widths = a->dk == 64 || a->dk == 128 || a->dk == 256 ? a->dv == a->dk : (a->dk == 192 && a->dv == 128) || (a->dk == LK && a->dv == 0 && a->n_head_kv == 1);
     if (!widths) return MLA_ERR_UNSUPPORTED;
     if (!(a->logit_softcap >= 0.f)) return MLA_ERR_UNSUPPORTED;
     if (a->n_seq == 0) return 0;

@@ -105,6 +105,13 @@ def test_latent_weights_refuse(kw, code):
     assert J.library().gqa_attn_check(C.byref(a)) == code
 
 
+@pytest.mark.parametrize("n_head,n_head_kv", [(128, 2), (128, 128), (4, 2)])
+def test_latent_weights_refuse_more_than_one_kv_head(n_head, n_head_kv):
+    a = _latent(n_head=n_head, n_head_kv=n_head_kv, k=_pool(576, n_head_kv))
+    assert J.library().gqa_attn_check(C.byref(a)) == UNSUPPORTED and J.library().gqa_attn_workspace_size(C.byref(a)) == 0
+    assert J.library().gqa_attn_launch(C.byref(a), None) == UNSUPPORTED
+
+
 def _rows(**kw):
     a = J.GqaNormRopeArgs()
     a.n_tok, a.n_head, a.n_head_kv, a.dk, a.dv, a.n_seq = 4, 8, 2, 128, 128, 3
