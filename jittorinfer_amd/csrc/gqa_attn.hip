@@ -721,13 +721,13 @@ __device__ __forceinline__ void sum_weights(const AttnP & p, int b, int kvh, int
         const int  h = (int) threadIdx.x / lanes, sub = (int) threadIdx.x & (lanes - 1), r = c + min(h, heads - 1);
         const int  hb = p.quad ? kvh >> 2 : kvh * p.row_blocks + r / p.rows, row = p.quad ? (kvh & 3) * p.group + r : r % p.rows;
         const int2 it = p.items[(int64_t) b * p.head_blocks + hb];
-        const int  v0 = it.x >> 1, n = it.y - v0 + 1;
+        const int  v0 = it.x >> 1, n = it.y - v0 + 1, slot0 = n > 1 ? it.x : 0;     // (a head of one run left no piece: the first of all is read, unused)
         float2 ml[AHEAD], got = p.lse[h0 + r];                    // (of a head that one run covered; else meaningless)
         auto pieces = [&](int i0) {
 #pragma unroll
             for (int e = 0; e < AHEAD; e++) {
                 const int i = min(i0 + e * lanes, n - 1);
-                ml[e] = p.part_ml[((int64_t) (i ? 2 * (v0 + i) : it.x)) * p.rows + row];
+                ml[e] = p.part_ml[((int64_t) (i ? 2 * (v0 + i) : slot0)) * p.rows + row];
             }
         };
         pieces(sub);

@@ -225,6 +225,14 @@ def test_weights_of_groups_past_256_heads(gpu, kw):
     _check_attn(gpu, *_attn_case(33, [1400, 0, 1345] + [0, 1] * 49, 11, 300, 1, 64, 64, BF16), **kw)
 
 
+@pytest.mark.parametrize("n_seq,heads", [(255, 16), (257, 16), (600, 3), (130, 130)])
+def test_weights_over_many_latent_caches(gpu, n_seq, heads):
+    """As many sequences (blocks of 128 heads) as workgroups, and more: runs of whole ones in turn, that leave no piece."""
+    gen = torch.Generator().manual_seed(n_seq)
+    lens = [int(x) for x in torch.randint(0, 200, (n_seq,), generator=gen)]
+    _check_attn(gpu, *_attn_case(36, lens, 2, heads, 1, 576, 0, BF16))
+
+
 def test_attn_scores_far_apart(gpu):
     """Scores that grow by hundreds along a sequence, and fall: the running maximum moves, and leaves nothing of what came before."""
     q, k, v, bt, lens = _attn_case(16, [512, 512], 4, 4, 2, 64, 64, F16)
