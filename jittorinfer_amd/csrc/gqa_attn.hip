@@ -119,6 +119,17 @@ struct Lengths {
         for (int b0 = 0; b0 < p.n_seq; b0 += 256) { fetch(p, lane, b0); total += lane_of(scan_wave(own[0] + own[1] + own[2] + own[3]), 63); }
         return total * p.head_blocks;
     }
+    __device__ __forceinline__ int all_units(const AttnP & p, int lane, int per) {           // after all_pages
+        int total = 0;
+        for (int b0 = 0; b0 < p.n_seq; b0 += 256) {
+            if (p.n_seq > 256) fetch(p, lane, b0);
+            int n = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) n += (own[e] + per - 1) / per;
+            total += lane_of(scan_wave(n), 63);
+        }
+        return total * p.head_blocks;
+    }
     __device__ __forceinline__ Place place(const AttnP & p, int lane, int u, int per) {      // after all_pages
         for (int b0 = 0, before = 0; b0 < p.n_seq; b0 += 256) {
             if (p.n_seq > 256) fetch(p, lane, b0);
@@ -494,8 +505,8 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
 // Scores of a latent cache (rows of 576, one KV head) for its weights: (m, l) and every score, as gqa_attn_kernel leaves them, without V.  Up to
 // 128 heads share a row, 128 flop a byte: the rows of Q lie in LDS (147 KB) and are read, 16 heads at a time, against a tile of 32 rows of K
 // in registers, by eight waves, so that every SIMD still has two.  The loop over blocks of heads is a loop: eight copies of its body, run once or
-// twice by a workgroup, took twice as long, most of it to fetch them.  8 x 8192 rows, 128 heads: 27 us, of which the rows are 11 at the
-// memory's rate and the products 6; then 11.6 to join and add them up.
+// twice by a workgroup, took twice as long, most of it to fetch them.  8 x 8192 rows, 128 heads: 30 us, of which the rows are 12 at the
+// memory's rate and the products 7; then 4 to join and 8 to add them up.
 constexpr int LK = 576, LPITCH = LK * 2 + 16, LWAVES = 8, LROWS = 128;
 template <bool F16, bool BIAS>
 __global__ void __launch_bounds__(64 * LWAVES) gqa_scores_kernel(const AttnP p) {
@@ -504,11 +515,20 @@ __global__ void __launch_bounds__(64 * LWAVES) gqa_scores_kernel(const AttnP p) 
     __shared__ float2 sh_ml[LWAVES][LROWS];
     const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), quarter = wave & 3, l15 = lane & 15, lg = lane >> 4;
     const int wg = blockIdx.x;
-    // A workgroup's Q is 147 KB to stage, so no run crosses from one (sequence, head block) to another: units of `per` pages, as many as there
-    // are workgroups at most; with as many head blocks as workgroups, whole ones in turn.
+    // A workgroup's Q is 147 KB to stage, so no run crosses from one (sequence, head block) to another: units of `per` pages, the fewest of which
+    // there are no more than workgroups (units of `top` pages are never more; taking those, 8 x 8192 rows came to 3 pages a unit and 37 us, not 2 and 30); with as many head blocks as workgroups, whole ones in turn.
     Lengths   lens;
     const int total = lens.all_pages(p, lane), spare = p.n_wg - p.n_seq * p.head_blocks;
-    const int per = spare > 0 ? max(1, uni((total + spare - 1) / spare)) : INT_MAX / 2;
+    int per = INT_MAX / 2;
+    if (spare > 0) {
+        per = uni((total + p.n_wg - 1) / p.n_wg);
+        for (int top = uni((total + spare - 1) / spare); per < top;) {
+            const int mid = (per + top) / 2;
+            if (uni(lens.all_units(p, lane, max(mid, 1))) <= p.n_wg) top = mid;
+            else per = mid + 1;
+        }
+        per = max(per, 1);
+    }
     for (int u = wg;; u += p.n_wg) {
         const Place at = lens.place(p, lane, u, per);
         const int b = uni(at.seq);
@@ -561,9 +581,10 @@ __global__ void __launch_bounds__(64 * LWAVES) gqa_scores_kernel(const AttnP p) 
 #pragma unroll
             for (int k = 0; k < 6; k++) *(u32x4 *) (lds + row_of(k) * LPITCH + col_of(k) * 16) = row_of(k) < heads ? v[k] : u32x4{ 0u, 0u, 0u, 0u };
         };
+        const int last = uni((min(LROWS, (heads + 15) & ~15) * (LK / 8) - 1) / (6 * 64 * LWAVES)) * 6;    // (blocks of 16 rows without a head are not read)
 #pragma unroll 1
-        for (int k0 = 0; k0 < PIECES - 6; k0 += 6) stage(k0, [] {});
-        stage(PIECES - 6, [&] { load_k(min(i, n - 1), good(id) ? id : 0); });     // (a wave without a page of its own: the last one's, unused)
+        for (int k0 = 0; k0 < last; k0 += 6) stage(k0, [] {});
+        stage(last, [&] { load_k(min(i, n - 1), good(id) ? id : 0); });           // (a wave without a page of its own: the last one's, unused)
         // (a wave's own rows of sh_ml hold its running maxima and sums: LDS operations of a wave stay in order)
         for (int r = lane; r < LROWS; r += 64) sh_ml[wave][r] = make_float2(-INFINITY, 0.f);
         __syncthreads();
@@ -695,6 +716,7 @@ __device__ __forceinline__ void join_head(const AttnP & p, int b, int kvh, int r
     }
     L = over_waves(L, false);
     const float inv = L == 0.f ? 0.f : 1.f / L;
+    if (p.scores && threadIdx.x == 0) p.lse[(int64_t) b * p.n_head + h] = make_float2(M == -INFINITY ? 0.f : M, inv);
     sum[threadIdx.x] = o;
     __syncthreads();
     if (g == 0) {
@@ -703,54 +725,68 @@ __device__ __forceinline__ void join_head(const AttnP & p, int b, int kvh, int r
     }
 }
 
+// (m, 1 / l) of head r of a group from its pieces, by `lanes` lanes of a wave (a power of two), this one `sub`; all of them get it.  AHEAD pieces a
+// lane are under way at a time, and what `meanwhile` requests behind the first.
+template <int AHEAD, typename F>
+__device__ __forceinline__ float2 join_sums(const AttnP & p, int b, int kvh, int r, int lanes, int sub, F meanwhile) {
+    const int  hb = p.quad ? kvh >> 2 : kvh * p.row_blocks + r / p.rows, row = p.quad ? (kvh & 3) * p.group + r : r % p.rows;
+    const int2 it = p.items[(int64_t) b * p.head_blocks + hb];
+    const int  v0 = it.x >> 1, n = it.y - v0 + 1, slot0 = n > 1 ? it.x : 0;     // (a head of one run left no piece: the first of all is read, unused)
+    const float2 whole = p.lse[(int64_t) b * p.n_head + kvh * p.group + r];     // (of a head that one run covered; else meaningless)
+    float2 ml[AHEAD];
+    auto pieces = [&](int i0) {
+#pragma unroll
+        for (int e = 0; e < AHEAD; e++) {
+            const int i = min(i0 + e * lanes, n - 1);
+            ml[e] = p.part_ml[((int64_t) (i ? 2 * (v0 + i) : slot0)) * p.rows + row];
+        }
+    };
+    pieces(sub);
+    meanwhile();
+    if (n == 1) return whole;
+    float M = -INFINITY, L = 0.f;
+    for (int i0 = sub; i0 < n; i0 += AHEAD * lanes) {
+        if (i0 != sub) pieces(i0);
+        float top = M;
+#pragma unroll
+        for (int e = 0; e < AHEAD; e++) top = fmaxf(top, ml[e].x);
+        L = L == 0.f ? 0.f : L * fast_exp2(M - top);
+#pragma unroll
+        for (int e = 0; e < AHEAD; e++) L += i0 + e * lanes >= n || ml[e].y == 0.f ? 0.f : ml[e].y * fast_exp2(ml[e].x - top);
+        M = top;
+    }
+    for (int d = 1; d < lanes; d <<= 1) {
+        const float m = __shfl_xor(M, d, 64), l = __shfl_xor(L, d, 64), top = fmaxf(M, m);
+        L = (L == 0.f ? 0.f : L * fast_exp2(M - top)) + (l == 0.f ? 0.f : l * fast_exp2(m - top));
+        M = top;
+    }
+    return make_float2(M == -INFINITY ? 0.f : M, L == 0.f ? 0.f : 1.f / L);
+}
+// The same for all heads ahead of the sums, a wave a head, where there is no result to join.  Grid: x = the heads of a group in fours, y = a (sequence, KV head).
+__global__ void __launch_bounds__(JOIN) gqa_lse_kernel(const AttnP p) {
+    const int b = blockIdx.y / p.n_head_kv, kvh = blockIdx.y - b * p.n_head_kv, r = (int) blockIdx.x * 4 + ((int) threadIdx.x >> 6);
+    if (r >= p.group || pages_of(span_of(p, b)) == 0) return;
+    const float2 got = join_sums<4>(p, b, kvh, r, 64, (int) threadIdx.x & 63, [] {});
+    if ((threadIdx.x & 63) == 0) p.lse[(int64_t) b * p.n_head + kvh * p.group + r] = got;
+}
+
 // weights[b][g][i] += sum over the group's heads of exp2(s - m) / l, from the scores the first kernel left.  A thread takes 4 rows and
 // every parts-th head (parts: 16, or the power of two that holds a smaller group); the parts are added in one order.  (m, l) of a head is
-// joined from its pieces by every workgroup for itself, while its first scores are under way, which costs less than a launch in between: 6.5 us with the
-// results of 8 x 4096 rows of 16 heads, where two launches took 10.2.  (2048 workgroups in all, or a quarter of them: 12.7 us either way over 8 x 8192 of 128.)
+// joined from its pieces by every workgroup for itself, while its first scores are under way, or, ready, by a launch ahead.
 constexpr int SUM_HEADS = 256, SUM_BLOCKS = 2048;
 template <int HEADS>                                          // scores under way at a time
-__device__ __forceinline__ void sum_weights(const AttnP & p, int b, int kvh, int block, int blocks, int parts, f32x4 * sum) {
+__device__ __forceinline__ void sum_weights(const AttnP & p, int b, int kvh, int block, int blocks, int parts, bool ready, f32x4 * sum) {
     __shared__ float2 lse[SUM_HEADS];
     const Span s = span_of(p, b);
     const int  quads = JOIN / parts, part = (int) threadIdx.x / quads, quad = (int) threadIdx.x - part * quads, rows = quads * 4;
     const int64_t h0 = (int64_t) b * p.n_head + (int64_t) kvh * p.group;
     auto join = [&](int c, int heads, auto load) {            // heads c .. c + heads - 1 of the group, some lanes of a wave each, and the first scores
-        constexpr int AHEAD = HEADS == 1 ? 2 : 8;             // pieces under way at a time a lane (16 lanes a head or more, or 1)
         int lanes = 64;
         while (lanes * heads > JOIN) lanes >>= 1;
-        const int  h = (int) threadIdx.x / lanes, sub = (int) threadIdx.x & (lanes - 1), r = c + min(h, heads - 1);
-        const int  hb = p.quad ? kvh >> 2 : kvh * p.row_blocks + r / p.rows, row = p.quad ? (kvh & 3) * p.group + r : r % p.rows;
-        const int2 it = p.items[(int64_t) b * p.head_blocks + hb];
-        const int  v0 = it.x >> 1, n = it.y - v0 + 1, slot0 = n > 1 ? it.x : 0;     // (a head of one run left no piece: the first of all is read, unused)
-        float2 ml[AHEAD], got = p.lse[h0 + r];                    // (of a head that one run covered; else meaningless)
-        auto pieces = [&](int i0) {
-#pragma unroll
-            for (int e = 0; e < AHEAD; e++) {
-                const int i = min(i0 + e * lanes, n - 1);
-                ml[e] = p.part_ml[((int64_t) (i ? 2 * (v0 + i) : slot0)) * p.rows + row];
-            }
-        };
-        pieces(sub);
-        load(c + part);
-        if (n > 1) {
-            float M = -INFINITY, L = 0.f;
-            for (int i0 = sub; i0 < n; i0 += AHEAD * lanes) {
-                if (i0 != sub) pieces(i0);
-                float top = M;
-#pragma unroll
-                for (int e = 0; e < AHEAD; e++) top = fmaxf(top, ml[e].x);
-                L = L == 0.f ? 0.f : L * fast_exp2(M - top);
-#pragma unroll
-                for (int e = 0; e < AHEAD; e++) L += i0 + e * lanes >= n || ml[e].y == 0.f ? 0.f : ml[e].y * fast_exp2(ml[e].x - top);
-                M = top;
-            }
-            for (int d = 1; d < lanes; d <<= 1) {
-                const float m = __shfl_xor(M, d, 64), l = __shfl_xor(L, d, 64), top = fmaxf(M, m);
-                L = (L == 0.f ? 0.f : L * fast_exp2(M - top)) + (l == 0.f ? 0.f : l * fast_exp2(m - top));
-                M = top;
-            }
-            got = make_float2(M == -INFINITY ? 0.f : M, L == 0.f ? 0.f : 1.f / L);
-        }
+        const int h = (int) threadIdx.x / lanes, sub = (int) threadIdx.x & (lanes - 1), r = c + min(h, heads - 1);
+        float2 got;
+        if (ready) { got = p.lse[h0 + r]; load(c + part); }
+        else got = join_sums<HEADS == 1 ? 2 : 8>(p, b, kvh, r, lanes, sub, [&] { load(c + part); });      // (16 lanes a head or more, or 1)
         if (h < heads && sub == 0) lse[h] = got;
         __syncthreads();
     };
@@ -798,11 +834,11 @@ __device__ __forceinline__ void sum_weights(const AttnP & p, int b, int kvh, int
 // What follows the runs, in one launch.  Grid: x = the heads of a group (none without a result), then the workgroups that share a sequence's
 // rows (none without weights); y = a (sequence, KV head).
 template <bool F16, int HEADS>
-__global__ void __launch_bounds__(JOIN) gqa_join_kernel(const AttnP p, const int joins, const int parts) {
+__global__ void __launch_bounds__(JOIN) gqa_join_kernel(const AttnP p, const int joins, const int parts, const int ready) {
     __shared__ f32x4 sum[JOIN];
     const int b = blockIdx.y / p.n_head_kv, kvh = blockIdx.y - b * p.n_head_kv;
     if ((int) blockIdx.x < joins) join_head<F16>(p, b, kvh, (int) blockIdx.x, sum);
-    else if constexpr (HEADS > 0) sum_weights<HEADS>(p, b, kvh, (int) blockIdx.x - joins, (int) gridDim.x - joins, parts, sum);
+    else if constexpr (HEADS > 0) sum_weights<HEADS>(p, b, kvh, (int) blockIdx.x - joins, (int) gridDim.x - joins, parts, ready != 0, sum);
 }
 
 // ---------------------------------------------------------------- host
@@ -811,6 +847,7 @@ struct Plan {
     int     nb, rows, row_blocks, head_blocks, n_wg;
     bool    quad;
     int64_t items;
+    int     pieces;                                           // of a head, where all sequences fill the block table
     size_t  off_ml, off_items, off_scores, off_lse, bytes;    // of the workspace; partial rows first
 };
 
@@ -822,6 +859,10 @@ struct Plan {
 // of 64, 32 x 8192 (8192) 51 against 52, 1 x 131072 (4096) 33.3 against 29.5.  Head by head a page of a head is contiguous anyway: 32 on 8 of 128,
 // 32 x 8192 194 against 186.  Heads of 256, 512 bytes a row each: 187 against 187.
 constexpr int64_t TWO_BLOCKS = 1024, QUADS_OF_MANY = 2048, QUADS = 8192;
+// Where weights are summed, heads are joined ahead of the sums if a workgroup of the sums would have this many pieces to read first (pieces of a head, in
+// brackets times heads of a group): 128 heads over one latent cache, 1 x 65536 rows (32768) 41 against 65 us, 8 x 8192 (4096) 42 against 42, 8 x 2048
+// (2048) 31.5 against 29.5; 16 heads over it, 1 x 65536 (4096) 27 against 31; 32 on 8 of 128, 8 x 2048 (128) 25.1 against 21.2.
+constexpr int64_t JOIN_AHEAD = 4096;
 Plan make_plan(const gqa_attn_args * a) {
     Plan pl;
     const int group = a->n_head / a->n_head_kv;
@@ -840,6 +881,8 @@ Plan make_plan(const gqa_attn_args * a) {
     const int fill = 256 * (a->dv ? wg_per_cu(a->dk, pl.nb) : 1);
     pl.n_wg = (int) (units < fill ? units : fill);
     if (a->n_workgroups > 0) pl.n_wg = (int) (units < a->n_workgroups ? units : a->n_workgroups);
+    const int64_t shares = (pl.n_wg + pl.items - 1) / pl.items;
+    pl.pieces = (int) (shares < a->bt_stride ? shares : a->bt_stride);
     size_t at = 0;
     auto take = [&](size_t n) { const size_t o = at; at += (n + 255) & ~(size_t) 255; return o; };
     take((size_t) 2 * pl.n_wg * pl.rows * a->dv * 4);
@@ -902,17 +945,20 @@ hipError_t launch_all(const AttnP & p, const Plan & pl, int dk, hipStream_t st) 
     else if (pl.nb == 2) e = bias ? launch_widths<F16, 2, true>(p, dk, st) : launch_widths<F16, 2, false>(p, dk, st);
     else                 e = bias ? launch_widths<F16, 1, true>(p, dk, st) : launch_widths<F16, 1, false>(p, dk, st);
     if (e != hipSuccess) return e;
-    const int joins = p.dv ? p.group : 0, groups = p.n_seq * p.n_head_kv;
-    if (!p.scores) {
-        hipLaunchKernelGGL((gqa_join_kernel<F16, 0>), dim3((unsigned) joins, (unsigned) groups), dim3(JOIN), 0, st, p, joins, 0);
-        return hipGetLastError();
-    }
+    int joins = p.dv ? p.group : 0;
+    const int  groups = p.n_seq * p.n_head_kv;
+    const bool ahead  = p.scores && (int64_t) pl.pieces * p.group >= JOIN_AHEAD;
+    if (!p.scores || (ahead && joins)) {
+        hipLaunchKernelGGL((gqa_join_kernel<F16, 0>), dim3((unsigned) joins, (unsigned) groups), dim3(JOIN), 0, st, p, joins, 0, 0);
+        joins = 0;
+    } else if (ahead) hipLaunchKernelGGL(gqa_lse_kernel, dim3((unsigned) ((p.group + 3) / 4), (unsigned) groups), dim3(JOIN), 0, st, p);
+    if ((e = hipGetLastError()) != hipSuccess || !p.scores) return e;
     int parts = 1;
     while (parts < 16 && parts < p.group) parts *= 2;
     const int64_t blocks = (p.cap * parts + 4 * JOIN - 1) / (4 * JOIN), share = (SUM_BLOCKS + groups - 1) / groups;
     const dim3 grid((unsigned) (joins + (blocks < share ? blocks : share)), (unsigned) groups);
-    if (p.group <= parts) hipLaunchKernelGGL((gqa_join_kernel<F16, 1>), grid, dim3(JOIN), 0, st, p, joins, parts);
-    else                  hipLaunchKernelGGL((gqa_join_kernel<F16, 8>), grid, dim3(JOIN), 0, st, p, joins, parts);
+    if (p.group <= parts) hipLaunchKernelGGL((gqa_join_kernel<F16, 1>), grid, dim3(JOIN), 0, st, p, joins, parts, (int) ahead);
+    else                  hipLaunchKernelGGL((gqa_join_kernel<F16, 8>), grid, dim3(JOIN), 0, st, p, joins, parts, (int) ahead);
     return hipGetLastError();
 }
 

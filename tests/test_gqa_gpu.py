@@ -218,6 +218,14 @@ def test_weights_of_many_rows(gpu, kw):
     _check_attn(gpu, *_attn_case(30, [2500, 2177, 1, 0, 129, 2400, 300, 2499], 20, 72, 8, 64, 64, BF16), **kw)
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(window=5000), dict(n_workgroups=200, window=3000)], ids=str)
+def test_weights_of_heads_in_many_pieces(gpu, kw):
+    """Heads joined ahead of the sums: over a latent cache, and with results; sequences of one piece and of none beside them."""
+    _check_attn(gpu, *_attn_case(37, [8001, 0, 100], 64, 128, 1, 576, 0, BF16), **kw)
+    _check_attn(gpu, *_attn_case(38, [16000, 1], 128, 64, 1, 64, 64, F16), **kw)
+    _check_attn(gpu, *_attn_case(39, [9001], 128, 40, 1, 576, 0, F16), mask=_mask(torch.Generator().manual_seed(5), 1, 9001), **kw)
+
+
 @pytest.mark.parametrize("kw", [dict(), dict(n_workgroups=5)], ids=str)
 def test_weights_of_groups_past_256_heads(gpu, kw):
     _check_attn(gpu, *_attn_case(31, [5, 300, 0, 129], 3, 600, 2, 64, 64, F16), **kw)
