@@ -725,6 +725,38 @@ def test_evict_in_a_graph(gpu):
         assert torch.equal(d[3].cpu(), want[3]) and torch.equal(d[4].cpu(), want[4])
 
 
+def test_latent_weights_and_a_long_eviction_in_a_graph(gpu):
+    """Heads joined ahead of the sums, selection by several workgroups and the move, captured together: every replay leaves what eager calls leave."""
+    import jittorinfer_amd as J
+    gen = torch.Generator().manual_seed(47)
+    width, n_keep = 260, 9000
+    q = torch.randn((2, 64, 576), generator=gen).to(BF16).to(gpu)
+    k0 = torch.randn((2 * width + 1, 128, 1, 576), generator=gen).to(BF16).to(gpu)
+    bt = R.make_table(gen, [width * 128] * 2, width, 2 * width + 1).to(gpu)
+    def step(k, w, lens, kept, new):
+        J.gqa_attn(q, k, None, bt, lens, scale=0.05, weights=w)
+        J.gqa_evict(w, bt, lens, k, n_keep=n_keep, n_sink=4, n_recent=500, weights_out=w, kept=kept, new_lens=new)
+    fresh = lambda: (k0.clone(), torch.zeros((2, 1, width * 128), device=gpu), torch.zeros(2, dtype=torch.int32, device=gpu),
+                     torch.empty((2, 1, n_keep), dtype=torch.int32, device=gpu), torch.empty(2, dtype=torch.int32, device=gpu))
+    held = fresh()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        step(*held)
+    for lens in ([33000, 20000], [100, 33280], [9001, 0], [33280, 33280]):
+        for t, x in zip(held, fresh()):
+            t.copy_(x)
+        held[2].copy_(torch.tensor(lens, dtype=torch.int32))
+        eager = [t.clone() for t in held]
+        g.replay()
+        torch.cuda.synchronize()
+        step(*eager)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, eager)), lens
+        assert eager[4].tolist() == [min(n, n_keep) for n in lens]
+
+
 # ---------------------------------------------------------------- refusals
 
 def _refused(call, args, wrong, errors=(AssertionError,)):
