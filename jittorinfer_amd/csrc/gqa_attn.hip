@@ -12,8 +12,8 @@
 //   * V: lane (i, g) loads, of the same 8 rows, the 16 bytes of columns 8i .. 8i + 7: 256 consecutive bytes a row.  An 8 x 8 block of
 //     values a lane, transposed in its own registers by v_perm_b32 (half an instruction a value), gives the B operands of 8 MFMAs, the
 //     columns {8i + c} one MFMA each.
-//   * P goes in as two 16-bit numbers, hi + lo: the matrix cores are idle otherwise, and P rounded once (2^-9 in bf16) would be the
-//     largest error of the whole pass.
+//   * P goes in as a sum of 16-bit numbers, three of bf16 (24 bits) or two of f16 (22 bits): the matrix cores are idle otherwise, and P
+//     rounded to one (2^-9 in bf16) or two of bf16 (2^-17) would be the largest error of the whole pass.
 //   * the running maximum moves only when a score passes it by more than 2^8 (2^4 in f16; sums then reach 2^8 a key, far from f32's range), so
 //     the common tile has no reduction across lanes and no rescaling.
 //   * K of the next tile is requested when this tile's scores are done, V when its products are.
@@ -180,7 +180,8 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
     constexpr int  KC    = DK / 32;
     constexpr int  ROWS  = NB * 16, NW = 4;
     // P is taken relative to a reference that lies REF below the maximum when it is set and stays until a score passes that maximum by SLACK (log2 units).
-    // Halves of 16 bits hold P to 2^-16 of itself; f16's end at 2^-25, so there P runs up to 2^15, and what is lost of a row is 2^-36 of the largest.
+    // Three parts of bf16 hold P to 2^-24 of itself, two of f16 to 2^-22; f16's end at 2^-25, so there P runs up to 2^15, and what is lost of a row is 2^-36 of the largest.
+    constexpr int   PARTS = F16 ? 2 : 3;
     constexpr float REF = F16 ? 11.f : 0.f, SLACK = F16 ? 4.f : 8.f;
     using VG = VGeom<DV>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -321,7 +322,7 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
                 }
             }
 
-            u32x4 ph[NB], pl[NB];
+            u32x4 pf[NB][PARTS];
 #pragma unroll
             for (int nb = 0; nb < NB; nb++) {
                 f32x4 sc[2] = { { 0.f, 0.f, 0.f, 0.f }, { 0.f, 0.f, 0.f, 0.f } };
@@ -371,10 +372,13 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
 #pragma unroll
                 for (int e = 0; e < 8; e++) { x[e] = fast_exp2(x[e] - mm); l[nb] += x[e]; }
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    ph[nb][e] = pair16<F16>(x[2 * e], x[2 * e + 1]);
-                    pl[nb][e] = pair16<F16>(x[2 * e] - from16<F16>((unsigned short) ph[nb][e]), x[2 * e + 1] - from16<F16>((unsigned short) (ph[nb][e] >> 16)));
-                }
+                for (int e = 0; e < 4; e++)
+#pragma unroll
+                    for (int part = 0; part < PARTS; part++) {  // what is left of it each time (exact)
+                        const unsigned h = pf[nb][part][e] = pair16<F16>(x[2 * e], x[2 * e + 1]);
+                        x[2 * e]     -= from16<F16>((unsigned short) h);
+                        x[2 * e + 1] -= from16<F16>((unsigned short) (h >> 16));
+                    }
             }
             if (use) {
                 if constexpr (BIAS) {
@@ -394,10 +398,9 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
                     for (int e = 0; e < 4; e++)
                         bf[e] = __builtin_amdgcn_perm(vf[2 * e + 1][c >> 2][(c >> 1) & 1], vf[2 * e][c >> 2][(c >> 1) & 1], c & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-                    for (int nb = 0; nb < NB; nb++) {
-                        acc[nb][c] = mfma16<F16>(ph[nb], bf, acc[nb][c]);
-                        acc[nb][c] = mfma16<F16>(pl[nb], bf, acc[nb][c]);
-                    }
+                    for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                        for (int part = 0; part < PARTS; part++) acc[nb][c] = mfma16<F16>(pf[nb][part], bf, acc[nb][c]);
                 }
             }
             if constexpr (MORE) load_v(i + 1, next);
