@@ -82,7 +82,7 @@ int gqa_norm_rope_launch(const gqa_norm_rope_args * args, void * stream);
 
 /* ---- attention of one new token of every sequence
  * dst[b][h] = sum_i p_i v_i over the sequence's rows i (of KV head h / (n_head / n_head_kv)), p = softmax over i of
- *   s_i = scale * (q . k_i), with a soft cap c > 0: c * tanh(s_i / c), with a mask: + mask[b][i].
+ *   s_i = scale * (q . k_i), with a soft cap c > 0 (any finite one): c * tanh(s_i / c), with a mask: + mask[b][i].
  * Rows i in [0, seq_lens[b]), with window > 0 only the last `window` of them.  A mask of -inf takes the row out whatever its key and value hold (NaN,
  * infinities); a row past the mask's end is out too.  A sequence with no row left (length 0, everything masked) gets zeros.  Lengths
  * below 0 count as 0, above the block table's room as that room.

@@ -26,6 +26,7 @@
 // Measured, 32 query heads on 8 of 128, bf16, a whole call: 32 x 8192 rows 191 us = 5.6 TB/s (head by head 186 = 5.8; a large copy moves 4.9), 64 x 16384
 // 748 us = 5.7 (702 = 6.1), 1 x 1024 rows 11.4 us, latency alone: 6.7 of it this kernel, 4.5 the join.
 
+#include <float.h>
 #include <limits.h>
 #include <math.h>
 
@@ -50,7 +51,7 @@ struct AttnP {
     float * weights; int64_t w_nb1, w_nb2;
     char * dst; int64_t d_nb1, d_nb2; int dst_f32;
     float scale_log2;             // scale * log2(e)
-    float cap_in, cap_out;        // soft cap c: c * tanh(x / c) = c - 2c / (exp2(cap_in * q.k) + 1), times log2(e); cap_out = 0: none
+    float cap_in, cap_out;        // soft cap c: scale / c and c * log2(e); cap_out = 0: none
     int window, n_seq, n_head, n_head_kv, group, row_blocks, head_blocks, dv, quad;
     int rows;                     // heads of a head block, as partial results lie: row_blocks of up to 16 or 32 (128) a KV head, or (quad) four KV heads' groups
     int n_wg;
@@ -162,10 +163,18 @@ __device__ __forceinline__ u32x2 mask4(const AttnP & p, int b, int t, Span s) {
     for (int j = 0; j < 4; j++) h[j] = t + j >= s.first && t + j < s.last ? *(const unsigned short *) (src + 2 * j) : (unsigned short) 0xfc00;
     return u32x2{ h[0] | ((unsigned) h[1] << 16), h[2] | ((unsigned) h[3] << 16) };
 }
-// A score in log2 units from the product q . k, before the mask.
+// A score in log2 units from the product q . k, before the mask.  A soft cap c turns a score s into c tanh(y), y = s / c: 1 - 2 / (e^2y + 1) from y = 3/4 on,
+// of which a small y would keep no digits; there s itself times tanh(y) / y, by Lambert's continued fraction to y^2 / 9 (off by y^10 / 10^7: 6e-9), so that a
+// cap far above the scores leaves them as they are.  Either is off by 2^-21 of itself at most, and they share the reciprocal.
 template <bool BIAS> __device__ __forceinline__ float scaled(const AttnP & p, float a) {
-    if (BIAS && p.cap_out != 0.f) return p.cap_out - 2.f * p.cap_out * __builtin_amdgcn_rcpf(fast_exp2(p.cap_in * a) + 1.f);
-    return p.scale_log2 * a;
+    const float s = p.scale_log2 * a;
+    if (BIAS && p.cap_out != 0.f) {
+        const float y = fabsf(p.cap_in * a), u = y * y;
+        const bool  small = y < 0.75f;
+        const float r = __builtin_amdgcn_rcpf(small ? fmaf(u, fmaf(u, 15.f, 420.f), 945.f) : fast_exp2(2.f * LOG2E * y) + 1.f);
+        return small ? s * (fmaf(u, u + 105.f, 945.f) * r) : copysignf(p.cap_out * fmaf(-2.f, r, 1.f), s);
+    }
+    return s;
 }
 // Page `page` of a pool, at a head's offset (products of 32 bits are the scalar unit's; one of 64 would put the address into vector registers).
 __device__ __forceinline__ const char * page_base(const char * data, int page, unsigned nb_page, int64_t head) {
@@ -981,7 +990,7 @@ extern "C" int gqa_attn_check(const gqa_attn_args * a) {
     if (a->n_seq < 0 || a->n_head < 1 || a->n_head_kv < 1 || a->n_head % a->n_head_kv || a->window < 0 || a->n_workgroups < 0 || a->n_workgroups > 65536) return MLA_ERR_BAD_SHAPE;
     const bool widths = a->dk == 64 || a->dk == 128 || a->dk == 256 ? a->dv == a->dk : (a->dk == 192 && a->dv == 128) || (a->dk == LK && a->dv == 0 && a->n_head_kv == 1);
     if (!widths) return MLA_ERR_UNSUPPORTED;
-    if (!(a->logit_softcap >= 0.f)) return MLA_ERR_UNSUPPORTED;
+    if (!(a->logit_softcap >= 0.f && a->logit_softcap <= FLT_MAX)) return MLA_ERR_UNSUPPORTED;
     if (a->n_seq == 0) return 0;
     if (!a->q || !a->block_table || !a->seq_lens) return MLA_ERR_NULL;
     if (a->n_pages < 1 || a->bt_stride < 1) return MLA_ERR_BAD_SHAPE;
@@ -1029,8 +1038,9 @@ extern "C" int gqa_attn_launch(const gqa_attn_args * a, void * stream) {
     p.weights = a->weights; p.w_nb1 = a->w_nb1; p.w_nb2 = a->w_nb2;
     p.dst = (char *) a->dst; p.d_nb1 = a->d_nb1; p.d_nb2 = a->d_nb2; p.dst_f32 = a->dst_type == MLA_TYPE_F32;
     p.scale_log2 = a->scale * LOG2E;
-    p.cap_in  = a->logit_softcap > 0.f ? 2.f * LOG2E * a->scale / a->logit_softcap : 0.f;
-    p.cap_out = a->logit_softcap * LOG2E;
+    // (a cap so small or large that these leave f32: the largest number does the same)
+    p.cap_in  = a->logit_softcap > 0.f ? fminf(fmaxf(a->scale / a->logit_softcap, -FLT_MAX), FLT_MAX) : 0.f;
+    p.cap_out = fminf(a->logit_softcap * LOG2E, FLT_MAX);
     p.window = a->window; p.n_seq = a->n_seq; p.n_head = a->n_head; p.n_head_kv = a->n_head_kv; p.group = a->n_head / a->n_head_kv;
     p.row_blocks = pl.row_blocks; p.head_blocks = pl.head_blocks; p.rows = pl.rows; p.quad = pl.quad; p.dv = a->dv; p.n_wg = pl.n_wg;
     p.part_o = (float *) ws; p.part_ml = (float2 *) (ws + pl.off_ml); p.items = (int2 *) (ws + pl.off_items);

@@ -12,20 +12,21 @@ pytestmark = pytest.mark.gpu
 EPS32 = 2.0 ** -24
 
 
-def _exact_scores_case(n, width, heads, kv_heads, dk, dv, dtype, seed=0):
-    """One sequence whose scores are known exactly (a query of one 1, keys of one number t = -j / 64, scale 1), whose row i has its weight to itself in column i of
-    128 or fewer: V is one-hot, so a result is the sum of few weights and nothing else."""
+def _exact_scores_case(n, width, heads, kv_heads, dk, dv, dtype, seed=0, step=-1 / 64):
+    """One sequence whose scores are known exactly (a query of one 1, keys of one number t = j * step, j <= 60, scale 1), whose row i has its weight to itself in column
+    i of dv or fewer: V is one-hot, so a result is the sum of few weights and nothing else."""
     gen = torch.Generator().manual_seed(seed)
     q, k, v, bt, lens = _attn_case(seed, [n], width, heads, kv_heads, dk, dv, dtype)
     at = torch.arange(n)
     page, row = bt[0].long()[at // 128], at % 128
-    t = -(torch.randint(0, 61, (n,), generator=gen).double() / 64)
+    t = torch.randint(0 if step < 0 else -60, 61, (n,), generator=gen).double() * step
     q.zero_()
     q[..., 0] = 1
     k[page, row] = 0
     k[page, row, :, 0] = t.to(dtype)[:, None]
-    v[page, row] = 0
-    v[page, row, :, at % dv] = 1
+    if dv:
+        v[page, row] = 0
+        v[page, row, :, at % dv] = 1
     return q, k, v, bt, lens, t
 
 
@@ -47,3 +48,43 @@ def test_attn_weights_of_single_rows(gpu, dtype, dk, dv, heads, kv_heads, width,
     assert n > 128 or rel < 2.0 ** -18.6               # (weights as two bf16 parts are off by 2^-17.5)
     bad = (got - want).abs() > rel * want
     assert not bad.any(), "%d of %d, worst %.3g of its bound" % (int(bad.sum()), bad.numel(), float(((got - want).abs() / (rel * want).clamp_min(1e-300)).max()))
+
+
+CAPS = [1e-38, 1e-3, 0.5, 5.0, 20.0, 50.0, 1e3, 1e6, 1e7, 1e8, 1e30, 3e38]
+
+
+@pytest.mark.parametrize("dk,dv", [(64, 64), (576, 0)])
+@pytest.mark.parametrize("step", [1 / 64, 1 / 8])
+@pytest.mark.parametrize("cap", CAPS)
+def test_attn_softcap_of_any_size(gpu, cap, step, dk, dv):
+    """A cap far above the scores leaves them as they are, one far below makes them equal: weights within 32-bit rounding of c tanh(s / c) for all of them."""
+    import jittorinfer_amd as J
+    n, heads = 64, 2
+    q, k, v, bt, lens, t = _exact_scores_case(n, 2, heads, 1, dk, dv, BF16, step=step)
+    s = cap * torch.tanh(t / cap)
+    p = torch.softmax(s, 0)
+    sums = torch.zeros((1, 1, 256), device=gpu)
+    out = torch.empty((1, heads, dv), dtype=F32, device=gpu) if dv else None
+    J.gqa_attn(*(x.to(gpu) if x is not None else None for x in (q, k, v, bt, lens)), scale=1.0, logit_softcap=cap, weights=sums, out=out)
+    # a capped score is off by 2^-21 of itself (a quotient's reciprocal and exp2 are 2 half steps each, four products and sums), its log2 form and the distance to the
+    # maximum by three half steps more; twice, in the weight and in the one it is compared with; exp2, parts, sum over two heads, joins as above
+    size = float(s.abs().max())
+    rel = 2 * (size * (8 + 2 * 3) + 2 + 4 + 7 + 2) * EPS32
+    for what, got in (("weights", sums[0, 0, :n]), ("out", out[0])) if dv else (("weights", sums[0, 0, :n]),):
+        got = got.cpu().double()
+        got = got / got[..., p.argmax()][..., None]
+        bad = (got - p / p.max()).abs() > rel * p / p.max()
+        assert not bad.any(), "%s: %d of %d, worst %.3g of its bound" % (what, int(bad.sum()), bad.numel(), float(((got - p / p.max()).abs() / (rel * p / p.max())).max()))
+    assert abs(float(sums.double().sum()) - heads) < heads * (n + 10) * EPS32 and (sums[0, 0, n:] == 0).all()
+
+
+@pytest.mark.parametrize("scale", [-0.125, 1e-6, 30.0])
+def test_attn_softcap_with_other_scales(gpu, scale):
+    """Scores of either sign from a negative scale, all far below the cap, and all at it."""
+    import jittorinfer_amd as J
+    q, k, v, bt, lens = _attn_case(50, [200, 1], 2, 4, 2, 64, 64, F16)
+    out, off, w, w_off = R.attn(q, k, v, bt, lens.tolist(), scale, 30.0)
+    sums = torch.zeros((2, 2, 256), device=gpu)
+    got = J.gqa_attn(*(x.to(gpu) for x in (q, k, v, bt, lens)), scale=scale, logit_softcap=30.0, weights=sums)
+    _near(got, out, off, F16)
+    _near(sums, w, w_off, F32)
