@@ -124,7 +124,7 @@ def native():
                  "mla_mul_mat_launch", "mla_copy_f32_launch", "mla_front_batch_launch", "gqa_norm_rope_launch", "gqa_attn_workspace_size",
                  "gqa_attn_launch", "gqa_evict_workspace_size", "gqa_evict_launch")
         mod.bind(*[C.cast(getattr(lib, n), C.c_void_p).value for n in names], _workspace, _workspaces, torch._C._cuda_getCurrentRawStream,
-                 torch._C._cuda_isCurrentStreamCapturing)
+                 torch._C._cuda_isCurrentStreamCapturing, _scratch_elsewhere)
         _native = mod
     return _native
 
@@ -147,7 +147,8 @@ def _workspace(device, nbytes, stream=None):
     queued earlier or recorded into a HIP graph keeps its address, so a larger request gets a new area and the old one is retired.
     Areas grow by at least half (requests that creep up -- a decode loop adding one key per step -- retire O(log size) areas, not
     one per step); release_workspaces() drops what has been retired.  Under graph capture the new area comes from the graph's own
-    memory pool, like any tensor made during capture."""
+    memory pool, like any tensor made during capture.  An area is allocated as its own stream's: a block that the allocator holds for
+    another stream may be free only to work queued there."""
     import torch
     if stream is None:
         stream = torch.cuda.current_stream(device).cuda_stream
@@ -158,9 +159,29 @@ def _workspace(device, nbytes, stream=None):
         if ws is not None:
             _retired.append(ws)
             have = ws.numel()
-        ws = torch.empty(max(nbytes, have + have // 2, 1 << 20), dtype=torch.uint8, device=device)
+        size = max(nbytes, have + have // 2, 1 << 20)
+        if int(stream) == torch.cuda.current_stream(device).cuda_stream:
+            ws = torch.empty(size, dtype=torch.uint8, device=device)
+        else:
+            with torch.cuda.stream(_stream(device, stream)):
+                ws = torch.empty(size, dtype=torch.uint8, device=device)
         _workspaces[key] = ws
     return ws
+
+
+def _stream(device, handle):
+    import torch
+    return torch.cuda.ExternalStream(int(handle), device=device) if handle else torch.cuda.default_stream(device)
+
+
+def _scratch_elsewhere(device, nbytes, stream):
+    """The scratch of a launch on another stream than the current one: what a call with that stream as the current one would take -- its area, or,
+    where that stream is being captured, memory of the graph, which the allocator gives on within that stream's part of the graph only."""
+    import torch
+    with torch.cuda.stream(_stream(device, stream)):
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(nbytes, dtype=torch.uint8, device=device)
+        return _workspace(device, nbytes, stream)
 
 
 def release_workspaces(stream=None, device=None):

@@ -60,7 +60,7 @@ struct Bound {
     decltype(&gqa_attn_launch)         gqa_attn;
     decltype(&gqa_evict_workspace_size) evict_workspace_size;
     decltype(&gqa_evict_launch)        evict;
-    PyObject * workspace, * workspaces, * raw_stream, * capturing;
+    PyObject * workspace, * workspaces, * raw_stream, * capturing, * elsewhere;
 } lib;
 
 #define REQUIRE(cond)                                        \
@@ -430,32 +430,48 @@ gqa_pool pool_of(const at::Tensor & c) {
     const int64_t es = (int64_t) c.element_size();
     return gqa_pool{ c.data_ptr(), c.stride(0) * es, c.stride(1) * es, c.stride(2) * es };
 }
-// The stream to launch on.  What a call makes for itself (results, scratch) belongs to the device's current stream, so a call on another one
+// The stream to launch on.  The result tensors a call makes for itself belong to the device's current stream, so a call on another one
 // brings its own (`makes` = false).
-bool gqa_stream(PyObject * o, const at::Tensor & t, bool makes, void *& st) {
-    if (!stream_of(Py_None, t, st)) return false;
-    if (o == Py_None) return true;
-    void * const current = st;
-    if (!stream_of(o, t, st)) return false;
-    if (!makes || st == current) return true;
-    PyErr_SetString(PyExc_ValueError, "a launch on another stream than the current one takes its result tensors from the caller");
-    return false;
-}
-// Scratch of a launch.  Under graph capture it is the graph's own: two graphs captured on one stream may be replayed side by side.
+struct GqaStream {
+    void * st;
+    bool   current;
+    bool take(PyObject * o, const at::Tensor & t, bool makes) {
+        if (!stream_of(Py_None, t, st)) return false;
+        current = true;
+        if (o == Py_None) return true;
+        void * const now = st;
+        if (!stream_of(o, t, st)) return false;
+        current = st == now;
+        if (!makes || current) return true;
+        PyErr_SetString(PyExc_ValueError, "a launch on another stream than the current one takes its result tensors from the caller");
+        return false;
+    }
+};
+// Scratch of a launch, the launch's stream's own.  Under graph capture it is the graph's: two graphs captured on one stream may be replayed side by side.
 struct GqaScratch {
     THPObjectPtr ws;
     at::Tensor   own;
-    template <typename Args> bool take(PyObject * o, const at::Tensor & t, void * st, size_t need, Args & a) {
+    template <typename Args> bool take(PyObject * o, const at::Tensor & t, const GqaStream & s, size_t need, Args & a) {
+        if (!need) return true;
+        if (!s.current) {
+            THPObjectPtr dev(PyObject_GetAttrString(o, "device")), n(PyLong_FromSize_t(need)), handle(PyLong_FromVoidPtr(s.st));
+            if (!dev || !n || !handle) return false;
+            ws = THPObjectPtr(PyObject_CallFunctionObjArgs(lib.elsewhere, dev.get(), n.get(), handle.get(), nullptr));
+            if (!ws) return false;
+            if (!THPVariable_Check(ws.get())) { PyErr_SetString(PyExc_TypeError, "expected a torch tensor"); return false; }
+            const at::Tensor & w = THPVariable_Unpack(ws.get());
+            a.workspace = w.data_ptr(); a.workspace_size = (size_t) w.numel();
+            return true;
+        }
         THPObjectPtr capturing(PyObject_CallNoArgs(lib.capturing));
         if (!capturing) return false;
         if (capturing.get() == Py_True) {
             own = at::empty({ (int64_t) need }, t.options().dtype(at::kByte));
             a.workspace = own.data_ptr(); a.workspace_size = need;
-        } else if (need) {
-            ws = workspace(o, st, need, a);
-            return (bool) ws;
+            return true;
         }
-        return true;
+        ws = workspace(o, s.st, need, a);
+        return (bool) ws;
     }
 };
 #define SAME_DEVICE(t) REQUIRE(!(t) || (t)->device() == q.device())
@@ -515,8 +531,8 @@ PyObject * gqa_norm_rope(PyObject *, PyObject * const * o, Py_ssize_t n) {
         }
     } else REQUIRE(!v && !kc && !vc && !kw);
     const c10::DeviceGuard guard(q.device());
-    void * st;
-    if (!gqa_stream(o[23], q, !outp, st)) return nullptr;
+    GqaStream stream;
+    if (!stream.take(o[23], q, !outp)) return nullptr;
     at::Tensor made;
     if (!outp) { made = at::empty(q.sizes(), q.options().dtype(kc ? kc->scalar_type() : q.scalar_type())); outp = &made; }
     const at::Tensor & out = *outp;
@@ -524,7 +540,7 @@ PyObject * gqa_norm_rope(PyObject *, PyObject * const * o, Py_ssize_t n) {
     REQUIRE(a.dst_type >= 0 && out.sizes() == q.sizes() && rows_ok(out, 3, true));
     const int64_t od = (int64_t) out.element_size();
     a.q_dst = out.data_ptr(); a.qd_nb1 = out.stride(1) * od; a.qd_nb2 = out.stride(0) * od;
-    const int rc = unlocked([&] { return lib.norm_rope(&a, st); });
+    const int rc = unlocked([&] { return lib.norm_rope(&a, stream.st); });
     if (rc) return failed("gqa_norm_rope_launch", rc);
     return made.defined() ? THPVariable_Wrap(made) : Py_NewRef(o[17]);
 }
@@ -567,8 +583,8 @@ PyObject * gqa_attn(PyObject *, PyObject * const * o, Py_ssize_t n) {
         a.weights = (float *) weights->data_ptr(); a.w_nb1 = weights->stride(1) * 4; a.w_nb2 = weights->stride(0) * 4;
     }
     const c10::DeviceGuard guard(q.device());
-    void * st;
-    if (!gqa_stream(o[12], q, vc && !outp, st)) return nullptr;
+    GqaStream stream;
+    if (!stream.take(o[12], q, vc && !outp)) return nullptr;
     at::Tensor made;
     if (vc) {
         if (!outp) { made = at::empty({ n_seq, n_head, (int64_t) a.dv }, q.options()); outp = &made; }
@@ -580,8 +596,8 @@ PyObject * gqa_attn(PyObject *, PyObject * const * o, Py_ssize_t n) {
     } else a.dst_type = MLA_TYPE_F32;
     const size_t need = lib.gqa_workspace_size(&a);
     GqaScratch scratch;
-    if (!scratch.take(o[0], q, st, need, a)) return nullptr;
-    const int rc = unlocked(a.workspace, [&] { return lib.gqa_attn(&a, st); });
+    if (!scratch.take(o[0], q, stream, need, a)) return nullptr;
+    const int rc = unlocked(a.workspace, [&] { return lib.gqa_attn(&a, stream.st); });
     if (rc) return failed("gqa_attn_launch", rc);
     return made.defined() ? THPVariable_Wrap(made) : Py_NewRef(vc ? o[10] : o[9]);
 }
@@ -612,8 +628,8 @@ PyObject * gqa_evict(PyObject *, PyObject * const * o, Py_ssize_t n) {
     REQUIRE(q.scalar_type() == at::kFloat && rows_ok(q, 3, false) && q.size(0) == n_seq && q.size(1) == a.n_head_kv && q.size(2) == cap);
     a.weights = (const float *) q.data_ptr(); a.w_nb1 = q.stride(1) * 4; a.w_nb2 = q.stride(0) * 4;
     const c10::DeviceGuard guard(q.device());
-    void * st;
-    if (!gqa_stream(o[11], q, !wop || !keptp || !newp, st)) return nullptr;
+    GqaStream stream;
+    if (!stream.take(o[11], q, !wop || !keptp || !newp)) return nullptr;
     at::Tensor wo = wop ? *wop : at::empty({ n_seq, (int64_t) a.n_head_kv, cap }, q.options());
     REQUIRE(a.n_keep >= 0);
     at::Tensor kept = keptp ? *keptp : at::empty({ n_seq, (int64_t) a.n_head_kv, (int64_t) a.n_keep }, q.options().dtype(at::kInt));
@@ -624,20 +640,20 @@ PyObject * gqa_evict(PyObject *, PyObject * const * o, Py_ssize_t n) {
     a.weights_dst = (float *) wo.data_ptr(); a.wd_nb1 = wo.stride(1) * 4; a.wd_nb2 = wo.stride(0) * 4;
     a.kept = (int32_t *) kept.data_ptr(); a.new_lens = (int32_t *) fresh.data_ptr();
     GqaScratch scratch;
-    if (!scratch.take(o[0], q, st, lib.evict_workspace_size(&a), a)) return nullptr;
-    const int rc = unlocked(a.workspace, [&] { return lib.evict(&a, st); });
+    if (!scratch.take(o[0], q, stream, lib.evict_workspace_size(&a), a)) return nullptr;
+    const int rc = unlocked(a.workspace, [&] { return lib.evict(&a, stream.st); });
     if (rc) return failed("gqa_evict_launch", rc);
     THPObjectPtr r0(keptp ? Py_NewRef(o[9]) : THPVariable_Wrap(kept)), r1(newp ? Py_NewRef(o[10]) : THPVariable_Wrap(fresh)), r2(wop ? Py_NewRef(o[8]) : THPVariable_Wrap(wo));
     return r0 && r1 && r2 ? PyTuple_Pack(3, r0.get(), r1.get(), r2.get()) : nullptr;
 }
 
-// bind(addresses of the thirteen entry points in Bound's order, workspace function, workspace table, torch's raw current stream, whether it is capturing)
+// bind(addresses of the thirteen entry points in Bound's order, workspace function, workspace table, torch's raw current stream, whether it is capturing, scratch on another stream)
 PyObject * bind(PyObject *, PyObject * const * v, Py_ssize_t n) {
-    if (!arg_count(n, 17)) return nullptr;
+    if (!arg_count(n, 18)) return nullptr;
     void * p[13];
     for (int i = 0; i < 13; i++) p[i] = PyLong_AsVoidPtr(v[i]);
     if (PyErr_Occurred()) return nullptr;
-    REQUIRE(PyCallable_Check(v[13]) && PyDict_Check(v[14]) && PyCallable_Check(v[15]) && PyCallable_Check(v[16]));
+    REQUIRE(PyCallable_Check(v[13]) && PyDict_Check(v[14]) && PyCallable_Check(v[15]) && PyCallable_Check(v[16]) && PyCallable_Check(v[17]));
     lib.workspace_size = (decltype(lib.workspace_size)) p[0]; lib.attn = (decltype(lib.attn)) p[1];
     lib.kv_write = (decltype(lib.kv_write)) p[2]; lib.kv_write_rope = (decltype(lib.kv_write_rope)) p[3];
     lib.rope = (decltype(lib.rope)) p[4]; lib.mul_mat = (decltype(lib.mul_mat)) p[5];
@@ -645,7 +661,7 @@ PyObject * bind(PyObject *, PyObject * const * v, Py_ssize_t n) {
     lib.norm_rope = (decltype(lib.norm_rope)) p[8]; lib.gqa_workspace_size = (decltype(lib.gqa_workspace_size)) p[9];
     lib.gqa_attn = (decltype(lib.gqa_attn)) p[10]; lib.evict_workspace_size = (decltype(lib.evict_workspace_size)) p[11];
     lib.evict = (decltype(lib.evict)) p[12];
-    lib.workspace = Py_NewRef(v[13]); lib.workspaces = Py_NewRef(v[14]); lib.raw_stream = Py_NewRef(v[15]); lib.capturing = Py_NewRef(v[16]);
+    lib.workspace = Py_NewRef(v[13]); lib.workspaces = Py_NewRef(v[14]); lib.raw_stream = Py_NewRef(v[15]); lib.capturing = Py_NewRef(v[16]); lib.elsewhere = Py_NewRef(v[17]);
     Py_RETURN_NONE;
 }
 

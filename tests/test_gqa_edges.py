@@ -12,3 +12,32 @@ def test_softcaps_are_finite(cap, code):
     """c tanh(s / c) has no value at an infinite c."""
     for a in (_attn(logit_softcap=cap), _latent(logit_softcap=cap)):
         assert J.library().gqa_attn_check(C.byref(a)) == code
+
+
+def test_scratch_is_allocated_as_its_own_streams(monkeypatch):
+    """An area for a stream that is not the current one is allocated with that stream as the current one (a stand-in for torch's allocator, on the CPU)."""
+    import contextlib
+    import sys
+    import types
+    import jittorinfer_amd.capi as capi
+
+    now, made = [7], []
+
+    @contextlib.contextmanager
+    def stream(s):
+        now.append(s)
+        yield
+        now.pop()
+    cuda = types.SimpleNamespace(current_stream=lambda d: types.SimpleNamespace(cuda_stream=now[-1]), stream=stream, ExternalStream=lambda h, device=None: h,
+                                 default_stream=lambda d: 0, is_current_stream_capturing=lambda: now[-1] == 11)
+    fake = types.SimpleNamespace(uint8=None, cuda=cuda, empty=lambda n, dtype=None, device=None: made.append(now[-1]) or types.SimpleNamespace(numel=lambda: n))
+    monkeypatch.setitem(sys.modules, "torch", fake)
+    monkeypatch.setattr(capi, "_workspaces", {})
+    monkeypatch.setattr(capi, "_retired", [])
+    for s in (7, 9, 0):
+        ws = capi._workspace("dev", 1 << 21, stream=s)
+        assert capi._workspace("dev", 1 << 20, stream=s) is ws and now == [7]
+    assert capi._scratch_elsewhere("dev", 1 << 21, 9) is capi._workspaces["dev", 9]
+    assert made == [7, 9, 0]
+    own = capi._scratch_elsewhere("dev", 100, 11)                    # under capture: the graph's own, kept in no table
+    assert made == [7, 9, 0, 11] and own.numel() == 100 and ("dev", 11) not in capi._workspaces and now == [7]

@@ -88,3 +88,105 @@ def test_attn_softcap_with_other_scales(gpu, scale):
     got = J.gqa_attn(*(x.to(gpu) for x in (q, k, v, bt, lens)), scale=scale, logit_softcap=30.0, weights=sums)
     _near(got, out, off, F16)
     _near(sums, w, w_off, F32)
+
+
+def test_scratch_of_another_stream_is_not_this_ones(gpu):
+    """A stream's first area is no block that the allocator keeps for work queued on the current stream."""
+    from jittorinfer_amd import capi
+    size = 96 << 20
+    side = torch.cuda.Stream()
+    old = torch.empty(size, dtype=torch.uint8, device=gpu)
+    held = old.data_ptr()
+    del old                                                           # free again, to the current stream's later work
+    ws = capi._workspace(gpu, size, side.cuda_stream)
+    again = torch.empty(size, dtype=torch.uint8, device=gpu)
+    assert again.data_ptr() == held and ws.data_ptr() != held
+    capi.release_workspaces(side.cuda_stream, gpu)
+
+
+def test_forked_branches_of_one_capture(gpu):
+    """Calls on the current stream and, through stream=, on a side stream of the same capture run side by side at every replay: neither uses the other's scratch."""
+    import jittorinfer_amd as J
+    cases = [[t.to(gpu) for t in _attn_case(51 + i, [1024, 600, 1000, 128 + i], 8, 8, 2, 128, 128, BF16)] for i in range(4)]
+    want = [J.gqa_attn(*c, scale=0.1) for c in cases]
+    outs = [torch.empty_like(w) for w in want]
+    sums = [torch.zeros((4, 2, 1024), device=gpu) for _ in cases]
+    want_sums = [torch.zeros_like(s) for s in sums]
+    for c, s in zip(cases, want_sums):
+        J.gqa_attn(*c, scale=0.1, weights=s)
+    cut = _evict_on(gpu, 60)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        fork = torch.cuda.Event()
+        fork.record()
+        side.wait_event(fork)
+        for i, c in enumerate(cases):
+            J.gqa_attn(*c, scale=0.1, weights=sums[i], out=outs[i], stream=side.cuda_stream if i % 2 else None)
+        cut["run"](stream=side.cuda_stream)
+        torch.cuda.current_stream().wait_stream(side)
+    for step in range(4):
+        for o, s in zip(outs, sums):
+            o.fill_(float("nan"))
+            s.zero_()
+        cut["reset"]()
+        J.gqa_attn(*cases[0], scale=0.1)                               # eager work between the replays
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want)) and all(torch.equal(a, b) for a, b in zip(sums, want_sums)), step
+        cut["check"]()
+
+
+def _evict_on(gpu, seed):
+    """An eviction with its results made ahead: run(stream=), reset() and check() against the plain form."""
+    import jittorinfer_amd as J
+    from tests.test_gqa_gpu import _evict_case
+    w, bt, lens, k, v = _evict_case(seed, [700, 1000, 90], 8, 2, 64, 64, BF16)
+    want = R.evict(w, bt, lens.tolist(), k, v, 300, 4, 30)
+    d = [t.to(gpu) for t in (w, bt, lens, k, v)]
+    outs = dict(weights_out=torch.empty_like(d[0]), kept=torch.empty((3, 2, 300), dtype=torch.int32, device=gpu), new_lens=torch.empty(3, dtype=torch.int32, device=gpu))
+
+    def check():
+        assert torch.equal(outs["kept"].cpu(), want[0]) and torch.equal(outs["new_lens"].cpu(), want[1]) and torch.equal(outs["weights_out"].cpu(), want[2])
+        assert torch.equal(R.bits(d[3].cpu()), R.bits(want[3])) and torch.equal(R.bits(d[4].cpu()), R.bits(want[4]))
+    return dict(run=lambda **kw: J.gqa_evict(*d, n_keep=300, n_sink=4, n_recent=30, **outs, **kw), check=check, reset=lambda: (d[3].copy_(k), d[4].copy_(v)))
+
+
+def test_calls_on_a_captured_stream_that_is_not_the_current_one(gpu):
+    """A capture on one stream, the call made while another is the current one: scratch is the graph's, not the area that eager calls of the stream share."""
+    import jittorinfer_amd as J
+    from jittorinfer_amd import capi
+    c = [t.to(gpu) for t in _attn_case(55, [1024, 600], 8, 8, 2, 128, 128, F16)]
+    want, out = J.gqa_attn(*c, scale=0.1), torch.empty((2, 8, 128), dtype=F16, device=gpu)
+    inner, other = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=inner):
+        with torch.cuda.stream(other):
+            J.gqa_attn(*c, scale=0.1, out=out, stream=inner.cuda_stream)
+    assert (gpu, inner.cuda_stream) not in capi._workspaces
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+def test_side_stream_calls_without_waiting(gpu):
+    """Eager calls on a side stream through stream=, ordered by events alone, while the current stream goes on allocating."""
+    import jittorinfer_amd as J
+    c = [t.to(gpu) for t in _attn_case(56, [1024, 600, 30], 8, 8, 2, 128, 128, BF16)]
+    want = J.gqa_attn(*c, scale=0.1)
+    outs = [torch.empty_like(want) for _ in range(20)]
+    cuts = _evict_on(gpu, 61)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for i, out in enumerate(outs):
+        J.gqa_attn(*c, scale=0.1, out=out, stream=side.cuda_stream)
+        torch.full((1 << 20,), float(i), device=gpu).add_(1.0)
+        assert torch.equal(J.gqa_attn(*c, scale=0.1), want)
+    cuts["run"](stream=side.cuda_stream)
+    side.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+    cuts["check"]()
