@@ -9,7 +9,6 @@
 #include <string.h>
 
 #include <algorithm>
-#include <mutex>
 #include <vector>
 
 #include <ATen/ops/empty.h>
@@ -22,6 +21,7 @@
 #include "../../include/mla_attn.h"
 #include "../../include/mla_front.h"
 #include "../../include/mla_kv_write.h"
+#include "scratch_lock.hpp"
 
 namespace {
 
@@ -37,11 +37,10 @@ template <typename F> int unlocked(F f) {
     return f();
 }
 // The same for a launch of several kernels that hand each other scratch: two threads on one stream share it, and the kernels of one call must
-// not be queued between those of another.  One lock per scratch area, by its address.
+// not be queued between those of another.
 template <typename F> int unlocked(const void * scratch, F f) {
-    static std::mutex locks[64];
     const Unlocked u;
-    const std::lock_guard<std::mutex> l(locks[((uintptr_t) scratch >> 9) % 64]);
+    const mla::ScratchLock l(scratch);
     return f();
 }
 

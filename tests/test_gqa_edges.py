@@ -1,10 +1,12 @@
 """The paged cache of ordinary heads without a GPU, at its edges: what the entry points of include/gqa_attn.h refuse and accept beside tests/test_gqa.py."""
 import ctypes as C
+import os
+import subprocess
 
 import pytest
 
 import jittorinfer_amd as J
-from tests.test_gqa import SHAPE, UNSUPPORTED, _attn, _cut, _latent, _pool, _rows
+from tests.test_gqa import ROOT, SHAPE, UNSUPPORTED, _attn, _cut, _latent, _pool, _rows
 
 
 @pytest.mark.parametrize("cap,code", [(float("inf"), UNSUPPORTED), (float("nan"), UNSUPPORTED), (3.4e38, 0), (1e-45, 0)])
@@ -41,3 +43,28 @@ def test_scratch_is_allocated_as_its_own_streams(monkeypatch):
     assert made == [7, 9, 0]
     own = capi._scratch_elsewhere("dev", 100, 11)                    # under capture: the graph's own, kept in no table
     assert made == [7, 9, 0, 11] and own.numel() == 100 and ("dev", 11) not in capi._workspaces and now == [7]
+
+
+def test_scratch_areas_have_locks_of_their_own(tmp_path):
+    """Areas as the allocator places them (2 MB apart and further, or 512 bytes) do not wait for each other; the same area does, and no area holds nothing."""
+    src = tmp_path / "t.cpp"
+    src.write_text(r"""
+#include "scratch_lock.hpp"
+#include <set>
+#include <thread>
+int main() {
+    for (uint64_t base : { 0x7f0000000000ull, 0x7e1c40000000ull }) for (uint64_t step : { 512ull, 1ull << 21, 1ull << 23, 1ull << 26, 1ull << 30 }) {
+        std::set<unsigned> seen;
+        for (uint64_t i = 0; i < 16; i++) seen.insert(mla::scratch_lock_index((const void *) (base + i * step)));
+        if (seen.size() < 14) return 1;
+        for (unsigned i : seen) if (i >= 256) return 2;
+    }
+    { const mla::ScratchLock a(nullptr), b(nullptr); const mla::ScratchLock c((const void *) 0x7f0000200000ull); }
+    int inside = 0, most = 0, done = 0;
+    auto work = [&] { for (int i = 0; i < 20000; i++) { const mla::ScratchLock l((const void *) 0x7f0000200000ull); most = ++inside > most ? inside : most; --inside; done++; } };
+    std::thread t(work); work(); t.join();
+    return most == 1 && done == 40000 ? 0 : 3;
+}
+""")
+    subprocess.run(["g++", "-std=c++17", "-O2", "-Wall", "-Werror", "-I", os.path.join(ROOT, "jittorinfer_amd", "csrc"), str(src), "-o", str(tmp_path / "t"), "-pthread"], check=True)
+    assert subprocess.run([str(tmp_path / "t")], timeout=60).returncode == 0
