@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(64 * LWAVES) gqa_scores_kernel(const AttnP p) 
 #pragma unroll 1
         for (int k0 = 0; k0 < last; k0 += 6) stage(k0, [] {});
         stage(last, [&] { load_k(min(i, n - 1), good(id) ? id : 0); });           // (a wave without a page of its own: the last one's, unused)
-        // (a wave's own rows of sh_ml hold its running maxima and sums: LDS operations of a wave stay in order)
+        // (a wave's own rows of sh_ml hold its running maxima and sums; what lanes 0 .. 15 write of a page the others read with the next one: a fence between)
         for (int r = lane; r < LROWS; r += 64) sh_ml[wave][r] = make_float2(-INFINITY, 0.f);
         __syncthreads();
 
@@ -649,6 +649,7 @@ __global__ void __launch_bounds__(64 * LWAVES) gqa_scores_kernel(const AttnP p) 
                 l += __shfl_xor(l, 32, 64);
                 if (lg == 0) sh_ml[wave][h] = make_float2(top, l + (ml.y == 0.f ? 0.f : ml.y * fast_exp2(ml.x - mm)));
             }
+            wave_fence();
             if (i + LWAVES / 4 < n) load_k(i + LWAVES / 4, good(id) ? id : 0);
         }
         __syncthreads();

@@ -34,6 +34,12 @@ __device__ __forceinline__ int scan_wave(int v) {
 // The value of lane `lane`, the same in every lane of the wave (`lane` too).
 __device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
+// What lanes of a wave have written to LDS is there for its other lanes, and what they have read may be overwritten.
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 inline bool al16(const void * ptr) { return ((uintptr_t) ptr & 15) == 0; }
 
 }  // namespace gqa

@@ -190,3 +190,9 @@ def test_side_stream_calls_without_waiting(gpu):
     side.synchronize()
     assert all(torch.equal(o, want) for o in outs)
     cuts["check"]()
+
+
+@pytest.mark.parametrize("heads", [1, 16, 40, 128])
+def test_weights_of_many_pages_a_unit(gpu, heads):
+    """A latent cache's running maxima and sums, handed from page to page of a unit."""
+    _check_attn(gpu, *_attn_case(81, [2500, 2177, 300], 20, heads, 1, 576, 0, BF16), n_workgroups=4)
