@@ -108,6 +108,12 @@ __device__ __forceinline__ void count_rows(const Group & g, int i0, const float 
             atomicAdd(&hist[(k >> shift_of(pass)) & ((1u << bits_of(pass)) - 1)], 1u);
     }
 }
+// The 8 rows are in registers before anything that follows (a barrier, or a flag, that lets others overwrite them): the compiler may otherwise leave a load under
+// way whose number it needs last.
+__device__ __forceinline__ void pin_rows(float (&x)[SEL_PER]) {
+#pragma unroll
+    for (int e = 0; e < SEL_PER; e++) asm volatile("" : "+v"(x[e]) :: "memory");
+}
 // Of 8 rows: those that stay whatever the others do (bits 0 .. 7), and those equal to the smallest weight that stays, `last` (bits 16 ..).
 __device__ __forceinline__ unsigned sort_rows(const Group & g, int i0, const float (&x)[SEL_PER], unsigned last) {
     unsigned m = 0;
@@ -195,6 +201,7 @@ __global__ void __launch_bounds__(SEL_THREADS) gqa_select_kernel(const EvictP p)
             m[r] = base + r * SEL_RUN < g.n ? sort_rows(g, base + r * SEL_RUN + tid * SEL_PER, x[r], got.digit) : 0u;
             incl[r] = scan_wave(count_both(m[r]));           // (at most 8192 of either in a run)
             if (lane == 63) part[r][wave] = incl[r];
+            if (base + r * SEL_RUN < g.n) pin_rows(x[r]);
         }
         __syncthreads();                                           // (also: every row of the chunk has been read before one is overwritten)
 #pragma unroll
@@ -294,6 +301,7 @@ __global__ void __launch_bounds__(SEL_THREADS) gqa_rank_kernel(const EvictP p, c
         const unsigned m = sort_rows(g, i0, x, got.digit);
         const int incl = scan_wave(count_both(m));
         if (lane == 63) part[wave] = incl;
+        pin_rows(x);
         __syncthreads();                                           // (every row of the run is in a register: it may be overwritten from here on)
         const int upto = scan_wave(lane < 16 ? part[lane] : 0);
         const int all = lane_of(upto, 15), ahead = wave ? lane_of(upto, wave - 1) : 0;

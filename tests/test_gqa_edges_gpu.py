@@ -192,6 +192,52 @@ def test_side_stream_calls_without_waiting(gpu):
     cuts["check"]()
 
 
+@pytest.mark.parametrize("heads,dk,dv", [(2, 32, 16), (5, 16, 16), (8, 16, 0)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_evict_many_heads_selected_by_several_workgroups(gpu, heads, dk, dv, in_place):
+    """Block tables of more than 24576 rows with several KV heads, K and V with room between their heads and rows, weights with room between theirs; lengths that end
+    inside a run of 8192, at its end, and below what is kept; sinks and recent rows that fill whole runs."""
+    import jittorinfer_amd as J
+    from tests.test_gqa_gpu import _evict_case
+    lens, width = [33000, 24577, 16384, 9000, 100], 260
+    assert len(lens) * heads <= 64                        # (as many groups as the rule takes)
+    w, bt, lens, k, v = _evict_case(70 + heads, lens, width, heads, dk, dv, BF16)
+    w[0, 0] = 1.0                                         # one head all ties
+    gen = torch.Generator().manual_seed(heads)
+    w[1, -1] = torch.randint(0, 3, (width * 128,), generator=gen).float()
+    for n_keep, n_sink, n_recent in ((9000, 4, 500), (20000, 8200, 9000), (24576, 0, 0)):
+        want = R.evict(w, bt, lens.tolist(), k, v, n_keep, n_sink, n_recent)
+        kk = torch.full((k.shape[0], 128, heads, dk + 8), 3.0, dtype=BF16, device=gpu)
+        kk[..., :dk] = k.to(gpu)
+        vv = None
+        if dv:
+            vv = torch.full((v.shape[0], 130, heads + 1, dv), 3.0, dtype=BF16, device=gpu)
+            vv[:, :128, :heads] = v.to(gpu)
+        ww = torch.full((len(lens), heads + 1, width * 128 + 12), 7.0, device=gpu)
+        ww[:, :heads, 4:4 + width * 128] = w.to(gpu)
+        ws = ww[:, :heads, 4:4 + width * 128]
+        kept, new, out = J.gqa_evict(ws, bt.to(gpu), lens.to(gpu), kk[..., :dk], vv[:, :128, :heads] if dv else None, n_keep=n_keep, n_sink=n_sink, n_recent=n_recent,
+                                     weights_out=ws if in_place else None)
+        torch.cuda.synchronize()
+        assert torch.equal(kept.cpu(), want[0]) and torch.equal(new.cpu(), want[1]), (n_keep, n_sink)
+        assert torch.equal(out.cpu(), want[2])
+        assert torch.equal(kk[..., :dk].cpu(), want[3]) and (kk[..., dk:] == 3).all()
+        if dv:
+            assert torch.equal(vv[:, :128, :heads].cpu(), want[4]) and (vv[:, 128:] == 3).all() and (vv[:, :, heads:] == 3).all()
+        assert (ww[:, heads:] == 7).all() and (ww[..., :4] == 7).all() and (ww[..., 4 + width * 128:] == 7).all()
+        assert in_place or torch.equal(ws.cpu(), w)
+
+
+@pytest.mark.parametrize("n_sink,n_recent", [(3000, 100), (100, 3000), (2000, 2000)])
+def test_evict_in_place_of_held_rows(gpu, n_sink, n_recent):
+    """Weights of rows that stay whatever they weigh move down over rows that other threads hold: one workgroup a group, one chunk and two."""
+    from tests.test_gqa_gpu import _evict_case
+    for width, n in ((40, 5000), (190, 24000)):
+        w, bt, lens, k, _ = _evict_case(80, [n, n - 37], width, 2, 16, 0, BF16)
+        for n_keep in (4000, n - 40):
+            _check_evict(gpu, w, bt, lens, k, None, n_keep, n_sink, n_recent, in_place=True)
+
+
 @pytest.mark.parametrize("heads", [1, 16, 40, 128])
 def test_weights_of_many_pages_a_unit(gpu, heads):
     """A latent cache's running maxima and sums, handed from page to page of a unit."""
