@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(SEL_THREADS) gqa_select_kernel(const EvictP p)
     if (blockIdx.x % p.n_head_kv == 0 && tid == 0) p.new_lens[blockIdx.x / p.n_head_kv] = min(g.n, p.n_keep);
     for (int i = blockIdx.x * SEL_THREADS + tid; i < p.n_sync; i += gridDim.x * SEL_THREADS) p.sync[i] = 0u;
     if (g.n <= p.n_keep) {                                         // nothing leaves
-        for (int i = tid; i < p.n_keep; i += SEL_THREADS) g.kept[i] = i < g.n ? i : -1;
+        for (int64_t i = tid; i < p.n_keep; i += SEL_THREADS) g.kept[i] = i < g.n ? (int) i : -1;      // (n_keep up to 2^31 - 1)
         for (int64_t i = tid; i < p.cap; i += SEL_THREADS) g.wd[i] = i < g.n ? g.w[i] : 0.f;
         return;
     }

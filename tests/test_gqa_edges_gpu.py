@@ -242,3 +242,18 @@ def test_evict_in_place_of_held_rows(gpu, n_sink, n_recent):
 def test_weights_of_many_pages_a_unit(gpu, heads):
     """A latent cache's running maxima and sums, handed from page to page of a unit."""
     _check_attn(gpu, *_attn_case(81, [2500, 2177, 300], 20, heads, 1, 576, 0, BF16), n_workgroups=4)
+
+
+def test_evict_keeps_as_many_as_there_may_be(gpu):
+    """n_keep of 2^31 - 1: nothing leaves, every place past the length is marked."""
+    import jittorinfer_amd as J
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    w, n = torch.rand((1, 1, 256), device=gpu), 200
+    k = torch.rand((2, 128, 1, 16), device=gpu).to(BF16)
+    before = k.clone()
+    kept, new, out = J.gqa_evict(w, torch.tensor([[1, 0]], dtype=torch.int32, device=gpu), torch.tensor([n], dtype=torch.int32, device=gpu), k, n_keep=2 ** 31 - 1)
+    torch.cuda.synchronize()
+    assert kept.shape == (1, 1, 2 ** 31 - 1) and new.tolist() == [n] and torch.equal(k, before)
+    assert torch.equal(kept[0, 0, :n].cpu(), torch.arange(n, dtype=torch.int32)) and int(kept[0, 0, n:].max()) == -1 == int(kept[0, 0, n:].min())
+    assert torch.equal(out[..., :n], w[..., :n]) and (out[..., n:] == 0).all()
