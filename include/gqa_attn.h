@@ -129,7 +129,8 @@ int    gqa_attn_launch(const gqa_attn_args * args, void * stream);
  * afterwards the pages past the new length are free. */
 typedef struct gqa_evict_args {
     int32_t n_seq, n_head_kv;
-    int32_t n_keep, n_sink, n_recent;   /* n_sink + n_recent <= n_keep */
+    int32_t n_keep, n_sink, n_recent;   /* n_sink + n_recent <= n_keep.  Rows move in segments of 96 KB (24 KB where a row, a stride or an address is no multiple of
+                                           16 bytes, or a row is below 32): n_seq * n_head_kv * segments of a head, K's and V's, has to stay below 2^23 */
     int32_t k_row_bytes, v_row_bytes;   /* bytes of a head's row: multiples of 4 from 8 to 16384 (any cache type, Q8_0 latent rows of 612 among them) */
     int32_t _pad;
     gqa_pool k, v;                      /* v.data NULL: keys only; else apart from each other (two halves of one row are) */

@@ -322,7 +322,6 @@ __global__ void __launch_bounds__(SEL_THREADS) gqa_rank_kernel(const EvictP p, c
 }
 
 constexpr int MOVE_THREADS = 512, MOVE_R = 12, MOVE_UNITS = MOVE_THREADS * MOVE_R;     // units a workgroup holds in registers: 96 KB of 16 bytes each
-constexpr int MOVE_SEGMENTS = 63 * MOVE_THREADS;                                        // of a head: a bit of a thread each
 
 // The segments of one kind of rows (K or V): `rows` of them a segment, `magic` = ceil(2^32 / units): f / units = f * magic >> 32 for f < MOVE_UNITS.
 struct Seg { int units, rows, count; unsigned magic; };
@@ -352,10 +351,11 @@ __global__ void __launch_bounds__(MOVE_THREADS) gqa_move_kernel(const EvictP p, 
     int      src[MOVE_R], from[MOVE_R], into[MOVE_R];
 #pragma unroll
     for (int r = 0; r < MOVE_R; r++) src[r] = kept[min(j0 + (int) __umulhi(r * MOVE_THREADS + threadIdx.x, sg.magic), last)];
-    // segments in front that read rows this one overwrites: bit k of thread t is segment t + 512 k (kept rises, so a segment reads a range)
-    uint64_t readers = 0;
-    for (int k = 0, s = (int) threadIdx.x; s < seg; k++, s += MOVE_THREADS)
-        readers |= (uint64_t) ((int) (kept[s * sg.rows] < j1) & (int) (kept[(s + 1) * sg.rows - 1] >= j0)) << k;
+    // Segments in front that may read rows this one overwrites: kept rises, so each of them reads from a range of its own at least as long as the rows it moves,
+    // as many as are overwritten here at least; two such ranges at most, side by side, reach into [j0, j1).  So a thread meets one at most: it looks at every 512th.
+    int reader = -1;
+    for (int s = (int) threadIdx.x; s < seg; s += MOVE_THREADS)
+        reader = (int) (kept[s * sg.rows] < j1) & (int) (kept[(s + 1) * sg.rows - 1] >= j0) ? s : reader;
 #pragma unroll
     for (int r = 0; r < MOVE_R; r++) {
         from[r] = bt[src[r] / PAGE];
@@ -374,9 +374,8 @@ __global__ void __launch_bounds__(MOVE_THREADS) gqa_move_kernel(const EvictP p, 
     for (int r = 0; r < MOVE_R; r++) asm volatile("" : "+v"(x[r]) :: "memory");
     __syncthreads();
     if (threadIdx.x == 0) __hip_atomic_store(flags + seg, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (int k = 0, s = (int) threadIdx.x; readers >> k; k++, s += MOVE_THREADS)
-        if (readers >> k & 1)
-            while (__hip_atomic_load(flags + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0u) __builtin_amdgcn_s_sleep(1);
+    if (reader >= 0)
+        while (__hip_atomic_load(flags + reader, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0u) __builtin_amdgcn_s_sleep(1);
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < MOVE_R; r++) {
@@ -448,7 +447,7 @@ extern "C" int gqa_evict_check(const gqa_evict_args * a) {
     if (apart && apart > -row && apart < row) return MLA_ERR_UNSUPPORTED;
     const Plan pl = make_plan(a);
     // (a launch holds fewer than 2^32 threads)
-    if (pl.k.count > MOVE_SEGMENTS || pl.v.count > MOVE_SEGMENTS || pl.segments >= ((int64_t) 1 << 32) / MOVE_THREADS) return MLA_ERR_BAD_SHAPE;
+    if (pl.segments >= ((int64_t) 1 << 32) / MOVE_THREADS) return MLA_ERR_BAD_SHAPE;
     return 0;
 }
 

@@ -68,3 +68,14 @@ int main() {
 """)
     subprocess.run(["g++", "-std=c++17", "-O2", "-Wall", "-Werror", "-I", os.path.join(ROOT, "jittorinfer_amd", "csrc"), str(src), "-o", str(tmp_path / "t"), "-pthread"], check=True)
     assert subprocess.run([str(tmp_path / "t")], timeout=60).returncode == 0
+
+
+def test_evict_of_many_segments_a_head():
+    """Rows that fill a segment of the move alone: as many may stay as a launch has workgroups for, whatever a head's share of them."""
+    lib = J.library()
+    one = dict(n_seq=1, n_head_kv=1, k_row_bytes=16384, v=J.GqaPool(), bt_stride=1 << 17, w_nb1=1 << 26, w_nb2=1 << 26, wd_nb1=1 << 26, wd_nb2=1 << 26, weights_dst=1 << 40)
+    odd = J.GqaPool(1 << 20, 128 * 16388, 16388, 16388)
+    for n_keep, code in ((32256, 0), (32257, 0), ((1 << 23) - 1, 0), (1 << 23, SHAPE)):
+        a = _cut(k=odd, n_keep=n_keep, **one)
+        assert lib.gqa_evict_check(C.byref(a)) == code, n_keep
+        assert (lib.gqa_evict_workspace_size(C.byref(a)) > 4 * n_keep) == (code == 0)

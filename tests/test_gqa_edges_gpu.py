@@ -257,3 +257,35 @@ def test_evict_keeps_as_many_as_there_may_be(gpu):
     assert kept.shape == (1, 1, 2 ** 31 - 1) and new.tolist() == [n] and torch.equal(k, before)
     assert torch.equal(kept[0, 0, :n].cpu(), torch.arange(n, dtype=torch.int32)) and int(kept[0, 0, n:].max()) == -1 == int(kept[0, 0, n:].min())
     assert torch.equal(out[..., :n], w[..., :n]) and (out[..., n:] == 0).all()
+
+
+@pytest.mark.parametrize("kind", ["spread", "late", "alternate"])
+def test_evict_moves_many_segments(gpu, kind):
+    """A segment a row, more of them than 63 a thread: rows that come from near and far, from the end alone, and every other one."""
+    import jittorinfer_amd as J
+    width, n, n_keep = 320, 40900, 33000
+    gen = torch.Generator().manual_seed(82)
+    w = torch.rand((1, 1, width * 128), generator=gen)
+    if kind == "late":
+        w[..., n - n_keep:n] += 2
+    elif kind == "alternate":
+        w[..., :2 * (n - n_keep):2] -= 2
+    bt = torch.randperm(width, generator=gen).to(torch.int32)[None]
+    # rows of 16384 bytes, 4 apart: every 4-byte number says which row and which place of it it is
+    store = torch.zeros((width, 128, 1, 4097), dtype=torch.int32, device=gpu)
+    k = store[..., :4096]
+    row = torch.arange(width * 128, device=gpu, dtype=torch.int32)
+    page = bt[0].to(gpu).long()
+    def pattern(rows):
+        return rows[:, None] * 4096 + torch.arange(4096, device=gpu, dtype=torch.int32)[None]
+    for j in range(width):
+        k[page[j], :, 0] = pattern(row[j * 128:(j + 1) * 128])
+    kept, new, out = J.gqa_evict(w.to(gpu), bt.to(gpu), torch.tensor([n], dtype=torch.int32, device=gpu), k, n_keep=n_keep, n_sink=2, n_recent=10)
+    key = w[0, 0, :n].clone()
+    key[:2], key[n - 10:] = 9, 9
+    want = torch.sort(torch.sort(key, descending=True, stable=True).indices[:n_keep]).values.to(gpu)
+    assert torch.equal(kept[0, 0].long(), want) and new.tolist() == [n_keep]
+    held = torch.cat((want.int(), row[n_keep:]))
+    for j in range(width):
+        assert torch.equal(k[page[j], :, 0], pattern(held[j * 128:(j + 1) * 128])), j
+    assert (store[..., 4096] == 0).all()
