@@ -138,7 +138,7 @@ typedef struct gqa_evict_args {
     const int32_t * block_table;
     int64_t         bt_stride;
     const int32_t * seq_lens;
-    const float * weights;              /* f32 [n_seq][n_head_kv][bt_stride * 128] */
+    const float * weights;              /* f32 [n_seq][n_head_kv][>= bt_stride * 128]; what lies past that is neither read nor written */
     int64_t w_nb1, w_nb2;
     float * weights_dst;                /* the same shape; may be `weights` itself with the same strides, else apart from it */
     int64_t wd_nb1, wd_nb2;

@@ -442,8 +442,10 @@ def gqa_evict(weights, block_table, seq_lens, k_cache, v_cache=None, *, n_keep, 
     move up, in order, inside the sequence's pages.  Caches are [pages, 128, n_head_kv, row] of any element type with rows of whole 4 bytes
     (a latent cache: [pages, 128, 1, 576], or 612 bytes of Q8_0).  Pages mapped by several sequences must not be evicted from
     (PageTable.seq_evict refuses them).
+
+    weights   float32 [n_seq, n_head_kv, >= width * 128] over the int32 block_table [n_seq, width], as gqa_attn adds them up; seq_lens int32 [n_seq]
     Returns kept int32 [n_seq, n_head_kv, n_keep] (the row that is now row j, -1 past the new length), new_lens int32 [n_seq] and the
-    weights that moved along, 0 past the new length (weights_out=weights: in place)."""
+    weights that moved along, 0 past the new length (weights_out=weights: in place; columns past width * 128 stay as they are)."""
     return (_native or native()).gqa_evict(weights, block_table, seq_lens, k_cache, v_cache, n_keep, n_sink, n_recent, weights_out, kept, new_lens, stream)
 
 

@@ -624,7 +624,7 @@ PyObject * gqa_evict(PyObject *, PyObject * const * o, Py_ssize_t n) {
         REQUIRE(rows_ok(*vc, 4, true) && vc->size(0) == a.n_pages && vc->size(1) == PAGE && vc->size(2) == a.n_head_kv && vc->size(3) < INTS / 16);
         a.v = pool_of(*vc); a.v_row_bytes = (int32_t) (vc->size(3) * (int64_t) vc->element_size());
     }
-    REQUIRE(q.scalar_type() == at::kFloat && rows_ok(q, 3, false) && q.size(0) == n_seq && q.size(1) == a.n_head_kv && q.size(2) == cap);
+    REQUIRE(q.scalar_type() == at::kFloat && rows_ok(q, 3, false) && q.size(0) == n_seq && q.size(1) == a.n_head_kv && q.size(2) >= cap);
     a.weights = (const float *) q.data_ptr(); a.w_nb1 = q.stride(1) * 4; a.w_nb2 = q.stride(0) * 4;
     const c10::DeviceGuard guard(q.device());
     GqaStream stream;
@@ -633,7 +633,7 @@ PyObject * gqa_evict(PyObject *, PyObject * const * o, Py_ssize_t n) {
     REQUIRE(a.n_keep >= 0);
     at::Tensor kept = keptp ? *keptp : at::empty({ n_seq, (int64_t) a.n_head_kv, (int64_t) a.n_keep }, q.options().dtype(at::kInt));
     at::Tensor fresh = newp ? *newp : at::empty({ n_seq }, q.options().dtype(at::kInt));
-    REQUIRE(wo.scalar_type() == at::kFloat && rows_ok(wo, 3, true) && wo.size(0) == n_seq && wo.size(1) == a.n_head_kv && wo.size(2) == cap);
+    REQUIRE(wo.scalar_type() == at::kFloat && rows_ok(wo, 3, true) && wo.size(0) == n_seq && wo.size(1) == a.n_head_kv && wo.size(2) >= cap);
     REQUIRE(kept.scalar_type() == at::kInt && kept.dim() == 3 && kept.is_contiguous() && kept.size(0) == n_seq && kept.size(1) == a.n_head_kv && kept.size(2) == a.n_keep);
     REQUIRE(ints(fresh, n_seq));
     a.weights_dst = (float *) wo.data_ptr(); a.wd_nb1 = wo.stride(1) * 4; a.wd_nb2 = wo.stride(0) * 4;

@@ -289,3 +289,22 @@ def test_evict_moves_many_segments(gpu, kind):
     for j in range(width):
         assert torch.equal(k[page[j], :, 0], pattern(held[j * 128:(j + 1) * 128])), j
     assert (store[..., 4096] == 0).all()
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_evict_takes_weights_as_wide_as_attention_does(gpu, in_place):
+    """Sums with room for more rows than the block table has: the columns past it stay."""
+    import jittorinfer_amd as J
+    from tests.test_gqa_gpu import _evict_case
+    w, bt, lens, k, v = _evict_case(83, [300, 384], 3, 2, 64, 64, F16)
+    wide = torch.full((2, 2, 512), 7.0, device=gpu)
+    wide[..., :384] = w.to(gpu)
+    want = R.evict(w, bt, lens.tolist(), k, v, 140, 2, 10)
+    dst = wide if in_place else torch.full((2, 2, 500), 8.0, device=gpu)
+    d = [t.to(gpu) for t in (bt, lens, k, v)]
+    kept, new, out = J.gqa_evict(wide, *d, n_keep=140, n_sink=2, n_recent=10, weights_out=dst)
+    assert out is dst and torch.equal(kept.cpu(), want[0]) and torch.equal(dst[..., :384].cpu(), want[2]) and (dst[..., 384:] == (7 if in_place else 8)).all()
+    assert torch.equal(d[2].cpu(), want[3]) and torch.equal(d[3].cpu(), want[4])
+    if not in_place:
+        d = [t.to(gpu) for t in (bt, lens, k, v)]
+        assert J.gqa_evict(wide, *d, n_keep=140)[2].shape == (2, 2, 384)
