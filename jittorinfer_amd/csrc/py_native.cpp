@@ -425,10 +425,9 @@ bool rows_ok(const at::Tensor & t, int64_t dim, bool written) {
     return true;
 }
 bool cache_ok(const at::Tensor & c, int type) { return mla_type(c) == type && rows_ok(c, 4, true) && c.size(0) >= 1 && c.size(1) == PAGE; }
-gqa_pool pool_of(const at::Tensor & c) {
-    const int64_t es = (int64_t) c.element_size();
-    return gqa_pool{ c.data_ptr(), c.stride(0) * es, c.stride(1) * es, c.stride(2) * es };
-}
+// Bytes from one to the next along a dimension; where there is no next one a stride may be anything, and is none.
+int64_t step(const at::Tensor & t, int64_t d) { return t.size(d) > 1 ? t.stride(d) * (int64_t) t.element_size() : 0; }
+gqa_pool pool_of(const at::Tensor & c) { return gqa_pool{ c.data_ptr(), step(c, 0), step(c, 1), step(c, 2) }; }
 // The stream to launch on.  The result tensors a call makes for itself belong to the device's current stream, so a call on another one
 // brings its own (`makes` = false).
 struct GqaStream {
@@ -494,10 +493,10 @@ PyObject * gqa_norm_rope(PyObject *, PyObject * const * o, Py_ssize_t n) {
     a.attn_factor = PyFloat_AsDouble(o[13]); a.beta_fast = PyFloat_AsDouble(o[14]); a.beta_slow = PyFloat_AsDouble(o[15]);
     if (PyErr_Occurred()) return nullptr;
     REQUIRE(mla_type(q) >= 0 && rows_ok(q, 3, false) && q.size(0) < INTS && q.size(1) < INTS && q.size(2) < INTS);
-    const int64_t n_tok = q.size(0), es = (int64_t) q.element_size();
+    const int64_t n_tok = q.size(0);
     a.n_tok = (int32_t) n_tok; a.n_head = (int32_t) q.size(1); a.dk = (int32_t) q.size(2);
     a.src_type = a.w_type = mla_type(q);
-    a.q = q.data_ptr(); a.q_nb1 = q.stride(1) * es; a.q_nb2 = q.stride(0) * es;
+    a.q = q.data_ptr(); a.q_nb1 = step(q, 1); a.q_nb2 = step(q, 0);
     REQUIRE(ints(*pos, n_tok));
     a.pos = (const int32_t *) pos->data_ptr();
     a.kv_type = MLA_TYPE_BF16;
@@ -517,7 +516,7 @@ PyObject * gqa_norm_rope(PyObject *, PyObject * const * o, Py_ssize_t n) {
         REQUIRE(a.kv_type > 0 && cache_ok(*kc, a.kv_type) && kc->size(2) == k->size(1) && kc->size(2) < INTS && kc->size(3) == a.dk);
         REQUIRE(table_ok(*table) && table->size(0) < INTS && ints(*ids, n_tok) && (!slots || ints(*slots, n_tok)));
         a.n_head_kv = (int32_t) k->size(1); a.n_seq = (int32_t) table->size(0); a.n_pages = kc->size(0);
-        a.k = k->data_ptr(); a.k_nb1 = k->stride(1) * es; a.k_nb2 = k->stride(0) * es;
+        a.k = k->data_ptr(); a.k_nb1 = step(*k, 1); a.k_nb2 = step(*k, 0);
         a.k_cache = pool_of(*kc);
         a.block_table = (const int32_t *) table->data_ptr(); a.bt_stride = table->size(1);
         a.seq_ids = (const int32_t *) ids->data_ptr(); a.slots = slots ? (const int32_t *) slots->data_ptr() : nullptr;
@@ -525,7 +524,7 @@ PyObject * gqa_norm_rope(PyObject *, PyObject * const * o, Py_ssize_t n) {
             REQUIRE(v->scalar_type() == q.scalar_type() && rows_ok(*v, 3, false) && v->size(0) == n_tok && v->size(1) == a.n_head_kv);
             REQUIRE(cache_ok(*vc, a.kv_type) && vc->size(0) == a.n_pages && vc->size(2) == a.n_head_kv && vc->size(3) == v->size(2) && v->size(2) < INTS);
             a.dv = (int32_t) v->size(2);
-            a.v = v->data_ptr(); a.v_nb1 = v->stride(1) * es; a.v_nb2 = v->stride(0) * es;
+            a.v = v->data_ptr(); a.v_nb1 = step(*v, 1); a.v_nb2 = step(*v, 0);
             a.v_cache = pool_of(*vc);
         }
     } else REQUIRE(!v && !kc && !vc && !kw);
@@ -537,8 +536,7 @@ PyObject * gqa_norm_rope(PyObject *, PyObject * const * o, Py_ssize_t n) {
     const at::Tensor & out = *outp;
     a.dst_type = mla_type(out);
     REQUIRE(a.dst_type >= 0 && out.sizes() == q.sizes() && rows_ok(out, 3, true));
-    const int64_t od = (int64_t) out.element_size();
-    a.q_dst = out.data_ptr(); a.qd_nb1 = out.stride(1) * od; a.qd_nb2 = out.stride(0) * od;
+    a.q_dst = out.data_ptr(); a.qd_nb1 = step(out, 1); a.qd_nb2 = step(out, 0);
     const int rc = unlocked([&] { return lib.norm_rope(&a, stream.st); });
     if (rc) return failed("gqa_norm_rope_launch", rc);
     return made.defined() ? THPVariable_Wrap(made) : Py_NewRef(o[17]);
@@ -560,9 +558,9 @@ PyObject * gqa_attn(PyObject *, PyObject * const * o, Py_ssize_t n) {
     REQUIRE(window >= 0 && window < INTS);
     a.window = (int32_t) window;
     REQUIRE(mla_type(q) >= 0 && rows_ok(q, 3, false) && q.size(0) < INTS && q.size(1) < INTS && q.size(2) < INTS);
-    const int64_t n_seq = q.size(0), n_head = q.size(1), es = (int64_t) q.element_size();
+    const int64_t n_seq = q.size(0), n_head = q.size(1);
     a.n_seq = (int32_t) n_seq; a.n_head = (int32_t) n_head; a.dk = (int32_t) q.size(2);
-    a.q_type = mla_type(q); a.q = q.data_ptr(); a.q_nb1 = q.stride(1) * es; a.q_nb2 = q.stride(0) * es;
+    a.q_type = mla_type(q); a.q = q.data_ptr(); a.q_nb1 = step(q, 1); a.q_nb2 = step(q, 0);
     a.kv_type = mla_type(*kc);
     REQUIRE(a.kv_type > 0 && cache_ok(*kc, a.kv_type) && kc->size(2) < INTS && kc->size(3) == a.dk);
     a.n_head_kv = (int32_t) kc->size(2); a.n_pages = kc->size(0); a.k = pool_of(*kc);
@@ -579,7 +577,7 @@ PyObject * gqa_attn(PyObject *, PyObject * const * o, Py_ssize_t n) {
     }
     if (weights) {
         REQUIRE(weights->scalar_type() == at::kFloat && rows_ok(*weights, 3, true) && weights->size(0) == n_seq && weights->size(1) == a.n_head_kv && weights->size(2) >= a.bt_stride * PAGE);
-        a.weights = (float *) weights->data_ptr(); a.w_nb1 = weights->stride(1) * 4; a.w_nb2 = weights->stride(0) * 4;
+        a.weights = (float *) weights->data_ptr(); a.w_nb1 = step(*weights, 1); a.w_nb2 = step(*weights, 0);
     }
     const c10::DeviceGuard guard(q.device());
     GqaStream stream;
@@ -588,10 +586,9 @@ PyObject * gqa_attn(PyObject *, PyObject * const * o, Py_ssize_t n) {
     if (vc) {
         if (!outp) { made = at::empty({ n_seq, n_head, (int64_t) a.dv }, q.options()); outp = &made; }
         const at::Tensor & out = *outp;
-        const int64_t od = (int64_t) out.element_size();
         a.dst_type = mla_type(out);
         REQUIRE(a.dst_type >= 0 && out.dim() == 3 && out.size(0) == n_seq && out.size(1) == n_head && out.size(2) == a.dv && rows_ok(out, 3, true));
-        a.dst = out.data_ptr(); a.d_nb1 = out.stride(1) * od; a.d_nb2 = out.stride(0) * od;
+        a.dst = out.data_ptr(); a.d_nb1 = step(out, 1); a.d_nb2 = step(out, 0);
     } else a.dst_type = MLA_TYPE_F32;
     const size_t need = lib.gqa_workspace_size(&a);
     GqaScratch scratch;
@@ -625,7 +622,7 @@ PyObject * gqa_evict(PyObject *, PyObject * const * o, Py_ssize_t n) {
         a.v = pool_of(*vc); a.v_row_bytes = (int32_t) (vc->size(3) * (int64_t) vc->element_size());
     }
     REQUIRE(q.scalar_type() == at::kFloat && rows_ok(q, 3, false) && q.size(0) == n_seq && q.size(1) == a.n_head_kv && q.size(2) >= cap);
-    a.weights = (const float *) q.data_ptr(); a.w_nb1 = q.stride(1) * 4; a.w_nb2 = q.stride(0) * 4;
+    a.weights = (const float *) q.data_ptr(); a.w_nb1 = step(q, 1); a.w_nb2 = step(q, 0);
     const c10::DeviceGuard guard(q.device());
     GqaStream stream;
     if (!stream.take(o[11], q, !wop || !keptp || !newp)) return nullptr;
@@ -636,7 +633,7 @@ PyObject * gqa_evict(PyObject *, PyObject * const * o, Py_ssize_t n) {
     REQUIRE(wo.scalar_type() == at::kFloat && rows_ok(wo, 3, true) && wo.size(0) == n_seq && wo.size(1) == a.n_head_kv && wo.size(2) >= cap);
     REQUIRE(kept.scalar_type() == at::kInt && kept.dim() == 3 && kept.is_contiguous() && kept.size(0) == n_seq && kept.size(1) == a.n_head_kv && kept.size(2) == a.n_keep);
     REQUIRE(ints(fresh, n_seq));
-    a.weights_dst = (float *) wo.data_ptr(); a.wd_nb1 = wo.stride(1) * 4; a.wd_nb2 = wo.stride(0) * 4;
+    a.weights_dst = (float *) wo.data_ptr(); a.wd_nb1 = step(wo, 1); a.wd_nb2 = step(wo, 0);
     a.kept = (int32_t *) kept.data_ptr(); a.new_lens = (int32_t *) fresh.data_ptr();
     GqaScratch scratch;
     if (!scratch.take(o[0], q, stream, lib.evict_workspace_size(&a), a)) return nullptr;

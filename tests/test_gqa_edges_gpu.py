@@ -308,3 +308,30 @@ def test_evict_takes_weights_as_wide_as_attention_does(gpu, in_place):
     if not in_place:
         d = [t.to(gpu) for t in (bt, lens, k, v)]
         assert J.gqa_evict(wide, *d, n_keep=140)[2].shape == (2, 2, 384)
+
+
+def test_strides_of_dimensions_of_one(gpu):
+    """One token, one sequence, one head, one page: where there is no next one, the stride to it is any number."""
+    import jittorinfer_amd as J
+    from tests.test_gqa_gpu import _evict_case
+    odd = lambda t, *dims: t.as_strided(t.shape, [13 if d in dims else s for d, s in enumerate(t.stride())])
+    q, k, v, bt, lens = (t.to(gpu) for t in _attn_case(90, [100], 1, 3, 1, 64, 64, BF16, spare=0, stale=0.0))
+    want, sums = J.gqa_attn(q, k, v, bt, lens, scale=0.1), torch.zeros((1, 1, 128), device=gpu)
+    J.gqa_attn(q, k, v, bt, lens, scale=0.1, weights=sums)
+    out, got = torch.empty_like(want), torch.zeros_like(sums)
+    J.gqa_attn(odd(q, 0), odd(k, 0, 2), odd(v, 0, 2), bt, lens, scale=0.1, weights=odd(got, 0, 1), out=odd(out, 0))
+    assert torch.equal(out, want) and torch.equal(got, sums)
+    one = q[:, :1].contiguous()
+    assert torch.equal(J.gqa_attn(odd(one, 0, 1), k, v, bt, lens, scale=0.1), want[:, :1])
+    pos, ids = torch.tensor([7], dtype=torch.int32, device=gpu), torch.zeros(1, dtype=torch.int32, device=gpu)
+    kc, vc, kc2, vc2 = k.clone(), v.clone(), k.clone(), v.clone()
+    x = torch.randn((1, 1, 64), device=gpu).to(BF16)
+    rope = dict(n_dims=64, mode=2, block_table=bt, seq_ids=ids)
+    want = J.gqa_norm_rope(q, x, x, pos, k_cache=kc, v_cache=vc, **rope)
+    got = torch.empty_like(want)
+    J.gqa_norm_rope(odd(q, 0), odd(x, 0, 1), odd(x, 0, 1), pos, k_cache=odd(kc2, 0, 2), v_cache=odd(vc2, 0, 2), q_out=odd(got, 0), **rope)
+    assert torch.equal(got, want) and torch.equal(kc, kc2) and torch.equal(vc, vc2)
+    w = torch.rand((1, 1, 128), device=gpu)
+    kept, new, moved = J.gqa_evict(w, bt, lens, kc, vc, n_keep=30)
+    kept2, new2, moved2 = J.gqa_evict(odd(w, 0, 1), bt, lens, odd(kc2, 0, 2), odd(vc2, 0, 2), n_keep=30, weights_out=odd(torch.empty_like(w), 0, 1))
+    assert torch.equal(kept, kept2) and torch.equal(moved, moved2) and torch.equal(kc, kc2) and torch.equal(vc, vc2)
