@@ -42,7 +42,8 @@ typedef struct gqa_pool {
  * Angles are taken in 64 bits, so they are exact to f32 at any position; ggml_rope_ext's own f32 recurrence (mla_rope_launch) is off by
  * about pos * 2^-22 radians.  Queries go to q_dst, keys (and values, as they are) to their rows of the cache: token t of sequence
  * seq_ids[t] to row slots[t] (NULL: pos[t]); rows outside the block table, negative ones and bad pages are skipped, as the cache write
- * of include/mla_kv_write.h skips them.  Two tokens of one call that name the same row leave parts of either there. */
+ * of include/mla_kv_write.h skips them.  Two tokens of one call that name the same row leave parts of either there; no token's k or v may lie
+ * on a row that another token of the call writes. */
 typedef struct gqa_norm_rope_args {
     int32_t n_tok, n_head, n_head_kv;   /* n_tok below 2^24 */
     int32_t dk, dv;          /* values per key / query head and per value head: multiples of 8, at most 256 */

@@ -1013,6 +1013,10 @@ extern "C" int gqa_attn_check(const gqa_attn_args * a) {
         if (((uintptr_t) a->mask & 1) || (a->mask_nb1 & 1)) return MLA_ERR_BAD_ALIGNMENT;
         if (a->mask_ne0 < 0) return MLA_ERR_BAD_SHAPE;
     }
+    // what is written is nothing that is read (by its address alone: strides may lay one between the other's rows)
+    for (const void * w : { (const void *) a->dst, (const void *) a->weights })
+        if (w && (w == a->q || w == a->k.data || w == a->v.data || w == a->mask || w == (const void *) a->seq_lens || w == (const void *) a->block_table)) return MLA_ERR_UNSUPPORTED;
+    if (a->dst && a->dst == a->weights) return MLA_ERR_UNSUPPORTED;
     if (a->weights && (((uintptr_t) a->weights & 3) || (a->w_nb1 & 3) || (a->w_nb2 & 3))) return MLA_ERR_BAD_ALIGNMENT;
     return 0;
 }

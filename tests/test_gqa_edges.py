@@ -79,3 +79,75 @@ def test_evict_of_many_segments_a_head():
         a = _cut(k=odd, n_keep=n_keep, **one)
         assert lib.gqa_evict_check(C.byref(a)) == code, n_keep
         assert (lib.gqa_evict_workspace_size(C.byref(a)) > 4 * n_keep) == (code == 0)
+
+
+@pytest.mark.parametrize("kw", [dict(dst=4096), dict(dst=1 << 20), dict(dst=1 << 24), dict(dst=16384), dict(weights=1 << 20), dict(weights=8192), dict(weights=32768), dict(weights=4096)], ids=str)
+def test_attn_refuses_results_on_its_operands(kw):
+    a = _attn(w_nb1=2048, w_nb2=4096, **kw)
+    assert J.library().gqa_attn_check(C.byref(a)) == UNSUPPORTED and J.library().gqa_attn_launch(C.byref(a), None) == UNSUPPORTED
+
+
+def test_overlap_of_strided_tensors(tmp_path):
+    """What says whether two tensors share bytes, against their sets of bytes: views of one buffer with the same strides, and any two."""
+    src = tmp_path / "t.cpp"
+    src.write_text(r"""
+#include "tensor_overlap.hpp"
+#include <random>
+#include <set>
+#include <vector>
+struct T { int64_t at, el; std::vector<int64_t> n, s; };
+static std::set<int64_t> bytes(const T & t) {
+    std::set<int64_t> r;
+    std::vector<int64_t> i(t.n.size(), 0);
+    for (auto x : t.n) if (!x) return r;
+    for (;;) {
+        int64_t a = t.at;
+        for (size_t d = 0; d < i.size(); d++) a += i[d] * t.s[d] * t.el;
+        for (int64_t e = 0; e < t.el; e++) r.insert(a + e);
+        size_t d = 0;
+        for (; d < i.size(); d++) { if (++i[d] < t.n[d]) break; i[d] = 0; }
+        if (d == i.size()) return r;
+    }
+}
+static mla::Extent extent(const T & t) { return mla::Extent((const void *) t.at, t.el, (int) t.n.size(), t.n.data(), t.s.data()); }
+int main() {
+    std::mt19937 g(1);
+    auto rnd = [&](int lo, int hi) { return (int64_t) (lo + g() % (hi - lo + 1)); };
+    long met = 0;
+    for (int it = 0; it < 20000; it++) {
+        T a, b;
+        const bool alike = it % 2;
+        a.el = 1 << rnd(0, 2); b.el = alike ? a.el : 1 << rnd(0, 2);
+        a.at = 10000; b.at = 10000 + (alike ? a.el * rnd(-60, 60) : rnd(-120, 120));
+        int64_t st = 1;
+        for (int i = 0, d = rnd(1, 3); i < d; i++) {
+            const int64_t na = rnd(1, 4), nb = rnd(1, 4);
+            a.n.push_back(na); a.s.push_back(st);
+            if (alike) { b.n.push_back(nb); b.s.push_back(st); }
+            st = st * (na > nb ? na : nb) + rnd(0, 3);
+        }
+        if (!alike) {
+            for (int i = 0, d = rnd(0, 3); i < d; i++) { b.n.push_back(rnd(0, 4)); b.s.push_back(rnd(0, 20)); }
+            if (rnd(0, 1)) for (auto & x : a.s) x = rnd(0, 20);
+        }
+        const auto p = bytes(a), q = bytes(b);
+        bool over = false;
+        for (auto x : p) over = over || q.count(x);
+        met += over;
+        const mla::Shares want = over ? mla::Shares::YES : mla::Shares::NO;
+        if (mla::shares(extent(a), extent(b)) != want || mla::shares(extent(b), extent(a)) != want) return 1;
+    }
+    if (met < 1000 || met > 19000) return 2;
+    // large ones: two caches side by side in every page; a tensor in the gaps of another, which takes more looks than there are
+    const int64_t big = (int64_t) 1 << 40;
+    T k{ big, 2, { 20000, 128, 8, 128 }, { 2 * 131072, 1024, 128, 1 } }, v = k, w{ big + 4096, 4, { 1 << 20 }, { 997 } };
+    v.at += 2 * 131072;
+    if (mla::shares(extent(k), extent(v)) != mla::Shares::NO) return 3;
+    v.at -= 2;
+    if (mla::shares(extent(k), extent(v)) != mla::Shares::YES) return 4;
+    if (mla::shares(extent(k), extent(w)) == mla::Shares::NO) return 5;
+    return 0;
+}
+""")
+    subprocess.run(["g++", "-std=c++17", "-O2", "-Wall", "-Werror", "-I", os.path.join(ROOT, "jittorinfer_amd", "csrc"), str(src), "-o", str(tmp_path / "t")], check=True)
+    assert subprocess.run([str(tmp_path / "t")], timeout=60).returncode == 0

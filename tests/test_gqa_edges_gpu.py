@@ -335,3 +335,50 @@ def test_strides_of_dimensions_of_one(gpu):
     kept, new, moved = J.gqa_evict(w, bt, lens, kc, vc, n_keep=30)
     kept2, new2, moved2 = J.gqa_evict(odd(w, 0, 1), bt, lens, odd(kc2, 0, 2), odd(vc2, 0, 2), n_keep=30, weights_out=odd(torch.empty_like(w), 0, 1))
     assert torch.equal(kept, kept2) and torch.equal(moved, moved2) and torch.equal(kc, kc2) and torch.equal(vc, vc2)
+
+
+def _shares(call, *args, **kw):
+    with pytest.raises(RuntimeError, match="share memory|failed with code -6"):
+        call(*args, **kw)
+
+
+def test_results_on_operands_are_refused(gpu):
+    """What a call writes may not lie on what it reads; views of one buffer that share no byte may."""
+    import jittorinfer_amd as J
+    z = lambda *s, dtype=BF16: torch.zeros(s, dtype=dtype, device=gpu)
+    i = lambda *s: z(*s, dtype=torch.int32)
+    buf, kv, bt, lens = z(4, 10, 64), z(3, 128, 4, 64), i(4, 2), i(4)
+    q, k, v, sums = buf[:, :4], kv[:, :, :2], kv[:, :, 2:], z(4, 2, 300, dtype=F32)
+    attn = dict(q=q, k_cache=k, v_cache=v, block_table=bt, seq_lens=lens, scale=1.0)
+    J.gqa_attn(**attn, out=buf[:, 4:8], weights=sums)
+    for out in (q, buf[:, 1:5], buf[:, 3:7], kv[2, :16].view(4, 4, 4, 64)[:, :, 0], sums.view(torch.uint8).view(-1)[:2048].view(BF16).view(4, 4, 64)):
+        _shares(J.gqa_attn, **attn, out=out, weights=sums)
+    bytes_of = lambda t: t.contiguous().view(-1).view(torch.uint8)
+    _shares(J.gqa_attn, **attn, weights=bytes_of(kv)[:4 * 2 * 256 * 4].view(F32).view(4, 2, 256))
+    mask = z(4, 256 * 2, dtype=F16)
+    wide = z(4, 2, 256, dtype=F32)
+    _shares(J.gqa_attn, **attn, weights=wide, mask=wide.view(-1).view(F16)[:1024].view(4, 256))
+    assert not buf.any() and not kv.any() and not mask.any()
+
+    pos, ids = i(4), i(4)
+    qkv = z(4, 12, 64)
+    rows = dict(q=qkv[:, :4], k=qkv[:, 8:10], v=qkv[:, 10:], pos=pos, n_dims=64, k_cache=k, v_cache=v, block_table=bt, seq_ids=ids)
+    J.gqa_norm_rope(**rows, q_out=qkv[:, 4:8])
+    J.gqa_norm_rope(**rows, q_out=qkv[:, :4])
+    for out in (qkv[:, 1:5], qkv[:, 5:9], qkv[:, 7:11], kv[0, :4]):
+        _shares(J.gqa_norm_rope, **rows, q_out=out)
+    for name, other in (("v_cache", kv[:, :, 1:3]), ("v_cache", k), ("k_cache", kv[:, :, 1:3])):
+        _shares(J.gqa_norm_rope, **{**rows, name: other})
+
+    w = z(5, 4, 256, dtype=F32)
+    cut = dict(weights=w[:4, :2], block_table=bt, seq_lens=lens, k_cache=k, v_cache=v, n_keep=20)
+    J.gqa_evict(**cut, weights_out=w[:4, 2:])
+    J.gqa_evict(**cut, weights_out=w[:4, :2])
+    for out in (w[1:5, :2], w[:4, 1:3]):
+        _shares(J.gqa_evict, **cut, weights_out=out)
+    both = i(4 * 2 * 20 + 4)
+    J.gqa_evict(**cut, kept=both[:160].view(4, 2, 20), new_lens=both[160:])
+    _shares(J.gqa_evict, **cut, kept=both[:160].view(4, 2, 20), new_lens=both[157:161])
+    _shares(J.gqa_evict, **cut, new_lens=bt.view(-1)[2:6])
+    _shares(J.gqa_evict, **{**cut, "v_cache": kv[:, :, 1:3]})
+    _shares(J.gqa_evict, **{**cut, "k_cache": kv[:, :, 1:3]})
