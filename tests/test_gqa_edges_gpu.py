@@ -382,3 +382,37 @@ def test_results_on_operands_are_refused(gpu):
     _shares(J.gqa_evict, **cut, new_lens=bt.view(-1)[2:6])
     _shares(J.gqa_evict, **{**cut, "v_cache": kv[:, :, 1:3]})
     _shares(J.gqa_evict, **{**cut, "k_cache": kv[:, :, 1:3]})
+
+
+# ---------------------------------------------------------------- the prompt form of norms and rotation: a workgroup a token, four sets of rows ahead, from 1024 tokens on
+
+@pytest.mark.parametrize("src,kv", [(F32, BF16), (F32, F16), (BF16, BF16), (BF16, F16), (F16, F16), (F16, BF16)])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (72, 40), (128, 128), (256, 256)])
+def test_norm_rope_prompts(gpu, src, kv, dk, dv):
+    for n_tok, n_head, n_head_kv, mode in ((1023, 4, 1, 0), (1024, 3, 2, 2), (1025, 5, 2, 0)):
+        _check_rows(gpu, src, kv, n_tok, n_head, n_head_kv, dk, dv, n_dims=dk // 16 * 16, mode=mode, w_type=src, out_type=F32 if n_tok == 1024 else None, seed=dk)
+
+
+@pytest.mark.parametrize("n_head,n_head_kv,dk", [(64, 2, 128), (66, 1, 128), (128, 1, 64), (39, 2, 256), (33, 8, 192), (160, 4, 64), (64, 0, 128)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_norm_rope_prompts_of_many_rows(gpu, n_head, n_head_kv, dk, in_place):
+    """More than the four sets of rows that are under way at once; a last set that is not full, one that holds queries and keys; in place."""
+    if n_head_kv:
+        _check_rows(gpu, BF16, BF16, 1100, n_head, n_head_kv, dk, 64, n_dims=dk, mode=2, in_place=in_place, seed=n_head)
+        _check_rows(gpu, BF16, BF16, 1030, n_head, n_head_kv, dk, 64, "heads", n_dims=32, mode=0, in_place=in_place, norm=False, seed=n_head)
+    else:
+        import jittorinfer_amd as J
+        gen = torch.Generator().manual_seed(1)
+        q, w, pos = torch.randn((1024, n_head, dk), generator=gen), torch.rand(dk, generator=gen) + 0.5, torch.arange(1024, dtype=torch.int32)
+        want, off = R.heads(q, w, 1e-6, pos, dk, 2)
+        d = q.to(gpu)
+        got = J.gqa_norm_rope(d, None, None, pos.to(gpu), n_dims=dk, mode=2, q_weight=w.to(gpu), q_out=d if in_place else None)
+        _near(got, want, off, F32)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_norm_rope_few_tokens_of_many_rows(gpu, in_place):
+    """More sets of rows than a token has workgroups (64): a workgroup takes several in turn."""
+    _check_rows(gpu, BF16, BF16, 3, 600, 2, 256, 64, n_dims=256, mode=2, in_place=in_place)
+    _check_rows(gpu, F32, F16, 2, 1030, 1, 128, 64, n_dims=64, mode=0, in_place=in_place)
+    _check_rows(gpu, F32, BF16, 1040, 9, 3, 128, 128, n_dims=128, mode=2, in_place=in_place, past=70000)
