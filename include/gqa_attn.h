@@ -101,7 +101,7 @@ typedef struct gqa_attn_args {
     int32_t n_workgroups;    /* tuning: workgroups the rows are dealt to, 0 = choose */
     const void * q;          /* [n_seq][n_head][dk] */
     int64_t q_nb1, q_nb2;    /* bytes from a head, a sequence to the next */
-    gqa_pool k, v;           /* rows 16-byte aligned */
+    gqa_pool k, v;           /* rows 16-byte aligned, at most 8 MB apart, pages less than 4 GB */
     int64_t n_pages;
     const int32_t * block_table; /* [n_seq][bt_stride] */
     int64_t         bt_stride;
@@ -126,8 +126,11 @@ int    gqa_attn_launch(const gqa_attn_args * args, void * stream);
  * up, in their order, to rows 0 .. n_keep - 1 of the same pages, keys, values and weights alike; new_lens[b] = n_keep.  Shorter
  * sequences stay as they are.  kept[b][g][j] = the row that is now row j, -1 past the new length; weights_dst past it: 0.
  * Keys keep the rotation they were written with: the next token's position goes on counting (gqa_norm_rope's pos), its row is the
- * sequence's new length (slots).  Pages that other sequences map too must not be evicted from (mla_page_table_seq_evict refuses them);
- * afterwards the pages past the new length are free. */
+ * sequence's new length (slots).  Heads keep rows of their own choice, so afterwards one row number stands for another position in every
+ * head: mask and window of gqa_attn go by rows, not positions.  Pages that other sequences map too must not be evicted from
+ * (mla_page_table_seq_evict refuses them); nor sequences with a page outside [0, n_pages) inside their length: nothing is read or written
+ * there, so a row kept from it leaves its new place as it was, while kept, new_lens and the weights count it.  Afterwards the pages past the
+ * new length are free. */
 typedef struct gqa_evict_args {
     int32_t n_seq, n_head_kv;
     int32_t n_keep, n_sink, n_recent;   /* n_sink + n_recent <= n_keep.  Rows move in segments of 96 KB (24 KB where a row, a stride or an address is no multiple of

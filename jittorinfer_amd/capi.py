@@ -413,7 +413,8 @@ def gqa_norm_rope(q, k, v, pos, *, n_dims, mode=0, n_ctx_orig=0, freq_base=10000
 
     q         [n_tok, n_head, dk], k [n_tok, n_head_kv, dk], v [n_tok, n_head_kv, dv]: float32, bfloat16 or float16 alike, any strides
               over contiguous rows (views of one projection's output); v may be None, and k with it: queries alone
-    pos       int32 [n_tok]; the rotation's keywords are those of ggml_rope_ext, n_dims=0 rotates nothing
+    pos       int32 [n_tok]; the rotation's keywords are those of ggml_rope_ext, of the first n_dims values of a head (rotated values that lie behind plain
+              ones: a call for each part, on views); n_dims=0 rotates nothing
     q_weight, k_weight  [dk] or None: no norm
     k_cache, v_cache    bfloat16 or float16 [pages, 128, n_head_kv, dk | dv]; token t goes to row slots[t] (default: pos[t]) of sequence
               seq_ids[t] of the int32 block_table [n_seq, pages]; rows outside it are skipped
@@ -441,7 +442,8 @@ def gqa_evict(weights, block_table, seq_lens, k_cache, v_cache=None, *, n_keep, 
     include/gqa_attn.h): for every KV head the first n_sink rows, the last n_recent and the heaviest of the rest (equal weights: the lower row)
     move up, in order, inside the sequence's pages.  Caches are [pages, 128, n_head_kv, row] of any element type with rows of whole 4 bytes
     (a latent cache: [pages, 128, 1, 576], or 612 bytes of Q8_0).  Pages mapped by several sequences must not be evicted from
-    (PageTable.seq_evict refuses them).
+    (PageTable.seq_evict refuses them), nor sequences with a bad page id inside their length.  Heads keep rows of their own choice: afterwards gqa_attn's
+    mask and window count rows, no longer positions.
 
     weights   float32 [n_seq, n_head_kv, >= width * 128] over the int32 block_table [n_seq, width], as gqa_attn adds them up; seq_lens int32 [n_seq]
     Returns kept int32 [n_seq, n_head_kv, n_keep] (the row that is now row j, -1 past the new length), new_lens int32 [n_seq] and the

@@ -416,3 +416,113 @@ def test_norm_rope_few_tokens_of_many_rows(gpu, in_place):
     _check_rows(gpu, BF16, BF16, 3, 600, 2, 256, 64, n_dims=256, mode=2, in_place=in_place)
     _check_rows(gpu, F32, F16, 2, 1030, 1, 128, 64, n_dims=64, mode=0, in_place=in_place)
     _check_rows(gpu, F32, BF16, 1040, 9, 3, 128, 128, n_dims=128, mode=2, in_place=in_place, past=70000)
+
+
+@pytest.mark.parametrize("n_tok", [5, 1200])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_norm_rope_of_heads_in_two_parts(gpu, n_tok, in_place):
+    """Heads of 128 plain values with 64 rotated ones behind, those of the keys shared by all heads: a call for each part, on views of queries, results and cache."""
+    import jittorinfer_amd as J
+    from tests.test_gqa_gpu import YARN
+    H, plain, turned, dv = 16, 128, 64, 128
+    gen = torch.Generator().manual_seed(n_tok)
+    q, kv, pe = (torch.randn(s, generator=gen).to(BF16) for s in ((n_tok, H, plain + turned), (n_tok, H, plain + dv), (n_tok, turned)))
+    pos, ids = torch.arange(n_tok, dtype=torch.int32) // 2 + 3000, torch.arange(n_tok, dtype=torch.int32) % 2
+    slots, width = torch.arange(n_tok, dtype=torch.int32) // 2, n_tok // 256 + 1
+    bt = R.make_table(gen, [width * 128] * 2, width, 2 * width)
+    kc, vc = (torch.full((2 * width, 128, H, d), 3.0, dtype=BF16, device=gpu) for d in (plain + turned, dv))
+    dq, dkv, dpe = q.to(gpu), kv.to(gpu), pe.to(gpu)
+    out = dq if in_place else torch.empty_like(dq)
+    rope = dict(n_dims=turned, mode=0, **YARN)
+    at = dict(block_table=bt.to(gpu), seq_ids=ids.to(gpu), slots=slots.to(gpu))
+    J.gqa_norm_rope(dq[..., :plain], dkv[..., :plain], dkv[..., plain:], pos.to(gpu), n_dims=0, k_cache=kc[..., :plain], v_cache=vc, q_out=out[..., :plain], **at)
+    J.gqa_norm_rope(dq[..., plain:], dpe[:, None].expand(n_tok, H, turned), None, pos.to(gpu), k_cache=kc[..., plain:], q_out=out[..., plain:], **rope, **at)
+    want, off = R.heads(q[..., plain:], None, 0, pos, **rope)
+    assert torch.equal(out[..., :plain].cpu(), q[..., :plain])
+    _near(out[..., plain:], want, off, BF16)
+    page, row = bt[ids.long(), slots.long() // 128].long(), slots.long() % 128
+    want, off = R.heads(pe[:, None], None, 0, pos, **rope)
+    got = kc.cpu()[page, row]
+    assert torch.equal(got[..., :plain], kv[..., :plain]) and torch.equal(vc.cpu()[page, row], kv[..., plain:])
+    _near(got[..., plain:], want.expand(n_tok, H, turned), off.expand(n_tok, H, turned), BF16)
+    mark = torch.ones((2 * width, 128), dtype=torch.bool)
+    mark[page, row] = False
+    assert (kc.cpu()[mark] == 3).all() and (vc.cpu()[mark] == 3).all()
+
+
+@pytest.mark.parametrize("n_tok", [7, 1100])
+def test_norm_rope_in_a_graph_and_on_another_stream(gpu, n_tok):
+    """Captured once, replayed while activations, positions and rows change under it; and launched through stream= with results of the caller's."""
+    import jittorinfer_amd as J
+    H, G, D, width = 6, 2, 128, n_tok // 128 + 2
+    gen = torch.Generator().manual_seed(n_tok)
+    wq, wk = (torch.rand(D, generator=gen) + 0.5 for _ in range(2))
+    bt = R.make_table(gen, [width * 128], width, width)
+    rope = dict(n_dims=D, mode=2, freq_base=10000.0)
+    qkv, pos, slots = torch.empty((n_tok, H + 2 * G, D), dtype=BF16, device=gpu), torch.zeros(n_tok, dtype=torch.int32, device=gpu), torch.zeros(n_tok, dtype=torch.int32, device=gpu)
+    ids, table, dwq, dwk = torch.zeros(n_tok, dtype=torch.int32, device=gpu), bt.to(gpu), wq.to(gpu), wk.to(gpu)
+    kc, vc = (torch.empty((width, 128, G, D), dtype=BF16, device=gpu) for _ in range(2))
+    out = torch.empty((n_tok, H, D), dtype=BF16, device=gpu)
+
+    def call(**kw):
+        J.gqa_norm_rope(qkv[:, :H], qkv[:, H:H + G], qkv[:, H + G:], pos, q_weight=dwq, k_weight=dwk, k_cache=kc, v_cache=vc, block_table=table, seq_ids=ids, slots=slots, q_out=out, **rope, **kw)
+    qkv.zero_()
+    torch.cuda.synchronize()
+    g, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(g):
+        call()
+    for step in range(4):
+        x, p, r = torch.randn(qkv.shape, generator=gen).to(BF16), torch.arange(n_tok, dtype=torch.int32) + 5000 * step, (torch.arange(n_tok, dtype=torch.int32) + 37 * step) % (width * 128)
+        qkv.copy_(x), pos.copy_(p), slots.copy_(r), kc.fill_(5.0), vc.fill_(5.0)
+        torch.cuda.synchronize()
+        if step < 3:
+            g.replay()
+        else:
+            call(stream=side.cuda_stream)
+        torch.cuda.synchronize()
+        want, off = R.heads(x[:, :H], wq, 1e-6, p, **rope)
+        _near(out, want, off, BF16, "q %d" % step)
+        want, off = R.heads(x[:, H:H + G], wk, 1e-6, p, **rope)
+        page, row = bt[0, r.long() // 128].long(), r.long() % 128
+        _near(kc.cpu()[page, row], want, off, BF16, "k %d" % step)
+        assert torch.equal(vc.cpu()[page, row], x[:, H + G:]) and int((kc != 5).any(-1).any(-1).sum()) == n_tok == int((vc != 5).any(-1).any(-1).sum())
+
+
+def test_a_captured_decode_step(gpu):
+    """Fill, attend with weights and cut, captured together with padding behind the last sequence, replayed for several steps beside eager calls: the same bits."""
+    import jittorinfer_amd as J
+    H, G, D, n_seq, width, keep = 16, 8, 128, 5, 260, 400
+    gen = torch.Generator().manual_seed(91)
+    bt = R.make_table(gen, [width * 128] * n_seq, width, n_seq * width + 1).to(gpu)
+    k0, v0 = (torch.randn((n_seq * width + 1, 128, G, D), generator=torch.Generator(device=gpu).manual_seed(i), device=gpu, dtype=F32).to(BF16) for i in range(2))
+    ids = torch.arange(n_seq, dtype=torch.int32, device=gpu)
+    fresh = lambda: dict(kc=k0.clone(), vc=v0.clone(), sums=torch.zeros((n_seq, G, width * 128), device=gpu), qkv=torch.zeros((n_seq, H + 2 * G, D), dtype=BF16, device=gpu),
+                         pos=torch.zeros(n_seq, dtype=torch.int32, device=gpu), slots=torch.zeros(n_seq, dtype=torch.int32, device=gpu), lens=torch.zeros(n_seq, dtype=torch.int32, device=gpu),
+                         q=torch.empty((n_seq, H, D), dtype=BF16, device=gpu), out=torch.empty((n_seq, H, D), dtype=BF16, device=gpu),
+                         kept=torch.empty((n_seq, G, keep), dtype=torch.int32, device=gpu), new=torch.empty(n_seq, dtype=torch.int32, device=gpu))
+
+    def step(s):
+        J.gqa_norm_rope(s["qkv"][:, :H], s["qkv"][:, H:H + G], s["qkv"][:, H + G:], s["pos"], n_dims=D, mode=2, k_cache=s["kc"], v_cache=s["vc"], block_table=bt, seq_ids=ids, slots=s["slots"], q_out=s["q"])
+        J.gqa_attn(s["q"], s["kc"], s["vc"], bt, s["lens"], scale=0.09, weights=s["sums"], out=s["out"])
+        J.gqa_evict(s["sums"], bt, s["lens"], s["kc"], s["vc"], n_keep=keep, n_sink=4, n_recent=60, weights_out=s["sums"], kept=s["kept"], new_lens=s["new"])
+    held, eager = fresh(), fresh()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step(held)
+    lens = [1, 33000, 401, 700, 0]                        # the last one is padding: no row, its token's row lies outside the table
+    for i in range(4):
+        x = torch.randn(held["qkv"].shape, generator=gen).to(BF16)
+        for s in (held, eager):
+            s["qkv"].copy_(x)
+            s["pos"].copy_(torch.tensor([n + 50 * i for n in lens], dtype=torch.int32))
+            s["slots"].copy_(torch.tensor([n - 1 for n in lens], dtype=torch.int32))
+            s["lens"].copy_(torch.tensor(lens, dtype=torch.int32))
+        torch.cuda.synchronize()
+        g.replay()
+        step(eager)
+        torch.cuda.synchronize()
+        for name in held:
+            assert torch.equal(held[name], eager[name]), (i, name)
+        assert held["new"].tolist() == [min(n, keep) for n in lens] and (held["out"][4] == 0).all() and not held["sums"][4].any()
+        lens = [n + 1 if n else 0 for n in held["new"].tolist()]
