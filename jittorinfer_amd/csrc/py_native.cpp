@@ -473,21 +473,42 @@ struct GqaScratch {
         return (bool) ws;
     }
 };
-// What is written has to lie apart from what is read, but for a tensor that the call may work on in place; views of one buffer that share no byte are apart.
-// Layouts too tangled to tell are let through.
-struct Named { const char * name; const at::Tensor * t; };
-bool lie_apart(const char * call, Named written, std::initializer_list<Named> others, const at::Tensor * in_place = nullptr) {
-    auto extent = [](const at::Tensor & t) { return mla::Extent(t.data_ptr(), (int64_t) t.element_size(), (int) t.dim(), t.sizes().data(), t.strides().data()); };
-    if (!written.t) return true;
-    const mla::Extent w = extent(*written.t);
-    for (const Named & o : others) {
-        if (!o.t || (o.t == in_place && o.t->data_ptr() == written.t->data_ptr())) continue;      // (in place: its strides and type are the launch's to check)
-        if (mla::shares(w, extent(*o.t)) != mla::Shares::YES) continue;
-        PyErr_Format(PyExc_RuntimeError, "%s: %s and %s share memory", call, written.name, o.name);
-        return false;
+// What a call writes has to lie apart from what it reads and from what else it writes, but for the one tensor it may work on in place; views of one buffer that
+// share no byte are apart.  Layouts too tangled to tell are let through.  (Most tensors lie in memory of their own: their ranges are taken once and compared first.)
+class Apart {
+    struct Item { const char * name; const at::Tensor * t; uintptr_t lo, hi; };
+    Item items[16];
+    int  n = 0;
+
+  public:
+    // a tensor or nullptr; those that are written come first
+    void add(const char * name, const at::Tensor * t) {
+        if (!t) return;
+        const auto sizes = t->sizes(), strides = t->strides();
+        int64_t span = 1;
+        for (size_t d = 0; d < sizes.size(); d++) {
+            if (sizes[d] == 0) return;
+            span += (sizes[d] - 1) * strides[d];
+        }
+        const uintptr_t lo = (uintptr_t) t->data_ptr();
+        items[n++] = Item{ name, t, lo, lo + (uintptr_t) (span * (int64_t) t->element_size()) };
     }
-    return true;
-}
+    int count() const { return n; }
+    // items 0 .. written - 1 against all that follow them
+    bool check(const char * call, int written, const at::Tensor * in_place_on = nullptr) const {
+        for (int i = 0; i < written; i++)
+            for (int k = i + 1; k < n; k++) {
+                const Item & a = items[i], & b = items[k];
+                if (a.lo >= b.hi || b.lo >= a.hi) continue;
+                if (i == 0 && b.t == in_place_on && a.lo == b.lo) continue;            // (its strides and type are the launch's to check)
+                auto extent = [](const Item & x) { return mla::Extent((const void *) x.lo, (int64_t) x.t->element_size(), (int) x.t->dim(), x.t->sizes().data(), x.t->strides().data()); };
+                if (mla::shares(extent(a), extent(b)) != mla::Shares::YES) continue;
+                PyErr_Format(PyExc_RuntimeError, "%s: %s and %s share memory", call, a.name, b.name);
+                return false;
+            }
+        return true;
+    }
+};
 #define SAME_DEVICE(t) REQUIRE(!(t) || (t)->device() == q.device())
 
 // gqa_norm_rope(q, k, v, pos, q_weight, k_weight, eps, n_dims, mode, n_ctx_orig, freq_base, freq_scale, ext_factor, attn_factor, beta_fast,
@@ -553,11 +574,17 @@ PyObject * gqa_norm_rope(PyObject *, PyObject * const * o, Py_ssize_t n) {
     a.dst_type = mla_type(out);
     REQUIRE(a.dst_type >= 0 && out.sizes() == q.sizes() && rows_ok(out, 3, true));
     a.q_dst = out.data_ptr(); a.qd_nb1 = step(out, 1); a.qd_nb2 = step(out, 0);
-    if ((!made.defined() && !lie_apart("gqa_norm_rope", { "q_out", &out }, { { "q", &q }, { "k", k }, { "v", v }, { "pos", pos }, { "q_weight", qw }, { "k_weight", kw }, { "freq_factors", ff },
-                                       { "k_cache", kc }, { "v_cache", vc }, { "block_table", table }, { "seq_ids", ids }, { "slots", slots } }, &q)) ||
-        !lie_apart("gqa_norm_rope", { "k_cache", kc }, { { "v_cache", vc }, { "q", &q }, { "pos", pos }, { "block_table", table }, { "seq_ids", ids }, { "slots", slots } }) ||
-        !lie_apart("gqa_norm_rope", { "v_cache", vc }, { { "q", &q }, { "pos", pos }, { "block_table", table }, { "seq_ids", ids }, { "slots", slots } }))
-        return nullptr;
+    Apart apart;                                              // (keys and values may lie in the cache, where the caller knows the rows)
+    if (!made.defined()) {
+        Apart result;
+        result.add("q_out", &out);
+        for (const auto & [name, t] : { std::pair<const char *, const at::Tensor *>{ "q", &q }, { "k", k }, { "v", v }, { "pos", pos }, { "q_weight", qw }, { "k_weight", kw }, { "freq_factors", ff },
+                                        { "k_cache", kc }, { "v_cache", vc }, { "block_table", table }, { "seq_ids", ids }, { "slots", slots } })
+            result.add(name, t);
+        if (n_tok && !result.check("gqa_norm_rope", 1, &q)) return nullptr;
+    }
+    apart.add("k_cache", kc); apart.add("v_cache", vc); apart.add("q", &q);
+    if (!apart.check("gqa_norm_rope", apart.count() - 1)) return nullptr;
     const int rc = unlocked([&] { return lib.norm_rope(&a, stream.st); });
     if (rc) return failed("gqa_norm_rope_launch", rc);
     return made.defined() ? THPVariable_Wrap(made) : Py_NewRef(o[17]);
@@ -611,9 +638,12 @@ PyObject * gqa_attn(PyObject *, PyObject * const * o, Py_ssize_t n) {
         REQUIRE(a.dst_type >= 0 && out.dim() == 3 && out.size(0) == n_seq && out.size(1) == n_head && out.size(2) == a.dv && rows_ok(out, 3, true));
         a.dst = out.data_ptr(); a.d_nb1 = step(out, 1); a.d_nb2 = step(out, 0);
     } else a.dst_type = MLA_TYPE_F32;
-    if (!lie_apart("gqa_attn", { "out", made.defined() ? nullptr : outp }, { { "q", &q }, { "k_cache", kc }, { "v_cache", vc }, { "block_table", table }, { "seq_lens", lens }, { "mask", mask }, { "weights", weights } }) ||
-        !lie_apart("gqa_attn", { "weights", weights }, { { "q", &q }, { "k_cache", kc }, { "v_cache", vc }, { "block_table", table }, { "seq_lens", lens }, { "mask", mask } }))
-        return nullptr;
+    Apart apart;
+    if (!made.defined()) apart.add("out", outp);
+    apart.add("weights", weights);
+    const int written = apart.count();
+    apart.add("q", &q); apart.add("k_cache", kc); apart.add("v_cache", vc); apart.add("block_table", table); apart.add("seq_lens", lens); apart.add("mask", mask);
+    if (!apart.check("gqa_attn", written)) return nullptr;
     const size_t need = lib.gqa_workspace_size(&a);
     GqaScratch scratch;
     if (!scratch.take(o[0], q, stream, need, a)) return nullptr;
@@ -659,13 +689,11 @@ PyObject * gqa_evict(PyObject *, PyObject * const * o, Py_ssize_t n) {
     REQUIRE(ints(fresh, n_seq));
     a.weights_dst = (float *) wo.data_ptr(); a.wd_nb1 = step(wo, 1); a.wd_nb2 = step(wo, 0);
     a.kept = (int32_t *) kept.data_ptr(); a.new_lens = (int32_t *) fresh.data_ptr();
-    const Named caches[] = { { "k_cache", kc }, { "v_cache", vc } };
-    if (!lie_apart("gqa_evict", { "weights_out", wop }, { { "weights", &q }, { "block_table", table }, { "seq_lens", lens }, caches[0], caches[1], { "kept", keptp }, { "new_lens", newp } }, &q) ||
-        !lie_apart("gqa_evict", { "kept", keptp }, { { "weights", &q }, { "block_table", table }, { "seq_lens", lens }, caches[0], caches[1], { "new_lens", newp } }) ||
-        !lie_apart("gqa_evict", { "new_lens", newp }, { { "weights", &q }, { "block_table", table }, { "seq_lens", lens }, caches[0], caches[1] }) ||
-        !lie_apart("gqa_evict", caches[0], { caches[1], { "weights", &q }, { "block_table", table }, { "seq_lens", lens } }) ||
-        !lie_apart("gqa_evict", caches[1], { { "weights", &q }, { "block_table", table }, { "seq_lens", lens } }))
-        return nullptr;
+    Apart apart;
+    apart.add("weights_out", wop); apart.add("kept", keptp); apart.add("new_lens", newp); apart.add("k_cache", kc); apart.add("v_cache", vc);
+    const int written = apart.count();
+    apart.add("weights", &q); apart.add("block_table", table); apart.add("seq_lens", lens);
+    if (!apart.check("gqa_evict", written, wop ? &q : nullptr)) return nullptr;
     GqaScratch scratch;
     if (!scratch.take(o[0], q, stream, lib.evict_workspace_size(&a), a)) return nullptr;
     const int rc = unlocked(a.workspace, [&] { return lib.evict(&a, stream.st); });
