@@ -517,8 +517,9 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
 // Scores of a latent cache (rows of 576, one KV head) for its weights: (m, l) and every score, as gqa_attn_kernel leaves them, without V.  Up to
 // 128 heads share a row, 128 flop a byte: the rows of Q lie in LDS (147 KB) and are read, 16 heads at a time, against a tile of 32 rows of K
 // in registers, by eight waves, so that every SIMD still has two.  The loop over blocks of heads is a loop: eight copies of its body, run once or
-// twice by a workgroup, took twice as long, most of it to fetch them.  8 x 8192 rows, 128 heads: 30 us, of which the rows are 12 at the
-// memory's rate and the products 7; then 4 to join and 8 to add them up.
+// twice by a workgroup, took twice as long, most of it to fetch them.  8 x 8192 rows, 128 heads: 30 us (8 of 5000
+// to 8192 rows: 27), of which the rows are 12 at the memory's rate, the products 4 to 7 and the reads of Q from LDS 4 side by side: what bounds it is one tile a
+// wave behind the staging of Q, and a chain of LDS reads, products, shuffles and exp2 a block of heads; then 4 to join and 8 to add them up.
 constexpr int LK = 576, LPITCH = LK * 2 + 16, LWAVES = 8, LROWS = 128;
 template <bool F16, bool BIAS>
 __global__ void __launch_bounds__(64 * LWAVES) gqa_scores_kernel(const AttnP p) {
