@@ -429,7 +429,7 @@ def gqa_attn(q, k_cache, v_cache, block_table, seq_lens, *, scale, logit_softcap
 
     q         [n_seq, n_head, dk], the cache's type or float32; n_head a multiple of the cache's heads
     k_cache, v_cache    bfloat16 or float16 [pages, 128, n_head_kv, dk | dv], (dk, dv) one of (64, 64), (128, 128), (192, 128), (256, 256)
-    block_table, seq_lens  int32 [n_seq, width], [n_seq]; window > 0: the last `window` rows alone
+    block_table, seq_lens  int32 [n_seq, width], [n_seq]; window > 0: the last `window` rows alone; logit_softcap: 0 or any finite cap
     mask      float16 [n_seq, n] or None, added to the scores; -inf takes a row out, a row past n is out
     weights   float32 [n_seq, n_head_kv, >= width * 128] or None: the softmax weights of a group's heads are added to it
     Returns out, [n_seq, n_head, dv] of q's type by default; a sequence without a row gets zeros.

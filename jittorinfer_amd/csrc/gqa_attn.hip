@@ -1000,6 +1000,7 @@ extern "C" int gqa_attn_check(const gqa_attn_args * a) {
     const int64_t lim = (int64_t) 1 << 31;
     if (a->bt_stride >= lim / 2 / PAGE || (int64_t) a->n_seq * a->n_head >= (1 << 24) || (int64_t) a->n_seq * a->n_head_kv > 65535 || (int64_t) a->n_seq * a->n_head * a->bt_stride >= lim)
         return MLA_ERR_BAD_SHAPE;
+    if (a->n_head / a->n_head_kv + SUM_BLOCKS >= (1 << 24)) return MLA_ERR_BAD_SHAPE;        // (the last launch: fewer than 2^32 threads, and nothing starts of a call whose last could not)
     int rc = check_pool(a->k);
     if (rc) return rc;
     if (a->dv) {

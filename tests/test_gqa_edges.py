@@ -151,3 +151,11 @@ int main() {
 """)
     subprocess.run(["g++", "-std=c++17", "-O2", "-Wall", "-Werror", "-I", os.path.join(ROOT, "jittorinfer_amd", "csrc"), str(src), "-o", str(tmp_path / "t")], check=True)
     assert subprocess.run([str(tmp_path / "t")], timeout=60).returncode == 0
+
+
+def test_attn_refuses_groups_whose_last_launch_could_not_start():
+    """A workgroup a head of a group and 2048 for the weights: fewer than 2^24."""
+    lib = J.library()
+    far = dict(n_seq=1, n_head_kv=1, bt_stride=1, q_nb1=256, q_nb2=1 << 33, weights=1 << 40, w_nb1=512, w_nb2=512, d_nb1=256, d_nb2=1 << 33)
+    assert lib.gqa_attn_check(C.byref(_attn(n_head=(1 << 24) - 2048, **far))) == SHAPE
+    assert lib.gqa_attn_check(C.byref(_attn(n_head=(1 << 24) - 2049, **far))) == 0
