@@ -145,7 +145,8 @@ __global__ void __launch_bounds__(256) gqa_norm_rope_kernel(const FrontP p) {
                     for (int e = 0; e < 8; e++) ss = fmaf(x[e], x[e], ss);
 #pragma unroll
                 for (int d = 1; d < LPR; d <<= 1) ss += __shfl_xor(ss, d, 64);
-                const float inv = __builtin_amdgcn_rsqf(fmaf(ss, p.inv_dk, p.eps));    // (off by 2^-23 of itself at most)
+                const float ms = fmaf(ss, p.inv_dk, p.eps);                              // (the instruction takes numbers below 2^-126 for 0)
+                const float inv = ms < 0x1p-100f ? __builtin_amdgcn_rsqf(ms * 0x1p64f) * 0x1p32f : __builtin_amdgcn_rsqf(ms);    // (off by 2^-23 of itself at most)
 #pragma unroll
                 for (int e = 0; e < 8; e++) x[e] = x[e] * inv * (isq ? gq[e] : gk[e]);
             }

@@ -526,3 +526,21 @@ def test_a_captured_decode_step(gpu):
             assert torch.equal(held[name], eager[name]), (i, name)
         assert held["new"].tolist() == [min(n, keep) for n in lens] and (held["out"][4] == 0).all() and not held["sums"][4].any()
         lens = [n + 1 if n else 0 for n in held["new"].tolist()]
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-40, 1e-38])
+def test_norm_rope_of_tiny_rows(gpu, eps):
+    """Mean squares below the smallest normal number with an eps that does not lift them: rows of unit size all the same, and zeros where eps holds them up."""
+    import jittorinfer_amd as J
+    gen = torch.Generator().manual_seed(92)
+    size = torch.tensor([1e-18, 1e-19, 5e-20, 1.0])[:, None, None]
+    q = (torch.rand((4, 3, 128), generator=gen) + 0.5) * size * torch.where(torch.rand((4, 3, 128), generator=gen) < 0.5, -1.0, 1.0)
+    w, pos = torch.rand(128, generator=gen) + 0.5, torch.arange(4, dtype=torch.int32)
+    want, off = R.heads(q, w, float(torch.tensor(eps, dtype=F32)), pos, 128, 2)
+    # squares, their sum, mean and eps step by 2^-149 down there: three times that of the mean square, half of it in its root
+    ms = (q.double() ** 2).mean(-1, keepdim=True) + eps
+    off = off + want.abs().amax(-1, keepdim=True) * 2 * 1.5 * 2.0 ** -149 / ms
+    got = J.gqa_norm_rope(q.to(gpu), None, None, pos.to(gpu), n_dims=128, mode=2, q_weight=w.to(gpu), eps=eps)
+    _near(got, want, off, F32)
+    if eps:
+        assert (J.gqa_norm_rope(torch.zeros((1, 2, 128), device=gpu), None, None, pos[:1].to(gpu), n_dims=128, mode=2, q_weight=w.to(gpu), eps=eps) == 0).all()
