@@ -160,7 +160,7 @@ def test_calls_on_a_captured_stream_that_is_not_the_current_one(gpu):
     c = [t.to(gpu) for t in _attn_case(55, [1024, 600], 8, 8, 2, 128, 128, F16)]
     want, out = J.gqa_attn(*c, scale=0.1), torch.empty((2, 8, 128), dtype=F16, device=gpu)
     inner, other = torch.cuda.Stream(), torch.cuda.Stream()
-    torch.cuda.synchronize()
+    capi.release_workspaces(inner.cuda_stream, gpu)                   # (streams come from a pool: this one may have had calls before)
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g, stream=inner):
         with torch.cuda.stream(other):
