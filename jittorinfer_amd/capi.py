@@ -72,11 +72,12 @@ def library():
             getattr(lib, name).argtypes = [C.POINTER(cls), C.c_void_p]
         lib.mla_front_batch_launch.restype = C.c_int
         lib.mla_front_batch_launch.argtypes = [C.POINTER(MlaFrontOp), C.c_int32, C.c_void_p]
-        for name, cls in (("gqa_norm_rope", GqaNormRopeArgs), ("gqa_attn", GqaAttnArgs), ("gqa_evict", GqaEvictArgs)):
+        for name, cls in (("gqa_norm_rope", GqaNormRopeArgs), ("gqa_attn", GqaAttnArgs), ("gqa_evict", GqaEvictArgs), ("gqa_prompt_attn", GqaPromptAttnArgs),
+                          ("gqa_cross_attn", GqaCrossAttnArgs)):
             getattr(lib, name + "_check").restype = getattr(lib, name + "_launch").restype = C.c_int
             getattr(lib, name + "_check").argtypes = [C.POINTER(cls)]
             getattr(lib, name + "_launch").argtypes = [C.POINTER(cls), C.c_void_p]
-        for name, cls in (("gqa_attn", GqaAttnArgs), ("gqa_evict", GqaEvictArgs)):
+        for name, cls in (("gqa_attn", GqaAttnArgs), ("gqa_evict", GqaEvictArgs), ("gqa_prompt_attn", GqaPromptAttnArgs), ("gqa_cross_attn", GqaCrossAttnArgs)):
             getattr(lib, name + "_workspace_size").restype = C.c_size_t
             getattr(lib, name + "_workspace_size").argtypes = [C.POINTER(cls)]
         lib.mla_page_table_create.restype = C.c_void_p
@@ -122,7 +123,8 @@ def native():
             raise RuntimeError("jittorinfer_amd/_native.so is missing or does not load (%s): build it with `python jittorinfer_amd/build.py`" % e)
         names = ("mla_attn_workspace_size", "mla_attn_launch", "mla_kv_write_launch", "mla_kv_write_rope_launch", "mla_rope_launch",
                  "mla_mul_mat_launch", "mla_copy_f32_launch", "mla_front_batch_launch", "gqa_norm_rope_launch", "gqa_attn_workspace_size",
-                 "gqa_attn_launch", "gqa_evict_workspace_size", "gqa_evict_launch")
+                 "gqa_attn_launch", "gqa_evict_workspace_size", "gqa_evict_launch", "gqa_prompt_attn_workspace_size", "gqa_prompt_attn_launch",
+                 "gqa_cross_attn_workspace_size", "gqa_cross_attn_launch")
         mod.bind(*[C.cast(getattr(lib, n), C.c_void_p).value for n in names], _workspace, _workspaces, torch._C._cuda_getCurrentRawStream,
                  torch._C._cuda_isCurrentStreamCapturing, _scratch_elsewhere)
         _native = mod
@@ -405,6 +407,24 @@ class GqaEvictArgs(C.Structure):
                 ("wd_nb2", C.c_int64), ("kept", C.c_void_p), ("new_lens", C.c_void_p), ("workspace", C.c_void_p), ("workspace_size", C.c_size_t)]
 
 
+class GqaPromptAttnArgs(C.Structure):
+    """gqa_prompt_attn_args of include/gqa_batch.h."""
+    _fields_ = [("n_tok", C.c_int32), ("n_seq", C.c_int32), ("n_head", C.c_int32), ("n_head_kv", C.c_int32), ("dk", C.c_int32), ("dv", C.c_int32),
+                ("type", C.c_int32), ("causal", C.c_int32), ("scale", C.c_float), ("logit_softcap", C.c_float), ("window", C.c_int32), ("n_workgroups", C.c_int32),
+                ("q", C.c_void_p), ("q_nb1", C.c_int64), ("q_nb2", C.c_int64), ("q_starts", C.c_void_p), ("k", GqaPool), ("v", GqaPool), ("n_pages", C.c_int64),
+                ("block_table", C.c_void_p), ("bt_stride", C.c_int64), ("seq_lens", C.c_void_p), ("mask", C.c_void_p), ("mask_nb1", C.c_int64),
+                ("mask_ne0", C.c_int64), ("dst", C.c_void_p), ("d_nb1", C.c_int64), ("d_nb2", C.c_int64), ("workspace", C.c_void_p), ("workspace_size", C.c_size_t)]
+
+
+class GqaCrossAttnArgs(C.Structure):
+    """gqa_cross_attn_args of include/gqa_batch.h."""
+    _fields_ = [("n_tok", C.c_int32), ("n_seq", C.c_int32), ("n_head", C.c_int32), ("n_head_kv", C.c_int32), ("dk", C.c_int32), ("dv", C.c_int32),
+                ("type", C.c_int32), ("n_workgroups", C.c_int32), ("scale", C.c_float), ("logit_softcap", C.c_float),
+                ("q", C.c_void_p), ("q_nb1", C.c_int64), ("q_nb2", C.c_int64), ("q_starts", C.c_void_p), ("k", GqaPool), ("v", GqaPool), ("n_kv", C.c_int64),
+                ("kv_starts", C.c_void_p), ("kv_lens", C.c_void_p), ("mask", C.c_void_p), ("mask_nb1", C.c_int64), ("mask_ne0", C.c_int64),
+                ("dst", C.c_void_p), ("d_nb1", C.c_int64), ("d_nb2", C.c_int64), ("workspace", C.c_void_p), ("workspace_size", C.c_size_t)]
+
+
 def gqa_norm_rope(q, k, v, pos, *, n_dims, mode=0, n_ctx_orig=0, freq_base=10000.0, freq_scale=1.0, ext_factor=0.0, attn_factor=1.0,
                   beta_fast=32.0, beta_slow=1.0, freq_factors=None, q_weight=None, k_weight=None, eps=1e-6, q_out=None,
                   k_cache=None, v_cache=None, block_table=None, seq_ids=None, slots=None, stream=None):
@@ -449,6 +469,34 @@ def gqa_evict(weights, block_table, seq_lens, k_cache, v_cache=None, *, n_keep, 
     Returns kept int32 [n_seq, n_head_kv, n_keep] (the row that is now row j, -1 past the new length), new_lens int32 [n_seq] and the
     weights that moved along, 0 past the new length (weights_out=weights: in place; columns past width * 128 stay as they are)."""
     return (_native or native()).gqa_evict(weights, block_table, seq_lens, k_cache, v_cache, n_keep, n_sink, n_recent, weights_out, kept, new_lens, stream)
+
+
+def gqa_prompt_attn(q, k_cache, v_cache, block_table, seq_lens, q_starts=None, *, scale, logit_softcap=0.0, window=0, causal=True, mask=None, out=None,
+                    n_workgroups=0, stream=None):
+    """Attention of many new tokens of every sequence over its pages -- a prompt, a chunk of one, draft tokens to verify -- whose keys and values gqa_norm_rope
+    has written, on the current torch stream (gqa_prompt_attn_launch, include/gqa_batch.h).
+
+    q         [n_tok, n_head, dk] of the cache's type; n_head a multiple of the cache's heads
+    k_cache, v_cache    bfloat16 or float16 [pages, 128, n_head_kv, dk | dv], (dk, dv) one of (64, 64), (128, 128), (192, 128), (256, 256)
+    block_table, seq_lens  int32 [n_seq, width], [n_seq]: rows of the cache, the new tokens' the last of them
+    q_starts  int32 [n_seq + 1], never falling: sequence b has the tokens q_starts[b] .. q_starts[b + 1] - 1 (None: n_tok / n_seq each); other tokens' rows of
+              out stay as they are
+    causal    a token sees the rows up to its own (False: all of its sequence's); window > 0: the last `window` of them alone; logit_softcap: 0 or any finite cap
+    mask      float16 [n_seq, n] or None, added to the scores of a sequence's tokens; -inf takes a row out, a row past n is out
+    Returns out, [n_tok, n_head, dv] of q's type; a token that sees no row gets zeros."""
+    return (_native or native()).gqa_prompt_attn(q, k_cache, v_cache, block_table, seq_lens, q_starts, scale, logit_softcap, window, causal, mask, out, n_workgroups, stream)
+
+
+def gqa_cross_attn(q, k, v, *, scale, q_starts=None, kv_starts=None, kv_lens=None, logit_softcap=0.0, mask=None, out=None, n_workgroups=0, stream=None):
+    """Attention of a decoder's tokens over an encoder's states, which have a length of their own, on the current torch stream (gqa_cross_attn_launch,
+    include/gqa_batch.h).
+
+    q         [n_tok, n_head, dk], the tokens of all sequences one behind the other; q_starts as in gqa_prompt_attn (None: n_tok / n_seq each -- one, in a decode step)
+    k, v      of q's type, any strides over contiguous rows: [n_seq, n, n_head_kv, dk | dv], padded, with kv_lens int32 [n_seq] (None: all n);
+              or [n, n_head_kv, dk | dv], packed, with kv_starts int32 [n_seq + 1] (with kv_lens too: [n_seq] is enough, and what lies behind a sequence's length is not read)
+    mask      float16 [n_seq, n] by state of the sequence, as in gqa_prompt_attn
+    Returns out, [n_tok, n_head, dv] of q's type; a token without a state gets zeros."""
+    return (_native or native()).gqa_cross_attn(q, k, v, q_starts, kv_starts, kv_lens, scale, logit_softcap, mask, out, n_workgroups, stream)
 
 
 class PageTable:

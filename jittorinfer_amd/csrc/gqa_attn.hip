@@ -30,7 +30,6 @@
 #include <limits.h>
 #include <math.h>
 
-#include <atomic>
 #include <type_traits>
 
 #include "gqa_common.hpp"
@@ -163,19 +162,7 @@ __device__ __forceinline__ u32x2 mask4(const AttnP & p, int b, int t, Span s) {
     for (int j = 0; j < 4; j++) h[j] = t + j >= s.first && t + j < s.last ? *(const unsigned short *) (src + 2 * j) : (unsigned short) 0xfc00;
     return u32x2{ h[0] | ((unsigned) h[1] << 16), h[2] | ((unsigned) h[3] << 16) };
 }
-// A score in log2 units from the product q . k, before the mask.  A soft cap c turns a score s into c tanh(y), y = s / c: 1 - 2 / (e^2y + 1) from y = 3/4 on,
-// of which a small y would keep no digits; there s itself times tanh(y) / y, by Lambert's continued fraction to y^2 / 9 (off by y^10 / 10^7: 6e-9), so that a
-// cap far above the scores leaves them as they are.  Either is off by 2^-21 of itself at most, and they share the reciprocal.
-template <bool BIAS> __device__ __forceinline__ float scaled(const AttnP & p, float a) {
-    const float s = p.scale_log2 * a;
-    if (BIAS && p.cap_out != 0.f) {
-        const float y = fabsf(p.cap_in * a), u = y * y;
-        const bool  small = y < 0.75f;
-        const float r = __builtin_amdgcn_rcpf(small ? fmaf(u, fmaf(u, 15.f, 420.f), 945.f) : fast_exp2(2.f * LOG2E * y) + 1.f);
-        return small ? s * (fmaf(u, u + 105.f, 945.f) * r) : copysignf(p.cap_out * fmaf(-2.f, r, 1.f), s);
-    }
-    return s;
-}
+template <bool BIAS> __device__ __forceinline__ float scaled(const AttnP & p, float a) { return BIAS ? scaled_score(p.scale_log2, p.cap_in, p.cap_out, a) : p.scale_log2 * a; }
 // Page `page` of a pool, at a head's offset (products of 32 bits are the scalar unit's; one of 64 would put the address into vector registers).
 __device__ __forceinline__ const char * page_base(const char * data, int page, unsigned nb_page, int64_t head) {
     return data + head + (int64_t) ((uint64_t) __umulhi((unsigned) page, nb_page) << 32 | (unsigned) page * nb_page);
@@ -911,18 +898,9 @@ Plan make_plan(const gqa_attn_args * a) {
     return pl;
 }
 
-// LDS over the 64 KB a kernel gets unasked: granted once a device, whatever it asks for later.
 template <typename K> hipError_t launch_lds(K kernel, const AttnP & p, int threads, int lds, std::atomic<uint64_t> & granted, hipStream_t st) {
-    if (lds >= 60 * 1024) {                                   // (the kernels' own shared arrays come on top)
-        int dev = 0;
-        hipError_t e = hipGetDevice(&dev);
-        if (e != hipSuccess) return e;
-        const uint64_t bit = dev < 64 ? (uint64_t) 1 << dev : 0;
-        if (!(granted.load(std::memory_order_relaxed) & bit)) {
-            if ((e = hipFuncSetAttribute((const void *) kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds)) != hipSuccess) return e;
-            granted.fetch_or(bit, std::memory_order_relaxed);
-        }
-    }
+    const hipError_t e = grant_lds(kernel, lds, granted);
+    if (e != hipSuccess) return e;
     hipLaunchKernelGGL(kernel, dim3((unsigned) p.n_wg), dim3((unsigned) threads), lds, st, p);
     return hipGetLastError();
 }

@@ -1,0 +1,44 @@
+// Attention of many query rows over the same keys (include/gqa_batch.h): what its host code and its kernels share.
+#pragma once
+
+#include "gqa_common.hpp"
+#include "../../include/gqa_batch.h"
+
+namespace mla {
+namespace gqa {
+
+// "Group": the queries that meet one run of keys -- the new tokens of a sequence, or a decoder's over its states.  Its query rows are
+// (token, head of the KV head's group), token-major, cut into blocks of BM.
+struct BatchP {
+    const char * q; int64_t q_nb1, q_nb2;
+    const char * k; int64_t k_page, k_head; int k_row;             // k_page: a page, or (no block table) a group's own part
+    const char * v; int64_t v_page, v_head; int v_row;
+    const int32_t * block_table; int64_t bt_stride, n_pages;       // block_table == nullptr: rows in one piece
+    const int32_t * kv_starts;
+    const int32_t * lens;
+    const int32_t * q_starts; int per;                             // q_starts == nullptr: `per` tokens a group
+    const char * mask; int64_t mask_nb1; int mask_len;             // mask_len: rows past it are out
+    char * dst; int64_t d_nb1, d_nb2;
+    float scale_log2;             // |scale| * log2(e)
+    unsigned flip;                // sign bits of a pair of values: Q is negated as it is read where the scale is negative
+    float cap_in, cap_out;        // soft cap c: |scale| / c and c * log2(e); cap_out = 0: none
+    int causal, window, n_grp, n_tok, n_head, n_head_kv, group;
+    int cap;                      // rows a group can have
+    int n_wg, min_tiles;          // workgroups, and the fewest tiles that are worth one
+    float *  part_o;              // [2 * n_wg][BM * dv]: unnormalized sums of the pieces of blocks that several workgroups share, in the lanes' order
+    float2 * part_ml;             // [2 * n_wg][BM]: reference (log2 units), sum
+    int4 *   items;               // [blocks at most][n_head_kv]: slot of the first piece, first workgroup, last workgroup
+};
+
+// Waves along the query rows and along the keys of a tile, keys of a tile.
+enum Shape { FOUR_ROWS, TWO_TWO, FOUR_KEYS };
+
+struct BatchPlan { Shape shape; int bm, n_wg, blocks; size_t off_ml, off_items, bytes; };
+
+template <bool F16> hipError_t batch_launch(const BatchP & p, const BatchPlan & pl, int dk, hipStream_t st);
+
+// Workgroups of a shape that a CU holds, by its registers and its tiles in LDS.
+constexpr int batch_wg_per_cu(int dk, Shape s) { return s == FOUR_KEYS ? (dk <= 64 ? 2 : 1) : dk <= 128 ? 2 : 1; }
+
+}  // namespace gqa
+}  // namespace mla

@@ -1,0 +1,604 @@
+// Attention of many query rows over the same keys (include/gqa_batch.h), for gfx950.
+//
+//   o[r] = sum_i p_i v_i,  p = softmax_i(scale * q[r] . k_i [soft cap] [+ mask]),  r = (token, head) of a group, i the rows that r sees
+//
+// A workgroup of four waves takes a block of query rows; tiles of keys and values come to LDS by direct loads (16 bytes a lane, no registers), the
+// next one while this one is worked on, swizzled so that both ways of reading them are free of bank conflicts.  Per tile and wave:
+//   * S^T = K Q^T by 32x32x16 MFMAs: a lane holds 16 scores of one query row a block of 32 keys, the other half of the wave the other 16.  Maximum and sum of
+//     a row are a lane's own business (and one exchange between the halves when the reference moves).
+//   * O^T += V^T P^T: the scores' registers, exponentiated and packed, are the second operand as they are (contraction index e of half g: key 4 g + e,
+//     then 8 + 4 g + e); V^T comes from LDS by transposing reads.  A lane's accumulators all belong to its query row: no rescaling across lanes.
+//   * the reference of a row moves only when a score passes it by 2^8 (f16: 2^4, with P up to 2^15, so that what f16 loses of a weight is 2^-11 of it down to
+//     2^-25 of the largest).
+//
+// Work: blocks in the order (group, KV head, block) have weights (keys they see, closed sums), and the workgroups take equal runs of the total weight, cut at
+// tiles, from the lengths on the device: a captured launch stays valid while they change.  A run that covers a block writes its result; the others
+// leave (o, m, l) for gqa_batch_join_kernel.
+#pragma once
+
+#include <limits.h>
+
+#include "gqa_batch.hpp"
+
+namespace mla {
+namespace gqa {
+namespace {
+
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ uint64_t uni64(uint64_t v) {
+    return (uint64_t) (unsigned) __builtin_amdgcn_readfirstlane((int) (v >> 32)) << 32 | (unsigned) __builtin_amdgcn_readfirstlane((int) v);
+}
+
+// 64 lanes, 16 bytes each: from base + off (a lane's own) to LDS at `lds`, lane by lane.  Waited for by dma_wait().
+__device__ __forceinline__ void dma16(uint64_t base, unsigned off, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(off), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void dma_wait() { __builtin_amdgcn_s_waitcnt(0x0f70); }              // vmcnt(0)
+
+// Place of 16-byte chunk c of row r in a tile of rows of D values: c ^ swizzle(r).  Rows 0 .. 15 of a chunk (the reads of K), and the 64 bytes that each of
+// four neighbouring rows gives to a transposing read of V, lie in banks of their own.
+template <int D> __device__ __forceinline__ int swizzle(int r) {
+    return D % 128 == 0 ? ((r & 3) << 2) | ((r >> 2) & 3) : ((r & 2) << 1) | ((r >> 2) & 3);
+}
+
+struct Group { int q0, nq, len; int64_t row0; };
+__device__ __forceinline__ Group group_of(const BatchP & p, int g) {
+    Group r;
+    r.q0 = p.q_starts ? min(max(p.q_starts[g], 0), p.n_tok) : g * p.per;
+    r.nq = p.q_starts ? min(max(p.q_starts[g + 1], r.q0), p.n_tok) - r.q0 : p.per;
+    r.row0 = 0;
+    int most = p.cap;
+    if (p.kv_starts) {
+        const int at = p.kv_starts[g];
+        most = at < 0 || at > p.cap ? 0 : p.cap - at;
+        r.row0 = most ? at : 0;
+    }
+    r.len = min(max(p.lens ? p.lens[g] : p.kv_starts ? p.kv_starts[g + 1] - p.kv_starts[g] : p.cap, 0), most);
+    return r;
+}
+// What token j of the group sees: rows [first, last).
+struct Span { int first, last; };
+__device__ __forceinline__ Span span_of(const BatchP & p, const Group & g, int j) {
+    const int end = p.causal ? min(max(g.len - g.nq + j + 1, 0), g.len) : g.len;
+    return Span{ p.window > 0 ? max(end - p.window, 0) : 0, min(end, p.mask_len) };
+}
+template <int BM> __device__ __forceinline__ int blocks_of(const BatchP & p, const Group & g) { return (int) (((int64_t) g.nq * p.group + BM - 1) / BM); }
+// The tiles that some row of block j sees: [first, last).
+template <int BM, int TK> __device__ __forceinline__ Span tiles_of(const BatchP & p, const Group & g, int j) {
+    const int64_t rows = (int64_t) g.nq * p.group, r0 = (int64_t) j * BM;
+    const int lo = span_of(p, g, (int) (r0 / p.group)).first, hi = span_of(p, g, (int) ((r0 + BM < rows ? r0 + BM : rows) - 1) / p.group).last;
+    return hi > lo ? Span{ lo / TK, (hi + TK - 1) / TK } : Span{ 0, 0 };
+}
+
+// ---- the deal
+// sum over i < n of a + i s, each held to [0, top]
+__device__ __forceinline__ int64_t sum_clamped(int64_t a, int s, int64_t top, int64_t n) {
+    const int64_t i0 = a >= 0 ? 0 : min(n, (-a + s - 1) / s), i1 = a >= top ? 0 : min(n, (top - a + s - 1) / s), mid = i1 - i0;
+    return mid * a + s * ((i0 + i1 - 1) * mid / 2) + (n - i1) * top;
+}
+// Weight of blocks 0 .. n - 1 of a group: the keys each sees, times the heads of the KV head's group, and 128 keys for what a block costs by itself.
+template <int BM> __device__ __forceinline__ int64_t weight_before(const BatchP & p, const Group & g, int64_t n) {
+    const int64_t G = p.group, all = G * g.len;
+    int64_t keys;
+    if (p.causal) {
+        keys = sum_clamped(G * (g.len - g.nq) + BM, BM, all, n);
+        if (p.window > 0) keys -= sum_clamped(G * (g.len - g.nq + 1 - (int64_t) p.window), BM, all, n);
+    } else keys = n * (p.window > 0 ? min(all, G * p.window) : all);
+    return keys + n * G * 128;
+}
+__device__ __forceinline__ int64_t scan64(int64_t v, int lane) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) { const int64_t o = __shfl_up(v, d, 64); if (lane >= d) v += o; }
+    return v;
+}
+template <int BM> __device__ __forceinline__ int64_t total_weight(const BatchP & p, int lane) {
+    int64_t total = 0;
+    for (int g0 = 0; g0 < p.n_grp; g0 += 64) {
+        int64_t w = 0;
+        if (g0 + lane < p.n_grp) { const Group g = group_of(p, g0 + lane); w = weight_before<BM>(p, g, blocks_of<BM>(p, g)) * p.n_head_kv; }
+        total += __shfl(scan64(w, lane), 63, 64);
+    }
+    return total;
+}
+struct Pos { int g, kvh, j, tile; };             // tile: counted from the block's first
+__device__ __forceinline__ bool same_item(const Pos & a, const Pos & b) { return a.g == b.g && a.kvh == b.kvh && a.j == b.j; }
+template <int BM, int TK> __device__ __forceinline__ Pos place(const BatchP & p, int lane, int64_t at) {
+    int64_t before = 0;
+    for (int g0 = 0; g0 < p.n_grp; g0 += 64) {
+        int64_t w = 0;
+        if (g0 + lane < p.n_grp) { const Group g = group_of(p, g0 + lane); w = weight_before<BM>(p, g, blocks_of<BM>(p, g)) * p.n_head_kv; }
+        const int64_t incl = scan64(w, lane) + before;
+        const uint64_t past = __ballot(at < incl);
+        if (past) {
+            const int l = __ffsll((unsigned long long) past) - 1, gi = uni(g0 + l);
+            const Group   g   = group_of(p, gi);
+            const int     nb  = blocks_of<BM>(p, g);
+            const int64_t per = weight_before<BM>(p, g, nb);
+            int64_t rest = at - __shfl(incl - w, l, 64);
+            const int kvh = (int) (rest / per);
+            rest -= kvh * per;
+            int lo = 0, hi = nb;                                  // weight_before(lo) <= rest < weight_before(hi)
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (weight_before<BM>(p, g, mid) <= rest) lo = mid;
+                else hi = mid;
+            }
+            rest -= weight_before<BM>(p, g, lo);
+            const int64_t mine = weight_before<BM>(p, g, lo + 1) - weight_before<BM>(p, g, lo);
+            const Span    t = tiles_of<BM, TK>(p, g, lo);
+            return Pos{ gi, uni(kvh), uni(lo), uni((int) (rest * (t.last - t.first) / mine)) };
+        }
+        before = __shfl(incl, 63, 64);
+    }
+    return Pos{ p.n_grp, 0, 0, 0 };
+}
+// Number of block j of group g among all, an upper bound's worth apart: blocks_of(g) are at most the numbers between two groups.
+template <int BM> __device__ __forceinline__ int64_t number_of(const BatchP & p, int g, int q0) { return (int64_t) q0 * p.group / BM + g; }
+
+__device__ __forceinline__ u32x4 lds128(unsigned at) { return *(LDS_PTR(const u32x4)) (uintptr_t) at; }
+// Four rows' values of this lane's column, twice: rows r .. r + 3 and r + 8 .. r + 11 of the transposed operand.
+__device__ __forceinline__ u32x4 lds_transposed(unsigned lo, unsigned hi) {
+    const u32x2 a = bitcast<u32x2>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4)) (uintptr_t) lo)), b = bitcast<u32x2>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4)) (uintptr_t) hi));
+    return u32x4{ a.x, a.y, b.x, b.y };
+}
+// l + the two 16-bit numbers of `pair`: the sum is over the weights as they are multiplied, so that a row of one key gets its value as it is.
+template <bool F16> __device__ __forceinline__ float add_pair(float l, unsigned pair) {
+    if constexpr (F16) return __builtin_amdgcn_fdot2(bitcast<f16x2>(pair), f16x2{ (_Float16) 1.f, (_Float16) 1.f }, l, false);
+    else               return __builtin_amdgcn_fdot2_f32_bf16(bitcast<bf16x2>(pair), bf16x2{ (__bf16) 1.f, (__bf16) 1.f }, l, false);
+}
+// ---- infinities and NaN among values: 0 * them must not count where a row does not see their key.  Two 16-bit numbers at a time.
+template <bool F16> __device__ __forceinline__ unsigned nonfinite(unsigned x) {                // bits 15 and 31: of the halves that are
+    return ((x & (F16 ? 0x7c007c00u : 0x7f807f80u)) + (F16 ? 0x04000400u : 0x00800080u)) & 0x80008000u;
+}
+__device__ __forceinline__ unsigned halves(unsigned bits15) { return (bits15 >> 15) * 0xffffu; }  // all bits of those halves
+
+template <bool F16> __device__ __forceinline__ u32x2 pack4(float a, float b, float c, float d) { return u32x2{ pair16<F16>(a, b), pair16<F16>(c, d) }; }
+
+template <bool F16, int DK, int DV, int NWQ, int NWK, int TK, int OCC, bool BIAS>
+__global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const BatchP p) {
+    constexpr int NW = NWQ * NWK, BM = 32 * NWQ, KW = TK / NWK, KB = KW / 32, KC = DK / 16, NV = DV / 32;
+    constexpr int KT = TK * DK * 2, VT = TK * DV * 2, KI = KT / 1024 / NW, VI = VT / 1024 / NW;
+    static_assert(KW % 32 == 0 && KI * 1024 * NW == KT && VI * 1024 * NW == VT, "whole pieces");
+    constexpr float REF = F16 ? 11.f : 0.f, SLACK = F16 ? 4.f : 8.f;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    __shared__ float2 sh_ml[NWK > 1 ? NW : 1][NWK > 1 ? 32 : 1];
+    __shared__ int    sh_bad[2][NW];
+
+    const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), wq = wave % NWQ, wk = wave / NWQ, l31 = lane & 31, hh = lane >> 5;
+    const unsigned lds0 = (unsigned) (uintptr_t) (LDS_PTR(char)) lds;
+
+    // ---- this workgroup's run
+    const int64_t total = total_weight<BM>(p, lane);
+    if (total == 0) return;
+    const int64_t least = (int64_t) p.min_tiles * TK * p.group;
+    const int     runs = (int) max((int64_t) 1, min((int64_t) p.n_wg, total / least));
+    // (workgroups go to the eight dies in turn: neighbouring runs, which share keys, to the same one)
+    if ((int) blockIdx.x >= runs) return;
+    const int x = blockIdx.x & 7, run = uni(x * (runs >> 3) + min(x, runs & 7) + (int) (blockIdx.x >> 3));
+    Pos       at  = place<BM, TK>(p, lane, total / runs * run + min((int64_t) run, total % runs));
+    const Pos end = place<BM, TK>(p, lane, total / runs * (run + 1) + min((int64_t) run + 1, total % runs));
+
+    // ---- what does not change: a lane's places in the tiles
+    const int thread = wave * 64 + lane;                              // load j of a tile: 16-byte pieces j * 64 * NW + thread of it
+    auto row_in = [&](int d, int j) { return (j * 64 * NW + thread) / (d / 8); };
+    auto chunk_in = [&](int d, int j) { const int r = row_in(d, j), c = (j * 64 * NW + thread) % (d / 8); return c ^ (d % 128 == 0 ? swizzle<128>(r) : swizzle<64>(r)); };
+    // rows of a tile that lie KS apart have the same places: one offset a lane, and the step is the base's
+    constexpr int KS = (512 * NW / DK) % 16 == 0 && 512 % DK == 0 ? 512 * NW / DK : 0, VS = (512 * NW / DV) % 16 == 0 && 512 % DV == 0 ? 512 * NW / DV : 0;
+    unsigned k_at[KS ? 1 : KI], v_at[VS ? 1 : VI];
+#pragma unroll
+    for (int j = 0; j < (KS ? 1 : KI); j++) k_at[j] = (unsigned) (row_in(DK, j) * p.k_row + chunk_in(DK, j) * 16);
+#pragma unroll
+    for (int j = 0; j < (VS ? 1 : VI); j++) v_at[j] = (unsigned) (row_in(DV, j) * p.v_row + chunk_in(DV, j) * 16);
+    // transposing reads: row, 16-byte chunk and half of it; the addresses of a chunk of 32 columns, for rows 0 .. 3 and 8 .. 11 of 16
+    const int vq = hh * 4 + ((lane >> 2) & 3), vc = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), vsub = (lane & 1) * 8;
+    unsigned v_lo[NV], v_hi[NV];
+#pragma unroll
+    for (int n = 0; n < NV; n++) {
+        v_lo[n] = vq * (DV * 2) + (((n * 4 + vc) ^ swizzle<DV>(vq)) * 16) + vsub;
+        v_hi[n] = (vq + 8) * (DV * 2) + (((n * 4 + vc) ^ swizzle<DV>(vq + 8)) * 16) + vsub;
+    }
+    unsigned k_lo[KC];
+#pragma unroll
+    for (int c = 0; c < KC; c++) k_lo[c] = l31 * (DK * 2) + (((2 * c + hh) ^ swizzle<DK>(l31)) * 16);
+
+    for (; at.g < p.n_grp;) {
+        const Group g = group_of(p, at.g);
+        const int   nb = blocks_of<BM>(p, g);
+        const Span  ts = nb > 0 ? tiles_of<BM, TK>(p, g, at.j) : Span{ 0, 0 };
+        const int   nt = ts.last - ts.first;
+        const bool  ends_here = same_item(at, end);
+        const int   t0 = uni(ts.first + at.tile), t1 = uni(ends_here ? ts.first + end.tile : ts.last);
+        const bool  begins = at.tile == 0, whole = begins && !ends_here;
+        const int   slot = 2 * run + (begins ? 1 : 0);
+        const int   row0 = at.j * BM + wq * 32;
+        const int64_t item = (number_of<BM>(p, at.g, g.q0) + at.j) * p.n_head_kv + at.kvh;
+
+        if (t0 < t1) {
+            if (threadIdx.x == 0) {
+                if (begins) { p.items[item].x = slot; p.items[item].y = run; }
+                if (!ends_here) p.items[item].z = run;
+            }
+            // ---- this lane's query row (rows past the last repeat it)
+            const int  rows = g.nq * p.group, r = min(row0 + l31, rows - 1), tok = r / p.group, head = at.kvh * p.group + r - tok * p.group;
+            const Span s = span_of(p, g, tok);
+            // the tiles all rows of the wave see whole, and those any sees: for all rows from the first's to the last's span (spans move on with the token)
+            const Span s_first = Span{ uni(__shfl(s.first, 0, 64)), uni(__shfl(s.last, 0, 64)) }, s_last = Span{ uni(__shfl(s.first, 31, 64)), uni(__shfl(s.last, 31, 64)) };
+            // and the first and the last row of the block
+            const int64_t last_row = min((int64_t) (at.j + 1) * BM, (int64_t) rows) - 1;
+            const Span b_first = span_of(p, g, at.j * BM / p.group), b_last = span_of(p, g, (int) last_row / p.group);
+            const char * mask = BIAS && p.mask ? p.mask + (int64_t) at.g * p.mask_nb1 : nullptr;
+
+            const int64_t k_off = (int64_t) at.kvh * p.k_head + (p.block_table ? 0 : at.g * p.k_page + g.row0 * p.k_row);
+            const int64_t v_off = (int64_t) at.kvh * p.v_head + (p.block_table ? 0 : at.g * p.v_page + g.row0 * p.v_row);
+            const uint64_t k_base = uni64((uint64_t) (uintptr_t) p.k + (uint64_t) k_off), v_base = uni64((uint64_t) (uintptr_t) p.v + (uint64_t) v_off);
+            const int32_t * pages = p.block_table + (p.block_table ? (int64_t) at.g * p.bt_stride : 0);
+            auto good = [&](int id) { return id >= 0 && id < p.n_pages; };
+            auto page_at = [&](int t) { return uni(pages[t * TK / PAGE]); };
+            auto fetch = [&](int t, int id, int buf) {                // tile t to LDS
+                const int key0 = t * TK, valid = min(TK, g.len - key0), pg = good(id) ? id : 0;       // (a bad id: page 0 is read, not used)
+                const int row = p.block_table ? key0 % PAGE : key0;
+                const uint64_t kb = uni64(k_base + (uint64_t) ((p.block_table ? pg * p.k_page : 0) + (int64_t) row * p.k_row));
+                const uint64_t vb = uni64(v_base + (uint64_t) ((p.block_table ? pg * p.v_page : 0) + (int64_t) row * p.v_row));
+                const unsigned to = uni(lds0 + buf * (KT + VT) + wave * 1024);
+                if (valid == TK) {
+#pragma unroll
+                    for (int j = 0; j < KI; j++) dma16(kb + (KS ? (uint64_t) (j * KS) * p.k_row : 0), k_at[KS ? 0 : j], to + j * NW * 1024);
+#pragma unroll
+                    for (int j = 0; j < VI; j++) dma16(vb + (VS ? (uint64_t) (j * VS) * p.v_row : 0), v_at[VS ? 0 : j], to + KT + j * NW * 1024);
+                } else {                                              // (rows past the last repeat it)
+#pragma unroll
+                    for (int j = 0; j < KI; j++) dma16(kb, (unsigned) (min(row_in(DK, j), valid - 1) * p.k_row + chunk_in(DK, j) * 16), to + j * NW * 1024);
+#pragma unroll
+                    for (int j = 0; j < VI; j++) dma16(vb, (unsigned) (min(row_in(DV, j), valid - 1) * p.v_row + chunk_in(DV, j) * 16), to + KT + j * NW * 1024);
+                }
+            };
+            // (the mask's numbers of the next tile are requested ahead of its keys: a wait for them is no wait for those)
+            u32x2 mk[KB][4], mk_next[KB][4];
+            auto fetch_mask = [&](int t, u32x2 (&to)[KB][4]) {
+                if constexpr (BIAS)
+                    if (mask)
+#pragma unroll
+                        for (int b = 0; b < KB; b++)
+#pragma unroll
+                            for (int c = 0; c < 4; c++) {
+                                const int i = t * TK + wk * KW + b * 32 + c * 8 + hh * 4;
+                                const char * src = mask + (int64_t) i * 2;
+                                if (i + 4 <= s.last && ((uintptr_t) src & 7) == 0) to[b][c] = *(const u32x2 *) src;
+                                else {
+                                    unsigned short h[4];
+#pragma unroll
+                                    for (int e = 0; e < 4; e++) h[e] = i + e < s.last ? *(const unsigned short *) (src + 2 * e) : (unsigned short) 0xfc00;
+                                    to[b][c] = u32x2{ h[0] | ((unsigned) h[1] << 16), h[2] | ((unsigned) h[3] << 16) };
+                                }
+                            }
+            };
+
+            __syncthreads();                                          // (LDS is free of the piece before)
+            fetch_mask(t0, mk);
+            int id = p.block_table ? page_at(t0) : 0, id_next = p.block_table && t0 + 1 < t1 ? page_at(t0 + 1) : 0;
+            fetch(t0, id, 0);
+            u32x4 qf[KC];
+            {
+                const char * src = p.q + (int64_t) (g.q0 + tok) * p.q_nb2 + (int64_t) head * p.q_nb1 + hh * 16;
+#pragma unroll
+                for (int c = 0; c < KC; c++) {
+                    qf[c] = *(const u32x4 *) (src + c * 32);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) qf[c][e] ^= p.flip;
+                }
+            }
+            float  m = -INFINITY, l = 0.f;
+            unsigned up[(NV + 1) / 2] = {}, down[(NV + 1) / 2] = {};  // results that a +infinity (-infinity, NaN: both) of a tile not seen by all rows belongs to
+            f32x16 acc[NV];
+#pragma unroll
+            for (int n = 0; n < NV; n++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[n][e] = 0.f;
+
+            // S^T of the wave's keys
+            auto products = [&](unsigned kt, f32x16 (&sc)[KB]) {
+#pragma unroll
+                for (int b = 0; b < KB; b++) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) sc[b][e] = 0.f;
+#pragma unroll
+                    for (int c = 0; c < KC; c++) sc[b] = mfma32<F16>(lds128(kt + b * 32 * (DK * 2) + k_lo[c]), qf[c], sc[b]);
+                }
+            };
+            auto value = [&](unsigned vt, int b, int kk, int n) { const unsigned at16 = vt + (b * 32 + kk * 16) * (DV * 2); return lds_transposed(at16 + v_lo[n], at16 + v_hi[n]); };
+
+            for (int t = t0; t < t1; t++) {
+                dma_wait();
+                __syncthreads();
+                const int  buf = (t - t0) & 1, key0 = t * TK + wk * KW;
+                const bool use = !p.block_table || good(id);
+                if (t + 1 < t1) {
+                    fetch_mask(t + 1, mk_next);
+                    id = id_next;
+                    fetch(t + 1, id, buf ^ 1);
+                    if (p.block_table && t + 2 < t1) id_next = page_at(t + 2);
+                }
+                const unsigned kt = uni(lds0 + buf * (KT + VT) + wk * KW * (DK * 2)), vt = uni(lds0 + buf * (KT + VT) + KT + wk * KW * (DV * 2));
+                // ---- a tile that not all rows of the block see whole: infinities and NaN among its values are noted for the rows that see them, and become zeros
+                if ((BIAS && mask) || t * TK < b_last.first || t * TK + TK > b_first.last) {
+                    unsigned bad = 0;
+                    const unsigned mine = lds0 + buf * (KT + VT) + KT + threadIdx.x * 16;
+#pragma unroll
+                    for (int i = 0; i < VI; i++) {
+                        const u32x4 x = lds128(mine + i * NW * 1024);
+                        bad |= nonfinite<F16>(x.x) | nonfinite<F16>(x.y) | nonfinite<F16>(x.z) | nonfinite<F16>(x.w);
+                    }
+                    const int found = __any(bad != 0);
+                    if (lane == 0) sh_bad[buf][wave] = found;
+                    __syncthreads();
+                    int any = 0;
+#pragma unroll
+                    for (int w = 0; w < NW; w++) any |= sh_bad[buf][w];
+                    if (uni(any)) {
+#pragma unroll 1
+                        for (int i = 0; i < KW; i++) {
+                            const int key = key0 + i;
+                            bool sees = use && key >= s.first && key < s.last;
+                            if constexpr (BIAS) if (mask && sees) sees = *(const unsigned short *) (mask + (int64_t) key * 2) != 0xfc00;
+#pragma unroll
+                            for (int n = 0; n < NV; n++)
+#pragma unroll
+                                for (int c = 0; c < 4; c++) {
+                                    const u32x2 x = *(LDS_PTR(const u32x2)) (uintptr_t) (vt + i * (DV * 2) + (((n * 4 + c) ^ swizzle<DV>(i)) * 16) + hh * 8);
+#pragma unroll
+                                    for (int e = 0; e < 4; e++) {
+                                        const float    f   = from16<F16>((unsigned short) (x[e >> 1] >> (16 * (e & 1))));
+                                        const unsigned bit = 1u << ((n & 1) * 16 + 4 * c + e);
+                                        if (sees && !(f < INFINITY)) up[n / 2] |= bit;                          // infinity or NaN
+                                        if (sees && !(f > -INFINITY)) down[n / 2] |= bit;
+                                    }
+                                }
+                        }
+                        __syncthreads();
+#pragma unroll
+                        for (int i = 0; i < VI; i++) {
+                            u32x4 x = lds128(mine + i * NW * 1024);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) x[e] &= ~halves(nonfinite<F16>(x[e]));
+                            *(LDS_PTR(u32x4)) (uintptr_t) (mine + i * NW * 1024) = x;
+                        }
+                        __syncthreads();
+                    }
+                }
+                if (use && key0 < s_last.last && key0 + KW > s_first.first) {
+                    f32x16 sc[KB];
+                    u32x4  pf[KB][2];
+                    products(kt, sc);
+                    float top, unit = p.scale_log2;                   // what makes log2 units of sc
+                    if (!BIAS && key0 + KW <= s_first.last && key0 >= s_last.first) {
+                        top = sc[0][0];
+#pragma unroll
+                        for (int b = 0; b < KB; b++)
+#pragma unroll
+                            for (int e = 0; e < 16; e++) top = fmaxf(top, sc[b][e]);
+                        top *= unit;
+                    } else {
+                        const bool all = key0 + KW <= s_first.last && key0 >= s_last.first;
+                        top = -INFINITY;
+#pragma unroll
+                        for (int b = 0; b < KB; b++)
+#pragma unroll
+                            for (int e = 0; e < 16; e++) {
+                                float v = sc[b][e];
+                                if constexpr (BIAS) {
+                                    v = scaled_score(p.scale_log2, p.cap_in, p.cap_out, v);
+                                    if (mask) {
+                                        const float f = f16_bits_to_f32((mk[b][e >> 2][(e >> 1) & 1] >> (16 * (e & 1))) & 0xffffu);
+                                        v = f == -INFINITY ? -INFINITY : fmaf(f, LOG2E, v);
+                                    }
+                                } else v *= p.scale_log2;
+                                if (!all) {
+                                    const int i = key0 + b * 32 + (e >> 2) * 8 + hh * 4 + (e & 3);
+                                    if (i < s.first || i >= s.last) v = -INFINITY;
+                                }
+                                sc[b][e] = v;
+                                top = fmaxf(top, v);
+                            }
+                        unit = 1.f;
+                    }
+                    if (__any(top > m + (REF + SLACK))) {             // the reference moves
+                        top = fmaxf(top, xor32(top));
+                        const float nm = fmaxf(top - REF, m);
+                        const float a  = m == nm ? 1.f : fast_exp2(m - nm);
+                        m = nm;
+                        l *= a;
+#pragma unroll
+                        for (int n = 0; n < NV; n++)
+#pragma unroll
+                            for (int e = 0; e < 16; e++) acc[n][e] *= a;
+                    }
+                    const float mm = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                    for (int b = 0; b < KB; b++)
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) {
+                            const unsigned h = pair16<F16>(fast_exp2(fmaf(sc[b][e], unit, -mm)), fast_exp2(fmaf(sc[b][e + 1], unit, -mm)));
+                            l = add_pair<F16>(l, h);
+                            pf[b][e >> 3][(e >> 1) & 3] = h;
+                        }
+#pragma unroll
+                    for (int b = 0; b < KB; b++)
+#pragma unroll
+                        for (int kk = 0; kk < 2; kk++)
+#pragma unroll
+                            for (int n = 0; n < NV; n++) acc[n] = mfma32<F16>(value(vt, b, kk, n), pf[b][kk], acc[n]);
+                }
+                if constexpr (BIAS)
+#pragma unroll
+                    for (int b = 0; b < KB; b++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) mk[b][c] = mk_next[b][c];
+            }
+            bool noted = false;
+#pragma unroll
+            for (int n = 0; n < (NV + 1) / 2; n++) noted = noted || (up[n] | down[n]) != 0;
+            if (__any(noted)) {
+#pragma unroll
+                for (int n = 0; n < NV; n++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const unsigned bit = 1u << ((n & 1) * 16 + e);
+                        if (up[n / 2] & bit) acc[n][e] += INFINITY;
+                        if (down[n / 2] & bit) acc[n][e] -= INFINITY;
+                    }
+            }
+            l += xor32(l);
+
+            if constexpr (NWK > 1) {                                  // the waves that took other keys of the same rows
+                if (hh == 0) sh_ml[wave][l31] = make_float2(m, l);
+                __syncthreads();
+                float M = -INFINITY, L = 0.f;
+#pragma unroll
+                for (int w = 0; w < NWK; w++) M = fmaxf(M, sh_ml[w * NWQ + wq][l31].x);
+#pragma unroll
+                for (int w = 0; w < NWK; w++) { const float2 ml = sh_ml[w * NWQ + wq][l31]; L += ml.y == 0.f ? 0.f : ml.y * fast_exp2(ml.x - M); }
+                const float f = l == 0.f ? 0.f : fast_exp2(m - M);
+                f32x4 * box = (f32x4 *) lds + (size_t) (wave - NWQ) * NV * 4 * 64 + lane;
+                if (wk > 0) {
+#pragma unroll
+                    for (int n = 0; n < NV; n++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) box[(n * 4 + c) * 64] = f32x4{ acc[n][4 * c], acc[n][4 * c + 1], acc[n][4 * c + 2], acc[n][4 * c + 3] } * f;
+                }
+                __syncthreads();
+                if (wk == 0) {
+#pragma unroll
+                    for (int n = 0; n < NV; n++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            f32x4 o = f32x4{ acc[n][4 * c], acc[n][4 * c + 1], acc[n][4 * c + 2], acc[n][4 * c + 3] } * f;
+#pragma unroll
+                            for (int w = 1; w < NWK; w++) o += ((const f32x4 *) lds)[(size_t) ((w - 1) * NWQ + wq) * NV * 4 * 64 + (n * 4 + c) * 64 + lane];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) acc[n][4 * c + e] = o[e];
+                        }
+                }
+                m = M; l = L;
+            }
+            if (wk == 0) {
+                if (whole) {
+                    const float inv = l == 0.f ? 0.f : 1.f / l;       // (a NaN stays one)
+                    char * dst = p.dst + (int64_t) (g.q0 + tok) * p.d_nb2 + (int64_t) head * p.d_nb1 + hh * 8;
+                    if (row0 + l31 < rows)
+#pragma unroll
+                        for (int n = 0; n < NV; n++)
+#pragma unroll
+                            for (int c = 0; c < 4; c++)
+                                *(u32x2 *) (dst + n * 64 + c * 16) = pack4<F16>(acc[n][4 * c] * inv, acc[n][4 * c + 1] * inv, acc[n][4 * c + 2] * inv, acc[n][4 * c + 3] * inv);
+                } else {
+                    f32x4 * to = (f32x4 *) p.part_o + (int64_t) slot * (BM * DV / 4) + wq * 64 + lane;
+#pragma unroll
+                    for (int n = 0; n < NV; n++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) to[(n * 4 + c) * NWQ * 64] = f32x4{ acc[n][4 * c], acc[n][4 * c + 1], acc[n][4 * c + 2], acc[n][4 * c + 3] };
+                    if (hh == 0) p.part_ml[(int64_t) slot * BM + wq * 32 + l31] = make_float2(m, l);
+                }
+            }
+        } else if (ends_here && at.tile > 0) {                        // nothing of a block that others share: an empty piece
+            for (int i = threadIdx.x; i < BM; i += 64 * NW) p.part_ml[(int64_t) slot * BM + i] = make_float2(-INFINITY, 0.f);
+        }
+        if (ends_here) return;
+        at.tile = 0;
+        if (++at.j >= nb) {
+            at.j = 0;
+            if (++at.kvh == p.n_head_kv) {
+                at.kvh = 0;
+                do at.g++; while (at.g < p.n_grp && blocks_of<BM>(p, group_of(p, at.g)) == 0);
+            }
+        }
+    }
+}
+
+// Joins the pieces of one block: o = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M), in the order of the keys.  Blocks that one run covered are done; rows without a key
+// get zeros.  Grid: x = block numbers, y = KV heads, z = 32 columns of the result.
+template <bool F16, int DV, int NWQ, int TK>
+__global__ void __launch_bounds__(256) gqa_batch_join_kernel(const BatchP p) {
+    constexpr int BM = 32 * NWQ;
+    const int lane = threadIdx.x & 63;
+    const int64_t id = blockIdx.x;
+    // the group this number belongs to: the last whose first number is not past it, 64 tried at a time
+    int lo = 0, n = p.n_grp;
+    while (n > 1) {
+        const int step = (n + 63) / 64, g = lo + lane * step;
+        const bool in = lane * step < n;
+        const int q0 = !in ? 0 : p.q_starts ? min(max(p.q_starts[g], 0), p.n_tok) : g * p.per;
+        const int last = 63 - __clzll((long long) (__ballot(in && number_of<BM>(p, g, q0) <= id) | 1));
+        n = min(step, n - last * step);
+        lo += last * step;
+    }
+    lo = uni(lo);
+    const Group   g = group_of(p, lo);
+    const int64_t j = id - number_of<BM>(p, lo, g.q0);
+    if (j < 0 || j >= blocks_of<BM>(p, g)) return;
+    const Span ts = tiles_of<BM, TK>(p, g, (int) j);
+    const bool none = ts.last == ts.first;
+    int4 it = make_int4(0, 0, 0, 0);
+    if (!none) {
+        it = p.items[id * p.n_head_kv + blockIdx.y];
+        if (it.y == it.z) return;
+    }
+    const int pieces = none ? 0 : uni(it.z - it.y + 1), first = uni(it.x), run0 = uni(it.y);
+    auto slot = [&](int i) -> int64_t { return i ? 2 * (run0 + i) : first; };
+    for (int e = threadIdx.x; e < 4 * NWQ * 64; e += 256) {
+        const int c = e / (NWQ * 64), wq = (e / 64) % NWQ, row = wq * 32 + (lane & 31);
+        float M = -INFINITY, L = 0.f;
+        for (int i = 0; i < pieces; i++) M = fmaxf(M, p.part_ml[slot(i) * BM + row].x);
+        f32x4 o = { 0.f, 0.f, 0.f, 0.f };
+        for (int i = 0; i < pieces; i++) {
+            const float2 ml = p.part_ml[slot(i) * BM + row];
+            if (ml.y == 0.f) continue;                                // (an empty piece has no sums)
+            const float w = fast_exp2(ml.x - M);
+            L += ml.y * w;
+            o += ((const f32x4 *) p.part_o)[slot(i) * (BM * DV / 4) + ((int) blockIdx.z * 4 + c) * NWQ * 64 + wq * 64 + lane] * w;
+        }
+        const int64_t r = j * BM + row;
+        if (r >= (int64_t) g.nq * p.group) continue;
+        const int tok = (int) (r / p.group), head = (int) blockIdx.y * p.group + (int) (r - (int64_t) tok * p.group);
+        o *= L == 0.f ? 0.f : 1.f / L;
+        *(u32x2 *) (p.dst + (int64_t) (g.q0 + tok) * p.d_nb2 + (int64_t) head * p.d_nb1 + ((int) blockIdx.z * 32 + c * 8 + (lane >> 5) * 4) * 2) = pack4<F16>(o.x, o.y, o.z, o.w);
+    }
+}
+
+// ---------------------------------------------------------------- host
+
+template <bool F16, int DK, int DV, int NWQ, int NWK, int TK, int OCC, bool BIAS>
+hipError_t launch_batch(const BatchP & p, const BatchPlan & pl, hipStream_t st) {
+    constexpr int lds = 2 * TK * (DK + DV) * 2;
+    static_assert(lds + NWQ * NWK * 32 * 8 <= 160 * 1024, "LDS");
+    static std::atomic<uint64_t> granted{ 0 };
+    hipError_t e = grant_lds(gqa_batch_kernel<F16, DK, DV, NWQ, NWK, TK, OCC, BIAS>, lds, granted);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((gqa_batch_kernel<F16, DK, DV, NWQ, NWK, TK, OCC, BIAS>), dim3((unsigned) p.n_wg), dim3(64 * NWQ * NWK), lds, st, p);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    hipLaunchKernelGGL((gqa_batch_join_kernel<F16, DV, NWQ, TK>), dim3((unsigned) pl.blocks, (unsigned) p.n_head_kv, DV / 32), dim3(256), 0, st, p);
+    return hipGetLastError();
+}
+template <bool F16, int DK, int DV, bool BIAS>
+hipError_t launch_shape(const BatchP & p, const BatchPlan & pl, hipStream_t st) {
+    if constexpr (DK <= 128) if (pl.shape == FOUR_KEYS) return launch_batch<F16, DK, DV, 1, 4, 128, batch_wg_per_cu(DK, FOUR_KEYS), BIAS>(p, pl, st);
+    if (pl.shape == FOUR_ROWS) return launch_batch<F16, DK, DV, 4, 1, 64, batch_wg_per_cu(DK, FOUR_ROWS), BIAS>(p, pl, st);
+    return launch_batch<F16, DK, DV, 2, 2, 64, batch_wg_per_cu(DK, TWO_TWO), BIAS>(p, pl, st);
+}
+template <bool F16, bool BIAS>
+hipError_t launch_widths(const BatchP & p, const BatchPlan & pl, int dk, hipStream_t st) {
+    switch (dk) {
+        case 64:  return launch_shape<F16, 64, 64, BIAS>(p, pl, st);
+        case 128: return launch_shape<F16, 128, 128, BIAS>(p, pl, st);
+        case 192: return launch_shape<F16, 192, 128, BIAS>(p, pl, st);
+        default:  return launch_shape<F16, 256, 256, BIAS>(p, pl, st);
+    }
+}
+
+}  // namespace
+
+template <bool F16> hipError_t batch_launch(const BatchP & p, const BatchPlan & pl, int dk, hipStream_t st) {
+    return p.mask || p.cap_out != 0.f ? launch_widths<F16, true>(p, pl, dk, st) : launch_widths<F16, false>(p, pl, dk, st);
+}
+
+}  // namespace gqa
+}  // namespace mla

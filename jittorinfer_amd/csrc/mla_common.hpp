@@ -15,6 +15,8 @@ typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
 typedef __attribute__((ext_vector_type(4))) short        s16x4;
 typedef __attribute__((ext_vector_type(16))) float       f32x16;
 typedef __attribute__((ext_vector_type(4))) float        f32x4;
+typedef __attribute__((ext_vector_type(2))) __bf16       bf16x2;
+typedef __attribute__((ext_vector_type(2))) _Float16     f16x2;
 typedef __attribute__((ext_vector_type(8))) __bf16       bf16x8;
 typedef __attribute__((ext_vector_type(8))) _Float16     f16x8;
 

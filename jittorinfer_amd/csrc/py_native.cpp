@@ -1,4 +1,4 @@
-// The Python entry points' way from torch tensors to the C ABI (include/mla_attn.h, mla_kv_write.h, mla_front.h, gqa_attn.h): one call that checks the
+// The Python entry points' way from torch tensors to the C ABI (include/mla_attn.h, mla_kv_write.h, mla_front.h, gqa_attn.h, gqa_batch.h): one call that checks the
 // tensors, fills the argument block and launches.  Filling a ctypes structure field by field took 6 us of a 13 us attention call and
 // most of the 70 us a layer of a decode step spent on the host, more than its kernels run for small batches; here it takes
 // under 1 us a call.  Every function takes its arguments by position; capi.py gives them names and defaults.
@@ -18,6 +18,7 @@
 #include <torch/csrc/utils/object_ptr.h>
 
 #include "../../include/gqa_attn.h"
+#include "../../include/gqa_batch.h"
 #include "../../include/mla_attn.h"
 #include "../../include/mla_front.h"
 #include "../../include/mla_kv_write.h"
@@ -60,6 +61,10 @@ struct Bound {
     decltype(&gqa_attn_launch)         gqa_attn;
     decltype(&gqa_evict_workspace_size) evict_workspace_size;
     decltype(&gqa_evict_launch)        evict;
+    decltype(&gqa_prompt_attn_workspace_size) prompt_workspace_size;
+    decltype(&gqa_prompt_attn_launch)  prompt_attn;
+    decltype(&gqa_cross_attn_workspace_size) cross_workspace_size;
+    decltype(&gqa_cross_attn_launch)   cross_attn;
     PyObject * workspace, * workspaces, * raw_stream, * capturing, * elsewhere;
 } lib;
 
@@ -702,13 +707,138 @@ PyObject * gqa_evict(PyObject *, PyObject * const * o, Py_ssize_t n) {
     return r0 && r1 && r2 ? PyTuple_Pack(3, r0.get(), r1.get(), r2.get()) : nullptr;
 }
 
-// bind(addresses of the thirteen entry points in Bound's order, workspace function, workspace table, torch's raw current stream, whether it is capturing, scratch on another stream)
+// ---- attention of many query rows over the same keys (include/gqa_batch.h)
+
+// Sequences' first tokens, or none and as many tokens each: q_starts int32 [n_seq + 1].
+template <typename Args> bool queries(Args & a, const at::Tensor & q, const at::Tensor * starts, int64_t n_seq) {
+    if (mla_type(q) <= 0 || !rows_ok(q, 3, false) || q.size(0) >= INTS || q.size(1) >= INTS || q.size(2) >= INTS || n_seq >= INTS) return false;
+    a.n_tok = (int32_t) q.size(0); a.n_seq = (int32_t) n_seq; a.n_head = (int32_t) q.size(1); a.dk = (int32_t) q.size(2);
+    a.type = mla_type(q); a.q = q.data_ptr(); a.q_nb1 = step(q, 1); a.q_nb2 = step(q, 0);
+    if (!starts) return n_seq ? q.size(0) % n_seq == 0 : q.size(0) == 0;
+    a.q_starts = (const int32_t *) starts->data_ptr();
+    return ints(*starts, n_seq + 1);
+}
+// mask f16 [n_seq, n]
+template <typename Args> bool row_mask(Args & a, const at::Tensor * mask, int64_t n_seq) {
+    if (!mask) return true;
+    if (mask->scalar_type() != at::kHalf || !rows_ok(*mask, 2, false) || mask->size(0) != n_seq) return false;
+    a.mask = mask->data_ptr(); a.mask_nb1 = step(*mask, 0); a.mask_ne0 = mask->size(1);
+    return a.mask || !n_seq;
+}
+// The result: the caller's or a new tensor, [rows of q, heads, dv].
+struct Result {
+    at::Tensor made;
+    const at::Tensor * t;
+    template <typename Args> bool take(Args & a, const at::Tensor & q, const at::Tensor * given) {
+        t = given;
+        if (!t) { made = at::empty({ q.size(0), q.size(1), (int64_t) a.dv }, q.options()); t = &made; }
+        if (t->scalar_type() != q.scalar_type() || t->dim() != 3 || t->size(0) != q.size(0) || t->size(1) != q.size(1) || t->size(2) != a.dv || !rows_ok(*t, 3, true)) return false;
+        a.dst = t->data_ptr(); a.d_nb1 = step(*t, 1); a.d_nb2 = step(*t, 0);
+        return true;
+    }
+    PyObject * give(PyObject * given) const { return made.defined() ? THPVariable_Wrap(made) : Py_NewRef(given); }
+};
+
+// gqa_prompt_attn(q, k_cache, v_cache, block_table, seq_lens, q_starts, scale, logit_softcap, window, causal, mask, out, n_workgroups, stream) -> out
+PyObject * gqa_prompt_attn(PyObject *, PyObject * const * o, Py_ssize_t n) {
+    if (!arg_count(n, 14)) return nullptr;
+    const at::Tensor * qp = tensor(o[0]), * kc = qp ? tensor(o[1]) : nullptr, * vc = kc ? tensor(o[2]) : nullptr, * table = vc ? tensor(o[3]) : nullptr, * lens = table ? tensor(o[4]) : nullptr;
+    const at::Tensor * starts, * mask, * outp;
+    if (!lens || !optional_tensor(o[5], starts) || !optional_tensor(o[10], mask) || !optional_tensor(o[11], outp)) return nullptr;
+    const at::Tensor & q = *qp;
+    if (!on_gpu(q)) return nullptr;
+    for (const at::Tensor * t : { kc, vc, table, lens, starts, mask, outp }) SAME_DEVICE(t);
+    gqa_prompt_attn_args a;
+    memset(&a, 0, sizeof a);
+    a.scale = (float) PyFloat_AsDouble(o[6]); a.logit_softcap = (float) PyFloat_AsDouble(o[7]);
+    const int64_t window = PyLong_AsLongLong(o[8]);
+    a.causal = PyObject_IsTrue(o[9]);
+    if (PyErr_Occurred() || !int_of(o[12], a.n_workgroups)) return nullptr;
+    REQUIRE(window >= 0 && window < INTS);
+    a.window = (int32_t) window;
+    REQUIRE(table_ok(*table) && ints(*lens, table->size(0)));
+    const int64_t n_seq = table->size(0);
+    REQUIRE(queries(a, q, starts, n_seq));
+    REQUIRE(cache_ok(*kc, a.type) && kc->size(2) < INTS && kc->size(3) == a.dk);
+    REQUIRE(cache_ok(*vc, a.type) && vc->size(0) == kc->size(0) && vc->size(2) == kc->size(2) && vc->size(3) < INTS);
+    a.n_head_kv = (int32_t) kc->size(2); a.n_pages = kc->size(0); a.dv = (int32_t) vc->size(3);
+    a.k = pool_of(*kc); a.v = pool_of(*vc);
+    a.block_table = (const int32_t *) table->data_ptr(); a.bt_stride = table->size(1); a.seq_lens = (const int32_t *) lens->data_ptr();
+    REQUIRE(row_mask(a, mask, n_seq));
+    const c10::DeviceGuard guard(q.device());
+    GqaStream stream;
+    if (!stream.take(o[13], q, !outp)) return nullptr;
+    Result result;
+    REQUIRE(result.take(a, q, outp));
+    Apart apart;
+    if (outp) {
+        apart.add("out", outp);
+        apart.add("q", &q); apart.add("k_cache", kc); apart.add("v_cache", vc); apart.add("block_table", table); apart.add("seq_lens", lens); apart.add("q_starts", starts); apart.add("mask", mask);
+        if (a.n_tok && !apart.check("gqa_prompt_attn", 1)) return nullptr;
+    }
+    GqaScratch scratch;
+    if (!scratch.take(o[0], q, stream, lib.prompt_workspace_size(&a), a)) return nullptr;
+    const int rc = unlocked(a.workspace, [&] { return lib.prompt_attn(&a, stream.st); });
+    return rc ? failed("gqa_prompt_attn_launch", rc) : result.give(o[11]);
+}
+
+// gqa_cross_attn(q, k, v, q_starts, kv_starts, kv_lens, scale, logit_softcap, mask, out, n_workgroups, stream) -> out
+PyObject * gqa_cross_attn(PyObject *, PyObject * const * o, Py_ssize_t n) {
+    if (!arg_count(n, 12)) return nullptr;
+    const at::Tensor * qp = tensor(o[0]), * k = qp ? tensor(o[1]) : nullptr, * v = k ? tensor(o[2]) : nullptr, * starts, * kv_starts, * kv_lens, * mask, * outp;
+    if (!v || !optional_tensor(o[3], starts) || !optional_tensor(o[4], kv_starts) || !optional_tensor(o[5], kv_lens) || !optional_tensor(o[8], mask) || !optional_tensor(o[9], outp)) return nullptr;
+    const at::Tensor & q = *qp;
+    if (!on_gpu(q)) return nullptr;
+    for (const at::Tensor * t : { k, v, starts, kv_starts, kv_lens, mask, outp }) SAME_DEVICE(t);
+    gqa_cross_attn_args a;
+    memset(&a, 0, sizeof a);
+    a.scale = (float) PyFloat_AsDouble(o[6]); a.logit_softcap = (float) PyFloat_AsDouble(o[7]);
+    if (PyErr_Occurred() || !int_of(o[10], a.n_workgroups)) return nullptr;
+    // [n_seq, n, heads, width] padded, or [n, heads, width] with the sequences' first rows
+    const bool packed = kv_starts != nullptr;
+    const int64_t d = packed ? 3 : 4;
+    for (const at::Tensor * t : { k, v }) REQUIRE(mla_type(*t) == mla_type(q) && rows_ok(*t, d, false) && t->size(d - 3) < INTS && t->size(d - 2) < INTS && t->size(d - 1) < INTS);
+    const int64_t n_seq = !packed ? k->size(0) : kv_lens ? kv_lens->numel() : kv_starts->numel() - 1;
+    REQUIRE(n_seq >= 0 && queries(a, q, starts, n_seq));
+    REQUIRE(k->size(d - 1) == a.dk && v->size(d - 2) == k->size(d - 2) && v->size(d - 3) == k->size(d - 3) && (packed || v->size(0) == n_seq));
+    if (packed) {
+        REQUIRE(ints(*kv_starts, kv_starts->numel()) && kv_starts->numel() >= n_seq);
+        a.kv_starts = (const int32_t *) kv_starts->data_ptr();
+    }
+    if (kv_lens) {
+        REQUIRE(ints(*kv_lens, n_seq));
+        a.kv_lens = (const int32_t *) kv_lens->data_ptr();
+    }
+    a.n_head_kv = (int32_t) k->size(d - 2); a.dv = (int32_t) v->size(d - 1); a.n_kv = k->size(d - 3);
+    a.k = gqa_pool{ k->data_ptr(), packed ? 0 : step(*k, 0), step(*k, d - 3), step(*k, d - 2) };
+    a.v = gqa_pool{ v->data_ptr(), packed ? 0 : step(*v, 0), step(*v, d - 3), step(*v, d - 2) };
+    REQUIRE(row_mask(a, mask, n_seq));
+    const c10::DeviceGuard guard(q.device());
+    GqaStream stream;
+    if (!stream.take(o[11], q, !outp)) return nullptr;
+    Result result;
+    REQUIRE(result.take(a, q, outp));
+    Apart apart;
+    if (outp) {
+        apart.add("out", outp);
+        apart.add("q", &q); apart.add("k", k); apart.add("v", v); apart.add("q_starts", starts); apart.add("kv_starts", kv_starts); apart.add("kv_lens", kv_lens); apart.add("mask", mask);
+        if (a.n_tok && !apart.check("gqa_cross_attn", 1)) return nullptr;
+    }
+    GqaScratch scratch;
+    if (!scratch.take(o[0], q, stream, lib.cross_workspace_size(&a), a)) return nullptr;
+    const int rc = unlocked(a.workspace, [&] { return lib.cross_attn(&a, stream.st); });
+    return rc ? failed("gqa_cross_attn_launch", rc) : result.give(o[9]);
+}
+
+// bind(addresses of the entry points in Bound's order, workspace function, workspace table, torch's raw current stream, whether it is capturing, scratch on another stream)
 PyObject * bind(PyObject *, PyObject * const * v, Py_ssize_t n) {
-    if (!arg_count(n, 18)) return nullptr;
-    void * p[13];
-    for (int i = 0; i < 13; i++) p[i] = PyLong_AsVoidPtr(v[i]);
+    constexpr int N = 17;
+    if (!arg_count(n, N + 5)) return nullptr;
+    void * p[N];
+    for (int i = 0; i < N; i++) p[i] = PyLong_AsVoidPtr(v[i]);
     if (PyErr_Occurred()) return nullptr;
-    REQUIRE(PyCallable_Check(v[13]) && PyDict_Check(v[14]) && PyCallable_Check(v[15]) && PyCallable_Check(v[16]) && PyCallable_Check(v[17]));
+    v += N;
+    REQUIRE(PyCallable_Check(v[0]) && PyDict_Check(v[1]) && PyCallable_Check(v[2]) && PyCallable_Check(v[3]) && PyCallable_Check(v[4]));
     lib.workspace_size = (decltype(lib.workspace_size)) p[0]; lib.attn = (decltype(lib.attn)) p[1];
     lib.kv_write = (decltype(lib.kv_write)) p[2]; lib.kv_write_rope = (decltype(lib.kv_write_rope)) p[3];
     lib.rope = (decltype(lib.rope)) p[4]; lib.mul_mat = (decltype(lib.mul_mat)) p[5];
@@ -716,7 +846,9 @@ PyObject * bind(PyObject *, PyObject * const * v, Py_ssize_t n) {
     lib.norm_rope = (decltype(lib.norm_rope)) p[8]; lib.gqa_workspace_size = (decltype(lib.gqa_workspace_size)) p[9];
     lib.gqa_attn = (decltype(lib.gqa_attn)) p[10]; lib.evict_workspace_size = (decltype(lib.evict_workspace_size)) p[11];
     lib.evict = (decltype(lib.evict)) p[12];
-    lib.workspace = Py_NewRef(v[13]); lib.workspaces = Py_NewRef(v[14]); lib.raw_stream = Py_NewRef(v[15]); lib.capturing = Py_NewRef(v[16]); lib.elsewhere = Py_NewRef(v[17]);
+    lib.prompt_workspace_size = (decltype(lib.prompt_workspace_size)) p[13]; lib.prompt_attn = (decltype(lib.prompt_attn)) p[14];
+    lib.cross_workspace_size = (decltype(lib.cross_workspace_size)) p[15]; lib.cross_attn = (decltype(lib.cross_attn)) p[16];
+    lib.workspace = Py_NewRef(v[0]); lib.workspaces = Py_NewRef(v[1]); lib.raw_stream = Py_NewRef(v[2]); lib.capturing = Py_NewRef(v[3]); lib.elsewhere = Py_NewRef(v[4]);
     Py_RETURN_NONE;
 }
 
@@ -730,7 +862,8 @@ template <PyObject * (*F)(PyObject *, PyObject * const *, Py_ssize_t)> PyObject 
 }
 
 #define FAST(name) { #name, (PyCFunction) (void (*)(void)) entry<name>, METH_FASTCALL, nullptr }
-PyMethodDef methods[] = { FAST(bind), FAST(attn), FAST(rope), FAST(mul_mat), FAST(copy), FAST(kv_write), FAST(front_batch), FAST(gqa_norm_rope), FAST(gqa_attn), FAST(gqa_evict), { nullptr, nullptr, 0, nullptr } };
+PyMethodDef methods[] = { FAST(bind), FAST(attn), FAST(rope), FAST(mul_mat), FAST(copy), FAST(kv_write), FAST(front_batch), FAST(gqa_norm_rope), FAST(gqa_attn), FAST(gqa_evict),
+                          FAST(gqa_prompt_attn), FAST(gqa_cross_attn), { nullptr, nullptr, 0, nullptr } };
 PyModuleDef module = { PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr };
 
 }  // namespace

@@ -1,0 +1,342 @@
+"""Attention of many query rows over the same keys on the GPU against plain forms in 64 bits (tests/gqa_batch_util.py)."""
+import math
+
+import pytest
+import torch
+
+from tests import gqa_batch_util as B
+from tests import gqa_util as R
+from tests.test_gqa_gpu import _near
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+WIDTHS = [(64, 64), (128, 128), (192, 128), (256, 256)]
+NAN = float("nan")
+
+
+def _starts(n):
+    return torch.tensor([0] + n, dtype=torch.int32).cumsum(0).to(torch.int32)
+
+
+def _case(seed, new, lens, width, heads, kv_heads, dk, dv, dtype, layout="cells", spare=2):
+    """New tokens and rows of every sequence; pages hold what the lengths need and NaN everywhere else."""
+    gen = torch.Generator().manual_seed(seed)
+    pages = sum((min(max(n, 0), width * 128) + 127) // 128 for n in lens) + spare
+    bt = R.make_table(gen, [min(n, width * 128) for n in lens], width, pages)
+    k, v = (R.make_cache(gen, pages, kv_heads, d, dtype, layout, fill=NAN) for d in (dk, dv))
+    for b, n in enumerate(lens):
+        at = torch.arange(min(max(n, 0), width * 128))
+        page = bt[b].long()[at // 128]
+        k[page, at % 128] = torch.randn((len(at), kv_heads, dk), generator=gen).to(dtype)
+        v[page, at % 128] = torch.randn((len(at), kv_heads, dv), generator=gen).to(dtype)
+    q = torch.randn((sum(new), heads, dk), generator=gen).to(dtype)
+    return q, k, v, bt, torch.tensor(lens, dtype=torch.int32), _starts(new)
+
+
+def _check(gpu, q, k, v, bt, lens, starts, what="", given=True, **kw):
+    import jittorinfer_amd as J
+    scale = kw.pop("scale", 1 / math.sqrt(q.shape[2]))
+    want, off = B.prompt(q, k, v, bt, lens, starts, scale, kw.get("logit_softcap", 0.0), kw.get("window", 0), kw.get("causal", True), kw.get("mask"))
+    d = {n: (t.to(gpu) if isinstance(t, torch.Tensor) else t) for n, t in kw.items()}
+    out = torch.full(want.shape, NAN, dtype=q.dtype, device=gpu)
+    got = J.gqa_prompt_attn(q.to(gpu), k.to(gpu), v.to(gpu), bt.to(gpu), lens.to(gpu), starts.to(gpu) if given else None, scale=scale, out=out, **d)
+    torch.cuda.synchronize()
+    mine = ~torch.isnan(want[:, 0, 0])
+    assert torch.isnan(got.cpu()[~mine]).all()
+    _near(got[mine.to(gpu)], want[mine], off[mine], q.dtype, what)
+    return got
+
+
+NEW = [1, 0, 40, 129, 3, 64, 200]
+LENS = [1, 70, 300, 129, 513, 64, 333]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dk,dv", WIDTHS)
+@pytest.mark.parametrize("layout", ["cells", "heads"])
+def test_prompt_widths_types_layouts(gpu, dk, dv, dtype, layout):
+    _check(gpu, *_case(dk, NEW, LENS, 5, 8, 2, dk, dv, dtype, layout), "%s %s" % ((dk, dv), dtype))
+
+
+@pytest.mark.parametrize("dk,dv", WIDTHS)
+@pytest.mark.parametrize("new", [[1, 1, 1], [2, 9, 1], [16, 12, 14], [30, 40, 25]])
+def test_prompt_few_tokens(gpu, dk, dv, new):
+    """Blocks of 32, 64 and 128 rows: waves that share the keys of a tile."""
+    _check(gpu, *_case(dk, new, [400, 130, 257], 4, 4, 2, dk, dv, BF16))
+    _check(gpu, *_case(dk, new, [40, 130, 64], 4, 2, 2, dk, dv, F16), n_workgroups=7)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (7, 7), (3, 1), (28, 4), (40, 1), (66, 1), (160, 1)])
+def test_prompt_groups(gpu, heads, kv_heads):
+    """Groups that no block holds a whole number of, and a token's heads in two blocks."""
+    _check(gpu, *_case(heads, [5, 33, 0, 70], [5, 200, 3, 129], 2, heads, kv_heads, 64, 64, BF16))
+
+
+@pytest.mark.parametrize("n_workgroups", [1, 2, 3, 5, 8, 13, 64, 1000])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (192, 128)])
+def test_prompt_any_number_of_workgroups(gpu, dk, dv, n_workgroups):
+    """Runs that hold several blocks, end inside one, or are empty."""
+    _check(gpu, *_case(3, [100, 1, 0, 60, 128, 7], [700, 1, 0, 200, 128, 513], 6, 4, 2, dk, dv, F16), n_workgroups=n_workgroups)
+    _check(gpu, *_case(4, [2, 1, 0, 3], [700, 1, 0, 200], 6, 4, 2, dk, dv, F16), n_workgroups=n_workgroups)
+
+
+def test_prompt_more_sequences_than_lanes(gpu):
+    gen = torch.Generator().manual_seed(5)
+    new = [int(x) for x in torch.randint(0, 4, (300,), generator=gen)]
+    lens = [n + int(x) for n, x in zip(new, torch.randint(0, 90, (300,), generator=gen))]
+    new[:100] = lens[:100] = [0] * 100
+    _check(gpu, *_case(5, new, lens, 1, 2, 1, 64, 64, BF16))
+
+
+@pytest.mark.parametrize("window", [1, 5, 64, 100, 129, 1000])
+def test_prompt_window(gpu, window):
+    case = _case(6, [70, 1, 200, 33], [300, 128, 200, 411], 4, 4, 2, 128, 128, BF16)
+    _check(gpu, *case, window=window)
+    _check(gpu, *case, window=window, causal=False)
+    _check(gpu, *case, window=window, n_workgroups=3)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("cap", [5.0, 50.0, 1e30])
+def test_prompt_softcap(gpu, cap, dtype):
+    _check(gpu, *_case(7, [1, 130, 20], [1, 200, 300], 3, 4, 1, 128, 128, dtype), logit_softcap=cap)
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 2.0])
+@pytest.mark.parametrize("cap", [0.0, 9.0])
+def test_prompt_scales(gpu, scale, cap):
+    """A negative scale, none, and one that leaves a row to its largest score."""
+    _check(gpu, *_case(8, [1, 130, 20], [1, 200, 300], 3, 4, 2, 64, 64, BF16), scale=scale, logit_softcap=cap)
+
+
+def test_prompt_not_causal_and_equal_tokens(gpu):
+    case = _case(9, [40, 40, 40], [40, 200, 300], 3, 4, 2, 64, 64, F16)
+    _check(gpu, *case, causal=False)
+    _check(gpu, *case, given=False)
+    _check(gpu, *_case(9, [1, 1, 1], [40, 200, 300], 3, 4, 2, 64, 64, F16), given=False)
+
+
+def test_prompt_lengths_outside_the_table_and_short_of_the_tokens(gpu):
+    """A negative length is none, one past the table's room is that room, one below the number of new tokens leaves the first of them nothing."""
+    case = _case(10, [4, 70, 20, 30], [0, 256, 200, 10], 2, 4, 2, 128, 128, BF16)
+    case[4][0], case[4][1] = -7, 100000
+    got = _check(gpu, *case)
+    assert (got[:4] == 0).all() and (got[94:94 + 20] == 0).all() and (got[94 + 20:] != 0).any()
+
+
+def _mask(gen, n_seq, n, dtype=F16):
+    m = torch.zeros((n_seq, n), dtype=dtype)
+    m[torch.rand((n_seq, n), generator=gen) < 0.3] = float("-inf")
+    return m
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dk,dv", WIDTHS)
+def test_prompt_mask(gpu, dk, dv, dtype):
+    """Rows struck out, a sequence without any left, values that are not 0 (the lowest among them), keys and values of struck-out rows that are NaN or infinite."""
+    q, k, v, bt, lens, starts = _case(11, [60, 129, 5, 40, 3], [300, 129, 64, 40, 200], 3, 6, 2, dk, dv, dtype)
+    gen = torch.Generator().manual_seed(9)
+    mask = _mask(gen, 5, 384)
+    mask[2] = float("-inf")
+    mask[3] = torch.randn(384, generator=gen).to(F16)
+    mask[3, 5:9] = torch.finfo(F16).min
+    for b, n in enumerate(lens.tolist()):
+        for i in torch.nonzero(mask[b, :n] == float("-inf"))[:, 0].tolist():
+            k[bt[b, i // 128], i % 128] = float("nan") if i % 2 else float("inf")
+            v[bt[b, i // 128], i % 128] = float("inf") if i % 3 else float("nan")
+    got = _check(gpu, q, k, v, bt, lens, starts, mask=mask)
+    assert (got[189:194] == 0).all()
+    for cut in (1, 64, 130, 299):
+        _check(gpu, q, k, v, bt, lens, starts, mask=mask[:, :cut])
+    wide = torch.full((5, 385), NAN, dtype=F16)[:, 1:]
+    wide[:, :] = mask
+    _check(gpu, q, k, v, bt, lens, starts, mask=wide, window=90, logit_softcap=20.0)
+    if dk <= 128:
+        _check(gpu, q[:64], k, v, bt, lens, _starts([10, 20, 5, 5, 3]), mask=mask)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dk,dv,new", [(64, 64, 300), (128, 128, 300), (192, 128, 300), (256, 256, 300), (64, 64, 7), (128, 128, 14), (256, 256, 14)])
+def test_prompt_infinities_of_rows_not_seen(gpu, dk, dv, new, dtype):
+    """A key and a value that are NaN or infinite reach the tokens that see them, and no others."""
+    q, k, v, bt, lens, starts = _case(12, [new, new], [300, 310], 3, 4, 2, dk, dv, dtype)
+    clean, _ = B.prompt(q, k, v, bt, lens, starts, 0.1, window=150)
+    at = 297
+    page = bt[0, at // 128].long()
+    kinds = [float("inf"), float("-inf"), NAN]
+    for c in range(dv):
+        if c % 5 < 3:
+            v[page, at % 128, 0, c] = kinds[c % 5]
+    import jittorinfer_amd as J
+    for n in (0, 5):
+        got = J.gqa_prompt_attn(q.to(gpu), k.to(gpu), v.to(gpu), bt.to(gpu), lens.to(gpu), starts.to(gpu), scale=0.1, window=150, n_workgroups=n).cpu().double()
+        first = at - (300 - new)                             # the token whose row it is
+        unseen = got[:first]
+        assert torch.isfinite(unseen).all() and torch.isfinite(got[new:]).all() and torch.isfinite(got[:new, 2:]).all()
+        assert (got[:, :, 3::5] - clean[:, :, 3::5]).abs().max() < 0.05
+        for c in range(dv):
+            seen = got[first:new, :2, c]
+            if c % 5 == 0:
+                assert (seen == float("inf")).all()
+            elif c % 5 == 1:
+                assert (seen == float("-inf")).all()
+            elif c % 5 == 2:
+                assert torch.isnan(seen).all()
+    k[page, at % 128, 0] = NAN
+    got = J.gqa_prompt_attn(q.to(gpu), k.to(gpu), v.to(gpu), bt.to(gpu), lens.to(gpu), starts.to(gpu), scale=0.1, window=150).cpu()
+    assert torch.isfinite(got[:first]).all() and torch.isnan(got[first:new, :2]).all() and torch.isfinite(got[new:]).all()
+
+
+def test_prompt_bad_pages_and_tokens_of_no_sequence(gpu):
+    """Rows of a page id outside the pool count as masked; tokens before the first sequence's and behind the last one's keep what out held."""
+    q, k, v, bt, lens, starts = _case(13, [60, 70, 30], [300, 256, 129], 3, 4, 2, 64, 64, BF16)
+    bt[0, 1], bt[1, 0], bt[2] = -1, 10 ** 9, k.shape[0]
+    _check(gpu, q, k, v, bt, lens, starts)
+    q = torch.cat((q, q, q))
+    got = _check(gpu, q, k, v, bt, lens, starts + 17)
+    assert torch.isnan(got[:17]).all() and torch.isnan(got[17 + 160:]).all() and torch.isfinite(got[17:177]).all()
+
+
+def test_prompt_strides(gpu):
+    """q a view of a projection's output, out a view with other strides, caches that share their rows' memory side by side, an empty batch."""
+    import jittorinfer_amd as J
+    q, k, v, bt, lens, starts = _case(14, [60, 70], [300, 256], 3, 4, 2, 64, 64, BF16)
+    want, off = B.prompt(q, k, v, bt, lens, starts, 0.125)
+    wide = torch.full((130, 4, 200), NAN, dtype=BF16)
+    wide[..., 8:72] = q
+    both = torch.full((k.shape[0], 128, 2, 136), NAN, dtype=BF16)
+    both[..., :64], both[..., 72:] = k, v
+    both = both.to(gpu)
+    out = torch.full((4, 130, 100), NAN, dtype=BF16, device=gpu)
+    view = out.transpose(0, 1)[..., 4:68]
+    got = J.gqa_prompt_attn(wide.to(gpu)[..., 8:72], both[..., :64], both[..., 72:], bt.to(gpu), lens.to(gpu), starts.to(gpu), scale=0.125, out=view)
+    assert got.data_ptr() == view.data_ptr()
+    _near(view, want, off, BF16)
+    assert torch.isnan(out[..., :4]).all() and torch.isnan(out[..., 68:]).all()
+    none = J.gqa_prompt_attn(q[:0].to(gpu), k.to(gpu), v.to(gpu), bt.to(gpu), lens.to(gpu), (starts * 0).to(gpu), scale=0.125)
+    assert none.shape == (0, 4, 64)
+    none = J.gqa_prompt_attn(q[:0].to(gpu), k.to(gpu), v.to(gpu), bt[:0].to(gpu), lens[:0].to(gpu), scale=0.125)
+    assert none.shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("dtype,dk,dv", [(BF16, 128, 128), (F16, 64, 64)])
+def test_prompt_long(gpu, dtype, dk, dv):
+    """A chunk behind a long context, and many tokens: against the same formula in f32 on the GPU, whose own error is below what is allowed."""
+    import jittorinfer_amd as J
+    q, k, v, bt, lens, starts = _case(15, [37, 1500], [20001, 1500], 160, 4, 2, dk, dv, dtype)
+    want, off = B.prompt(q, k, v, bt, lens, starts, 0.1)
+    got = J.gqa_prompt_attn(q.to(gpu), k.to(gpu), v.to(gpu), bt.to(gpu), lens.to(gpu), starts.to(gpu), scale=0.1)
+    _near(got, want, off, dtype)
+    again = J.gqa_prompt_attn(q.to(gpu), k.to(gpu), v.to(gpu), bt.to(gpu), lens.to(gpu), starts.to(gpu), scale=0.1)
+    assert torch.equal(got, again)
+
+
+def test_prompt_of_one_token_is_gqa_attn(gpu):
+    """One new token a sequence: what gqa_attn answers, but for the rounding of the weights."""
+    import jittorinfer_amd as J
+    q, k, v, bt, lens, starts = (t.to(gpu) for t in _case(16, [1] * 5, [1, 70, 300, 129, 511], 4, 8, 2, 128, 128, F16))
+    a = J.gqa_attn(q, k, v, bt, lens, scale=0.1).double()
+    b = J.gqa_prompt_attn(q, k, v, bt, lens, scale=0.1).double()
+    assert (a - b).abs().max() < 2.0 ** -10 * v[torch.isfinite(v)].abs().max().double()
+
+
+# ---------------------------------------------------------------- an encoder's states
+
+def _states(seed, new, n, heads, kv_heads, dk, dv, dtype, most=None):
+    gen = torch.Generator().manual_seed(seed)
+    most = most or max(n + [1])
+    k, v = (torch.full((len(n), most, kv_heads, d), NAN, dtype=dtype) for d in (dk, dv))
+    for b, x in enumerate(n):
+        k[b, :x] = torch.randn((x, kv_heads, dk), generator=gen).to(dtype)
+        v[b, :x] = torch.randn((x, kv_heads, dv), generator=gen).to(dtype)
+    return torch.randn((sum(new), heads, dk), generator=gen).to(dtype), k, v, _starts(new), torch.tensor(n, dtype=torch.int32)
+
+
+def _cross(gpu, q, k, v, starts, lens, given=True, packed=False, **kw):
+    import jittorinfer_amd as J
+    scale = 1 / math.sqrt(q.shape[2])
+    want, off = B.cross(q, k, v, starts, lens, scale, kw.get("logit_softcap", 0.0), kw.get("mask"))
+    if packed:
+        at = {"kv_starts": _starts(lens.tolist())}
+        k, v = (torch.cat([x[b, :n] for b, n in enumerate(lens.tolist())]) for x in (k, v))
+    else:
+        at = {"kv_lens": lens}
+    d = {n: (t.to(gpu) if isinstance(t, torch.Tensor) else t) for n, t in {**kw, **at}.items()}
+    got = J.gqa_cross_attn(q.to(gpu), k.to(gpu), v.to(gpu), q_starts=starts.to(gpu) if given else None, scale=scale, **d)
+    torch.cuda.synchronize()
+    _near(got, want, off, q.dtype)
+    return got
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dk,dv", WIDTHS)
+@pytest.mark.parametrize("packed", [False, True])
+def test_cross_widths_types(gpu, dk, dv, dtype, packed):
+    _cross(gpu, *_states(dk, [40, 1, 129, 0, 7], [300, 1, 77, 5, 0], 4, 2, dk, dv, dtype), packed=packed)
+    _cross(gpu, *_states(dk, [3, 1, 2, 1, 7], [300, 1, 77, 5, 0], 4, 4, dk, dv, dtype), packed=packed)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dk,dv", WIDTHS)
+@pytest.mark.parametrize("heads,kv_heads", [(8, 8), (8, 2), (40, 1), (24, 8)])
+@pytest.mark.parametrize("packed", [False, True])
+def test_cross_of_one_token(gpu, dk, dv, dtype, heads, kv_heads, packed):
+    """A decode step: one token a sequence, over states of odd numbers, none among them."""
+    case = _states(dk + heads, [1] * 7, [300, 1, 129, 0, 640, 31, 128], heads, kv_heads, dk, dv, dtype)
+    got = _cross(gpu, *case, given=False, packed=packed)
+    assert (got[3] == 0).all()
+    _cross(gpu, *case, given=True, packed=packed, n_workgroups=5)
+
+
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("new", [1, 30])
+def test_cross_mask_and_cap(gpu, new, given):
+    """Padding masked, a sequence without any state left, NaN and infinities behind the mask and behind the lengths."""
+    q, k, v, starts, lens = _states(20, [new] * 4, [300, 77, 129, 5], 4, 2, 64, 64, BF16, most=310)
+    gen = torch.Generator().manual_seed(3)
+    mask = _mask(gen, 4, 310)
+    mask[1] = float("-inf")
+    for b in range(4):
+        k[b, mask[b] == float("-inf")] = NAN
+        v[b, mask[b] == float("-inf")] = float("inf")
+    got = _cross(gpu, q, k, v, starts, lens, given=given, mask=mask)
+    assert (got[new:2 * new] == 0).all()
+    _cross(gpu, q, k, v, starts, lens, given=given, mask=mask[:, :50], logit_softcap=10.0)
+
+
+def test_cross_lengths_and_starts_out_of_range(gpu):
+    """No lengths: all states; lengths below 0 and past the states; starts outside the buffer, sequences whose states overlap."""
+    import jittorinfer_amd as J
+    q, k, v, starts, lens = _states(21, [9, 4, 2], [200, 200, 200], 4, 2, 64, 64, F16)
+    d = [t.to(gpu) for t in (q, k, v)]
+    want, off = B.cross(q, k, v, starts, lens, 0.125)
+    _near(J.gqa_cross_attn(*d, q_starts=starts.to(gpu), scale=0.125), want, off, F16)
+    odd = torch.tensor([-3, 1000, 5], dtype=torch.int32)
+    want, off = B.cross(q, k, v, starts, odd, 0.125)
+    _near(J.gqa_cross_attn(*d, q_starts=starts.to(gpu), kv_lens=odd.to(gpu), scale=0.125), want, off, F16)
+    flat = [t.reshape(600, 2, 64) for t in (k, v)]
+    at, n = torch.tensor([-1, 550, 100], dtype=torch.int32), torch.tensor([50, 500, 300], dtype=torch.int32)
+    want, off = B.cross(q, *flat, starts, n, 0.125, kv_starts=at)
+    got = J.gqa_cross_attn(d[0], *[t.to(gpu) for t in flat], q_starts=starts.to(gpu), kv_starts=at.to(gpu), kv_lens=n.to(gpu), scale=0.125)
+    _near(got, want, off, F16)
+    assert (got[:9] == 0).all()
+    at[1] = 601
+    got = J.gqa_cross_attn(d[0], *[t.to(gpu) for t in flat], q_starts=starts.to(gpu), kv_starts=at.to(gpu), kv_lens=n.to(gpu), scale=0.125)
+    assert (got[:13] == 0).all() and (got[13:] != 0).any()
+
+
+@pytest.mark.parametrize("new", [1, 20])
+def test_cross_strides(gpu, new):
+    """States with heads outermost, expanded over the heads or over the sequences, out given."""
+    import jittorinfer_amd as J
+    q, k, v, starts, lens = _states(22, [new] * 3, [150, 150, 150], 4, 2, 64, 64, BF16)
+    want, off = B.cross(q, k, v, starts, lens, 0.125)
+    k2, v2 = (t.transpose(1, 2).contiguous().transpose(1, 2).to(gpu) for t in (k, v))
+    out = torch.full((3 * new, 4, 64), NAN, dtype=BF16, device=gpu)
+    got = J.gqa_cross_attn(q.to(gpu), k2, v2, scale=0.125, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    _near(got, want, off, BF16)
+    one = [t[:1, :, :1].expand(3, 150, 2, 64) for t in (k, v)]
+    want, off = B.cross(q, *one, starts, lens, 0.125)
+    _near(J.gqa_cross_attn(q.to(gpu), *[t[:1, :, :1].to(gpu).expand(3, 150, 2, 64) for t in (k, v)], scale=0.125), want, off, BF16)
