@@ -95,6 +95,38 @@ int    gqa_cross_attn_check(const gqa_cross_attn_args * args);
 size_t gqa_cross_attn_workspace_size(const gqa_cross_attn_args * args);
 int    gqa_cross_attn_launch(const gqa_cross_attn_args * args, void * stream);
 
+/* ---- one new token of every sequence, where sequences share their first rows
+ * What gqa_attn (include/gqa_attn.h) answers, with the shared rows read once a group.  Group g is the sequences prefix_starts[g] .. prefix_starts[g + 1] - 1 of the batch, side
+ * by side; their first prefix_lens[g] rows hold the same keys and values, and are read through the block table of the first of them (rows of a page that is not
+ * shared whole, too).  A sequence shorter than its group's prefix sees what it has of it; sequences outside [prefix_starts[0],
+ * prefix_starts[n_prefix]) share nothing.  Numbers in prefix_starts are taken to lie in [0, n_seq] and never fall; lengths of prefixes count as seq_lens do. */
+typedef struct gqa_prefix_attn_args {
+    int32_t n_seq, n_prefix, n_head, n_head_kv;
+    int32_t dk, dv;
+    int32_t type;
+    int32_t n_workgroups;
+    float   scale, logit_softcap;
+    const void * q;          /* [n_seq][n_head][dk] */
+    int64_t q_nb1, q_nb2;
+    gqa_pool k, v;           /* rows 16-byte aligned, at most 8 MB apart, pages less than 4 GB */
+    int64_t n_pages;
+    const int32_t * block_table;   /* [n_seq][bt_stride] */
+    int64_t         bt_stride;
+    const int32_t * seq_lens;      /* [n_seq] rows, the shared ones among them */
+    const int32_t * prefix_starts; /* [n_prefix + 1] */
+    const int32_t * prefix_lens;   /* [n_prefix] */
+    const void * mask;       /* f16 [n_seq][mask_ne0] or NULL */
+    int64_t mask_nb1, mask_ne0;
+    void *  dst;             /* [n_seq][n_head][dv] */
+    int64_t d_nb1, d_nb2;
+    void *  workspace;
+    size_t  workspace_size;
+} gqa_prefix_attn_args;
+
+int    gqa_prefix_attn_check(const gqa_prefix_attn_args * args);
+size_t gqa_prefix_attn_workspace_size(const gqa_prefix_attn_args * args);
+int    gqa_prefix_attn_launch(const gqa_prefix_attn_args * args, void * stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -19,6 +19,8 @@
  *                                   (:182-240) leaves the other's cells in place and the next find_slot takes other cells; with
  *                                   pages the same sequence of calls -- copy, roll the copy or the source back into the
  *                                   shared prefix, append -- needs the partly used shared page copied first
+ *   mla_page_table_shared_prefixes  no counterpart: its attention reads a shared cell for every query of the batch; here the groups of sequences whose
+ *                                   shared pages gqa_prefix_attn_launch (include/gqa_batch.h) reads once
  *   mla_page_table_seq_keep         llama_kv_cache_seq_keep, :285-313
  *   mla_page_table_seq_evict        no counterpart (the reference's cache drops ranges of positions only): the pages a sequence gives back
  *                                   when gqa_evict_launch (include/gqa_attn.h) cuts it to some rows of its own choice, moved up in place
@@ -104,6 +106,11 @@ int32_t mla_page_table_used_cells(const mla_page_table * t);
 
 /* Fills block_table[n_seqs][max_blocks] (unused entries 0) and seq_lens[n_seqs] for the given sequences, in order. */
 int mla_page_table_fill_inputs(const mla_page_table * t, int32_t n_seqs, const int32_t * seq_ids, int32_t * block_table, int32_t * seq_lens);
+
+/* Which of the given sequences, in this order, share their leading pages: cuts the batch into groups of sequences side by side, so that reading a group's common pages
+ * once spares the most page reads.  Group g is the sequences starts[g] .. starts[g + 1] - 1, with lens[g] shared rows (whole pages, no more
+ * than its longest sequence has; 0 for a group of one).  starts has room for n_seqs + 1 numbers, lens for n_seqs.  Returns the number of groups (0 for an empty batch). */
+int32_t mla_page_table_shared_prefixes(const mla_page_table * t, int32_t n_seqs, const int32_t * seq_ids, int32_t * starts, int32_t * lens);
 
 #ifdef __cplusplus
 }

@@ -36,8 +36,8 @@ def build(verbose=False):
         return obj
 
     with ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:
-        objs = list(pool.map(compile, ("mla_kernels.hip", "mla_decode_kernel.hip", "mla_kv_write.hip", "mla_front.hip", "gqa_front.hip", "gqa_attn.hip",
-                                       "gqa_evict.hip", "gqa_batch.hip", "gqa_batch_bf16.hip", "gqa_batch_f16.hip", "ggml_mla_backend.cpp", "mla_page_table.cpp")))
+        objs = list(pool.map(compile, ("gqa_attn.hip", "gqa_batch_bf16.hip", "gqa_batch_f16.hip", "mla_kernels.hip", "mla_decode_kernel.hip", "mla_kv_write.hip", "mla_front.hip",
+                                       "gqa_front.hip", "gqa_evict.hip", "gqa_batch.hip", "gqa_prefix.hip", "ggml_mla_backend.cpp", "mla_page_table.cpp")))
     _run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs + ["-ldl"])
     return LIB
 

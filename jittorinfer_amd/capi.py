@@ -73,11 +73,12 @@ def library():
         lib.mla_front_batch_launch.restype = C.c_int
         lib.mla_front_batch_launch.argtypes = [C.POINTER(MlaFrontOp), C.c_int32, C.c_void_p]
         for name, cls in (("gqa_norm_rope", GqaNormRopeArgs), ("gqa_attn", GqaAttnArgs), ("gqa_evict", GqaEvictArgs), ("gqa_prompt_attn", GqaPromptAttnArgs),
-                          ("gqa_cross_attn", GqaCrossAttnArgs)):
+                          ("gqa_cross_attn", GqaCrossAttnArgs), ("gqa_prefix_attn", GqaPrefixAttnArgs)):
             getattr(lib, name + "_check").restype = getattr(lib, name + "_launch").restype = C.c_int
             getattr(lib, name + "_check").argtypes = [C.POINTER(cls)]
             getattr(lib, name + "_launch").argtypes = [C.POINTER(cls), C.c_void_p]
-        for name, cls in (("gqa_attn", GqaAttnArgs), ("gqa_evict", GqaEvictArgs), ("gqa_prompt_attn", GqaPromptAttnArgs), ("gqa_cross_attn", GqaCrossAttnArgs)):
+        for name, cls in (("gqa_attn", GqaAttnArgs), ("gqa_evict", GqaEvictArgs), ("gqa_prompt_attn", GqaPromptAttnArgs), ("gqa_cross_attn", GqaCrossAttnArgs),
+                          ("gqa_prefix_attn", GqaPrefixAttnArgs)):
             getattr(lib, name + "_workspace_size").restype = C.c_size_t
             getattr(lib, name + "_workspace_size").argtypes = [C.POINTER(cls)]
         lib.mla_page_table_create.restype = C.c_void_p
@@ -98,6 +99,8 @@ def library():
         lib.mla_page_table_free_pages.argtypes = [C.c_void_p]
         lib.mla_page_table_used_cells.argtypes = [C.c_void_p]
         lib.mla_page_table_fill_inputs.argtypes = [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]
+        lib.mla_page_table_shared_prefixes.restype = C.c_int32
+        lib.mla_page_table_shared_prefixes.argtypes = [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]
         lib.mla_attn_target_arch.restype = C.c_char_p
         lib.ggml_backend_init.restype = C.c_void_p
         lib.ggml_backend_score.restype = C.c_int
@@ -124,7 +127,7 @@ def native():
         names = ("mla_attn_workspace_size", "mla_attn_launch", "mla_kv_write_launch", "mla_kv_write_rope_launch", "mla_rope_launch",
                  "mla_mul_mat_launch", "mla_copy_f32_launch", "mla_front_batch_launch", "gqa_norm_rope_launch", "gqa_attn_workspace_size",
                  "gqa_attn_launch", "gqa_evict_workspace_size", "gqa_evict_launch", "gqa_prompt_attn_workspace_size", "gqa_prompt_attn_launch",
-                 "gqa_cross_attn_workspace_size", "gqa_cross_attn_launch")
+                 "gqa_cross_attn_workspace_size", "gqa_cross_attn_launch", "gqa_prefix_attn_workspace_size", "gqa_prefix_attn_launch")
         mod.bind(*[C.cast(getattr(lib, n), C.c_void_p).value for n in names], _workspace, _workspaces, torch._C._cuda_getCurrentRawStream,
                  torch._C._cuda_isCurrentStreamCapturing, _scratch_elsewhere)
         _native = mod
@@ -425,6 +428,16 @@ class GqaCrossAttnArgs(C.Structure):
                 ("dst", C.c_void_p), ("d_nb1", C.c_int64), ("d_nb2", C.c_int64), ("workspace", C.c_void_p), ("workspace_size", C.c_size_t)]
 
 
+class GqaPrefixAttnArgs(C.Structure):
+    """gqa_prefix_attn_args of include/gqa_batch.h."""
+    _fields_ = [("n_seq", C.c_int32), ("n_prefix", C.c_int32), ("n_head", C.c_int32), ("n_head_kv", C.c_int32), ("dk", C.c_int32), ("dv", C.c_int32),
+                ("type", C.c_int32), ("n_workgroups", C.c_int32), ("scale", C.c_float), ("logit_softcap", C.c_float),
+                ("q", C.c_void_p), ("q_nb1", C.c_int64), ("q_nb2", C.c_int64), ("k", GqaPool), ("v", GqaPool), ("n_pages", C.c_int64),
+                ("block_table", C.c_void_p), ("bt_stride", C.c_int64), ("seq_lens", C.c_void_p), ("prefix_starts", C.c_void_p), ("prefix_lens", C.c_void_p),
+                ("mask", C.c_void_p), ("mask_nb1", C.c_int64), ("mask_ne0", C.c_int64), ("dst", C.c_void_p), ("d_nb1", C.c_int64), ("d_nb2", C.c_int64),
+                ("workspace", C.c_void_p), ("workspace_size", C.c_size_t)]
+
+
 def gqa_norm_rope(q, k, v, pos, *, n_dims, mode=0, n_ctx_orig=0, freq_base=10000.0, freq_scale=1.0, ext_factor=0.0, attn_factor=1.0,
                   beta_fast=32.0, beta_slow=1.0, freq_factors=None, q_weight=None, k_weight=None, eps=1e-6, q_out=None,
                   k_cache=None, v_cache=None, block_table=None, seq_ids=None, slots=None, stream=None):
@@ -497,6 +510,20 @@ def gqa_cross_attn(q, k, v, *, scale, q_starts=None, kv_starts=None, kv_lens=Non
     mask      float16 [n_seq, n] by state of the sequence, as in gqa_prompt_attn
     Returns out, [n_tok, n_head, dv] of q's type; a token without a state gets zeros."""
     return (_native or native()).gqa_cross_attn(q, k, v, q_starts, kv_starts, kv_lens, scale, logit_softcap, mask, out, n_workgroups, stream)
+
+
+def gqa_prefix_attn(q, k_cache, v_cache, block_table, seq_lens, prefix_starts, prefix_lens, *, scale, logit_softcap=0.0, mask=None, out=None,
+                    n_workgroups=0, stream=None):
+    """gqa_attn for a batch in which groups of sequences share their first rows (a system prompt, answers sampled from one context), which are read once a
+    group, on the current torch stream (gqa_prefix_attn_launch, include/gqa_batch.h).
+
+    q, k_cache, v_cache, block_table, seq_lens  as in gqa_attn, all of one 16-bit type; seq_lens counts the shared rows too
+    prefix_starts, prefix_lens  int32 [n + 1], [n]: the sequences prefix_starts[g] .. prefix_starts[g + 1] - 1 lie side by side in the batch, and their first
+              prefix_lens[g] rows are the same keys and values (read through the first one's block table); sequences outside share nothing.
+              PageTable.shared_prefixes finds them
+    mask      float16 [n_seq, n] or None, as in gqa_attn
+    Returns out, [n_seq, n_head, dv] of q's type; a sequence without a row gets zeros."""
+    return (_native or native()).gqa_prefix_attn(q, k_cache, v_cache, block_table, seq_lens, prefix_starts, prefix_lens, scale, logit_softcap, mask, out, n_workgroups, stream)
 
 
 class PageTable:
@@ -598,3 +625,14 @@ class PageTable:
         if rc != 0:
             raise ValueError("mla_page_table_fill_inputs: %d" % rc)
         return bt, sl
+
+    def shared_prefixes(self, seq_ids):
+        """(prefix_starts int32 [n + 1], prefix_lens int32 [n]) of gqa_prefix_attn for a batch of these sequences, in this order: neighbours whose block
+        tables begin with the same pages are a group (others are one alone, with a length of 0)."""
+        import numpy as np
+        seq_ids = np.ascontiguousarray(seq_ids, dtype=np.int32)
+        starts, lens = np.zeros(len(seq_ids) + 1, dtype=np.int32), np.zeros(len(seq_ids), dtype=np.int32)
+        n = self._lib.mla_page_table_shared_prefixes(self._h, len(seq_ids), seq_ids.ctypes.data, starts.ctypes.data, lens.ctypes.data)
+        if n < 0:
+            raise ValueError("mla_page_table_shared_prefixes: %d" % n)
+        return starts[:n + 1].copy(), lens[:n].copy()

@@ -32,12 +32,16 @@
 
 #include <type_traits>
 
-#include "gqa_common.hpp"
+#include "gqa_attn.hpp"
 
 using namespace mla;
 using namespace mla::gqa;
 
 namespace {
+
+// What a launch makes of a sequence's rows: all of them (within the window), or those behind the first `behind[b]`, whose pieces another kernel joins with what it has
+// made of the first ones.
+enum Mode { ALL_ROWS, BEHIND };
 
 struct AttnP {
     const char * q; int64_t q_nb1, q_nb2; int q_f32;
@@ -60,6 +64,7 @@ struct AttnP {
     float *  scores;              // [n_seq][n_head][cap] in log2 units, or nullptr
     float2 * lse;                 // [n_seq][n_head]: maximum, 1 / sum
     int64_t  cap;                 // bt_stride * 128
+    const int32_t * behind;       // [n_seq] (BEHIND)
 };
 
 // Workgroups a CU holds: a wave's tile of K and V, its Q fragments and its accumulators take up to 256 registers for heads up to 192 wide
@@ -83,9 +88,15 @@ __device__ __forceinline__ Span span_from(const AttnP & p, int n) {
     n = min(n, p.mask_len);
     return n > first ? Span{ first, n } : Span{ 0, 0 };
 }
-__device__ __forceinline__ Span span_of(const AttnP & p, int b) { return span_from(p, p.seq_lens[b]); }
-__device__ __forceinline__ Span span_uni(const AttnP & p, int b) {        // b the same in every lane
-    const Span s = span_from(p, scalar_at(p.seq_lens, b));
+__device__ __forceinline__ Span span_behind(Span s, int first) { return s.last > first ? Span{ max(s.first, first), s.last } : Span{ 0, 0 }; }
+template <Mode MODE = ALL_ROWS> __device__ __forceinline__ Span span_of(const AttnP & p, int b) {
+    const Span s = span_from(p, p.seq_lens[b]);
+    if constexpr (MODE == BEHIND) return span_behind(s, p.behind[b]);
+    else                          return s;
+}
+template <Mode MODE = ALL_ROWS> __device__ __forceinline__ Span span_uni(const AttnP & p, int b) {        // b the same in every lane
+    Span s = span_from(p, scalar_at(p.seq_lens, b));
+    if constexpr (MODE == BEHIND) s = span_behind(s, scalar_at(p.behind, b));
     return Span{ uni(s.first), uni(s.last) };
 }
 __device__ __forceinline__ int pages_of(Span s) { return s.last > s.first ? (s.last + PAGE - 1) / PAGE - s.first / PAGE : 0; }
@@ -108,11 +119,11 @@ template <int DV> struct VGeom {
 // head blocks, and the sequence of unit u, where a unit is `per` pages of a head block (the last of a head block fewer).  A lane takes 4
 // consecutive sequences of 256.
 struct Place { int seq, before; };           // the sequence a unit lies in (-1: past the last), and the units before that sequence
-struct Lengths {
+template <Mode MODE = ALL_ROWS> struct Lengths {
     int own[4];                              // pages of this lane's sequences
     __device__ __forceinline__ void fetch(const AttnP & p, int lane, int b0) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) { const int b = b0 + lane * 4 + e; own[e] = b < p.n_seq ? pages_of(span_of(p, b)) : 0; }
+        for (int e = 0; e < 4; e++) { const int b = b0 + lane * 4 + e; own[e] = b < p.n_seq ? pages_of(span_of<MODE>(p, b)) : 0; }
     }
     __device__ __forceinline__ int all_pages(const AttnP & p, int lane) {
         int total = 0;
@@ -170,7 +181,8 @@ __device__ __forceinline__ const char * page_base(const char * data, int page, u
 
 // Wave w takes quarter w of every page of the run.  QUAD: wave w takes whole pages of KV head w of four, which are the run's head block: a row's four
 // heads are read side by side, and the waves have nothing to join.
-template <bool F16, int DK, int DV, int NB, bool BIAS, bool QUAD>
+// BEHIND: what covers a head whole is left like a piece, in dst (f32) and lse.
+template <bool F16, int DK, int DV, int NB, bool BIAS, bool QUAD, Mode MODE = ALL_ROWS>
 __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const AttnP p) {
     static_assert(NB == 1 || !QUAD, "one block of heads a wave");
     constexpr int  KC    = DK / 32;
@@ -187,7 +199,7 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
     const int wg = blockIdx.x;
 
     // ---- which units are this workgroup's
-    Lengths    lens;
+    Lengths<MODE> lens;
     const int  total = lens.all_pages(p, lane);
     const Deal deal{ uni(total / p.n_wg), uni(total % p.n_wg) };
     int        u = uni(run_start(deal, wg));
@@ -195,7 +207,7 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
     if (u >= u_end) return;
     const Place at = lens.place(p, lane, u, 1);
     int  b = uni(at.seq);
-    Span s = span_uni(p, b);
+    Span s = span_uni<MODE>(p, b);
     int  np = uni(pages_of(s));
     int  hb = uni((u - uni(at.before)) / np), pg = u - uni(at.before) - hb * np;
 
@@ -415,12 +427,13 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
             const float inv = l[0] == 0.f ? 0.f : 1.f / l[0];    // (a NaN stays one)
             if (lg == 0 && l15 < heads) {
                 if (!whole) p.part_ml[piece * p.rows + wave * p.group + l15] = make_float2(m[0], l[0]);
+                else if (MODE == BEHIND) p.lse[(int64_t) b * p.n_head + head0 + l15] = make_float2(m[0], l[0]);
                 else if (p.scores) p.lse[(int64_t) b * p.n_head + head0 + l15] = make_float2(m[0] == -INFINITY ? 0.f : m[0], inv);
             }
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int   row = lg * 4 + j;
-                const float f = whole ? __shfl(inv, row, 64) : 1.f;
+                const float f = whole && MODE != BEHIND ? __shfl(inv, row, 64) : 1.f;
                 if (row >= heads) continue;
                 char *  dst = p.dst + (int64_t) b * p.d_nb2 + (int64_t) (head0 + row) * p.d_nb1;
                 float * part = p.part_o + (piece * p.rows + wave * p.group + row) * DV;
@@ -452,6 +465,7 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
         for (int r = threadIdx.x; r < heads; r += 256) {
             const float2 ml = joined(r);
             if (!whole) p.part_ml[piece * p.rows + r] = ml;
+            else if (MODE == BEHIND) p.lse[(int64_t) b * p.n_head + head0 + r] = ml;
             else if (p.scores) p.lse[(int64_t) b * p.n_head + head0 + r] = make_float2(ml.x == -INFINITY ? 0.f : ml.x, ml.y == 0.f ? 0.f : 1.f / ml.y);
         }
         float * part = (float *) lds;                         // [4][16][DV]
@@ -482,7 +496,7 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
                 for (int w = 1; w < 4; w++) o += *(const f32x4 *) (part + (w * 16 + r) * DV + c);
                 if (!whole) *(f32x4 *) (p.part_o + (piece * p.rows + row) * DV + c) = o;
                 else {
-                    const float L = joined(row).y, inv = L == 0.f ? 0.f : 1.f / L;   // (a NaN stays one)
+                    const float L = MODE == BEHIND ? 1.f : joined(row).y, inv = L == 0.f ? 0.f : 1.f / L;   // (a NaN stays one)
                     char * to = p.dst + (int64_t) b * p.d_nb2 + (int64_t) (head0 + row) * p.d_nb1;
                     o *= inv;
                     if (p.dst_f32) *(f32x4 *) (to + c * 4) = o;
@@ -496,7 +510,7 @@ __global__ void __launch_bounds__(256, wg_per_cu(DK, NB)) gqa_attn_kernel(const 
         u += n; pg = 0;
         if (++hb == p.head_blocks && u < u_end) {
             hb = 0;
-            do { b++; s = span_uni(p, b); np = uni(pages_of(s)); } while (np == 0);   // (u < u_end <= total: there is such a sequence)
+            do { b++; s = span_uni<MODE>(p, b); np = uni(pages_of(s)); } while (np == 0);   // (u < u_end <= total: there is such a sequence)
         }
     }
 }
@@ -517,7 +531,7 @@ __global__ void __launch_bounds__(64 * LWAVES) gqa_scores_kernel(const AttnP p) 
     const int wg = blockIdx.x;
     // A workgroup's Q is 147 KB to stage, so no run crosses from one (sequence, head block) to another: units of `per` pages, the fewest of which
     // there are no more than workgroups (units of `top` pages are never more; taking those, 8 x 8192 rows came to 3 pages a unit and 37 us, not 2 and 30); with as many head blocks as workgroups, whole ones in turn.
-    Lengths   lens;
+    Lengths<> lens;
     const int total = lens.all_pages(p, lane), spare = p.n_wg - p.n_seq * p.head_blocks;
     int per = INT_MAX / 2;
     if (spare > 0) {
@@ -904,11 +918,11 @@ template <typename K> hipError_t launch_lds(K kernel, const AttnP & p, int threa
     hipLaunchKernelGGL(kernel, dim3((unsigned) p.n_wg), dim3((unsigned) threads), lds, st, p);
     return hipGetLastError();
 }
-template <bool F16, int DK, int DV, int NB, bool BIAS>
+template <bool F16, int DK, int DV, int NB, bool BIAS, Mode MODE>
 hipError_t launch_main(const AttnP & p, hipStream_t st) {
     static std::atomic<uint64_t> granted{ 0 };
-    if constexpr (NB == 1 && DK < 256) if (p.quad) return launch_lds(gqa_attn_kernel<F16, DK, DV, NB, BIAS, true>, p, 256, 0, granted, st);
-    return launch_lds(gqa_attn_kernel<F16, DK, DV, NB, BIAS, false>, p, 256, 4 * 16 * DV * 4, granted, st);
+    if constexpr (NB == 1 && DK < 256) if (p.quad) return launch_lds(gqa_attn_kernel<F16, DK, DV, NB, BIAS, true, MODE>, p, 256, 0, granted, st);
+    return launch_lds(gqa_attn_kernel<F16, DK, DV, NB, BIAS, false, MODE>, p, 256, 4 * 16 * DV * 4, granted, st);
 }
 template <bool F16, bool BIAS>
 hipError_t launch_scores(const AttnP & p, hipStream_t st) {
@@ -917,14 +931,14 @@ hipError_t launch_scores(const AttnP & p, hipStream_t st) {
     return launch_lds(gqa_scores_kernel<F16, BIAS>, p, 64 * LWAVES, LROWS * LPITCH, granted, st);
 }
 
-template <bool F16, int NB, bool BIAS>
+template <bool F16, int NB, bool BIAS, Mode MODE = ALL_ROWS>
 hipError_t launch_widths(const AttnP & p, int dk, hipStream_t st) {
     switch (dk) {
-        case 64:  return launch_main<F16, 64, 64, NB, BIAS>(p, st);
-        case 128: return launch_main<F16, 128, 128, NB, BIAS>(p, st);
-        case 192: return launch_main<F16, 192, 128, NB, BIAS>(p, st);
+        case 64:  return launch_main<F16, 64, 64, NB, BIAS, MODE>(p, st);
+        case 128: return launch_main<F16, 128, 128, NB, BIAS, MODE>(p, st);
+        case 192: return launch_main<F16, 192, 128, NB, BIAS, MODE>(p, st);
         default:
-            if constexpr (NB == 1) return launch_main<F16, 256, 256, NB, BIAS>(p, st);
+            if constexpr (NB == 1) return launch_main<F16, 256, 256, NB, BIAS, MODE>(p, st);
             else                   return hipErrorInvalidValue;        // (make_plan: one block)
     }
 }
@@ -952,6 +966,27 @@ hipError_t launch_all(const AttnP & p, const Plan & pl, int dk, hipStream_t st) 
     if (p.group <= parts) hipLaunchKernelGGL((gqa_join_kernel<F16, 1>), grid, dim3(JOIN), 0, st, p, joins, parts, (int) ahead);
     else                  hipLaunchKernelGGL((gqa_join_kernel<F16, 8>), grid, dim3(JOIN), 0, st, p, joins, parts, (int) ahead);
     return hipGetLastError();
+}
+
+void fill(AttnP & p, const gqa_attn_args * a, const Plan & pl, char * ws) {
+    p.q = (const char *) a->q; p.q_nb1 = a->q_nb1; p.q_nb2 = a->q_nb2; p.q_f32 = a->q_type == MLA_TYPE_F32;
+    p.k = (const char *) a->k.data; p.k_page = (unsigned) a->k.nb_page; p.k_head = a->k.nb_head; p.k_row = (int) a->k.nb_row;
+    p.v = (const char *) a->v.data; p.v_page = (unsigned) a->v.nb_page; p.v_head = a->v.nb_head; p.v_row = (int) a->v.nb_row;
+    p.n_pages = a->n_pages; p.block_table = a->block_table; p.bt_stride = a->bt_stride; p.seq_lens = a->seq_lens;
+    p.mask = (const char *) a->mask; p.mask_nb1 = a->mask_nb1;
+    p.mask_len = a->mask && a->mask_ne0 < a->bt_stride * PAGE ? (int) a->mask_ne0 : (int) (a->bt_stride * PAGE);
+    p.weights = a->weights; p.w_nb1 = a->w_nb1; p.w_nb2 = a->w_nb2;
+    p.dst = (char *) a->dst; p.d_nb1 = a->d_nb1; p.d_nb2 = a->d_nb2; p.dst_f32 = a->dst_type == MLA_TYPE_F32;
+    p.scale_log2 = a->scale * LOG2E;
+    // (a cap so small or large that these leave f32: the largest number does the same)
+    p.cap_in  = a->logit_softcap > 0.f ? fminf(fmaxf(a->scale / a->logit_softcap, -FLT_MAX), FLT_MAX) : 0.f;
+    p.cap_out = fminf(a->logit_softcap * LOG2E, FLT_MAX);
+    p.window = a->window; p.n_seq = a->n_seq; p.n_head = a->n_head; p.n_head_kv = a->n_head_kv; p.group = a->n_head / a->n_head_kv;
+    p.row_blocks = pl.row_blocks; p.head_blocks = pl.head_blocks; p.rows = pl.rows; p.quad = pl.quad; p.dv = a->dv; p.n_wg = pl.n_wg;
+    p.part_o = (float *) ws; p.part_ml = (float2 *) (ws + pl.off_ml); p.items = (int2 *) (ws + pl.off_items);
+    p.scores = a->weights ? (float *) (ws + pl.off_scores) : nullptr; p.lse = a->weights ? (float2 *) (ws + pl.off_lse) : nullptr;
+    p.cap = a->bt_stride * PAGE;
+    p.behind = nullptr;
 }
 
 int check_pool(const gqa_pool & c) {
@@ -1012,24 +1047,33 @@ extern "C" int gqa_attn_launch(const gqa_attn_args * a, void * stream) {
     if (a->n_seq == 0) return 0;
     const Plan pl = make_plan(a);
     if (!a->workspace || ((uintptr_t) a->workspace & 255) || a->workspace_size < pl.bytes) return MLA_ERR_WORKSPACE;
-    char * ws = (char *) a->workspace;
-    AttnP  p;
-    p.q = (const char *) a->q; p.q_nb1 = a->q_nb1; p.q_nb2 = a->q_nb2; p.q_f32 = a->q_type == MLA_TYPE_F32;
-    p.k = (const char *) a->k.data; p.k_page = (unsigned) a->k.nb_page; p.k_head = a->k.nb_head; p.k_row = (int) a->k.nb_row;
-    p.v = (const char *) a->v.data; p.v_page = (unsigned) a->v.nb_page; p.v_head = a->v.nb_head; p.v_row = (int) a->v.nb_row;
-    p.n_pages = a->n_pages; p.block_table = a->block_table; p.bt_stride = a->bt_stride; p.seq_lens = a->seq_lens;
-    p.mask = (const char *) a->mask; p.mask_nb1 = a->mask_nb1;
-    p.mask_len = a->mask && a->mask_ne0 < a->bt_stride * PAGE ? (int) a->mask_ne0 : (int) (a->bt_stride * PAGE);
-    p.weights = a->weights; p.w_nb1 = a->w_nb1; p.w_nb2 = a->w_nb2;
-    p.dst = (char *) a->dst; p.d_nb1 = a->d_nb1; p.d_nb2 = a->d_nb2; p.dst_f32 = a->dst_type == MLA_TYPE_F32;
-    p.scale_log2 = a->scale * LOG2E;
-    // (a cap so small or large that these leave f32: the largest number does the same)
-    p.cap_in  = a->logit_softcap > 0.f ? fminf(fmaxf(a->scale / a->logit_softcap, -FLT_MAX), FLT_MAX) : 0.f;
-    p.cap_out = fminf(a->logit_softcap * LOG2E, FLT_MAX);
-    p.window = a->window; p.n_seq = a->n_seq; p.n_head = a->n_head; p.n_head_kv = a->n_head_kv; p.group = a->n_head / a->n_head_kv;
-    p.row_blocks = pl.row_blocks; p.head_blocks = pl.head_blocks; p.rows = pl.rows; p.quad = pl.quad; p.dv = a->dv; p.n_wg = pl.n_wg;
-    p.part_o = (float *) ws; p.part_ml = (float2 *) (ws + pl.off_ml); p.items = (int2 *) (ws + pl.off_items);
-    p.scores = a->weights ? (float *) (ws + pl.off_scores) : nullptr; p.lse = a->weights ? (float2 *) (ws + pl.off_lse) : nullptr;
-    p.cap = a->bt_stride * PAGE;
+    AttnP p;
+    fill(p, a, pl, (char *) a->workspace);
     return (int) (a->kv_type == MLA_TYPE_F16 ? launch_all<true>(p, pl, a->dk, (hipStream_t) stream) : launch_all<false>(p, pl, a->dk, (hipStream_t) stream));
+}
+
+// ---------------------------------------------------------------- the rows behind a shared prefix
+
+namespace {
+size_t behind_results(const gqa_attn_args * a) { return ((size_t) a->n_seq * a->n_head * a->dv * 4 + 255) & ~(size_t) 255; }
+}  // namespace
+
+size_t mla::gqa::attn_behind_size(const gqa_attn_args * a) { return make_plan(a).bytes + behind_results(a) + (size_t) a->n_seq * a->n_head * 8; }
+
+hipError_t mla::gqa::attn_behind(const gqa_attn_args * a, const int32_t * behind, char * ws, AttnPieces & out, hipStream_t st) {
+    const Plan pl = make_plan(a);
+    AttnP p;
+    fill(p, a, pl, ws);
+    ws += pl.bytes;
+    p.behind = behind;
+    p.dst = ws; p.dst_f32 = 1; p.d_nb1 = a->dv * 4; p.d_nb2 = (int64_t) a->n_head * a->dv * 4;
+    p.lse = (float2 *) (ws + behind_results(a));
+    out = AttnPieces{ p.part_o, (const float *) p.dst, p.part_ml, p.lse, p.items, p.seq_lens, behind, p.mask_len, (int) p.cap, p.rows, p.row_blocks, p.head_blocks, p.quad };
+    const bool bias = p.mask || p.cap_out != 0.f, f16 = a->kv_type == MLA_TYPE_F16;
+    if (pl.nb == 2) {
+        if (f16) return bias ? launch_widths<true, 2, true, BEHIND>(p, a->dk, st) : launch_widths<true, 2, false, BEHIND>(p, a->dk, st);
+        return bias ? launch_widths<false, 2, true, BEHIND>(p, a->dk, st) : launch_widths<false, 2, false, BEHIND>(p, a->dk, st);
+    }
+    if (f16) return bias ? launch_widths<true, 1, true, BEHIND>(p, a->dk, st) : launch_widths<true, 1, false, BEHIND>(p, a->dk, st);
+    return bias ? launch_widths<false, 1, true, BEHIND>(p, a->dk, st) : launch_widths<false, 1, false, BEHIND>(p, a->dk, st);
 }

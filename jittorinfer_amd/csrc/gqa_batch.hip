@@ -11,23 +11,14 @@ using namespace mla::gqa;
 
 namespace {
 
-// What the three calls have in common.
-struct Call {
-    int32_t n_tok, n_seq, n_head, n_head_kv, dk, dv, type, n_workgroups;
-    float   scale, logit_softcap;
-    const void * q; int64_t q_nb1, q_nb2;
-    const int32_t * q_starts;
-    gqa_pool k, v;
-    int64_t cap;                  // rows a sequence can have
-    const void * mask; int64_t mask_nb1, mask_ne0;
-    void * dst; int64_t d_nb1, d_nb2;
-};
-template <typename A> Call call_of(const A * a, int64_t cap) {
-    return Call{ a->n_tok, a->n_seq, a->n_head, a->n_head_kv, a->dk, a->dv, a->type, a->n_workgroups, a->scale, a->logit_softcap, a->q, a->q_nb1, a->q_nb2, a->q_starts, a->k, a->v, cap,
+template <typename A> BatchCall call_of(const A * a, int64_t cap) {
+    return BatchCall{ a->n_tok, a->n_seq, a->n_head, a->n_head_kv, a->dk, a->dv, a->type, a->n_workgroups, a->scale, a->logit_softcap, a->q, a->q_nb1, a->q_nb2, a->q_starts, a->k, a->v, cap,
                  a->mask, a->mask_nb1, a->mask_ne0, a->dst, a->d_nb1, a->d_nb2 };
 }
 
-BatchPlan make_plan(const Call & c) {
+}  // namespace
+
+BatchPlan mla::gqa::batch_plan(const BatchCall & c, bool whole_blocks) {
     BatchPlan pl;
     const int     group = c.n_head / c.n_head_kv;
     const int64_t rows = ((int64_t) c.n_tok * group + c.n_seq - 1) / c.n_seq;     // of a sequence, on average
@@ -40,20 +31,24 @@ BatchPlan make_plan(const Call & c) {
     pl.n_wg = (int) (have < 1 ? 1 : have < most ? have : most);
     size_t at = 0;
     auto take = [&](size_t n) { const size_t o = at; at += (n + 255) & ~(size_t) 255; return o; };
-    take((size_t) 2 * pl.n_wg * pl.bm * c.dv * 4);
-    pl.off_ml    = take((size_t) 2 * pl.n_wg * pl.bm * 8);
+    const size_t slots = 2 * (size_t) pl.n_wg + (whole_blocks ? (size_t) pl.blocks * c.n_head_kv : 0);
+    take(slots * pl.bm * c.dv * 4);
+    pl.off_ml    = take(slots * pl.bm * 8);
     pl.off_items = take((size_t) pl.blocks * c.n_head_kv * 16);
     pl.bytes = at;
     return pl;
 }
 
+namespace {
 int check_pool(const gqa_pool & c) {
     if (!c.data) return MLA_ERR_NULL;
     if (!al16(c.data) || (c.nb_page & 15) || (c.nb_row & 15) || (c.nb_head & 15)) return MLA_ERR_BAD_ALIGNMENT;
     return c.nb_page < 0 || c.nb_head < 0 || c.nb_row < 0 || c.nb_row > (1 << 23) ? MLA_ERR_BAD_SHAPE : 0;   // (a tile's rows lie within 32 bits)
 }
 
-int check(const Call & c) {
+}  // namespace
+
+int mla::gqa::batch_check(const BatchCall & c) {
     if (c.type != MLA_TYPE_BF16 && c.type != MLA_TYPE_F16) return MLA_ERR_BAD_TYPE;
     if (c.n_tok < 0 || c.n_seq < 0 || c.n_head < 1 || c.n_head_kv < 1 || c.n_head % c.n_head_kv || c.n_workgroups < 0 || c.n_workgroups > 65536) return MLA_ERR_BAD_SHAPE;
     if (c.dk == 64 || c.dk == 128 || c.dk == 256 ? c.dv != c.dk : c.dk != 192 || c.dv != 128) return MLA_ERR_UNSUPPORTED;
@@ -72,16 +67,16 @@ int check(const Call & c) {
     }
     // what is written is nothing that is read (by its address alone: strides may lay one between the other's rows)
     if (c.dst == c.q || c.dst == c.k.data || c.dst == c.v.data || c.dst == c.mask || c.dst == (const void *) c.q_starts) return MLA_ERR_UNSUPPORTED;
-    const BatchPlan pl = make_plan(c);
+    const BatchPlan pl = batch_plan(c, false);
     // (the last launch: fewer than 2^32 threads, and nothing starts of a call whose last could not)
     return (uint64_t) pl.blocks * c.n_head_kv * (c.dv / 32) >= (1 << 24) ? MLA_ERR_BAD_SHAPE : 0;
 }
 
-void fill(BatchP & p, const Call & c, const BatchPlan & pl, void * workspace) {
+void mla::gqa::batch_fill(BatchP & p, const BatchCall & c, const BatchPlan & pl, char * ws) {
     p.q = (const char *) c.q; p.q_nb1 = c.q_nb1; p.q_nb2 = c.q_nb2;
     p.k = (const char *) c.k.data; p.k_page = c.k.nb_page; p.k_head = c.k.nb_head; p.k_row = (int) c.k.nb_row;
     p.v = (const char *) c.v.data; p.v_page = c.v.nb_page; p.v_head = c.v.nb_head; p.v_row = (int) c.v.nb_row;
-    p.block_table = nullptr; p.bt_stride = p.n_pages = 0; p.kv_starts = p.lens = nullptr;
+    p.block_table = nullptr; p.bt_stride = p.n_pages = 0; p.kv_starts = p.lens = p.own_lens = nullptr; p.shared = p.shared_group = nullptr;
     p.q_starts = c.q_starts; p.per = c.n_tok / c.n_seq;
     p.mask = (const char *) c.mask; p.mask_nb1 = c.mask_nb1; p.mask_len = c.mask && c.mask_ne0 < c.cap ? (int) c.mask_ne0 : (int) c.cap;
     p.dst = (char *) c.dst; p.d_nb1 = c.d_nb1; p.d_nb2 = c.d_nb2;
@@ -93,14 +88,14 @@ void fill(BatchP & p, const Call & c, const BatchPlan & pl, void * workspace) {
     p.cap = (int) c.cap; p.n_wg = pl.n_wg;
     // a piece of a block is bm x dv numbers to write and to read again: 4 tiles of 64 keys or more each, fewer for the smaller blocks
     p.min_tiles = c.n_workgroups > 0 || pl.shape == FOUR_KEYS ? 1 : pl.shape == TWO_TWO ? 2 : 4;
-    char * ws = (char *) workspace;
     p.part_o = (float *) ws; p.part_ml = (float2 *) (ws + pl.off_ml); p.items = (int4 *) (ws + pl.off_items);
 }
 
+namespace {
 template <typename A> int ready(const A * a, const BatchPlan & pl) {
     return !a->workspace || ((uintptr_t) a->workspace & 255) || a->workspace_size < pl.bytes ? MLA_ERR_WORKSPACE : 0;
 }
-int launch(const BatchP & p, const Call & c, const BatchPlan & pl, void * stream) {
+int launch(const BatchP & p, const BatchCall & c, const BatchPlan & pl, void * stream) {
     return (int) (c.type == MLA_TYPE_F16 ? batch_launch<true>(p, pl, c.dk, (hipStream_t) stream) : batch_launch<false>(p, pl, c.dk, (hipStream_t) stream));
 }
 
@@ -108,7 +103,7 @@ int launch(const BatchP & p, const Call & c, const BatchPlan & pl, void * stream
 
 // ---------------------------------------------------------------- prompts
 
-static Call prompt_call(const gqa_prompt_attn_args * a) { return call_of(a, a->bt_stride >= 0 && a->bt_stride < INT_MAX ? a->bt_stride * PAGE : INT64_MAX); }
+static BatchCall prompt_call(const gqa_prompt_attn_args * a) { return call_of(a, a->bt_stride >= 0 && a->bt_stride < INT_MAX ? a->bt_stride * PAGE : INT64_MAX); }
 
 extern "C" int gqa_prompt_attn_check(const gqa_prompt_attn_args * a) {
     if (!a) return MLA_ERR_NULL;
@@ -118,19 +113,19 @@ extern "C" int gqa_prompt_attn_check(const gqa_prompt_attn_args * a) {
         if (a->n_pages < 1 || a->bt_stride < 1) return MLA_ERR_BAD_SHAPE;
         if (a->dst && (a->dst == (const void *) a->block_table || a->dst == (const void *) a->seq_lens)) return MLA_ERR_UNSUPPORTED;
     }
-    return check(prompt_call(a));
+    return batch_check(prompt_call(a));
 }
 extern "C" size_t gqa_prompt_attn_workspace_size(const gqa_prompt_attn_args * a) {
-    return gqa_prompt_attn_check(a) || a->n_tok == 0 || a->n_seq == 0 ? 0 : make_plan(prompt_call(a)).bytes;
+    return gqa_prompt_attn_check(a) || a->n_tok == 0 || a->n_seq == 0 ? 0 : batch_plan(prompt_call(a), false).bytes;
 }
 extern "C" int gqa_prompt_attn_launch(const gqa_prompt_attn_args * a, void * stream) {
     int rc = gqa_prompt_attn_check(a);
     if (rc || a->n_tok == 0 || a->n_seq == 0) return rc;
-    const Call      c  = prompt_call(a);
-    const BatchPlan pl = make_plan(c);
+    const BatchCall      c  = prompt_call(a);
+    const BatchPlan pl = batch_plan(c, false);
     if ((rc = ready(a, pl))) return rc;
     BatchP p;
-    fill(p, c, pl, a->workspace);
+    batch_fill(p, c, pl, (char *) a->workspace);
     p.block_table = a->block_table; p.bt_stride = a->bt_stride; p.n_pages = a->n_pages; p.lens = a->seq_lens;
     p.causal = a->causal != 0; p.window = a->window;
     return launch(p, c, pl, stream);
@@ -138,7 +133,7 @@ extern "C" int gqa_prompt_attn_launch(const gqa_prompt_attn_args * a, void * str
 
 // ---------------------------------------------------------------- an encoder's states
 
-static Call cross_call(const gqa_cross_attn_args * a) { return call_of(a, a->n_kv); }
+static BatchCall cross_call(const gqa_cross_attn_args * a) { return call_of(a, a->n_kv); }
 
 extern "C" int gqa_cross_attn_check(const gqa_cross_attn_args * a) {
     if (!a) return MLA_ERR_NULL;
@@ -147,19 +142,19 @@ extern "C" int gqa_cross_attn_check(const gqa_cross_attn_args * a) {
         if (a->kv_starts && (a->k.nb_page || a->v.nb_page)) return MLA_ERR_BAD_SHAPE;
         if (a->dst && (a->dst == (const void *) a->kv_starts || a->dst == (const void *) a->kv_lens)) return MLA_ERR_UNSUPPORTED;
     }
-    return check(cross_call(a));
+    return batch_check(cross_call(a));
 }
 extern "C" size_t gqa_cross_attn_workspace_size(const gqa_cross_attn_args * a) {
-    return gqa_cross_attn_check(a) || a->n_tok == 0 || a->n_seq == 0 ? 0 : make_plan(cross_call(a)).bytes;
+    return gqa_cross_attn_check(a) || a->n_tok == 0 || a->n_seq == 0 ? 0 : batch_plan(cross_call(a), false).bytes;
 }
 extern "C" int gqa_cross_attn_launch(const gqa_cross_attn_args * a, void * stream) {
     int rc = gqa_cross_attn_check(a);
     if (rc || a->n_tok == 0 || a->n_seq == 0) return rc;
-    const Call      c  = cross_call(a);
-    const BatchPlan pl = make_plan(c);
+    const BatchCall      c  = cross_call(a);
+    const BatchPlan pl = batch_plan(c, false);
     if ((rc = ready(a, pl))) return rc;
     BatchP p;
-    fill(p, c, pl, a->workspace);
+    batch_fill(p, c, pl, (char *) a->workspace);
     p.kv_starts = a->kv_starts; p.lens = a->kv_lens;
     return launch(p, c, pl, stream);
 }

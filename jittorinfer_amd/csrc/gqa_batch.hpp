@@ -7,8 +7,8 @@
 namespace mla {
 namespace gqa {
 
-// "Group": the queries that meet one run of keys -- the new tokens of a sequence, or a decoder's over its states.  Its query rows are
-// (token, head of the KV head's group), token-major, cut into blocks of BM.
+// "Group": the queries that meet one run of keys -- the new tokens of a sequence, a decoder's over its states, or (own_lens) one token of each of the sequences that
+// share a prefix, which is read through the first one's pages.  Its query rows are (token, head of the KV head's group), token-major, cut into blocks of BM.
 struct BatchP {
     const char * q; int64_t q_nb1, q_nb2;
     const char * k; int64_t k_page, k_head; int k_row;             // k_page: a page, or (no block table) a group's own part
@@ -17,6 +17,8 @@ struct BatchP {
     const int32_t * kv_starts;
     const int32_t * lens;
     const int32_t * q_starts; int per;                             // q_starts == nullptr: `per` tokens a group
+    const int32_t * own_lens;     // [n_tok] rows of the token's own sequence, or nullptr
+    int32_t * shared, * shared_group;                              // (own_lens) [n_tok]: rows that the token's sequence shares, its group or -1: left for the kernels behind this one
     const char * mask; int64_t mask_nb1; int mask_len;             // mask_len: rows past it are out
     char * dst; int64_t d_nb1, d_nb2;
     float scale_log2;             // |scale| * log2(e)
@@ -25,8 +27,8 @@ struct BatchP {
     int causal, window, n_grp, n_tok, n_head, n_head_kv, group;
     int cap;                      // rows a group can have
     int n_wg, min_tiles;          // workgroups, and the fewest tiles that are worth one
-    float *  part_o;              // [2 * n_wg][BM * dv]: unnormalized sums of the pieces of blocks that several workgroups share, in the lanes' order
-    float2 * part_ml;             // [2 * n_wg][BM]: reference (log2 units), sum
+    float *  part_o;              // [2 * n_wg][BM * dv]: unnormalized sums of the pieces of blocks that several workgroups share, in the lanes' order;
+    float2 * part_ml;             // [2 * n_wg][BM]: reference (log2 units), sum; (own_lens) behind them [block number][n_head_kv]: blocks that one workgroup covered
     int4 *   items;               // [blocks at most][n_head_kv]: slot of the first piece, first workgroup, last workgroup
 };
 
@@ -34,6 +36,21 @@ struct BatchP {
 enum Shape { FOUR_ROWS, TWO_TWO, FOUR_KEYS };
 
 struct BatchPlan { Shape shape; int bm, n_wg, blocks; size_t off_ml, off_items, bytes; };
+
+// What the three calls have in common.
+struct BatchCall {
+    int32_t n_tok, n_seq, n_head, n_head_kv, dk, dv, type, n_workgroups;
+    float   scale, logit_softcap;
+    const void * q; int64_t q_nb1, q_nb2;
+    const int32_t * q_starts;
+    gqa_pool k, v;
+    int64_t cap;                  // rows a sequence can have
+    const void * mask; int64_t mask_nb1, mask_ne0;
+    void * dst; int64_t d_nb1, d_nb2;
+};
+int       batch_check(const BatchCall & c);
+BatchPlan batch_plan(const BatchCall & c, bool whole_blocks);     // whole_blocks: with room for the blocks that one workgroup covers
+void      batch_fill(BatchP & p, const BatchCall & c, const BatchPlan & pl, char * workspace);
 
 template <bool F16> hipError_t batch_launch(const BatchP & p, const BatchPlan & pl, int dk, hipStream_t st);
 

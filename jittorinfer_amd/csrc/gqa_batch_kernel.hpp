@@ -59,13 +59,14 @@ __device__ __forceinline__ Group group_of(const BatchP & p, int g) {
 // What token j of the group sees: rows [first, last).
 struct Span { int first, last; };
 __device__ __forceinline__ Span span_of(const BatchP & p, const Group & g, int j) {
-    const int end = p.causal ? min(max(g.len - g.nq + j + 1, 0), g.len) : g.len;
+    const int end = p.causal ? min(max(g.len - g.nq + j + 1, 0), g.len) : p.own_lens ? min(max(p.own_lens[g.q0 + j], 0), g.len) : g.len;
     return Span{ p.window > 0 ? max(end - p.window, 0) : 0, min(end, p.mask_len) };
 }
 template <int BM> __device__ __forceinline__ int blocks_of(const BatchP & p, const Group & g) { return (int) (((int64_t) g.nq * p.group + BM - 1) / BM); }
 // The tiles that some row of block j sees: [first, last).
 template <int BM, int TK> __device__ __forceinline__ Span tiles_of(const BatchP & p, const Group & g, int j) {
     const int64_t rows = (int64_t) g.nq * p.group, r0 = (int64_t) j * BM;
+    if (p.own_lens) return Span{ 0, (min(g.len, p.mask_len) + TK - 1) / TK };     // (some sequence's whole prefix)
     const int lo = span_of(p, g, (int) (r0 / p.group)).first, hi = span_of(p, g, (int) ((r0 + BM < rows ? r0 + BM : rows) - 1) / p.group).last;
     return hi > lo ? Span{ lo / TK, (hi + TK - 1) / TK } : Span{ 0, 0 };
 }
@@ -167,6 +168,19 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
     const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), wq = wave % NWQ, wk = wave / NWQ, l31 = lane & 31, hh = lane >> 5;
     const unsigned lds0 = (unsigned) (uintptr_t) (LDS_PTR(char)) lds;
 
+    if (p.own_lens)                                                   // whose prefix is whose
+        for (int b = blockIdx.x * 64 * NW + threadIdx.x; b < p.n_tok; b += gridDim.x * 64 * NW) {
+            int lo = 0, hi = p.n_grp;                                 // q_starts[lo] <= b < q_starts[hi], where there are such
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (p.q_starts[mid] <= b) lo = mid;
+                else hi = mid;
+            }
+            const Group g = group_of(p, lo);
+            const bool  in = b >= g.q0 && b < g.q0 + g.nq;
+            p.shared[b] = in ? g.len : 0;
+            p.shared_group[b] = in ? lo : -1;
+        }
     // ---- this workgroup's run
     const int64_t total = total_weight<BM>(p, lane);
     if (total == 0) return;
@@ -209,29 +223,39 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
         const bool  ends_here = same_item(at, end);
         const int   t0 = uni(ts.first + at.tile), t1 = uni(ends_here ? ts.first + end.tile : ts.last);
         const bool  begins = at.tile == 0, whole = begins && !ends_here;
-        const int   slot = 2 * run + (begins ? 1 : 0);
         const int   row0 = at.j * BM + wq * 32;
         const int64_t item = (number_of<BM>(p, at.g, g.q0) + at.j) * p.n_head_kv + at.kvh;
+        const bool  direct = whole && !p.own_lens;
+        const int64_t slot = whole ? 2 * (int64_t) p.n_wg + item : 2 * run + (begins ? 1 : 0);
 
         if (t0 < t1) {
             if (threadIdx.x == 0) {
-                if (begins) { p.items[item].x = slot; p.items[item].y = run; }
+                if (begins) { p.items[item].x = (int) slot; p.items[item].y = run; }
                 if (!ends_here) p.items[item].z = run;
             }
             // ---- this lane's query row (rows past the last repeat it)
             const int  rows = g.nq * p.group, r = min(row0 + l31, rows - 1), tok = r / p.group, head = at.kvh * p.group + r - tok * p.group;
             const Span s = span_of(p, g, tok);
-            // the tiles all rows of the wave see whole, and those any sees: for all rows from the first's to the last's span (spans move on with the token)
-            const Span s_first = Span{ uni(__shfl(s.first, 0, 64)), uni(__shfl(s.last, 0, 64)) }, s_last = Span{ uni(__shfl(s.first, 31, 64)), uni(__shfl(s.last, 31, 64)) };
-            // and the first and the last row of the block
+            // the rows that all of the wave's and that any of them see, and the same of the block: spans move on with the token, but for sequences' own lengths
             const int64_t last_row = min((int64_t) (at.j + 1) * BM, (int64_t) rows) - 1;
-            const Span b_first = span_of(p, g, at.j * BM / p.group), b_last = span_of(p, g, (int) last_row / p.group);
-            const char * mask = BIAS && p.mask ? p.mask + (int64_t) at.g * p.mask_nb1 : nullptr;
+            Span s_first, s_last, b_first, b_last;
+            if (p.own_lens) {
+                int lo = s.last, hi = s.last, least = s.last;
+                if constexpr (BM > 32) for (int i = lane; i < BM; i += 64) least = min(least, span_of(p, g, (int) (min((int64_t) at.j * BM + i, last_row) / p.group)).last);
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) { lo = min(lo, __shfl_xor(lo, d, 64)); hi = max(hi, __shfl_xor(hi, d, 64)); least = min(least, __shfl_xor(least, d, 64)); }
+                s_first = Span{ 0, uni(lo) }; s_last = Span{ 0, uni(hi) }; b_first = b_last = Span{ 0, uni(least) };
+            } else {
+                s_first = Span{ uni(__shfl(s.first, 0, 64)), uni(__shfl(s.last, 0, 64)) }; s_last = Span{ uni(__shfl(s.first, 31, 64)), uni(__shfl(s.last, 31, 64)) };
+                b_first = span_of(p, g, at.j * BM / p.group); b_last = span_of(p, g, (int) last_row / p.group);
+            }
+            const int64_t seq = p.own_lens ? g.q0 : at.g;             // whose pages
+            const char * mask = BIAS && p.mask ? p.mask + (p.own_lens ? (int64_t) (g.q0 + tok) : at.g) * p.mask_nb1 : nullptr;
 
             const int64_t k_off = (int64_t) at.kvh * p.k_head + (p.block_table ? 0 : at.g * p.k_page + g.row0 * p.k_row);
             const int64_t v_off = (int64_t) at.kvh * p.v_head + (p.block_table ? 0 : at.g * p.v_page + g.row0 * p.v_row);
             const uint64_t k_base = uni64((uint64_t) (uintptr_t) p.k + (uint64_t) k_off), v_base = uni64((uint64_t) (uintptr_t) p.v + (uint64_t) v_off);
-            const int32_t * pages = p.block_table + (p.block_table ? (int64_t) at.g * p.bt_stride : 0);
+            const int32_t * pages = p.block_table + (p.block_table ? seq * p.bt_stride : 0);
             auto good = [&](int id) { return id >= 0 && id < p.n_pages; };
             auto page_at = [&](int t) { return uni(pages[t * TK / PAGE]); };
             auto fetch = [&](int t, int id, int buf) {                // tile t to LDS
@@ -481,7 +505,7 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                 m = M; l = L;
             }
             if (wk == 0) {
-                if (whole) {
+                if (direct) {
                     const float inv = l == 0.f ? 0.f : 1.f / l;       // (a NaN stays one)
                     char * dst = p.dst + (int64_t) (g.q0 + tok) * p.d_nb2 + (int64_t) head * p.d_nb1 + hh * 8;
                     if (row0 + l31 < rows)
@@ -491,16 +515,16 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                             for (int c = 0; c < 4; c++)
                                 *(u32x2 *) (dst + n * 64 + c * 16) = pack4<F16>(acc[n][4 * c] * inv, acc[n][4 * c + 1] * inv, acc[n][4 * c + 2] * inv, acc[n][4 * c + 3] * inv);
                 } else {
-                    f32x4 * to = (f32x4 *) p.part_o + (int64_t) slot * (BM * DV / 4) + wq * 64 + lane;
+                    f32x4 * to = (f32x4 *) p.part_o + slot * (BM * DV / 4) + wq * 64 + lane;
 #pragma unroll
                     for (int n = 0; n < NV; n++)
 #pragma unroll
                         for (int c = 0; c < 4; c++) to[(n * 4 + c) * NWQ * 64] = f32x4{ acc[n][4 * c], acc[n][4 * c + 1], acc[n][4 * c + 2], acc[n][4 * c + 3] };
-                    if (hh == 0) p.part_ml[(int64_t) slot * BM + wq * 32 + l31] = make_float2(m, l);
+                    if (hh == 0) p.part_ml[slot * BM + wq * 32 + l31] = make_float2(m, l);
                 }
             }
         } else if (ends_here && at.tile > 0) {                        // nothing of a block that others share: an empty piece
-            for (int i = threadIdx.x; i < BM; i += 64 * NW) p.part_ml[(int64_t) slot * BM + i] = make_float2(-INFINITY, 0.f);
+            for (int i = threadIdx.x; i < BM; i += 64 * NW) p.part_ml[slot * BM + i] = make_float2(-INFINITY, 0.f);
         }
         if (ends_here) return;
         at.tile = 0;
@@ -574,7 +598,7 @@ hipError_t launch_batch(const BatchP & p, const BatchPlan & pl, hipStream_t st) 
     hipError_t e = grant_lds(gqa_batch_kernel<F16, DK, DV, NWQ, NWK, TK, OCC, BIAS>, lds, granted);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((gqa_batch_kernel<F16, DK, DV, NWQ, NWK, TK, OCC, BIAS>), dim3((unsigned) p.n_wg), dim3(64 * NWQ * NWK), lds, st, p);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
+    if ((e = hipGetLastError()) != hipSuccess || p.own_lens) return e;
     hipLaunchKernelGGL((gqa_batch_join_kernel<F16, DV, NWQ, TK>), dim3((unsigned) pl.blocks, (unsigned) p.n_head_kv, DV / 32), dim3(256), 0, st, p);
     return hipGetLastError();
 }

@@ -231,4 +231,41 @@ int mla_page_table_fill_inputs(const mla_page_table * t, int32_t n_seqs, const i
     return 0;
 }
 
+int32_t mla_page_table_shared_prefixes(const mla_page_table * t, int32_t n_seqs, const int32_t * seq_ids, int32_t * starts, int32_t * lens) {
+    if (!t || n_seqs < 0 || !starts || (n_seqs > 0 && (!seq_ids || !lens))) return MLA_PT_ERR_BAD_ARG;
+    for (int32_t i = 0; i < n_seqs; i++) if (!seq_ok(t, seq_ids[i])) return MLA_PT_ERR_BAD_ARG;
+    // pages that sequence i shares with the one before it: what a run of neighbours shares is the least of them
+    std::vector<int32_t> with_last(n_seqs, 0), from(n_seqs + 1, 0), common(n_seqs + 1, 0);
+    for (int32_t i = 1; i < n_seqs; i++) {
+        const auto & a = t->pages[seq_ids[i - 1]], & b = t->pages[seq_ids[i]];
+        const size_t n = std::min(a.size(), b.size());
+        size_t k = 0;
+        while (k < n && a[k] == b[k]) k++;
+        with_last[i] = (int32_t) k;
+    }
+    // best[i]: page reads spared among the first i sequences, the last of their groups from[i] .. i - 1
+    std::vector<int64_t> best(n_seqs + 1, 0);
+    for (int32_t i = 1; i <= n_seqs; i++) {
+        best[i] = best[i - 1]; from[i] = i - 1;
+        int32_t shared = INT32_MAX;
+        for (int32_t j = i - 2; j >= 0; j--) {
+            shared = std::min(shared, with_last[j + 1]);
+            if (shared == 0) break;
+            const int64_t spared = best[j] + (int64_t) (i - 1 - j) * shared;
+            if (spared >= best[i]) { best[i] = spared; from[i] = j; common[i] = shared; }
+        }
+    }
+    int32_t n = 0;
+    for (int32_t i = n_seqs; i > 0; i = from[i]) n++;
+    int32_t g = n;
+    starts[n] = n_seqs;
+    for (int32_t i = n_seqs; i > 0; i = from[i]) {
+        int32_t longest = 0;
+        for (int32_t k = from[i]; k < i; k++) longest = std::max(longest, t->len[seq_ids[k]]);
+        starts[--g] = from[i];
+        lens[g] = i - from[i] > 1 ? std::min(common[i] * PAGE, longest) : 0;
+    }
+    return n;
+}
+
 }  // extern "C"

@@ -65,6 +65,8 @@ struct Bound {
     decltype(&gqa_prompt_attn_launch)  prompt_attn;
     decltype(&gqa_cross_attn_workspace_size) cross_workspace_size;
     decltype(&gqa_cross_attn_launch)   cross_attn;
+    decltype(&gqa_prefix_attn_workspace_size) prefix_workspace_size;
+    decltype(&gqa_prefix_attn_launch)  prefix_attn;
     PyObject * workspace, * workspaces, * raw_stream, * capturing, * elsewhere;
 } lib;
 
@@ -830,9 +832,54 @@ PyObject * gqa_cross_attn(PyObject *, PyObject * const * o, Py_ssize_t n) {
     return rc ? failed("gqa_cross_attn_launch", rc) : result.give(o[9]);
 }
 
+// gqa_prefix_attn(q, k_cache, v_cache, block_table, seq_lens, prefix_starts, prefix_lens, scale, logit_softcap, mask, out, n_workgroups, stream) -> out
+PyObject * gqa_prefix_attn(PyObject *, PyObject * const * o, Py_ssize_t n) {
+    if (!arg_count(n, 13)) return nullptr;
+    const at::Tensor * in[7];
+    for (int i = 0; i < 7; i++) if (!(in[i] = tensor(o[i]))) return nullptr;
+    const at::Tensor & q = *in[0], * kc = in[1], * vc = in[2], * table = in[3], * lens = in[4], * starts = in[5], * plens = in[6], * mask, * outp;
+    if (!optional_tensor(o[9], mask) || !optional_tensor(o[10], outp)) return nullptr;
+    if (!on_gpu(q)) return nullptr;
+    for (const at::Tensor * t : { kc, vc, table, lens, starts, plens, mask, outp }) SAME_DEVICE(t);
+    gqa_prefix_attn_args a;
+    memset(&a, 0, sizeof a);
+    a.scale = (float) PyFloat_AsDouble(o[7]); a.logit_softcap = (float) PyFloat_AsDouble(o[8]);
+    if (PyErr_Occurred() || !int_of(o[11], a.n_workgroups)) return nullptr;
+    REQUIRE(mla_type(q) > 0 && rows_ok(q, 3, false) && q.size(0) < INTS && q.size(1) < INTS && q.size(2) < INTS);
+    const int64_t n_seq = q.size(0);
+    a.n_seq = (int32_t) n_seq; a.n_head = (int32_t) q.size(1); a.dk = (int32_t) q.size(2); a.type = mla_type(q);
+    a.q = q.data_ptr(); a.q_nb1 = step(q, 1); a.q_nb2 = step(q, 0);
+    REQUIRE(cache_ok(*kc, a.type) && kc->size(2) < INTS && kc->size(3) == a.dk);
+    REQUIRE(cache_ok(*vc, a.type) && vc->size(0) == kc->size(0) && vc->size(2) == kc->size(2) && vc->size(3) < INTS);
+    a.n_head_kv = (int32_t) kc->size(2); a.n_pages = kc->size(0); a.dv = (int32_t) vc->size(3);
+    a.k = pool_of(*kc); a.v = pool_of(*vc);
+    REQUIRE(table_ok(*table) && table->size(0) == n_seq && ints(*lens, n_seq));
+    a.block_table = (const int32_t *) table->data_ptr(); a.bt_stride = table->size(1); a.seq_lens = (const int32_t *) lens->data_ptr();
+    REQUIRE(plens->numel() < INTS - 1 && ints(*plens, plens->numel()) && ints(*starts, plens->numel() + 1));
+    a.n_prefix = (int32_t) plens->numel();
+    a.prefix_starts = (const int32_t *) starts->data_ptr(); a.prefix_lens = (const int32_t *) plens->data_ptr();
+    REQUIRE(row_mask(a, mask, n_seq));
+    const c10::DeviceGuard guard(q.device());
+    GqaStream stream;
+    if (!stream.take(o[12], q, !outp)) return nullptr;
+    Result result;
+    REQUIRE(result.take(a, q, outp));
+    if (outp) {
+        Apart apart;
+        apart.add("out", outp);
+        apart.add("q", &q); apart.add("k_cache", kc); apart.add("v_cache", vc); apart.add("block_table", table); apart.add("seq_lens", lens); apart.add("prefix_starts", starts);
+        apart.add("prefix_lens", plens); apart.add("mask", mask);
+        if (n_seq && !apart.check("gqa_prefix_attn", 1)) return nullptr;
+    }
+    GqaScratch scratch;
+    if (!scratch.take(o[0], q, stream, lib.prefix_workspace_size(&a), a)) return nullptr;
+    const int rc = unlocked(a.workspace, [&] { return lib.prefix_attn(&a, stream.st); });
+    return rc ? failed("gqa_prefix_attn_launch", rc) : result.give(o[10]);
+}
+
 // bind(addresses of the entry points in Bound's order, workspace function, workspace table, torch's raw current stream, whether it is capturing, scratch on another stream)
 PyObject * bind(PyObject *, PyObject * const * v, Py_ssize_t n) {
-    constexpr int N = 17;
+    constexpr int N = 19;
     if (!arg_count(n, N + 5)) return nullptr;
     void * p[N];
     for (int i = 0; i < N; i++) p[i] = PyLong_AsVoidPtr(v[i]);
@@ -847,6 +894,7 @@ PyObject * bind(PyObject *, PyObject * const * v, Py_ssize_t n) {
     lib.gqa_attn = (decltype(lib.gqa_attn)) p[10]; lib.evict_workspace_size = (decltype(lib.evict_workspace_size)) p[11];
     lib.evict = (decltype(lib.evict)) p[12];
     lib.prompt_workspace_size = (decltype(lib.prompt_workspace_size)) p[13]; lib.prompt_attn = (decltype(lib.prompt_attn)) p[14];
+    lib.prefix_workspace_size = (decltype(lib.prefix_workspace_size)) p[17]; lib.prefix_attn = (decltype(lib.prefix_attn)) p[18];
     lib.cross_workspace_size = (decltype(lib.cross_workspace_size)) p[15]; lib.cross_attn = (decltype(lib.cross_attn)) p[16];
     lib.workspace = Py_NewRef(v[0]); lib.workspaces = Py_NewRef(v[1]); lib.raw_stream = Py_NewRef(v[2]); lib.capturing = Py_NewRef(v[3]); lib.elsewhere = Py_NewRef(v[4]);
     Py_RETURN_NONE;
@@ -863,7 +911,7 @@ template <PyObject * (*F)(PyObject *, PyObject * const *, Py_ssize_t)> PyObject 
 
 #define FAST(name) { #name, (PyCFunction) (void (*)(void)) entry<name>, METH_FASTCALL, nullptr }
 PyMethodDef methods[] = { FAST(bind), FAST(attn), FAST(rope), FAST(mul_mat), FAST(copy), FAST(kv_write), FAST(front_batch), FAST(gqa_norm_rope), FAST(gqa_attn), FAST(gqa_evict),
-                          FAST(gqa_prompt_attn), FAST(gqa_cross_attn), { nullptr, nullptr, 0, nullptr } };
+                          FAST(gqa_prompt_attn), FAST(gqa_cross_attn), FAST(gqa_prefix_attn), { nullptr, nullptr, 0, nullptr } };
 PyModuleDef module = { PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr };
 
 }  // namespace

@@ -30,7 +30,9 @@ def _set(a, kw):
 
 
 def _common(a):
-    a.n_tok, a.n_seq, a.n_head, a.n_head_kv, a.dk, a.dv = 30, 3, 8, 2, 128, 128
+    if hasattr(a, "n_tok"):
+        a.n_tok, a.n_seq = 30, 3
+    a.n_head, a.n_head_kv, a.dk, a.dv = 8, 2, 128, 128
     a.type, a.scale = J.MLA_TYPE_BF16, 0.1
     a.q, a.q_nb1, a.q_nb2 = 4096, 256, 2048
     a.k, a.v = _pool(128), _pool(128, base=1 << 24)
@@ -48,6 +50,12 @@ def _prompt(**kw):
 def _cross(**kw):
     a = _common(J.GqaCrossAttnArgs())
     a.n_kv = 500
+    return _set(a, kw)
+
+
+def _prefix(**kw):
+    a = _common(J.GqaPrefixAttnArgs())
+    a.n_seq, a.n_prefix, a.n_pages, a.block_table, a.bt_stride, a.seq_lens, a.prefix_starts, a.prefix_lens = 30, 2, 16, 8192, 4, 16384, 16640, 17408
     return _set(a, kw)
 
 
@@ -72,6 +80,19 @@ CROSS_REFUSED = COMMON_REFUSED + [
 ]
 
 
+PREFIX_REFUSED = [(kw, code) for kw, code in COMMON_REFUSED if not {"n_tok", "q_starts"} & set(kw) and kw != dict(dk=576, dv=512)] + [
+    (dict(n_prefix=-1), SHAPE), (dict(block_table=None), NULL), (dict(seq_lens=None), NULL), (dict(prefix_starts=None), NULL), (dict(prefix_lens=None), NULL), (dict(n_pages=0), SHAPE), (dict(bt_stride=0), SHAPE),
+    (dict(bt_stride=1 << 23), SHAPE), (dict(k__nb_page=1 << 32), SHAPE), (dict(n_seq=32768), SHAPE), (dict(dk=576, dv=0, n_head_kv=1), UNSUPPORTED),
+    (dict(dst=8192), UNSUPPORTED), (dict(dst=16384), UNSUPPORTED), (dict(dst=16640), UNSUPPORTED), (dict(dst=17408), UNSUPPORTED),
+]
+
+
+@pytest.mark.parametrize("kw,code", PREFIX_REFUSED, ids=_name)
+def test_prefix_refuses(kw, code):
+    lib, a = J.library(), _prefix(**kw)
+    assert lib.gqa_prefix_attn_check(C.byref(a)) == code and lib.gqa_prefix_attn_launch(C.byref(a), None) == code and lib.gqa_prefix_attn_workspace_size(C.byref(a)) == 0
+
+
 @pytest.mark.parametrize("kw,code", PROMPT_REFUSED, ids=_name)
 def test_prompt_refuses(kw, code):
     lib, a = J.library(), _prompt(**kw)
@@ -92,7 +113,7 @@ def _accepted(name, make, calls):
         a = make(**kw)
         assert check(C.byref(a)) == 0, kw
         need = size(C.byref(a))
-        assert (need > 0) == (a.n_tok > 0 and a.n_seq > 0), kw
+        assert (need > 0) == (getattr(a, "n_tok", 1) > 0 and a.n_seq > 0), kw
         if not need:
             assert launch(C.byref(a), None) == 0
             continue
@@ -114,6 +135,10 @@ def test_cross_accepts():
     _accepted("gqa_cross_attn", _cross, COMMON_ACCEPTED + [dict(n_kv=0), dict(kv_lens=8192), dict(kv_starts=8192, k__nb_page=0, v__nb_page=0), dict(k__nb_page=1 << 40)])
 
 
+def test_prefix_accepts():
+    _accepted("gqa_prefix_attn", _prefix, [kw for kw in COMMON_ACCEPTED if not {"n_tok", "q_starts"} & set(kw)] + [dict(n_prefix=0), dict(n_prefix=0, prefix_starts=None, prefix_lens=None), dict(n_prefix=100)])
+
+
 def test_launches_of_more_threads_than_there_are_refused():
     """Nothing starts of a call whose last kernel could not: 2^24 workgroups of 256 threads that join blocks."""
     lib = J.library()
@@ -128,7 +153,7 @@ def test_exports_and_mirrors_match_the_header(tmp_path):
     text = open(os.path.join(ROOT, "include", "gqa_batch.h")).read()
     bare = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
     declared = set(re.findall(r"\b(gqa_\w+)\s*\(", bare))
-    mirrors = {"gqa_prompt_attn_args": J.GqaPromptAttnArgs, "gqa_cross_attn_args": J.GqaCrossAttnArgs}
+    mirrors = {"gqa_prompt_attn_args": J.GqaPromptAttnArgs, "gqa_cross_attn_args": J.GqaCrossAttnArgs, "gqa_prefix_attn_args": J.GqaPrefixAttnArgs}
     assert declared == {n[:-5] + s for n in mirrors for s in ("_check", "_workspace_size", "_launch")}
     for name in declared:
         assert hasattr(J.library(), name)
@@ -157,6 +182,7 @@ with FakeTensorMode():
     wide = f(3, 128, 2, 64, dtype=torch.float32)
 P = lambda **kw: J.gqa_prompt_attn(**{**dict(q=q, k_cache=k, v_cache=v, block_table=bt, seq_lens=lens, q_starts=starts, scale=1.0), **kw})
 X = lambda **kw: J.gqa_cross_attn(**{**dict(q=q, k=ek, v=ev, q_starts=starts, scale=1.0), **kw})
+S = lambda **kw: J.gqa_prefix_attn(**{**dict(q=q[:2], k_cache=k, v_cache=v, block_table=bt, seq_lens=lens, prefix_starts=lens, prefix_lens=lens[:1], scale=1.0), **kw})
 cpu = torch.zeros(2, dtype=torch.int32)
 calls = dict(
     prompt_cpu=lambda: P(q=torch.zeros(10, 4, 64)), prompt_lens_cpu=lambda: P(seq_lens=cpu), prompt_f32=lambda: P(q=q.float()), prompt_types=lambda: P(q=q.half()), prompt_cache_f32=lambda: P(k_cache=wide, v_cache=wide),
@@ -169,6 +195,9 @@ calls = dict(
     cross_packed_dims=lambda: X(kv_starts=starts), cross_seqs=lambda: X(k=ek[:1], v=ev[:1]), cross_v_rows=lambda: X(v=ev[:, :49]), cross_v_heads=lambda: X(v=ev[:, :, :1]), cross_lens=lambda: X(kv_lens=starts),
     cross_starts=lambda: X(k=ek[0], v=ev[0], kv_starts=lens), cross_starts_short=lambda: X(k=ek[0], v=ev[0], kv_starts=lens[:1], kv_lens=lens), cross_uneven=lambda: X(q=q[:9], q_starts=None), cross_mask=lambda: X(mask=m[:1]),
     cross_out=lambda: X(out=q[:9]), cross_alloc=lambda: X(),
+    prefix_cpu=lambda: S(q=torch.zeros(2, 4, 64)), prefix_lens_cpu=lambda: S(prefix_lens=cpu[:1]), prefix_f32=lambda: S(q=q[:2].float()), prefix_cache=lambda: S(k_cache=wide, v_cache=wide), prefix_seqs=lambda: S(q=q),
+    prefix_table=lambda: S(block_table=bt[:1]), prefix_starts=lambda: S(prefix_starts=starts), prefix_starts_type=lambda: S(prefix_starts=lens.long()), prefix_none=lambda: S(prefix_lens=None), prefix_out=lambda: S(out=q),
+    prefix_mask=lambda: S(mask=m[:1]), prefix_alloc=lambda: S(),
 )
 J.capi.native()
 seen = {}
@@ -188,7 +217,7 @@ def test_python_entry_points_raise():
     r = subprocess.run([sys.executable, "-c", CALLS], cwd=ROOT, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=300)
     assert r.returncode == 0, r.stdout[-2000:]
     seen = json.loads([l for l in r.stdout.splitlines() if l.startswith("SEEN ")][0][5:])
-    assert len(seen) > 40 and set(seen.values()) == {"raised"}, {k: v for k, v in seen.items() if v != "raised"}
+    assert len(seen) > 50 and set(seen.values()) == {"raised"}, {k: v for k, v in seen.items() if v != "raised"}
 
 
 # ---------------------------------------------------------------- the plain forms themselves
@@ -225,3 +254,28 @@ def test_plain_cross_is_prompt_without_order():
     b, _ = B.prompt(q, k, v, torch.tensor([[0], [1]], dtype=torch.int32), [100, 3], [0, 2, 5], 0.3, causal=False)
     c, _ = B.cross(q, torch.cat((k[0, :100], k[1, :3])), torch.cat((v[0, :100], v[1, :3])), [0, 2, 5], [100, 3], 0.3, kv_starts=[0, 100])
     assert torch.allclose(a, b, rtol=1e-12) and torch.allclose(a, c, rtol=1e-12)
+
+
+def test_shared_prefixes_of_a_batch():
+    """Groups are neighbours whose tables begin with the same pages, cut so that the most page reads are spared."""
+    pt = J.PageTable(64, 8, 16)
+    pt.find_slot([0] * 1000, list(range(1000)))          # 7 whole pages and 104 rows
+    for s in (1, 2, 3):
+        pt.seq_cp(0, s, -1, [0, 1000, 700, 300][s])      # 7, 5 and 2 pages shared
+    pt.find_slot([4] * 200, list(range(200)))
+    pt.seq_cp(4, 5)                                      # 1 page shared
+    groups = lambda ids: tuple(x.tolist() for x in pt.shared_prefixes(ids))
+    assert groups([0, 1]) == ([0, 2], [896])
+    assert groups([0, 1, 2]) == ([0, 3], [640])          # 2 x 5 pages spared, 7 without the third
+    assert groups([0, 1, 2, 3]) == ([0, 3, 4], [640, 0])  # 10, against 3 x 2 of all four
+    assert groups([0, 1, 3, 2]) == ([0, 2, 4], [896, 256])
+    assert groups([4, 0, 1, 5]) == ([0, 1, 3, 4], [0, 896, 0])
+    assert groups([4, 5, 0, 1, 6]) == ([0, 2, 4, 5], [128, 896, 0])
+    assert groups([7]) == ([0, 1], [0]) and groups([]) == ([0], []) and groups([6, 7]) == ([0, 1, 2], [0, 0])
+    pt.seq_rm(0, 100)
+    pt.seq_rm(1, 90)
+    assert groups([0, 1]) == ([0, 2], [100])             # one page, of which the longer one has 100 rows
+    with pytest.raises(ValueError):
+        pt.shared_prefixes([0, 8])
+    lib = J.library()
+    assert lib.mla_page_table_shared_prefixes(None, 0, None, None, None) == -2

@@ -340,3 +340,170 @@ def test_cross_strides(gpu, new):
     one = [t[:1, :, :1].expand(3, 150, 2, 64) for t in (k, v)]
     want, off = B.cross(q, *one, starts, lens, 0.125)
     _near(J.gqa_cross_attn(q.to(gpu), *[t[:1, :, :1].to(gpu).expand(3, 150, 2, 64) for t in (k, v)], scale=0.125), want, off, BF16)
+
+
+# ---------------------------------------------------------------- shared prefixes
+
+def _shared(seed, groups, own, heads, kv_heads, dk, dv, dtype, layout="cells", before=0, spare=2, width=None):
+    """groups: (sequences, shared rows); own: rows of its own of every sequence; the first `before` sequences and those past the groups share nothing.  Whole
+    pages of a prefix are the same pages, the one it ends in is each sequence's own copy."""
+    gen = torch.Generator().manual_seed(seed)
+    n_seq = len(own)
+    shared = [0] * before + [p for m, p in groups for _ in range(m)]
+    shared += [0] * (n_seq - len(shared))
+    starts = torch.tensor([before] + [m for m, _ in groups], dtype=torch.int32).cumsum(0).to(torch.int32)
+    lens = [s + o for s, o in zip(shared, own)]
+    width = width or max(1, max((n + 127) // 128 for n in lens))
+    n_pages = sum(p // 128 for _, p in groups) + sum((n + 127) // 128 for n in lens) + spare
+    ids = torch.randperm(n_pages, generator=gen).tolist()
+    k, v = (R.make_cache(gen, n_pages, kv_heads, d, dtype, layout, fill=NAN) for d in (dk, dv))
+    bt = torch.zeros((n_seq, width), dtype=torch.int32)
+    fill = lambda page, rows: [c.__setitem__((page, slice(0, rows)), torch.randn((rows, kv_heads, c.shape[3]), generator=gen).to(dtype)) for c in (k, v)]
+    for g, (m, p) in enumerate(groups):
+        pages = [ids.pop() for _ in range(p // 128)]
+        for page in pages:
+            fill(page, 128)
+        for b in range(int(starts[g]), int(starts[g + 1])):
+            bt[b, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
+    for b in range(n_seq):
+        for j in range(shared[b] // 128, (lens[b] + 127) // 128):
+            bt[b, j] = ids.pop()
+            fill(int(bt[b, j]), min(128, lens[b] - j * 128))
+    for g, (m, p) in enumerate(groups):
+        for b in range(int(starts[g]) + 1, int(starts[g + 1])):
+            if p % 128:
+                for c in (k, v):
+                    c[bt[b, p // 128].long(), :p % 128] = c[bt[int(starts[g]), p // 128].long(), :p % 128]
+    q = torch.randn((n_seq, heads, dk), generator=gen).to(dtype)
+    return q, k, v, bt, torch.tensor(lens, dtype=torch.int32), starts, torch.tensor([p for _, p in groups], dtype=torch.int32)
+
+
+def _prefix(gpu, q, k, v, bt, lens, starts, plens, nan=(), **kw):
+    """nan: sequences that see a NaN."""
+    import jittorinfer_amd as J
+    scale = 1 / math.sqrt(q.shape[2])
+    each = torch.arange(len(lens) + 1)
+    want, off = B.prompt(q, k, v, bt, lens, each, scale, kw.get("logit_softcap", 0.0), 0, True, kw.get("mask"))
+    d = {n: (t.to(gpu) if isinstance(t, torch.Tensor) else t) for n, t in kw.items()}
+    got = J.gqa_prefix_attn(*[t.to(gpu) for t in (q, k, v, bt, lens, starts, plens)], scale=scale, **d)
+    torch.cuda.synchronize()
+    fine = [b for b in range(len(lens)) if b not in nan]
+    assert torch.isnan(got[list(nan)]).all() and torch.isnan(want[list(nan)]).all()
+    _near(got[fine], want[fine], off[fine], q.dtype)
+    return got
+
+
+GROUPS = [(3, 300), (1, 128), (2, 77), (4, 640)]
+OWN = [5, 0, 130, 1, 300, 64, 10, 0, 1, 200, 129, 7]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dk,dv", WIDTHS)
+@pytest.mark.parametrize("layout", ["cells", "heads"])
+def test_prefix_widths_types_layouts(gpu, dk, dv, dtype, layout):
+    _prefix(gpu, *_shared(dk, GROUPS, OWN, 8, 2, dk, dv, dtype, layout, before=1))
+
+
+@pytest.mark.parametrize("dk,dv", WIDTHS)
+@pytest.mark.parametrize("members,heads,kv_heads", [(2, 4, 4), (20, 8, 4), (40, 4, 2), (9, 7, 1), (70, 8, 2), (5, 40, 1)])
+def test_prefix_blocks_of_all_sizes(gpu, dk, dv, members, heads, kv_heads):
+    """32, 64 and 128 rows a block, groups that fill several, heads of one sequence in two blocks."""
+    gen = torch.Generator().manual_seed(members)
+    own = [int(x) for x in torch.randint(0, 40, (members,), generator=gen)]
+    _prefix(gpu, *_shared(members, [(members, 500)], own, heads, kv_heads, dk, dv, BF16))
+    _prefix(gpu, *_shared(members, [(members, 500)], own, heads, kv_heads, dk, dv, F16), n_workgroups=5)
+
+
+@pytest.mark.parametrize("n_workgroups", [1, 2, 3, 7, 16, 100])
+def test_prefix_any_number_of_workgroups(gpu, n_workgroups):
+    _prefix(gpu, *_shared(3, GROUPS, OWN, 4, 2, 64, 64, BF16), n_workgroups=n_workgroups)
+
+
+def test_prefix_four_heads_a_workgroup_behind_it(gpu):
+    """A block table with room for many pages: the rows behind the prefixes are read by waves of a KV head each."""
+    _prefix(gpu, *_shared(4, GROUPS, OWN, 16, 8, 128, 128, BF16, width=40))
+    _prefix(gpu, *_shared(4, GROUPS, OWN, 16, 8, 128, 128, F16, width=40), n_workgroups=3)
+    _prefix(gpu, *_shared(5, [(3, 300), (9, 200)], OWN, 40, 1, 128, 128, BF16, width=300))
+
+
+def test_prefix_groups_of_none_and_lengths_out_of_range(gpu):
+    """Groups without a sequence, prefixes of no row, below 0 and past the table's room, sequences shorter than their prefix, sequences without a row, no group at all."""
+    import jittorinfer_amd as J
+    q, k, v, bt, lens, starts, plens = _shared(6, [(5, 512)], [0, 1, 30, 0, 9, 77], 4, 2, 64, 64, BF16)
+    lens[:4] = torch.tensor([0, 100, 512, 300])
+    got = _prefix(gpu, q, k, v, bt, lens, starts, plens)
+    assert (got[0] == 0).all()
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)
+    for s, n in ((i32(0, 0, 5, 5, 5), i32(100, 512, 3, 0)), (i32(0, 5), i32(0)), (i32(0, 5), i32(-9)), (i32(2, 5), i32(256)), (i32(0, 3, 5), i32(512, 128)), (i32(0), i32())):
+        _prefix(gpu, q, k, v, bt, lens, s, n)
+    q, k, v, bt, lens, starts, plens = _shared(7, [(3, 512)], [0, 0, 0], 4, 2, 64, 64, F16)
+    _prefix(gpu, q, k, v, bt, lens, starts, i32(100000))
+    lens[1] = 100000
+    _prefix(gpu, q, k, v, bt, lens, starts, plens)
+    none = J.gqa_prefix_attn(q[:0].to(gpu), k.to(gpu), v.to(gpu), bt[:0].to(gpu), lens[:0].to(gpu), (starts * 0).to(gpu), plens.to(gpu), scale=1.0)
+    assert none.shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (192, 128), (256, 256)])
+def test_prefix_mask_and_cap(gpu, dk, dv, dtype):
+    """Every sequence its own mask over the shared rows, one that leaves nothing; keys and values that all of them but one take out are NaN or infinite."""
+    q, k, v, bt, lens, starts, plens = _shared(8, GROUPS, OWN, 6, 2, dk, dv, dtype, before=1)
+    mask = _mask(torch.Generator().manual_seed(5), 12, bt.shape[1] * 128)
+    mask[:, 10:14] = float("-inf")
+    mask[:, 130] = float("-inf")
+    mask[8] = float("-inf")
+    mask[9] = torch.randn(mask.shape[1], generator=torch.Generator().manual_seed(6)).to(F16)
+    mask[9, 130] = float("-inf")
+    for b in range(12):
+        for i in (10, 11, 12, 13, 130):
+            if i < lens[b]:
+                k[bt[b, i // 128].long(), i % 128] = NAN
+                v[bt[b, i // 128].long(), i % 128] = float("inf") if i % 2 else NAN
+    got = _prefix(gpu, q, k, v, bt, lens, starts, plens, nan=[9], mask=mask)
+    assert (got[8] == 0).all()
+    _prefix(gpu, q, k, v, bt, lens, starts, plens, nan=[9], mask=mask[:, :200], logit_softcap=15.0, n_workgroups=4)
+    _prefix(gpu, q, k, v, bt, lens, starts, plens, nan=[9], mask=mask[:, :90])
+    mask[9, 10:14] = float("-inf")
+    _prefix(gpu, q, k, v, bt, lens, starts, plens, mask=mask)
+    # a shared row that half of a group of 4 masks: the others' results are not finite, theirs are
+    import jittorinfer_amd as J
+    b0 = int(starts[3])
+    at = 200
+    mask[b0:b0 + 4, at] = 0.0
+    mask[b0, at] = mask[b0 + 2, at] = float("-inf")
+    v[bt[b0, at // 128].long(), at % 128] = float("inf")
+    got = J.gqa_prefix_attn(*[t.to(gpu) for t in (q, k, v, bt, lens, starts, plens)], scale=0.1, mask=mask.to(gpu)).cpu()
+    assert (got[b0 + 1] == float("inf")).all() and (got[b0 + 3] == float("inf")).all()
+    for b in set(range(12)) - {b0 + 1, b0 + 3}:
+        assert torch.isfinite(got[b]).all(), b
+
+
+def test_prefix_bad_pages(gpu):
+    q, k, v, bt, lens, starts, plens = _shared(9, [(3, 512), (2, 300)], [100, 3, 50, 9, 200, 10], 4, 2, 64, 64, BF16)
+    bt[:3, 1], bt[4, 2], bt[5] = -1, k.shape[0], 10 ** 9
+    import jittorinfer_amd as J
+    got = J.gqa_prefix_attn(*[t.to(gpu) for t in (q, k, v, bt, lens, starts, plens)], scale=0.125)
+    # the shared rows of the page that sequence 4 lacks are read through sequence 3's table; its own ones of that page, 300 .. 383, count as masked
+    own, mask = bt.clone(), torch.zeros((6, bt.shape[1] * 128), dtype=F16)
+    own[4, 2] = bt[3, 2]
+    mask[4, 300:384] = float("-inf")
+    want, off = B.prompt(q, k, v, own, lens, torch.arange(7), 0.125, mask=mask)
+    _near(got, want, off, BF16)
+
+
+def test_prefix_many_sequences(gpu):
+    gen = torch.Generator().manual_seed(5)
+    own = [int(x) for x in torch.randint(0, 200, (310,), generator=gen)]
+    _prefix(gpu, *_shared(10, [(100, 200), (1, 128), (150, 300), (40, 256)], own, 2, 1, 64, 64, BF16, before=9))
+
+
+def test_prefix_is_gqa_attn(gpu):
+    """The same call without groups is gqa_attn; with them it differs by the rounding of the weights over the prefix."""
+    import jittorinfer_amd as J
+    q, k, v, bt, lens, starts, plens = (t.to(gpu) for t in _shared(11, GROUPS, OWN, 8, 2, 128, 128, BF16, before=1))
+    a = J.gqa_attn(q, k, v, bt, lens, scale=0.1)
+    assert torch.equal(a, J.gqa_prefix_attn(q, k, v, bt, lens, starts[:1], plens[:0], scale=0.1))
+    b = J.gqa_prefix_attn(q, k, v, bt, lens, starts, plens, scale=0.1)
+    assert (a.double() - b.double()).abs().max() < 2.0 ** -6 * v[torch.isfinite(v)].abs().max().double()
+    assert torch.equal(b, J.gqa_prefix_attn(q, k, v, bt, lens, starts, plens, scale=0.1))
