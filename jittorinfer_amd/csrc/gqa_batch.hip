@@ -35,6 +35,10 @@ BatchPlan mla::gqa::batch_plan(const BatchCall & c, bool whole_blocks) {
     take(slots * pl.bm * c.dv * 4);
     pl.off_ml    = take(slots * pl.bm * 8);
     pl.off_items = take((size_t) pl.blocks * c.n_head_kv * 16);
+    pl.off_tasks = take((size_t) pl.n_wg * 16);
+    // Whole blocks: of one sequence none is heavier than twice the mean, so that the number of them tells; of several the device looks.
+    const int64_t full = (int64_t) c.n_tok * group / pl.bm * c.n_head_kv;
+    pl.deal = whole_blocks || c.n_workgroups > 0 || full * WHOLE_SHARE < fill ? RUNS : c.n_seq == 1 && full * WHOLE_SHARE >= 2 * fill ? WHOLE : EITHER;
     pl.bytes = at;
     return pl;
 }
@@ -68,8 +72,8 @@ int mla::gqa::batch_check(const BatchCall & c) {
     // what is written is nothing that is read (by its address alone: strides may lay one between the other's rows)
     if (c.dst == c.q || c.dst == c.k.data || c.dst == c.v.data || c.dst == c.mask || c.dst == (const void *) c.q_starts) return MLA_ERR_UNSUPPORTED;
     const BatchPlan pl = batch_plan(c, false);
-    // (the last launch: fewer than 2^32 threads, and nothing starts of a call whose last could not)
-    return (uint64_t) pl.blocks * c.n_head_kv * (c.dv / 32) >= (1 << 24) ? MLA_ERR_BAD_SHAPE : 0;
+    // (a launch holds fewer than 2^32 threads, and items are counted in 31 bits)
+    return (uint64_t) pl.blocks * c.n_head_kv >= (1 << 24) ? MLA_ERR_BAD_SHAPE : 0;
 }
 
 void mla::gqa::batch_fill(BatchP & p, const BatchCall & c, const BatchPlan & pl, char * ws) {
@@ -89,6 +93,7 @@ void mla::gqa::batch_fill(BatchP & p, const BatchCall & c, const BatchPlan & pl,
     // a piece of a block is bm x dv numbers to write and to read again: 4 tiles of 64 keys or more each, fewer for the smaller blocks
     p.min_tiles = c.n_workgroups > 0 || pl.shape == FOUR_KEYS ? 1 : pl.shape == TWO_TWO ? 2 : 4;
     p.part_o = (float *) ws; p.part_ml = (float2 *) (ws + pl.off_ml); p.items = (int4 *) (ws + pl.off_items);
+    p.tasks = (int4 *) (ws + pl.off_tasks); p.blocks = pl.blocks; p.deal = pl.deal;
 }
 
 namespace {

@@ -29,13 +29,20 @@ struct BatchP {
     int n_wg, min_tiles;          // workgroups, and the fewest tiles that are worth one
     float *  part_o;              // [2 * n_wg][BM * dv]: unnormalized sums of the pieces of blocks that several workgroups share, in the lanes' order;
     float2 * part_ml;             // [2 * n_wg][BM]: reference (log2 units), sum; (own_lens) behind them [block number][n_head_kv]: blocks that one workgroup covered
-    int4 *   items;               // [blocks at most][n_head_kv]: slot of the first piece, first workgroup, last workgroup
+    int4 *   items;               // [block number][n_head_kv]: slot of the first piece, first run, last run
+    int4 *   tasks;               // [n_wg]: the block that begins in a run and goes on in others (item, first token of the group, its rows, block), or item -1
+    int      blocks, deal;        // block numbers, and a Dealing
 };
+
+// Blocks are dealt in equal runs, one to a workgroup, or the one or the other by what the device finds: whole blocks where the heaviest is at most WHOLE_SHARE of a
+// workgroup's share.
+enum Dealing { RUNS, EITHER, WHOLE };
+constexpr float WHOLE_SHARE = 0.67f;
 
 // Waves along the query rows and along the keys of a tile, keys of a tile.
 enum Shape { FOUR_ROWS, TWO_TWO, FOUR_KEYS };
 
-struct BatchPlan { Shape shape; int bm, n_wg, blocks; size_t off_ml, off_items, bytes; };
+struct BatchPlan { Shape shape; int bm, n_wg, blocks, deal; size_t off_ml, off_items, off_tasks, bytes; };
 
 // What the three calls have in common.
 struct BatchCall {

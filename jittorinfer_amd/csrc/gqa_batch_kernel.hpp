@@ -11,9 +11,9 @@
 //   * the reference of a row moves only when a score passes it by 2^8 (f16: 2^4, with P up to 2^15, so that what f16 loses of a weight is 2^-11 of it down to
 //     2^-25 of the largest).
 //
-// Work: blocks in the order (group, KV head, block) have weights (keys they see, closed sums), and the workgroups take equal runs of the total weight, cut at
-// tiles, from the lengths on the device: a captured launch stays valid while they change.  A run that covers a block writes its result; the others
-// leave (o, m, l) for gqa_batch_join_kernel.
+// Work: where there are blocks enough, a workgroup each, the heavy ones first.  Else blocks in the order (group, KV head, block) have weights (keys they see, closed
+// sums), and the workgroups take equal runs of the total weight, cut at tiles.  A run that covers a block writes its result; the others leave (o, m, l)
+// for gqa_batch_join_kernel.  All of that is decided from the lengths on the device: a captured launch stays valid while they change.
 #pragma once
 
 #include <limits.h>
@@ -92,49 +92,83 @@ __device__ __forceinline__ int64_t scan64(int64_t v, int lane) {
     for (int d = 1; d < 64; d <<= 1) { const int64_t o = __shfl_up(v, d, 64); if (lane >= d) v += o; }
     return v;
 }
-template <int BM> __device__ __forceinline__ int64_t total_weight(const BatchP & p, int lane) {
-    int64_t total = 0;
-    for (int g0 = 0; g0 < p.n_grp; g0 += 64) {
-        int64_t w = 0;
-        if (g0 + lane < p.n_grp) { const Group g = group_of(p, g0 + lane); w = weight_before<BM>(p, g, blocks_of<BM>(p, g)) * p.n_head_kv; }
-        total += __shfl(scan64(w, lane), 63, 64);
-    }
-    return total;
-}
 struct Pos { int g, kvh, j, tile; };             // tile: counted from the block's first
 __device__ __forceinline__ bool same_item(const Pos & a, const Pos & b) { return a.g == b.g && a.kvh == b.kvh && a.j == b.j; }
-template <int BM, int TK> __device__ __forceinline__ Pos place(const BatchP & p, int lane, int64_t at) {
-    int64_t before = 0;
-    for (int g0 = 0; g0 < p.n_grp; g0 += 64) {
-        int64_t w = 0;
-        if (g0 + lane < p.n_grp) { const Group g = group_of(p, g0 + lane); w = weight_before<BM>(p, g, blocks_of<BM>(p, g)) * p.n_head_kv; }
-        const int64_t incl = scan64(w, lane) + before;
-        const uint64_t past = __ballot(at < incl);
-        if (past) {
-            const int l = __ffsll((unsigned long long) past) - 1, gi = uni(g0 + l);
-            const Group   g   = group_of(p, gi);
-            const int     nb  = blocks_of<BM>(p, g);
-            const int64_t per = weight_before<BM>(p, g, nb);
-            int64_t rest = at - __shfl(incl - w, l, 64);
-            const int kvh = (int) (rest / per);
-            rest -= kvh * per;
-            int lo = 0, hi = nb;                                  // weight_before(lo) <= rest < weight_before(hi)
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) / 2;
-                if (weight_before<BM>(p, g, mid) <= rest) lo = mid;
-                else hi = mid;
-            }
-            rest -= weight_before<BM>(p, g, lo);
-            const int64_t mine = weight_before<BM>(p, g, lo + 1) - weight_before<BM>(p, g, lo);
-            const Span    t = tiles_of<BM, TK>(p, g, lo);
-            return Pos{ gi, uni(kvh), uni(lo), uni((int) (rest * (t.last - t.first) / mine)) };
-        }
-        before = __shfl(incl, 63, 64);
+// Every wave works it out for itself, a group a lane; quotients are taken in 64-bit floating point, the same in all workgroups.
+template <int BM, int TK> struct Deal {
+    const BatchP & p;
+    const int lane;
+    Group   g;                                   // this lane's
+    int64_t w;                                   // its weight, over all KV heads
+    __device__ __forceinline__ void fetch(int g0) {
+        w = 0;
+        if (g0 + lane >= p.n_grp) return;
+        g = group_of(p, g0 + lane);
+        w = weight_before<BM>(p, g, blocks_of<BM>(p, g)) * p.n_head_kv;
     }
-    return Pos{ p.n_grp, 0, 0, 0 };
-}
+    // the weight of all blocks, and of the heaviest (the last of a group, at most)
+    __device__ __forceinline__ int64_t total(float & most) {
+        int64_t all = 0;
+        most = 0.f;
+        for (int g0 = 0; g0 < p.n_grp; g0 += 64) {
+            fetch(g0);
+            all += __shfl(scan64(w, lane), 63, 64);
+            const int nb = w ? blocks_of<BM>(p, g) : 0;
+            float last = nb ? (float) (weight_before<BM>(p, g, nb) - weight_before<BM>(p, g, nb - 1)) : 0.f;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) last = fmaxf(last, __shfl_xor(last, d, 64));
+            most = fmaxf(most, last);
+        }
+        return all;
+    }
+    __device__ __forceinline__ Pos place(int64_t at) {           // after total()
+        int64_t before = 0;
+        for (int g0 = 0; g0 < p.n_grp; g0 += 64) {
+            if (p.n_grp > 64) fetch(g0);
+            const int64_t  incl = scan64(w, lane) + before;
+            const uint64_t past = __ballot(at < incl);
+            if (past) {
+                const int l = uni(__ffsll((unsigned long long) past) - 1);
+                const Group o{ __builtin_amdgcn_readlane(g.q0, l), __builtin_amdgcn_readlane(g.nq, l), __builtin_amdgcn_readlane(g.len, l), 0 };
+                const int     nb = blocks_of<BM>(p, o);
+                const int64_t per = weight_before<BM>(p, o, nb);
+                int64_t rest = at - __shfl(incl - w, l, 64);
+                const int kvh = min((int) ((double) rest / (double) per), p.n_head_kv - 1);
+                rest -= kvh * per;
+                int lo = 0, hi = nb;                              // weight_before(lo) <= rest < weight_before(hi)
+                if (!p.causal) lo = max(min((int) ((double) rest / (double) weight_before<BM>(p, o, 1)), nb - 1), 0);
+                else
+                    while (hi - lo > 1) {
+                        const int mid = (lo + hi) / 2;
+                        if (weight_before<BM>(p, o, mid) <= rest) lo = mid;
+                        else hi = mid;
+                    }
+                const int64_t w0 = weight_before<BM>(p, o, lo), mine = weight_before<BM>(p, o, lo + 1) - w0;
+                const Span    t = tiles_of<BM, TK>(p, o, lo);
+                const int     nt = t.last - t.first;
+                return Pos{ uni(g0 + l), uni(kvh), uni(lo), uni(max(min((int) ((double) (rest - w0) * nt / (double) mine), nt - 1), 0)) };
+            }
+            before = __shfl(incl, 63, 64);
+        }
+        return Pos{ p.n_grp, 0, 0, 0 };
+    }
+};
 // Number of block j of group g among all, an upper bound's worth apart: blocks_of(g) are at most the numbers between two groups.
 template <int BM> __device__ __forceinline__ int64_t number_of(const BatchP & p, int g, int q0) { return (int64_t) q0 * p.group / BM + g; }
+
+// The group that a block number belongs to: the last whose first number is not past it, 64 tried at a time.
+template <int BM> __device__ __forceinline__ int group_with(const BatchP & p, int64_t id, int lane) {
+    int lo = 0, n = p.n_grp;
+    while (n > 1) {
+        const int step = (n + 63) / 64, g = lo + lane * step;
+        const bool in = lane * step < n;
+        const int q0 = !in ? 0 : p.q_starts ? min(max(p.q_starts[g], 0), p.n_tok) : g * p.per;
+        const int last = 63 - __clzll((long long) (__ballot(in && number_of<BM>(p, g, q0) <= id) | 1));
+        n = min(step, n - last * step);
+        lo += last * step;
+    }
+    return uni(lo);
+}
 
 __device__ __forceinline__ u32x4 lds128(unsigned at) { return *(LDS_PTR(const u32x4)) (uintptr_t) at; }
 // Four rows' values of this lane's column, twice: rows r .. r + 3 and r + 8 .. r + 11 of the transposed operand.
@@ -181,16 +215,42 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
             p.shared[b] = in ? g.len : 0;
             p.shared_group[b] = in ? lo : -1;
         }
-    // ---- this workgroup's run
-    const int64_t total = total_weight<BM>(p, lane);
-    if (total == 0) return;
-    const int64_t least = (int64_t) p.min_tiles * TK * p.group;
-    const int     runs = (int) max((int64_t) 1, min((int64_t) p.n_wg, total / least));
-    // (workgroups go to the eight dies in turn: neighbouring runs, which share keys, to the same one)
-    if ((int) blockIdx.x >= runs) return;
-    const int x = blockIdx.x & 7, run = uni(x * (runs >> 3) + min(x, runs & 7) + (int) (blockIdx.x >> 3));
-    Pos       at  = place<BM, TK>(p, lane, total / runs * run + min((int64_t) run, total % runs));
-    const Pos end = place<BM, TK>(p, lane, total / runs * (run + 1) + min((int64_t) run + 1, total % runs));
+    // ---- this workgroup's run, or its block
+    Deal<BM, TK> deal{ p, lane };
+    bool single = p.deal == WHOLE;
+    Pos  at, end = { 0, 0, 0, 0 };
+    int  run = blockIdx.x;
+    if (!single) {
+        float         most;
+        const int64_t total = deal.total(most);
+        single = p.deal == EITHER && most * p.n_wg <= WHOLE_SHARE * (float) total;
+        if (!single) {
+            const int64_t least = (int64_t) p.min_tiles * TK * p.group;
+            const int     runs = (int) max((int64_t) (total > 0), min((int64_t) p.n_wg, total / least));
+            if ((int) blockIdx.x >= runs) {
+                if ((int) blockIdx.x < p.n_wg && threadIdx.x == 0) p.tasks[blockIdx.x] = make_int4(-1, 0, 0, 0);
+                return;
+            }
+            // (workgroups go to the eight dies in turn: neighbouring runs, which share keys, to the same one)
+            const int x = blockIdx.x & 7;
+            run = uni(x * (runs >> 3) + min(x, runs & 7) + (int) (blockIdx.x >> 3));
+            // (the block that begins in this run and goes on in others is joined by the workgroup of this number: set where it is left)
+            if (threadIdx.x == 0) p.tasks[run] = make_int4(-1, 0, 0, 0);
+            auto mark = [&](int r) { return (int64_t) ((double) total * r / runs); };
+            at = deal.place(mark(run));
+            if (run + 1 < runs) end = deal.place(mark(run + 1));
+            else end.g = p.n_grp;
+        }
+    }
+    if (single) {                                                     // blocks by falling number: the later ones of a group see the more keys
+        const int64_t id = (int64_t) p.blocks - 1 - blockIdx.x / p.n_head_kv;
+        if (id < 0) return;
+        at.g = group_with<BM>(p, id, lane); at.kvh = blockIdx.x % p.n_head_kv; at.tile = 0;
+        const Group g = group_of(p, at.g);
+        at.j = (int) max(id - number_of<BM>(p, at.g, g.q0), (int64_t) -1);
+        if ((int) blockIdx.x < p.n_wg && threadIdx.x == 0) p.tasks[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        if (at.j < 0 || at.j >= blocks_of<BM>(p, g)) return;
+    }
 
     // ---- what does not change: a lane's places in the tiles
     const int thread = wave * 64 + lane;                              // load j of a tile: 16-byte pieces j * 64 * NW + thread of it
@@ -215,12 +275,16 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
 #pragma unroll
     for (int c = 0; c < KC; c++) k_lo[c] = l31 * (DK * 2) + (((2 * c + hh) ^ swizzle<DK>(l31)) * 16);
 
-    for (; at.g < p.n_grp;) {
+    end = Pos{ uni(end.g), uni(end.kvh), uni(end.j), uni(end.tile) };
+    single = uni(single);
+    for (;;) {
+        at = Pos{ uni(at.g), uni(at.kvh), uni(at.j), uni(at.tile) };
+        if (at.g >= p.n_grp) return;
         const Group g = group_of(p, at.g);
         const int   nb = blocks_of<BM>(p, g);
         const Span  ts = nb > 0 ? tiles_of<BM, TK>(p, g, at.j) : Span{ 0, 0 };
         const int   nt = ts.last - ts.first;
-        const bool  ends_here = same_item(at, end);
+        const bool  ends_here = !single && same_item(at, end);
         const int   t0 = uni(ts.first + at.tile), t1 = uni(ends_here ? ts.first + end.tile : ts.last);
         const bool  begins = at.tile == 0, whole = begins && !ends_here;
         const int   row0 = at.j * BM + wq * 32;
@@ -523,10 +587,18 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                     if (hh == 0) p.part_ml[slot * BM + wq * 32 + l31] = make_float2(m, l);
                 }
             }
+            if (begins && ends_here && threadIdx.x == 0) p.tasks[run] = make_int4((int) item, g.q0, rows, at.j);
+        } else if (nt == 0) {                                         // no row of this block sees a key (several workgroups may find so)
+            for (int i = threadIdx.x; i < BM * (DV / 4) && !p.own_lens; i += 64 * NW) {
+                const int64_t r = (int64_t) at.j * BM + i / (DV / 4);
+                if (r >= (int64_t) g.nq * p.group) break;
+                const int tok = (int) (r / p.group), head = at.kvh * p.group + (int) (r - (int64_t) tok * p.group);
+                *(u32x2 *) (p.dst + (int64_t) (g.q0 + tok) * p.d_nb2 + (int64_t) head * p.d_nb1 + i % (DV / 4) * 8) = u32x2{ 0u, 0u };
+            }
         } else if (ends_here && at.tile > 0) {                        // nothing of a block that others share: an empty piece
             for (int i = threadIdx.x; i < BM; i += 64 * NW) p.part_ml[slot * BM + i] = make_float2(-INFINITY, 0.f);
         }
-        if (ends_here) return;
+        if (ends_here || single) return;
         at.tile = 0;
         if (++at.j >= nb) {
             at.j = 0;
@@ -538,54 +610,72 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
     }
 }
 
-// Joins the pieces of one block: o = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M), in the order of the keys.  Blocks that one run covered are done; rows without a key
-// get zeros.  Grid: x = block numbers, y = KV heads, z = 32 columns of the result.
-template <bool F16, int DV, int NWQ, int TK>
+// Joins the pieces of one block: o = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M).  Grid: x = runs, each of which may leave one block that goes on in others, y = 32 columns of
+// the result.  A thread takes 16 columns of its row (4 loads a piece) and, where a block has fewer than 128 rows, every second or fourth piece.
+template <bool F16, int DV, int NWQ>
 __global__ void __launch_bounds__(256) gqa_batch_join_kernel(const BatchP p) {
-    constexpr int BM = 32 * NWQ;
-    const int lane = threadIdx.x & 63;
-    const int64_t id = blockIdx.x;
-    // the group this number belongs to: the last whose first number is not past it, 64 tried at a time
-    int lo = 0, n = p.n_grp;
-    while (n > 1) {
-        const int step = (n + 63) / 64, g = lo + lane * step;
-        const bool in = lane * step < n;
-        const int q0 = !in ? 0 : p.q_starts ? min(max(p.q_starts[g], 0), p.n_tok) : g * p.per;
-        const int last = 63 - __clzll((long long) (__ballot(in && number_of<BM>(p, g, q0) <= id) | 1));
-        n = min(step, n - last * step);
-        lo += last * step;
-    }
-    lo = uni(lo);
-    const Group   g = group_of(p, lo);
-    const int64_t j = id - number_of<BM>(p, lo, g.q0);
-    if (j < 0 || j >= blocks_of<BM>(p, g)) return;
-    const Span ts = tiles_of<BM, TK>(p, g, (int) j);
-    const bool none = ts.last == ts.first;
-    int4 it = make_int4(0, 0, 0, 0);
-    if (!none) {
-        it = p.items[id * p.n_head_kv + blockIdx.y];
-        if (it.y == it.z) return;
-    }
-    const int pieces = none ? 0 : uni(it.z - it.y + 1), first = uni(it.x), run0 = uni(it.y);
-    auto slot = [&](int i) -> int64_t { return i ? 2 * (run0 + i) : first; };
-    for (int e = threadIdx.x; e < 4 * NWQ * 64; e += 256) {
-        const int c = e / (NWQ * 64), wq = (e / 64) % NWQ, row = wq * 32 + (lane & 31);
-        float M = -INFINITY, L = 0.f;
-        for (int i = 0; i < pieces; i++) M = fmaxf(M, p.part_ml[slot(i) * BM + row].x);
-        f32x4 o = { 0.f, 0.f, 0.f, 0.f };
-        for (int i = 0; i < pieces; i++) {
-            const float2 ml = p.part_ml[slot(i) * BM + row];
-            if (ml.y == 0.f) continue;                                // (an empty piece has no sums)
-            const float w = fast_exp2(ml.x - M);
-            L += ml.y * w;
-            o += ((const f32x4 *) p.part_o)[slot(i) * (BM * DV / 4) + ((int) blockIdx.z * 4 + c) * NWQ * 64 + wq * 64 + lane] * w;
+    constexpr int BM = 32 * NWQ, PG = 4 / NWQ, AHEAD = 4;
+    __shared__ float2 sh_ml[PG > 1 ? PG - 1 : 1][PG > 1 ? BM * 2 : 1];
+    __shared__ f32x4  sh_o[PG > 1 ? PG - 1 : 1][4][PG > 1 ? BM * 2 : 1];
+    const int4 task = p.tasks[blockIdx.x];                            // item, first token of the group, its rows, block
+    if (task.x < 0) return;
+    const int4 it = p.items[task.x];                                  // slot of the first piece, first and last run
+    const int lane = threadIdx.x & 63, wq = (threadIdx.x >> 6) % NWQ, pg = (threadIdx.x >> 6) / NWQ, row = wq * 32 + (lane & 31), mine = wq * 64 + lane;
+    const int pieces = it.z - it.y + 1;
+    auto slot = [&](int i) -> int64_t { return i ? 2 * (it.y + (int64_t) i) : it.x; };
+    float M = -INFINITY, L = 0.f;
+    f32x4 o[4] = {};
+    for (int i0 = pg; i0 < pieces; i0 += PG * AHEAD) {                // (pieces past the last repeat it, without weight)
+        float2 ml[AHEAD];
+        f32x4  x[AHEAD][4];
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) {
+            const int64_t s = slot(min(i0 + a * PG, pieces - 1));
+            ml[a] = p.part_ml[s * BM + row];
+#pragma unroll
+            for (int c = 0; c < 4; c++) x[a][c] = ((const f32x4 *) p.part_o)[s * (BM * DV / 4) + ((int) blockIdx.y * 4 + c) * NWQ * 64 + mine];
         }
-        const int64_t r = j * BM + row;
-        if (r >= (int64_t) g.nq * p.group) continue;
-        const int tok = (int) (r / p.group), head = (int) blockIdx.y * p.group + (int) (r - (int64_t) tok * p.group);
-        o *= L == 0.f ? 0.f : 1.f / L;
-        *(u32x2 *) (p.dst + (int64_t) (g.q0 + tok) * p.d_nb2 + (int64_t) head * p.d_nb1 + ((int) blockIdx.z * 32 + c * 8 + (lane >> 5) * 4) * 2) = pack4<F16>(o.x, o.y, o.z, o.w);
+        float top = M;
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) if (ml[a].y != 0.f) top = fmaxf(top, ml[a].x);
+        const float f = M == top ? 1.f : fast_exp2(M - top);
+        L *= f; M = top;
+#pragma unroll
+        for (int c = 0; c < 4; c++) o[c] *= f;
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) {
+            if (ml[a].y == 0.f || i0 + a * PG >= pieces) continue;    // (an empty piece has no sums)
+            const float w = fast_exp2(ml[a].x - top);
+            L += ml[a].y * w;
+#pragma unroll
+            for (int c = 0; c < 4; c++) o[c] += x[a][c] * w;
+        }
     }
+    if constexpr (PG > 1) {
+        if (pg) {
+            sh_ml[pg - 1][mine] = make_float2(M, L);
+#pragma unroll
+            for (int c = 0; c < 4; c++) sh_o[pg - 1][c][mine] = o[c];
+        }
+        __syncthreads();
+        if (pg) return;
+#pragma unroll
+        for (int q = 0; q < PG - 1; q++) {
+            const float2 ml = sh_ml[q][mine];
+            if (ml.y == 0.f) continue;
+            const float top = fmaxf(M, ml.x), f = M == top ? 1.f : fast_exp2(M - top), w = fast_exp2(ml.x - top);
+            L = L * f + ml.y * w; M = top;
+#pragma unroll
+            for (int c = 0; c < 4; c++) o[c] = o[c] * f + sh_o[q][c][mine] * w;
+        }
+    }
+    const int r = task.w * BM + row;
+    if (r >= task.z) return;
+    const int tok = r / p.group, head = task.x % p.n_head_kv * p.group + r - tok * p.group;
+    const float inv = L == 0.f ? 0.f : 1.f / L;                       // (a NaN stays one)
+    char * dst = p.dst + (int64_t) (task.y + tok) * p.d_nb2 + (int64_t) head * p.d_nb1 + ((int) blockIdx.y * 32 + (lane >> 5) * 4) * 2;
+#pragma unroll
+    for (int c = 0; c < 4; c++) *(u32x2 *) (dst + c * 16) = pack4<F16>(o[c].x * inv, o[c].y * inv, o[c].z * inv, o[c].w * inv);
 }
 
 // ---------------------------------------------------------------- host
@@ -597,9 +687,10 @@ hipError_t launch_batch(const BatchP & p, const BatchPlan & pl, hipStream_t st) 
     static std::atomic<uint64_t> granted{ 0 };
     hipError_t e = grant_lds(gqa_batch_kernel<F16, DK, DV, NWQ, NWK, TK, OCC, BIAS>, lds, granted);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((gqa_batch_kernel<F16, DK, DV, NWQ, NWK, TK, OCC, BIAS>), dim3((unsigned) p.n_wg), dim3(64 * NWQ * NWK), lds, st, p);
-    if ((e = hipGetLastError()) != hipSuccess || p.own_lens) return e;
-    hipLaunchKernelGGL((gqa_batch_join_kernel<F16, DV, NWQ, TK>), dim3((unsigned) pl.blocks, (unsigned) p.n_head_kv, DV / 32), dim3(256), 0, st, p);
+    const int64_t grid = p.deal == RUNS ? p.n_wg : (int64_t) p.blocks * p.n_head_kv;
+    hipLaunchKernelGGL((gqa_batch_kernel<F16, DK, DV, NWQ, NWK, TK, OCC, BIAS>), dim3((unsigned) (grid > p.n_wg ? grid : p.n_wg)), dim3(64 * NWQ * NWK), lds, st, p);
+    if ((e = hipGetLastError()) != hipSuccess || p.own_lens || p.deal == WHOLE) return e;
+    hipLaunchKernelGGL((gqa_batch_join_kernel<F16, DV, NWQ>), dim3((unsigned) p.n_wg, DV / 32), dim3(256), 0, st, p);
     return hipGetLastError();
 }
 template <bool F16, int DK, int DV, bool BIAS>

@@ -16,58 +16,90 @@ using namespace mla::gqa;
 
 namespace {
 
-// Grid: x = sequences, y = KV heads.  A thread takes 4 columns of a head at a time.
+// Grid: x = sequences, y = KV heads.  A thread takes 4 columns of a head at a time and, where a group's heads are few, one of several shares of the pieces: those of the
+// prefix first, then those behind it; AHEAD of them are under way at a time.
+constexpr int JOIN = 256, AHEAD = 4;
 template <bool F16>
-__global__ void __launch_bounds__(256) gqa_prefix_join_kernel(const BatchP p, const AttnPieces a, const int bm, const int dv) {
-    const int b = blockIdx.x, kvh = blockIdx.y, G = p.group;
-    // the prefix's pieces
-    const int g = p.shared_group[b], shared = min(p.shared[b], p.mask_len);
-    int4 it = make_int4(0, 0, 0, 0);
-    int  pre = 0, pre_row = 0;
-    if (g >= 0 && shared > 0) {
-        const int q0 = min(max(p.q_starts[g], 0), p.n_tok), row = (b - q0) * G, j = row / bm;
-        // (a sequence's heads may lie in two blocks: the others' pieces are looked up with them)
-        it = p.items[((int64_t) q0 * G / bm + g + j) * p.n_head_kv + kvh];
-        pre = it.z - it.y + 1; pre_row = row;
-    }
+__global__ void __launch_bounds__(JOIN) gqa_prefix_join_kernel(const BatchP p, const AttnPieces a, const int bm, const int dv) {
+    __shared__ f32x4  sh_o[JOIN];
+    __shared__ float2 sh_ml[JOIN];
+    const int b = blockIdx.x, kvh = blockIdx.y, G = p.group, n_el = G * (dv / 4);
+    const int g = p.shared_group[b];
     const int n = min(min(max(a.seq_lens[b], 0), a.cap), a.mask_len);
-    const bool behind = n > a.behind[b];
-    for (int e = threadIdx.x; e < G * (dv / 4); e += 256) {
-        const int r = e % G, c0 = e / G * 4;
+    const bool has = g >= 0 && min(p.shared[b], p.mask_len) > 0, behind = n > a.behind[b];
+    int64_t item0 = 0;
+    int     row0 = 0;
+    if (has) {
+        const int q0 = min(max(p.q_starts[g], 0), p.n_tok);
+        row0 = (b - q0) * G;
+        item0 = (int64_t) q0 * G / bm + g;
+    }
+    // shares of the pieces: as many as there are threads for (a power of two)
+    int shares = 1;
+    while (shares * 2 * n_el <= JOIN) shares *= 2;
+    for (int e0 = 0; e0 < n_el; e0 += JOIN) {
+        const int e = shares > 1 ? (int) threadIdx.x % n_el : e0 + (int) threadIdx.x, share = shares > 1 ? (int) threadIdx.x / n_el : 0;
+        const bool live = e < n_el && share < shares;
+        const int r = live ? e % G : 0, c0 = live ? e / G * 4 : 0, h = kvh * G + r;
         float M = -INFINITY, L = 0.f;
         f32x4 o = { 0.f, 0.f, 0.f, 0.f };
-        auto add = [&](float2 ml, const f32x4 * from) {               // pieces in order, relative to the largest reference so far
-            if (ml.y == 0.f) return;                                  // (an empty piece has no sums)
-            const f32x4 x = *from;
-            const float top = fmaxf(M, ml.x), f = M == top ? 1.f : fast_exp2(M - top), w = fast_exp2(ml.x - top);
-            o = o * f + x * w; L = L * f + ml.y * w; M = top;
-        };
-        if (pre) {
-            const int row = pre_row + r, j = row / bm, rr = row - j * bm;
-            int4 mine = it;
-            if (j != pre_row / bm) {
-                const int q0 = min(max(p.q_starts[g], 0), p.n_tok);
-                mine = p.items[((int64_t) q0 * G / bm + g + j) * p.n_head_kv + kvh];
-            }
+        if (live) {
+            // the prefix's pieces: runs v0 .. v0 + n0 - 1; those behind it: runs v1 .. v1 + n1 - 1, or one result
+            const int row = row0 + r, j = row / bm, rr = row - j * bm;
             const int at = (((c0 >> 5) * 4 + ((c0 >> 3) & 3)) * (bm / 32) + (rr >> 5)) * 64 + ((c0 >> 2) & 1) * 32 + (rr & 31);
-            for (int v = mine.y; v <= mine.z; v++) {
-                const int64_t slot = v == mine.y ? mine.x : 2 * (int64_t) v;
-                add(p.part_ml[slot * bm + rr], (const f32x4 *) p.part_o + slot * (bm * dv / 4) + at);
+            int4 it = make_int4(0, 0, -1, 0);
+            int2 i2 = make_int2(0, -1);
+            const int hb = a.quad ? kvh >> 2 : kvh * a.row_blocks + r / a.rows, row2 = a.quad ? (kvh & 3) * G + r : r % a.rows;
+            if (has) it = p.items[(item0 + j) * p.n_head_kv + kvh];
+            if (behind) i2 = a.items[(int64_t) b * a.head_blocks + hb];
+            const int v1 = i2.x >> 1, n0 = it.z - it.y + 1, n1 = i2.y - v1 + 1;
+            for (int i0 = share; i0 < n0 + n1; i0 += shares * AHEAD) {
+                float2 ml[AHEAD];
+                f32x4  x[AHEAD];
+#pragma unroll
+                for (int k = 0; k < AHEAD; k++) {                     // (pieces past the last repeat it, without weight)
+                    const int i = min(i0 + k * shares, n0 + n1 - 1);
+                    const float2 * mls;
+                    const float *  os;
+                    if (i < n0) {
+                        const int64_t slot = i ? 2 * (int64_t) (it.y + i) : it.x;
+                        mls = p.part_ml + slot * bm + rr; os = p.part_o + slot * bm * dv + at * 4;
+                    } else if (n1 == 1) {
+                        mls = a.whole_ml + (int64_t) b * p.n_head + h; os = a.whole_o + ((int64_t) b * p.n_head + h) * dv + c0;
+                    } else {
+                        const int64_t slot = i > n0 ? 2 * (int64_t) (v1 + i - n0) : i2.x;
+                        mls = a.part_ml + slot * a.rows + row2; os = a.part_o + (slot * a.rows + row2) * dv + c0;
+                    }
+                    ml[k] = *mls; x[k] = *(const f32x4 *) os;
+                    if (i0 + k * shares >= n0 + n1) ml[k].y = 0.f;
+                }
+                float top = M;
+#pragma unroll
+                for (int k = 0; k < AHEAD; k++) if (ml[k].y != 0.f) top = fmaxf(top, ml[k].x);
+                const float f = M == top ? 1.f : fast_exp2(M - top);
+                o *= f; L *= f; M = top;
+#pragma unroll
+                for (int k = 0; k < AHEAD; k++) {
+                    if (ml[k].y == 0.f) continue;                     // (an empty piece has no sums)
+                    const float w = fast_exp2(ml[k].x - top);
+                    o += x[k] * w; L += ml[k].y * w;
+                }
             }
         }
-        if (behind) {
-            const int h = kvh * G + r, hb = a.quad ? kvh >> 2 : kvh * a.row_blocks + r / a.rows, row = a.quad ? (kvh & 3) * G + r : r % a.rows;
-            const int2 i2 = a.items[(int64_t) b * a.head_blocks + hb];
-            const int  v0 = i2.x >> 1;
-            if (v0 == i2.y) add(a.whole_ml[(int64_t) b * p.n_head + h], (const f32x4 *) (a.whole_o + ((int64_t) b * p.n_head + h) * dv + c0));
-            else
-                for (int v = v0; v <= i2.y; v++) {
-                    const int64_t slot = v == v0 ? i2.x : 2 * (int64_t) v;
-                    add(a.part_ml[slot * a.rows + row], (const f32x4 *) (a.part_o + (slot * a.rows + row) * dv + c0));
-                }
+        if (shares > 1) {
+            sh_o[threadIdx.x] = o; sh_ml[threadIdx.x] = make_float2(M, L);
+            __syncthreads();
+            if (!live || share) return;
+            for (int q = 1; q < shares; q++) {
+                const float2 ml = sh_ml[q * n_el + e];
+                if (ml.y == 0.f) continue;
+                const float top = fmaxf(M, ml.x), f = M == top ? 1.f : fast_exp2(M - top), w = fast_exp2(ml.x - top);
+                o = o * f + sh_o[q * n_el + e] * w; L = L * f + ml.y * w; M = top;
+            }
         }
+        if (!live) continue;
         o *= L == 0.f ? 0.f : 1.f / L;                                // (a NaN stays one)
-        *(u32x2 *) (p.dst + (int64_t) b * p.d_nb2 + (int64_t) (kvh * G + r) * p.d_nb1 + c0 * 2) = u32x2{ pair16<F16>(o.x, o.y), pair16<F16>(o.z, o.w) };
+        *(u32x2 *) (p.dst + (int64_t) b * p.d_nb2 + (int64_t) h * p.d_nb1 + c0 * 2) = u32x2{ pair16<F16>(o.x, o.y), pair16<F16>(o.z, o.w) };
     }
 }
 

@@ -140,9 +140,9 @@ def test_prefix_accepts():
 
 
 def test_launches_of_more_threads_than_there_are_refused():
-    """Nothing starts of a call whose last kernel could not: 2^24 workgroups of 256 threads that join blocks."""
+    """Nothing starts of a call whose last kernel could not: 2^24 workgroups of 256 threads, one a block."""
     lib = J.library()
-    a = _prompt(n_tok=(1 << 28) - 1, n_head=4, n_head_kv=1, dk=256, dv=256)
+    a = _prompt(n_tok=(1 << 28) - 1, n_head=7, n_head_kv=1, dk=256, dv=256)
     assert lib.gqa_prompt_attn_check(C.byref(a)) == SHAPE
     a.n_tok = 1 << 24
     assert lib.gqa_prompt_attn_check(C.byref(a)) == 0

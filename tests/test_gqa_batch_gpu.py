@@ -507,3 +507,12 @@ def test_prefix_is_gqa_attn(gpu):
     b = J.gqa_prefix_attn(q, k, v, bt, lens, starts, plens, scale=0.1)
     assert (a.double() - b.double()).abs().max() < 2.0 ** -6 * v[torch.isfinite(v)].abs().max().double()
     assert torch.equal(b, J.gqa_prefix_attn(q, k, v, bt, lens, starts, plens, scale=0.1))
+
+
+@pytest.mark.parametrize("new,lens", [([900, 0, 700, 130], [1000, 70, 700, 1300]), ([2, 1600, 3], [12000, 1600, 3]), ([3200], [3200]), ([1600, 1600], [100, 1700])])
+def test_prompt_of_many_blocks(gpu, new, lens):
+    """Blocks enough for a workgroup each, by what the device finds (a few that are much longer than the others among them) or in any case."""
+    case = _case(17, new, lens, 96, 64, 64, 64, 64, BF16)
+    _check(gpu, *case, window=300)
+    if sum(lens) < 3000:
+        _check(gpu, *case)
