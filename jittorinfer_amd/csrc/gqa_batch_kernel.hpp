@@ -24,14 +24,30 @@ namespace mla {
 namespace gqa {
 namespace {
 
+// The kernel's arguments where they lie: read again wherever `fresh` has been, which keeps those that the loop over tiles does not need out of its scalar registers.
+typedef const __attribute__((address_space(4))) BatchP Params;
+__device__ __forceinline__ Params * fresh() {
+    Params * p = (Params *) __builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return p;
+}
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ uint64_t uni64(uint64_t v) {
     return (uint64_t) (unsigned) __builtin_amdgcn_readfirstlane((int) (v >> 32)) << 32 | (unsigned) __builtin_amdgcn_readfirstlane((int) v);
 }
 
-// 64 lanes, 16 bytes each: from base + off (a lane's own) to LDS at `lds`, lane by lane.  Waited for by dma_wait().
-__device__ __forceinline__ void dma16(uint64_t base, unsigned off, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(off), "s"(base) : "memory", "m0");
+// N times 64 lanes, 16 bytes each: from base + off[j] (a lane's own) plus the instruction's offset to LDS at `lds` + 1024 j, lane by lane.  Waited for by dma_wait().
+template <int N> __device__ __forceinline__ void dma_tile(uint64_t base, const unsigned (&off)[N], unsigned lds) {
+    static_assert(N == 2 || N == 4 || N == 6 || N == 8, "");
+    if constexpr (N % 4 == 2)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %1\n\tglobal_load_lds_dwordx4 %3, %1 offset:1024"
+                     : : "s"(lds), "s"(base), "v"(off[0]), "v"(off[1]) : "memory", "m0");
+    constexpr int AT = N % 4;
+#pragma unroll
+    for (int j = AT; j < N; j += 4)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %1\n\tglobal_load_lds_dwordx4 %3, %1 offset:1024\n\t"
+                     "global_load_lds_dwordx4 %4, %1 offset:2048\n\tglobal_load_lds_dwordx4 %5, %1 offset:3072"
+                     : : "s"(lds + j * 1024), "s"(base), "v"(off[j]), "v"(off[j + 1]), "v"(off[j + 2]), "v"(off[j + 3]) : "memory", "m0");
 }
 __device__ __forceinline__ void dma_wait() { __builtin_amdgcn_s_waitcnt(0x0f70); }              // vmcnt(0)
 
@@ -42,7 +58,7 @@ template <int D> __device__ __forceinline__ int swizzle(int r) {
 }
 
 struct Group { int q0, nq, len; int64_t row0; };
-__device__ __forceinline__ Group group_of(const BatchP & p, int g) {
+__device__ __forceinline__ Group group_of(Params & p, int g) {
     Group r;
     r.q0 = p.q_starts ? min(max(p.q_starts[g], 0), p.n_tok) : g * p.per;
     r.nq = p.q_starts ? min(max(p.q_starts[g + 1], r.q0), p.n_tok) - r.q0 : p.per;
@@ -58,13 +74,13 @@ __device__ __forceinline__ Group group_of(const BatchP & p, int g) {
 }
 // What token j of the group sees: rows [first, last).
 struct Span { int first, last; };
-__device__ __forceinline__ Span span_of(const BatchP & p, const Group & g, int j) {
+__device__ __forceinline__ Span span_of(Params & p, const Group & g, int j) {
     const int end = p.causal ? min(max(g.len - g.nq + j + 1, 0), g.len) : p.own_lens ? min(max(p.own_lens[g.q0 + j], 0), g.len) : g.len;
     return Span{ p.window > 0 ? max(end - p.window, 0) : 0, min(end, p.mask_len) };
 }
-template <int BM> __device__ __forceinline__ int blocks_of(const BatchP & p, const Group & g) { return (int) (((int64_t) g.nq * p.group + BM - 1) / BM); }
+template <int BM> __device__ __forceinline__ int blocks_of(Params & p, const Group & g) { return (int) (((int64_t) g.nq * p.group + BM - 1) / BM); }
 // The tiles that some row of block j sees: [first, last).
-template <int BM, int TK> __device__ __forceinline__ Span tiles_of(const BatchP & p, const Group & g, int j) {
+template <int BM, int TK> __device__ __forceinline__ Span tiles_of(Params & p, const Group & g, int j) {
     const int64_t rows = (int64_t) g.nq * p.group, r0 = (int64_t) j * BM;
     if (p.own_lens) return Span{ 0, (min(g.len, p.mask_len) + TK - 1) / TK };     // (some sequence's whole prefix)
     const int lo = span_of(p, g, (int) (r0 / p.group)).first, hi = span_of(p, g, (int) ((r0 + BM < rows ? r0 + BM : rows) - 1) / p.group).last;
@@ -78,7 +94,7 @@ __device__ __forceinline__ int64_t sum_clamped(int64_t a, int s, int64_t top, in
     return mid * a + s * ((i0 + i1 - 1) * mid / 2) + (n - i1) * top;
 }
 // Weight of blocks 0 .. n - 1 of a group: the keys each sees, times the heads of the KV head's group, and 128 keys for what a block costs by itself.
-template <int BM> __device__ __forceinline__ int64_t weight_before(const BatchP & p, const Group & g, int64_t n) {
+template <int BM> __device__ __forceinline__ int64_t weight_before(Params & p, const Group & g, int64_t n) {
     const int64_t G = p.group, all = G * g.len;
     int64_t keys;
     if (p.causal) {
@@ -96,7 +112,7 @@ struct Pos { int g, kvh, j, tile; };             // tile: counted from the block
 __device__ __forceinline__ bool same_item(const Pos & a, const Pos & b) { return a.g == b.g && a.kvh == b.kvh && a.j == b.j; }
 // Every wave works it out for itself, a group a lane; quotients are taken in 64-bit floating point, the same in all workgroups.
 template <int BM, int TK> struct Deal {
-    const BatchP & p;
+    Params & p;
     const int lane;
     Group   g;                                   // this lane's
     int64_t w;                                   // its weight, over all KV heads
@@ -154,10 +170,10 @@ template <int BM, int TK> struct Deal {
     }
 };
 // Number of block j of group g among all, an upper bound's worth apart: blocks_of(g) are at most the numbers between two groups.
-template <int BM> __device__ __forceinline__ int64_t number_of(const BatchP & p, int g, int q0) { return (int64_t) q0 * p.group / BM + g; }
+template <int BM> __device__ __forceinline__ int64_t number_of(Params & p, int g, int q0) { return (int64_t) q0 * p.group / BM + g; }
 
 // The group that a block number belongs to: the last whose first number is not past it, 64 tried at a time.
-template <int BM> __device__ __forceinline__ int group_with(const BatchP & p, int64_t id, int lane) {
+template <int BM> __device__ __forceinline__ int group_with(Params & p, int64_t id, int lane) {
     int lo = 0, n = p.n_grp;
     while (n > 1) {
         const int step = (n + 63) / 64, g = lo + lane * step;
@@ -176,6 +192,14 @@ __device__ __forceinline__ u32x4 lds_transposed(unsigned lo, unsigned hi) {
     const u32x2 a = bitcast<u32x2>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4)) (uintptr_t) lo)), b = bitcast<u32x2>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4)) (uintptr_t) hi));
     return u32x4{ a.x, a.y, b.x, b.y };
 }
+// Two numbers to 16 bits each, to nearest even, in one instruction.
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+template <bool F16> __device__ __forceinline__ unsigned packed16(float a, float b) {
+    if constexpr (F16) return bitcast<unsigned>(__builtin_convertvector(f32x2{ a, b }, f16x2));
+    else               return bitcast<unsigned>(__builtin_convertvector(f32x2{ a, b }, bf16x2));
+}
+// An address in a register of its own, so that constants added to it become the instructions' offsets.
+__device__ __forceinline__ unsigned base_of(unsigned a) { asm("" : "+v"(a)); return a; }
 // l + the two 16-bit numbers of `pair`: the sum is over the weights as they are multiplied, so that a row of one key gets its value as it is.
 template <bool F16> __device__ __forceinline__ float add_pair(float l, unsigned pair) {
     if constexpr (F16) return __builtin_amdgcn_fdot2(bitcast<f16x2>(pair), f16x2{ (_Float16) 1.f, (_Float16) 1.f }, l, false);
@@ -187,10 +211,10 @@ template <bool F16> __device__ __forceinline__ unsigned nonfinite(unsigned x) { 
 }
 __device__ __forceinline__ unsigned halves(unsigned bits15) { return (bits15 >> 15) * 0xffffu; }  // all bits of those halves
 
-template <bool F16> __device__ __forceinline__ u32x2 pack4(float a, float b, float c, float d) { return u32x2{ pair16<F16>(a, b), pair16<F16>(c, d) }; }
+template <bool F16> __device__ __forceinline__ u32x2 pack4(float a, float b, float c, float d) { return u32x2{ packed16<F16>(a, b), packed16<F16>(c, d) }; }
 
 template <bool F16, int DK, int DV, int NWQ, int NWK, int TK, int OCC, bool BIAS>
-__global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const BatchP p) {
+__global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const BatchP) {
     constexpr int NW = NWQ * NWK, BM = 32 * NWQ, KW = TK / NWK, KB = KW / 32, KC = DK / 16, NV = DV / 32;
     constexpr int KT = TK * DK * 2, VT = TK * DV * 2, KI = KT / 1024 / NW, VI = VT / 1024 / NW;
     static_assert(KW % 32 == 0 && KI * 1024 * NW == KT && VI * 1024 * NW == VT, "whole pieces");
@@ -201,6 +225,11 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
 
     const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), wq = wave % NWQ, wk = wave / NWQ, l31 = lane & 31, hh = lane >> 5;
     const unsigned lds0 = (unsigned) (uintptr_t) (LDS_PTR(char)) lds;
+    Pos  at, end = { 0, 0, 0, 0 };
+    int  run = blockIdx.x;
+    bool single;
+    {
+    Params & p = *fresh();
 
     if (p.own_lens)                                                   // whose prefix is whose
         for (int b = blockIdx.x * 64 * NW + threadIdx.x; b < p.n_tok; b += gridDim.x * 64 * NW) {
@@ -217,9 +246,7 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
         }
     // ---- this workgroup's run, or its block
     Deal<BM, TK> deal{ p, lane };
-    bool single = p.deal == WHOLE;
-    Pos  at, end = { 0, 0, 0, 0 };
-    int  run = blockIdx.x;
+    single = p.deal == WHOLE;
     if (!single) {
         float         most;
         const int64_t total = deal.total(most);
@@ -251,18 +278,23 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
         if ((int) blockIdx.x < p.n_wg && threadIdx.x == 0) p.tasks[blockIdx.x] = make_int4(-1, 0, 0, 0);
         if (at.j < 0 || at.j >= blocks_of<BM>(p, g)) return;
     }
+    }
 
     // ---- what does not change: a lane's places in the tiles
-    const int thread = wave * 64 + lane;                              // load j of a tile: 16-byte pieces j * 64 * NW + thread of it
-    auto row_in = [&](int d, int j) { return (j * 64 * NW + thread) / (d / 8); };
-    auto chunk_in = [&](int d, int j) { const int r = row_in(d, j), c = (j * 64 * NW + thread) % (d / 8); return c ^ (d % 128 == 0 ? swizzle<128>(r) : swizzle<64>(r)); };
-    // rows of a tile that lie KS apart have the same places: one offset a lane, and the step is the base's
-    constexpr int KS = (512 * NW / DK) % 16 == 0 && 512 % DK == 0 ? 512 * NW / DK : 0, VS = (512 * NW / DV) % 16 == 0 && 512 % DV == 0 ? 512 * NW / DV : 0;
-    unsigned k_at[KS ? 1 : KI], v_at[VS ? 1 : VI];
+    // (a wave's loads of a tile lie one behind the other; an instruction's offset counts for both its places, so one that is ahead in LDS is taken back in memory)
+    auto step_of = [](int per, int j) { return j < per % 4 ? j : (j - per % 4) % 4; };
+    auto row_in = [&](int d, int per, int j) { return ((wave * per + j) * 64 + lane) / (d / 8); };
+    auto place_in = [&](int d, int per, int j) { const int r = row_in(d, per, j), c = ((wave * per + j) * 64 + lane) % (d / 8); return (c ^ (d % 128 == 0 ? swizzle<128>(r) : swizzle<64>(r))) * 16 + (4 - step_of(per, j)) * 1024; };
+    int k_row, v_row;
+    unsigned k_at[KI], v_at[VI];
+    {
+        Params & p = *fresh();
+        k_row = p.k_row; v_row = p.v_row;
 #pragma unroll
-    for (int j = 0; j < (KS ? 1 : KI); j++) k_at[j] = (unsigned) (row_in(DK, j) * p.k_row + chunk_in(DK, j) * 16);
+        for (int j = 0; j < KI; j++) k_at[j] = (unsigned) (row_in(DK, KI, j) * k_row + place_in(DK, KI, j));
 #pragma unroll
-    for (int j = 0; j < (VS ? 1 : VI); j++) v_at[j] = (unsigned) (row_in(DV, j) * p.v_row + chunk_in(DV, j) * 16);
+        for (int j = 0; j < VI; j++) v_at[j] = (unsigned) (row_in(DV, VI, j) * v_row + place_in(DV, VI, j));
+    }
     // transposing reads: row, 16-byte chunk and half of it; the addresses of a chunk of 32 columns, for rows 0 .. 3 and 8 .. 11 of 16
     const int vq = hh * 4 + ((lane >> 2) & 3), vc = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), vsub = (lane & 1) * 8;
     unsigned v_lo[NV], v_hi[NV];
@@ -279,6 +311,7 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
     single = uni(single);
     for (;;) {
         at = Pos{ uni(at.g), uni(at.kvh), uni(at.j), uni(at.tile) };
+        Params & p = *fresh();
         if (at.g >= p.n_grp) return;
         const Group g = group_of(p, at.g);
         const int   nb = blocks_of<BM>(p, g);
@@ -320,24 +353,26 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
             const int64_t v_off = (int64_t) at.kvh * p.v_head + (p.block_table ? 0 : at.g * p.v_page + g.row0 * p.v_row);
             const uint64_t k_base = uni64((uint64_t) (uintptr_t) p.k + (uint64_t) k_off), v_base = uni64((uint64_t) (uintptr_t) p.v + (uint64_t) v_off);
             const int32_t * pages = p.block_table + (p.block_table ? seq * p.bt_stride : 0);
-            auto good = [&](int id) { return id >= 0 && id < p.n_pages; };
+            const int64_t n_pages = p.n_pages, k_page = p.block_table ? p.k_page : 0, v_page = p.block_table ? p.v_page : 0;
+            const bool paged = p.block_table != nullptr;
+            auto good = [&](int id) { return id >= 0 && id < n_pages; };
             auto page_at = [&](int t) { return uni(pages[t * TK / PAGE]); };
             auto fetch = [&](int t, int id, int buf) {                // tile t to LDS
-                const int key0 = t * TK, valid = min(TK, g.len - key0), pg = good(id) ? id : 0;       // (a bad id: page 0 is read, not used)
-                const int row = p.block_table ? key0 % PAGE : key0;
-                const uint64_t kb = uni64(k_base + (uint64_t) ((p.block_table ? pg * p.k_page : 0) + (int64_t) row * p.k_row));
-                const uint64_t vb = uni64(v_base + (uint64_t) ((p.block_table ? pg * p.v_page : 0) + (int64_t) row * p.v_row));
-                const unsigned to = uni(lds0 + buf * (KT + VT) + wave * 1024);
-                if (valid == TK) {
-#pragma unroll
-                    for (int j = 0; j < KI; j++) dma16(kb + (KS ? (uint64_t) (j * KS) * p.k_row : 0), k_at[KS ? 0 : j], to + j * NW * 1024);
-#pragma unroll
-                    for (int j = 0; j < VI; j++) dma16(vb + (VS ? (uint64_t) (j * VS) * p.v_row : 0), v_at[VS ? 0 : j], to + KT + j * NW * 1024);
+                const int key0 = t * TK, row = paged ? key0 % PAGE : key0, pg = good(id) ? id : 0;    // (a bad id: page 0 is read, not used)
+                const uint64_t kb = uni64(k_base + (uint64_t) (pg * k_page + (int64_t) row * k_row)) - 4096, vb = uni64(v_base + (uint64_t) (pg * v_page + (int64_t) row * v_row)) - 4096;
+                const unsigned to = uni(lds0 + buf * (KT + VT)), k_to = to + wave * (KI * 1024), v_to = to + KT + wave * (VI * 1024);
+                if (key0 + TK <= g.len) {
+                    dma_tile<KI>(kb, k_at, k_to);
+                    dma_tile<VI>(vb, v_at, v_to);
                 } else {                                              // (rows past the last repeat it)
+                    const int last = g.len - key0 - 1;
+                    unsigned k_end[KI], v_end[VI];
 #pragma unroll
-                    for (int j = 0; j < KI; j++) dma16(kb, (unsigned) (min(row_in(DK, j), valid - 1) * p.k_row + chunk_in(DK, j) * 16), to + j * NW * 1024);
+                    for (int j = 0; j < KI; j++) k_end[j] = (unsigned) (min(row_in(DK, KI, j), last) * k_row + place_in(DK, KI, j));
 #pragma unroll
-                    for (int j = 0; j < VI; j++) dma16(vb, (unsigned) (min(row_in(DV, j), valid - 1) * p.v_row + chunk_in(DV, j) * 16), to + KT + j * NW * 1024);
+                    for (int j = 0; j < VI; j++) v_end[j] = (unsigned) (min(row_in(DV, VI, j), last) * v_row + place_in(DV, VI, j));
+                    dma_tile<KI>(kb, k_end, k_to);
+                    dma_tile<VI>(vb, v_end, v_to);
                 }
             };
             // (the mask's numbers of the next tile are requested ahead of its keys: a wait for them is no wait for those)
@@ -385,15 +420,26 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
 
             // S^T of the wave's keys
             auto products = [&](unsigned kt, f32x16 (&sc)[KB]) {
+                unsigned at[KC];
+#pragma unroll
+                for (int c = 0; c < KC; c++) at[c] = base_of(kt + k_lo[c]);
 #pragma unroll
                 for (int b = 0; b < KB; b++) {
 #pragma unroll
                     for (int e = 0; e < 16; e++) sc[b][e] = 0.f;
 #pragma unroll
-                    for (int c = 0; c < KC; c++) sc[b] = mfma32<F16>(lds128(kt + b * 32 * (DK * 2) + k_lo[c]), qf[c], sc[b]);
+                    for (int c = 0; c < KC; c++) sc[b] = mfma32<F16>(lds128(at[c] + b * 32 * (DK * 2)), qf[c], sc[b]);
                 }
+                // the order of it: reads some ahead of the products
+                constexpr int LEAD = KC < 8 ? KC : 8;
+                __builtin_amdgcn_sched_group_barrier(0x100, LEAD, 0);
+#pragma unroll
+                for (int i = 0; i < KB * KC - LEAD; i++) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, LEAD, 0);
             };
-            auto value = [&](unsigned vt, int b, int kk, int n) { const unsigned at16 = vt + (b * 32 + kk * 16) * (DV * 2); return lds_transposed(at16 + v_lo[n], at16 + v_hi[n]); };
 
             for (int t = t0; t < t1; t++) {
                 dma_wait();
@@ -501,20 +547,42 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                             for (int e = 0; e < 16; e++) acc[n][e] *= a;
                     }
                     const float mm = m == -INFINITY ? 0.f : m;
+                    // O^T += V^T P^T, 32 columns and 16 keys a product, in the order as it stands here: values are read LEAD products ahead, and between the products
+                    // of 16 keys lie the weights of the next 16 (a pair's exponentials in one place, its rounding and sum in the next).
+                    constexpr int LEAD = NV < 4 ? NV : 4, ALL = KB * 2 * NV, PAIRS = KB * 8;
+                    unsigned lo[NV], hi[NV];
 #pragma unroll
-                    for (int b = 0; b < KB; b++)
-#pragma unroll
-                        for (int e = 0; e < 16; e += 2) {
-                            const unsigned h = pair16<F16>(fast_exp2(fmaf(sc[b][e], unit, -mm)), fast_exp2(fmaf(sc[b][e + 1], unit, -mm)));
+                    for (int n = 0; n < NV; n++) { lo[n] = base_of(vt + v_lo[n]); hi[n] = base_of(vt + v_hi[n]); }
+                    auto value = [&](int i) { const int off = i / NV * 16 * (DV * 2); return lds_transposed(lo[i % NV] + off, hi[i % NV] + off); };
+                    float  e0 = 0.f, e1 = 0.f;
+                    auto power = [&](int i) {                         // pair i: keys 2 i, 2 i + 1 of the lane's
+                        if (i > 0 && i <= PAIRS) {
+                            const unsigned h = packed16<F16>(e0, e1);
                             l = add_pair<F16>(l, h);
-                            pf[b][e >> 3][(e >> 1) & 3] = h;
+                            pf[(i - 1) >> 3][((i - 1) >> 2) & 1][(i - 1) & 3] = h;
                         }
+                        if (i < PAIRS) {
+                            e0 = fast_exp2(fmaf(sc[i >> 3][(2 * i) & 15], unit, -mm));
+                            e1 = fast_exp2(fmaf(sc[i >> 3][(2 * i + 1) & 15], unit, -mm));
+                        }
+                    };
+                    u32x4 vf[LEAD];
 #pragma unroll
-                    for (int b = 0; b < KB; b++)
+                    for (int i = 0; i < LEAD; i++) vf[i] = value(i);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                        for (int kk = 0; kk < 2; kk++)
+                    for (int i = 0; i < 5; i++) power(i);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                            for (int n = 0; n < NV; n++) acc[n] = mfma32<F16>(value(vt, b, kk, n), pf[b][kk], acc[n]);
+                    for (int i = 0; i < ALL; i++) {
+                        acc[i % NV] = mfma32<F16>(vf[i % LEAD], pf[i / NV >> 1][i / NV & 1], acc[i % NV]);
+                        if (i + LEAD < ALL) vf[i % LEAD] = value(i + LEAD);
+                        if (NV <= 4) {
+#pragma unroll
+                            for (int k = 0; k < 4 / (NV < 4 ? NV : 4); k++) power(5 + i * (4 / (NV < 4 ? NV : 4)) + k);
+                        } else if (i % (NV / 4) == 0) power(5 + i / (NV / 4));
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
                 if constexpr (BIAS)
 #pragma unroll
