@@ -84,7 +84,7 @@ void mla::gqa::batch_fill(BatchP & p, const BatchCall & c, const BatchPlan & pl,
     p.q_starts = c.q_starts; p.per = c.n_tok / c.n_seq;
     p.mask = (const char *) c.mask; p.mask_nb1 = c.mask_nb1; p.mask_len = c.mask && c.mask_ne0 < c.cap ? (int) c.mask_ne0 : (int) c.cap;
     p.dst = (char *) c.dst; p.d_nb1 = c.d_nb1; p.d_nb2 = c.d_nb2;
-    p.scale_log2 = fabsf(c.scale) * LOG2E; p.flip = c.scale < 0.f ? 0x80008000u : 0u;
+    p.scale_log2 = fabsf(c.scale) * LOG2E; p.mask_unit = 1.f / fabsf(c.scale); p.flip = c.scale < 0.f ? 0x80008000u : 0u;
     // (a cap so small or large that these leave f32: the largest number does the same)
     p.cap_in  = c.logit_softcap > 0.f ? fminf(fabsf(c.scale) / c.logit_softcap, FLT_MAX) : 0.f;
     p.cap_out = fminf(c.logit_softcap * LOG2E, FLT_MAX);

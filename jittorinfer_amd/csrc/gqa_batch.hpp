@@ -22,6 +22,7 @@ struct BatchP {
     const char * mask; int64_t mask_nb1; int mask_len;             // mask_len: rows past it are out
     char * dst; int64_t d_nb1, d_nb2;
     float scale_log2;             // |scale| * log2(e)
+    float mask_unit;              // 1 / |scale|
     unsigned flip;                // sign bits of a pair of values: Q is negated as it is read where the scale is negative
     float cap_in, cap_out;        // soft cap c: |scale| / c and c * log2(e); cap_out = 0: none
     int causal, window, n_grp, n_tok, n_head, n_head_kv, group;
@@ -62,7 +63,7 @@ void      batch_fill(BatchP & p, const BatchCall & c, const BatchPlan & pl, char
 template <bool F16> hipError_t batch_launch(const BatchP & p, const BatchPlan & pl, int dk, hipStream_t st);
 
 // Workgroups of a shape that a CU holds, by its registers and its tiles in LDS.
-constexpr int batch_wg_per_cu(int dk, Shape s) { return s == FOUR_KEYS ? (dk <= 64 ? 2 : 1) : dk <= 128 ? 2 : 1; }
+constexpr int batch_wg_per_cu(int dk, Shape s) { return s == FOUR_KEYS ? (dk <= 64 ? 2 : 1) : dk <= 128 || (dk == 192 && s == FOUR_ROWS) ? 2 : 1; }
 
 }  // namespace gqa
 }  // namespace mla

@@ -38,11 +38,14 @@ __device__ __forceinline__ uint64_t uni64(uint64_t v) {
 
 // N times 64 lanes, 16 bytes each: from base + off[j] (a lane's own) plus the instruction's offset to LDS at `lds` + 1024 j, lane by lane.  Waited for by dma_wait().
 template <int N> __device__ __forceinline__ void dma_tile(uint64_t base, const unsigned (&off)[N], unsigned lds) {
-    static_assert(N == 2 || N == 4 || N == 6 || N == 8, "");
-    if constexpr (N % 4 == 2)
+    constexpr int AT = N % 4;
+    if constexpr (AT == 1) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %1" : : "s"(lds), "s"(base), "v"(off[0]) : "memory", "m0");
+    if constexpr (AT == 2)
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %1\n\tglobal_load_lds_dwordx4 %3, %1 offset:1024"
                      : : "s"(lds), "s"(base), "v"(off[0]), "v"(off[1]) : "memory", "m0");
-    constexpr int AT = N % 4;
+    if constexpr (AT == 3)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %1\n\tglobal_load_lds_dwordx4 %3, %1 offset:1024\n\tglobal_load_lds_dwordx4 %4, %1 offset:2048"
+                     : : "s"(lds), "s"(base), "v"(off[0]), "v"(off[1]), "v"(off[2]) : "memory", "m0");
 #pragma unroll
     for (int j = AT; j < N; j += 4)
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %1\n\tglobal_load_lds_dwordx4 %3, %1 offset:1024\n\t"
@@ -213,7 +216,10 @@ __device__ __forceinline__ unsigned halves(unsigned bits15) { return (bits15 >> 
 
 template <bool F16> __device__ __forceinline__ u32x2 pack4(float a, float b, float c, float d) { return u32x2{ packed16<F16>(a, b), packed16<F16>(c, d) }; }
 
-template <bool F16, int DK, int DV, int NWQ, int NWK, int TK, int OCC, bool BIAS>
+// What is done to scores besides scaling them: a mask added, or a soft cap and perhaps a mask behind it.
+enum Extra { NOTHING, MASK, CAP };
+
+template <bool F16, int DK, int DV, int NWQ, int NWK, int TK, int OCC, Extra EXTRA>
 __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const BatchP) {
     constexpr int NW = NWQ * NWK, BM = 32 * NWQ, KW = TK / NWK, KB = KW / 32, KC = DK / 16, NV = DV / 32;
     constexpr int KT = TK * DK * 2, VT = TK * DV * 2, KI = KT / 1024 / NW, VI = VT / 1024 / NW;
@@ -347,7 +353,7 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                 b_first = span_of(p, g, at.j * BM / p.group); b_last = span_of(p, g, (int) last_row / p.group);
             }
             const int64_t seq = p.own_lens ? g.q0 : at.g;             // whose pages
-            const char * mask = BIAS && p.mask ? p.mask + (p.own_lens ? (int64_t) (g.q0 + tok) : at.g) * p.mask_nb1 : nullptr;
+            const char * mask = EXTRA != NOTHING && p.mask ? p.mask + (p.own_lens ? (int64_t) (g.q0 + tok) : at.g) * p.mask_nb1 : nullptr;
 
             const int64_t k_off = (int64_t) at.kvh * p.k_head + (p.block_table ? 0 : at.g * p.k_page + g.row0 * p.k_row);
             const int64_t v_off = (int64_t) at.kvh * p.v_head + (p.block_table ? 0 : at.g * p.v_page + g.row0 * p.v_row);
@@ -375,31 +381,32 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                     dma_tile<VI>(vb, v_end, v_to);
                 }
             };
-            // (the mask's numbers of the next tile are requested ahead of its keys: a wait for them is no wait for those)
-            u32x2 mk[KB][4], mk_next[KB][4];
-            auto fetch_mask = [&](int t, u32x2 (&to)[KB][4]) {
-                if constexpr (BIAS)
-                    if (mask)
+            // the mask's numbers of a tile; rows past the last that the lane's query sees: -infinity
+            const bool mask_whole = EXTRA != NOTHING && mask && !uni(__any(((uintptr_t) mask & 7) != 0));
+            u32x2 mk[KB][4];
+            auto fetch_mask = [&](int t) {
+                if constexpr (EXTRA != NOTHING)
+                    if (mask) {
+                        const int  i0 = t * TK + wk * KW + hh * 4;
+                        const bool whole_tile = mask_whole && t * TK + TK <= b_first.last;
 #pragma unroll
                         for (int b = 0; b < KB; b++)
 #pragma unroll
                             for (int c = 0; c < 4; c++) {
-                                const int i = t * TK + wk * KW + b * 32 + c * 8 + hh * 4;
+                                const int i = i0 + b * 32 + c * 8;
                                 const char * src = mask + (int64_t) i * 2;
-                                if (i + 4 <= s.last && ((uintptr_t) src & 7) == 0) to[b][c] = *(const u32x2 *) src;
+                                if (whole_tile) mk[b][c] = *(const u32x2 *) src;
                                 else {
                                     unsigned short h[4];
 #pragma unroll
                                     for (int e = 0; e < 4; e++) h[e] = i + e < s.last ? *(const unsigned short *) (src + 2 * e) : (unsigned short) 0xfc00;
-                                    to[b][c] = u32x2{ h[0] | ((unsigned) h[1] << 16), h[2] | ((unsigned) h[3] << 16) };
+                                    mk[b][c] = u32x2{ h[0] | ((unsigned) h[1] << 16), h[2] | ((unsigned) h[3] << 16) };
                                 }
                             }
+                    }
             };
+            auto masked_by = [&](int b, int e) { return f16_bits_to_f32((mk[b][e >> 2][(e >> 1) & 1] >> (16 * (e & 1))) & 0xffffu); };
 
-            __syncthreads();                                          // (LDS is free of the piece before)
-            fetch_mask(t0, mk);
-            int id = p.block_table ? page_at(t0) : 0, id_next = p.block_table && t0 + 1 < t1 ? page_at(t0 + 1) : 0;
-            fetch(t0, id, 0);
             u32x4 qf[KC];
             {
                 const char * src = p.q + (int64_t) (g.q0 + tok) * p.q_nb2 + (int64_t) head * p.q_nb1 + hh * 16;
@@ -410,23 +417,33 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                     for (int e = 0; e < 4; e++) qf[c][e] ^= p.flip;
                 }
             }
-            float  m = -INFINITY, l = 0.f;
-            unsigned up[(NV + 1) / 2] = {}, down[(NV + 1) / 2] = {};  // results that a +infinity (-infinity, NaN: both) of a tile not seen by all rows belongs to
+            float  m, l;
             f32x16 acc[NV];
-#pragma unroll
-            for (int n = 0; n < NV; n++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) acc[n][e] = 0.f;
+            // Infinities and NaN among keys and values must not count where a row does not see them, and 0 * them does.  The piece is worked on as if there were none; if a result
+            // is not finite, once more from the start, `safe`: with the infinities and NaN among the values of every tile that not all rows see whole noted for the rows that
+            // see them, and taken for zeros, and with masked scores set and not added to.
+            unsigned up[(NV + 1) / 2], down[(NV + 1) / 2];            // safe: results that a +infinity (-infinity, NaN: both) belongs to
+            bool safe = false;
 
-            // S^T of the wave's keys
+            // S^T of the wave's keys; a mask is where the sums begin (in units of the products)
             auto products = [&](unsigned kt, f32x16 (&sc)[KB]) {
                 unsigned at[KC];
 #pragma unroll
                 for (int c = 0; c < KC; c++) at[c] = base_of(kt + k_lo[c]);
+                f32x16 start[KB];
+#pragma unroll
+                for (int b = 0; b < KB; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) start[b][e] = 0.f;
+                if constexpr (EXTRA == MASK)
+                    if (!safe)
+#pragma unroll
+                        for (int b = 0; b < KB; b++)
+#pragma unroll
+                            for (int e = 0; e < 16; e++) start[b][e] = masked_by(b, e) * p.mask_unit;
 #pragma unroll
                 for (int b = 0; b < KB; b++) {
-#pragma unroll
-                    for (int e = 0; e < 16; e++) sc[b][e] = 0.f;
+                    sc[b] = start[b];
 #pragma unroll
                     for (int c = 0; c < KC; c++) sc[b] = mfma32<F16>(lds128(at[c] + b * 32 * (DK * 2)), qf[c], sc[b]);
                 }
@@ -441,20 +458,30 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                 __builtin_amdgcn_sched_group_barrier(0x008, LEAD, 0);
             };
 
+            for (;;) {
+                m = -INFINITY; l = 0.f;
+#pragma unroll
+                for (int n = 0; n < NV; n++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) acc[n][e] = 0.f;
+#pragma unroll
+                for (int n = 0; n < (NV + 1) / 2; n++) up[n] = down[n] = 0;
+            __syncthreads();                                          // (LDS is free of what was before)
+            fetch_mask(t0);
+            int id = paged ? page_at(t0) : 0, id_next = paged && t0 + 1 < t1 ? page_at(t0 + 1) : 0;
+            fetch(t0, id, 0);
             for (int t = t0; t < t1; t++) {
                 dma_wait();
                 __syncthreads();
                 const int  buf = (t - t0) & 1, key0 = t * TK + wk * KW;
-                const bool use = !p.block_table || good(id);
+                const bool use = !paged || good(id);
                 if (t + 1 < t1) {
-                    fetch_mask(t + 1, mk_next);
                     id = id_next;
                     fetch(t + 1, id, buf ^ 1);
-                    if (p.block_table && t + 2 < t1) id_next = page_at(t + 2);
+                    if (paged && t + 2 < t1) id_next = page_at(t + 2);
                 }
                 const unsigned kt = uni(lds0 + buf * (KT + VT) + wk * KW * (DK * 2)), vt = uni(lds0 + buf * (KT + VT) + KT + wk * KW * (DV * 2));
-                // ---- a tile that not all rows of the block see whole: infinities and NaN among its values are noted for the rows that see them, and become zeros
-                if ((BIAS && mask) || t * TK < b_last.first || t * TK + TK > b_first.last) {
+                if (safe && ((EXTRA != NOTHING && p.mask) || t * TK < b_last.first || t * TK + TK > b_first.last)) {
                     unsigned bad = 0;
                     const unsigned mine = lds0 + buf * (KT + VT) + KT + threadIdx.x * 16;
 #pragma unroll
@@ -473,7 +500,7 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                         for (int i = 0; i < KW; i++) {
                             const int key = key0 + i;
                             bool sees = use && key >= s.first && key < s.last;
-                            if constexpr (BIAS) if (mask && sees) sees = *(const unsigned short *) (mask + (int64_t) key * 2) != 0xfc00;
+                            if constexpr (EXTRA != NOTHING) if (mask && sees) sees = *(const unsigned short *) (mask + (int64_t) key * 2) != 0xfc00;
 #pragma unroll
                             for (int n = 0; n < NV; n++)
 #pragma unroll
@@ -504,7 +531,8 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                     u32x4  pf[KB][2];
                     products(kt, sc);
                     float top, unit = p.scale_log2;                   // what makes log2 units of sc
-                    if (!BIAS && key0 + KW <= s_first.last && key0 >= s_last.first) {
+                    const bool all = key0 + KW <= s_first.last && key0 >= s_last.first;
+                    if (EXTRA != CAP && all && !(EXTRA == MASK && safe)) {
                         top = sc[0][0];
 #pragma unroll
                         for (int b = 0; b < KB; b++)
@@ -512,29 +540,25 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                             for (int e = 0; e < 16; e++) top = fmaxf(top, sc[b][e]);
                         top *= unit;
                     } else {
-                        const bool all = key0 + KW <= s_first.last && key0 >= s_last.first;
                         top = -INFINITY;
+                        const int from = s.first - key0 - hh * 4, to = s.last - key0 - hh * 4;
 #pragma unroll
                         for (int b = 0; b < KB; b++)
 #pragma unroll
                             for (int e = 0; e < 16; e++) {
-                                float v = sc[b][e];
-                                if constexpr (BIAS) {
-                                    v = scaled_score(p.scale_log2, p.cap_in, p.cap_out, v);
-                                    if (mask) {
-                                        const float f = f16_bits_to_f32((mk[b][e >> 2][(e >> 1) & 1] >> (16 * (e & 1))) & 0xffffu);
-                                        v = f == -INFINITY ? -INFINITY : fmaf(f, LOG2E, v);
-                                    }
-                                } else v *= p.scale_log2;
-                                if (!all) {
-                                    const int i = key0 + b * 32 + (e >> 2) * 8 + hh * 4 + (e & 3);
-                                    if (i < s.first || i >= s.last) v = -INFINITY;
+                                float v = EXTRA == CAP ? scaled_score(p.scale_log2, p.cap_in, p.cap_out, sc[b][e]) : sc[b][e] * p.scale_log2;
+                                if (EXTRA == CAP ? mask != nullptr : EXTRA == MASK && safe) {
+                                    const float f = masked_by(b, e);
+                                    v = f == -INFINITY ? -INFINITY : fmaf(f, LOG2E, v);
                                 }
+                                const int i = b * 32 + (e >> 2) * 8 + (e & 3);
+                                if (!all && (i < from || i >= to)) v = -INFINITY;
                                 sc[b][e] = v;
                                 top = fmaxf(top, v);
                             }
                         unit = 1.f;
                     }
+                    if (EXTRA != NOTHING && t + 1 < t1) fetch_mask(t + 1);
                     if (__any(top > m + (REF + SLACK))) {             // the reference moves
                         top = fmaxf(top, xor32(top));
                         const float nm = fmaxf(top - REF, m);
@@ -584,11 +608,22 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
-                if constexpr (BIAS)
+                else if (EXTRA != NOTHING && t + 1 < t1) fetch_mask(t + 1);
+            }
+                if (safe) break;
+                float odd = l * 0.f;                                  // NaN if anything is not finite
 #pragma unroll
-                    for (int b = 0; b < KB; b++)
+                for (int n = 0; n < NV; n++)
 #pragma unroll
-                        for (int c = 0; c < 4; c++) mk[b][c] = mk_next[b][c];
+                    for (int e = 0; e < 16; e++) odd = fmaf(acc[n][e], 0.f, odd);
+                const int found = __any(!(odd == 0.f));
+                if (lane == 0) sh_bad[0][wave] = found;
+                __syncthreads();
+                int any = 0;
+#pragma unroll
+                for (int w = 0; w < NW; w++) any |= sh_bad[0][w];
+                if (!uni(any)) break;
+                safe = true;
             }
             bool noted = false;
 #pragma unroll
@@ -748,39 +783,42 @@ __global__ void __launch_bounds__(256) gqa_batch_join_kernel(const BatchP p) {
 
 // ---------------------------------------------------------------- host
 
-template <bool F16, int DK, int DV, int NWQ, int NWK, int TK, int OCC, bool BIAS>
+template <bool F16, int DK, int DV, int NWQ, int NWK, int TK, int OCC, Extra EXTRA>
 hipError_t launch_batch(const BatchP & p, const BatchPlan & pl, hipStream_t st) {
     constexpr int lds = 2 * TK * (DK + DV) * 2;
     static_assert(lds + NWQ * NWK * 32 * 8 <= 160 * 1024, "LDS");
     static std::atomic<uint64_t> granted{ 0 };
-    hipError_t e = grant_lds(gqa_batch_kernel<F16, DK, DV, NWQ, NWK, TK, OCC, BIAS>, lds, granted);
+    hipError_t e = grant_lds(gqa_batch_kernel<F16, DK, DV, NWQ, NWK, TK, OCC, EXTRA>, lds, granted);
     if (e != hipSuccess) return e;
     const int64_t grid = p.deal == RUNS ? p.n_wg : (int64_t) p.blocks * p.n_head_kv;
-    hipLaunchKernelGGL((gqa_batch_kernel<F16, DK, DV, NWQ, NWK, TK, OCC, BIAS>), dim3((unsigned) (grid > p.n_wg ? grid : p.n_wg)), dim3(64 * NWQ * NWK), lds, st, p);
+    hipLaunchKernelGGL((gqa_batch_kernel<F16, DK, DV, NWQ, NWK, TK, OCC, EXTRA>), dim3((unsigned) (grid > p.n_wg ? grid : p.n_wg)), dim3(64 * NWQ * NWK), lds, st, p);
     if ((e = hipGetLastError()) != hipSuccess || p.own_lens || p.deal == WHOLE) return e;
     hipLaunchKernelGGL((gqa_batch_join_kernel<F16, DV, NWQ>), dim3((unsigned) p.n_wg, DV / 32), dim3(256), 0, st, p);
     return hipGetLastError();
 }
-template <bool F16, int DK, int DV, bool BIAS>
+// (heads of 192: tiles of 32 keys, so that two workgroups' lie in a CU's LDS)
+template <bool F16, int DK, int DV, Extra EXTRA>
 hipError_t launch_shape(const BatchP & p, const BatchPlan & pl, hipStream_t st) {
-    if constexpr (DK <= 128) if (pl.shape == FOUR_KEYS) return launch_batch<F16, DK, DV, 1, 4, 128, batch_wg_per_cu(DK, FOUR_KEYS), BIAS>(p, pl, st);
-    if (pl.shape == FOUR_ROWS) return launch_batch<F16, DK, DV, 4, 1, 64, batch_wg_per_cu(DK, FOUR_ROWS), BIAS>(p, pl, st);
-    return launch_batch<F16, DK, DV, 2, 2, 64, batch_wg_per_cu(DK, TWO_TWO), BIAS>(p, pl, st);
+    if constexpr (DK <= 128) if (pl.shape == FOUR_KEYS) return launch_batch<F16, DK, DV, 1, 4, 128, batch_wg_per_cu(DK, FOUR_KEYS), EXTRA>(p, pl, st);
+    if (pl.shape == FOUR_ROWS) return launch_batch<F16, DK, DV, 4, 1, DK == 192 ? 32 : 64, batch_wg_per_cu(DK, FOUR_ROWS), EXTRA>(p, pl, st);
+    return launch_batch<F16, DK, DV, 2, 2, 64, batch_wg_per_cu(DK, TWO_TWO), EXTRA>(p, pl, st);
 }
-template <bool F16, bool BIAS>
+template <bool F16, Extra EXTRA>
 hipError_t launch_widths(const BatchP & p, const BatchPlan & pl, int dk, hipStream_t st) {
     switch (dk) {
-        case 64:  return launch_shape<F16, 64, 64, BIAS>(p, pl, st);
-        case 128: return launch_shape<F16, 128, 128, BIAS>(p, pl, st);
-        case 192: return launch_shape<F16, 192, 128, BIAS>(p, pl, st);
-        default:  return launch_shape<F16, 256, 256, BIAS>(p, pl, st);
+        case 64:  return launch_shape<F16, 64, 64, EXTRA>(p, pl, st);
+        case 128: return launch_shape<F16, 128, 128, EXTRA>(p, pl, st);
+        case 192: return launch_shape<F16, 192, 128, EXTRA>(p, pl, st);
+        default:  return launch_shape<F16, 256, 256, EXTRA>(p, pl, st);
     }
 }
 
 }  // namespace
 
 template <bool F16> hipError_t batch_launch(const BatchP & p, const BatchPlan & pl, int dk, hipStream_t st) {
-    return p.mask || p.cap_out != 0.f ? launch_widths<F16, true>(p, pl, dk, st) : launch_widths<F16, false>(p, pl, dk, st);
+    // (the mask in units of the products needs a scale that it can be divided by)
+    if (p.cap_out != 0.f || (p.mask && !(p.scale_log2 > 1e-30f))) return launch_widths<F16, CAP>(p, pl, dk, st);
+    return p.mask ? launch_widths<F16, MASK>(p, pl, dk, st) : launch_widths<F16, NOTHING>(p, pl, dk, st);
 }
 
 }  // namespace gqa
