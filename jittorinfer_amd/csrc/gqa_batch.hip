@@ -26,7 +26,7 @@ BatchPlan mla::gqa::batch_plan(const BatchCall & c, bool whole_blocks) {
     pl.bm     = pl.shape == FOUR_KEYS ? 32 : pl.shape == TWO_TWO ? 64 : 128;
     const int64_t blocks = (int64_t) c.n_tok * group / pl.bm + c.n_seq;
     pl.blocks = blocks < INT_MAX ? (int) blocks : INT_MAX;
-    const int64_t tiles = (c.cap + 63) / 64 < INT_MAX ? (c.cap + 63) / 64 : INT_MAX, fill = 256 * batch_wg_per_cu(c.dk, pl.shape);
+    const int64_t tiles = (c.cap + 63) / 64 < INT_MAX ? (c.cap + 63) / 64 : INT_MAX, fill = 256 * batch_wg_per_cu(c.dk, pl.shape, !c.mask && c.logit_softcap == 0.f);
     const int64_t most = c.n_workgroups > 0 ? c.n_workgroups : fill, have = tiles > most ? most : tiles * pl.blocks > most ? most : tiles * pl.blocks * c.n_head_kv;
     pl.n_wg = (int) (have < 1 ? 1 : have < most ? have : most);
     size_t at = 0;

@@ -303,15 +303,16 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
     }
     // transposing reads: row, 16-byte chunk and half of it; the addresses of a chunk of 32 columns, for rows 0 .. 3 and 8 .. 11 of 16
     const int vq = hh * 4 + ((lane >> 2) & 3), vc = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), vsub = (lane & 1) * 8;
-    unsigned v_lo[NV], v_hi[NV];
+    // (chunks beyond those that the swizzle moves among are whole steps further on)
+    constexpr int VP = DV % 128 == 0 ? 4 : 2, KP = DK % 128 == 0 ? 8 : 4;
+    unsigned v_lo[VP], v_hi[VP], k_lo[KP];
 #pragma unroll
-    for (int n = 0; n < NV; n++) {
+    for (int n = 0; n < VP; n++) {
         v_lo[n] = vq * (DV * 2) + (((n * 4 + vc) ^ swizzle<DV>(vq)) * 16) + vsub;
         v_hi[n] = (vq + 8) * (DV * 2) + (((n * 4 + vc) ^ swizzle<DV>(vq + 8)) * 16) + vsub;
     }
-    unsigned k_lo[KC];
 #pragma unroll
-    for (int c = 0; c < KC; c++) k_lo[c] = l31 * (DK * 2) + (((2 * c + hh) ^ swizzle<DK>(l31)) * 16);
+    for (int c = 0; c < KP; c++) k_lo[c] = l31 * (DK * 2) + (((2 * c + hh) ^ swizzle<DK>(l31)) * 16);
 
     end = Pos{ uni(end.g), uni(end.kvh), uni(end.j), uni(end.tile) };
     single = uni(single);
@@ -362,7 +363,8 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
             const int64_t n_pages = p.n_pages, k_page = p.block_table ? p.k_page : 0, v_page = p.block_table ? p.v_page : 0;
             const bool paged = p.block_table != nullptr;
             auto good = [&](int id) { return id >= 0 && id < n_pages; };
-            auto page_at = [&](int t) { return uni(pages[t * TK / PAGE]); };
+            // (through the scalar cache, nothing writes them meanwhile: a vector load would be waited for together with the tiles that are under way)
+            auto page_at = [&](int t) { return *(const int32_t __attribute__((address_space(4))) *) (uintptr_t) (pages + t * TK / PAGE); };
             auto fetch = [&](int t, int id, int buf) {                // tile t to LDS
                 const int key0 = t * TK, row = paged ? key0 % PAGE : key0, pg = good(id) ? id : 0;    // (a bad id: page 0 is read, not used)
                 const uint64_t kb = uni64(k_base + (uint64_t) (pg * k_page + (int64_t) row * k_row)) - 4096, vb = uni64(v_base + (uint64_t) (pg * v_page + (int64_t) row * v_row)) - 4096;
@@ -427,9 +429,9 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
 
             // S^T of the wave's keys; a mask is where the sums begin (in units of the products)
             auto products = [&](unsigned kt, f32x16 (&sc)[KB]) {
-                unsigned at[KC];
+                unsigned at[KP];
 #pragma unroll
-                for (int c = 0; c < KC; c++) at[c] = base_of(kt + k_lo[c]);
+                for (int c = 0; c < KP; c++) at[c] = base_of(kt + k_lo[c]);
                 f32x16 start[KB];
 #pragma unroll
                 for (int b = 0; b < KB; b++)
@@ -445,7 +447,7 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                 for (int b = 0; b < KB; b++) {
                     sc[b] = start[b];
 #pragma unroll
-                    for (int c = 0; c < KC; c++) sc[b] = mfma32<F16>(lds128(at[c] + b * 32 * (DK * 2)), qf[c], sc[b]);
+                    for (int c = 0; c < KC; c++) sc[b] = mfma32<F16>(lds128(at[c % KP] + c / KP * KP * 32 + b * 32 * (DK * 2)), qf[c], sc[b]);
                 }
                 // the order of it: reads some ahead of the products
                 constexpr int LEAD = KC < 8 ? KC : 8;
@@ -497,23 +499,26 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                     for (int w = 0; w < NW; w++) any |= sh_bad[buf][w];
                     if (uni(any)) {
 #pragma unroll 1
-                        for (int i = 0; i < KW; i++) {
-                            const int key = key0 + i;
-                            bool sees = use && key >= s.first && key < s.last;
-                            if constexpr (EXTRA != NOTHING) if (mask && sees) sees = *(const unsigned short *) (mask + (int64_t) key * 2) != 0xfc00;
-#pragma unroll
-                            for (int n = 0; n < NV; n++)
+                        for (int n = 0; n < NV; n++) {
+                            unsigned u = 0, d = 0;
+#pragma unroll 1
+                            for (int i = 0; i < KW; i++) {
+                                const int key = key0 + i;
+                                bool sees = use && key >= s.first && key < s.last;
+                                if constexpr (EXTRA != NOTHING) if (mask && sees) sees = *(const unsigned short *) (mask + (int64_t) key * 2) != 0xfc00;
 #pragma unroll
                                 for (int c = 0; c < 4; c++) {
                                     const u32x2 x = *(LDS_PTR(const u32x2)) (uintptr_t) (vt + i * (DV * 2) + (((n * 4 + c) ^ swizzle<DV>(i)) * 16) + hh * 8);
 #pragma unroll
                                     for (int e = 0; e < 4; e++) {
-                                        const float    f   = from16<F16>((unsigned short) (x[e >> 1] >> (16 * (e & 1))));
-                                        const unsigned bit = 1u << ((n & 1) * 16 + 4 * c + e);
-                                        if (sees && !(f < INFINITY)) up[n / 2] |= bit;                          // infinity or NaN
-                                        if (sees && !(f > -INFINITY)) down[n / 2] |= bit;
+                                        const float f = from16<F16>((unsigned short) (x[e >> 1] >> (16 * (e & 1))));
+                                        if (sees && !(f < INFINITY)) u |= 1u << (4 * c + e);                    // infinity or NaN
+                                        if (sees && !(f > -INFINITY)) d |= 1u << (4 * c + e);
                                     }
                                 }
+                            }
+#pragma unroll
+                            for (int k = 0; k < (NV + 1) / 2; k++) if (k == n / 2) { up[k] |= u << (n & 1) * 16; down[k] |= d << (n & 1) * 16; }
                         }
                         __syncthreads();
 #pragma unroll
@@ -541,12 +546,27 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                         top *= unit;
                     } else {
                         top = -INFINITY;
+                        // a soft cap far above the scores of this tile: tanh(y) / y by its series to y^10, off by 2^-31 where |y| < 1/4
+                        bool small = false;
+                        if constexpr (EXTRA == CAP) {
+                            float most = 0.f;
+#pragma unroll
+                            for (int b = 0; b < KB; b++)
+#pragma unroll
+                                for (int e = 0; e < 16; e++) most = fmaxf(most, fabsf(sc[b][e]));
+                            small = !uni(__any(!(most * p.cap_in < 0.25f)));
+                        }
+                        auto capped = [&](float a) {
+                            if (!small) return scaled_score(p.scale_log2, p.cap_in, p.cap_out, a);
+                            const float y = p.cap_in * a, u = y * y;
+                            return p.scale_log2 * a * fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, -1382.f / 155925, 62.f / 2835), -17.f / 315), 2.f / 15), -1.f / 3), 1.f);
+                        };
                         const int from = s.first - key0 - hh * 4, to = s.last - key0 - hh * 4;
 #pragma unroll
                         for (int b = 0; b < KB; b++)
 #pragma unroll
                             for (int e = 0; e < 16; e++) {
-                                float v = EXTRA == CAP ? scaled_score(p.scale_log2, p.cap_in, p.cap_out, sc[b][e]) : sc[b][e] * p.scale_log2;
+                                float v = EXTRA == CAP ? capped(sc[b][e]) : sc[b][e] * p.scale_log2;
                                 if (EXTRA == CAP ? mask != nullptr : EXTRA == MASK && safe) {
                                     const float f = masked_by(b, e);
                                     v = f == -INFINITY ? -INFINITY : fmaf(f, LOG2E, v);
@@ -574,10 +594,10 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                     // O^T += V^T P^T, 32 columns and 16 keys a product, in the order as it stands here: values are read LEAD products ahead, and between the products
                     // of 16 keys lie the weights of the next 16 (a pair's exponentials in one place, its rounding and sum in the next).
                     constexpr int LEAD = NV < 4 ? NV : 4, ALL = KB * 2 * NV, PAIRS = KB * 8;
-                    unsigned lo[NV], hi[NV];
+                    unsigned lo[VP], hi[VP];
 #pragma unroll
-                    for (int n = 0; n < NV; n++) { lo[n] = base_of(vt + v_lo[n]); hi[n] = base_of(vt + v_hi[n]); }
-                    auto value = [&](int i) { const int off = i / NV * 16 * (DV * 2); return lds_transposed(lo[i % NV] + off, hi[i % NV] + off); };
+                    for (int n = 0; n < VP; n++) { lo[n] = base_of(vt + v_lo[n]); hi[n] = base_of(vt + v_hi[n]); }
+                    auto value = [&](int i) { const int off = i / NV * 16 * (DV * 2) + i % NV / VP * VP * 64; return lds_transposed(lo[i % VP] + off, hi[i % VP] + off); };
                     float  e0 = 0.f, e1 = 0.f;
                     auto power = [&](int i) {                         // pair i: keys 2 i, 2 i + 1 of the lane's
                         if (i > 0 && i <= PAIRS) {
@@ -796,12 +816,12 @@ hipError_t launch_batch(const BatchP & p, const BatchPlan & pl, hipStream_t st) 
     hipLaunchKernelGGL((gqa_batch_join_kernel<F16, DV, NWQ>), dim3((unsigned) p.n_wg, DV / 32), dim3(256), 0, st, p);
     return hipGetLastError();
 }
-// (heads of 192: tiles of 32 keys, so that two workgroups' lie in a CU's LDS)
+// (heads of 192: tiles of 32 keys, so that two workgroups' lie in a CU's LDS; of 256: so that a wave's scores leave room in its registers)
 template <bool F16, int DK, int DV, Extra EXTRA>
 hipError_t launch_shape(const BatchP & p, const BatchPlan & pl, hipStream_t st) {
-    if constexpr (DK <= 128) if (pl.shape == FOUR_KEYS) return launch_batch<F16, DK, DV, 1, 4, 128, batch_wg_per_cu(DK, FOUR_KEYS), EXTRA>(p, pl, st);
-    if (pl.shape == FOUR_ROWS) return launch_batch<F16, DK, DV, 4, 1, DK == 192 ? 32 : 64, batch_wg_per_cu(DK, FOUR_ROWS), EXTRA>(p, pl, st);
-    return launch_batch<F16, DK, DV, 2, 2, 64, batch_wg_per_cu(DK, TWO_TWO), EXTRA>(p, pl, st);
+    if constexpr (DK <= 128) if (pl.shape == FOUR_KEYS) return launch_batch<F16, DK, DV, 1, 4, 128, batch_wg_per_cu(DK, FOUR_KEYS, EXTRA == NOTHING), EXTRA>(p, pl, st);
+    if (pl.shape == FOUR_ROWS) return launch_batch<F16, DK, DV, 4, 1, DK >= 192 ? 32 : 64, batch_wg_per_cu(DK, FOUR_ROWS, EXTRA == NOTHING), EXTRA>(p, pl, st);
+    return launch_batch<F16, DK, DV, 2, 2, 64, batch_wg_per_cu(DK, TWO_TWO, EXTRA == NOTHING), EXTRA>(p, pl, st);
 }
 template <bool F16, Extra EXTRA>
 hipError_t launch_widths(const BatchP & p, const BatchPlan & pl, int dk, hipStream_t st) {
