@@ -26,6 +26,7 @@ struct BatchP {
     unsigned flip;                // sign bits of a pair of values: Q is negated as it is read where the scale is negative
     float cap_in, cap_out;        // soft cap c: |scale| / c and c * log2(e); cap_out = 0: none
     int causal, window, n_grp, n_tok, n_head, n_head_kv, group;
+    double per_head;              // 1 / group
     int cap;                      // rows a group can have
     int n_wg, min_tiles;          // workgroups, and the fewest tiles that are worth one
     float *  part_o;              // [2 * n_wg][BM * dv]: unnormalized sums of the pieces of blocks that several workgroups share, in the lanes' order;

@@ -82,57 +82,64 @@ __device__ __forceinline__ Span span_of(Params & p, const Group & g, int j) {
     return Span{ p.window > 0 ? max(end - p.window, 0) : 0, min(end, p.mask_len) };
 }
 template <int BM> __device__ __forceinline__ int blocks_of(Params & p, const Group & g) { return (int) (((int64_t) g.nq * p.group + BM - 1) / BM); }
+// Row / heads of a KV head's group (the quotient is off by 2^-52 of itself, and half a step from the next number).
+__device__ __forceinline__ int token_of(Params & p, int row) { return (int) (((double) row + 0.5) * p.per_head); }
 // The tiles that some row of block j sees: [first, last).
 template <int BM, int TK> __device__ __forceinline__ Span tiles_of(Params & p, const Group & g, int j) {
-    const int64_t rows = (int64_t) g.nq * p.group, r0 = (int64_t) j * BM;
     if (p.own_lens) return Span{ 0, (min(g.len, p.mask_len) + TK - 1) / TK };     // (some sequence's whole prefix)
-    const int lo = span_of(p, g, (int) (r0 / p.group)).first, hi = span_of(p, g, (int) ((r0 + BM < rows ? r0 + BM : rows) - 1) / p.group).last;
+    const int64_t rows = (int64_t) g.nq * p.group, r0 = (int64_t) j * BM;
+    const int lo = p.window > 0 ? span_of(p, g, token_of(p, (int) r0)).first : 0, hi = span_of(p, g, p.causal ? token_of(p, (int) ((r0 + BM < rows ? r0 + BM : rows) - 1)) : 0).last;
     return hi > lo ? Span{ lo / TK, (hi + TK - 1) / TK } : Span{ 0, 0 };
 }
 
-// ---- the deal
+// ---- the deal, in 64-bit floating point (whole numbers below 2^53), the same in all workgroups
 // sum over i < n of a + i s, each held to [0, top]
-__device__ __forceinline__ int64_t sum_clamped(int64_t a, int s, int64_t top, int64_t n) {
-    const int64_t i0 = a >= 0 ? 0 : min(n, (-a + s - 1) / s), i1 = a >= top ? 0 : min(n, (top - a + s - 1) / s), mid = i1 - i0;
-    return mid * a + s * ((i0 + i1 - 1) * mid / 2) + (n - i1) * top;
+__device__ __forceinline__ double sum_clamped(double a, double s, double per_s, double top, double n) {
+    const double i0 = fmin(n, fmax(0., ceil(-a * per_s))), i1 = fmin(n, fmax(0., ceil((top - a) * per_s))), mid = i1 - i0;
+    return mid * a + s * ((i0 + i1 - 1.) * mid * 0.5) + (n - i1) * top;
 }
 // Weight of blocks 0 .. n - 1 of a group: the keys each sees, times the heads of the KV head's group, and 128 keys for what a block costs by itself.
-template <int BM> __device__ __forceinline__ int64_t weight_before(Params & p, const Group & g, int64_t n) {
-    const int64_t G = p.group, all = G * g.len;
-    int64_t keys;
+template <int BM> __device__ __forceinline__ double weight_before(Params & p, const Group & g, double n) {
+    const double G = p.group, all = G * g.len, base = G * (g.len - g.nq);
+    double keys;
     if (p.causal) {
-        keys = sum_clamped(G * (g.len - g.nq) + BM, BM, all, n);
-        if (p.window > 0) keys -= sum_clamped(G * (g.len - g.nq + 1 - (int64_t) p.window), BM, all, n);
-    } else keys = n * (p.window > 0 ? min(all, G * p.window) : all);
-    return keys + n * G * 128;
-}
-__device__ __forceinline__ int64_t scan64(int64_t v, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) { const int64_t o = __shfl_up(v, d, 64); if (lane >= d) v += o; }
-    return v;
+        keys = sum_clamped(base + BM, BM, 1. / BM, all, n);
+        if (p.window > 0) keys -= sum_clamped(base + G * (1. - p.window), BM, 1. / BM, all, n);
+    } else keys = n * (p.window > 0 ? fmin(all, G * p.window) : all);
+    return keys + n * G * 128.;
 }
 struct Pos { int g, kvh, j, tile; };             // tile: counted from the block's first
 __device__ __forceinline__ bool same_item(const Pos & a, const Pos & b) { return a.g == b.g && a.kvh == b.kvh && a.j == b.j; }
-// Every wave works it out for itself, a group a lane; quotients are taken in 64-bit floating point, the same in all workgroups.
+// Every wave works it out for itself, a group a lane.
 template <int BM, int TK> struct Deal {
     Params & p;
     const int lane;
-    Group   g;                                   // this lane's
-    int64_t w;                                   // its weight, over all KV heads
+    Group  g;                                    // this lane's
+    double w, incl;                              // its weight over all KV heads, and with those of the groups before it in these 64
+    // the last block that place() found: weights before it and its own, its tiles
+    double before, mine;
+    int    nt;
     __device__ __forceinline__ void fetch(int g0) {
-        w = 0;
-        if (g0 + lane >= p.n_grp) return;
-        g = group_of(p, g0 + lane);
-        w = weight_before<BM>(p, g, blocks_of<BM>(p, g)) * p.n_head_kv;
+        w = 0.;
+        g = Group{ 0, 0, 0, 0 };
+        if (g0 + lane < p.n_grp) {
+            g = group_of(p, g0 + lane);
+            w = weight_before<BM>(p, g, blocks_of<BM>(p, g)) * p.n_head_kv;
+        }
+        incl = w;
+        if (p.n_grp > 1)
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) { const double o = __shfl_up(incl, d, 64); if (lane >= d) incl += o; }
     }
     // the weight of all blocks, and of the heaviest (the last of a group, at most)
-    __device__ __forceinline__ int64_t total(float & most) {
-        int64_t all = 0;
+    __device__ __forceinline__ double total(float & most) {
+        double all = 0.;
         most = 0.f;
         for (int g0 = 0; g0 < p.n_grp; g0 += 64) {
             fetch(g0);
-            all += __shfl(scan64(w, lane), 63, 64);
-            const int nb = w ? blocks_of<BM>(p, g) : 0;
+            all += __shfl(incl, p.n_grp > 1 ? 63 : 0, 64);
+            if (p.deal != EITHER) continue;
+            const int nb = w > 0. ? blocks_of<BM>(p, g) : 0;
             float last = nb ? (float) (weight_before<BM>(p, g, nb) - weight_before<BM>(p, g, nb - 1)) : 0.f;
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) last = fmaxf(last, __shfl_xor(last, d, 64));
@@ -140,34 +147,36 @@ template <int BM, int TK> struct Deal {
         }
         return all;
     }
-    __device__ __forceinline__ Pos place(int64_t at) {           // after total()
-        int64_t before = 0;
+    __device__ __forceinline__ int tile_at(double at) const { return uni(max(min((int) ((at - before) * nt / mine), nt - 1), 0)); }
+    __device__ __forceinline__ Pos place(double at) {            // after total()
+        double ahead = 0.;
         for (int g0 = 0; g0 < p.n_grp; g0 += 64) {
             if (p.n_grp > 64) fetch(g0);
-            const int64_t  incl = scan64(w, lane) + before;
-            const uint64_t past = __ballot(at < incl);
+            const uint64_t past = __ballot(at < ahead + incl);
             if (past) {
-                const int l = uni(__ffsll((unsigned long long) past) - 1);
+                const int l = p.n_grp > 1 ? uni(__ffsll((unsigned long long) past) - 1) : 0;
                 const Group o{ __builtin_amdgcn_readlane(g.q0, l), __builtin_amdgcn_readlane(g.nq, l), __builtin_amdgcn_readlane(g.len, l), 0 };
-                const int     nb = blocks_of<BM>(p, o);
-                const int64_t per = weight_before<BM>(p, o, nb);
-                int64_t rest = at - __shfl(incl - w, l, 64);
-                const int kvh = min((int) ((double) rest / (double) per), p.n_head_kv - 1);
-                rest -= kvh * per;
-                int lo = 0, hi = nb;                              // weight_before(lo) <= rest < weight_before(hi)
-                if (!p.causal) lo = max(min((int) ((double) rest / (double) weight_before<BM>(p, o, 1)), nb - 1), 0);
+                const int    nb = blocks_of<BM>(p, o);
+                const double per = weight_before<BM>(p, o, nb);
+                before = ahead + __shfl(incl - w, l, 64);
+                const int kvh = min((int) ((at - before) / per), p.n_head_kv - 1);
+                before += kvh * per;
+                int lo = 0, hi = nb;                              // weight_before(lo) <= at - before < weight_before(hi)
+                if (!p.causal) lo = max(min((int) ((at - before) / weight_before<BM>(p, o, 1.)), nb - 1), 0);
                 else
                     while (hi - lo > 1) {
                         const int mid = (lo + hi) / 2;
-                        if (weight_before<BM>(p, o, mid) <= rest) lo = mid;
+                        if (weight_before<BM>(p, o, mid) <= at - before) lo = mid;
                         else hi = mid;
                     }
-                const int64_t w0 = weight_before<BM>(p, o, lo), mine = weight_before<BM>(p, o, lo + 1) - w0;
-                const Span    t = tiles_of<BM, TK>(p, o, lo);
-                const int     nt = t.last - t.first;
-                return Pos{ uni(g0 + l), uni(kvh), uni(lo), uni(max(min((int) ((double) (rest - w0) * nt / (double) mine), nt - 1), 0)) };
+                const double w0 = weight_before<BM>(p, o, lo);
+                mine = weight_before<BM>(p, o, lo + 1.) - w0;
+                before += w0;
+                const Span t = tiles_of<BM, TK>(p, o, lo);
+                nt = t.last - t.first;
+                return Pos{ uni(g0 + l), uni(kvh), uni(lo), tile_at(at) };
             }
-            before = __shfl(incl, 63, 64);
+            ahead += __shfl(incl, p.n_grp > 1 ? 63 : 0, 64);
         }
         return Pos{ p.n_grp, 0, 0, 0 };
     }
@@ -255,11 +264,10 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
     single = p.deal == WHOLE;
     if (!single) {
         float         most;
-        const int64_t total = deal.total(most);
+        const double  total = deal.total(most);
         single = p.deal == EITHER && most * p.n_wg <= WHOLE_SHARE * (float) total;
         if (!single) {
-            const int64_t least = (int64_t) p.min_tiles * TK * p.group;
-            const int     runs = (int) max((int64_t) (total > 0), min((int64_t) p.n_wg, total / least));
+            const int runs = (int) fmax(total > 0. ? 1. : 0., fmin((double) p.n_wg, total / ((double) p.min_tiles * TK * p.group)));
             if ((int) blockIdx.x >= runs) {
                 if ((int) blockIdx.x < p.n_wg && threadIdx.x == 0) p.tasks[blockIdx.x] = make_int4(-1, 0, 0, 0);
                 return;
@@ -269,10 +277,11 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
             run = uni(x * (runs >> 3) + min(x, runs & 7) + (int) (blockIdx.x >> 3));
             // (the block that begins in this run and goes on in others is joined by the workgroup of this number: set where it is left)
             if (threadIdx.x == 0) p.tasks[run] = make_int4(-1, 0, 0, 0);
-            auto mark = [&](int r) { return (int64_t) ((double) total * r / runs); };
+            auto mark = [&](int r) { return floor(total * r / runs); };
             at = deal.place(mark(run));
-            if (run + 1 < runs) end = deal.place(mark(run + 1));
-            else end.g = p.n_grp;
+            if (run + 1 == runs) end.g = p.n_grp;
+            else if (mark(run + 1) < deal.before + deal.mine) { end = at; end.tile = deal.tile_at(mark(run + 1)); }   // (in the same block)
+            else end = deal.place(mark(run + 1));
         }
     }
     if (single) {                                                     // blocks by falling number: the later ones of a group see the more keys
@@ -338,20 +347,20 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                 if (!ends_here) p.items[item].z = run;
             }
             // ---- this lane's query row (rows past the last repeat it)
-            const int  rows = g.nq * p.group, r = min(row0 + l31, rows - 1), tok = r / p.group, head = at.kvh * p.group + r - tok * p.group;
+            const int  rows = g.nq * p.group, r = min(row0 + l31, rows - 1), tok = token_of(p, r), head = at.kvh * p.group + r - tok * p.group;
             const Span s = span_of(p, g, tok);
             // the rows that all of the wave's and that any of them see, and the same of the block: spans move on with the token, but for sequences' own lengths
             const int64_t last_row = min((int64_t) (at.j + 1) * BM, (int64_t) rows) - 1;
             Span s_first, s_last, b_first, b_last;
             if (p.own_lens) {
                 int lo = s.last, hi = s.last, least = s.last;
-                if constexpr (BM > 32) for (int i = lane; i < BM; i += 64) least = min(least, span_of(p, g, (int) (min((int64_t) at.j * BM + i, last_row) / p.group)).last);
+                if constexpr (BM > 32) for (int i = lane; i < BM; i += 64) least = min(least, span_of(p, g, token_of(p, (int) min((int64_t) at.j * BM + i, last_row))).last);
 #pragma unroll
                 for (int d = 1; d < 64; d <<= 1) { lo = min(lo, __shfl_xor(lo, d, 64)); hi = max(hi, __shfl_xor(hi, d, 64)); least = min(least, __shfl_xor(least, d, 64)); }
                 s_first = Span{ 0, uni(lo) }; s_last = Span{ 0, uni(hi) }; b_first = b_last = Span{ 0, uni(least) };
             } else {
                 s_first = Span{ uni(__shfl(s.first, 0, 64)), uni(__shfl(s.last, 0, 64)) }; s_last = Span{ uni(__shfl(s.first, 31, 64)), uni(__shfl(s.last, 31, 64)) };
-                b_first = span_of(p, g, at.j * BM / p.group); b_last = span_of(p, g, (int) last_row / p.group);
+                b_first = span_of(p, g, token_of(p, at.j * BM)); b_last = span_of(p, g, token_of(p, (int) last_row));
             }
             const int64_t seq = p.own_lens ? g.q0 : at.g;             // whose pages
             const char * mask = EXTRA != NOTHING && p.mask ? p.mask + (p.own_lens ? (int64_t) (g.q0 + tok) : at.g) * p.mask_nb1 : nullptr;
