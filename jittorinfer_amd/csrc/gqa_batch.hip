@@ -91,7 +91,7 @@ void mla::gqa::batch_fill(BatchP & p, const BatchCall & c, const BatchPlan & pl,
     p.causal = 0; p.window = 0; p.n_grp = c.n_seq; p.n_tok = c.n_tok; p.n_head = c.n_head; p.n_head_kv = c.n_head_kv; p.group = c.n_head / c.n_head_kv; p.per_head = 1.0 / p.group;
     p.cap = (int) c.cap; p.n_wg = pl.n_wg;
     // a piece of a block is bm x dv numbers to write and to read again: 4 tiles of 64 keys or more each, fewer for the smaller blocks
-    p.min_tiles = c.n_workgroups > 0 || pl.shape == FOUR_KEYS ? 1 : pl.shape == TWO_TWO ? 2 : 4;
+    p.min_tiles = c.n_workgroups > 0 ? 1 : pl.shape == FOUR_ROWS ? 4 : 2;
     p.part_o = (float *) ws; p.part_ml = (float2 *) (ws + pl.off_ml); p.items = (int4 *) (ws + pl.off_items);
     p.tasks = (int4 *) (ws + pl.off_tasks); p.blocks = pl.blocks; p.deal = pl.deal;
 }

@@ -3,7 +3,7 @@
 //   o[r] = sum_i p_i v_i,  p = softmax_i(scale * q[r] . k_i [soft cap] [+ mask]),  r = (token, head) of a group, i the rows that r sees
 //
 // A workgroup of four waves takes a block of query rows; tiles of keys and values come to LDS by direct loads (16 bytes a lane, no registers), the
-// next one while this one is worked on, swizzled so that both ways of reading them are free of bank conflicts.  Per tile and wave:
+// next ones while this one is worked on, swizzled so that both ways of reading them are free of bank conflicts.  Per tile and wave:
 //   * S^T = K Q^T by 32x32x16 MFMAs: a lane holds 16 scores of one query row a block of 32 keys, the other half of the wave the other 16.  Maximum and sum of
 //     a row are a lane's own business (and one exchange between the halves when the reference moves).
 //   * O^T += V^T P^T: the scores' registers, exponentiated and packed, are the second operand as they are (contraction index e of half g: key 4 g + e,
@@ -52,7 +52,7 @@ template <int N> __device__ __forceinline__ void dma_tile(uint64_t base, const u
                      "global_load_lds_dwordx4 %4, %1 offset:2048\n\tglobal_load_lds_dwordx4 %5, %1 offset:3072"
                      : : "s"(lds + j * 1024), "s"(base), "v"(off[j]), "v"(off[j + 1]), "v"(off[j + 2]), "v"(off[j + 3]) : "memory", "m0");
 }
-__device__ __forceinline__ void dma_wait() { __builtin_amdgcn_s_waitcnt(0x0f70); }              // vmcnt(0)
+template <int LEFT> __device__ __forceinline__ void dma_wait() { __builtin_amdgcn_s_waitcnt((LEFT & 15) | 0x0f70 | (LEFT >> 4) << 14); }     // all but the last LEFT loads
 
 // Place of 16-byte chunk c of row r in a tile of rows of D values: c ^ swizzle(r).  Rows 0 .. 15 of a chunk (the reads of K), and the 64 bytes that each of
 // four neighbouring rows gives to a transposing read of V, lie in banks of their own.
@@ -212,6 +212,13 @@ template <bool F16> __device__ __forceinline__ unsigned packed16(float a, float 
 }
 // An address in a register of its own, so that constants added to it become the instructions' offsets.
 __device__ __forceinline__ unsigned base_of(unsigned a) { asm("" : "+v"(a)); return a; }
+// scaled_score with a cap, without branches.
+__device__ __forceinline__ float capped_score(float scale_log2, float cap_in, float cap_out, float a) {
+    const float s = scale_log2 * a, y = fabsf(cap_in * a), u = y * y;
+    const float near = fmaf(u, fmaf(u, 15.f, 420.f), 945.f), far = fast_exp2(2.f * LOG2E * y) + 1.f;
+    const float r = __builtin_amdgcn_rcpf(y < 0.75f ? near : far), x = s * (fmaf(u, u + 105.f, 945.f) * r), z = copysignf(cap_out * fmaf(-2.f, r, 1.f), s);
+    return y < 0.75f ? x : z;
+}
 // l + the two 16-bit numbers of `pair`: the sum is over the weights as they are multiplied, so that a row of one key gets its value as it is.
 template <bool F16> __device__ __forceinline__ float add_pair(float l, unsigned pair) {
     if constexpr (F16) return __builtin_amdgcn_fdot2(bitcast<f16x2>(pair), f16x2{ (_Float16) 1.f, (_Float16) 1.f }, l, false);
@@ -228,7 +235,7 @@ template <bool F16> __device__ __forceinline__ u32x2 pack4(float a, float b, flo
 // What is done to scores besides scaling them: a mask added, or a soft cap and perhaps a mask behind it.
 enum Extra { NOTHING, MASK, CAP };
 
-template <bool F16, int DK, int DV, int NWQ, int NWK, int TK, int OCC, Extra EXTRA>
+template <bool F16, int DK, int DV, int NWQ, int NWK, int TK, int NS, int OCC, Extra EXTRA>
 __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const BatchP) {
     constexpr int NW = NWQ * NWK, BM = 32 * NWQ, KW = TK / NWK, KB = KW / 32, KC = DK / 16, NV = DV / 32;
     constexpr int KT = TK * DK * 2, VT = TK * DV * 2, KI = KT / 1024 / NW, VI = VT / 1024 / NW;
@@ -298,17 +305,17 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
     // ---- what does not change: a lane's places in the tiles
     // (a wave's loads of a tile lie one behind the other; an instruction's offset counts for both its places, so one that is ahead in LDS is taken back in memory)
     auto step_of = [](int per, int j) { return j < per % 4 ? j : (j - per % 4) % 4; };
-    auto row_in = [&](int d, int per, int j) { return ((wave * per + j) * 64 + lane) / (d / 8); };
-    auto place_in = [&](int d, int per, int j) { const int r = row_in(d, per, j), c = ((wave * per + j) * 64 + lane) % (d / 8); return (c ^ (d % 128 == 0 ? swizzle<128>(r) : swizzle<64>(r))) * 16 + (4 - step_of(per, j)) * 1024; };
+    auto row_in = [&](int d, int per, int j, int lane) { return ((wave * per + j) * 64 + lane) / (d / 8); };
+    auto place_in = [&](int d, int per, int j, int lane) { const int r = row_in(d, per, j, lane), c = ((wave * per + j) * 64 + lane) % (d / 8); return (c ^ (d % 128 == 0 ? swizzle<128>(r) : swizzle<64>(r))) * 16 + (4 - step_of(per, j)) * 1024; };
     int k_row, v_row;
     unsigned k_at[KI], v_at[VI];
     {
         Params & p = *fresh();
         k_row = p.k_row; v_row = p.v_row;
 #pragma unroll
-        for (int j = 0; j < KI; j++) k_at[j] = (unsigned) (row_in(DK, KI, j) * k_row + place_in(DK, KI, j));
+        for (int j = 0; j < KI; j++) k_at[j] = (unsigned) (row_in(DK, KI, j, lane) * k_row + place_in(DK, KI, j, lane));
 #pragma unroll
-        for (int j = 0; j < VI; j++) v_at[j] = (unsigned) (row_in(DV, VI, j) * v_row + place_in(DV, VI, j));
+        for (int j = 0; j < VI; j++) v_at[j] = (unsigned) (row_in(DV, VI, j, lane) * v_row + place_in(DV, VI, j, lane));
     }
     // transposing reads: row, 16-byte chunk and half of it; the addresses of a chunk of 32 columns, for rows 0 .. 3 and 8 .. 11 of 16
     const int vq = hh * 4 + ((lane >> 2) & 3), vc = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), vsub = (lane & 1) * 8;
@@ -346,6 +353,9 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                 if (begins) { p.items[item].x = (int) slot; p.items[item].y = run; }
                 if (!ends_here) p.items[item].z = run;
             }
+            // (what the loop over tiles needs of the arguments)
+            const float scale_log2 = p.scale_log2, cap_in = EXTRA == CAP ? p.cap_in : 0.f, cap_out = EXTRA == CAP ? p.cap_out : 0.f, mask_unit = EXTRA == MASK ? p.mask_unit : 0.f;
+            const bool  masks = EXTRA != NOTHING && p.mask;
             // ---- this lane's query row (rows past the last repeat it)
             const int  rows = g.nq * p.group, r = min(row0 + l31, rows - 1), tok = token_of(p, r), head = at.kvh * p.group + r - tok * p.group;
             const Span s = span_of(p, g, tok);
@@ -382,12 +392,12 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                     dma_tile<KI>(kb, k_at, k_to);
                     dma_tile<VI>(vb, v_at, v_to);
                 } else {                                              // (rows past the last repeat it)
-                    const int last = g.len - key0 - 1;
+                    const int last = g.len - key0 - 1, me = (int) base_of(lane);     // (worked out here, and not kept for here)
                     unsigned k_end[KI], v_end[VI];
 #pragma unroll
-                    for (int j = 0; j < KI; j++) k_end[j] = (unsigned) (min(row_in(DK, KI, j), last) * k_row + place_in(DK, KI, j));
+                    for (int j = 0; j < KI; j++) k_end[j] = (unsigned) (min(row_in(DK, KI, j, me), last) * k_row + place_in(DK, KI, j, me));
 #pragma unroll
-                    for (int j = 0; j < VI; j++) v_end[j] = (unsigned) (min(row_in(DV, VI, j), last) * v_row + place_in(DV, VI, j));
+                    for (int j = 0; j < VI; j++) v_end[j] = (unsigned) (min(row_in(DV, VI, j, me), last) * v_row + place_in(DV, VI, j, me));
                     dma_tile<KI>(kb, k_end, k_to);
                     dma_tile<VI>(vb, v_end, v_to);
                 }
@@ -451,7 +461,7 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
 #pragma unroll
                         for (int b = 0; b < KB; b++)
 #pragma unroll
-                            for (int e = 0; e < 16; e++) start[b][e] = masked_by(b, e) * p.mask_unit;
+                            for (int e = 0; e < 16; e++) start[b][e] = masked_by(b, e) * mask_unit;
 #pragma unroll
                 for (int b = 0; b < KB; b++) {
                     sc[b] = start[b];
@@ -479,20 +489,25 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                 for (int n = 0; n < (NV + 1) / 2; n++) up[n] = down[n] = 0;
             __syncthreads();                                          // (LDS is free of what was before)
             fetch_mask(t0);
-            int id = paged ? page_at(t0) : 0, id_next = paged && t0 + 1 < t1 ? page_at(t0 + 1) : 0;
-            fetch(t0, id, 0);
+            // (NS - 1 tiles are under way at a time; page ids are read a tile ahead of that)
+            int ids[NS];
+#pragma unroll
+            for (int i = 0; i < NS; i++) ids[i] = paged ? page_at(min(t0 + i, t1 - 1)) : 0;
+#pragma unroll
+            for (int i = 0; i < NS - 1; i++) if (t0 + i < t1) fetch(t0 + i, ids[i], i);
+            int buf = 0;
             for (int t = t0; t < t1; t++) {
-                dma_wait();
+                if (NS > 2 && t + NS - 2 < t1) dma_wait<(NS - 2) * (KI + VI)>();
+                else                           dma_wait<0>();
                 __syncthreads();
-                const int  buf = (t - t0) & 1, key0 = t * TK + wk * KW;
-                const bool use = !paged || good(id);
-                if (t + 1 < t1) {
-                    id = id_next;
-                    fetch(t + 1, id, buf ^ 1);
-                    if (paged && t + 2 < t1) id_next = page_at(t + 2);
-                }
+                const int  key0 = t * TK + wk * KW;
+                const bool use = !paged || good(ids[0]);
+                if (t + NS - 1 < t1) fetch(t + NS - 1, ids[NS - 1], buf == 0 ? NS - 1 : buf - 1);
+#pragma unroll
+                for (int i = 0; i + 1 < NS; i++) ids[i] = ids[i + 1];
+                if (paged && t + NS < t1) ids[NS - 1] = page_at(t + NS);
                 const unsigned kt = uni(lds0 + buf * (KT + VT) + wk * KW * (DK * 2)), vt = uni(lds0 + buf * (KT + VT) + KT + wk * KW * (DV * 2));
-                if (safe && ((EXTRA != NOTHING && p.mask) || t * TK < b_last.first || t * TK + TK > b_first.last)) {
+                if (safe && ((EXTRA != NOTHING && masks) || t * TK < b_last.first || t * TK + TK > b_first.last)) {
                     unsigned bad = 0;
                     const unsigned mine = lds0 + buf * (KT + VT) + KT + threadIdx.x * 16;
 #pragma unroll
@@ -501,11 +516,11 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                         bad |= nonfinite<F16>(x.x) | nonfinite<F16>(x.y) | nonfinite<F16>(x.z) | nonfinite<F16>(x.w);
                     }
                     const int found = __any(bad != 0);
-                    if (lane == 0) sh_bad[buf][wave] = found;
+                    if (lane == 0) sh_bad[t & 1][wave] = found;
                     __syncthreads();
                     int any = 0;
 #pragma unroll
-                    for (int w = 0; w < NW; w++) any |= sh_bad[buf][w];
+                    for (int w = 0; w < NW; w++) any |= sh_bad[t & 1][w];
                     if (uni(any)) {
 #pragma unroll 1
                         for (int n = 0; n < NV; n++) {
@@ -544,7 +559,7 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                     f32x16 sc[KB];
                     u32x4  pf[KB][2];
                     products(kt, sc);
-                    float top, unit = p.scale_log2;                   // what makes log2 units of sc
+                    float top, unit = scale_log2;                   // what makes log2 units of sc
                     const bool all = key0 + KW <= s_first.last && key0 >= s_last.first;
                     if (EXTRA != CAP && all && !(EXTRA == MASK && safe)) {
                         top = sc[0][0];
@@ -563,28 +578,48 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                             for (int b = 0; b < KB; b++)
 #pragma unroll
                                 for (int e = 0; e < 16; e++) most = fmaxf(most, fabsf(sc[b][e]));
-                            small = !uni(__any(!(most * p.cap_in < 0.25f)));
+                            small = cap_out != 0.f && !uni(__any(!(most * cap_in < 0.25f)));
                         }
-                        auto capped = [&](float a) {
-                            if (!small) return scaled_score(p.scale_log2, p.cap_in, p.cap_out, a);
-                            const float y = p.cap_in * a, u = y * y;
-                            return p.scale_log2 * a * fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, -1382.f / 155925, 62.f / 2835), -17.f / 315), 2.f / 15), -1.f / 3), 1.f);
-                        };
-                        const int from = s.first - key0 - hh * 4, to = s.last - key0 - hh * 4;
+                        // (a pass over the scores for each thing that is done to them, none with a branch in it)
+                        if (EXTRA == CAP && small) {
+#pragma unroll
+                            for (int b = 0; b < KB; b++)
+#pragma unroll
+                                for (int e = 0; e < 16; e++) {
+                                    const float y = cap_in * sc[b][e], u = y * y;
+                                    sc[b][e] *= scale_log2 * fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, -1382.f / 155925, 62.f / 2835), -17.f / 315), 2.f / 15), -1.f / 3), 1.f);
+                                }
+                        } else if (EXTRA == CAP && cap_out != 0.f) {
+#pragma unroll
+                            for (int b = 0; b < KB; b++)
+#pragma unroll
+                                for (int e = 0; e < 16; e++) sc[b][e] = capped_score(scale_log2, cap_in, cap_out, sc[b][e]);
+                        } else {
+#pragma unroll
+                            for (int b = 0; b < KB; b++)
+#pragma unroll
+                                for (int e = 0; e < 16; e++) sc[b][e] *= scale_log2;
+                        }
+                        if (EXTRA == CAP ? mask != nullptr : EXTRA == MASK && safe)
+#pragma unroll
+                            for (int b = 0; b < KB; b++)
+#pragma unroll
+                                for (int e = 0; e < 16; e++) {
+                                    const float f = masked_by(b, e), v = fmaf(f, LOG2E, sc[b][e]);
+                                    sc[b][e] = f == -INFINITY ? -INFINITY : v;
+                                }
+                        if (!all) {
+                            const int from = s.first - key0 - hh * 4;
+                            const unsigned n = max(s.last - s.first, 0);
+#pragma unroll
+                            for (int b = 0; b < KB; b++)
+#pragma unroll
+                                for (int e = 0; e < 16; e++) sc[b][e] = (unsigned) (b * 32 + (e >> 2) * 8 + (e & 3) - from) < n ? sc[b][e] : -INFINITY;
+                        }
 #pragma unroll
                         for (int b = 0; b < KB; b++)
 #pragma unroll
-                            for (int e = 0; e < 16; e++) {
-                                float v = EXTRA == CAP ? capped(sc[b][e]) : sc[b][e] * p.scale_log2;
-                                if (EXTRA == CAP ? mask != nullptr : EXTRA == MASK && safe) {
-                                    const float f = masked_by(b, e);
-                                    v = f == -INFINITY ? -INFINITY : fmaf(f, LOG2E, v);
-                                }
-                                const int i = b * 32 + (e >> 2) * 8 + (e & 3);
-                                if (!all && (i < from || i >= to)) v = -INFINITY;
-                                sc[b][e] = v;
-                                top = fmaxf(top, v);
-                            }
+                            for (int e = 0; e < 16; e++) top = fmaxf(top, sc[b][e]);
                         unit = 1.f;
                     }
                     if (EXTRA != NOTHING && t + 1 < t1) fetch_mask(t + 1);
@@ -638,6 +673,7 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                     }
                 }
                 else if (EXTRA != NOTHING && t + 1 < t1) fetch_mask(t + 1);
+                buf = buf + 1 == NS ? 0 : buf + 1;
             }
                 if (safe) break;
                 float odd = l * 0.f;                                  // NaN if anything is not finite
@@ -812,15 +848,15 @@ __global__ void __launch_bounds__(256) gqa_batch_join_kernel(const BatchP p) {
 
 // ---------------------------------------------------------------- host
 
-template <bool F16, int DK, int DV, int NWQ, int NWK, int TK, int OCC, Extra EXTRA>
+template <bool F16, int DK, int DV, int NWQ, int NWK, int TK, int NS, int OCC, Extra EXTRA>
 hipError_t launch_batch(const BatchP & p, const BatchPlan & pl, hipStream_t st) {
-    constexpr int lds = 2 * TK * (DK + DV) * 2;
-    static_assert(lds + NWQ * NWK * 32 * 8 <= 160 * 1024, "LDS");
+    constexpr int lds = NS * TK * (DK + DV) * 2;
+    static_assert(OCC * (lds + NWQ * NWK * 8 + (NWK > 1 ? NWQ * NWK * 32 * 8 : 0)) <= 160 * 1024, "LDS");
     static std::atomic<uint64_t> granted{ 0 };
-    hipError_t e = grant_lds(gqa_batch_kernel<F16, DK, DV, NWQ, NWK, TK, OCC, EXTRA>, lds, granted);
+    hipError_t e = grant_lds(gqa_batch_kernel<F16, DK, DV, NWQ, NWK, TK, NS, OCC, EXTRA>, lds, granted);
     if (e != hipSuccess) return e;
     const int64_t grid = p.deal == RUNS ? p.n_wg : (int64_t) p.blocks * p.n_head_kv;
-    hipLaunchKernelGGL((gqa_batch_kernel<F16, DK, DV, NWQ, NWK, TK, OCC, EXTRA>), dim3((unsigned) (grid > p.n_wg ? grid : p.n_wg)), dim3(64 * NWQ * NWK), lds, st, p);
+    hipLaunchKernelGGL((gqa_batch_kernel<F16, DK, DV, NWQ, NWK, TK, NS, OCC, EXTRA>), dim3((unsigned) (grid > p.n_wg ? grid : p.n_wg)), dim3(64 * NWQ * NWK), lds, st, p);
     if ((e = hipGetLastError()) != hipSuccess || p.own_lens || p.deal == WHOLE) return e;
     hipLaunchKernelGGL((gqa_batch_join_kernel<F16, DV, NWQ>), dim3((unsigned) p.n_wg, DV / 32), dim3(256), 0, st, p);
     return hipGetLastError();
@@ -828,9 +864,9 @@ hipError_t launch_batch(const BatchP & p, const BatchPlan & pl, hipStream_t st) 
 // (heads of 192: tiles of 32 keys, so that two workgroups' lie in a CU's LDS; of 256: so that a wave's scores leave room in its registers)
 template <bool F16, int DK, int DV, Extra EXTRA>
 hipError_t launch_shape(const BatchP & p, const BatchPlan & pl, hipStream_t st) {
-    if constexpr (DK <= 128) if (pl.shape == FOUR_KEYS) return launch_batch<F16, DK, DV, 1, 4, 128, batch_wg_per_cu(DK, FOUR_KEYS, EXTRA == NOTHING), EXTRA>(p, pl, st);
-    if (pl.shape == FOUR_ROWS) return launch_batch<F16, DK, DV, 4, 1, DK >= 192 ? 32 : 64, batch_wg_per_cu(DK, FOUR_ROWS, EXTRA == NOTHING), EXTRA>(p, pl, st);
-    return launch_batch<F16, DK, DV, 2, 2, 64, batch_wg_per_cu(DK, TWO_TWO, EXTRA == NOTHING), EXTRA>(p, pl, st);
+    if constexpr (DK <= 128) if (pl.shape == FOUR_KEYS) return launch_batch<F16, DK, DV, 1, 4, 128, 2, batch_wg_per_cu(DK, FOUR_KEYS, EXTRA == NOTHING), EXTRA>(p, pl, st);
+    if (pl.shape == FOUR_ROWS) return launch_batch<F16, DK, DV, 4, 1, DK >= 192 ? 32 : 64, DK == 256 ? 4 : DK == 192 ? 3 : 2, batch_wg_per_cu(DK, FOUR_ROWS, EXTRA == NOTHING), EXTRA>(p, pl, st);
+    return launch_batch<F16, DK, DV, 2, 2, 64, DK == 192 ? 3 : 2, batch_wg_per_cu(DK, TWO_TWO, EXTRA == NOTHING), EXTRA>(p, pl, st);
 }
 template <bool F16, Extra EXTRA>
 hipError_t launch_widths(const BatchP & p, const BatchPlan & pl, int dk, hipStream_t st) {
