@@ -22,7 +22,13 @@ BatchPlan mla::gqa::batch_plan(const BatchCall & c, bool whole_blocks) {
     BatchPlan pl;
     const int     group = c.n_head / c.n_head_kv;
     const int64_t rows = ((int64_t) c.n_tok * group + c.n_seq - 1) / c.n_seq;     // of a sequence, on average
-    pl.shape  = rows <= 32 && c.dk <= 128 ? FOUR_KEYS : rows <= 64 ? TWO_TWO : FOUR_ROWS;
+    // Waves along the keys where rows are few; and up to 192 of them where there are few runs of keys (KV heads of all groups), which then lie in more workgroups'
+    // hands and are read again from the caches.  Four along the keys / two and two / four along the rows, us, 4000 rows of keys, 32 heads on 8 of 128: 1 x 8
+    // tokens (32 rows) 24 / 30 / 35, 1 x 16 (64) 23 / 31 / 36, 1 x 48 (192) 32 / 36 / 41, 16 x 8 55 / 62 / 73, 16 x 16 68 / 64 / 75, 16 x 24 (96) 124 / 73 / 77, 16 x 48 232 /
+    // 147 / 100; 16 on 4 of 64: 16 x 16 28 / 32 / 46, 16 x 32 35 / 33 / 46; 16 on 4 of 256 (two and two, four along the rows): 1 x 32 49 / 59, 16 x 16 67 / 91, 16 x 32 99 / 93.
+    const int64_t runs = (int64_t) c.n_seq * c.n_head_kv;
+    if (rows <= 64 || (rows <= 192 && runs <= 32)) pl.shape = c.dk <= 128 ? FOUR_KEYS : TWO_TWO;
+    else pl.shape = rows <= 128 && c.dk <= 128 ? TWO_TWO : FOUR_ROWS;
     pl.bm     = pl.shape == FOUR_KEYS ? 32 : pl.shape == TWO_TWO ? 64 : 128;
     const int64_t blocks = (int64_t) c.n_tok * group / pl.bm + c.n_seq;
     pl.blocks = blocks < INT_MAX ? (int) blocks : INT_MAX;
@@ -36,9 +42,9 @@ BatchPlan mla::gqa::batch_plan(const BatchCall & c, bool whole_blocks) {
     pl.off_ml    = take(slots * pl.bm * 8);
     pl.off_items = take((size_t) pl.blocks * c.n_head_kv * 16);
     pl.off_tasks = take((size_t) pl.n_wg * 16);
-    // Whole blocks: of one sequence none is heavier than twice the mean, so that the number of them tells; of several the device looks.
+    // (four blocks a workgroup of one sequence are taken whole in any case: no more than an eighth of the time is lost at the end)
     const int64_t full = (int64_t) c.n_tok * group / pl.bm * c.n_head_kv;
-    pl.deal = whole_blocks || c.n_workgroups > 0 || full * WHOLE_SHARE < fill ? RUNS : c.n_seq == 1 && full * WHOLE_SHARE >= 2 * fill ? WHOLE : EITHER;
+    pl.deal = whole_blocks || c.n_workgroups > 0 ? RUNS : c.n_seq == 1 && full >= 4 * fill ? WHOLE : EITHER;
     pl.bytes = at;
     return pl;
 }
@@ -90,8 +96,9 @@ void mla::gqa::batch_fill(BatchP & p, const BatchCall & c, const BatchPlan & pl,
     p.cap_out = fminf(c.logit_softcap * LOG2E, FLT_MAX);
     p.causal = 0; p.window = 0; p.n_grp = c.n_seq; p.n_tok = c.n_tok; p.n_head = c.n_head; p.n_head_kv = c.n_head_kv; p.group = c.n_head / c.n_head_kv; p.per_head = 1.0 / p.group;
     p.cap = (int) c.cap; p.n_wg = pl.n_wg;
-    // a piece of a block is bm x dv numbers to write and to read again: 4 tiles of 64 keys or more each, fewer for the smaller blocks
-    p.min_tiles = c.n_workgroups > 0 ? 1 : pl.shape == FOUR_ROWS ? 4 : 2;
+    // A piece of a block is bm x dv numbers to write and to read again: 4 tiles or more a workgroup.  1, 2, 4, 8, 16 of them, us: 8 tokens behind 4000 rows 24.0, 24.3, 23.2, 28.3,
+    // 38.0; 64 tokens 79, 79, 41, 39, 45; 32 users behind 8192 shared rows 49.6, 49.2, 47.5, 46.3, 54.3; one token of 16 over 1500 states 29.6, 29.4, 29.4, 30.7, 34.4.
+    p.min_tiles = c.n_workgroups > 0 ? 1 : 4;
     p.part_o = (float *) ws; p.part_ml = (float2 *) (ws + pl.off_ml); p.items = (int4 *) (ws + pl.off_items);
     p.tasks = (int4 *) (ws + pl.off_tasks); p.blocks = pl.blocks; p.deal = pl.deal;
 }

@@ -36,10 +36,12 @@ struct BatchP {
     int      blocks, deal;        // block numbers, and a Dealing
 };
 
-// Blocks are dealt in equal runs, one to a workgroup, or the one or the other by what the device finds: whole blocks where the heaviest is at most WHOLE_SHARE of a
-// workgroup's share.
+// Blocks are dealt in equal runs, one to a workgroup, or the one or the other by what the device finds.  Runs cost pieces that are written, read again and joined: as
+// much as JOIN_KEYS keys of a block; whole blocks leave workgroups idle at the end.  Both sides, us (32 heads on 8 of 128, bf16, where no other is named): prompts of
+// 2 x 512 tokens 40 against 22, 4 x 1024 85 / 60, 1 x 4096 181 / 155, 4 x 1500 to 2048 178 / 141, 32 x 448 tokens over 1500 states (16 heads of 64) 174 / 143; 3 x
+// 600 to 1024 over 3000 to 8192 states 371 / 383, 8 x 512 behind 5000 to 16384 rows (16 on 4 of 64) 272 / 367.
 enum Dealing { RUNS, EITHER, WHOLE };
-constexpr float WHOLE_SHARE = 0.67f;
+constexpr int JOIN_KEYS = 1280;
 
 // Waves along the query rows and along the keys of a tile, keys of a tile.
 enum Shape { FOUR_ROWS, TWO_TWO, FOUR_KEYS };

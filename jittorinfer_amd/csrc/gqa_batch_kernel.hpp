@@ -131,19 +131,19 @@ template <int BM, int TK> struct Deal {
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) { const double o = __shfl_up(incl, d, 64); if (lane >= d) incl += o; }
     }
-    // the weight of all blocks, and of the heaviest (the last of a group, at most)
-    __device__ __forceinline__ double total(float & most) {
+    // the weight of all blocks; of the heaviest (the last of a group, at most) and of the heaviest among the first ones of the groups, which are the last to be begun
+    __device__ __forceinline__ double total(float & most, float & late) {
         double all = 0.;
-        most = 0.f;
+        most = late = 0.f;
         for (int g0 = 0; g0 < p.n_grp; g0 += 64) {
             fetch(g0);
             all += __shfl(incl, p.n_grp > 1 ? 63 : 0, 64);
             if (p.deal != EITHER) continue;
             const int nb = w > 0. ? blocks_of<BM>(p, g) : 0;
-            float last = nb ? (float) (weight_before<BM>(p, g, nb) - weight_before<BM>(p, g, nb - 1)) : 0.f;
+            float last = nb ? (float) (weight_before<BM>(p, g, nb) - weight_before<BM>(p, g, nb - 1)) : 0.f, first = nb ? (float) weight_before<BM>(p, g, 1) : 0.f;
 #pragma unroll
-            for (int d = 1; d < 64; d <<= 1) last = fmaxf(last, __shfl_xor(last, d, 64));
-            most = fmaxf(most, last);
+            for (int d = 1; d < 64; d <<= 1) { last = fmaxf(last, __shfl_xor(last, d, 64)); first = fmaxf(first, __shfl_xor(first, d, 64)); }
+            most = fmaxf(most, last); late = fmaxf(late, first);
         }
         return all;
     }
@@ -270,9 +270,10 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
     Deal<BM, TK> deal{ p, lane };
     single = p.deal == WHOLE;
     if (!single) {
-        float         most;
-        const double  total = deal.total(most);
-        single = p.deal == EITHER && most * p.n_wg <= WHOLE_SHARE * (float) total;
+        float        most, late;
+        const double total = deal.total(most, late);
+        const float  share = (float) total / p.n_wg;
+        single = p.deal == EITHER && fmaxf(most, share + 0.5f * late) <= share + (float) JOIN_KEYS * p.group;
         if (!single) {
             const int runs = (int) fmax(total > 0. ? 1. : 0., fmin((double) p.n_wg, total / ((double) p.min_tiles * TK * p.group)));
             if ((int) blockIdx.x >= runs) {
@@ -293,11 +294,12 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
     }
     if (single) {                                                     // blocks by falling number: the later ones of a group see the more keys
         const int64_t id = (int64_t) p.blocks - 1 - blockIdx.x / p.n_head_kv;
+        // (no block is left to be joined: every workgroup that the join looks at says so, those without a block among them)
+        if ((int) blockIdx.x < p.n_wg && threadIdx.x == 0) p.tasks[blockIdx.x] = make_int4(-1, 0, 0, 0);
         if (id < 0) return;
         at.g = group_with<BM>(p, id, lane); at.kvh = blockIdx.x % p.n_head_kv; at.tile = 0;
         const Group g = group_of(p, at.g);
         at.j = (int) max(id - number_of<BM>(p, at.g, g.q0), (int64_t) -1);
-        if ((int) blockIdx.x < p.n_wg && threadIdx.x == 0) p.tasks[blockIdx.x] = make_int4(-1, 0, 0, 0);
         if (at.j < 0 || at.j >= blocks_of<BM>(p, g)) return;
     }
     }
