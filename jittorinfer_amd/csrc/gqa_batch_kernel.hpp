@@ -444,7 +444,8 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
             f32x16 acc[NV];
             // Infinities and NaN among keys and values must not count where a row does not see them, and 0 * them does.  The piece is worked on as if there were none; if a result
             // is not finite, once more from the start, `safe`: with the infinities and NaN among the values of every tile that not all rows see whole noted for the rows that
-            // see them, and taken for zeros, and with masked scores set and not added to.
+            // see them, and taken for zeros, and with masked scores set and not added to.  So is a piece whose largest scores come of a large finite number of the mask: sums that
+            // begin with one of size x lose up to dk / 16 half steps of it (2^-20 x), added last it costs a single one.
             unsigned up[(NV + 1) / 2], down[(NV + 1) / 2];            // safe: results that a +infinity (-infinity, NaN: both) belongs to
             bool safe = false;
 
@@ -679,6 +680,7 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
             }
                 if (safe) break;
                 float odd = l * 0.f;                                  // NaN if anything is not finite
+                if (EXTRA == MASK && fabsf(m) > 1024.f && m != -INFINITY) odd = NAN;
 #pragma unroll
                 for (int n = 0; n < NV; n++)
 #pragma unroll

@@ -156,6 +156,35 @@ def test_prompt_mask(gpu, dk, dv, dtype):
         _check(gpu, q[:64], k, v, bt, lens, _starts([10, 20, 5, 5, 3]), mask=mask)
 
 
+@pytest.mark.parametrize("new", [[60, 129, 40], [2, 9, 1]])
+@pytest.mark.parametrize("dk,dv", WIDTHS)
+def test_prompt_mask_of_the_lowest_value_alone(gpu, dk, dv, new):
+    """A number added to every row of a sequence changes nothing but the scores' rounding; rows of the lowest value beside others have no weight."""
+    import jittorinfer_amd as J
+    q, k, v, bt, lens, starts = _case(13, new, [300, 129, 260], 3, 6, 2, dk, dv, F16)
+    low = torch.finfo(F16).min
+    mask = torch.full((3, 384), low, dtype=F16)
+    mask[1, ::2] = -30000.0                     # (a page of rows and one: every token sees one of these)
+    hard = torch.zeros((3, 384), dtype=F16)
+    hard[1, 1::2] = float("-inf")
+    scale = dk ** -0.5
+    want, off = B.prompt(q, k, v, bt, lens, starts, scale, mask=hard)
+    # a score and the number are added in log2 units, below 2^17 in size: the sum is off by half a step, 2^-8, which is 2^-8 ln 2 of a weight, and a
+    # softmax turns that into twice as much of a result; the score itself as without a mask
+    gathered = torch.zeros_like(off)
+    for b in range(3):
+        n = int(lens[b])
+        at = torch.arange(n)
+        vv = v[bt[b].long()[at // 128], at % 128].double().abs().amax(0).repeat_interleave(3, 0)
+        gathered[starts[b]:starts[b + 1]] = vv
+    off = off + 2 * 2.0 ** -8 * math.log(2) * gathered
+    out = J.gqa_prompt_attn(q.to(gpu), k.to(gpu), v.to(gpu), bt.to(gpu), lens.to(gpu), starts.to(gpu), scale=scale, mask=mask.to(gpu))
+    _near(out, want, off, F16)
+    # and as a whole: those errors are of either sign and independent, sqrt(3) below the bound each, and a result is off by its weights' errors as it is made of its weights
+    err = (out.cpu().double() - want).norm() / want.norm()
+    assert err < 2.0 ** -8 * math.log(2), err
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("dk,dv,new", [(64, 64, 300), (128, 128, 300), (192, 128, 300), (256, 256, 300), (64, 64, 7), (128, 128, 14), (256, 256, 14)])
 def test_prompt_infinities_of_rows_not_seen(gpu, dk, dv, new, dtype):
