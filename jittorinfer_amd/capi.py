@@ -519,7 +519,7 @@ def gqa_prefix_attn(q, k_cache, v_cache, block_table, seq_lens, prefix_starts, p
 
     q, k_cache, v_cache, block_table, seq_lens  as in gqa_attn, all of one 16-bit type; seq_lens counts the shared rows too
     prefix_starts, prefix_lens  int32 [n + 1], [n]: the sequences prefix_starts[g] .. prefix_starts[g + 1] - 1 lie side by side in the batch, and their first
-              prefix_lens[g] rows are the same keys and values (read through the first one's block table); sequences outside share nothing.
+              prefix_lens[g] rows are the same keys and values (read through the first one's block table or each one's own); sequences outside share nothing.
               PageTable.shared_prefixes finds them
     mask      float16 [n_seq, n] or None, as in gqa_attn
     Returns out, [n_seq, n_head, dv] of q's type; a sequence without a row gets zeros."""

@@ -14,6 +14,13 @@
 // Work: where there are blocks enough, a workgroup each, the heavy ones first.  Else blocks in the order (group, KV head, block) have weights (keys they see, closed
 // sums), and the workgroups take equal runs of the total weight, cut at tiles.  A run that covers a block writes its result; the others leave (o, m, l)
 // for gqa_batch_join_kernel.  All of that is decided from the lengths on the device: a captured launch stays valid while they change.
+//
+// What bounds it: the matrix units with the exponentials between their products (a tile of 64 keys of heads of 128: 64 MFMAs of 16 cycles a wave, and 32 exponentials,
+// 16 roundings of pairs and as many sums beside some 250 other vector instructions; two waves a SIMD, each in the other's gaps).  Prompts of 4 x 4096 tokens, 32 heads on 8,
+// bf16, TFLOP/s without anything / with a mask / with a soft cap: heads of 64 596 / 463 / 388 (twice the exponentials a product), 128 909 / 745 / 669, 192 875 / 644 /
+// 613, 256 532 / 432 / 421 (one wave a SIMD: 512 registers); f16 of 64 667.  One prompt of 16384 tokens, heads of 128: 2.1 ms, 1.04 PFLOP/s, where an 8192 x 8192 x 8192 library
+// product reaches 1.20; its matrix units are busy 44 % of the time at a clock of 2.0 GHz, and LDS has no bank conflicts.  Fewer rows than 128 a block are bound by what a
+// run waits for: 8 tokens behind 4000 rows 15 us here and 5 in the join, of which 3.2 would be the bytes.
 #pragma once
 
 #include <limits.h>
@@ -783,7 +790,8 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
 }
 
 // Joins the pieces of one block: o = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M).  Grid: x = runs, each of which may leave one block that goes on in others, y = 32 columns of
-// the result.  A thread takes 16 columns of its row (4 loads a piece) and, where a block has fewer than 128 rows, every second or fourth piece.
+// the result.  A thread takes 16 columns of its row (4 loads a piece) and, where a block has fewer than 128 rows, every second or fourth piece.  Its three dependent loads (task, item,
+// pieces) bound it where pieces are few: 4.3 us when nothing is to be joined, 5.3 for 8 tokens behind 4000 rows; 12 for 8 x 512 tokens behind 5000 to 16384 rows (768 runs).
 template <bool F16, int DV, int NWQ>
 __global__ void __launch_bounds__(256) gqa_batch_join_kernel(const BatchP p) {
     constexpr int BM = 32 * NWQ, PG = 4 / NWQ, AHEAD = 4;
@@ -865,7 +873,9 @@ hipError_t launch_batch(const BatchP & p, const BatchPlan & pl, hipStream_t st) 
     hipLaunchKernelGGL((gqa_batch_join_kernel<F16, DV, NWQ>), dim3((unsigned) p.n_wg, DV / 32), dim3(256), 0, st, p);
     return hipGetLastError();
 }
-// (heads of 192: tiles of 32 keys, so that two workgroups' lie in a CU's LDS; of 256: so that a wave's scores leave room in its registers)
+// Heads of 192: tiles of 32 keys in three stages, so that two workgroups' lie in a CU's LDS; of 256: tiles of 32, so that a wave's scores leave room in its registers (6 x 700
+// tokens, window and cap: 277 us with 64 keys, 235 with 32), in four stages (228 with two, 219 with four).  Narrower heads have two stages of 64: a third one for heads of 64 made
+// 8 x 512 tokens behind 16384 rows 293 us, not 283.
 template <bool F16, int DK, int DV, Extra EXTRA>
 hipError_t launch_shape(const BatchP & p, const BatchPlan & pl, hipStream_t st) {
     if constexpr (DK <= 128) if (pl.shape == FOUR_KEYS) return launch_batch<F16, DK, DV, 1, 4, 128, 2, batch_wg_per_cu(DK, FOUR_KEYS, EXTRA == NOTHING), EXTRA>(p, pl, st);

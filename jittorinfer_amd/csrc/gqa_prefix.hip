@@ -4,7 +4,9 @@
 //   2. the rows behind them, a sequence at a time, by gqa_attn's kernel; every head is left as pieces
 //   3. the join, here: out = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M) over the pieces of both, in the order of the rows
 //
-// The keys of a prefix are read once a group and KV head for up to 128 rows, where gqa_attn reads them once a sequence.
+// The keys of a prefix are read once a group and KV head for up to 128 rows, where gqa_attn reads them once a sequence.  32 users behind 8192 shared rows (32 heads on 8 of 128): 46 us, of
+// which the prefix is 25, the rows behind it 12.4 and the join 6.9 (8192 pieces' rows); 16 would be the bytes, and gqa_attn takes 142.  Each launch waits for lengths, page ids and
+// rows in turn, and for the one before it.  Five users behind 100000 rows: 102 us (gqa_attn 289), 4.0 TB/s of the call.
 
 #include <limits.h>
 
@@ -107,7 +109,7 @@ BatchCall call_of(const gqa_prefix_attn_args * a) {
     return BatchCall{ a->n_seq, a->n_prefix, a->n_head, a->n_head_kv, a->dk, a->dv, a->type, a->n_workgroups, a->scale, a->logit_softcap, a->q, a->q_nb1, a->q_nb2, a->prefix_starts, a->k, a->v,
                       a->bt_stride >= 0 && a->bt_stride < INT_MAX ? a->bt_stride * PAGE : INT64_MAX, a->mask, a->mask_nb1, a->mask_ne0, a->dst, a->d_nb1, a->d_nb2 };
 }
-// gqa_attn's call for what is behind the prefixes (or, without any, for all rows)
+// gqa_attn's call for what is behind the prefixes (or for all rows)
 gqa_attn_args attn_of(const gqa_prefix_attn_args * a) {
     gqa_attn_args t = {};
     t.n_seq = a->n_seq; t.n_head = a->n_head; t.n_head_kv = a->n_head_kv; t.dk = a->dk; t.dv = a->dv; t.q_type = t.kv_type = t.dst_type = a->type;
@@ -117,6 +119,13 @@ gqa_attn_args attn_of(const gqa_prefix_attn_args * a) {
     t.mask = a->mask; t.mask_nb1 = a->mask_nb1; t.mask_ne0 = a->mask_ne0;
     t.dst = a->dst; t.d_nb1 = a->d_nb1; t.d_nb2 = a->d_nb2; t.workspace = a->workspace; t.workspace_size = a->workspace_size;
     return t;
+}
+// The prefixes by themselves, or every sequence whole by gqa_attn: a table with room for less than 2^28 bytes of rows (the last cache's size) has the shared ones read from caches again
+// and again, for less than the two further launches take.  us, prefixes by themselves / gqa_attn, 512 .. 8192 shared rows and 200 own ones a user, 32 heads on 8 of 128:
+// 4 users with room for 13 MB 31 / 12, 38 MB 30 / 15, 138 MB 37 / 30; 16 of one group 50 MB 31 / 15, 151 MB 34 / 26, 285 MB 36 / 38, 554 MB 35 / 86; 64 of 8 groups 201 MB 40 / 31, 336 MB
+// 41 / 47, 604 MB 42 / 93; 16 on 4 of 64: 138 MB 27 / 25, 285 MB 32 / 36, 554 MB 36 / 61; 16 on 4 of 256: 151 MB 42 / 28, 285 MB 44 / 46, 336 MB 45 / 34, 604 MB 49 / 52.
+bool apart(const gqa_prefix_attn_args * a) {
+    return a->n_prefix > 0 && (a->n_workgroups > 0 || 2.0 * a->n_seq * a->bt_stride * PAGE * a->n_head_kv * (a->dk + a->dv) >= (double) (1 << 28));
 }
 size_t shared_bytes(const gqa_prefix_attn_args * a) { return (2 * (size_t) a->n_seq * 4 + 255) & ~(size_t) 255; }
 
@@ -136,14 +145,14 @@ extern "C" int gqa_prefix_attn_check(const gqa_prefix_attn_args * a) {
 extern "C" size_t gqa_prefix_attn_workspace_size(const gqa_prefix_attn_args * a) {
     if (gqa_prefix_attn_check(a) || a->n_seq == 0) return 0;
     const gqa_attn_args t = attn_of(a);
-    return a->n_prefix == 0 ? gqa_attn_workspace_size(&t) : batch_plan(call_of(a), true).bytes + shared_bytes(a) + attn_behind_size(&t);
+    return !apart(a) ? gqa_attn_workspace_size(&t) : batch_plan(call_of(a), true).bytes + shared_bytes(a) + attn_behind_size(&t);
 }
 extern "C" int gqa_prefix_attn_launch(const gqa_prefix_attn_args * a, void * stream) {
     const int rc = gqa_prefix_attn_check(a);
     if (rc || a->n_seq == 0) return rc;
     if (!a->workspace || ((uintptr_t) a->workspace & 255) || a->workspace_size < gqa_prefix_attn_workspace_size(a)) return MLA_ERR_WORKSPACE;
     const gqa_attn_args t = attn_of(a);
-    if (a->n_prefix == 0) return gqa_attn_launch(&t, stream);
+    if (!apart(a)) return gqa_attn_launch(&t, stream);
     const BatchCall   c  = call_of(a);
     const BatchPlan   pl = batch_plan(c, true);
     const hipStream_t st = (hipStream_t) stream;

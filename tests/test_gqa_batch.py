@@ -139,10 +139,23 @@ def test_prefix_accepts():
     _accepted("gqa_prefix_attn", _prefix, [kw for kw in COMMON_ACCEPTED if not {"n_tok", "q_starts"} & set(kw)] + [dict(n_prefix=0), dict(n_prefix=0, prefix_starts=None, prefix_lens=None), dict(n_prefix=100)])
 
 
+def test_prefixes_are_worked_on_by_themselves_where_the_table_has_room_for_many_rows():
+    """Scratch of the prefixes' pieces from 2^28 bytes of rows on, or where the workgroups are given; else of gqa_attn alone."""
+    lib = J.library()
+    size = lambda **kw: lib.gqa_prefix_attn_workspace_size(C.byref(_prefix(**kw)))
+    a = _prefix()
+    page = a.n_seq * 128 * a.n_head_kv * (a.dk + a.dv) * 2
+    least = -(-2 ** 28 // page)
+    for stride in (1, least - 1, least, least + 1):
+        alone = size(bt_stride=stride, n_prefix=0)
+        assert (size(bt_stride=stride) > alone) == (stride >= least)
+        assert size(bt_stride=stride, n_workgroups=16) > size(bt_stride=stride, n_workgroups=16, n_prefix=0)
+
+
 def test_launches_of_more_threads_than_there_are_refused():
     """Nothing starts of a call whose last kernel could not: 2^24 workgroups of 256 threads, one a block."""
     lib = J.library()
-    a = _prompt(n_tok=(1 << 28) - 1, n_head=7, n_head_kv=1, dk=256, dv=256)
+    a = _prompt(n_tok=(1 << 28) - 1, n_head=8, n_head_kv=1, dk=256, dv=256)
     assert lib.gqa_prompt_attn_check(C.byref(a)) == SHAPE
     a.n_tok = 1 << 24
     assert lib.gqa_prompt_attn_check(C.byref(a)) == 0

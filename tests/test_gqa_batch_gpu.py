@@ -407,18 +407,26 @@ def _shared(seed, groups, own, heads, kv_heads, dk, dv, dtype, layout="cells", b
     return q, k, v, bt, torch.tensor(lens, dtype=torch.int32), starts, torch.tensor([p for _, p in groups], dtype=torch.int32)
 
 
+def _wide(bt, k, v):
+    """A block table with room for 2^28 bytes of rows, pages that are none behind those it has: the prefixes are worked on by themselves."""
+    row = k.shape[2] * (k.shape[3] + v.shape[3]) * 2
+    width = -(-2 ** 28 // (bt.shape[0] * 128 * row))
+    return torch.cat([bt, torch.full((bt.shape[0], max(0, width - bt.shape[1])), -1, dtype=torch.int32, device=bt.device)], 1)
+
+
 def _prefix(gpu, q, k, v, bt, lens, starts, plens, nan=(), **kw):
-    """nan: sequences that see a NaN."""
+    """Twice, with a block table that has little room and one that has much.  nan: sequences that see a NaN."""
     import jittorinfer_amd as J
     scale = 1 / math.sqrt(q.shape[2])
     each = torch.arange(len(lens) + 1)
     want, off = B.prompt(q, k, v, bt, lens, each, scale, kw.get("logit_softcap", 0.0), 0, True, kw.get("mask"))
     d = {n: (t.to(gpu) if isinstance(t, torch.Tensor) else t) for n, t in kw.items()}
-    got = J.gqa_prefix_attn(*[t.to(gpu) for t in (q, k, v, bt, lens, starts, plens)], scale=scale, **d)
-    torch.cuda.synchronize()
     fine = [b for b in range(len(lens)) if b not in nan]
-    assert torch.isnan(got[list(nan)]).all() and torch.isnan(want[list(nan)]).all()
-    _near(got[fine], want[fine], off[fine], q.dtype)
+    for table in (bt, _wide(bt, k, v)):
+        got = J.gqa_prefix_attn(*[t.to(gpu) for t in (q, k, v, table, lens, starts, plens)], scale=scale, **d)
+        torch.cuda.synchronize()
+        assert torch.isnan(got[list(nan)]).all() and torch.isnan(want[list(nan)]).all()
+        _near(got[fine], want[fine], off[fine], q.dtype)
     return got
 
 
@@ -502,7 +510,7 @@ def test_prefix_mask_and_cap(gpu, dk, dv, dtype):
     mask[b0:b0 + 4, at] = 0.0
     mask[b0, at] = mask[b0 + 2, at] = float("-inf")
     v[bt[b0, at // 128].long(), at % 128] = float("inf")
-    got = J.gqa_prefix_attn(*[t.to(gpu) for t in (q, k, v, bt, lens, starts, plens)], scale=0.1, mask=mask.to(gpu)).cpu()
+    got = J.gqa_prefix_attn(*[t.to(gpu) for t in (q, k, v, _wide(bt, k, v), lens, starts, plens)], scale=0.1, mask=mask.to(gpu)).cpu()
     assert (got[b0 + 1] == float("inf")).all() and (got[b0 + 3] == float("inf")).all()
     for b in set(range(12)) - {b0 + 1, b0 + 3}:
         assert torch.isfinite(got[b]).all(), b
@@ -512,7 +520,7 @@ def test_prefix_bad_pages(gpu):
     q, k, v, bt, lens, starts, plens = _shared(9, [(3, 512), (2, 300)], [100, 3, 50, 9, 200, 10], 4, 2, 64, 64, BF16)
     bt[:3, 1], bt[4, 2], bt[5] = -1, k.shape[0], 10 ** 9
     import jittorinfer_amd as J
-    got = J.gqa_prefix_attn(*[t.to(gpu) for t in (q, k, v, bt, lens, starts, plens)], scale=0.125)
+    got = J.gqa_prefix_attn(*[t.to(gpu) for t in (q, k, v, _wide(bt, k, v), lens, starts, plens)], scale=0.125)
     # the shared rows of the page that sequence 4 lacks are read through sequence 3's table; its own ones of that page, 300 .. 383, count as masked
     own, mask = bt.clone(), torch.zeros((6, bt.shape[1] * 128), dtype=F16)
     own[4, 2] = bt[3, 2]
@@ -533,6 +541,8 @@ def test_prefix_is_gqa_attn(gpu):
     q, k, v, bt, lens, starts, plens = (t.to(gpu) for t in _shared(11, GROUPS, OWN, 8, 2, 128, 128, BF16, before=1))
     a = J.gqa_attn(q, k, v, bt, lens, scale=0.1)
     assert torch.equal(a, J.gqa_prefix_attn(q, k, v, bt, lens, starts[:1], plens[:0], scale=0.1))
+    assert torch.equal(a, J.gqa_prefix_attn(q, k, v, bt, lens, starts, plens, scale=0.1))       # (a table with little room)
+    bt = _wide(bt, k, v)
     b = J.gqa_prefix_attn(q, k, v, bt, lens, starts, plens, scale=0.1)
     assert (a.double() - b.double()).abs().max() < 2.0 ** -6 * v[torch.isfinite(v)].abs().max().double()
     assert torch.equal(b, J.gqa_prefix_attn(q, k, v, bt, lens, starts, plens, scale=0.1))

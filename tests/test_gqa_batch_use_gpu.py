@@ -6,21 +6,23 @@ import torch
 
 from tests import gqa_batch_util as B
 from tests import gqa_util as R
-from tests.test_gqa_batch_gpu import GROUPS, NAN, OWN, _case, _shared, _starts, _states
+from tests.test_gqa_batch_gpu import GROUPS, NAN, OWN, _case, _shared, _starts, _states, _wide
 from tests.test_gqa_gpu import BF16, F16, _near
 
 pytestmark = pytest.mark.gpu
 
 
 def _calls(gpu, seed=0, dtype=BF16):
-    """One call of each operator: (call(out=, stream=), what it gives)."""
+    """One call of each operator and form: (call(out=, stream=), what it gives)."""
     import jittorinfer_amd as J
     p = [t.to(gpu) for t in _case(30 + seed, [70, 1, 200, 33], [300, 128, 500, 900], 8, 8, 2, 128, 128, dtype)]
     x = [t.to(gpu) for t in _states(31 + seed, [40, 1, 129], [700, 30, 900], 8, 2, 64, 64, dtype)]
     one = [t.to(gpu) for t in _states(32 + seed, [1] * 6, [700, 30, 900, 0, 128, 500], 8, 8, 64, 64, dtype)]
     s = [t.to(gpu) for t in _shared(33 + seed, GROUPS, OWN, 8, 2, 128, 128, dtype, before=1)]
+    far = _wide(s[3], s[1], s[2])
     calls = [lambda **kw: J.gqa_prompt_attn(*p, scale=0.1, **kw), lambda **kw: J.gqa_cross_attn(*x[:3], q_starts=x[3], kv_lens=x[4], scale=0.1, **kw),
-             lambda **kw: J.gqa_cross_attn(*one[:3], kv_lens=one[4], scale=0.1, **kw), lambda **kw: J.gqa_prefix_attn(*s, scale=0.1, **kw)]
+             lambda **kw: J.gqa_cross_attn(*one[:3], kv_lens=one[4], scale=0.1, **kw), lambda **kw: J.gqa_prefix_attn(*s, scale=0.1, **kw),
+             lambda **kw: J.gqa_prefix_attn(*s[:3], far, *s[4:], scale=0.1, **kw)]
     return [(c, c()) for c in calls]
 
 
@@ -125,6 +127,7 @@ def test_groups_change_under_a_graph(gpu):
     import jittorinfer_amd as J
     case = _shared(41, [(4, 512), (4, 300)], [5, 9, 0, 30, 200, 1, 77, 3, 50], 8, 2, 64, 64, F16)
     d = [t.to(gpu) for t in case]
+    d[3] = _wide(d[3], d[1], d[2])
     out = torch.empty((9, 8, 64), dtype=F16, device=gpu)
     J.gqa_prefix_attn(*d, scale=0.125, out=out)
     torch.cuda.synchronize()
@@ -237,9 +240,9 @@ def test_a_serving_loop_with_a_shared_prompt(gpu, dtype):
         q, bt, lens = feed(seqs, [1] * len(seqs))
         starts, plens = pt.shared_prefixes(seqs)
         assert max(plens) >= 384
-        got = J.gqa_prefix_attn(q, kc, vc, i32(bt), i32(lens), i32(starts), i32(plens), scale=SCALE)
         want, off = B.prompt(q.cpu(), kc.cpu(), vc.cpu(), torch.from_numpy(bt), lens.tolist(), torch.arange(len(seqs) + 1), SCALE)
-        _near(got, want, off, dtype, "step")
+        for table in (i32(bt), _wide(i32(bt), kc, vc)):
+            _near(J.gqa_prefix_attn(q, kc, vc, table, i32(lens), i32(starts), i32(plens), scale=SCALE), want, off, dtype, "step")
         return starts.tolist(), plens.tolist()
 
     prompt([0], [300])
@@ -277,7 +280,7 @@ def test_offsets_past_32_bits(gpu):
     each = torch.arange(3, dtype=torch.int32)
     want, off = B.prompt(q[:2], k, v, bt, lens, each, 0.1)
     for group, shared in (([0, 1, 2], [300, 0]), ([0, 1], [256])):
-        got = J.gqa_prefix_attn(q[:2].to(gpu), *big, table, lens.to(gpu), torch.tensor(group, dtype=torch.int32, device=gpu), torch.tensor(shared, dtype=torch.int32, device=gpu), scale=0.1)
+        got = J.gqa_prefix_attn(q[:2].to(gpu), *big, _wide(table, k, v), lens.to(gpu), torch.tensor(group, dtype=torch.int32, device=gpu), torch.tensor(shared, dtype=torch.int32, device=gpu), scale=0.1)
         _near(got, want, off, BF16)
     # the same memory as packed states, rows of 2 KB
     flat = [b.view(-1, 8, 128) for b in big]
