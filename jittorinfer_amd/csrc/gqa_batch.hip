@@ -67,8 +67,8 @@ int mla::gqa::batch_check(const BatchCall & c) {
     if (!c.q || !c.dst) return MLA_ERR_NULL;
     if (!c.q_starts && c.n_tok % c.n_seq) return MLA_ERR_BAD_SHAPE;
     if (c.cap >= (int64_t) 1 << 30 || (int64_t) c.n_tok * c.n_head >= (int64_t) 1 << 31 || c.n_head_kv > 65535) return MLA_ERR_BAD_SHAPE;
-    int rc = check_pool(c.k);
-    if (!rc) rc = check_pool(c.v);
+    int rc = c.cap ? check_pool(c.k) : 0;                          // (states of no row need not lie anywhere)
+    if (!rc && c.cap) rc = check_pool(c.v);
     if (rc) return rc;
     if (!al16(c.q) || (c.q_nb1 & 15) || (c.q_nb2 & 15) || ((uintptr_t) c.dst & 7) || (c.d_nb1 & 7) || (c.d_nb2 & 7)) return MLA_ERR_BAD_ALIGNMENT;
     if (c.mask) {

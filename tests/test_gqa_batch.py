@@ -132,7 +132,7 @@ def test_prompt_accepts():
 
 
 def test_cross_accepts():
-    _accepted("gqa_cross_attn", _cross, COMMON_ACCEPTED + [dict(n_kv=0), dict(kv_lens=8192), dict(kv_starts=8192, k__nb_page=0, v__nb_page=0), dict(k__nb_page=1 << 40)])
+    _accepted("gqa_cross_attn", _cross, COMMON_ACCEPTED + [dict(n_kv=0), dict(n_kv=0, k__data=None, v__data=None), dict(kv_lens=8192), dict(kv_starts=8192, k__nb_page=0, v__nb_page=0), dict(k__nb_page=1 << 40)])
 
 
 def test_prefix_accepts():

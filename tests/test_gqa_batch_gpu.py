@@ -355,6 +355,20 @@ def test_cross_lengths_and_starts_out_of_range(gpu):
     assert (got[:13] == 0).all() and (got[13:] != 0).any()
 
 
+def test_cross_without_states(gpu):
+    """No row at all, padded and packed: zeros."""
+    import jittorinfer_amd as J
+    for new in (1, 50):
+        q = torch.randn((2 * new, 4, 64), device=gpu).to(F16)
+        none = torch.empty((2, 0, 2, 64), dtype=F16, device=gpu)
+        zero = torch.zeros(3, dtype=torch.int32, device=gpu)
+        for kw in (dict(), dict(kv_lens=zero[:2]), dict(logit_softcap=9.0)):
+            out = torch.full_like(q, NAN)
+            assert (J.gqa_cross_attn(q, none, none, scale=0.1, out=out, **kw) == 0).all()
+        out = torch.full_like(q, NAN)
+        assert (J.gqa_cross_attn(q, none[0], none[0], kv_starts=zero, scale=0.1, out=out) == 0).all()
+
+
 @pytest.mark.parametrize("new", [1, 20])
 def test_cross_strides(gpu, new):
     """States with heads outermost, expanded over the heads or over the sequences, out given."""
