@@ -20,7 +20,7 @@
 // bf16, TFLOP/s without anything / with a mask / with a soft cap: heads of 64 596 / 463 / 388 (twice the exponentials a product), 128 909 / 745 / 669, 192 875 / 644 /
 // 613, 256 532 / 432 / 421 (one wave a SIMD: 512 registers); f16 of 64 667.  One prompt of 16384 tokens, heads of 128: 2.1 ms, 1.04 PFLOP/s, where an 8192 x 8192 x 8192 library
 // product reaches 1.20; its matrix units are busy 44 % of the time at a clock of 2.0 GHz, and LDS has no bank conflicts.  Fewer rows than 128 a block are bound by what a
-// run waits for: 8 tokens behind 4000 rows 15 us here and 5 in the join, of which 3.2 would be the bytes.
+// run waits for: 8 tokens behind 4000 rows 18 us here and 5 in the join, of which 3.2 would be the bytes.
 #pragma once
 
 #include <limits.h>
