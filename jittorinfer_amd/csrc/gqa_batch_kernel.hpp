@@ -18,7 +18,7 @@
 // What bounds it: the matrix units with the exponentials between their products (a tile of 64 keys of heads of 128: 64 MFMAs of 16 cycles a wave, and 32 exponentials,
 // 16 roundings of pairs and as many sums beside some 250 other vector instructions; two waves a SIMD, each in the other's gaps).  Prompts of 4 x 4096 tokens, 32 heads on 8,
 // bf16, TFLOP/s without anything / with a mask / with a soft cap: heads of 64 596 / 463 / 388 (twice the exponentials a product), 128 909 / 745 / 669, 192 875 / 644 /
-// 613, 256 532 / 432 / 421 (one wave a SIMD: 512 registers); f16 of 64 667.  One prompt of 16384 tokens, heads of 128: 2.1 ms, 1.04 PFLOP/s, where an 8192 x 8192 x 8192 library
+// 613, 256 594 / 432 / 466 (one wave a SIMD: 512 registers); f16 of 64 667.  One prompt of 16384 tokens, heads of 128: 2.1 ms, 1.04 PFLOP/s, where an 8192 x 8192 x 8192 library
 // product reaches 1.20; its matrix units are busy 44 % of the time at a clock of 2.0 GHz, and LDS has no bank conflicts.  Fewer rows than 128 a block are bound by what a
 // run waits for: 8 tokens behind 4000 rows 18 us here and 5 in the join, of which 3.2 would be the bytes.
 #pragma once
@@ -247,6 +247,11 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
     constexpr int NW = NWQ * NWK, BM = 32 * NWQ, KW = TK / NWK, KB = KW / 32, KC = DK / 16, NV = DV / 32;
     constexpr int KT = TK * DK * 2, VT = TK * DV * 2, KI = KT / 1024 / NW, VI = VT / 1024 / NW;
     static_assert(KW % 32 == 0 && KI * 1024 * NW == KT && VI * 1024 * NW == VT, "whole pieces");
+    // One wave a SIMD has nobody to fill its gaps: the scores' products of the next tile lie among what is done to this tile's scores.  Without / with that: 6 x 700 tokens,
+    // window and cap 188 / 172 us; 4 x 4096 tokens 532 / 594 TFLOP/s, with a cap 421 / 466.  (Narrower heads: two waves a SIMD, and no registers for it.  A mask would be needed
+    // for two tiles at a time.)
+    constexpr bool NEXT = DK == 256 && NWK == 1 && EXTRA != MASK;
+    static_assert(!NEXT || (KB == 1 && KC == 16 && NS > 2), "a score beside each product, two tiles there at a time");
     constexpr float REF = F16 ? 11.f : 0.f, SLACK = F16 ? 4.f : 8.f;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     __shared__ float2 sh_ml[NWK > 1 ? NW : 1][NWK > 1 ? 32 : 1];
@@ -489,6 +494,33 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                 __builtin_amdgcn_sched_group_barrier(0x008, LEAD, 0);
             };
 
+            f32x16 next;                                              // NEXT: the scores of the tile that comes
+            // something for every score of a tile, each(0 .. KB * 16 - 1); NEXT: beside the products of the tile at kn, keys read LEAD products ahead
+            auto beside = [&](unsigned kn, auto && each) {
+                if constexpr (NEXT) {
+                    constexpr int LEAD = 4;
+                    unsigned at[KP];
+                    u32x4    kf[LEAD];
+#pragma unroll
+                    for (int c = 0; c < KP; c++) at[c] = base_of(kn + k_lo[c]);
+                    auto key = [&](int c) { return lds128(at[c % KP] + c / KP * KP * 32); };
+#pragma unroll
+                    for (int c = 0; c < LEAD; c++) kf[c] = key(c);
+#pragma unroll
+                    for (int e = 0; e < 16; e++) next[e] = 0.f;
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int c = 0; c < KC; c++) {
+                        next = mfma32<F16>(kf[c % LEAD], qf[c], next);
+                        if (c + LEAD < KC) kf[c % LEAD] = key(c + LEAD);
+                        each(c);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                } else
+#pragma unroll
+                    for (int i = 0; i < KB * 16; i++) each(i);
+            };
+
             for (;;) {
                 m = -INFINITY; l = 0.f;
 #pragma unroll
@@ -506,9 +538,16 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
 #pragma unroll
             for (int i = 0; i < NS - 1; i++) if (t0 + i < t1) fetch(t0 + i, ids[i], i);
             int buf = 0;
+            if constexpr (NEXT) {
+                if (t0 + NS - 2 < t1) dma_wait<(NS - 2) * (KI + VI)>();
+                else                  dma_wait<0>();
+                __syncthreads();
+                beside(uni(lds0), [](int) {});
+            }
             for (int t = t0; t < t1; t++) {
-                if (NS > 2 && t + NS - 2 < t1) dma_wait<(NS - 2) * (KI + VI)>();
-                else                           dma_wait<0>();
+                constexpr int AHEAD = NS - 2 - NEXT;                  // tiles that need not be there yet
+                if (AHEAD > 0 && t + NS - 2 < t1) dma_wait<AHEAD * (KI + VI)>();
+                else                              dma_wait<0>();
                 __syncthreads();
                 const int  key0 = t * TK + wk * KW;
                 const bool use = !paged || good(ids[0]);
@@ -516,6 +555,7 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
 #pragma unroll
                 for (int i = 0; i + 1 < NS; i++) ids[i] = ids[i + 1];
                 if (paged && t + NS < t1) ids[NS - 1] = page_at(t + NS);
+                const unsigned kn = uni(lds0 + (buf + 1 == NS ? 0 : buf + 1) * (KT + VT));                                   // (behind the last tile: what was there)
                 const unsigned kt = uni(lds0 + buf * (KT + VT) + wk * KW * (DK * 2)), vt = uni(lds0 + buf * (KT + VT) + KT + wk * KW * (DV * 2));
                 if (safe && ((EXTRA != NOTHING && masks) || t * TK < b_last.first || t * TK + TK > b_first.last)) {
                     unsigned bad = 0;
@@ -568,15 +608,13 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                 if (use && key0 < s_last.last && key0 + KW > s_first.first) {
                     f32x16 sc[KB];
                     u32x4  pf[KB][2];
-                    products(kt, sc);
+                    if constexpr (NEXT) sc[0] = next;
+                    else                products(kt, sc);
                     float top, unit = scale_log2;                   // what makes log2 units of sc
                     const bool all = key0 + KW <= s_first.last && key0 >= s_last.first;
                     if (EXTRA != CAP && all && !(EXTRA == MASK && safe)) {
                         top = sc[0][0];
-#pragma unroll
-                        for (int b = 0; b < KB; b++)
-#pragma unroll
-                            for (int e = 0; e < 16; e++) top = fmaxf(top, sc[b][e]);
+                        beside(kn, [&](int i) { top = fmaxf(top, sc[i >> 4][i & 15]); });
                         top *= unit;
                     } else {
                         top = -INFINITY;
@@ -591,25 +629,13 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                             small = cap_out != 0.f && !uni(__any(!(most * cap_in < 0.25f)));
                         }
                         // (a pass over the scores for each thing that is done to them, none with a branch in it)
-                        if (EXTRA == CAP && small) {
-#pragma unroll
-                            for (int b = 0; b < KB; b++)
-#pragma unroll
-                                for (int e = 0; e < 16; e++) {
-                                    const float y = cap_in * sc[b][e], u = y * y;
-                                    sc[b][e] *= scale_log2 * fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, -1382.f / 155925, 62.f / 2835), -17.f / 315), 2.f / 15), -1.f / 3), 1.f);
-                                }
-                        } else if (EXTRA == CAP && cap_out != 0.f) {
-#pragma unroll
-                            for (int b = 0; b < KB; b++)
-#pragma unroll
-                                for (int e = 0; e < 16; e++) sc[b][e] = capped_score(scale_log2, cap_in, cap_out, sc[b][e]);
-                        } else {
-#pragma unroll
-                            for (int b = 0; b < KB; b++)
-#pragma unroll
-                                for (int e = 0; e < 16; e++) sc[b][e] *= scale_log2;
-                        }
+                        if (EXTRA == CAP && small)
+                            beside(kn, [&](int i) {
+                                const float x = sc[i >> 4][i & 15], y = cap_in * x, u = y * y;
+                                sc[i >> 4][i & 15] = x * (scale_log2 * fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, -1382.f / 155925, 62.f / 2835), -17.f / 315), 2.f / 15), -1.f / 3), 1.f));
+                            });
+                        else if (EXTRA == CAP && cap_out != 0.f) beside(kn, [&](int i) { sc[i >> 4][i & 15] = capped_score(scale_log2, cap_in, cap_out, sc[i >> 4][i & 15]); });
+                        else beside(kn, [&](int i) { sc[i >> 4][i & 15] *= scale_log2; });
                         if (EXTRA == CAP ? mask != nullptr : EXTRA == MASK && safe)
 #pragma unroll
                             for (int b = 0; b < KB; b++)
@@ -682,7 +708,10 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
-                else if (EXTRA != NOTHING && t + 1 < t1) fetch_mask(t + 1);
+                else {
+                    if (EXTRA != NOTHING && t + 1 < t1) fetch_mask(t + 1);
+                    if constexpr (NEXT) beside(kn, [](int) {});
+                }
                 buf = buf + 1 == NS ? 0 : buf + 1;
             }
                 if (safe) break;
