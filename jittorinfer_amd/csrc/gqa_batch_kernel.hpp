@@ -15,15 +15,17 @@
 // sums), and the workgroups take equal runs of the total weight, cut at tiles.  A run that covers a block writes its result; the others leave (o, m, l)
 // for gqa_batch_join_kernel.  All of that is decided from the lengths on the device: a captured launch stays valid while they change.
 //
-// What bounds it: the matrix units with the exponentials between their products (a tile of 64 keys of heads of 128: 64 MFMAs of 16 cycles a wave, and 32 exponentials,
-// 16 roundings of pairs and as many sums beside some 250 other vector instructions; two waves a SIMD, each in the other's gaps).  Prompts of 4 x 4096 tokens, 32 heads on 8,
-// bf16, TFLOP/s without anything / with a mask / with a soft cap: heads of 64 596 / 463 / 388 (twice the exponentials a product), 128 909 / 745 / 669, 192 875 / 644 /
-// 613, 256 594 / 432 / 466 (one wave a SIMD: 512 registers); f16 of 64 667.  One prompt of 16384 tokens, heads of 128: 2.1 ms, 1.04 PFLOP/s, where an 8192 x 8192 x 8192 library
+// What bounds it: the matrix units with the vector work between their products (a tile of 64 keys of heads of 128: 32 MFMAs of 32 cycles a wave, and 32 exponentials
+// of 16 cycles with some 90 other instructions of 4; two waves a SIMD, each in the other's gaps; of heads of 64: as much vector work to half the MFMAs, so 700 TFLOP/s at best).  Prompts of 4 x 4096 tokens, 32 heads on 8,
+// bf16, TFLOP/s without anything / with a mask / with a soft cap: heads of 64 596 / 477 / 388 (twice the exponentials a product), 128 909 / 775 / 669, 192 875 / 662 /
+// 613, 256 594 / 437 / 466 (one wave a SIMD: 512 registers); f16 of 64 667.  One prompt of 16384 tokens, heads of 128: 2.1 ms, 1.04 PFLOP/s, where an 8192 x 8192 x 8192 library
 // product reaches 1.20; its matrix units are busy 44 % of the time at a clock of 2.0 GHz, and LDS has no bank conflicts.  Fewer rows than 128 a block are bound by what a
 // run waits for: 8 tokens behind 4000 rows 18 us here and 5 in the join, of which 3.2 would be the bytes.
 #pragma once
 
 #include <limits.h>
+
+#include <type_traits>
 
 #include "gqa_batch.hpp"
 
@@ -462,7 +464,7 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
             bool safe = false;
 
             // S^T of the wave's keys; a mask is where the sums begin (in units of the products)
-            auto products = [&](unsigned kt, f32x16 (&sc)[KB]) {
+            auto products = [&](unsigned kt, f32x16 (&sc)[KB], auto with_mask) {
                 unsigned at[KP];
 #pragma unroll
                 for (int c = 0; c < KP; c++) at[c] = base_of(kt + k_lo[c]);
@@ -471,12 +473,11 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                 for (int b = 0; b < KB; b++)
 #pragma unroll
                     for (int e = 0; e < 16; e++) start[b][e] = 0.f;
-                if constexpr (EXTRA == MASK)
-                    if (!safe)
+                if constexpr (decltype(with_mask)::value)
 #pragma unroll
-                        for (int b = 0; b < KB; b++)
+                    for (int b = 0; b < KB; b++)
 #pragma unroll
-                            for (int e = 0; e < 16; e++) start[b][e] = masked_by(b, e) * mask_unit;
+                        for (int e = 0; e < 16; e++) start[b][e] = fmaf((float) bitcast<f16x2>(mk[b][e >> 2][(e >> 1) & 1])[e & 1], mask_unit, 0.f);   // (one instruction, converting; a product alone is two)
 #pragma unroll
                 for (int b = 0; b < KB; b++) {
                     sc[b] = start[b];
@@ -608,8 +609,9 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
                 if (use && key0 < s_last.last && key0 + KW > s_first.first) {
                     f32x16 sc[KB];
                     u32x4  pf[KB][2];
-                    if constexpr (NEXT) sc[0] = next;
-                    else                products(kt, sc);
+                    if constexpr (NEXT)              sc[0] = next;
+                    else if (EXTRA == MASK && !safe) products(kt, sc, std::bool_constant<EXTRA == MASK>());
+                    else                             products(kt, sc, std::false_type());
                     float top, unit = scale_log2;                   // what makes log2 units of sc
                     const bool all = key0 + KW <= s_first.last && key0 >= s_last.first;
                     if (EXTRA != CAP && all && !(EXTRA == MASK && safe)) {
