@@ -98,7 +98,8 @@ int    gqa_cross_attn_launch(const gqa_cross_attn_args * args, void * stream);
 /* ---- one new token of every sequence, where sequences share their first rows
  * What gqa_attn (include/gqa_attn.h) answers, with the shared rows read once a group.  Group g is the sequences prefix_starts[g] .. prefix_starts[g + 1] - 1 of the batch, side
  * by side; their first prefix_lens[g] rows hold the same keys and values, and are read through the block table of the first of them (rows of a page that is not
- * shared whole, too) or, where the table has room for so few rows that reading them once does not pay (and n_workgroups is 0), through each one's own.  A sequence
+ * shared whole, too: that table names all of the prefix's pages, whatever the length of the first) or, where the table has room for so few rows that reading them once does not
+ * pay, or there are as many groups as sequences (and n_workgroups is 0), through each one's own.  A sequence
  * shorter than its group's prefix sees what it has of it; sequences outside [prefix_starts[0], prefix_starts[n_prefix]) share nothing.  Numbers in prefix_starts are
  * taken to lie in [0, n_seq] and never fall; lengths of prefixes count as seq_lens do.
  */

@@ -124,8 +124,11 @@ gqa_attn_args attn_of(const gqa_prefix_attn_args * a) {
 // and again, for less than the two further launches take.  us, prefixes by themselves / gqa_attn, 512 .. 8192 shared rows and 200 own ones a user, 32 heads on 8 of 128:
 // 4 users with room for 13 MB 31 / 12, 38 MB 30 / 15, 138 MB 37 / 30; 16 of one group 50 MB 31 / 15, 151 MB 34 / 26, 285 MB 36 / 38, 554 MB 35 / 86; 64 of 8 groups 201 MB 40 / 31, 336 MB
 // 41 / 47, 604 MB 42 / 93; 16 on 4 of 64: 138 MB 27 / 25, 285 MB 32 / 36, 554 MB 36 / 61; 16 on 4 of 256: 151 MB 42 / 28, 285 MB 44 / 46, 336 MB 45 / 34, 604 MB 49 / 52.
+// So with as many groups as sequences, none of which has two then (or others have none): 64 users alone with 2000 rows each 109 / 100, 40 / 31 (16 on 4 of 64), 110 / 98 (of 256); one
+// user's 100000 rows 122 / 87, 26 / 26, 104 / 82.
 bool apart(const gqa_prefix_attn_args * a) {
-    return a->n_prefix > 0 && (a->n_workgroups > 0 || 2.0 * a->n_seq * a->bt_stride * PAGE * a->n_head_kv * (a->dk + a->dv) >= (double) (1 << 28));
+    if (a->n_workgroups > 0) return a->n_prefix > 0;
+    return a->n_prefix > 0 && a->n_prefix < a->n_seq && 2.0 * a->n_seq * a->bt_stride * PAGE * a->n_head_kv * (a->dk + a->dv) >= (double) (1 << 28);
 }
 size_t shared_bytes(const gqa_prefix_attn_args * a) { return (2 * (size_t) a->n_seq * 4 + 255) & ~(size_t) 255; }
 
