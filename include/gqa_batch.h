@@ -17,7 +17,8 @@
  *   s_i = scale * (q . k_i), with a soft cap c > 0 (any finite one): c * tanh(s_i / c), with a mask: + mask[b][i] of the token's sequence b.
  * A mask of -inf takes the row out whatever its key and value hold (NaN, infinities), and so do all rules of what a token sees; a row past the mask's end is out
  * too.  A token that sees no row gets zeros.  Queries, keys, values and results are of one 16-bit type; scores, maxima and sums are f32, the
- * weights p are rounded to that type (relative to a reference near the row's maximum) for the second product, as the result is after it.
+ * weights p are rounded to that type (relative to a reference near the row's maximum) for the second product, as the result is after it.  A mask's number is where
+ * a score's sum begins: a score is off by up to 2^-13 (bf16: 2^-10) of log2 units for it, or by half a step of the score where it is too large for that.
  * Supported widths (dk, dv): (64, 64), (128, 128), (192, 128), (256, 256).
  * The result lies apart from all that is read.
  */

@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
     // for two tiles at a time.)
     constexpr bool NEXT = DK == 256 && NWK == 1 && EXTRA != MASK;
     static_assert(!NEXT || (KB == 1 && KC == 16 && NS > 2), "a score beside each product, two tiles there at a time");
-    constexpr float REF = F16 ? 11.f : 0.f, SLACK = F16 ? 4.f : 8.f;
+    constexpr float REF = F16 ? 11.f : 0.f, SLACK = F16 ? 4.f : 8.f, MOST = F16 ? 32768.f / DK : 1024.f;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     __shared__ float2 sh_ml[NWK > 1 ? NW : 1][NWK > 1 ? 32 : 1];
     __shared__ int    sh_bad[2][NW];
@@ -459,7 +459,8 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
             // Infinities and NaN among keys and values must not count where a row does not see them, and 0 * them does.  The piece is worked on as if there were none; if a result
             // is not finite, once more from the start, `safe`: with the infinities and NaN among the values of every tile that not all rows see whole noted for the rows that
             // see them, and taken for zeros, and with masked scores set and not added to.  So is a piece whose largest scores come of a large finite number of the mask: sums that
-            // begin with one of size x lose up to dk / 16 half steps of it (2^-20 x), added last it costs a single one.
+            // begin with one of size x lose up to dk / 16 half steps of it (2^-20 x for heads of 256), added last it costs a single one.  Up to `MOST` that is no more than 2^-13
+            // of a score in log2 units for f16, 2^-10 for bf16: less than a fifth of what the weights' own rounding is off by.
             unsigned up[(NV + 1) / 2], down[(NV + 1) / 2];            // safe: results that a +infinity (-infinity, NaN: both) belongs to
             bool safe = false;
 
@@ -718,7 +719,7 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, OCC) gqa_batch_kernel(const Ba
             }
                 if (safe) break;
                 float odd = l * 0.f;                                  // NaN if anything is not finite
-                if (EXTRA == MASK && fabsf(m) > 1024.f && m != -INFINITY) odd = NAN;
+                if (EXTRA == MASK && fabsf(m + REF) > MOST - SLACK && m != -INFINITY) odd = NAN;
 #pragma unroll
                 for (int n = 0; n < NV; n++)
 #pragma unroll
