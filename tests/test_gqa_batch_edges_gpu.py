@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from tests import gqa_util as R
-from tests.test_gqa_batch_gpu import _shared, _wide
+from tests.test_gqa_batch_gpu import _case, _check, _prefix, _shared, _wide
 from tests.test_gqa_gpu import BF16, F16
 
 pytestmark = pytest.mark.gpu
@@ -55,3 +55,41 @@ def test_prompt_mask_of_one_number_on_every_row(gpu, number, dk, dv, dtype):
         q[:, 0, 1] = 1.0
         out = J.gqa_prompt_attn(q.to(gpu), k.to(gpu), v.to(gpu), bt, lens, scale=scale, causal=False, mask=mask)
         assert out.abs().max() <= off, (new, float(out.abs().max()) / off)
+
+
+@pytest.mark.parametrize("dk,dtype,heads", [(64, F16, 1600), (128, BF16, 1600), (256, BF16, 1600)])
+@pytest.mark.parametrize("new,rows", [(300, 300), (257, 400)])
+def test_prompt_of_one_sequence_with_blocks_for_all(gpu, dk, dtype, heads, new, rows):
+    """Four blocks and more for every workgroup that the card holds: one sequence's blocks are taken whole whatever its length, and no join is launched."""
+    assert new // 128 * heads >= 4 * 256 * 3                                 # (blocks of 128 rows of all KV heads; three workgroups a CU at most)
+    case = _case(new + dk, [new], [rows], -(-rows // 128), heads, heads, dk, dk, dtype)
+    _check(gpu, *case)
+
+
+def _many(gen, n_seq, long_at, long_rows, chunk):
+    """One new token of most sequences, none of some, behind a few rows; one sequence far back in the batch is longer than all others together."""
+    new = [1 if int(x) else 0 for x in torch.randint(0, 4, (n_seq,), generator=gen)]
+    lens = [n + int(x) for n, x in zip(new, torch.randint(0, 90, (n_seq,), generator=gen))]
+    new[long_at], lens[long_at] = chunk, long_rows
+    return new, lens
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("n_workgroups", [0, 1, 7, 64, 1000])
+@pytest.mark.parametrize("n_seq,long_at,long_rows,chunk", [(300, 299, 90, 1), (300, 130, 6000, 1), (129, 128, 5000, 40), (65, 64, 9000, 3), (200, 70, 4000, 300)])
+def test_prompt_runs_of_more_sequences_than_lanes(gpu, n_seq, long_at, long_rows, chunk, n_workgroups, causal):
+    """Equal runs that begin and end in any set of 64 sequences: of a given number of workgroups, or because one sequence is far longer than a share."""
+    gen = torch.Generator().manual_seed(n_seq)
+    new, lens = _many(gen, n_seq, long_at, long_rows, chunk)
+    _check(gpu, *_case(n_seq, new, lens, -(-max(lens) // 128), 4, 2, 64, 64, BF16), n_workgroups=n_workgroups, causal=causal)
+
+
+@pytest.mark.parametrize("n_workgroups", [0, 1, 7, 64, 1000])
+@pytest.mark.parametrize("dk,dtype", [(64, BF16), (128, F16)])
+def test_prefixes_of_more_groups_than_lanes(gpu, dk, dtype, n_workgroups):
+    """150 groups of one to four sequences, some without a shared row, one far back whose prefix is longer than all others together."""
+    gen = torch.Generator().manual_seed(dk)
+    groups = [(1 + int(m), [0, 77, 128, 200][int(p)]) for m, p in zip(torch.randint(0, 4, (150,), generator=gen), torch.randint(0, 4, (150,), generator=gen))]
+    groups[100] = (3, 5000)
+    own = [int(x) for x in torch.randint(0, 60, (2 + sum(m for m, _ in groups),), generator=gen)]
+    _prefix(gpu, *_shared(dk, groups, own, 4, 2, dk, dk, dtype, before=2), n_workgroups=n_workgroups)
