@@ -5,6 +5,8 @@ import pytest
 import torch
 
 from tests import gqa_util as R
+from tests.test_gqa_batch import CALLS
+from tests.test_gqa_batch_edges import REFUSED
 from tests.test_gqa_batch_gpu import _case, _check, _prefix, _shared, _wide
 from tests.test_gqa_gpu import BF16, F16
 
@@ -93,3 +95,20 @@ def test_prefixes_of_more_groups_than_lanes(gpu, dk, dtype, n_workgroups):
     groups[100] = (3, 5000)
     own = [int(x) for x in torch.randint(0, 60, (2 + sum(m for m, _ in groups),), generator=gen)]
     _prefix(gpu, *_shared(dk, groups, own, 4, 2, dk, dk, dtype, before=2), n_workgroups=n_workgroups)
+
+
+def test_python_entry_points_refuse_what_is_wrong(gpu):
+    """The calls of the same table on tensors that there are: the accepted ones run, a wrong result tensor is refused like any other, before a launch."""
+    source = CALLS.split("J.capi.native()\n")[0].replace("with FakeTensorMode():", "if True:").replace("torch.empty(", "torch.zeros(")
+    scope = {}
+    exec(source, scope)
+    assert set(scope["calls"]) == set(REFUSED)
+    for name, call in scope["calls"].items():
+        if name.endswith("_alloc"):
+            assert torch.isfinite(call()).all()
+            continue
+        with pytest.raises((AssertionError, TypeError, RuntimeError)) as e:
+            call()
+        kind, text = REFUSED[name] or ("AssertionError", "result.take(a, q, outp)")
+        assert type(e.value).__name__ == kind and text in str(e.value), (name, e.value)
+    torch.cuda.synchronize()
