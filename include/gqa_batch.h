@@ -102,7 +102,8 @@ int    gqa_cross_attn_launch(const gqa_cross_attn_args * args, void * stream);
  * shared whole, too: that table names all of the prefix's pages, whatever the length of the first) or, where the table has room for so few rows that reading them once does not
  * pay, or there are as many groups as sequences (and n_workgroups is 0), through each one's own.  A sequence
  * shorter than its group's prefix sees what it has of it; sequences outside [prefix_starts[0], prefix_starts[n_prefix]) share nothing.  Numbers in prefix_starts are
- * taken to lie in [0, n_seq] and never fall; lengths of prefixes count as seq_lens do.
+ * taken to lie in [0, n_seq] and never fall; lengths of prefixes count as seq_lens do.  Rows that are read through a sequence's own table are gqa_attn's in all (weights in several parts,
+ * as precise as f32; a result that an infinite value makes infinite may be NaN there).
  */
 typedef struct gqa_prefix_attn_args {
     int32_t n_seq, n_prefix, n_head, n_head_kv;

@@ -39,7 +39,9 @@ struct BatchP {
 // Blocks are dealt in equal runs, one to a workgroup, or the one or the other by what the device finds.  Runs cost pieces that are written, read again and joined: as
 // much as JOIN_KEYS keys of a block; whole blocks leave workgroups idle at the end.  Both sides, us (32 heads on 8 of 128, bf16, where no other is named): prompts of
 // 2 x 512 tokens 40 against 22, 4 x 1024 85 / 60, 1 x 4096 181 / 155, 4 x 1500 to 2048 178 / 141, 32 x 448 tokens over 1500 states (16 heads of 64) 174 / 143; 3 x
-// 600 to 1024 over 3000 to 8192 states 371 / 383, 8 x 512 behind 5000 to 16384 rows (16 on 4 of 64) 272 / 367.
+// 600 to 1024 over 3000 to 8192 states 371 / 383, 8 x 512 behind 5000 to 16384 rows (16 on 4 of 64) 272 / 367.  Wide heads, masks and caps, runs by 512 (256 for heads of 256) workgroups
+// against what is chosen, whole blocks: 2 x 3500 to 4096 tokens, 16 heads of 192, mask 271 / 234; 6 x 300 to 700, 16 on 4 of 256, cap and window 164 to 169 / 167 to 171; 8 x 100 to
+// 448 over 300 to 1500 states, 16 of 64, mask 49 to 52 / 53.  (One number for all: a key of heads of 256 costs four times one of 64, and so do its pieces.)
 enum Dealing { RUNS, EITHER, WHOLE };
 constexpr int JOIN_KEYS = 1280;
 
@@ -66,7 +68,8 @@ void      batch_fill(BatchP & p, const BatchCall & c, const BatchPlan & pl, char
 template <bool F16> hipError_t batch_launch(const BatchP & p, const BatchPlan & pl, int dk, hipStream_t st);
 
 // Workgroups of a shape that a CU holds, by its registers and its tiles in LDS (plain: no mask, no cap).  Heads of 64, three or two: 8 x 512 tokens behind 5000 to 16384 rows 302 or
-// 312 us; with a mask a third one's registers spill, 8 x 448 tokens over states 68 or 54 us.
+// 312 us, although the third one's 168 vector registers spill 36 (none among the products); with a mask more of them do, 8 x 448 tokens over states 68 or 54 us.  Blocks of 128 rows of
+// heads of 128 spill 14 of 256 with a mask, 19 with a cap (none among the products either); no other build spills any.
 constexpr int batch_wg_per_cu(int dk, Shape s, bool plain) { return s == FOUR_KEYS ? (dk <= 64 ? 2 : 1) : dk == 64 && plain ? 3 : dk <= 128 || (dk == 192 && s == FOUR_ROWS) ? 2 : 1; }
 
 }  // namespace gqa

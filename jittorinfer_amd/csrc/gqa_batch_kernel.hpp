@@ -15,11 +15,12 @@
 // sums), and the workgroups take equal runs of the total weight, cut at tiles.  A run that covers a block writes its result; the others leave (o, m, l)
 // for gqa_batch_join_kernel.  All of that is decided from the lengths on the device: a captured launch stays valid while they change.
 //
-// What bounds it: the matrix units with the vector work between their products (a tile of 64 keys of heads of 128: 32 MFMAs of 32 cycles a wave, and 32 exponentials
-// of 16 cycles with some 90 other instructions of 4; two waves a SIMD, each in the other's gaps; of heads of 64: as much vector work to half the MFMAs, so 700 TFLOP/s at best).  Prompts of 4 x 4096 tokens, 32 heads on 8,
+// What bounds it: the matrix units and the vector work between their products, one after the other (a tile of 64 keys of heads of 128: 32 MFMAs of 32 cycles a wave, and 32
+// exponentials of 16 cycles with some 90 other instructions of 4; of heads of 64: as much vector work to half the MFMAs).  Though two or three waves share a SIMD, the cycles that either
+// keeps busy add up to all there are: heads of 128 50 + 50 %, of 64 34 + 68 % (instructions counted, times their cycles); if they overlapped, heads of 64 would reach 0.95 PFLOP/s.  Prompts of 4 x 4096 tokens, 32 heads on 8,
 // bf16, TFLOP/s without anything / with a mask / with a soft cap: heads of 64 596 / 477 / 388 (twice the exponentials a product), 128 909 / 775 / 669, 192 875 / 662 /
-// 613, 256 594 / 437 / 466 (one wave a SIMD: 512 registers); f16 of 64 667.  One prompt of 16384 tokens, heads of 128: 2.1 ms, 1.04 PFLOP/s, where an 8192 x 8192 x 8192 library
-// product reaches 1.20; its matrix units are busy 44 % of the time at a clock of 2.0 GHz, and LDS has no bank conflicts.  Fewer rows than 128 a block are bound by what a
+// 613, 256 594 / 437 / 466 (one wave a SIMD: 512 registers, and 28 to 46 moves between its halves a tile beside the score products); f16 of 64 667.  One prompt of 16384 tokens,
+// heads of 128: 2.1 to 2.3 ms box to box, 0.96 to 1.04 PFLOP/s, where an 8192 x 8192 x 8192 library product reaches 1.20, at a clock of 1.9 to 2.0 GHz; LDS has no bank conflicts.  Fewer rows than 128 a block are bound by what a
 // run waits for: 8 tokens behind 4000 rows 18 us here and 5 in the join, of which 3.2 would be the bytes.
 #pragma once
 

@@ -4,7 +4,9 @@
 //   2. the rows behind them, a sequence at a time, by gqa_attn's kernel; every head is left as pieces
 //   3. the join, here: out = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M) over the pieces of both, in the order of the rows
 //
-// The keys of a prefix are read once a group and KV head for up to 128 rows, where gqa_attn reads them once a sequence.  32 users behind 8192 shared rows (32 heads on 8 of 128): 46 us, of
+// The keys of a prefix are read once a block of rows -- 128, 64 or 32 of them by the rows a group on average, groups of one among them -- where gqa_attn reads them once a sequence; a
+// group's blocks find them in the caches.  (64 users, 4 / 16 / 32 of them behind 8192 shared rows, each of the others a group of one or in no group: 125 / 117 / 96 or 134 / 120 / 91 us; 16
+// heads on 4 of 64 44 / 43 / 41 or 47 / 46 / 42, of 256 149 / 132 / 106 or 163 / 145 / 109.)  32 users behind 8192 shared rows (32 heads on 8 of 128): 46 us, of
 // which the prefix is 25, the rows behind it 12.4 and the join 6.9 (8192 pieces' rows); 16 would be the bytes, and gqa_attn takes 142.  Each launch waits for lengths, page ids and
 // rows in turn, and for the one before it.  Five users behind 100000 rows: 102 us (gqa_attn 289), 4.0 TB/s of the call.
 
